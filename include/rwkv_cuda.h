@@ -44,6 +44,9 @@ enum {
 
 enum { RWKV_F32 = 0, RWKV_BF16 = 1, RWKV_F16 = 2 };
 
+/* activations of the projection epilogue: z, max(z, 0)^2, tanh z, 1 / (1 + e^-z) */
+enum { RWKV_ACT_NONE = 0, RWKV_ACT_RELU2 = 1, RWKV_ACT_TANH = 2, RWKV_ACT_SIGMOID = 3 };
+
 #define RWKV_WKV7_HEAD_SIZE 64 /* WKV7_HEAD_SIZE, Sources/RWKVKernel/WKV7.swift:7 */
 #define RWKV_WKV7_CHUNK 16     /* WKV7_CHUNK, Sources/RWKVKernel/WKV7.swift:8 */
 
@@ -493,6 +496,101 @@ int rwkv_adamw_clip_step(float* param, float* m, float* v, const float* grad, in
                          float grad_scale, float clip, float lr, float beta1, float beta2, float eps,
                          float weight_decay, float bias_c1, float bias_c2, float* norm_out,
                          void* workspace, int64_t workspace_bytes, rwkv_stream_t stream);
+
+/* ---------------------------------------------------- block operators
+ * What an x070 block is made of around the WKV path (ln1 / ln2, the r/k/v/o and
+ * cmix projections and the low-rank branches, Sources/RWKVGen/RWKVBlock.swift:
+ * 163-307), forward and backward, with trainable weights.  The reference runs
+ * these as MLX layerNorm / matmul / elementwise ops under MLX's autograd.
+ *
+ * 8-bit activation checkpoints.  What a backward pass reads of an activation
+ * [rows, D] can be kept in 1 + 1/32 bytes per element: int8 codes [rows, D]
+ * and one exponent byte per row and group of 32 channels, exps
+ * [rows, ceil(D / 32)].  A code q stands for q * 2^(e - 127).  Per group the
+ * scale is the power of two with max|x| / scale in [64, 128) (e >= 1) and
+ * q = round(x / scale), ties to even, clipped to [-127, 127], so that
+ * |x - value| <= max|x| / 127.5; a group holding an infinity or a NaN is
+ * stored as e = 255 with codes 0 and stands for NaN.
+ */
+
+/* Layer norm over the last dimension: y = (x - mean) * rstd * weight + bias,
+ * rstd = 1 / sqrt(var + eps), two passes over the row in fp32 (X070Backbone.
+ * swift:62-65).  x, y: [rows, D] in dtype; weight, bias: [D] in wdtype; mean,
+ * rstd: [rows] fp32 (both NULL, or both kept for the backward pass); codes /
+ * exps: both NULL, or the 8-bit checkpoint of x, written in the same pass.
+ * Any D >= 1.  y may be x. */
+int rwkv_layer_norm_forward(int dtype, const void* x, int wdtype, const void* weight, const void* bias,
+                            float eps, void* y, float* mean, float* rstd, int8_t* codes, uint8_t* exps,
+                            int rows, int D, rwkv_stream_t stream);
+
+/* Its gradient: with h = (x - mean) * rstd and g = dy * weight,
+ *     dx = rstd * (g - mean(g) - h * mean(g h)) [+ dres],
+ *     dweight = sum over rows of dy * h,  dbias = sum over rows of dy.
+ * dy, dx, dres: [rows, D] in dtype; dres (may be NULL) is the gradient that
+ * reaches x past the norm (the residual stream); dx may be dy or dres.  x in
+ * dtype, or NULL with codes / exps, the forward's 8-bit checkpoint of it.
+ * mean, rstd: the forward's.  weight, dweight, dbias: [D] in wdtype; dweight
+ * and dbias both NULL (a frozen norm) or both written.  Sums in fp32 in a
+ * fixed order (deterministic).  `workspace`: device memory of
+ * rwkv_layer_norm_backward_workspace_size bytes, 16-byte aligned; not needed
+ * (may be NULL) without dweight / dbias. */
+int64_t rwkv_layer_norm_backward_workspace_size(int rows, int D);
+int rwkv_layer_norm_backward(int dtype, const void* dy, const void* x, const int8_t* codes, const uint8_t* exps,
+                             int wdtype, const void* weight, const float* mean, const float* rstd,
+                             const void* dres, void* dx, void* dweight, void* dbias, int rows, int D,
+                             void* workspace, int64_t workspace_bytes, rwkv_stream_t stream);
+
+/* The 8-bit checkpoint of x [rows, D] (dtype). */
+int rwkv_ckpt8_pack(int dtype, const void* x, int8_t* codes, uint8_t* exps, int rows, int D,
+                    rwkv_stream_t stream);
+/* out = act(value) [rows, D] in odtype, one rounding: a checkpoint restored
+ * (RWKV_ACT_NONE), or the activation behind a checkpointed pre-activation. */
+int rwkv_ckpt8_values(const int8_t* codes, const uint8_t* exps, int act, int odtype, void* out, int rows, int D,
+                      rwkv_stream_t stream);
+/* dz = dy * act'(z) [rows, D] in dtype; z in dtype, or NULL with codes / exps,
+ * its 8-bit checkpoint.  dz may be dy. */
+int rwkv_act_backward(int dtype, const void* dy, const void* z, const int8_t* codes, const uint8_t* exps, int act,
+                      void* dz, int rows, int D, rwkv_stream_t stream);
+
+/* Trainable projections.  x [rows, IN], w [OUT, IN], y [rows, OUT] and their
+ * gradients; x, w and dY in `dtype`, BF16 or F16 (both operands of a
+ * tensor-core product in one type); accumulation in fp32, one rounding at the
+ * store.  IN % 8 == 0 and OUT % 8 == 0, tensors 16-byte aligned (exps and fp32
+ * vectors to their element); any rows >= 1.  tcgen05 tensor cores; these calls
+ * share rwkv_q_gemm's wait-error record (rwkv_q_gemm_status), and a stream may
+ * be captured once one call has run on its device.  `workspace`: device memory of
+ * the matching _workspace_size bytes, 16-byte aligned (NULL when that is 0);
+ * calls that may overlap on the GPU need one each.
+ *
+ * Forward: z = x W^T + bias, y = act(z) + residual.  bias (may be NULL): [OUT]
+ * in bdtype; y in ydtype (dtype or F32); residual (may be NULL): [rows, OUT] in
+ * ydtype, may be y.  Kept for the backward pass where not NULL: z [rows, OUT]
+ * in dtype, and codes / exps, the 8-bit checkpoint of z (taken from the fp32
+ * sums).  Stands for ctx.project with the activation, bias and residual that
+ * follow it (RWKVBlock.swift:163-307). */
+int64_t rwkv_projection_forward_workspace_size(int rows, int OUT, int IN);
+int rwkv_projection_forward(int dtype, const void* x, const void* w, int bdtype, const void* bias, int act,
+                            int ydtype, const void* residual, void* y, void* z, int8_t* codes, uint8_t* exps,
+                            int rows, int OUT, int IN, void* workspace, int64_t workspace_bytes,
+                            rwkv_stream_t stream);
+/* dX [rows, IN] = (dY W) * act'(z) + addend in dxdtype (dtype or F32).  z, the
+ * pre-activation of the layer below [rows, IN]: dense in dtype, or codes / exps
+ * its 8-bit checkpoint; both NULL (and act RWKV_ACT_NONE): the plain product.
+ * addend (may be NULL): [rows, IN] in dxdtype, may be dX. */
+int64_t rwkv_projection_dx_workspace_size(int rows, int OUT, int IN);
+int rwkv_projection_dx(int dtype, const void* dy, const void* w, int act, const void* z, const int8_t* codes,
+                       const uint8_t* exps, int dxdtype, const void* addend, void* dx, int rows, int OUT, int IN,
+                       void* workspace, int64_t workspace_bytes, rwkv_stream_t stream);
+/* dW [OUT, IN] = dY^T act(X) in dwdtype (dtype or F32), and db [OUT] = sum over
+ * rows of dY, fp32; either may be NULL (without dW, X is not read).  X [rows, IN]: dense in dtype, or
+ * codes / exps its 8-bit checkpoint.  act(X) is rounded to dtype, the type the
+ * tensor cores take (a checkpoint's values are exact there, so only act !=
+ * RWKV_ACT_NONE rounds).  `restore` of the workspace query: nonzero when act !=
+ * RWKV_ACT_NONE or X comes as a checkpoint. */
+int64_t rwkv_projection_dw_workspace_size(int rows, int OUT, int IN, int restore);
+int rwkv_projection_dw(int dtype, const void* dy, int act, const void* x, const int8_t* codes, const uint8_t* exps,
+                       int dwdtype, void* dw, float* db, int rows, int OUT, int IN, void* workspace,
+                       int64_t workspace_bytes, rwkv_stream_t stream);
 
 #ifdef __cplusplus
 }

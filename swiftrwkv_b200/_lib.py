@@ -15,6 +15,7 @@ HEADER_PATH = os.path.join(os.path.dirname(_HERE), "include", "rwkv_cuda.h")
 
 OK, E_NULL, E_SHAPE, E_DTYPE, E_UNSUPPORTED, E_CUDA, E_TIMEOUT, E_WORKSPACE = 0, -1, -2, -3, -4, -5, -6, -7
 F32, BF16, F16 = 0, 1, 2
+ACTS = {"none": 0, "relu2": 1, "tanh": 2, "sigmoid": 3}
 RWKV_NOALLOC_MAX_HEADS = 240  # rwkv_cuda.h: (batch, head) pairs of rwkv_wkv7_backward_noalloc
 
 
@@ -86,6 +87,18 @@ _SIGS = {
     "rwkv_state_grad_sum": [P, P, I, I, I, I, P],
     "rwkv_adamw_workspace_size": [I64],
     "rwkv_adamw_clip_step": [P, P, P, P, I64, F, F, F, F, F, F, F, F, F, P, P, I64, P],
+    "rwkv_layer_norm_forward": [I, P, I, P, P, F, P, P, P, P, P, I, I, P],
+    "rwkv_layer_norm_backward_workspace_size": [I, I],
+    "rwkv_layer_norm_backward": [I, P, P, P, P, I, P, P, P, P, P, P, P, I, I, P, I64, P],
+    "rwkv_ckpt8_pack": [I, P, P, P, I, I, P],
+    "rwkv_ckpt8_values": [P, P, I, I, P, I, I, P],
+    "rwkv_act_backward": [I, P, P, P, P, I, P, I, I, P],
+    "rwkv_projection_forward_workspace_size": [I, I, I],
+    "rwkv_projection_forward": [I, P, P, I, P, I, I, P, P, P, P, P, I, I, I, P, I64, P],
+    "rwkv_projection_dx_workspace_size": [I, I, I],
+    "rwkv_projection_dx": [I, P, P, I, P, P, P, I, P, P, I, I, I, P, I64, P],
+    "rwkv_projection_dw_workspace_size": [I, I, I, I],
+    "rwkv_projection_dw": [I, P, I, P, P, P, I, P, P, I, I, I, P, I64, P],
 }
 _RESTYPES = {
     "rwkv_status_string": ctypes.c_char_p,
@@ -95,6 +108,10 @@ _RESTYPES = {
     "rwkv_wkv7_backward_chunked_workspace_size": I64,
     "rwkv_x070_weight_bytes": I64,
     "rwkv_adamw_workspace_size": I64,
+    "rwkv_layer_norm_backward_workspace_size": I64,
+    "rwkv_projection_forward_workspace_size": I64,
+    "rwkv_projection_dx_workspace_size": I64,
+    "rwkv_projection_dw_workspace_size": I64,
 }
 
 _lib = None

@@ -1,0 +1,472 @@
+"""The operators of an x070 block around the WKV path, forward and backward.
+
+* Layer norm (ln0 / ln1 / ln2 / ln_out): `layerNormForward`,
+  `layerNormBackward`, and `layerNorm`, differentiable.
+* Projections with trainable weights (r / k / v / o, cmix key / value, the
+  low-rank branches): `projectionForward` with bias, activation and residual in
+  its epilogue, `projectionBackwardInput`, `projectionBackwardWeight`, and
+  `projection`, differentiable.
+* 8-bit activation checkpoints: `checkpoint8`, `checkpoint8Values`,
+  `activationBackward`; every backward above takes a `Checkpoint8` in place of
+  the activation it stands for.
+* `channelMix`, the two projections of cmix around the squared ReLU,
+  differentiable, with the pre-activation kept in 8 bits.
+
+The reference runs these as MLX layerNorm / matmul / elementwise ops under
+MLX's autograd (Sources/RWKVGen/RWKVBlock.swift:163-307, X070Backbone.swift:
+43-74); the C entry points are declared in include/rwkv_cuda.h.
+
+Arrays are torch CUDA tensors of [..., D]; leading dimensions are rows, of any
+number (also none).  All arithmetic runs in librwkvcuda, on the current stream
+of the tensors' device.  Arguments that do not fit raise ValueError; a failed
+CUDA call raises RWKVError.  The differentiable forms refuse to record a graph
+while a CUDA stream is being captured: capture the explicit forward and
+backward calls.
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+
+from . import _lib
+from ._lib import ACTS, BF16, F16, F32
+
+_DT = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
+_HALF = (torch.bfloat16, torch.float16)
+CKPT_GROUP = 32  # channels per scale of a checkpoint
+
+
+@dataclass
+class Checkpoint8:
+    """An activation [..., D] in 8 bits: int8 codes [..., D] and one exponent
+    byte per group of 32 channels, exps [..., ceil(D / 32)]; a code q stands
+    for q * 2^(e - 127).  `dtype` is the activation's own type."""
+    codes: torch.Tensor
+    exps: torch.Tensor
+    dtype: torch.dtype
+
+    @property
+    def shape(self):
+        return self.codes.shape
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    @property
+    def nbytes(self):
+        return self.codes.numel() + self.exps.numel()
+
+
+# ---------------------------------------------------------------- plumbing
+
+def _call(dev, name, *args):
+    """An entry point on `dev` and its current stream (appended)."""
+    L = _lib.lib()
+    if dev.index == torch.cuda.current_device():
+        st = getattr(L, name)(*args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            st = getattr(L, name)(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if st:
+        raise _lib.RWKVError(name, st, L.rwkv_last_error().decode())
+
+
+def _p(t):
+    return None if t is None else t.data_ptr()
+
+
+def _tensor(name, t, dev=None, dtypes=None, shape=None):
+    """t, contiguous, after its checks."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{name}: a CUDA tensor is needed")
+    if dev is not None and t.device != dev:
+        raise ValueError(f"{name} is on {t.device}, the call's other tensors on {dev}")
+    if t.dtype not in (dtypes or _DT):
+        raise ValueError(f"{name}: dtype {t.dtype} not taken")
+    if shape is not None and t.shape != shape:
+        raise ValueError(f"{name} {tuple(t.shape)} must be {list(shape)}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _some(name, t):
+    if t.dim() < 1 or t.shape[-1] < 1:
+        raise ValueError(f"{name} {tuple(t.shape)} must be [..., D] with D >= 1")
+    return t
+
+
+def _aligned(t):
+    """t at a 16-byte aligned address (a view may start anywhere)."""
+    return t if t is None or t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _rows(shape):
+    n = 1
+    for s in shape[:-1]:
+        n *= s
+    return n
+
+
+def _act(act):
+    if act not in ACTS:
+        raise ValueError(f"activation {act!r}: one of {sorted(ACTS)}")
+    return ACTS[act]
+
+
+def _activation(name, x, dev, dtype, shape):
+    """An activation given as a tensor or as its checkpoint: (x, codes, exps)."""
+    if isinstance(x, Checkpoint8):
+        groups = shape[:-1] + (-(-shape[-1] // CKPT_GROUP),)
+        return (None, _tensor(f"{name}.codes", x.codes, dev, (torch.int8,), shape),
+                _tensor(f"{name}.exps", x.exps, dev, (torch.uint8,), torch.Size(groups)))
+    return _tensor(name, x, dev, (dtype,), shape), None, None
+
+
+def _new_checkpoint(shape, dev, dtype):
+    return Checkpoint8(torch.empty(shape, device=dev, dtype=torch.int8),
+                       torch.empty(shape[:-1] + (-(-shape[-1] // CKPT_GROUP),), device=dev, dtype=torch.uint8), dtype)
+
+
+def _workspace(nbytes, dev):
+    return torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
+
+
+# ------------------------------------------------------- 8-bit checkpoints
+
+def checkpoint8(x) -> Checkpoint8:
+    """The 8-bit checkpoint of x [..., D]."""
+    x = _some("x", _tensor("x", x))
+    ck = _new_checkpoint(x.shape, x.device, x.dtype)
+    rows = _rows(x.shape)
+    if rows:
+        _call(x.device, "rwkv_ckpt8_pack", _DT[x.dtype], x.data_ptr(), ck.codes.data_ptr(), ck.exps.data_ptr(), rows,
+              x.shape[-1])
+    return ck
+
+
+def checkpoint8Values(ck: Checkpoint8, act: str = "none", dtype=None):
+    """What a checkpoint stands for, or the activation behind a checkpointed
+    pre-activation: act(value) in `dtype` (default: the activation's own)."""
+    a, dtype = _act(act), dtype or ck.dtype
+    if dtype not in _DT:
+        raise ValueError(f"checkpoint8Values: dtype {dtype} not taken")
+    _, codes, exps = _activation("ck", ck, ck.codes.device, None, ck.codes.shape)
+    out = torch.empty(codes.shape, device=codes.device, dtype=dtype)
+    rows = _rows(codes.shape)
+    if rows:
+        _call(codes.device, "rwkv_ckpt8_values", codes.data_ptr(), exps.data_ptr(), a, _DT[dtype], out.data_ptr(), rows,
+              codes.shape[-1])
+    return out
+
+
+def activationBackward(dy, pre, act: str):
+    """dy * act'(pre) in dy's dtype; `pre` is a tensor or a Checkpoint8."""
+    a = _act(act)
+    dy = _some("dy", _tensor("dy", dy))
+    z, codes, exps = _activation("pre", pre, dy.device, dy.dtype, dy.shape)
+    dz = torch.empty_like(dy)
+    rows = _rows(dy.shape)
+    if rows:
+        _call(dy.device, "rwkv_act_backward", _DT[dy.dtype], dy.data_ptr(), _p(z), _p(codes), _p(exps), a, dz.data_ptr(),
+              rows, dy.shape[-1])
+    return dz
+
+
+# --------------------------------------------------------------- layer norm
+
+def layerNormForward(x, weight, bias, eps: float = 1e-5, checkpoint: bool = False):
+    """Layer norm over the last dimension: (y, mean, rstd, ck).  mean / rstd
+    [...] fp32 are what the backward pass needs; ck is the 8-bit checkpoint of x
+    (None without `checkpoint`)."""
+    x = _some("x", _tensor("x", x))
+    dev, D = x.device, x.shape[-1]
+    weight = _tensor("weight", weight, dev, None, (D,))
+    bias = _tensor("bias", bias, dev, (weight.dtype,), (D,))
+    y = torch.empty_like(x)
+    stats = torch.empty((2,) + x.shape[:-1], device=dev, dtype=torch.float32)
+    mean, rstd = stats[0], stats[1]
+    ck = _new_checkpoint(x.shape, dev, x.dtype) if checkpoint else None
+    rows = _rows(x.shape)
+    if rows:
+        _call(dev, "rwkv_layer_norm_forward", _DT[x.dtype], x.data_ptr(), _DT[weight.dtype], weight.data_ptr(),
+              bias.data_ptr(), eps, y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), ck and ck.codes.data_ptr(),
+              ck and ck.exps.data_ptr(), rows, D)
+    return y, mean, rstd, ck
+
+
+def layerNormBackward(dy, x, weight, mean, rstd, dres=None, params: bool = True):
+    """(dx, dweight, dbias) of layerNormForward.  x: its input, or the
+    checkpoint of it; mean, rstd: its statistics; dres: the gradient that
+    reaches x past the norm, added to dx.  Without `params` dweight and dbias
+    are None."""
+    dy = _some("dy", _tensor("dy", dy))
+    dev, D = dy.device, dy.shape[-1]
+    xt, codes, exps = _activation("x", x, dev, dy.dtype, dy.shape)
+    weight = _tensor("weight", weight, dev, None, (D,))
+    mean = _tensor("mean", mean, dev, (torch.float32,), dy.shape[:-1])
+    rstd = _tensor("rstd", rstd, dev, (torch.float32,), dy.shape[:-1])
+    if dres is not None:
+        dres = _tensor("dres", dres, dev, (dy.dtype,), dy.shape)
+    dx = torch.empty_like(dy)
+    rows = _rows(dy.shape)
+    dw = torch.empty_like(weight) if params else None
+    db = torch.empty_like(weight) if params else None
+    if not rows:
+        return dx, dw.zero_() if params else None, db.zero_() if params else None
+    n = _lib.lib().rwkv_layer_norm_backward_workspace_size(rows, D) if params else 0
+    ws = _workspace(n, dev)
+    _call(dev, "rwkv_layer_norm_backward", _DT[dy.dtype], dy.data_ptr(), _p(xt), _p(codes), _p(exps), _DT[weight.dtype],
+          weight.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _p(dres), dx.data_ptr(), _p(dw), _p(db), rows, D, _p(ws),
+          n)
+    return dx, dw, db
+
+
+# -------------------------------------------------------------- projections
+
+def _weight(w, dev=None, dtype=None):
+    w = _tensor("w", w, dev, _HALF if dtype is None else (dtype,))
+    if w.dim() != 2:
+        raise ValueError(f"w {tuple(w.shape)} must be [OUT, IN]")
+    if w.shape[0] % 8 or w.shape[1] % 8 or not w.numel():
+        raise ValueError(f"w {tuple(w.shape)}: OUT and IN must be multiples of 8")
+    return _aligned(w)
+
+
+def projectionForward(x, w, bias=None, act: str = "none", residual=None, checkpoint: bool = False,
+                      preactivation: bool = False, out_dtype=None):
+    """y = act(x w^T + bias) + residual: (y, kept).  x [..., IN] and w [OUT, IN]
+    in one 16-bit type; y and residual in `out_dtype` (that type, or fp32).
+    kept is the 8-bit checkpoint of z = x w^T + bias with `checkpoint`, z itself
+    with `preactivation`, else None."""
+    a = _act(act)
+    x = _aligned(_tensor("x", x, None, _HALF))
+    dev = x.device
+    w = _weight(w, dev, x.dtype)
+    OUT, IN = w.shape
+    if x.dim() < 1 or x.shape[-1] != IN:
+        raise ValueError(f"x {tuple(x.shape)} must be [..., {IN}]")
+    if checkpoint and preactivation:
+        raise ValueError("projectionForward: keep either the checkpoint or the pre-activation")
+    ydt = out_dtype or x.dtype
+    if ydt != x.dtype and ydt != torch.float32:
+        raise ValueError(f"projectionForward: out_dtype {ydt} (x's own type or fp32)")
+    shape = x.shape[:-1] + (OUT,)
+    if bias is not None:
+        bias = _tensor("bias", bias, dev, None, (OUT,))
+    if residual is not None:
+        residual = _aligned(_tensor("residual", residual, dev, (ydt,), shape))
+    y = torch.empty(shape, device=dev, dtype=ydt)
+    ck = _new_checkpoint(torch.Size(shape), dev, x.dtype) if checkpoint else None
+    z = torch.empty(shape, device=dev, dtype=x.dtype) if preactivation else None
+    rows = _rows(shape)
+    if rows:
+        n = _lib.lib().rwkv_projection_forward_workspace_size(rows, OUT, IN)
+        ws = _workspace(n, dev)
+        _call(dev, "rwkv_projection_forward", _DT[x.dtype], x.data_ptr(), w.data_ptr(),
+              F32 if bias is None else _DT[bias.dtype], _p(bias), a, _DT[ydt], _p(residual), y.data_ptr(), _p(z),
+              ck and ck.codes.data_ptr(), ck and ck.exps.data_ptr(), rows, OUT, IN, _p(ws), n)
+    return y, ck if checkpoint else z
+
+
+def projectionBackwardInput(dy, w, pre=None, act: str = "none", addend=None, out_dtype=None):
+    """dx = (dy w) * act'(pre) + addend in dy's dtype (or `out_dtype` fp32).
+    pre [..., IN]: the pre-activation of the layer below, a tensor or a
+    Checkpoint8 (None: the plain product); addend in dx's type."""
+    a = _act(act)
+    dy = _aligned(_tensor("dy", dy, None, _HALF))
+    dev = dy.device
+    w = _weight(w, dev, dy.dtype)
+    OUT, IN = w.shape
+    if dy.dim() < 1 or dy.shape[-1] != OUT:
+        raise ValueError(f"dy {tuple(dy.shape)} must be [..., {OUT}]")
+    xdt = out_dtype or dy.dtype
+    if xdt != dy.dtype and xdt != torch.float32:
+        raise ValueError(f"projectionBackwardInput: out_dtype {xdt} (dy's own type or fp32)")
+    shape = torch.Size(dy.shape[:-1] + (IN,))
+    z = codes = exps = None
+    if pre is not None:
+        z, codes, exps = _activation("pre", pre, dev, dy.dtype, shape)
+        z, codes = _aligned(z), _aligned(codes)
+    elif act != "none":
+        raise ValueError(f"projectionBackwardInput: act {act!r} needs pre")
+    if addend is not None:
+        addend = _aligned(_tensor("addend", addend, dev, (xdt,), shape))
+    dx = torch.empty(shape, device=dev, dtype=xdt)
+    rows = _rows(shape)
+    if rows:
+        n = _lib.lib().rwkv_projection_dx_workspace_size(rows, OUT, IN)
+        ws = _workspace(n, dev)
+        _call(dev, "rwkv_projection_dx", _DT[dy.dtype], dy.data_ptr(), w.data_ptr(), a, _p(z), _p(codes), _p(exps),
+              _DT[xdt], _p(addend), dx.data_ptr(), rows, OUT, IN, _p(ws), n)
+    return dx
+
+
+def projectionBackwardWeight(dy, x, act: str = "none", bias: bool = False, out_dtype=None):
+    """(dw, db): dw [OUT, IN] = sum over rows of dy act(x)^T in dy's dtype (or
+    `out_dtype` fp32), db [OUT] fp32 = sum over rows of dy (None without
+    `bias`).  x [..., IN]: the projection's input, or with `act` the
+    pre-activation behind it; a tensor or a Checkpoint8; None: only db (dw is
+    None)."""
+    a = _act(act)
+    dy = _aligned(_some("dy", _tensor("dy", dy, None, _HALF)))
+    dev = dy.device
+    if x is None:
+        if not bias or a:
+            raise ValueError("projectionBackwardWeight: without x only db can be asked for")
+    elif len(x.shape) < 1:
+        raise ValueError("projectionBackwardWeight: x must be [..., IN]")
+    OUT, IN = dy.shape[-1], 8 if x is None else x.shape[-1]
+    if OUT % 8 or IN % 8 or not IN:
+        raise ValueError(f"projectionBackwardWeight: OUT={OUT} and IN={IN} must be multiples of 8")
+    wdt = out_dtype or dy.dtype
+    if wdt != dy.dtype and wdt != torch.float32:
+        raise ValueError(f"projectionBackwardWeight: out_dtype {wdt} (dy's own type or fp32)")
+    xt = codes = exps = dw = None
+    if x is not None:
+        xt, codes, exps = _activation("x", x, dev, dy.dtype, torch.Size(dy.shape[:-1] + (IN,)))
+        xt, codes = _aligned(xt), _aligned(codes)
+        dw = torch.empty((OUT, IN), device=dev, dtype=wdt)
+    db = torch.empty(OUT, device=dev, dtype=torch.float32) if bias else None
+    rows = _rows(dy.shape)
+    if not rows:
+        return dw if dw is None else dw.zero_(), db.zero_() if bias else None
+    n = _lib.lib().rwkv_projection_dw_workspace_size(rows, OUT, IN, int(codes is not None or a != 0))
+    ws = _workspace(n, dev)
+    _call(dev, "rwkv_projection_dw", _DT[dy.dtype], dy.data_ptr(), a, _p(xt), _p(codes), _p(exps), _DT[wdt],
+          _p(dw), _p(db), rows, OUT, IN, _p(ws), n)
+    return dw, db
+
+
+# --------------------------------------------------- the differentiable forms
+
+def _recording(*ts):
+    """Whether autograd records this call; refused while a stream is captured."""
+    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in ts):
+        return False
+    if torch.cuda.is_current_stream_capturing():
+        raise ValueError("the differentiable block operators do not record a graph during stream capture: "
+                         "capture the explicit forward and backward calls")
+    return True
+
+
+def _save(ctx, kept, *ts):
+    """Saves tensors and activations kept as tensors or as checkpoints."""
+    flat, ctx.kept = list(ts), []
+    for k in kept:
+        if isinstance(k, Checkpoint8):
+            ctx.kept.append(k.dtype)
+            flat += [k.codes, k.exps]
+        else:
+            ctx.kept.append(None)
+            flat.append(k)
+    ctx.n_plain = len(ts)
+    ctx.save_for_backward(*flat)
+
+
+def _saved(ctx):
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("the differentiable block operators' backward does not run during stream capture: "
+                           "capture the explicit backward calls")
+    ts = list(ctx.saved_tensors)
+    plain, rest, kept = ts[:ctx.n_plain], ts[ctx.n_plain:], []
+    for dt in ctx.kept:
+        kept.append(rest.pop(0) if dt is None else Checkpoint8(rest.pop(0), rest.pop(0), dt))
+    return plain, kept
+
+
+def _kept(x, checkpoint, needed):
+    """A projection's input as its weight gradient needs it, or None."""
+    return (checkpoint8(x) if checkpoint else x) if needed else None
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, checkpoint):
+        y, mean, rstd, ck = layerNormForward(x, weight, bias, eps, checkpoint)
+        _save(ctx, [ck if checkpoint else x], weight, mean, rstd)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        (weight, mean, rstd), (x,) = _saved(ctx)
+        params = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+        return (*layerNormBackward(dy, x, weight, mean, rstd, params=params), None, None)
+
+
+def layerNorm(x, weight, bias, eps: float = 1e-5, checkpoint: bool = False):
+    """Differentiable layer norm.  With `checkpoint` its input is kept for the
+    backward pass as an 8-bit checkpoint instead of in its own type."""
+    if not _recording(x, weight, bias):
+        return layerNormForward(x, weight, bias, eps)[0]
+    return _LayerNorm.apply(x, weight, bias, eps, checkpoint)
+
+
+class _Projection(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, bias, act, residual, checkpoint):
+        keep = act != "none"
+        y, z = projectionForward(x, w, bias, act, residual, checkpoint=keep and checkpoint,
+                                 preactivation=keep and not checkpoint)
+        kept = [_kept(x, checkpoint, ctx.needs_input_grad[1])]
+        ctx.act = act
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        _save(ctx, kept + ([z] if keep else []), w)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        (w,), kept = _saved(ctx)
+        need = ctx.needs_input_grad
+        dz = activationBackward(dy, kept[1], ctx.act) if ctx.act != "none" else dy
+        dx = projectionBackwardInput(dz, w) if need[0] else None
+        dw = db = None
+        if need[1] or need[2]:
+            dw, db = projectionBackwardWeight(dz, kept[0], bias=need[2])
+        if db is not None:
+            db = db.to(ctx.bias_dtype)
+        return dx, dw, db, None, dy if need[4] else None, None
+
+
+def projection(x, w, bias=None, act: str = "none", residual=None, checkpoint: bool = False):
+    """Differentiable y = act(x w^T + bias) + residual.  With `checkpoint` the
+    backward pass works from 8-bit checkpoints of x and of the pre-activation."""
+    if not _recording(x, w, bias, residual):
+        return projectionForward(x, w, bias, act, residual)[0]
+    return _Projection.apply(x, w, bias, act, residual, checkpoint)
+
+
+class _ChannelMix(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, key, value, residual, checkpoint):
+        k, z = projectionForward(x, key, act="relu2", checkpoint=checkpoint, preactivation=not checkpoint)
+        y, _ = projectionForward(k, value, residual=residual)
+        _save(ctx, [_kept(x, checkpoint, ctx.needs_input_grad[1]), z], key, value)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        (key, value), (x, z) = _saved(ctx)
+        need = ctx.needs_input_grad
+        dv = projectionBackwardWeight(dy, z, act="relu2")[0] if need[2] else None
+        dx = dk = None
+        if need[0] or need[1]:
+            dz = projectionBackwardInput(dy, value, pre=z, act="relu2")
+            dk = projectionBackwardWeight(dz, x)[0] if need[1] else None
+            dx = projectionBackwardInput(dz, key) if need[0] else None
+        return dx, dk, dv, dy if need[3] else None, None
+
+
+def channelMix(x, key, value, residual=None, checkpoint: bool = True):
+    """The projections of cmix, differentiable: relu(x key^T)^2 value^T +
+    residual (RWKVBlock.swift:299-307, after the token shift).  The squared
+    ReLU ends the first product and its gradient the backward's, which reads the
+    pre-activation z; with `checkpoint` z and x are kept in 8 bits (1 + 1/32
+    bytes per channel) and the squared ReLU itself is not kept at all."""
+    if not _recording(x, key, value, residual):
+        k, _ = projectionForward(x, key, act="relu2")
+        return projectionForward(k, value, residual=residual)[0]
+    return _ChannelMix.apply(x, key, value, residual, checkpoint)

@@ -1,0 +1,216 @@
+// Trainable projections: y = act(x W^T + bias) + residual, dX and dW, over the
+// tcgen05 kernel of gemm_proj.cuh.
+#include "gemm_proj.cuh"
+
+namespace rwkv {
+
+// qaffine.cu, ckpt8.cu
+int gemm_wait_record(cudaStream_t st, const char* fn, int** err, int** err_host, int* sm_count);
+int launch_ckpt8_values(const int8_t* codes, const uint8_t* exps, int act, int odtype, void* out, int rows, int D,
+                        cudaStream_t st);
+int launch_act(int dtype, const void* z, int act, void* out, int rows, int D, cudaStream_t st);
+
+namespace {
+
+// Column sums of dY [rows, OUT] (16 bits): a thread takes 8 columns of every
+// 8th row of its block's slice; the 8 row lanes meet in shared memory.
+constexpr int CS_COLS = 256;
+__global__ void __launch_bounds__(256) col_sum_kernel(const void* __restrict__ dy, float* __restrict__ part, int rows,
+                                                      int OUT, int bf16) {
+    __shared__ float red[8][CS_COLS];
+    const int cv = threadIdx.x & 31, rl = threadIdx.x >> 5;
+    const int col = blockIdx.x * CS_COLS + cv * 8;
+    float s[8] = {};
+    if (col < OUT)
+        for (int64_t r = (int64_t)blockIdx.y * 8 + rl; r < rows; r += 8 * (int64_t)gridDim.y) {
+            float v[8];
+            load8_16(dy, r * OUT + col, bf16, v);
+#pragma unroll
+            for (int k = 0; k < 8; k++) s[k] += v[k];
+        }
+#pragma unroll
+    for (int k = 0; k < 8; k++) red[rl][cv * 8 + k] = s[k];
+    __syncthreads();
+    const int c = blockIdx.x * CS_COLS + threadIdx.x;
+    if (c < OUT) {
+        float t = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; k++) t += red[k][threadIdx.x];
+        part[(int64_t)blockIdx.y * OUT + c] = t;
+    }
+}
+__global__ void __launch_bounds__(256) col_join_kernel(const float* __restrict__ part, float* __restrict__ db, int OUT,
+                                                       int slices) {
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    if (c >= OUT) return;
+    float s = 0.f;
+    for (int k = 0; k < slices; k++) s += part[(int64_t)k * OUT + c];
+    db[c] = s;
+}
+int col_slices(int rows, int OUT) {
+    return std::max(1, std::min(ceil_div(rows, 64), 148 * 4 / ceil_div(OUT, CS_COLS)));
+}
+
+int64_t al256(int64_t n) { return (n + 255) / 256 * 256; }
+bool al(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+
+int check_common(int dtype, int rows, int OUT, int IN, const char* fn) {
+    RWKV_REQUIRE(dtype == RWKV_BF16 || dtype == RWKV_F16, RWKV_E_DTYPE, "%s: dtype %d (bf16 or fp16)", fn, dtype);
+    RWKV_REQUIRE(rows >= 1 && OUT >= 1 && IN >= 1, RWKV_E_SHAPE, "%s: rows=%d OUT=%d IN=%d must be >= 1", fn, rows, OUT,
+                 IN);
+    RWKV_REQUIRE(IN % 8 == 0 && OUT % 8 == 0, RWKV_E_UNSUPPORTED, "%s: IN=%d and OUT=%d must be multiples of 8", fn,
+                 IN, OUT);
+    RWKV_REQUIRE(rows <= 1 << 26 && OUT <= 1 << 20 && IN <= 1 << 20 &&
+                     (int64_t)ceil_div(rows, 128) * ceil_div(std::max(OUT, IN), 64) < 1 << 30,
+                 RWKV_E_SHAPE, "%s: rows=%d OUT=%d IN=%d too large", fn, rows, OUT, IN);
+    return RWKV_OK;
+}
+int check_ws(const void* ws, int64_t bytes, int64_t need, const char* fn) {
+    RWKV_REQUIRE(need == 0 || (ws && bytes >= need), RWKV_E_WORKSPACE, "%s: workspace of %lld bytes, need %lld", fn,
+                 (long long)bytes, (long long)need);
+    RWKV_REQUIRE(need == 0 || al(ws, 16), RWKV_E_UNSUPPORTED, "%s: workspace not 16-byte aligned", fn);
+    return RWKV_OK;
+}
+bool out_ok(int out, int dtype) { return out == dtype || out == RWKV_F32; }
+
+bool sizes_ok(int rows, int OUT, int IN) {
+    return check_common(RWKV_BF16, rows, OUT, IN, "workspace_size") == RWKV_OK;
+}
+
+}  // namespace
+}  // namespace rwkv
+
+using namespace rwkv;
+
+extern "C" int64_t rwkv_projection_forward_workspace_size(int rows, int OUT, int IN) {
+    return sizes_ok(rows, OUT, IN) ? proj_plan(rows, OUT, IN).ws_bytes : 0;
+}
+
+extern "C" int rwkv_projection_forward(int dtype, const void* x, const void* w, int bdtype, const void* bias, int act,
+                                       int ydtype, const void* residual, void* y, void* z, int8_t* codes,
+                                       uint8_t* exps, int rows, int OUT, int IN, void* workspace,
+                                       int64_t workspace_bytes, rwkv_stream_t stream) {
+    const char* fn = "rwkv_projection_forward";
+    if (int rc = check_common(dtype, rows, OUT, IN, fn)) return rc;
+    RWKV_REQUIRE(x && w && y, RWKV_E_NULL, "%s: NULL argument", fn);
+    RWKV_REQUIRE(!codes == !exps, RWKV_E_NULL, "%s: give both codes and exps or neither", fn);
+    RWKV_REQUIRE(out_ok(ydtype, dtype) && (!bias || valid_dtype(bdtype)), RWKV_E_DTYPE, "%s: dtypes y=%d bias=%d", fn,
+                 ydtype, bdtype);
+    RWKV_REQUIRE(valid_act(act), RWKV_E_UNSUPPORTED, "%s: activation %d", fn, act);
+    RWKV_REQUIRE(al(x, 16) && al(w, 16) && al(y, 16) && al(residual, 16) && al(z, 16) && al(codes, 16) &&
+                     al(bias, bdtype == RWKV_F32 ? 4 : 2),
+                 RWKV_E_UNSUPPORTED, "%s: a tensor is not 16-byte aligned", fn);
+    if (int rc = check_ws(workspace, workspace_bytes, proj_plan(rows, OUT, IN).ws_bytes, fn)) return rc;
+    int *err, *err_host, sms;
+    if (int rc = gemm_wait_record((cudaStream_t)stream, fn, &err, &err_host, &sms)) return rc;
+    ProjEpi e{};
+    e.bf16 = dtype == RWKV_BF16;
+    e.out_f32 = ydtype == RWKV_F32;
+    e.act = act;
+    e.bias = bias;
+    e.bias_dtype = bdtype;
+    e.add = residual;
+    e.codes = codes;
+    e.exps = exps;
+    e.z = z;
+    const cudaError_t rc = proj_gemm<false, false>(x, w, y, rows, OUT, IN, e, static_cast<float*>(workspace), err,
+                                                   err_host, sms, (cudaStream_t)stream);
+    if (rc != cudaSuccess) return fail(RWKV_E_CUDA, "%s: %s", fn, cudaGetErrorString(rc));
+    return ok();
+}
+
+extern "C" int64_t rwkv_projection_dx_workspace_size(int rows, int OUT, int IN) {
+    return sizes_ok(rows, OUT, IN) ? proj_plan(rows, IN, OUT).ws_bytes : 0;
+}
+
+extern "C" int rwkv_projection_dx(int dtype, const void* dy, const void* w, int act, const void* z,
+                                  const int8_t* codes, const uint8_t* exps, int dxdtype, const void* addend, void* dx,
+                                  int rows, int OUT, int IN, void* workspace, int64_t workspace_bytes,
+                                  rwkv_stream_t stream) {
+    const char* fn = "rwkv_projection_dx";
+    if (int rc = check_common(dtype, rows, OUT, IN, fn)) return rc;
+    RWKV_REQUIRE(dy && w && dx, RWKV_E_NULL, "%s: NULL argument", fn);
+    RWKV_REQUIRE(valid_act(act), RWKV_E_UNSUPPORTED, "%s: activation %d", fn, act);
+    RWKV_REQUIRE(!codes == !exps && !(z && codes), RWKV_E_NULL, "%s: z, or codes and exps, or neither", fn);
+    RWKV_REQUIRE(z || codes || act == RWKV_ACT_NONE, RWKV_E_NULL, "%s: the activation needs its pre-activation", fn);
+    RWKV_REQUIRE(out_ok(dxdtype, dtype), RWKV_E_DTYPE, "%s: dX dtype %d", fn, dxdtype);
+    RWKV_REQUIRE(al(dy, 16) && al(w, 16) && al(z, 16) && al(codes, 16) && al(addend, 16) && al(dx, 16),
+                 RWKV_E_UNSUPPORTED, "%s: a tensor is not 16-byte aligned", fn);
+    if (int rc = check_ws(workspace, workspace_bytes, proj_plan(rows, IN, OUT).ws_bytes, fn)) return rc;
+    int *err, *err_host, sms;
+    if (int rc = gemm_wait_record((cudaStream_t)stream, fn, &err, &err_host, &sms)) return rc;
+    ProjEpi e{};
+    e.bf16 = dtype == RWKV_BF16;
+    e.out_f32 = dxdtype == RWKV_F32;
+    e.act = act;
+    e.grad = act != RWKV_ACT_NONE;
+    e.pre = z;
+    e.pre_codes = codes;
+    e.pre_exps = exps;
+    e.add = addend;
+    const cudaError_t rc = proj_gemm<false, true>(dy, w, dx, rows, IN, OUT, e, static_cast<float*>(workspace), err,
+                                                  err_host, sms, (cudaStream_t)stream);
+    if (rc != cudaSuccess) return fail(RWKV_E_CUDA, "%s: %s", fn, cudaGetErrorString(rc));
+    return ok();
+}
+
+namespace {
+// dW's workspace: the restored operand, the split-K partials, the partial column sums
+struct DwPlan {
+    int64_t operand, parts, total;
+    int slices;
+};
+DwPlan dw_plan(int rows, int OUT, int IN, bool restore) {
+    DwPlan p{};
+    p.operand = restore ? al256((int64_t)rows * IN * 2) : 0;
+    p.parts = al256(proj_plan(OUT, IN, rows).ws_bytes);
+    p.slices = col_slices(rows, OUT);
+    p.total = p.operand + p.parts + al256((int64_t)p.slices * OUT * 4);
+    return p;
+}
+}  // namespace
+
+extern "C" int64_t rwkv_projection_dw_workspace_size(int rows, int OUT, int IN, int restore) {
+    return sizes_ok(rows, OUT, IN) ? dw_plan(rows, OUT, IN, restore != 0).total : 0;
+}
+
+extern "C" int rwkv_projection_dw(int dtype, const void* dy, int act, const void* x, const int8_t* codes,
+                                  const uint8_t* exps, int dwdtype, void* dw, float* db, int rows, int OUT, int IN,
+                                  void* workspace, int64_t workspace_bytes, rwkv_stream_t stream) {
+    const char* fn = "rwkv_projection_dw";
+    if (int rc = check_common(dtype, rows, OUT, IN, fn)) return rc;
+    RWKV_REQUIRE(dy && (dw || db), RWKV_E_NULL, "%s: NULL argument", fn);
+    RWKV_REQUIRE(!dw || (x ? !codes && !exps : codes && exps), RWKV_E_NULL, "%s: give either x or codes and exps", fn);
+    RWKV_REQUIRE(valid_act(act), RWKV_E_UNSUPPORTED, "%s: activation %d", fn, act);
+    RWKV_REQUIRE(out_ok(dwdtype, dtype), RWKV_E_DTYPE, "%s: dW dtype %d", fn, dwdtype);
+    RWKV_REQUIRE(al(dy, 16) && al(x, 16) && al(codes, 16) && al(dw, 16) && al(db, 4), RWKV_E_UNSUPPORTED,
+                 "%s: a tensor is not 16-byte aligned", fn);
+    const bool restore = dw && (codes || act != RWKV_ACT_NONE);
+    const DwPlan p = dw_plan(rows, OUT, IN, restore);
+    if (int rc = check_ws(workspace, workspace_bytes, p.total, fn)) return rc;
+    cudaStream_t st = (cudaStream_t)stream;
+    int *err, *err_host, sms;
+    if (int rc = gemm_wait_record(st, fn, &err, &err_host, &sms)) return rc;
+    char* ws = static_cast<char*>(workspace);
+    const void* operand = x;
+    if (restore) {
+        operand = ws;
+        if (int rc = codes ? launch_ckpt8_values(codes, exps, act, dtype, ws, rows, IN, st)
+                           : launch_act(dtype, x, act, ws, rows, IN, st))
+            return rc;
+    }
+    ProjEpi e{};
+    e.bf16 = dtype == RWKV_BF16;
+    e.out_f32 = dwdtype == RWKV_F32;
+    if (dw) {
+        const cudaError_t rc = proj_gemm<true, true>(dy, operand, dw, OUT, IN, rows, e,
+                                                     reinterpret_cast<float*>(ws + p.operand), err, err_host, sms, st);
+        if (rc != cudaSuccess) return fail(RWKV_E_CUDA, "%s: %s", fn, cudaGetErrorString(rc));
+    }
+    if (!db) return ok();
+    float* part = reinterpret_cast<float*>(ws + p.operand + p.parts);
+    col_sum_kernel<<<dim3(ceil_div(OUT, CS_COLS), p.slices), 256, 0, st>>>(dy, part, rows, OUT, e.bf16);
+    if (int r = check_launch("col_sum_kernel")) return r;
+    col_join_kernel<<<ceil_div(OUT, 256), 256, 0, st>>>(part, db, OUT, p.slices);
+    return check_launch("col_join_kernel");
+}

@@ -273,7 +273,7 @@ struct GemmScratch {
     std::mutex mu;
 };
 
-static GemmScratch* gemm_scratch() {
+static GemmScratch* gemm_scratch(bool create = true) {
     static std::mutex m;
     static std::unordered_map<int, GemmScratch*> per_dev;
     int dev = 0;
@@ -281,6 +281,7 @@ static GemmScratch* gemm_scratch() {
     std::lock_guard<std::mutex> lk(m);
     auto it = per_dev.find(dev);
     if (it != per_dev.end()) return it->second;
+    if (!create) return nullptr;
     GemmScratch* s = new GemmScratch();
     cudaDeviceGetAttribute(&s->sm_count, cudaDevAttrMultiProcessorCount, dev);
     s->floats = (size_t)(4 * s->sm_count + 64) * GW_BM * 64;
@@ -428,6 +429,32 @@ int launch_gemm_dx_any(int wfmt, const void* dy, const void* w, const uint32_t* 
     a.err_host = sc->flag.host_dev;
     cudaError_t e = launch_gemm_dx(wfmt, a, dy, w, wq, sc->sm_count, st);
     if (e != cudaSuccess) return fail(RWKV_E_CUDA, "gemm_dx_kernel: %s", cudaGetErrorString(e));
+    return ok();
+}
+
+// The current device's wait-error record and SM count for the projection
+// kernels (projection.cu), which share rwkv_q_gemm's record.  Reports a wait
+// that an earlier call gave up, like the other tensor-core entry points.  While
+// `st` is being captured nothing is allocated, cleared or reported as cleared:
+// the record has to exist already, and a set one stays set.
+int gemm_wait_record(cudaStream_t st, const char* fn, int** err, int** err_host, int* sm_count) {
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(st, &cap) != cudaSuccess) {
+        cudaGetLastError();
+        cap = cudaStreamCaptureStatusNone;
+    }
+    const bool capturing = cap != cudaStreamCaptureStatusNone;
+    GemmScratch* sc = gemm_scratch(!capturing);
+    if (!sc)
+        return capturing ? fail(RWKV_E_CUDA, "%s: make one projection call on this device before capturing", fn)
+                         : fail(RWKV_E_CUDA, "%s: workspace allocation failed", fn);
+    if (capturing ? *(volatile int*)sc->flag.host != 0 : sc->flag.take(st))
+        return fail(RWKV_E_TIMEOUT, "%s: a tensor-core GEMM wait of an earlier call gave up; its outputs are not "
+                                    "valid (%s, nothing launched)",
+                    fn, capturing ? "flag kept" : "flag cleared");
+    *err = sc->err;
+    *err_host = sc->flag.host_dev;
+    *sm_count = sc->sm_count;
     return ok();
 }
 

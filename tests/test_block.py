@@ -1,0 +1,181 @@
+"""CPU tests of the block operators (layer norm, projections, 8-bit
+checkpoints): every refusal happens on the host, before anything launches."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from swiftrwkv_b200 import _lib
+from swiftrwkv_b200 import block as B
+
+FAKE = ctypes.c_void_p(0x1000)   # aligned, never dereferenced: checks fail first
+ODD = ctypes.c_void_p(0x1001)
+HALF = ctypes.c_void_p(0x1008)   # 8-byte aligned only
+F32, BF16, F16 = _lib.F32, _lib.BF16, _lib.F16
+
+
+def st(name, *a):
+    return _lib.status(name, *a)
+
+
+def norm_fwd(dt=BF16, x=FAKE, wdt=F32, w=FAKE, b=FAKE, eps=1e-5, y=FAKE, mean=FAKE, rstd=FAKE, c=None, e=None, rows=4,
+             D=64):
+    return st("rwkv_layer_norm_forward", dt, x, wdt, w, b, ctypes.c_float(eps), y, mean, rstd, c, e, rows, D, None)
+
+
+def test_layer_norm_forward_refusals():
+    assert norm_fwd(dt=7) == _lib.E_DTYPE
+    assert norm_fwd(wdt=-1) == _lib.E_DTYPE
+    for k in ("x", "w", "b", "y"):
+        assert norm_fwd(**{k: None}) == _lib.E_NULL
+    assert norm_fwd(mean=None) == _lib.E_NULL       # statistics come together
+    assert norm_fwd(c=FAKE) == _lib.E_NULL          # so do codes and exps
+    assert norm_fwd(rows=0) == _lib.E_SHAPE
+    assert norm_fwd(D=0) == _lib.E_SHAPE
+    assert norm_fwd(D=(1 << 30) + 8) == _lib.E_SHAPE
+    assert norm_fwd(eps=-1.0) == _lib.E_SHAPE
+    assert norm_fwd(x=ODD) == _lib.E_UNSUPPORTED
+    assert b"aligned" in _lib.lib().rwkv_last_error()
+
+
+def norm_bwd(dt=BF16, dy=FAKE, x=FAKE, c=None, e=None, wdt=F32, w=FAKE, mean=FAKE, rstd=FAKE, dres=None, dx=FAKE,
+             dw=FAKE, db=FAKE, rows=4, D=64, ws=FAKE, n=1 << 30):
+    return st("rwkv_layer_norm_backward", dt, dy, x, c, e, wdt, w, mean, rstd, dres, dx, dw, db, rows, D, ws, n, None)
+
+
+def test_layer_norm_backward_refusals():
+    assert norm_bwd(dt=3) == _lib.E_DTYPE
+    for k in ("dy", "w", "mean", "rstd", "dx"):
+        assert norm_bwd(**{k: None}) == _lib.E_NULL
+    assert norm_bwd(x=None) == _lib.E_NULL                   # neither x nor its checkpoint
+    assert norm_bwd(c=FAKE, e=FAKE) == _lib.E_NULL           # both
+    assert norm_bwd(x=None, c=FAKE) == _lib.E_NULL
+    assert norm_bwd(db=None) == _lib.E_NULL
+    need = _lib.lib().rwkv_layer_norm_backward_workspace_size(4, 64)
+    assert need > 0
+    assert norm_bwd(n=need - 1) == _lib.E_WORKSPACE
+    assert norm_bwd(ws=None) == _lib.E_WORKSPACE
+    assert norm_bwd(ws=HALF) == _lib.E_UNSUPPORTED
+    assert norm_bwd(dres=ODD) == _lib.E_UNSUPPORTED
+    assert norm_bwd(rows=-1) == _lib.E_SHAPE
+
+
+def test_checkpoint_refusals():
+    pack = lambda dt=BF16, x=FAKE, c=FAKE, e=FAKE, rows=4, D=64: st("rwkv_ckpt8_pack", dt, x, c, e, rows, D, None)
+    assert pack(dt=9) == _lib.E_DTYPE
+    for k in ("x", "c", "e"):
+        assert pack(**{k: None}) == _lib.E_NULL
+    assert pack(rows=0) == _lib.E_SHAPE
+    assert pack(D=-3) == _lib.E_SHAPE
+    assert pack(x=ODD) == _lib.E_UNSUPPORTED
+    vals = lambda act=0, dt=BF16, out=FAKE, rows=1: st("rwkv_ckpt8_values", FAKE, FAKE, act, dt, out, rows, 32, None)
+    assert vals(act=4) == _lib.E_UNSUPPORTED
+    assert vals(dt=5) == _lib.E_DTYPE
+    assert vals(out=None) == _lib.E_NULL
+    assert vals(rows=0) == _lib.E_SHAPE
+    back = lambda z=FAKE, c=None, e=None, act=1, dt=F32: st("rwkv_act_backward", dt, FAKE, z, c, e, act, FAKE, 2, 32, None)
+    assert back(z=None) == _lib.E_NULL
+    assert back(c=FAKE, e=FAKE) == _lib.E_NULL
+    assert back(act=-1) == _lib.E_UNSUPPORTED
+    assert back(dt=4) == _lib.E_DTYPE
+    assert back(z=ODD) == _lib.E_UNSUPPORTED
+
+
+def proj_fwd(dt=BF16, x=FAKE, w=FAKE, bdt=F32, b=None, act=0, ydt=BF16, res=None, y=FAKE, z=None, c=None, e=None,
+             rows=4096, OUT=2048, IN=2048, ws=None, n=0):
+    return st("rwkv_projection_forward", dt, x, w, bdt, b, act, ydt, res, y, z, c, e, rows, OUT, IN, ws, n, None)
+
+
+def test_projection_forward_refusals():
+    assert proj_fwd(dt=F32) == _lib.E_DTYPE
+    assert proj_fwd(ydt=F16) == _lib.E_DTYPE          # the operands' own type, or fp32
+    assert proj_fwd(b=FAKE, bdt=8) == _lib.E_DTYPE
+    for k in ("x", "w", "y"):
+        assert proj_fwd(**{k: None}) == _lib.E_NULL
+    assert proj_fwd(c=FAKE) == _lib.E_NULL
+    assert proj_fwd(rows=0) == _lib.E_SHAPE
+    assert proj_fwd(IN=0) == _lib.E_SHAPE
+    assert proj_fwd(rows=(1 << 26) + 1) == _lib.E_SHAPE
+    assert proj_fwd(IN=2044) == _lib.E_UNSUPPORTED
+    assert proj_fwd(OUT=2052) == _lib.E_UNSUPPORTED
+    assert proj_fwd(act=9) == _lib.E_UNSUPPORTED
+    assert proj_fwd(x=HALF) == _lib.E_UNSUPPORTED
+    need = _lib.lib().rwkv_projection_forward_workspace_size(64, 256, 8192)
+    assert need > 0
+    assert proj_fwd(rows=64, OUT=256, IN=8192, ws=FAKE, n=need - 1) == _lib.E_WORKSPACE
+    assert proj_fwd(rows=64, OUT=256, IN=8192) == _lib.E_WORKSPACE
+    assert _lib.lib().rwkv_projection_forward_workspace_size(0, 256, 8192) == 0
+
+
+def proj_dx(dt=BF16, dy=FAKE, w=FAKE, act=0, z=None, c=None, e=None, xdt=BF16, add=None, dx=FAKE, rows=4096, OUT=2048,
+            IN=2048, ws=None, n=0):
+    return st("rwkv_projection_dx", dt, dy, w, act, z, c, e, xdt, add, dx, rows, OUT, IN, ws, n, None)
+
+
+def test_projection_dx_refusals():
+    assert proj_dx(dt=F32) == _lib.E_DTYPE
+    assert proj_dx(xdt=F16) == _lib.E_DTYPE
+    for k in ("dy", "w", "dx"):
+        assert proj_dx(**{k: None}) == _lib.E_NULL
+    assert proj_dx(act=1) == _lib.E_NULL              # an activation needs its pre-activation
+    assert proj_dx(z=FAKE, c=FAKE, e=FAKE) == _lib.E_NULL
+    assert proj_dx(c=FAKE) == _lib.E_NULL
+    assert proj_dx(act=-2) == _lib.E_UNSUPPORTED
+    assert proj_dx(OUT=12) == _lib.E_UNSUPPORTED
+    assert proj_dx(add=HALF) == _lib.E_UNSUPPORTED
+    assert proj_dx(rows=-5) == _lib.E_SHAPE
+
+
+def proj_dw(dt=BF16, dy=FAKE, act=0, x=FAKE, c=None, e=None, wdt=BF16, dw=FAKE, db=None, rows=4096, OUT=2048, IN=2048,
+            ws=FAKE, n=1 << 40):
+    return st("rwkv_projection_dw", dt, dy, act, x, c, e, wdt, dw, db, rows, OUT, IN, ws, n, None)
+
+
+def test_projection_dw_refusals():
+    assert proj_dw(dt=F32) == _lib.E_DTYPE
+    assert proj_dw(wdt=F16) == _lib.E_DTYPE
+    assert proj_dw(dy=None) == _lib.E_NULL
+    assert proj_dw(dw=None) == _lib.E_NULL            # neither output
+    assert proj_dw(x=None) == _lib.E_NULL
+    assert proj_dw(c=FAKE, e=FAKE) == _lib.E_NULL
+    assert proj_dw(act=5) == _lib.E_UNSUPPORTED
+    assert proj_dw(IN=100) == _lib.E_UNSUPPORTED
+    assert proj_dw(rows=0) == _lib.E_SHAPE
+    L = _lib.lib()
+    dense = L.rwkv_projection_dw_workspace_size(4096, 2048, 2048, 0)
+    kept = L.rwkv_projection_dw_workspace_size(4096, 2048, 2048, 1)
+    assert kept >= dense + 4096 * 2048 * 2            # the restored operand
+    assert proj_dw(act=1, n=kept - 1) == _lib.E_WORKSPACE
+    assert proj_dw(db=ODD) == _lib.E_UNSUPPORTED
+
+
+def test_python_refusals_come_before_any_launch():
+    x = torch.zeros(4, 64)
+    with pytest.raises(ValueError, match="CUDA tensor"):
+        B.layerNormForward(x, torch.ones(64), torch.zeros(64))
+    with pytest.raises(ValueError, match="CUDA tensor"):
+        B.checkpoint8(x)
+    with pytest.raises(ValueError, match="CUDA tensor"):
+        B.projectionForward(x, torch.zeros(8, 64))
+    with pytest.raises(ValueError, match="activation"):
+        B.activationBackward(x, x, "gelu")
+    with pytest.raises(ValueError, match="activation"):
+        B.projectionForward(x, x, act="silu")
+
+
+def test_weight_gradient_without_x_asks_for_db_only(monkeypatch):
+    monkeypatch.setattr(B, "_tensor", lambda name, t, *a, **k: t)  # a CPU tensor as far as the check that raises
+    with pytest.raises(ValueError, match="only db"):
+        B.projectionBackwardWeight(torch.zeros(4, 64, dtype=torch.bfloat16), None)
+
+
+@pytest.mark.parametrize("rows,OUT,IN", [(1, 8, 8), (64, 2048, 8192), (129, 2048, 2048), (16384, 8192, 2048),
+                                         (4093, 96, 2048), (1000, 256, 10240)])
+def test_workspace_sizes_cover_split_partials(rows, OUT, IN):
+    """A split product's partials are whole fp32 copies of the result."""
+    L = _lib.lib()
+    for n, size in ((L.rwkv_projection_forward_workspace_size(rows, OUT, IN), rows * OUT * 4),
+                    (L.rwkv_projection_dx_workspace_size(rows, OUT, IN), rows * IN * 4)):
+        assert n % size == 0 and n // size != 1

@@ -1,0 +1,720 @@
+"""GPU tests of the block operators against plain implementations in 64 bits.
+
+Tolerances.  u(t) = finfo(t).eps / 2 bounds the relative error of one rounding
+to type t.  A sum of n terms taken in fp32 in any order is off by at most
+n 2^-24 sum|terms|; each term adds a few roundings of its own (counted as 16).
+The tensor core adds its products in fp32 with rounding of its own, in far
+fewer sequential steps than terms: 2^-20 sum|terms|, the bound that the
+projection-backward tests of the frozen base use too.  A result is then off by
+the error of its sums carried through the formula, plus its one rounding
+u(t) |result|.
+"""
+from __future__ import annotations
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+U32 = 2.0 ** -24
+TC = 2.0 ** -20
+
+
+def u(dt):
+    return torch.finfo(dt).eps / 2
+
+
+def rnd(shape, seed, dt=torch.float32, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(shape, generator=g, device="cuda") * scale).to(dt)
+
+
+def check(got, want, tol, what=""):
+    """|got - want| <= tol elementwise; NaN at the same places.  u(t) |x| bounds
+    a rounding only of normal numbers: below finfo.tiny a type's values are
+    tiny eps apart, so that a rounding there is off by up to tiny eps / 2, which
+    is added (fp16: 2^-14 2^-10 / 2 = 2^-25; the other types: below 1e-40)."""
+    f = torch.finfo(got.dtype)
+    tol = tol + f.tiny * f.eps / 2
+    got, want = got.double(), want.double()
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    fin = torch.isfinite(want)
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), what
+    off = (got - want).abs()[fin]
+    lim = tol.expand_as(want)[fin] if torch.is_tensor(tol) else tol
+    bad = ~(off <= lim)
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {off.numel()} beyond the bound, worst {float((off / lim).max()):.3g} of it"
+
+
+# ------------------------------------------------------------------ formulas
+
+def values64(x):
+    """What the checkpoint of x stands for, from the definition, in 64 bits."""
+    D = x.shape[-1]
+    v = torch.nn.functional.pad(x.double(), (0, -D % 32))
+    v = v.view(*x.shape[:-1], -1, 32)
+    top = v.abs().amax(-1, keepdim=True)
+    bad = ~torch.isfinite(top)
+    top = torch.where(bad, torch.ones_like(top), top)
+    e = torch.where(top > 0, torch.frexp(top).exponent - 7, -126).clamp(min=-126)
+    s = torch.ldexp(torch.ones_like(top), e)
+    q = torch.round(v / s).clamp(-127, 127) * s
+    q = torch.where(bad.expand_as(q), torch.full_like(q, float("nan")), q)
+    return q.flatten(-2)[..., :D]
+
+
+def top_of_group(x):
+    """max|x| of each element's group, as a tensor like x."""
+    D = x.shape[-1]
+    v = torch.nn.functional.pad(x.double(), (0, -D % 32)).view(*x.shape[:-1], -1, 32)
+    return v.abs().amax(-1, keepdim=True).expand_as(v).flatten(-2)[..., :D]
+
+
+def act64(z, act):
+    if act == "relu2":
+        return z.clamp(min=0) ** 2
+    return torch.tanh(z) if act == "tanh" else torch.sigmoid(z) if act == "sigmoid" else z
+
+
+def grad64(z, act):
+    if act == "relu2":
+        return 2 * z.clamp(min=0)
+    if act == "tanh":
+        return 1 / torch.cosh(z) ** 2
+    if act == "sigmoid":
+        return torch.sigmoid(z) * torch.sigmoid(-z)
+    return torch.ones_like(z)
+
+
+def slope(z, act, dz):
+    """A bound of |act(z + d) - act(z)| for |d| <= dz."""
+    if act == "relu2":
+        return (2 * z.abs() + dz) * dz
+    return dz
+
+
+# --------------------------------------------------------------- checkpoints
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,D", [(1, 1), (3, 31), (2, 32), (5, 40), (7, 33), (1, 2048), (257, 96), (64, 1000)])
+def test_checkpoint_is_its_definition(cuda, dt, rows, D):
+    from swiftrwkv_b200 import block as B
+    x = rnd((rows, D), 1, DTYPES[dt])
+    x[:, ::3] *= 1e-3
+    ck = B.checkpoint8(x)
+    assert ck.codes.shape == (rows, D) and ck.exps.shape == (rows, -(-D // 32))
+    want = values64(x)
+    got = B.checkpoint8Values(ck)
+    assert got.dtype == x.dtype and torch.equal(got.double(), want)       # exact in every type
+    assert torch.equal(B.checkpoint8Values(ck, dtype=torch.float32).double(), want)
+    assert bool(((want - x.double()).abs() <= top_of_group(x) / 127.5).all())
+    assert ck.nbytes == rows * (D + -(-D // 32))
+
+
+def test_checkpoint_of_extremes(cuda):
+    """Zeros, one huge value, the largest and smallest of the types, ties,
+    infinities and NaN (their group stands for NaN, others are unharmed)."""
+    from swiftrwkv_b200 import block as B
+    for dt in DTYPES.values():
+        f = torch.finfo(dt)
+        x = torch.zeros(8, 96, device="cuda", dtype=dt)
+        x[1, 5] = f.max
+        x[2, 40] = f.tiny
+        x[2, 41] = -f.smallest_normal
+        x[3, :] = f.max
+        x[4, :32] = torch.arange(32, device="cuda").to(dt) + 0.5      # top 31.5: ties at s = 1/4 do not occur
+        x[4, 32:64] = torch.arange(32, device="cuda").to(dt) * 4 + 2  # top 126, s = 1: exact
+        x[4, 64:] = torch.arange(32, device="cuda").to(dt) * 4 + 1.5  # ties to even at s = 1
+        x[5, 33] = float("inf")
+        x[6, 64] = float("nan")
+        x[7, 1] = -float("inf")
+        ck = B.checkpoint8(x)
+        got, want = B.checkpoint8Values(ck, dtype=torch.float32), values64(x)
+        assert torch.equal(torch.isnan(got), torch.isnan(want))
+        assert torch.equal(torch.nan_to_num(got.double(), nan=7.0), torch.nan_to_num(want, nan=7.0))
+        assert torch.isnan(got[5, 32:64]).all() and torch.isfinite(got[5, :32]).all() and torch.isfinite(got[5, 64:]).all()
+    sub = torch.full((1, 32), 1e-42, device="cuda")                   # far below the smallest scale
+    assert torch.equal(B.checkpoint8Values(B.checkpoint8(sub)), torch.zeros_like(sub))
+
+
+@pytest.mark.parametrize("act", ["none", "relu2", "tanh", "sigmoid"])
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,D", [(3, 31), (33, 96), (5, 200)])
+def test_checkpoint_uses(cuda, act, dt, rows, D):
+    """act(value) and dy * act'(value): elementary functions to 16 ulp of
+    fp32 (twice over in a product), one rounding."""
+    from swiftrwkv_b200 import block as B
+    t = DTYPES[dt]
+    x, dy = rnd((rows, D), 2, t, 3.0), rnd((rows, D), 3, t)
+    ck = B.checkpoint8(x)
+    v = values64(x)
+    tiny = torch.finfo(t).tiny * u(t) * 2      # half a subnormal step
+    y = act64(v, act)
+    check(B.checkpoint8Values(ck, act), y, y.abs() * (u(t) + 16 * U32) + tiny, "value")
+    for pre, z in ((ck, v), (x, x.double())):
+        w = dy.double() * grad64(z, act)
+        check(B.activationBackward(dy, pre, act), w, w.abs() * (u(t) + 32 * U32) + tiny, "gradient")
+
+
+def test_activation_gradient_matches_differences(cuda):
+    """act' against central differences of act, both the library's, fp32."""
+    from swiftrwkv_b200 import block as B
+    z = torch.linspace(-4, 4, 1024, device="cuda").view(32, 32)
+    h = 2.0 ** -6
+    for act in ("relu2", "tanh", "sigmoid"):
+        # the library's act on exact inputs: projections with the identity would round; use the checkpoint of a grid
+        zq = B.checkpoint8Values(B.checkpoint8(z))
+        up, dn = (act64(zq.double() + s * h, act) for s in (1, -1))
+        g = B.activationBackward(torch.ones_like(zq), zq, act)
+        # central difference: exact for a square away from 0; h^2/6 max|act'''| (<= 2) elsewhere, h at relu's kink
+        lim = 2 * h * h / 6 + 1e-5
+        off = (g.double() - (up - dn) / (2 * h)).abs()
+        near = zq.abs() <= h
+        assert bool((off[~near] <= lim).all()) and bool((off[near] <= h + lim).all())
+
+
+def test_activation_backward_may_write_over_dy(cuda):
+    from swiftrwkv_b200 import _lib, block as B
+    dy, z = rnd((65, 72), 5, torch.bfloat16), rnd((65, 72), 6, torch.bfloat16)
+    want = B.activationBackward(dy, z, "tanh")
+    buf = dy.clone()
+    _lib.call("rwkv_act_backward", _lib.BF16, buf.data_ptr(), z.data_ptr(), None, None, 2, buf.data_ptr(), 65, 72,
+              torch.cuda.current_stream().cuda_stream)
+    assert torch.equal(buf, want)
+
+
+# ----------------------------------------------------------------- layer norm
+
+NORM_SIZES = [(1, 1), (1, 2048), (3, 7), (5, 64), (17, 96), (2, 768), (33, 1003), (4, 2560), (3, 4096), (2, 8200), (1, 10240),
+              (2, 33000), (1003, 128)]
+
+
+def norm64(x, w, b, eps):
+    x = x.double()
+    mean = x.mean(-1, keepdim=True)
+    var = ((x - mean) ** 2).mean(-1, keepdim=True)
+    rstd = 1 / torch.sqrt(var + eps)
+    return (x - mean) * rstd * w.double() + b.double(), mean, rstd
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,D", NORM_SIZES)
+def test_layer_norm_forward(cuda, dt, rows, D):
+    from swiftrwkv_b200 import block as B
+    t = DTYPES[dt]
+    x = (rnd((rows, D), 7) * 2 + 0.5).to(t)
+    w, b = rnd((D,), 8) * 0.2 + 1, rnd((D,), 9) * 0.2
+    eps = 1e-5
+    y, mean, rstd, ck = B.layerNormForward(x, w, b, eps, checkpoint=True)
+    y64, m64, r64 = norm64(x, w, b, eps)
+    n = D + 16
+    dm = n * U32 * x.double().abs().mean(-1, keepdim=True)           # error of the mean
+    check(mean, m64[:, 0], dm[:, 0] + 2 * U32 * m64.abs()[:, 0], "mean")
+    dev = (x.double() - m64).abs()
+    # variance: terms off by 2 |d| dm + dm^2, the sum by n 2^-24; rstd by half its relative error
+    dvar = (2 * dev * dm + dm * dm).mean(-1, keepdim=True) + n * U32 * (dev ** 2).mean(-1, keepdim=True)
+    drel = 0.5 * dvar * r64 ** 2 * 1.01 + 8 * U32
+    check(rstd, r64[:, 0], (r64 * drel)[:, 0], "rstd")
+    tol = (w.double().abs() * r64 * (dm + dev * (drel + 4 * U32))) + 2 * U32 * (y64.abs() + b.double().abs())
+    check(y, y64, tol * 1.01 + u(t) * (y64.abs() + tol), "y")
+    assert torch.equal(B.checkpoint8Values(ck).double(), values64(x))
+    y2, _, _, none = B.layerNormForward(x, w, b, eps)
+    assert none is None and torch.equal(y2, y)
+
+
+@pytest.mark.parametrize("kept", [False, True])
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,D", NORM_SIZES)
+def test_layer_norm_backward(cuda, dt, kept, rows, D):
+    from swiftrwkv_b200 import block as B
+    t = DTYPES[dt]
+    x = (rnd((rows, D), 10) * 2 + 0.5).to(t)
+    w, b = rnd((D,), 11) * 0.2 + 1, rnd((D,), 12)
+    dy, dres = rnd((rows, D), 13, t), rnd((rows, D), 14, t)
+    _, mean, rstd, ck = B.layerNormForward(x, w, b, checkpoint=True)
+    dx, dw, db = B.layerNormBackward(dy, ck if kept else x, w, mean, rstd, dres=dres)
+    xv = values64(x) if kept else x.double()
+    m, r = mean.double()[:, None], rstd.double()[:, None]
+    h = (xv - m) * r
+    g = dy.double() * w.double()
+    along, mg = (g * h).mean(1, keepdim=True), g.mean(1, keepdim=True)
+    want = r * (g - mg - h * along) + dres.double()
+    n = (D + 16) * U32
+    hd = 3 * U32 * r * (xv.abs() + m.abs())                           # error of h
+    tol = r * (g.abs() * 4 * U32 + n * g.abs().mean(1, keepdim=True) +
+               h.abs() * (n * (g * h).abs().mean(1, keepdim=True) + (g.abs() * hd).mean(1, keepdim=True)) +
+               hd * along.abs()) + 8 * U32 * (r * (g.abs() + mg.abs() + (h * along).abs()) + dres.double().abs())
+    check(dx, want, tol * 1.01 + u(t) * (want.abs() + tol), "dx")
+    k = (rows + 16) * U32
+    check(dw, (dy.double() * h).sum(0), k * (dy.double() * h).abs().sum(0) + (dy.double().abs() * hd).sum(0) + 1e-38, "dw")
+    check(db, dy.double().sum(0), k * dy.double().abs().sum(0) + 1e-38, "db")
+    dx2, none, _ = B.layerNormBackward(dy, ck if kept else x, w, mean, rstd, dres=dres, params=False)
+    assert none is None and torch.equal(dx2, dx)
+    dx3, dw3, db3 = B.layerNormBackward(dy, ck if kept else x, w, mean, rstd, dres=dres)
+    assert torch.equal(dx3, dx) and torch.equal(dw3, dw) and torch.equal(db3, db)   # deterministic
+
+
+def test_layer_norm_gradient_matches_differences(cuda):
+    """The gradients against central differences of the forward in fp32: 1e-2
+    of the largest gradient at a step of 2^-6 (the forward's own error,
+    about 1e-6, divided by the step, and the third derivative)."""
+    from swiftrwkv_b200 import block as B
+    x, w, b, dy = rnd((4, 24), 15), rnd((24,), 16) * 0.2 + 1, rnd((24,), 17), rnd((4, 24), 18)
+    f = lambda: (B.layerNormForward(x, w, b)[0].double() * dy.double()).sum()
+    _, mean, rstd, _ = B.layerNormForward(x, w, b)
+    grads = B.layerNormBackward(dy, x, w, mean, rstd)
+    for p, g in zip((x, w, b), grads):
+        flat, gf = p.view(-1), g.reshape(-1)
+        for i in range(0, flat.numel(), 7):
+            keep = float(flat[i])
+            flat[i] = keep + 2.0 ** -6
+            up = f()
+            flat[i] = keep - 2.0 ** -6
+            dn = f()
+            flat[i] = keep
+            assert abs(float(up - dn) * 2 ** 5 - float(gf[i])) < 1e-2 * float(g.abs().max())
+
+
+def test_layer_norm_constant_rows_and_nan(cuda):
+    """A constant row (variance 0) gives bias and finite gradients; a NaN or an
+    infinity stays in its row."""
+    from swiftrwkv_b200 import block as B
+    x = rnd((6, 96), 19, torch.bfloat16)
+    x[1] = 3.0
+    x[3, 7] = float("nan")
+    x[4, 50] = float("inf")
+    w, b, dy = rnd((96,), 20), rnd((96,), 21), rnd((6, 96), 22, torch.bfloat16)
+    y, mean, rstd, ck = B.layerNormForward(x, w, b, checkpoint=True)
+    assert torch.equal(y[1], b.to(torch.bfloat16))
+    assert torch.isnan(y[3]).all() and torch.isfinite(y[[0, 1, 2, 5]]).all() and torch.isnan(y[4]).any()
+    dx, dw, _ = B.layerNormBackward(dy, x, w, mean, rstd)
+    assert torch.isfinite(dx[[0, 1, 2, 5]]).all() and torch.isnan(dx[3]).all()
+    assert torch.isnan(dw).any()
+
+
+def test_layer_norm_types_and_views(cuda):
+    """Parameters in 16 bits, non-contiguous and misaligned inputs, leading
+    dimensions, no rows."""
+    from swiftrwkv_b200 import block as B
+    x, w, b = rnd((2, 3, 64), 23, torch.bfloat16), rnd((64,), 24, torch.bfloat16), rnd((64,), 25, torch.bfloat16)
+    y, mean, rstd, _ = B.layerNormForward(x, w, b)
+    ref, _, _, _ = B.layerNormForward(x, w.float(), b.float())
+    assert mean.shape == (2, 3) and torch.equal(y, ref)
+    dy = rnd((2, 3, 64), 26, torch.bfloat16)
+    _, dw, db = B.layerNormBackward(dy, x, w, mean, rstd)
+    _, dw32, db32 = B.layerNormBackward(dy, x, w.float(), mean, rstd)
+    assert dw.dtype == torch.bfloat16 and torch.equal(dw, dw32.to(dw.dtype)) and torch.equal(db, db32.to(db.dtype))
+    big = rnd((2, 65, 3), 27, torch.bfloat16)
+    v = big[:, :64].transpose(1, 2)                       # strided
+    assert torch.equal(B.layerNormForward(v, w, b)[0], B.layerNormForward(v.contiguous(), w, b)[0])
+    flat = rnd((6 * 64 + 1,), 28, torch.bfloat16)
+    odd = flat[1:].view(6, 64)                            # 2-byte aligned rows take the scalar kernel
+    n = 64 + 16
+    a, m = B.layerNormForward(odd, w, b)[0], B.layerNormForward(odd.clone(), w, b)[0]
+    assert bool(((a.double() - m.double()).abs() <= (2 * u(torch.bfloat16) + n * 16 * U32) * (m.double().abs() + 1)).all())
+    y0, mean0, _, ck0 = B.layerNormForward(x[:, :0], w, b, checkpoint=True)
+    assert y0.shape == (2, 0, 64) and mean0.shape == (2, 0) and ck0.codes.shape == (2, 0, 64)
+    dx0, dw0, db0 = B.layerNormBackward(dy[:, :0], x[:, :0], w, mean0, mean0)
+    assert dx0.shape == (2, 0, 64) and not dw0.any() and not db0.any()
+
+
+# ---------------------------------------------------------------- projections
+
+PROJ_SIZES = [(1, 8, 8), (1, 2048, 2048), (2, 24, 72), (3, 8192, 264), (7, 104, 2048), (16, 256, 1000), (17, 64, 64), (33, 520, 136),
+              (64, 2048, 4096), (128, 128, 64), (129, 264, 72), (300, 96, 2048), (1000, 2048, 96), (257, 1032, 520),
+              (2051, 768, 768)]
+
+
+def proj_sums(a, b):
+    """sum over the last dim of a b^T, and of |a| |b|^T, in 64 bits."""
+    a, b = a.double(), b.double()
+    return a @ b.t(), a.abs() @ b.abs().t()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("rows,OUT,IN", PROJ_SIZES)
+def test_projection_forward(cuda, dt, rows, OUT, IN):
+    from swiftrwkv_b200 import block as B
+    t = DTYPES[dt]
+    x, w = rnd((rows, IN), 30, t), rnd((OUT, IN), 31, t, IN ** -0.5)
+    z0, s0 = proj_sums(x, w)
+    y, none = B.projectionForward(x, w)
+    assert none is None and y.dtype == t
+    check(y, z0, TC * s0 + u(t) * (z0.abs() + TC * s0), "plain")
+    f, _ = B.projectionForward(x, w, out_dtype=torch.float32)
+    check(f, z0, TC * s0 + U32 * z0.abs(), "fp32 out")
+    bias, res = rnd((OUT,), 32), rnd((rows, OUT), 33, t)
+    z, dz = z0 + bias.double(), TC * (s0 + bias.double().abs())
+    for act in ("none", "relu2", "tanh", "sigmoid"):
+        want = act64(z, act) + res.double()
+        tol = slope(z, act, dz) + 32 * U32 * (act64(z, act).abs() + want.abs())
+        y, ck = B.projectionForward(x, w, bias, act, res, checkpoint=True)
+        check(y, want, tol + u(t) * (want.abs() + tol), act)
+        y2, pre = B.projectionForward(x, w, bias, act, res, preactivation=True)
+        assert torch.equal(y2, y)
+        check(pre, z, dz + u(t) * (z.abs() + dz), "z")
+        # a code stands for z up to a 127.5th of its group's largest, both as the kernel saw them
+        v = B.checkpoint8Values(ck, dtype=torch.float32)
+        check(v, z, (top_of_group(z) + top_of_group(dz)) / 127.5 + top_of_group(dz), "checkpoint")
+    h, _ = B.projectionForward(x, w, bias.to(t), "none", res)
+    zb = z0 + bias.to(t).double() + res.double()
+    tb = TC * s0 + 4 * U32 * (z0.abs() + 1 + res.double().abs() + bias.double().abs())
+    check(h, zb, tb + u(t) * (zb.abs() + tb), "16-bit bias")
+    f, _ = B.projectionForward(x, w, bias, "sigmoid", res.float(), out_dtype=torch.float32)
+    want = act64(z, "sigmoid") + res.double()
+    check(f, want, dz + 32 * U32 * (1 + want.abs()), "fp32 out with epilogue")
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("rows,OUT,IN", PROJ_SIZES)
+def test_projection_backward_input(cuda, dt, rows, OUT, IN):
+    from swiftrwkv_b200 import block as B
+    t = DTYPES[dt]
+    dy, w = rnd((rows, OUT), 34, t), rnd((OUT, IN), 35, t, OUT ** -0.5)
+    g, s = proj_sums(dy, w.t())
+    dx = B.projectionBackwardInput(dy, w)
+    check(dx, g, TC * s + u(t) * (g.abs() + TC * s), "plain")
+    z, add = rnd((rows, IN), 36, t), rnd((rows, IN), 37, t)
+    ck = B.checkpoint8(z)
+    for act in ("none", "relu2", "tanh", "sigmoid"):
+        for pre, zv in ((z, z.double()), (ck, values64(z))):
+            d = grad64(zv, act)
+            want = g * d + add.double()
+            tol = TC * s * d.abs() + 64 * U32 * ((g * d).abs() + want.abs())
+            got = B.projectionBackwardInput(dy, w, pre=pre, act=act, addend=add)
+            check(got, want, tol + u(t) * (want.abs() + tol), act)
+    f = B.projectionBackwardInput(dy, w, pre=ck, act="relu2", addend=add.float(), out_dtype=torch.float32)
+    d = grad64(values64(z), "relu2")
+    want = g * d + add.double()
+    check(f, want, TC * s * d + 64 * U32 * ((g * d).abs() + want.abs() + add.double().abs()), "fp32 out")
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("rows,OUT,IN", PROJ_SIZES)
+def test_projection_backward_weight(cuda, dt, rows, OUT, IN):
+    from swiftrwkv_b200 import block as B
+    t = DTYPES[dt]
+    dy, x = rnd((rows, OUT), 38, t), rnd((rows, IN), 39, t)
+    want, s = proj_sums(dy.t(), x.t())
+    dw, db = B.projectionBackwardWeight(dy, x, bias=True)
+    check(dw, want, TC * s + u(t) * (want.abs() + TC * s), "dense")
+    dbs = dy.double().abs().sum(0)
+    check(db, dy.double().sum(0), (rows + 16) * U32 * dbs + 1e-38, "db")
+    none, db2 = B.projectionBackwardWeight(dy, None, bias=True)
+    assert none is None and torch.equal(db2, db)
+    ck = B.checkpoint8(x)
+    v = values64(x)
+    want, s = proj_sums(dy.t(), v.t())
+    f, none = B.projectionBackwardWeight(dy, ck, out_dtype=torch.float32)
+    assert none is None
+    check(f, want, TC * s + U32 * want.abs(), "checkpoint, fp32 out")     # the operand is exact
+    for act in ("relu2", "tanh", "sigmoid"):
+        for op, zv in ((ck, v), (x, x.double())):
+            want, s = proj_sums(dy.t(), act64(zv, act).t())
+            # each operand value rounded once: by u(t) of it, or by half of the
+            # subnormal spacing tiny eps where it is below tiny (fp16 squares are)
+            sub = torch.finfo(t).tiny * torch.finfo(t).eps / 2 * dy.double().abs().sum(0)[:, None]
+            tol = (u(t) + 16 * U32 + TC) * s + sub
+            got, _ = B.projectionBackwardWeight(dy, op, act=act)
+            check(got, want, tol + u(t) * (want.abs() + tol), act)
+
+
+def test_projection_results_repeat(cuda):
+    """Split products and column sums are joined in a fixed order."""
+    from swiftrwkv_b200 import block as B
+    x, w, dy = rnd((700, 2048), 40, torch.bfloat16), rnd((96, 2048), 41, torch.bfloat16), rnd((700, 96), 42, torch.bfloat16)
+    first = (B.projectionForward(x, w)[0], B.projectionBackwardInput(dy, w), *B.projectionBackwardWeight(dy, x, bias=True))
+    for _ in range(3):
+        again = (B.projectionForward(x, w)[0], B.projectionBackwardInput(dy, w),
+                 *B.projectionBackwardWeight(dy, x, bias=True))
+        assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+@pytest.mark.parametrize("rows,OUT,IN", [(5, 72, 64), (200, 264, 1032)])
+def test_projection_leaves_what_lies_behind_its_outputs(cuda, rows, OUT, IN):
+    """Outputs inside larger buffers: nothing past their end is written."""
+    from swiftrwkv_b200 import _lib
+    t = torch.bfloat16
+    x, w = rnd((rows, IN), 43, t), rnd((OUT, IN), 44, t)
+    n, groups = rows * OUT, rows * -(-OUT // 32)
+    y = torch.full((n + 4096,), 7.0, device="cuda", dtype=t)
+    z = torch.full((n + 4096,), 7.0, device="cuda", dtype=t)
+    codes = torch.full((n + 4096,), 7, device="cuda", dtype=torch.int8)
+    exps = torch.full((groups + 4096,), 7, device="cuda", dtype=torch.uint8)
+    nb = _lib.lib().rwkv_projection_forward_workspace_size(rows, OUT, IN)
+    ws = torch.full((nb + 4096,), 7, device="cuda", dtype=torch.uint8)
+    _lib.call("rwkv_projection_forward", _lib.BF16, x.data_ptr(), w.data_ptr(), 0, None, 1, _lib.BF16, None, y.data_ptr(),
+              z.data_ptr(), codes.data_ptr(), exps.data_ptr(), rows, OUT, IN, ws.data_ptr(), nb,
+              torch.cuda.current_stream().cuda_stream)
+    for buf, k in ((y, n), (z, n), (codes, n), (exps, groups), (ws, nb)):
+        assert bool((buf[k:] == 7).all())
+
+
+def test_projection_residual_may_be_the_output(cuda):
+    from swiftrwkv_b200 import _lib, block as B
+    for rows, OUT, IN in ((64, 256, 4096), (1000, 512, 128), (1, 512, 512)):
+        x, w, res = rnd((rows, IN), 45, torch.float16), rnd((OUT, IN), 46, torch.float16, 0.02), rnd((rows, OUT), 47, torch.float16)
+        want, _ = B.projectionForward(x, w, residual=res)
+        nb = _lib.lib().rwkv_projection_forward_workspace_size(rows, OUT, IN)
+        ws = torch.empty(max(nb, 16), device="cuda", dtype=torch.uint8)
+        buf = res.clone()
+        _lib.call("rwkv_projection_forward", _lib.F16, x.data_ptr(), w.data_ptr(), 0, None, 0, _lib.F16, buf.data_ptr(),
+                  buf.data_ptr(), None, None, None, rows, OUT, IN, ws.data_ptr(), nb, torch.cuda.current_stream().cuda_stream)
+        assert torch.equal(buf, want)
+
+
+def test_projection_views_and_empty_batches(cuda):
+    from swiftrwkv_b200 import block as B
+    t = torch.bfloat16
+    big, wb = rnd((3, 5, 2 * 64 + 3), 48, t), rnd((72, 65), 49, t)
+    x, w = big[..., 1:65], wb[:, 1:]                       # strided, misaligned
+    y, _ = B.projectionForward(x, w)
+    assert y.shape == (3, 5, 72) and torch.equal(y, B.projectionForward(x.contiguous(), w.contiguous())[0])
+    flat = rnd((64 * 64 + 3,), 50, t)[3:].view(64, 64)     # contiguous at an odd address
+    assert torch.equal(B.projectionForward(flat, w)[0], B.projectionForward(flat.clone(), w)[0])
+    v = rnd((64,), 51, t)                                  # no leading dimension
+    assert torch.equal(B.projectionForward(v, w)[0], B.projectionForward(v[None], w)[0][0])
+    y0, ck0 = B.projectionForward(x[:0], w, checkpoint=True)
+    assert y0.shape == (0, 5, 72) and ck0.exps.shape == (0, 5, 3)
+    assert B.projectionBackwardInput(y0, w).shape == (0, 5, 64)
+    dw0, db0 = B.projectionBackwardWeight(y0, x[:0], bias=True)
+    assert dw0.shape == (72, 64) and not dw0.any() and not db0.any()
+
+
+def test_projection_of_infinities_and_nan(cuda):
+    """A NaN or an infinity of x stays in its row, one of w in its column."""
+    from swiftrwkv_b200 import block as B
+    t = torch.bfloat16
+    x, w = rnd((200, 136), 52, t), rnd((72, 136), 53, t)
+    x[5, 100] = float("nan")
+    x[150, 3] = float("inf")
+    w[60, 7] = float("nan")
+    for act in ("none", "relu2", "tanh", "sigmoid"):
+        y, ck = B.projectionForward(x, w, act=act, checkpoint=True)
+        rows = torch.ones(200, dtype=torch.bool, device="cuda")
+        rows[[5, 150]] = False
+        cols = torch.ones(72, dtype=torch.bool, device="cuda")
+        cols[60] = False
+        assert torch.isnan(y[5]).all() and torch.isnan(y[:, 60]).all()
+        assert torch.isfinite(y[rows][:, cols]).all()
+        v = B.checkpoint8Values(ck)
+        assert torch.isnan(v[5]).all() and torch.isnan(v[:, 32:64]).all() and torch.isfinite(v[rows][:, :32]).all()
+    dy = rnd((200, 72), 54, t)
+    dx = B.projectionBackwardInput(dy, w[:, :], pre=x, act="relu2")
+    assert torch.isnan(dx[:, 7]).all()
+    dw, _ = B.projectionBackwardWeight(dy, x)
+    assert torch.isnan(dw[:, 100]).all() and torch.isfinite(dw[:, 4:100]).all()
+
+
+def test_python_refusals_on_cuda_tensors(cuda):
+    from swiftrwkv_b200 import block as B
+    x, w = rnd((4, 64), 55, torch.bfloat16), rnd((72, 64), 56, torch.bfloat16)
+    bad = [lambda: B.projectionForward(x.float(), w), lambda: B.projectionForward(x, w.half()),
+           lambda: B.projectionForward(x, w[:, :56]), lambda: B.projectionForward(x[:, :60], w[:, :60]),
+           lambda: B.projectionForward(x, w, residual=x), lambda: B.projectionForward(x, w, out_dtype=torch.float16),
+           lambda: B.projectionForward(x, w, bias=torch.zeros(71, device="cuda")),
+           lambda: B.projectionForward(x, w, checkpoint=True, preactivation=True),
+           lambda: B.projectionForward(x, w, bias=torch.zeros(72)),
+           lambda: B.projectionBackwardInput(rnd((4, 72), 1, torch.bfloat16), w, act="tanh"),
+           lambda: B.projectionBackwardInput(x, w), lambda: B.projectionBackwardWeight(x, w),
+           lambda: B.layerNormForward(x, torch.ones(63, device="cuda"), torch.zeros(64, device="cuda")),
+           lambda: B.layerNormForward(x, torch.ones(64, device="cuda"), torch.zeros(64, device="cuda").half()),
+           lambda: B.layerNormForward(x.double(), torch.ones(64, device="cuda"), torch.zeros(64, device="cuda")),
+           lambda: B.layerNormBackward(x, x.half(), torch.ones(64, device="cuda"), *torch.zeros(2, 4, device="cuda")),
+           lambda: B.layerNormBackward(x, x, torch.ones(64, device="cuda"), *torch.zeros(2, 5, device="cuda")),
+           lambda: B.activationBackward(x, x[:2], "tanh"), lambda: B.checkpoint8(x.to(torch.int8)),
+           lambda: B.activationBackward(x, B.Checkpoint8(x.to(torch.int8), torch.zeros(4, 3, dtype=torch.uint8, device="cuda"),
+                                                         x.dtype), "tanh")]
+    for i, f in enumerate(bad):
+        with pytest.raises(ValueError):
+            f()
+            pytest.fail(f"call {i} was taken")
+
+
+# ------------------------------------------------- streams, graphs, together
+
+def test_two_streams_at_once(cuda):
+    """Calls on two streams, each with its own workspace, agree with calls made
+    one after the other."""
+    from swiftrwkv_b200 import block as B
+    t = torch.bfloat16
+    cases = [(rnd((700, 1024), s, t), rnd((256, 1024), s + 9, t), rnd((700, 256), s + 17, t)) for s in (60, 61)]
+    def work(x, w, dy):
+        y, ck = B.projectionForward(x, w, act="tanh", checkpoint=True)
+        return y, B.activationBackward(dy, ck, "tanh"), B.projectionBackwardInput(dy, w), *B.projectionBackwardWeight(dy, x, bias=True)
+    want = [work(*c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(5):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[k].append(work(*cases[k]))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for g in got[k]:
+            assert all(torch.equal(a, b) for a, b in zip(g, want[k]))
+
+
+def test_captured_calls_replay_on_new_inputs(cuda):
+    """The explicit calls captured into two graphs, replayed in turn with new
+    inputs in the captured buffers."""
+    from swiftrwkv_b200 import block as B
+    t = torch.bfloat16
+    w1, w2 = rnd((512, 256), 70, t, 0.06), rnd((256, 512), 71, t, 0.06)
+    g, b = rnd((256,), 72) * 0.1 + 1, rnd((256,), 73)
+    def step(x, dy):
+        h, mean, rstd, ckx = B.layerNormForward(x, g, b, checkpoint=True)
+        k, ck = B.projectionForward(h, w1, act="relu2", checkpoint=True)
+        y, _ = B.projectionForward(k, w2, residual=x)
+        dz = B.projectionBackwardInput(dy, w2, pre=ck, act="relu2")
+        dw2, _ = B.projectionBackwardWeight(dy, ck, act="relu2")
+        dw1, db1 = B.projectionBackwardWeight(dz, h, bias=True)
+        dh = B.projectionBackwardInput(dz, w1)
+        return [y, dw1, db1, dw2, *B.layerNormBackward(dh, ckx, g, mean, rstd, dres=dy)]
+    bufs, graphs = [], []
+    for rows in (40, 300):
+        x, dy = rnd((rows, 256), 74, t), rnd((rows, 256), 75, t)
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            step(x, dy)
+        torch.cuda.current_stream().wait_stream(s)
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            out = step(x, dy)
+        bufs.append((x, dy, out))
+        graphs.append(gr)
+    for seed in (80, 81):
+        for k, rows in enumerate((40, 300)):
+            bufs[k][0].copy_(rnd((rows, 256), seed, t))
+            bufs[k][1].copy_(rnd((rows, 256), seed + 10, t))
+            graphs[k].replay()
+        for k in range(2):
+            x, dy, out = bufs[k]
+            assert all(torch.equal(a, c) for a, c in zip(out, step(x, dy)))
+
+
+def test_differentiable_forms_refuse_capture(cuda):
+    from swiftrwkv_b200 import block as B
+    x = rnd((4, 64), 76, torch.bfloat16).requires_grad_(True)
+    w, b = torch.ones(64, device="cuda"), torch.zeros(64, device="cuda")
+    B.layerNorm(x.detach(), w, b)
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        with pytest.raises(ValueError, match="capture"):
+            B.layerNorm(x, w, b)
+        y = B.layerNorm(x.detach(), w, b)       # nothing is recorded: taken
+    gr.replay()
+    assert torch.equal(y, B.layerNorm(x.detach(), w, b))
+
+
+def block_run(B, x, p, checkpoint):
+    """ln -> low-rank branch (tanh, sigmoid with bias) -> cmix projections with
+    the residual, as a block runs them."""
+    h = B.layerNorm(x, p["g"], p["b"], checkpoint=checkpoint)
+    d = B.projection(h, p["down"], act="tanh", checkpoint=checkpoint)
+    s = B.projection(d, p["up"], bias=p["up_b"], act="sigmoid", residual=h, checkpoint=checkpoint)
+    return B.channelMix(s, p["key"], p["value"], residual=x, checkpoint=checkpoint)
+
+
+class Block64:
+    """The same operators in 64 bits under torch's autograd."""
+    @staticmethod
+    def layerNorm(x, g, b, checkpoint):
+        return torch.nn.functional.layer_norm(x, x.shape[-1:], g, b, 1e-5)
+
+    @staticmethod
+    def projection(x, w, bias=None, act="none", residual=None, checkpoint=False):
+        z = x @ w.t()
+        z = act64(z if bias is None else z + bias, act)
+        return z if residual is None else z + residual
+
+    @staticmethod
+    def channelMix(x, key, value, residual=None, checkpoint=True):
+        return torch.relu(x @ key.t()) ** 2 @ value.t() + residual
+
+
+@pytest.mark.parametrize("checkpoint", [False, True])
+@pytest.mark.parametrize("rows", [1, 37, 600])
+def test_block_run_and_its_gradients(cuda, checkpoint, rows):
+    """Outputs and every gradient of a run of the operators against the same
+    run in 64 bits.  In the 2-norm: about ten roundings to bf16 along the
+    longest path, each at most 2^-8 and of either sign, sqrt(10) 2^-8 = 1.3 %,
+    bound 4 %; with checkpoints four activations are read back with an error
+    of up to a 128th of their group's largest, about 1 % each in the 2-norm:
+    bound 8 %."""
+    from swiftrwkv_b200 import block as B
+    D, R, F, t = 256, 64, 1024, torch.bfloat16
+    p = {"g": rnd((D,), 90) * 0.1 + 1, "b": rnd((D,), 91) * 0.1, "down": rnd((R, D), 92, t, D ** -0.5),
+         "up": rnd((D, R), 93, t, R ** -0.5), "up_b": rnd((D,), 94), "key": rnd((F, D), 95, t, D ** -0.5),
+         "value": rnd((D, F), 96, t, F ** -0.5)}
+    x = rnd((rows, D), 97, t)
+    dy = rnd((rows, D), 98, t)
+    p = {k: v.requires_grad_(True) for k, v in p.items()}
+    x.requires_grad_(True)
+    y = block_run(B, x, p, checkpoint)
+    y.backward(dy)
+    p64 = {k: v.detach().double().requires_grad_(True) for k, v in p.items()}
+    x64 = x.detach().double().requires_grad_(True)
+    y64 = block_run(Block64, x64, p64, checkpoint)
+    y64.backward(dy.double())
+    lim = 0.08 if checkpoint else 0.04
+    rel = lambda a, b: float((a.double() - b).norm() / b.norm())
+    assert rel(y.detach(), y64.detach()) < 0.04
+    for name, a, b in [("x", x.grad, x64.grad)] + [(k, p[k].grad, p64[k].grad) for k in p]:
+        assert a.dtype == (x.dtype if name == "x" else p[name].dtype)
+        assert rel(a, b) < lim, (name, rel(a, b))
+
+
+def test_differentiable_forms_compute_what_is_needed(cuda):
+    """Frozen weights, frozen inputs and a bias alone; no gradient, no graph."""
+    from swiftrwkv_b200 import block as B
+    t = torch.bfloat16
+    x, w, b = rnd((20, 64), 100, t), rnd((72, 64), 101, t, 0.1), rnd((72,), 102, t)
+    dy = rnd((20, 72), 103, t)
+    assert not B.projection(x, w, b, "tanh").requires_grad
+    grads = []
+    for need in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 1, 1)):
+        ts = [v.clone().requires_grad_(bool(n)) for v, n in zip((x, w, b), need)]
+        B.projection(*ts, "tanh").backward(dy)
+        assert [v.grad is not None for v in ts] == [bool(n) for n in need]
+        grads.append([v.grad for v in ts])
+    for k in range(3):
+        assert torch.equal(grads[k][k], grads[3][k])
+    xs = x.clone().requires_grad_(True)
+    with torch.no_grad():
+        assert not B.channelMix(xs, rnd((128, 64), 104, t), rnd((64, 128), 105, t)).requires_grad
+
+
+def test_checkpoint_saves_memory_for_the_backward_pass(cuda):
+    """What a checkpointed channelMix keeps between forward and backward: codes
+    and exponents of x and z, no 16-bit activation."""
+    from swiftrwkv_b200 import block as B
+    t, rows, D, F = torch.bfloat16, 512, 256, 1024
+    key, value = rnd((F, D), 106, t).requires_grad_(True), rnd((D, F), 107, t).requires_grad_(True)
+    x = rnd((rows, D), 108, t)
+    kept = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda s: kept.append(s) or s, lambda s: s):
+        B.channelMix(x, key, value)
+    acts = [s for s in kept if s.data_ptr() not in (key.data_ptr(), value.data_ptr())]
+    assert sum(s.numel() * s.element_size() for s in acts) == rows * (D + F) * 33 // 32
+
+
+def test_wait_errors_are_reported_by_the_projections(cuda):
+    """The projections share the tensor-core GEMMs' wait-error record: a set
+    host record is reported once, and the next call is right."""
+    from swiftrwkv_b200 import _lib, block as B
+    t = torch.bfloat16
+    x, w = rnd((300, 256), 110, t), rnd((256, 256), 111, t)
+    want, _ = B.projectionForward(x, w)
+    _lib.call("rwkv_q_gemm_inject_wait_error", 1, torch.cuda.current_stream().cuda_stream)
+    with pytest.raises(_lib.RWKVError) as err:
+        B.projectionForward(x, w)
+    assert err.value.status == _lib.E_TIMEOUT
+    assert torch.equal(B.projectionForward(x, w)[0], want)
+    _lib.call("rwkv_q_gemm_inject_wait_error", 0, torch.cuda.current_stream().cuda_stream)
+    B.projectionBackwardInput(x, w)                       # skips its work: the device flag is set
+    assert _lib.status("rwkv_q_gemm_status", torch.cuda.current_stream().cuda_stream) == _lib.E_TIMEOUT
+    assert torch.equal(B.projectionForward(x, w)[0], want)
