@@ -61,14 +61,21 @@ class Checkpoint8:
 
 # ---------------------------------------------------------------- plumbing
 
+# what torch.cuda.current_device() and current_stream(...).cuda_stream return,
+# without building a Stream object (2 us of a small call's 10)
+_current_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
 def _call(dev, name, *args):
     """An entry point on `dev` and its current stream (appended)."""
     L = _lib.lib()
-    if dev.index == torch.cuda.current_device():
-        st = getattr(L, name)(*args, torch.cuda.current_stream(dev).cuda_stream)
+    k = dev.index
+    if k == _current_device():
+        st = getattr(L, name)(*args, _raw_stream(k))
     else:
         with torch.cuda.device(dev):
-            st = getattr(L, name)(*args, torch.cuda.current_stream(dev).cuda_stream)
+            st = getattr(L, name)(*args, _raw_stream(k))
     if st:
         raise _lib.RWKVError(name, st, L.rwkv_last_error().decode())
 
@@ -184,10 +191,10 @@ def layerNormForward(x, weight, bias, eps: float = 1e-5, checkpoint: bool = Fals
     weight = _tensor("weight", weight, dev, None, (D,))
     bias = _tensor("bias", bias, dev, (weight.dtype,), (D,))
     y = torch.empty_like(x)
-    stats = torch.empty((2,) + x.shape[:-1], device=dev, dtype=torch.float32)
-    mean, rstd = stats[0], stats[1]
+    mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    rstd = torch.empty_like(mean)
     ck = _new_checkpoint(x.shape, dev, x.dtype) if checkpoint else None
-    rows = _rows(x.shape)
+    rows = x.numel() // D
     if rows:
         _call(dev, "rwkv_layer_norm_forward", _DT[x.dtype], x.data_ptr(), _DT[weight.dtype], weight.data_ptr(),
               bias.data_ptr(), eps, y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), ck and ck.codes.data_ptr(),
@@ -253,7 +260,7 @@ def projectionForward(x, w, bias=None, act: str = "none", residual=None, checkpo
         raise ValueError(f"projectionForward: out_dtype {ydt} (x's own type or fp32)")
     shape = x.shape[:-1] + (OUT,)
     if bias is not None:
-        bias = _tensor("bias", bias, dev, None, (OUT,))
+        bias = _aligned(_tensor("bias", bias, dev, None, (OUT,)))
     if residual is not None:
         residual = _aligned(_tensor("residual", residual, dev, (ydt,), shape))
     y = torch.empty(shape, device=dev, dtype=ydt)

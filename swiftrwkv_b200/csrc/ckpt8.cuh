@@ -14,6 +14,8 @@
 // element.
 #pragma once
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace rwkv {
@@ -42,46 +44,90 @@ __device__ __forceinline__ float ck_scale(uint32_t e) { return __uint_as_float(e
 __device__ __forceinline__ int ck_code(float x, float inv) {
     return max(-127, min(127, __float2int_rn(__fmul_rn(x, inv))));
 }
+// Four codes as a word.  x / s + 1.5 2^23 is rounded once, to the integer round(x
+// / s) above 1.5 2^23, whose low byte is the code; clipping is on that scale.
+// One fused multiply-add and two min / max per code, where a conversion to
+// integer runs at a quarter of the rate.
 __device__ __forceinline__ uint32_t ck_pack4(float a, float b, float c, float d, float inv) {
-    return (uint32_t)(ck_code(a, inv) & 255) | ((uint32_t)(ck_code(b, inv) & 255) << 8) |
-           ((uint32_t)(ck_code(c, inv) & 255) << 16) | ((uint32_t)(ck_code(d, inv) & 255) << 24);
+    constexpr float M = 12582912.f;
+    auto code = [inv](float x) {
+        return __float_as_uint(fminf(fmaxf(fmaf(x, inv, M), M - 127.f), M + 127.f));
+    };
+    const uint32_t w = __byte_perm(__byte_perm(code(a), code(b), 0x0040), __byte_perm(code(c), code(d), 0x0040), 0x5410);
+    return inv == 0.f ? 0u : w;  // a NaN group
 }
-// The four values of a word of codes.  Byte ^ 0x80 is q + 128; placed in the
-// low mantissa of 2^23 it reads 2^23 + q + 128 exactly.
-__device__ __forceinline__ void ck_unpack4(uint32_t w, float s, float* v) {
+// Bits of the largest |x| of a 16-byte vector of T, comparable across a group
+// (for 16-bit types in 16 bits, compared two at a time), and its fp32 form.
+template <typename T>
+__device__ __forceinline__ uint32_t top_bits(const uint4& r) {
+    if constexpr (sizeof(T) == 4) {
+        return max(max(r.x & 0x7fffffffu, r.y & 0x7fffffffu), max(r.z & 0x7fffffffu, r.w & 0x7fffffffu));
+    } else {
+        const uint32_t m = __vmaxu2(__vmaxu2(r.x & 0x7fff7fffu, r.y & 0x7fff7fffu),
+                                    __vmaxu2(r.z & 0x7fff7fffu, r.w & 0x7fff7fffu));
+        return max(m >> 16, m & 0xffffu);
+    }
+}
+template <typename T>
+__device__ __forceinline__ uint32_t top_f32(uint32_t top) {
+    if constexpr (sizeof(T) == 4) return top;
+    else if constexpr (std::is_same_v<T, __nv_bfloat16>) return top << 16;
+    else return abs_bits(__half2float(__ushort_as_half((unsigned short)top)));
+}
+// The four codes of a word as floats.  Byte ^ 0x80 is q + 128; placed in the low
+// mantissa of 2^23 it reads 2^23 + q + 128 exactly.
+__device__ __forceinline__ void ck_codes4(uint32_t w, float* q) {
     w ^= 0x80808080u;
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-        v[i] = (__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7440u | (uint32_t)i)) - 8388736.f) * s;
+    for (int i = 0; i < 4; i++) q[i] = __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7440u | (uint32_t)i)) - 8388736.f;
+}
+__device__ __forceinline__ void ck_unpack4(uint32_t w, float s, float* v) {
+    ck_codes4(w, v);
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] *= s;
 }
 
 // ---------------------------------------------------------------- activations
 
-// act(z).  Comparisons are written so that a NaN passes through.
-template <int ACT>
+// act(z) and act'(z).  Comparisons are written so that a NaN passes through.
+// tanh and sigmoid and their derivatives come from e = exp(-2|z|) or exp(-|z|),
+// which is at most 1, so that nothing overflows and no derivative cancels:
+//   tanh = (1 - e) / (1 + e) with z's sign, tanh' = 4 e / (1 + e)^2
+//   sigmoid = (1 or e) / (1 + e) by z's sign, sigmoid' = e / (1 + e)^2
+// FAST: __expf and __fdividef, relative errors of about 2^-19 over the range
+// where the result is not negligible, for results that are rounded to 16 bits
+// or come out of a tensor-core sum; below |z| = 2^-6, where 1 - e cancels,
+// tanh z = z - z^3 / 3 (next term z^5 2/15 < 2^-26 z).  Otherwise expf, tanhf
+// and IEEE division.
+template <int ACT, bool FAST>
 __device__ __forceinline__ float act_t(float z) {
     if constexpr (ACT == RWKV_ACT_RELU2) {
         const float m = z < 0.f ? 0.f : z;
         return m * m;
     } else if constexpr (ACT == RWKV_ACT_TANH) {
-        return tanhf(z);
+        if constexpr (!FAST) return tanhf(z);
+        const float e = __expf(-2.f * fabsf(z));
+        const float t = copysignf(__fdividef(1.f - e, 1.f + e), z);
+        return fabsf(z) < 0.015625f ? fmaf(z * z * z, -1.f / 3.f, z) : t;
     } else if constexpr (ACT == RWKV_ACT_SIGMOID) {
-        return 1.f / (1.f + expf(-z));
+        if constexpr (!FAST) return 1.f / (1.f + expf(-z));
+        const float e = __expf(-fabsf(z));
+        return __fdividef(z < 0.f ? e : 1.f, 1.f + e);
     }
     return z;
 }
-// act'(z).  tanh' = 4 e / (1 + e)^2 with e = exp(-2|z|) and sigmoid' =
-// e / (1 + e)^2 with e = exp(-|z|): no cancellation for large |z|.
-template <int ACT>
+template <int ACT, bool FAST>
 __device__ __forceinline__ float act_grad_t(float z) {
     if constexpr (ACT == RWKV_ACT_RELU2) {
         return z < 0.f ? 0.f : 2.f * z;
-    } else if constexpr (ACT == RWKV_ACT_TANH) {
-        const float e = expf(-2.f * fabsf(z)), d = 1.f + e;
-        return 4.f * e / (d * d);
-    } else if constexpr (ACT == RWKV_ACT_SIGMOID) {
-        const float e = expf(-fabsf(z)), d = 1.f + e;
-        return e / (d * d);
+    } else if constexpr (ACT == RWKV_ACT_TANH || ACT == RWKV_ACT_SIGMOID) {
+        constexpr float k = ACT == RWKV_ACT_TANH ? 2.f : 1.f;
+        if constexpr (!FAST) {
+            const float e = expf(-k * fabsf(z)), d = 1.f + e;
+            return k * k * e / (d * d);
+        }
+        const float e = __expf(-k * fabsf(z)), r = __fdividef(k, 1.f + e);
+        return e * r * r;
     }
     return 1.f;
 }
@@ -114,6 +160,35 @@ struct Vec16 {
     }
 };
 
+// VE (4 or 8) consecutive elements of a parameter vector kept in fp32, bf16 or
+// fp16, from a 16-byte aligned vector; one element of it.
+template <int VE>
+__device__ __forceinline__ void load_params(const void* p, int dtype, int64_t i, float* v) {
+    if (dtype == RWKV_F32) {
+#pragma unroll
+        for (int k = 0; k < VE; k += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i + k);
+            v[k] = f.x, v[k + 1] = f.y, v[k + 2] = f.z, v[k + 3] = f.w;
+        }
+        return;
+    }
+    uint32_t w[VE / 2];
+    const uint32_t* q = reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(p) + i);
+    if constexpr (VE == 8) {
+        const uint4 r = *reinterpret_cast<const uint4*>(q);
+        w[0] = r.x, w[1] = r.y, w[2] = r.z, w[3] = r.w;
+    } else {
+        const uint2 r = *reinterpret_cast<const uint2*>(q);
+        w[0] = r.x, w[1] = r.y;
+    }
+#pragma unroll
+    for (int k = 0; k < VE / 2; k++) {
+        const float2 f = dtype == RWKV_BF16 ? make_float2(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u))
+                                            : __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+        v[2 * k] = f.x;
+        v[2 * k + 1] = f.y;
+    }
+}
 // One element of a parameter vector kept in fp32, bf16 or fp16.
 __device__ __forceinline__ float load_param(const void* p, int dtype, int64_t i) {
     if (dtype == RWKV_F32) return static_cast<const float*>(p)[i];

@@ -109,8 +109,13 @@ __device__ __forceinline__ void proj_epilogue32(float* v, const ProjEpi& e, int6
     const int64_t at = row * N + col;
     if (e.bias) {
 #pragma unroll
-        for (int i = 0; i < 32; i++)
-            if (i < nv) v[i] += load_param(e.bias, e.bias_dtype, col + i);
+        for (int i = 0; i < 4; i++)
+            if (8 * i < nv) {
+                float b[8];
+                load_params<8>(e.bias, e.bias_dtype, col + 8 * i, b);
+#pragma unroll
+                for (int k = 0; k < 8; k++) v[8 * i + k] += b[k];
+            }
     }
     if (e.codes) {
         uint32_t top = 0;
@@ -151,12 +156,12 @@ __device__ __forceinline__ void proj_epilogue32(float* v, const ProjEpi& e, int6
         with_act(e.act, [&]<int ACT>() {
 #pragma unroll
             for (int i = 0; i < 32; i++)
-                if (i < nv) v[i] *= act_grad_t<ACT>(p[i]);
+                if (i < nv) v[i] *= act_grad_t<ACT, true>(p[i]);
         });
     } else {
         with_act(e.act, [&]<int ACT>() {
 #pragma unroll
-            for (int i = 0; i < 32; i++) v[i] = act_t<ACT>(v[i]);
+            for (int i = 0; i < 32; i++) v[i] = act_t<ACT, true>(v[i]);
         });
     }
     if (e.add) {

@@ -11,6 +11,8 @@
 // in registers between its passes.  Rows are read in 16-byte vectors; the raw
 // vectors are kept (half the registers of fp32 for 16-bit types) and unpacked
 // in each pass.
+#include <algorithm>
+
 #include "ckpt8.cuh"
 
 namespace rwkv {
@@ -47,10 +49,12 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
 }
 
 // TPR threads per row (32: a warp, several rows per block; else one block per
-// row), at most NV vectors per thread: vector j of thread t is t + j TPR.
+// row), at most NV vectors per thread: vector j of thread t is t + j TPR.  Rows
+// of at most 80 elements per thread are held in fp32, longer ones as read.
 template <typename T, int TPR, int NV>
 __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) ln_fwd_kernel(const LnFwdArgs a) {
     constexpr int VE = Vec16<T>::N;
+    constexpr bool F32 = NV * VE <= 80;
     __shared__ float red[32];
     const int t = threadIdx.x & (TPR - 1);
     const int64_t row = TPR == 32 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
@@ -61,12 +65,36 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) ln_fwd_kernel(const LnF
 #pragma unroll
     for (int j = 0; j < NV; j++) {
         const int v = t + j * TPR;
-        raw[j] = v < nvec ? xr[v] : make_uint4(0, 0, 0, 0);
+        raw[j] = v < nvec ? __ldcs(xr + v) : make_uint4(0, 0, 0, 0);
     }
+    if (a.codes) {
+        // a group of 32 channels is 32 / VE neighbouring threads
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            const int v = t + j * TPR;
+            uint32_t top = top_bits<T>(raw[j]);
+#pragma unroll
+            for (int o = 1; o < CK_GROUP / VE; o *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const uint32_t e = ck_exponent(top_f32<T>(top));
+            const float inv = ck_inv_scale(e);
+            if (v < nvec) {
+                float f[VE];
+                Vec16<T>::unpack(raw[j], f);
+                int8_t* c = a.codes + row * a.D + (int64_t)v * VE;
+                if constexpr (VE == 8)
+                    *reinterpret_cast<uint2*>(c) = make_uint2(ck_pack4(f[0], f[1], f[2], f[3], inv),
+                                                              ck_pack4(f[4], f[5], f[6], f[7], inv));
+                else
+                    *reinterpret_cast<uint32_t*>(c) = ck_pack4(f[0], f[1], f[2], f[3], inv);
+                if (v % (CK_GROUP / VE) == 0) a.exps[row * a.G + v / (CK_GROUP / VE)] = (uint8_t)e;
+            }
+        }
+    }
+    float x[F32 ? NV : 1][VE];
     float s = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; j++) {
-        float f[VE];
+        float* f = x[F32 ? j : 0];
         Vec16<T>::unpack(raw[j], f);
 #pragma unroll
         for (int k = 0; k < VE; k++) s += f[k];
@@ -75,8 +103,8 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) ln_fwd_kernel(const LnF
     float q = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; j++) {
-        float f[VE];
-        Vec16<T>::unpack(raw[j], f);
+        float* f = x[F32 ? j : 0];
+        if constexpr (!F32) Vec16<T>::unpack(raw[j], f);
         if (t + j * TPR < nvec) {
 #pragma unroll
             for (int k = 0; k < VE; k++) {
@@ -86,6 +114,7 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) ln_fwd_kernel(const LnF
         }
     }
     const float rstd = 1.f / sqrtf(row_sum<TPR>(q, red) / (float)a.D + a.eps);
+    const float shift = -mean * rstd;
     if (t == 0 && a.mean) {
         a.mean[row] = mean;
         a.rstd[row] = rstd;
@@ -94,39 +123,67 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) ln_fwd_kernel(const LnF
 #pragma unroll
     for (int j = 0; j < NV; j++) {
         const int v = t + j * TPR;
-        float f[VE];
-        Vec16<T>::unpack(raw[j], f);
-        if (a.codes) {
-            // a group of 32 channels is 32 / VE neighbouring threads
-            uint32_t top = 0;
-#pragma unroll
-            for (int k = 0; k < VE; k++) top = max(top, abs_bits(f[k]));
-#pragma unroll
-            for (int o = 1; o < CK_GROUP / VE; o *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const uint32_t e = ck_exponent(top);
-            const float inv = ck_inv_scale(e);
-            if (v < nvec) {
-                uint32_t* c = reinterpret_cast<uint32_t*>(a.codes + row * a.D + (int64_t)v * VE);
-#pragma unroll
-                for (int k = 0; k < VE; k += 4) c[k / 4] = ck_pack4(f[k], f[k + 1], f[k + 2], f[k + 3], inv);
-                if (v % (CK_GROUP / VE) == 0) a.exps[row * a.G + v / (CK_GROUP / VE)] = (uint8_t)e;
-            }
-        }
         if (v < nvec) {
+            float* f = x[F32 ? j : 0];
+            if constexpr (!F32) Vec16<T>::unpack(raw[j], f);
+            float w[VE], b[VE];
+            load_params<VE>(a.w, a.wdtype, v * VE, w);
+            load_params<VE>(a.b, a.wdtype, v * VE, b);
 #pragma unroll
-            for (int k = 0; k < VE; k++)
-                f[k] = fmaf((f[k] - mean) * rstd, load_param(a.w, a.wdtype, v * VE + k),
-                            load_param(a.b, a.wdtype, v * VE + k));
-            yr[v] = Vec16<T>::pack(f);
+            for (int k = 0; k < VE; k++) f[k] = fmaf(fmaf(f[k], rstd, shift), w[k], b[k]);
+            __stcs(yr + v, Vec16<T>::pack(f));
         }
     }
 }
 
-// Any length and alignment: a block per row, single elements, the row re-read
-// (from L1 / L2) in each pass.  y may be x: every element is read for the last
-// time by the thread that writes it, after the sums.
+// Any alignment: single elements, element j of thread t is t + j TPR (a warp's
+// 32 elements are a checkpoint group), at most NE per thread, in registers.
+template <typename T, int TPR, int NE>
+__global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) ln_fwd_any_kernel(const LnFwdArgs a) {
+    __shared__ float red[32];
+    const int t = threadIdx.x & (TPR - 1);
+    const int64_t row = TPR == 32 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
+    if (row >= a.rows) return;
+    const T* xr = static_cast<const T*>(a.x) + row * a.D;
+    T* yr = static_cast<T*>(a.y) + row * a.D;
+    float x[NE];
+#pragma unroll
+    for (int j = 0; j < NE; j++) x[j] = t + j * TPR < a.D ? to_f<T>(xr[t + j * TPR]) : 0.f;
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < NE; j++) s += x[j];
+    const float mean = row_sum<TPR>(s, red) / (float)a.D;
+    float q = 0.f;
+#pragma unroll
+    for (int j = 0; j < NE; j++) {
+        const float d = t + j * TPR < a.D ? x[j] - mean : 0.f;
+        q = fmaf(d, d, q);
+    }
+    const float rstd = 1.f / sqrtf(row_sum<TPR>(q, red) / (float)a.D + a.eps);
+    if (t == 0 && a.mean) {
+        a.mean[row] = mean;
+        a.rstd[row] = rstd;
+    }
+#pragma unroll
+    for (int j = 0; j < NE; j++) {
+        const int i = t + j * TPR;
+        if (a.codes) {
+            const uint32_t e = ck_exponent(__reduce_max_sync(0xffffffffu, abs_bits(x[j])));
+            if (i < a.D) {
+                a.codes[row * a.D + i] = (int8_t)ck_code(x[j], ck_inv_scale(e));
+                if (i % CK_GROUP == 0) a.exps[row * a.G + i / CK_GROUP] = (uint8_t)e;
+            }
+        }
+        if (i < a.D)
+            yr[i] = from_f<T>(fmaf((x[j] - mean) * rstd, load_param(a.w, a.wdtype, i), load_param(a.b, a.wdtype, i)));
+    }
+}
+
+// Any length: a block per row, the row re-read (from L1 / L2) in each pass.  y
+// may be x: every element is read for the last time by the thread that writes
+// it, after the sums.
 template <typename T>
-__global__ void __launch_bounds__(256) ln_fwd_any_kernel(const LnFwdArgs a) {
+__global__ void __launch_bounds__(256) ln_fwd_long_kernel(const LnFwdArgs a) {
     __shared__ float red[32];
     const int64_t row = blockIdx.x;
     const T* xr = static_cast<const T*>(a.x) + row * a.D;
@@ -164,14 +221,27 @@ template <typename T>
 int launch_ln_fwd(const LnFwdArgs& a, bool vec, cudaStream_t st) {
     const int nvec = a.D / Vec16<T>::N;
     if (vec && nvec <= 32 * 16) {
-        const int grid = ceil_div(a.rows, 4);
-        if (nvec <= 32 * 4) ln_fwd_kernel<T, 32, 4><<<grid, 128, 0, st>>>(a);
-        else if (nvec <= 32 * 8) ln_fwd_kernel<T, 32, 8><<<grid, 128, 0, st>>>(a);
+        const int grid = ceil_div(a.rows, 4), nv = ceil_div(nvec, 32);
+        if (nv <= 2) ln_fwd_kernel<T, 32, 2><<<grid, 128, 0, st>>>(a);
+        else if (nv <= 4) ln_fwd_kernel<T, 32, 4><<<grid, 128, 0, st>>>(a);
+        else if (nv <= 6) ln_fwd_kernel<T, 32, 6><<<grid, 128, 0, st>>>(a);
+        else if (nv <= 8) ln_fwd_kernel<T, 32, 8><<<grid, 128, 0, st>>>(a);
+        else if (nv <= 10) ln_fwd_kernel<T, 32, 10><<<grid, 128, 0, st>>>(a);
         else ln_fwd_kernel<T, 32, 16><<<grid, 128, 0, st>>>(a);
+    } else if (vec && nvec <= 256 * 4) {
+        ln_fwd_kernel<T, 256, 4><<<a.rows, 256, 0, st>>>(a);
     } else if (vec && nvec <= 512 * 8) {
         ln_fwd_kernel<T, 512, 8><<<a.rows, 512, 0, st>>>(a);
+    } else if (a.D <= 32 * 32) {
+        const int grid = ceil_div(a.rows, 4);
+        if (a.D <= 32 * 8) ln_fwd_any_kernel<T, 32, 8><<<grid, 128, 0, st>>>(a);
+        else ln_fwd_any_kernel<T, 32, 32><<<grid, 128, 0, st>>>(a);
+    } else if (a.D <= 256 * 40) {
+        if (a.D <= 256 * 8) ln_fwd_any_kernel<T, 256, 8><<<a.rows, 256, 0, st>>>(a);
+        else if (a.D <= 256 * 16) ln_fwd_any_kernel<T, 256, 16><<<a.rows, 256, 0, st>>>(a);
+        else ln_fwd_any_kernel<T, 256, 40><<<a.rows, 256, 0, st>>>(a);
     } else {
-        ln_fwd_any_kernel<T><<<a.rows, 256, 0, st>>>(a);
+        ln_fwd_long_kernel<T><<<a.rows, 256, 0, st>>>(a);
     }
     return check_launch("ln_fwd_kernel");
 }
@@ -192,112 +262,187 @@ struct LnBwdArgs {
     int wdtype, rows, D, G;
 };
 
-// A block takes R rows at a time, blockIdx.x R + i, with stride gridDim.x R;
-// thread t owns the vectors t + j blockDim.x of every row, so its sums over
-// rows of dy h and dy stay in registers until the end.  One barrier per R rows
-// (the two row sums of R rows in one exchange, buffers alternating).
+// The sums over a warp of N values per lane (N a power of two), value i in the
+// lanes i 32 / N .. : each exchange halves the values a lane holds, so that N
+// sums take N - 1 + log2(32 / N) shuffles instead of 5 N.
+template <int N>
+__device__ __forceinline__ float lanes_sum(float* v, int lane) {
+#pragma unroll
+    for (int n = N, o = 16; n > 1; n /= 2, o /= 2) {
+        const bool up = lane & o;
+#pragma unroll
+        for (int i = 0; i < n / 2; i++) {
+            const float keep = up ? v[i + n / 2] : v[i], send = up ? v[i] : v[i + n / 2];
+            v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+        }
+    }
+    float s = v[0];
+#pragma unroll
+    for (int o = 16 / N; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    return s;
+}
+
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* dst, const void* src) {
+    const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(d), "l"(src), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+constexpr int LN_STAGES = 3;
+
+// A block takes R rows at a time, R (blockIdx.x + i gridDim.x); thread t owns
+// the vectors t + j blockDim.x of every row, so its sums over rows of dy h and
+// dy stay in registers until the end.  dy, x (or its codes) and dres run
+// LN_STAGES - 1 steps ahead through a ring in shared memory; a thread copies
+// (cp.async) and reads only its own vectors, so the ring needs no barrier, and
+// HBM stays busy while the block computes and waits at its barrier: one per R
+// rows, for the two row sums (buffers alternating).
 template <typename T, bool CK, int NV, int R>
 __global__ void __launch_bounds__(512) ln_bwd_kernel(const LnBwdArgs a) {
     constexpr int VE = Vec16<T>::N;
-    __shared__ float2 red[2][R][16];
+    extern __shared__ uint4 ring[];  // [stage][row][dy | x | dres][NV][thread]
+    __shared__ float red[2][16][2 * R];
     const int t = threadIdx.x, nt = blockDim.x, warp = t >> 5, lane = t & 31, nw = nt >> 5;
     const int nvec = a.D / VE;
     const float inv_d = 1.f / (float)a.D;
     float w[NV][VE], sw[NV][VE], sb[NV][VE];
 #pragma unroll
-    for (int j = 0; j < NV; j++)
+    for (int j = 0; j < NV; j++) {
+        const int v = t + j * nt;
 #pragma unroll
-        for (int k = 0; k < VE; k++) {
-            const int v = t + j * nt;
-            w[j][k] = v < nvec ? load_param(a.w, a.wdtype, v * VE + k) : 0.f;
-            sw[j][k] = sb[j][k] = 0.f;
-        }
-    int buf = 0;
-    for (int64_t r0 = (int64_t)blockIdx.x * R; r0 < a.rows; r0 += (int64_t)gridDim.x * R, buf ^= 1) {
-        uint4 rdy[R][NV], rx[R][NV];
-        float mean[R], rstd[R];
+        for (int k = 0; k < VE; k++) w[j][k] = sw[j][k] = sb[j][k] = 0.f;
+        if (v < nvec) load_params<VE>(a.w, a.wdtype, (int64_t)v * VE, w[j]);
+    }
+    const int64_t step = (int64_t)gridDim.x * R;
+    auto slot = [&](int stage, int r, int part, int j) { return ring + (((stage * R + r) * 3 + part) * NV + j) * nt + t; };
+    auto fetch = [&](int64_t r0, int stage) {
 #pragma unroll
-        for (int r = 0; r < R; r++) {
-            const int64_t row = r0 + r;
-            const bool ok = row < a.rows;
-            mean[r] = ok ? a.mean[row] : 0.f;
-            rstd[r] = ok ? a.rstd[row] : 0.f;
+        for (int r = 0; r < R; r++)
 #pragma unroll
             for (int j = 0; j < NV; j++) {
                 const int v = t + j * nt;
-                rdy[r][j] = rx[r][j] = make_uint4(0, 0, 0, 0);
-                if (ok && v < nvec) {
-                    const int64_t at = row * a.D + (int64_t)v * VE;
-                    rdy[r][j] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.dy) + at);
-                    if constexpr (CK) {
-                        const uint32_t* c = reinterpret_cast<const uint32_t*>(a.codes + at);
-                        rx[r][j].x = c[0];
-                        if constexpr (VE == 8) rx[r][j].y = c[1];
-                        rx[r][j].z = a.exps[row * a.G + v / (CK_GROUP / VE)];
-                    } else {
-                        rx[r][j] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + at);
-                    }
+                if (r0 + r < a.rows && v < nvec) {
+                    const int64_t at = (r0 + r) * a.D + (int64_t)v * VE;
+                    copy_async<16>(slot(stage, r, 0, j), static_cast<const T*>(a.dy) + at);
+                    if constexpr (CK) copy_async<VE>(slot(stage, r, 1, j), a.codes + at);
+                    else copy_async<16>(slot(stage, r, 1, j), static_cast<const T*>(a.x) + at);
+                    if (a.dres) copy_async<16>(slot(stage, r, 2, j), static_cast<const T*>(a.dres) + at);
+                }
+            }
+        copy_commit();
+    };
+    // the rows' statistics and exponents, one step ahead in registers
+    float mean[R], rstd[R], nmean[R], nrstd[R];
+    uint32_t ex[R][NV], nex[R][NV];
+    auto fetch_small = [&](int64_t r0) {
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const bool ok = r0 + r < a.rows;
+            nmean[r] = ok ? a.mean[r0 + r] : 0.f;
+            nrstd[r] = ok ? a.rstd[r0 + r] : 0.f;
+            if constexpr (CK) {
+#pragma unroll
+                for (int j = 0; j < NV; j++) {
+                    const int v = t + j * nt;
+                    nex[r][j] = ok && v < nvec ? a.exps[(r0 + r) * a.G + v / (CK_GROUP / VE)] : 0u;
                 }
             }
         }
-        // h of a vector (0 beyond the row's end)
-        auto normed = [&](int r, int j, float* h) {
-            if constexpr (CK) {
-                const float s = ck_scale(rx[r][j].z);
-                ck_unpack4(rx[r][j].x, s, h);
-                if constexpr (VE == 8) ck_unpack4(rx[r][j].y, s, h + 4);
-            } else {
-                Vec16<T>::unpack(rx[r][j], h);
-            }
+    };
+    const int64_t first = (int64_t)blockIdx.x * R;
 #pragma unroll
-            for (int k = 0; k < VE; k++) h[k] = (h[k] - mean[r]) * rstd[r];
-        };
+    for (int i = 0; i < LN_STAGES - 1; i++) fetch(first + i * step, i);
+    fetch_small(first);
+    int stage = 0, buf = 0;
+    for (int64_t r0 = first; r0 < a.rows; r0 += step, buf ^= 1) {
+        fetch(r0 + (LN_STAGES - 1) * step, stage == 0 ? LN_STAGES - 1 : stage - 1);
+        copy_wait<LN_STAGES - 1>();
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            float s1 = 0.f, s2 = 0.f;
+            mean[r] = nmean[r];
+            rstd[r] = nrstd[r];
+            if constexpr (CK)
+#pragma unroll
+                for (int j = 0; j < NV; j++) ex[r][j] = nex[r][j];
+        }
+        fetch_small(r0 + step);
+        // pass 1: h, the sums over the row (g, g h) and over the rows (dy h, dy)
+        float h[R][NV][VE], rs[2 * R];
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            rs[2 * r] = rs[2 * r + 1] = 0.f;
 #pragma unroll
             for (int j = 0; j < NV; j++) {
-                float dy[VE], h[VE];
-                Vec16<T>::unpack(rdy[r][j], dy);
-                normed(r, j, h);
+                if (r0 + r >= a.rows || t + j * nt >= nvec) continue;
+                float dy[VE];
+                Vec16<T>::unpack(*slot(stage, r, 0, j), dy);
+                const float shift = -mean[r] * rstd[r];
+                float scale = rstd[r];
+                if constexpr (CK) {
+                    const uint32_t* c = reinterpret_cast<const uint32_t*>(slot(stage, r, 1, j));
+                    ck_codes4(c[0], h[r][j]);
+                    if constexpr (VE == 8) ck_codes4(c[1], h[r][j] + 4);
+                    scale *= ck_scale(ex[r][j]);
+                } else {
+                    Vec16<T>::unpack(*slot(stage, r, 1, j), h[r][j]);
+                }
 #pragma unroll
                 for (int k = 0; k < VE; k++) {
+                    h[r][j][k] = fmaf(h[r][j][k], scale, shift);
                     const float g = dy[k] * w[j][k];
-                    s1 += g;
-                    s2 = fmaf(g, h[k], s2);
-                    sw[j][k] = fmaf(dy[k], h[k], sw[j][k]);
+                    rs[2 * r] += g;
+                    rs[2 * r + 1] = fmaf(g, h[r][j][k], rs[2 * r + 1]);
+                    sw[j][k] = fmaf(dy[k], h[r][j][k], sw[j][k]);
                     sb[j][k] += dy[k];
                 }
             }
-            s1 = warp_sum(s1);
-            s2 = warp_sum(s2);
-            if (lane == 0) red[buf][r][warp] = make_float2(s1, s2);
         }
+        // over the warp: value i ends up in lanes 16 i / R .. (32 / 2R lanes each)
+        constexpr int N = 2 * R, L = 32 / N;
+        const float p = lanes_sum<N>(rs, lane);
+        if (lane % L == 0) red[buf][warp][lane / L] = p;
         __syncthreads();
+        float tot = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16 / L + (16 % L != 0); i++) {
+            const int k = lane % L + i * L;
+            if (k < nw) tot += red[buf][k][lane / L];
+        }
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1) tot += __shfl_xor_sync(0xffffffffu, tot, o);
+        tot *= inv_d;
+        // pass 2: dx = rstd (g - m1 - h m2) + dres
 #pragma unroll
         for (int r = 0; r < R; r++) {
+            const float c0 = -rstd[r] * __shfl_sync(0xffffffffu, tot, 2 * r * L);
+            const float c1 = -rstd[r] * __shfl_sync(0xffffffffu, tot, (2 * r + 1) * L);
             const int64_t row = r0 + r;
-            float2 p = lane < nw ? red[buf][r][lane] : make_float2(0.f, 0.f);
-            const float m1 = warp_sum(p.x) * inv_d, m2 = warp_sum(p.y) * inv_d;
-            if (row >= a.rows) continue;
 #pragma unroll
             for (int j = 0; j < NV; j++) {
                 const int v = t + j * nt;
-                if (v >= nvec) continue;
-                float dy[VE], h[VE], o[VE];
-                Vec16<T>::unpack(rdy[r][j], dy);
-                normed(r, j, h);
-                const int64_t at = row * a.D + (int64_t)v * VE;
-                if (a.dres) Vec16<T>::unpack(*reinterpret_cast<const uint4*>(static_cast<const T*>(a.dres) + at), o);
+                if (row >= a.rows || v >= nvec) continue;
+                float dy[VE], o[VE];
+                Vec16<T>::unpack(*slot(stage, r, 0, j), dy);
+                if (a.dres) {
+                    Vec16<T>::unpack(*slot(stage, r, 2, j), o);
 #pragma unroll
-                for (int k = 0; k < VE; k++) {
-                    const float d = rstd[r] * (dy[k] * w[j][k] - m1 - h[k] * m2);
-                    o[k] = a.dres ? o[k] + d : d;
+                    for (int k = 0; k < VE; k++) o[k] += c0;
+                } else {
+#pragma unroll
+                    for (int k = 0; k < VE; k++) o[k] = c0;
                 }
-                *reinterpret_cast<uint4*>(static_cast<T*>(a.dx) + at) = Vec16<T>::pack(o);
+#pragma unroll
+                for (int k = 0; k < VE; k++) o[k] = fmaf(dy[k] * w[j][k], rstd[r], fmaf(h[r][j][k], c1, o[k]));
+                __stcs(reinterpret_cast<uint4*>(static_cast<T*>(a.dx) + row * a.D + (int64_t)v * VE), Vec16<T>::pack(o));
             }
         }
+        stage = stage == LN_STAGES - 1 ? 0 : stage + 1;
     }
+    copy_wait<0>();
     if (!a.part) return;
     float* p = a.part + (int64_t)blockIdx.x * 2 * a.D;
 #pragma unroll
@@ -319,10 +464,70 @@ __device__ __forceinline__ float bwd_x(const LnBwdArgs& a, int64_t row, int i) {
     else return to_f<T>(static_cast<const T*>(a.x)[row * a.D + i]);
 }
 
-// Any length and alignment.  dx: a block per row, single elements.  dx may be
-// dy, so the column sums (ln_bwd_cols_any_kernel) are launched first.
+// Any alignment: a block per row at a time, single elements, element t + j NT of
+// thread t, at most NE; the sums over rows stay in registers.
+template <typename T, bool CK, int NT, int NE>
+__global__ void __launch_bounds__(NT) ln_bwd_any_kernel(const LnBwdArgs a) {
+    __shared__ float2 red[2][NT / 32];
+    const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+    const float inv_d = 1.f / (float)a.D;
+    float w[NE], sw[NE], sb[NE];
+#pragma unroll
+    for (int j = 0; j < NE; j++) {
+        w[j] = t + j * NT < a.D ? load_param(a.w, a.wdtype, t + j * NT) : 0.f;
+        sw[j] = sb[j] = 0.f;
+    }
+    int buf = 0;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, buf ^= 1) {
+        const T* dyr = static_cast<const T*>(a.dy) + row * a.D;
+        const float mean = a.mean[row], rstd = a.rstd[row];
+        float dy[NE], h[NE];
+#pragma unroll
+        for (int j = 0; j < NE; j++) {
+            const int i = t + j * NT;
+            dy[j] = i < a.D ? to_f<T>(dyr[i]) : 0.f;
+            h[j] = i < a.D ? bwd_x<T, CK>(a, row, i) : 0.f;
+        }
+        float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int j = 0; j < NE; j++) {
+            h[j] = t + j * NT < a.D ? (h[j] - mean) * rstd : 0.f;
+            const float g = dy[j] * w[j];
+            s1 += g;
+            s2 = fmaf(g, h[j], s2);
+            sw[j] = fmaf(dy[j], h[j], sw[j]);
+            sb[j] += dy[j];
+        }
+        s1 = warp_sum(s1);
+        s2 = warp_sum(s2);
+        if (lane == 0) red[buf][warp] = make_float2(s1, s2);
+        __syncthreads();
+        const float2 p = lane < NT / 32 ? red[buf][lane] : make_float2(0.f, 0.f);
+        const float m1 = warp_sum(p.x) * inv_d, m2 = warp_sum(p.y) * inv_d;
+#pragma unroll
+        for (int j = 0; j < NE; j++) {
+            const int i = t + j * NT;
+            if (i >= a.D) break;
+            float d = rstd * (dy[j] * w[j] - m1 - h[j] * m2);
+            if (a.dres) d += to_f<T>(static_cast<const T*>(a.dres)[row * a.D + i]);
+            static_cast<T*>(a.dx)[row * a.D + i] = from_f<T>(d);
+        }
+    }
+    if (!a.part) return;
+    float* p = a.part + (int64_t)blockIdx.x * 2 * a.D;
+#pragma unroll
+    for (int j = 0; j < NE; j++) {
+        const int i = t + j * NT;
+        if (i >= a.D) break;
+        p[i] = sw[j];
+        p[a.D + i] = sb[j];
+    }
+}
+
+// Any length.  dx: a block per row, the row re-read (from L1 / L2).  dx may be dy, so
+// the column sums (ln_bwd_cols_kernel) are launched first.
 template <typename T, bool CK>
-__global__ void __launch_bounds__(256) ln_bwd_any_kernel(const LnBwdArgs a) {
+__global__ void __launch_bounds__(256) ln_bwd_long_kernel(const LnBwdArgs a) {
     __shared__ float red[32];
     const int64_t row = blockIdx.x;
     const float mean = a.mean[row], rstd = a.rstd[row];
@@ -343,7 +548,7 @@ __global__ void __launch_bounds__(256) ln_bwd_any_kernel(const LnBwdArgs a) {
 }
 // Column sums over the rows blockIdx.y, blockIdx.y + gridDim.y, ...
 template <typename T, bool CK>
-__global__ void __launch_bounds__(256) ln_bwd_cols_any_kernel(const LnBwdArgs a) {
+__global__ void __launch_bounds__(256) ln_bwd_cols_kernel(const LnBwdArgs a) {
     const int i = blockIdx.x * 256 + threadIdx.x;
     if (i >= a.D) return;
     float sw = 0.f, sb = 0.f;
@@ -358,55 +563,78 @@ __global__ void __launch_bounds__(256) ln_bwd_cols_any_kernel(const LnBwdArgs a)
 }
 
 // out[c] = sum over the blocks of part[block][c], c < 2D (dweight, dbias): 32
-// columns per block, 8 interleaved slices of the partials, in a fixed order.
-__global__ void __launch_bounds__(256) ln_bwd_params_kernel(const float* __restrict__ part, int blocks, int D,
-                                                            void* dw, void* db, int wdtype) {
-    __shared__ float red[8][33];
+// columns per block, 32 interleaved slices of the partials, in a fixed order.
+// Launched to start beside the row kernel's end (pdl_wait).
+__global__ void __launch_bounds__(1024) ln_bwd_params_kernel(const float* __restrict__ part, int blocks, int D,
+                                                             void* dw, void* db, int wdtype) {
+    __shared__ float red[32][33];
     const int col = threadIdx.x & 31, slice = threadIdx.x >> 5;
     const int64_t c = (int64_t)blockIdx.x * 32 + col, width = 2 * (int64_t)D;
+    pdl_wait();
     float s = 0.f;
-    if (c < width)
-        for (int b = slice; b < blocks; b += 8) s += part[b * width + c];
+    if (c < width) {
+#pragma unroll 4
+        for (int b = slice; b < blocks; b += 32) s += part[b * width + c];
+    }
     red[slice][col] = s;
     __syncthreads();
-    if (slice == 0 && c < width) {
-#pragma unroll
-        for (int k = 1; k < 8; k++) s += red[k][col];
-        if (c < D) store_param(dw, wdtype, c, s);
-        else store_param(db, wdtype, c - D, s);
+    // warp w sums column w over the slices
+    const float t = warp_sum(red[col][slice]);
+    const int64_t o = (int64_t)blockIdx.x * 32 + slice;
+    if (col == 0 && o < width) {
+        if (o < D) store_param(dw, wdtype, o, t);
+        else store_param(db, wdtype, o - D, t);
     }
 }
 
-constexpr int LN_BWD_BLOCKS = 148 * 2;  // at most: two resident blocks per SM
+constexpr int LN_BWD_BLOCKS = 148 * 4;  // at most: four resident blocks per SM
 
-// Blocks of the row kernel and rows it takes at a time, from the vectors of a
-// row (16-byte ones; the 16-bit types have half as many).
-inline int bwd_rows_at_once(int nvec) { return nvec <= 512 ? 4 : nvec <= 1024 ? 2 : 1; }
-inline int bwd_blocks(int rows, int R) { return std::min(ceil_div(rows, R), LN_BWD_BLOCKS); }
+template <typename T, bool CK, int NV, int R>
+cudaError_t launch_ln_bwd_t(const LnBwdArgs& a, int nt, int* blocks, cudaStream_t st) {
+    auto kern = ln_bwd_kernel<T, CK, NV, R>;
+    const int smem = LN_STAGES * R * 3 * NV * nt * 16;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    // as many blocks as are resident by shared memory and threads
+    const int per_sm = std::max(1, std::min({4, 220 * 1024 / (smem + 2048), 1280 / nt}));
+    *blocks = std::min({ceil_div(a.rows, R), 148 * per_sm, LN_BWD_BLOCKS});
+    kern<<<*blocks, nt, smem, st>>>(a);
+    return cudaGetLastError();
+}
 
 template <typename T, bool CK>
 int launch_ln_bwd(LnBwdArgs a, bool vec, void* dw, void* db, cudaStream_t st) {
     const int nvec = a.D / Vec16<T>::N;
     int blocks;
-    if (vec && nvec <= 2048) {
-        const int NV = nvec <= 512 ? 1 : nvec <= 1024 ? 2 : 4;
+    if (vec && nvec <= 512 * 3) {
+        // vectors per thread: the fewest with at most 512 threads
+        const int NV = ceil_div(nvec, 512);
         const int nt = ceil_div(ceil_div(nvec, NV), 32) * 32;
-        blocks = bwd_blocks(a.rows, bwd_rows_at_once(nvec));
-        if (NV == 1) ln_bwd_kernel<T, CK, 1, 4><<<blocks, nt, 0, st>>>(a);
-        else if (NV == 2) ln_bwd_kernel<T, CK, 2, 2><<<blocks, nt, 0, st>>>(a);
-        else ln_bwd_kernel<T, CK, 4, 1><<<blocks, nt, 0, st>>>(a);
+        const cudaError_t e = NV == 1   ? launch_ln_bwd_t<T, CK, 1, 2>(a, nt, &blocks, st)
+                              : NV == 2 ? launch_ln_bwd_t<T, CK, 2, 1>(a, nt, &blocks, st)
+                                        : launch_ln_bwd_t<T, CK, 3, 1>(a, nt, &blocks, st);
+        if (e != cudaSuccess) return fail(RWKV_E_CUDA, "ln_bwd_kernel: %s", cudaGetErrorString(e));
+    } else if (a.D <= 512 * 20) {
+        blocks = std::min(a.rows, LN_BWD_BLOCKS);
+        if (a.D <= 256 * 2) ln_bwd_any_kernel<T, CK, 256, 2><<<blocks, 256, 0, st>>>(a);
+        else if (a.D <= 256 * 4) ln_bwd_any_kernel<T, CK, 256, 4><<<blocks, 256, 0, st>>>(a);
+        else if (a.D <= 256 * 8) ln_bwd_any_kernel<T, CK, 256, 8><<<blocks, 256, 0, st>>>(a);
+        else if (a.D <= 512 * 8) ln_bwd_any_kernel<T, CK, 512, 8><<<blocks, 512, 0, st>>>(a);
+        else ln_bwd_any_kernel<T, CK, 512, 20><<<blocks, 512, 0, st>>>(a);
     } else {
         blocks = std::min(a.rows, 64);
         if (a.part) {
-            ln_bwd_cols_any_kernel<T, CK><<<dim3(ceil_div(a.D, 256), blocks), 256, 0, st>>>(a);
+            ln_bwd_cols_kernel<T, CK><<<dim3(ceil_div(a.D, 256), blocks), 256, 0, st>>>(a);
             if (int rc = check_launch("ln_bwd_cols_kernel")) return rc;
         }
-        ln_bwd_any_kernel<T, CK><<<a.rows, 256, 0, st>>>(a);
+        ln_bwd_long_kernel<T, CK><<<a.rows, 256, 0, st>>>(a);
     }
     if (int rc = check_launch("ln_bwd_kernel")) return rc;
     if (!a.part) return ok();
-    ln_bwd_params_kernel<<<ceil_div(2 * (int64_t)a.D, 32), 256, 0, st>>>(a.part, blocks, a.D, dw, db, a.wdtype);
-    return check_launch("ln_bwd_params_kernel");
+    const cudaError_t e = launch_pdl(ln_bwd_params_kernel, dim3(ceil_div(2 * (int64_t)a.D, 32)), dim3(1024), 0, st,
+                                     (const float*)a.part, blocks, a.D, dw, db, a.wdtype);
+    if (e != cudaSuccess) return fail(RWKV_E_CUDA, "ln_bwd_params_kernel: %s", cudaGetErrorString(e));
+    return ok();
 }
 
 bool al(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
@@ -437,7 +665,7 @@ extern "C" int rwkv_layer_norm_forward(int dtype, const void* x, int wdtype, con
                      al(mean, 4) && al(rstd, 4),
                  RWKV_E_UNSUPPORTED, "%s: a tensor is not aligned to its element type", fn);
     const LnFwdArgs a{x, weight, bias, y, mean, rstd, codes, exps, wdtype, rows, D, ceil_div(D, CK_GROUP), eps};
-    const bool vec = D % 8 == 0 && al(x, 16) && al(y, 16) && al(codes, 8);
+    const bool vec = D % 8 == 0 && al(x, 16) && al(y, 16) && al(codes, 8) && al(weight, 16) && al(bias, 16);
     return dispatch_dtype(dtype, [&]<typename T>() { return launch_ln_fwd<T>(a, vec, (cudaStream_t)stream); });
 }
 
@@ -469,7 +697,8 @@ extern "C" int rwkv_layer_norm_backward(int dtype, const void* dy, const void* x
     }
     const LnBwdArgs a{dy,   x,  codes, exps, weight, mean, rstd, dres, dx, dweight ? static_cast<float*>(workspace) : nullptr,
                       wdtype, rows, D, ceil_div(D, CK_GROUP)};
-    const bool vec = D % 8 == 0 && al(dy, 16) && al(x, 16) && al(codes, 8) && al(dres, 16) && al(dx, 16);
+    const bool vec =
+        D % 8 == 0 && al(dy, 16) && al(x, 16) && al(codes, 8) && al(dres, 16) && al(dx, 16) && al(weight, 16);
     return dispatch_dtype(dtype, [&]<typename T>() {
         return codes ? launch_ln_bwd<T, true>(a, vec, dweight, dbias, (cudaStream_t)stream)
                      : launch_ln_bwd<T, false>(a, vec, dweight, dbias, (cudaStream_t)stream);

@@ -98,7 +98,7 @@ extern "C" int rwkv_projection_forward(int dtype, const void* x, const void* w, 
                  ydtype, bdtype);
     RWKV_REQUIRE(valid_act(act), RWKV_E_UNSUPPORTED, "%s: activation %d", fn, act);
     RWKV_REQUIRE(al(x, 16) && al(w, 16) && al(y, 16) && al(residual, 16) && al(z, 16) && al(codes, 16) &&
-                     al(bias, bdtype == RWKV_F32 ? 4 : 2),
+                     al(bias, 16),
                  RWKV_E_UNSUPPORTED, "%s: a tensor is not 16-byte aligned", fn);
     if (int rc = check_ws(workspace, workspace_bytes, proj_plan(rows, OUT, IN).ws_bytes, fn)) return rc;
     int *err, *err_host, sms;
