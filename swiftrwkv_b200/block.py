@@ -25,6 +25,7 @@ backward calls.
 """
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 
 import torch
@@ -109,10 +110,7 @@ def _aligned(t):
 
 
 def _rows(shape):
-    n = 1
-    for s in shape[:-1]:
-        n *= s
-    return n
+    return math.prod(shape[:-1])
 
 
 def _act(act):
@@ -130,13 +128,13 @@ def _activation(name, x, dev, dtype, shape):
     return _tensor(name, x, dev, (dtype,), shape), None, None
 
 
-def _new_checkpoint(shape, dev, dtype):
-    return Checkpoint8(torch.empty(shape, device=dev, dtype=torch.int8),
-                       torch.empty(shape[:-1] + (-(-shape[-1] // CKPT_GROUP),), device=dev, dtype=torch.uint8), dtype)
+def _new_checkpoint(shape, like):
+    return Checkpoint8(like.new_empty(shape, dtype=torch.int8),
+                       like.new_empty(shape[:-1] + (-(-shape[-1] // CKPT_GROUP),), dtype=torch.uint8), like.dtype)
 
 
-def _workspace(nbytes, dev):
-    return torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
+def _workspace(nbytes, like):
+    return like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
 
 
 # ------------------------------------------------------- 8-bit checkpoints
@@ -144,7 +142,7 @@ def _workspace(nbytes, dev):
 def checkpoint8(x) -> Checkpoint8:
     """The 8-bit checkpoint of x [..., D]."""
     x = _some("x", _tensor("x", x))
-    ck = _new_checkpoint(x.shape, x.device, x.dtype)
+    ck = _new_checkpoint(x.shape, x)
     rows = _rows(x.shape)
     if rows:
         _call(x.device, "rwkv_ckpt8_pack", _DT[x.dtype], x.data_ptr(), ck.codes.data_ptr(), ck.exps.data_ptr(), rows,
@@ -159,7 +157,7 @@ def checkpoint8Values(ck: Checkpoint8, act: str = "none", dtype=None):
     if dtype not in _DT:
         raise ValueError(f"checkpoint8Values: dtype {dtype} not taken")
     _, codes, exps = _activation("ck", ck, ck.codes.device, None, ck.codes.shape)
-    out = torch.empty(codes.shape, device=codes.device, dtype=dtype)
+    out = codes.new_empty(codes.shape, dtype=dtype)
     rows = _rows(codes.shape)
     if rows:
         _call(codes.device, "rwkv_ckpt8_values", codes.data_ptr(), exps.data_ptr(), a, _DT[dtype], out.data_ptr(), rows,
@@ -193,7 +191,7 @@ def layerNormForward(x, weight, bias, eps: float = 1e-5, checkpoint: bool = Fals
     y = torch.empty_like(x)
     mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
     rstd = torch.empty_like(mean)
-    ck = _new_checkpoint(x.shape, dev, x.dtype) if checkpoint else None
+    ck = _new_checkpoint(x.shape, x) if checkpoint else None
     rows = x.numel() // D
     if rows:
         _call(dev, "rwkv_layer_norm_forward", _DT[x.dtype], x.data_ptr(), _DT[weight.dtype], weight.data_ptr(),
@@ -222,7 +220,7 @@ def layerNormBackward(dy, x, weight, mean, rstd, dres=None, params: bool = True)
     if not rows:
         return dx, dw.zero_() if params else None, db.zero_() if params else None
     n = _lib.lib().rwkv_layer_norm_backward_workspace_size(rows, D) if params else 0
-    ws = _workspace(n, dev)
+    ws = _workspace(n, dy)
     _call(dev, "rwkv_layer_norm_backward", _DT[dy.dtype], dy.data_ptr(), _p(xt), _p(codes), _p(exps), _DT[weight.dtype],
           weight.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _p(dres), dx.data_ptr(), _p(dw), _p(db), rows, D, _p(ws),
           n)
@@ -263,13 +261,13 @@ def projectionForward(x, w, bias=None, act: str = "none", residual=None, checkpo
         bias = _aligned(_tensor("bias", bias, dev, None, (OUT,)))
     if residual is not None:
         residual = _aligned(_tensor("residual", residual, dev, (ydt,), shape))
-    y = torch.empty(shape, device=dev, dtype=ydt)
-    ck = _new_checkpoint(torch.Size(shape), dev, x.dtype) if checkpoint else None
-    z = torch.empty(shape, device=dev, dtype=x.dtype) if preactivation else None
+    y = x.new_empty(shape, dtype=ydt)
+    ck = _new_checkpoint(shape, x) if checkpoint else None
+    z = x.new_empty(shape) if preactivation else None
     rows = _rows(shape)
     if rows:
         n = _lib.lib().rwkv_projection_forward_workspace_size(rows, OUT, IN)
-        ws = _workspace(n, dev)
+        ws = _workspace(n, x)
         _call(dev, "rwkv_projection_forward", _DT[x.dtype], x.data_ptr(), w.data_ptr(),
               F32 if bias is None else _DT[bias.dtype], _p(bias), a, _DT[ydt], _p(residual), y.data_ptr(), _p(z),
               ck and ck.codes.data_ptr(), ck and ck.exps.data_ptr(), rows, OUT, IN, _p(ws), n)
@@ -299,11 +297,11 @@ def projectionBackwardInput(dy, w, pre=None, act: str = "none", addend=None, out
         raise ValueError(f"projectionBackwardInput: act {act!r} needs pre")
     if addend is not None:
         addend = _aligned(_tensor("addend", addend, dev, (xdt,), shape))
-    dx = torch.empty(shape, device=dev, dtype=xdt)
+    dx = dy.new_empty(shape, dtype=xdt)
     rows = _rows(shape)
     if rows:
         n = _lib.lib().rwkv_projection_dx_workspace_size(rows, OUT, IN)
-        ws = _workspace(n, dev)
+        ws = _workspace(n, dy)
         _call(dev, "rwkv_projection_dx", _DT[dy.dtype], dy.data_ptr(), w.data_ptr(), a, _p(z), _p(codes), _p(exps),
               _DT[xdt], _p(addend), dx.data_ptr(), rows, OUT, IN, _p(ws), n)
     return dx
@@ -333,13 +331,13 @@ def projectionBackwardWeight(dy, x, act: str = "none", bias: bool = False, out_d
     if x is not None:
         xt, codes, exps = _activation("x", x, dev, dy.dtype, torch.Size(dy.shape[:-1] + (IN,)))
         xt, codes = _aligned(xt), _aligned(codes)
-        dw = torch.empty((OUT, IN), device=dev, dtype=wdt)
-    db = torch.empty(OUT, device=dev, dtype=torch.float32) if bias else None
+        dw = dy.new_empty((OUT, IN), dtype=wdt)
+    db = dy.new_empty(OUT, dtype=torch.float32) if bias else None
     rows = _rows(dy.shape)
     if not rows:
         return dw if dw is None else dw.zero_(), db.zero_() if bias else None
     n = _lib.lib().rwkv_projection_dw_workspace_size(rows, OUT, IN, int(codes is not None or a != 0))
-    ws = _workspace(n, dev)
+    ws = _workspace(n, dy)
     _call(dev, "rwkv_projection_dw", _DT[dy.dtype], dy.data_ptr(), a, _p(xt), _p(codes), _p(exps), _DT[wdt],
           _p(dw), _p(db), rows, OUT, IN, _p(ws), n)
     return dw, db

@@ -144,19 +144,51 @@ inline bool valid_act(int a) { return a >= RWKV_ACT_NONE && a <= RWKV_ACT_SIGMOI
 // --------------------------------------------------- 16-byte vectors of T
 
 template <typename T>
-struct Vec16 {
-    static constexpr int N = 16 / (int)sizeof(T);
+struct Vec16;
+template <>
+struct Vec16<float> {
+    static constexpr int N = 4;
     static __device__ __forceinline__ void unpack(const uint4& r, float* v) {
-        const T* p = reinterpret_cast<const T*>(&r);
-#pragma unroll
-        for (int i = 0; i < N; i++) v[i] = to_f<T>(p[i]);
+        v[0] = __uint_as_float(r.x), v[1] = __uint_as_float(r.y);
+        v[2] = __uint_as_float(r.z), v[3] = __uint_as_float(r.w);
     }
     static __device__ __forceinline__ uint4 pack(const float* v) {
-        uint4 r;
-        T* p = reinterpret_cast<T*>(&r);
+        return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    }
+};
+// Two 16-bit values in a word: one instruction each way for bf16 where element
+// access through the vector's address takes two.
+template <typename T>
+__device__ __forceinline__ float2 word_floats(uint32_t w) {
+    if constexpr (std::is_same_v<T, __nv_bfloat16>)
+        return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    else
+        return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t floats_word(float lo, float hi) {
+    if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    } else {
+        const __half2 v = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+}
+template <typename T>
+struct Vec16 {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ void unpack(const uint4& r, float* v) {
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-        for (int i = 0; i < N; i++) p[i] = from_f<T>(v[i]);
-        return r;
+        for (int i = 0; i < 4; i++) {
+            const float2 f = word_floats<T>(w[i]);
+            v[2 * i] = f.x, v[2 * i + 1] = f.y;
+        }
+    }
+    static __device__ __forceinline__ uint4 pack(const float* v) {
+        return make_uint4(floats_word<T>(v[0], v[1]), floats_word<T>(v[2], v[3]), floats_word<T>(v[4], v[5]),
+                          floats_word<T>(v[6], v[7]));
     }
 };
 

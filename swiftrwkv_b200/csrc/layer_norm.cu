@@ -33,105 +33,140 @@ struct LnFwdArgs {
     float eps;
 };
 
-// Sum over the TPR threads of a row: a warp, or the whole block.
+// Sums over the TPR threads of a row (a warp, or the whole block) of R values.
+template <int TPR, int R>
+__device__ __forceinline__ void row_sums(float* v, float* red) {
+#pragma unroll
+    for (int r = 0; r < R; r++) v[r] = warp_sum(v[r]);
+    if constexpr (TPR > 32) {
+        const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+        __syncthreads();  // the previous sums' readers are done
+#pragma unroll
+        for (int r = 0; r < R; r++)
+            if (lane == 0) red[r * 32 + w] = v[r];
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            if constexpr (TPR == 64) {
+                v[r] = red[r * 32] + red[r * 32 + 1];
+            } else {
+                v[r] = lane < TPR / 32 ? red[r * 32 + lane] : 0.f;
+                v[r] = warp_sum(v[r]);
+            }
+        }
+    }
+}
 template <int TPR>
 __device__ __forceinline__ float row_sum(float v, float* red) {
-    v = warp_sum(v);
-    if constexpr (TPR > 32) {
-        const int w = threadIdx.x >> 5;
-        __syncthreads();  // the previous sum's readers are done
-        if ((threadIdx.x & 31) == 0) red[w] = v;
-        __syncthreads();
-        v = (threadIdx.x & 31) < TPR / 32 ? red[threadIdx.x & 31] : 0.f;
-        v = warp_sum(v);
-    }
+    row_sums<TPR, 1>(&v, red);
     return v;
 }
 
-// TPR threads per row (32: a warp, several rows per block; else one block per
-// row), at most NV vectors per thread: vector j of thread t is t + j TPR.  Rows
-// of at most 80 elements per thread are held in fp32, longer ones as read.
-template <typename T, int TPR, int NV>
-__global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) ln_fwd_kernel(const LnFwdArgs a) {
+// A block of TPR threads takes R rows, at most NV vectors of a row per thread:
+// vector j of thread t is t + j TPR.  The R rows share the loads of weight and bias, which in fp32 are twice a bf16 row's own
+// bytes from L1.  Rows of at most 80 elements per thread are held in fp32,
+// longer ones as read.  WF32: weight and bias in fp32 (no branch between their
+// loads); CK: write the checkpoint.
+template <typename T, int TPR, int NV, int R, bool WF32, bool CK>
+__global__ void __launch_bounds__(TPR) ln_fwd_kernel(const LnFwdArgs a) {
     constexpr int VE = Vec16<T>::N;
-    constexpr bool F32 = NV * VE <= 80;
-    __shared__ float red[32];
-    const int t = threadIdx.x & (TPR - 1);
-    const int64_t row = TPR == 32 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
-    if (row >= a.rows) return;  // whole rows of threads leave
+    constexpr bool F32 = R * NV * VE <= 80;
+    __shared__ float red[32 * R];
+    const int t = threadIdx.x;
+    const int64_t row0 = (int64_t)blockIdx.x * R;
     const int nvec = a.D / VE;
-    const uint4* xr = reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + row * a.D);
-    uint4 raw[NV];
+    const uint4* xr = static_cast<const uint4*>(a.x) + row0 * nvec + t;
+    uint4 raw[R][NV];
 #pragma unroll
-    for (int j = 0; j < NV; j++) {
-        const int v = t + j * TPR;
-        raw[j] = v < nvec ? __ldcs(xr + v) : make_uint4(0, 0, 0, 0);
-    }
-    if (a.codes) {
+    for (int r = 0; r < R; r++)
+#pragma unroll
+        for (int j = 0; j < NV; j++)
+            raw[r][j] = row0 + r < a.rows && t + j * TPR < nvec ? __ldcs(xr + (int64_t)r * nvec + j * TPR)
+                                                               : make_uint4(0, 0, 0, 0);
+    if constexpr (CK) {
         // a group of 32 channels is 32 / VE neighbouring threads
 #pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int j = 0; j < NV; j++) {
+                const int v = t + j * TPR;
+                uint32_t top = top_bits<T>(raw[r][j]);
+#pragma unroll
+                for (int o = 1; o < CK_GROUP / VE; o *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+                const uint32_t e = ck_exponent(top_f32<T>(top));
+                const float inv = ck_inv_scale(e);
+                if (row0 + r < a.rows && v < nvec) {
+                    float f[VE];
+                    Vec16<T>::unpack(raw[r][j], f);
+                    int8_t* c = a.codes + (row0 + r) * a.D + (int64_t)v * VE;
+                    if constexpr (VE == 8)
+                        *reinterpret_cast<uint2*>(c) = make_uint2(ck_pack4(f[0], f[1], f[2], f[3], inv),
+                                                                  ck_pack4(f[4], f[5], f[6], f[7], inv));
+                    else
+                        *reinterpret_cast<uint32_t*>(c) = ck_pack4(f[0], f[1], f[2], f[3], inv);
+                    if (v % (CK_GROUP / VE) == 0) a.exps[(row0 + r) * a.G + v / (CK_GROUP / VE)] = (uint8_t)e;
+                }
+            }
+    }
+    float x[F32 ? R : 1][F32 ? NV : 1][VE];
+    auto vec = [&](int r, int j) -> float* { return x[F32 ? r : 0][F32 ? j : 0]; };
+    float mean[R], rstd[R], shift[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        mean[r] = 0.f;
+#pragma unroll
         for (int j = 0; j < NV; j++) {
-            const int v = t + j * TPR;
-            uint32_t top = top_bits<T>(raw[j]);
+            float* f = vec(r, j);
+            Vec16<T>::unpack(raw[r][j], f);
 #pragma unroll
-            for (int o = 1; o < CK_GROUP / VE; o *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const uint32_t e = ck_exponent(top_f32<T>(top));
-            const float inv = ck_inv_scale(e);
-            if (v < nvec) {
-                float f[VE];
-                Vec16<T>::unpack(raw[j], f);
-                int8_t* c = a.codes + row * a.D + (int64_t)v * VE;
-                if constexpr (VE == 8)
-                    *reinterpret_cast<uint2*>(c) = make_uint2(ck_pack4(f[0], f[1], f[2], f[3], inv),
-                                                              ck_pack4(f[4], f[5], f[6], f[7], inv));
-                else
-                    *reinterpret_cast<uint32_t*>(c) = ck_pack4(f[0], f[1], f[2], f[3], inv);
-                if (v % (CK_GROUP / VE) == 0) a.exps[row * a.G + v / (CK_GROUP / VE)] = (uint8_t)e;
+            for (int k = 0; k < VE; k++) mean[r] += f[k];
+        }
+    }
+    row_sums<TPR, R>(mean, red);
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        mean[r] /= (float)a.D;
+        rstd[r] = 0.f;
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            float* f = vec(r, j);
+            if constexpr (!F32) Vec16<T>::unpack(raw[r][j], f);
+            if (t + j * TPR < nvec) {
+#pragma unroll
+                for (int k = 0; k < VE; k++) {
+                    const float d = f[k] - mean[r];
+                    rstd[r] = fmaf(d, d, rstd[r]);
+                }
             }
         }
     }
-    float x[F32 ? NV : 1][VE];
-    float s = 0.f;
+    row_sums<TPR, R>(rstd, red);
 #pragma unroll
-    for (int j = 0; j < NV; j++) {
-        float* f = x[F32 ? j : 0];
-        Vec16<T>::unpack(raw[j], f);
-#pragma unroll
-        for (int k = 0; k < VE; k++) s += f[k];
-    }
-    const float mean = row_sum<TPR>(s, red) / (float)a.D;
-    float q = 0.f;
-#pragma unroll
-    for (int j = 0; j < NV; j++) {
-        float* f = x[F32 ? j : 0];
-        if constexpr (!F32) Vec16<T>::unpack(raw[j], f);
-        if (t + j * TPR < nvec) {
-#pragma unroll
-            for (int k = 0; k < VE; k++) {
-                const float d = f[k] - mean;
-                q = fmaf(d, d, q);
-            }
+    for (int r = 0; r < R; r++) {
+        rstd[r] = 1.f / sqrtf(rstd[r] / (float)a.D + a.eps);
+        shift[r] = -mean[r] * rstd[r];
+        if (t == 0 && a.mean && row0 + r < a.rows) {
+            a.mean[row0 + r] = mean[r];
+            a.rstd[row0 + r] = rstd[r];
         }
     }
-    const float rstd = 1.f / sqrtf(row_sum<TPR>(q, red) / (float)a.D + a.eps);
-    const float shift = -mean * rstd;
-    if (t == 0 && a.mean) {
-        a.mean[row] = mean;
-        a.rstd[row] = rstd;
-    }
-    uint4* yr = reinterpret_cast<uint4*>(static_cast<T*>(a.y) + row * a.D);
+    uint4* yr = static_cast<uint4*>(a.y) + row0 * nvec + t;
 #pragma unroll
     for (int j = 0; j < NV; j++) {
         const int v = t + j * TPR;
         if (v < nvec) {
-            float* f = x[F32 ? j : 0];
-            if constexpr (!F32) Vec16<T>::unpack(raw[j], f);
             float w[VE], b[VE];
-            load_params<VE>(a.w, a.wdtype, v * VE, w);
-            load_params<VE>(a.b, a.wdtype, v * VE, b);
+            load_params<VE>(a.w, WF32 ? RWKV_F32 : a.wdtype, v * VE, w);
+            load_params<VE>(a.b, WF32 ? RWKV_F32 : a.wdtype, v * VE, b);
 #pragma unroll
-            for (int k = 0; k < VE; k++) f[k] = fmaf(fmaf(f[k], rstd, shift), w[k], b[k]);
-            __stcs(yr + v, Vec16<T>::pack(f));
+            for (int r = 0; r < R; r++) {
+                float* f = vec(r, j);
+                if constexpr (!F32) Vec16<T>::unpack(raw[r][j], f);
+                float o[VE];
+#pragma unroll
+                for (int k = 0; k < VE; k++) o[k] = fmaf(fmaf(f[k], rstd[r], shift[r]), w[k], b[k]);
+                if (row0 + r < a.rows) __stcs(yr + (int64_t)r * nvec + j * TPR, Vec16<T>::pack(o));
+            }
         }
     }
 }
@@ -217,21 +252,36 @@ __global__ void __launch_bounds__(256) ln_fwd_long_kernel(const LnFwdArgs a) {
     }
 }
 
+template <typename T, int TPR, int NV, int R>
+void launch_ln_fwd_t(const LnFwdArgs& a, cudaStream_t st) {
+    const int grid = ceil_div(a.rows, R);
+    if (a.wdtype == RWKV_F32) {
+        if (a.codes) ln_fwd_kernel<T, TPR, NV, R, true, true><<<grid, TPR, 0, st>>>(a);
+        else ln_fwd_kernel<T, TPR, NV, R, true, false><<<grid, TPR, 0, st>>>(a);
+    } else {
+        if (a.codes) ln_fwd_kernel<T, TPR, NV, R, false, true><<<grid, TPR, 0, st>>>(a);
+        else ln_fwd_kernel<T, TPR, NV, R, false, false><<<grid, TPR, 0, st>>>(a);
+    }
+}
+
 template <typename T>
 int launch_ln_fwd(const LnFwdArgs& a, bool vec, cudaStream_t st) {
     const int nvec = a.D / Vec16<T>::N;
-    if (vec && nvec <= 32 * 16) {
-        const int grid = ceil_div(a.rows, 4), nv = ceil_div(nvec, 32);
-        if (nv <= 2) ln_fwd_kernel<T, 32, 2><<<grid, 128, 0, st>>>(a);
-        else if (nv <= 4) ln_fwd_kernel<T, 32, 4><<<grid, 128, 0, st>>>(a);
-        else if (nv <= 6) ln_fwd_kernel<T, 32, 6><<<grid, 128, 0, st>>>(a);
-        else if (nv <= 8) ln_fwd_kernel<T, 32, 8><<<grid, 128, 0, st>>>(a);
-        else if (nv <= 10) ln_fwd_kernel<T, 32, 10><<<grid, 128, 0, st>>>(a);
-        else ln_fwd_kernel<T, 32, 16><<<grid, 128, 0, st>>>(a);
-    } else if (vec && nvec <= 256 * 4) {
-        ln_fwd_kernel<T, 256, 4><<<a.rows, 256, 0, st>>>(a);
-    } else if (vec && nvec <= 512 * 8) {
-        ln_fwd_kernel<T, 512, 8><<<a.rows, 512, 0, st>>>(a);
+    // Threads and vectors per thread by length, two rows at a time (16384 x
+    // 2560 bf16: 36 us against 40 us one by one, 16384 x 1024: 16 against 19);
+    // with a checkpoint, above 256 vectors, one row (45 against 50 us), since the
+    // packing hides the parameters' loads and two rows leave fewer threads.  A
+    // row's sums run the same way with and without a checkpoint.
+    const bool one = a.codes != nullptr;
+    if (vec && nvec <= 512 * 8) {
+        if (nvec <= 64) launch_ln_fwd_t<T, 64, 1, 2>(a, st);
+        else if (nvec <= 64 * 2) launch_ln_fwd_t<T, 64, 2, 2>(a, st);
+        else if (nvec <= 64 * 3) launch_ln_fwd_t<T, 64, 3, 2>(a, st);
+        else if (nvec <= 128 * 2) launch_ln_fwd_t<T, 128, 2, 2>(a, st);
+        else if (nvec <= 64 * 5) one ? launch_ln_fwd_t<T, 64, 5, 1>(a, st) : launch_ln_fwd_t<T, 64, 5, 2>(a, st);
+        else if (nvec <= 256 * 2) one ? launch_ln_fwd_t<T, 256, 2, 1>(a, st) : launch_ln_fwd_t<T, 256, 2, 2>(a, st);
+        else if (nvec <= 256 * 5) one ? launch_ln_fwd_t<T, 256, 5, 1>(a, st) : launch_ln_fwd_t<T, 256, 5, 2>(a, st);
+        else launch_ln_fwd_t<T, 512, 8, 1>(a, st);
     } else if (a.D <= 32 * 32) {
         const int grid = ceil_div(a.rows, 4);
         if (a.D <= 32 * 8) ln_fwd_any_kernel<T, 32, 8><<<grid, 128, 0, st>>>(a);
@@ -302,7 +352,7 @@ constexpr int LN_STAGES = 3;
 // HBM stays busy while the block computes and waits at its barrier: one per R
 // rows, for the two row sums (buffers alternating).
 template <typename T, bool CK, int NV, int R>
-__global__ void __launch_bounds__(512) ln_bwd_kernel(const LnBwdArgs a) {
+__global__ void __launch_bounds__(512, 1) ln_bwd_kernel(const LnBwdArgs a) {
     constexpr int VE = Vec16<T>::N;
     extern __shared__ uint4 ring[];  // [stage][row][dy | x | dres][NV][thread]
     __shared__ float red[2][16][2 * R];
@@ -318,7 +368,9 @@ __global__ void __launch_bounds__(512) ln_bwd_kernel(const LnBwdArgs a) {
         if (v < nvec) load_params<VE>(a.w, a.wdtype, (int64_t)v * VE, w[j]);
     }
     const int64_t step = (int64_t)gridDim.x * R;
-    auto slot = [&](int stage, int r, int part, int j) { return ring + (((stage * R + r) * 3 + part) * NV + j) * nt + t; };
+    auto slot = [&](int stage, int r, int part, int j) {
+        return ring + t + (uint32_t)nt * (uint32_t)(((stage * R + r) * 3 + part) * NV + j);
+    };
     auto fetch = [&](int64_t r0, int stage) {
 #pragma unroll
         for (int r = 0; r < R; r++)
@@ -590,8 +642,9 @@ __global__ void __launch_bounds__(1024) ln_bwd_params_kernel(const float* __rest
 constexpr int LN_BWD_BLOCKS = 148 * 4;  // at most: four resident blocks per SM
 
 template <typename T, bool CK, int NV, int R>
-cudaError_t launch_ln_bwd_t(const LnBwdArgs& a, int nt, int* blocks, cudaStream_t st) {
+cudaError_t launch_ln_bwd_t(const LnBwdArgs& a, int* blocks, cudaStream_t st) {
     auto kern = ln_bwd_kernel<T, CK, NV, R>;
+    const int nt = ceil_div(ceil_div(a.D / Vec16<T>::N, NV), 32) * 32;
     const int smem = LN_STAGES * R * 3 * NV * nt * 16;
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
@@ -607,12 +660,12 @@ int launch_ln_bwd(LnBwdArgs a, bool vec, void* dw, void* db, cudaStream_t st) {
     const int nvec = a.D / Vec16<T>::N;
     int blocks;
     if (vec && nvec <= 512 * 3) {
-        // vectors per thread: the fewest with at most 512 threads
-        const int NV = ceil_div(nvec, 512);
-        const int nt = ceil_div(ceil_div(nvec, NV), 32) * 32;
-        const cudaError_t e = NV == 1   ? launch_ln_bwd_t<T, CK, 1, 2>(a, nt, &blocks, st)
-                              : NV == 2 ? launch_ln_bwd_t<T, CK, 2, 1>(a, nt, &blocks, st)
-                                        : launch_ln_bwd_t<T, CK, 3, 1>(a, nt, &blocks, st);
+        // vectors per thread: the fewest with at most 512 threads.  Two rows
+        // at a time from a dense x (16384 x 2048 bf16: 51 us, one row 65 us), one
+        // from a checkpoint, whose decoding takes more registers (65 against 68 us)
+        const cudaError_t e = nvec > 1024  ? launch_ln_bwd_t<T, CK, 3, 1>(a, &blocks, st)
+                              : nvec > 512 ? launch_ln_bwd_t<T, CK, 2, 1>(a, &blocks, st)
+                                           : launch_ln_bwd_t<T, CK, 1, CK ? 1 : 2>(a, &blocks, st);
         if (e != cudaSuccess) return fail(RWKV_E_CUDA, "ln_bwd_kernel: %s", cudaGetErrorString(e));
     } else if (a.D <= 512 * 20) {
         blocks = std::min(a.rows, LN_BWD_BLOCKS);
