@@ -1,6 +1,7 @@
 // Trainable projections: y = act(x W^T + bias) + residual, dX and dW, over the
-// tcgen05 kernel of gemm_proj.cuh.
-#include "gemm_proj.cuh"
+// tcgen05 kernel of gemm_proj.cuh, and the weight-streaming kernel of
+// gemv_proj.cuh for a forward of a few rows.
+#include "gemv_proj.cuh"
 
 namespace rwkv {
 
@@ -83,7 +84,7 @@ bool sizes_ok(int rows, int OUT, int IN) {
 using namespace rwkv;
 
 extern "C" int64_t rwkv_projection_forward_workspace_size(int rows, int OUT, int IN) {
-    return sizes_ok(rows, OUT, IN) ? proj_plan(rows, OUT, IN).ws_bytes : 0;
+    return sizes_ok(rows, OUT, IN) && rows > GP_ROWS ? proj_plan(rows, OUT, IN).ws_bytes : 0;
 }
 
 extern "C" int rwkv_projection_forward(int dtype, const void* x, const void* w, int bdtype, const void* bias, int act,
@@ -100,7 +101,9 @@ extern "C" int rwkv_projection_forward(int dtype, const void* x, const void* w, 
     RWKV_REQUIRE(al(x, 16) && al(w, 16) && al(y, 16) && al(residual, 16) && al(z, 16) && al(codes, 16) &&
                      al(bias, 16),
                  RWKV_E_UNSUPPORTED, "%s: a tensor is not 16-byte aligned", fn);
-    if (int rc = check_ws(workspace, workspace_bytes, proj_plan(rows, OUT, IN).ws_bytes, fn)) return rc;
+    const bool few = rows <= GP_ROWS;  // stream the weights (gemv_proj.cuh)
+    if (!few)
+        if (int rc = check_ws(workspace, workspace_bytes, proj_plan(rows, OUT, IN).ws_bytes, fn)) return rc;
     int *err, *err_host, sms;
     if (int rc = gemm_wait_record((cudaStream_t)stream, fn, &err, &err_host, &sms)) return rc;
     ProjEpi e{};
@@ -113,8 +116,10 @@ extern "C" int rwkv_projection_forward(int dtype, const void* x, const void* w, 
     e.codes = codes;
     e.exps = exps;
     e.z = z;
-    const cudaError_t rc = proj_gemm<false, false>(x, w, y, rows, OUT, IN, e, static_cast<float*>(workspace), err,
-                                                   err_host, sms, (cudaStream_t)stream);
+    const cudaError_t rc =
+        few ? launch_gemv_proj(GemvProjArgs{x, w, y, e, rows, OUT, IN}, sms, (cudaStream_t)stream)
+            : proj_gemm<false, false>(x, w, y, rows, OUT, IN, e, static_cast<float*>(workspace), err, err_host, sms,
+                                      (cudaStream_t)stream);
     if (rc != cudaSuccess) return fail(RWKV_E_CUDA, "%s: %s", fn, cudaGetErrorString(rc));
     return ok();
 }
