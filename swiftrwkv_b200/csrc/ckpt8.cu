@@ -54,7 +54,7 @@ constexpr int CU = 4;
 // FLAT: D % 32 == 0, rows run on.  Otherwise units are counted in rows padded
 // to whole groups (4 units), so that a group's units are neighbours in a warp.
 template <typename T, bool FLAT>
-__global__ void __launch_bounds__(CT) ckpt8_pack_kernel(const T* __restrict__ x, int8_t* __restrict__ codes,
+__global__ void __launch_bounds__(CT, 1) ckpt8_pack_kernel(const T* __restrict__ x, int8_t* __restrict__ codes,
                                                         uint8_t* __restrict__ exps, int64_t units, int D, int G) {
     const int64_t i0 = blockIdx.x * (int64_t)(CT * CU) + threadIdx.x;
     Raw8<T> raw[CU];
@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(CT) ckpt8_pack_kernel(const T* __restrict__ x,
 
 // Any D and alignment: a warp per group, 8 groups at a time.
 template <typename T>
-__global__ void __launch_bounds__(CT) ckpt8_pack_any_kernel(const T* __restrict__ x, int8_t* __restrict__ codes,
+__global__ void __launch_bounds__(CT, 1) ckpt8_pack_any_kernel(const T* __restrict__ x, int8_t* __restrict__ codes,
                                                             uint8_t* __restrict__ exps, int64_t groups, int D, int G) {
     const int lane = threadIdx.x & 31;
     const int64_t g0 = ((blockIdx.x * (int64_t)CT + threadIdx.x) >> 5) * 8;
@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(CT) ckpt8_pack_any_kernel(const T* __restrict_
 // dy * act'(z), z dense.  MODE 3: out = act(z).  Elementary functions in fp32
 // precision where the result is fp32.
 template <int MODE, int ACT, typename T, bool FLAT>
-__global__ void __launch_bounds__(CT) ckpt8_use_kernel(const T* dy, const T* __restrict__ z,
+__global__ void __launch_bounds__(CT, 1) ckpt8_use_kernel(const T* dy, const T* __restrict__ z,
                                                        const int8_t* __restrict__ codes,
                                                        const uint8_t* __restrict__ exps, T* out, int64_t n, int D,
                                                        int G) {
@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(CT) ckpt8_use_kernel(const T* dy, const T* __r
 
 // Misaligned tensors: single elements.
 template <int MODE, int ACT, typename T>
-__global__ void __launch_bounds__(CT) ckpt8_use_any_kernel(const T* dy, const T* __restrict__ z,
+__global__ void __launch_bounds__(CT, 1) ckpt8_use_any_kernel(const T* dy, const T* __restrict__ z,
                                                            const int8_t* __restrict__ codes,
                                                            const uint8_t* __restrict__ exps, T* out, int64_t n, int D,
                                                            int G) {

@@ -9,10 +9,11 @@
 // consecutive k of weight rows g and g + 8 and of activation row g, and the two
 // MMAs of the piece take words (0, 1) and (2, 3) of all three: the same permutation
 // of k on both sides, so that every load is 16 bytes and no shuffle is needed.
-// GP_U pieces are in flight per warp (8 in place of 4 changed nothing).  Measured,
-// weights from HBM, in a graph: 1 row, 8192 outputs of 2048 8.9 us (3.8 TB/s), 2048
-// of 8192 13.8 us, 65536 of 2048 49 us (5.4 TB/s); the tile kernel takes 19 us for
-// the first.  The warps' sums meet in shared memory and
+// GP_U pieces are in flight per warp; the launch bound of one block per SM is what
+// makes the compiler keep them in registers (without it 2048 outputs of 8192 take
+// 13.8 us).  Measured, weights from HBM, in a graph, 1 row: 8192 outputs of 2048
+// 7.8 us (4.3 TB/s), 2048 of 8192 8.8 us, 65536 of 2048 41 us (6.5 TB/s); the tile
+// kernel takes 19 us for the first.  The warps' sums meet in shared memory and
 // are added in warp order (deterministic).
 #pragma once
 
@@ -46,7 +47,7 @@ __device__ __forceinline__ void mma_16816(float* c, uint32_t a0, uint32_t a1, ui
 
 // NT: groups of 8 activation rows; NW warps; MT groups of 16 outputs.
 template <bool BF16, int NT, int NW, int MT>
-__global__ void __launch_bounds__(NW * 32) gemv_proj_kernel(const GemvProjArgs a) {
+__global__ void __launch_bounds__(NW * 32, 1) gemv_proj_kernel(const GemvProjArgs a) {
     constexpr int O = 16 * MT, U = GP_U;
     __shared__ float red[NW][8 * NT][O + 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;

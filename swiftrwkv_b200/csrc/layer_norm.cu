@@ -68,7 +68,7 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
 // longer ones as read.  WF32: weight and bias in fp32 (no branch between their
 // loads); CK: write the checkpoint.
 template <typename T, int TPR, int NV, int R, bool WF32, bool CK>
-__global__ void __launch_bounds__(TPR) ln_fwd_kernel(const LnFwdArgs a) {
+__global__ void __launch_bounds__(TPR, 1) ln_fwd_kernel(const LnFwdArgs a) {
     constexpr int VE = Vec16<T>::N;
     constexpr bool F32 = R * NV * VE <= 80;
     __shared__ float red[32 * R];
@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(TPR) ln_fwd_kernel(const LnFwdArgs a) {
 // Any alignment: single elements, element j of thread t is t + j TPR (a warp's
 // 32 elements are a checkpoint group), at most NE per thread, in registers.
 template <typename T, int TPR, int NE>
-__global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) ln_fwd_any_kernel(const LnFwdArgs a) {
+__global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, 1) ln_fwd_any_kernel(const LnFwdArgs a) {
     __shared__ float red[32];
     const int t = threadIdx.x & (TPR - 1);
     const int64_t row = TPR == 32 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
@@ -282,14 +282,15 @@ int launch_ln_fwd(const LnFwdArgs& a, bool vec, cudaStream_t st) {
         else if (nvec <= 256 * 2) one ? launch_ln_fwd_t<T, 256, 2, 1>(a, st) : launch_ln_fwd_t<T, 256, 2, 2>(a, st);
         else if (nvec <= 256 * 5) one ? launch_ln_fwd_t<T, 256, 5, 1>(a, st) : launch_ln_fwd_t<T, 256, 5, 2>(a, st);
         else launch_ln_fwd_t<T, 512, 8, 1>(a, st);
-    } else if (a.D <= 32 * 32) {
-        const int grid = ceil_div(a.rows, 4);
-        if (a.D <= 32 * 8) ln_fwd_any_kernel<T, 32, 8><<<grid, 128, 0, st>>>(a);
-        else ln_fwd_any_kernel<T, 32, 32><<<grid, 128, 0, st>>>(a);
-    } else if (a.D <= 256 * 40) {
-        if (a.D <= 256 * 8) ln_fwd_any_kernel<T, 256, 8><<<a.rows, 256, 0, st>>>(a);
-        else if (a.D <= 256 * 16) ln_fwd_any_kernel<T, 256, 16><<<a.rows, 256, 0, st>>>(a);
-        else ln_fwd_any_kernel<T, 256, 40><<<a.rows, 256, 0, st>>>(a);
+    } else if (a.D <= 32 * 8) {
+        ln_fwd_any_kernel<T, 32, 8><<<ceil_div(a.rows, 4), 128, 0, st>>>(a);
+    } else if (a.D <= 512 * 20) {
+        if (a.D <= 128 * 4) ln_fwd_any_kernel<T, 128, 4><<<a.rows, 128, 0, st>>>(a);
+        else if (a.D <= 128 * 8) ln_fwd_any_kernel<T, 128, 8><<<a.rows, 128, 0, st>>>(a);
+        else if (a.D <= 256 * 8) ln_fwd_any_kernel<T, 256, 8><<<a.rows, 256, 0, st>>>(a);
+        else if (a.D <= 512 * 6) ln_fwd_any_kernel<T, 512, 6><<<a.rows, 512, 0, st>>>(a);
+        else if (a.D <= 512 * 12) ln_fwd_any_kernel<T, 512, 12><<<a.rows, 512, 0, st>>>(a);
+        else ln_fwd_any_kernel<T, 512, 20><<<a.rows, 512, 0, st>>>(a);
     } else {
         ln_fwd_long_kernel<T><<<a.rows, 256, 0, st>>>(a);
     }
@@ -529,17 +530,33 @@ __global__ void __launch_bounds__(NT) ln_bwd_any_kernel(const LnBwdArgs a) {
         w[j] = t + j * NT < a.D ? load_param(a.w, a.wdtype, t + j * NT) : 0.f;
         sw[j] = sb[j] = 0.f;
     }
-    int buf = 0;
-    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, buf ^= 1) {
+    // the next row is read while this one is computed
+    float ndy[NE], nx[NE], nmean = 0.f, nrstd = 0.f;
+    auto fetch = [&](int64_t row) {
+        if (row >= a.rows) return;
         const T* dyr = static_cast<const T*>(a.dy) + row * a.D;
-        const float mean = a.mean[row], rstd = a.rstd[row];
-        float dy[NE], h[NE];
+        nmean = a.mean[row];
+        nrstd = a.rstd[row];
 #pragma unroll
         for (int j = 0; j < NE; j++) {
             const int i = t + j * NT;
-            dy[j] = i < a.D ? to_f<T>(dyr[i]) : 0.f;
-            h[j] = i < a.D ? bwd_x<T, CK>(a, row, i) : 0.f;
+            ndy[j] = i < a.D ? to_f<T>(dyr[i]) : 0.f;
+            nx[j] = i < a.D ? bwd_x<T, CK>(a, row, i) : 0.f;
         }
+    };
+    fetch(blockIdx.x);
+    int buf = 0;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, buf ^= 1) {
+        const float mean = nmean, rstd = nrstd;
+        float dy[NE], h[NE], res[NE];
+#pragma unroll
+        for (int j = 0; j < NE; j++) {
+            const int i = t + j * NT;
+            dy[j] = ndy[j];
+            h[j] = nx[j];
+            res[j] = a.dres && i < a.D ? to_f<T>(static_cast<const T*>(a.dres)[row * a.D + i]) : 0.f;
+        }
+        fetch(row + gridDim.x);
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int j = 0; j < NE; j++) {
@@ -560,9 +577,8 @@ __global__ void __launch_bounds__(NT) ln_bwd_any_kernel(const LnBwdArgs a) {
         for (int j = 0; j < NE; j++) {
             const int i = t + j * NT;
             if (i >= a.D) break;
-            float d = rstd * (dy[j] * w[j] - m1 - h[j] * m2);
-            if (a.dres) d += to_f<T>(static_cast<const T*>(a.dres)[row * a.D + i]);
-            static_cast<T*>(a.dx)[row * a.D + i] = from_f<T>(d);
+            const float d = rstd * (dy[j] * w[j] - m1 - h[j] * m2);
+            static_cast<T*>(a.dx)[row * a.D + i] = from_f<T>(res[j] + d);
         }
     }
     if (!a.part) return;
@@ -669,10 +685,14 @@ int launch_ln_bwd(LnBwdArgs a, bool vec, void* dw, void* db, cudaStream_t st) {
         if (e != cudaSuccess) return fail(RWKV_E_CUDA, "ln_bwd_kernel: %s", cudaGetErrorString(e));
     } else if (a.D <= 512 * 20) {
         blocks = std::min(a.rows, LN_BWD_BLOCKS);
-        if (a.D <= 256 * 2) ln_bwd_any_kernel<T, CK, 256, 2><<<blocks, 256, 0, st>>>(a);
+        if (a.D <= 256) ln_bwd_any_kernel<T, CK, 256, 1><<<blocks, 256, 0, st>>>(a);
+        else if (a.D <= 256 * 2) ln_bwd_any_kernel<T, CK, 256, 2><<<blocks, 256, 0, st>>>(a);
         else if (a.D <= 256 * 4) ln_bwd_any_kernel<T, CK, 256, 4><<<blocks, 256, 0, st>>>(a);
-        else if (a.D <= 256 * 8) ln_bwd_any_kernel<T, CK, 256, 8><<<blocks, 256, 0, st>>>(a);
+        else if (a.D <= 512 * 3) ln_bwd_any_kernel<T, CK, 512, 3><<<blocks, 512, 0, st>>>(a);
+        else if (a.D <= 512 * 4) ln_bwd_any_kernel<T, CK, 512, 4><<<blocks, 512, 0, st>>>(a);
+        else if (a.D <= 512 * 6) ln_bwd_any_kernel<T, CK, 512, 6><<<blocks, 512, 0, st>>>(a);
         else if (a.D <= 512 * 8) ln_bwd_any_kernel<T, CK, 512, 8><<<blocks, 512, 0, st>>>(a);
+        else if (a.D <= 512 * 12) ln_bwd_any_kernel<T, CK, 512, 12><<<blocks, 512, 0, st>>>(a);
         else ln_bwd_any_kernel<T, CK, 512, 20><<<blocks, 512, 0, st>>>(a);
     } else {
         blocks = std::min(a.rows, 64);
