@@ -118,14 +118,14 @@ __global__ void __launch_bounds__(CT, 1) ckpt8_pack_any_kernel(const T* __restri
 }
 
 // MODE 0: out = act(value).  MODE 1: out = dy * act'(value), MODE 2: out =
-// dy * act'(z), z dense.  MODE 3: out = act(z).  Elementary functions in fp32
-// precision where the result is fp32.
+// dy * act'(z), z dense.  Elementary functions in fp32 precision where the result
+// is fp32.
 template <int MODE, int ACT, typename T, bool FLAT>
 __global__ void __launch_bounds__(CT, 1) ckpt8_use_kernel(const T* dy, const T* __restrict__ z,
                                                        const int8_t* __restrict__ codes,
                                                        const uint8_t* __restrict__ exps, T* out, int64_t n, int D,
                                                        int G) {
-    constexpr bool FAST = sizeof(T) == 2, HAS_DY = MODE == 1 || MODE == 2;
+    constexpr bool FAST = sizeof(T) == 2, HAS_DY = MODE != 0;
     const int64_t i0 = blockIdx.x * (int64_t)(CT * CU) + threadIdx.x, units = n / 8;
     Raw8<T> rz[CU], rd[CU];
     uint2 w[CU];
@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(CT, 1) ckpt8_use_kernel(const T* dy, const T* 
     for (int j = 0; j < CU; j++) {
         const int64_t i = i0 + j * CT;
         if (i >= units) continue;
-        if constexpr (MODE >= 2) rz[j].load(z + 8 * i);
+        if constexpr (MODE == 2) rz[j].load(z + 8 * i);
         else w[j] = __ldcs(reinterpret_cast<const uint2*>(codes + 8 * i));
         if constexpr (MODE < 2 && FLAT) e[j] = exps[i >> 2];
         if constexpr (HAS_DY) rd[j].load(dy + 8 * i);
@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(CT, 1) ckpt8_use_kernel(const T* dy, const T* 
         const int64_t i = i0 + j * CT;
         if (i >= units) continue;
         float v[8], d[8];
-        if constexpr (MODE >= 2) {
+        if constexpr (MODE == 2) {
             rz[j].floats(v);
         } else {
             if constexpr (FLAT) {
@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(CT, 1) ckpt8_use_kernel(const T* dy, const T* 
     const int64_t t = 8 * units + threadIdx.x;
     if (blockIdx.x == 0 && t < n) {
         float f;
-        if constexpr (MODE >= 2) f = to_f<T>(z[t]);
+        if constexpr (MODE == 2) f = to_f<T>(z[t]);
         else f = (float)codes[t] * ck_scale(exps[t / D * G + (int)(t % D) / CK_GROUP]);
         if constexpr (HAS_DY) out[t] = from_f<T>(to_f<T>(dy[t]) * act_grad_t<ACT, FAST>(f));
         else out[t] = from_f<T>(act_t<ACT, FAST>(f));
@@ -190,9 +190,9 @@ __global__ void __launch_bounds__(CT, 1) ckpt8_use_any_kernel(const T* dy, const
     for (int64_t i = blockIdx.x * (int64_t)CT + threadIdx.x; i < n; i += (int64_t)gridDim.x * CT) {
         const int64_t row = i / D;
         float v;
-        if constexpr (MODE >= 2) v = to_f<T>(z[i]);
+        if constexpr (MODE == 2) v = to_f<T>(z[i]);
         else v = (float)codes[i] * ck_scale(exps[row * G + (int)(i - row * D) / CK_GROUP]);
-        if constexpr (MODE == 0 || MODE == 3) out[i] = from_f<T>(act_t<ACT, FAST>(v));
+        if constexpr (MODE == 0) out[i] = from_f<T>(act_t<ACT, FAST>(v));
         else out[i] = from_f<T>(to_f<T>(dy[i]) * act_grad_t<ACT, FAST>(v));
     }
 }
@@ -224,7 +224,7 @@ int launch_use(int dtype, const void* dy, const void* z, const int8_t* codes, co
             if (!vec)
                 ckpt8_use_any_kernel<MODE, ACT, T>
                     <<<(int)std::min<int64_t>((n + CT - 1) / CT, 148 * 16), CT, 0, st>>>(d, x, codes, exps, o, n, D, G);
-            else if (flat || MODE >= 2)  // dense z needs no groups
+            else if (flat || MODE == 2)  // dense z needs no groups
                 ckpt8_use_kernel<MODE, ACT, T, true><<<units_grid(n / 8), CT, 0, st>>>(d, x, codes, exps, o, n, D, G);
             else
                 ckpt8_use_kernel<MODE, ACT, T, false><<<units_grid(n / 8), CT, 0, st>>>(d, x, codes, exps, o, n, D, G);
@@ -234,14 +234,6 @@ int launch_use(int dtype, const void* dy, const void* z, const int8_t* codes, co
 }
 
 }  // namespace
-
-int launch_ckpt8_values(const int8_t* codes, const uint8_t* exps, int act, int odtype, void* out, int rows, int D,
-                        cudaStream_t st) {
-    return launch_use<0>(odtype, nullptr, nullptr, codes, exps, act, out, rows, D, st, "ckpt8_values_kernel");
-}
-int launch_act(int dtype, const void* z, int act, void* out, int rows, int D, cudaStream_t st) {
-    return launch_use<3>(dtype, nullptr, z, nullptr, nullptr, act, out, rows, D, st, "act_kernel");
-}
 
 }  // namespace rwkv
 
@@ -287,7 +279,7 @@ extern "C" int rwkv_ckpt8_values(const int8_t* codes, const uint8_t* exps, int a
     RWKV_REQUIRE(codes && exps && out, RWKV_E_NULL, "%s: NULL argument", fn);
     if (int rc = check_rows(rows, D, fn)) return rc;
     RWKV_REQUIRE(aligned_to(out, odtype), RWKV_E_UNSUPPORTED, "%s: out not aligned to its element type", fn);
-    return launch_ckpt8_values(codes, exps, act, odtype, out, rows, D, (cudaStream_t)stream);
+    return launch_use<0>(odtype, nullptr, nullptr, codes, exps, act, out, rows, D, (cudaStream_t)stream, fn);
 }
 
 extern "C" int rwkv_act_backward(int dtype, const void* dy, const void* z, const int8_t* codes, const uint8_t* exps,

@@ -20,8 +20,9 @@
 //   warp 0      TMA producer, ST stages
 //   warp 1      TMEM owner; one thread issues 4 tcgen05.mma (M=128, N=BN, K=16)
 //               per stage and commits the stage / the tile
-//   warps 2-9   epilogue: TMEM lane quadrant (warp & 3) = 32 rows of D, column half
-//               (warp - 2) / 4; 32 columns at a time.  A thread holds 32 consecutive
+//   warps 2-9   epilogue: TMEM lane quadrant (warp & 3) = 32 rows of D, half of the
+//               columns per 4 warps, 32 columns at a time, the other inputs
+//               (residual, pre-activation) one step ahead.  A thread holds 32 consecutive
 //               columns of one row, exactly a checkpoint group, so a group's largest
 //               |z| needs no exchange.  Results go through a swizzled 32 x 32 tile in
 //               shared memory and leave by TMA store (full 64-byte row pieces, clipped
@@ -29,10 +30,11 @@
 // Tiles are walked in groups of 8 row blocks, so that the CTAs at work at one
 // time share a few row blocks of A and a few of B in L2.
 //
-// Split-K (S > 1, when there are fewer tiles than SMs): split z of a tile sums its
-// share of the stages into a fp32 partial tile in the workspace, and
-// proj_join_kernel adds the partials in split order (deterministic) and runs
-// the epilogue.
+// Whole waves of tiles (148 at a time) run as they are; the tiles of the last,
+// partial wave are split S ways along K, so that the SMs left over share them
+// (a product of fewer tiles than SMs is all last wave).  A split writes its fp32
+// sums as a tile into the workspace, and the join kernel adds the splits in order
+// (deterministic) and runs the epilogue.
 //
 // Every mbarrier wait is bounded (tc::mbar_wait); a wait that gives up sets the
 // shared error flag, every role winds down, the producer waits (bounded) for its
@@ -46,9 +48,18 @@ namespace rwkv {
 
 constexpr int PJ_BK = 64;
 constexpr int PJ_GROUP_M = 8;      // row blocks walked together
-constexpr int PJ_EPI_WARPS = 8;
-constexpr int PJ_THREADS = 64 + 32 * PJ_EPI_WARPS;
+constexpr int PJ_SMS = 148;
 constexpr int PJ_STAGE_OUT = 4096;  // staging bytes per epilogue warp: 32 x 32 fp32, or two 32 x 32 of 16 bits
+
+// Which epilogue a kernel has, at compile time: one that can do everything keeps
+// the registers of everything alive (16384 x 8192 over 96 takes 270 us with a
+// plain result in it, __ us in its own kernel).
+enum : int {
+    PJ_PLAIN = 0,  // the sums
+    PJ_FWD = 1,    // bias, z, activation, residual
+    PJ_FWD_CK = 2, // and the checkpoint of z
+    PJ_GRAD = 3,   // times act'(pre), addend
+};
 
 // What happens to the sums; all tensors are row-major [M, N].
 struct ProjEpi {
@@ -65,14 +76,20 @@ struct ProjEpi {
     const void* pre;    // grad: pre-activation in the operand type, or
     const int8_t* pre_codes;  // its checkpoint
     const uint8_t* pre_exps;
+
+    int kind() const {
+        return grad ? PJ_GRAD : codes ? PJ_FWD_CK : bias || z || add || act != RWKV_ACT_NONE ? PJ_FWD : PJ_PLAIN;
+    }
 };
 
 struct ProjArgs {
     CUtensorMap amap, bmap;
-    CUtensorMap dmap;   // D, box {32, 32}; split-K: the partials {N, M, S} fp32, box {32, 32, 1}
+    CUtensorMap dmap;   // D, box {32, 32}
+    CUtensorMap pmap;   // the splits' tiles {BN, 128 units} fp32, box {32, 32}
     ProjEpi e;
     int M, N, nk;       // D's size, K stages
-    int mt, nt, S;      // tiles along M and N, splits
+    int mt, nt;         // tiles along M and N
+    int full, S;        // tiles that run whole; splits of each of the others
     uint32_t idesc;
     int* err;           // device flag: a wait gave up
     int* err_host;      // mapped host record
@@ -103,11 +120,79 @@ __device__ __forceinline__ uint4 pack8_16(const float* v, int bf16) {
                       pack2(v[6], v[7], bf16));
 }
 
+// The other inputs of 32 columns of one row, as read.
+struct ProjAux {
+    uint4 add[4];  // residual / addend in 16 bits (an fp32 one is read where it is added)
+    uint4 pre[4];  // pre-activation, or its 32 codes in the first two
+    uint32_t exp;  // and their exponent
+};
+__device__ __forceinline__ int64_t proj_group(int64_t row, int col, int N) {
+    return row * ((N + CK_GROUP - 1) / CK_GROUP) + col / CK_GROUP;
+}
+// 32 codes at p, the first nv (a multiple of 8) of which exist; one row in two
+// starts 8 bytes off a 16-byte boundary where N % 16 == 8.
+__device__ __forceinline__ void proj_load_codes(const int8_t* p, int nv, uint4* w) {
+    if (nv == 32 && ((uintptr_t)p & 15) == 0) {
+        w[0] = reinterpret_cast<const uint4*>(p)[0];
+        w[1] = reinterpret_cast<const uint4*>(p)[1];
+    } else {
+        const uint2 z = make_uint2(0, 0), *q = reinterpret_cast<const uint2*>(p);
+        const uint2 a = nv > 0 ? q[0] : z, b = nv > 8 ? q[1] : z, c = nv > 16 ? q[2] : z, d = nv > 24 ? q[3] : z;
+        w[0] = make_uint4(a.x, a.y, b.x, b.y);
+        w[1] = make_uint4(c.x, c.y, d.x, d.y);
+    }
+}
+__device__ __forceinline__ void proj_store_codes(int8_t* p, int nv, const uint4* w) {
+    if (nv == 32 && ((uintptr_t)p & 15) == 0) {
+        reinterpret_cast<uint4*>(p)[0] = w[0];
+        reinterpret_cast<uint4*>(p)[1] = w[1];
+    } else {
+        uint2* q = reinterpret_cast<uint2*>(p);
+        if (nv > 0) q[0] = make_uint2(w[0].x, w[0].y);
+        if (nv > 8) q[1] = make_uint2(w[0].z, w[0].w);
+        if (nv > 16) q[2] = make_uint2(w[1].x, w[1].y);
+        if (nv > 24) q[3] = make_uint2(w[1].z, w[1].w);
+    }
+}
+template <int KIND>
+__device__ __forceinline__ void proj_load_aux(const ProjEpi& e, int64_t row, int col, int nv, int N, ProjAux& x) {
+    const int64_t at = row * N + col;
+    if constexpr (KIND == PJ_GRAD) {
+        if (e.pre_codes) {
+            proj_load_codes(e.pre_codes + at, nv, x.pre);
+            x.exp = e.pre_exps[proj_group(row, col, N)];
+        } else {
+            const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(e.pre) + at);
+#pragma unroll
+            for (int i = 0; i < 4; i++) x.pre[i] = 8 * i < nv ? p[i] : make_uint4(0, 0, 0, 0);
+        }
+    }
+    if (KIND != PJ_PLAIN && e.add && !e.out_f32) {
+        const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(e.add) + at);
+#pragma unroll
+        for (int i = 0; i < 4; i++) x.add[i] = 8 * i < nv ? p[i] : make_uint4(0, 0, 0, 0);
+    }
+}
+__device__ __forceinline__ void floats8_16(const uint4& r, int bf16, float* v) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 f = unpack2(w[i], bf16);
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+    }
+}
+
 // The epilogue of columns col .. col + 31 of one row, of which the first nv (a
 // multiple of 8) exist; v holds the sums, 0 in columns that do not exist.
-__device__ __forceinline__ void proj_epilogue32(float* v, const ProjEpi& e, int64_t row, int col, int nv, int N) {
+// Returns the exponent byte of the checkpoint group, which the caller stores.
+template <int KIND>
+__device__ __forceinline__ uint32_t proj_epilogue32(float* v, const ProjEpi& e, const ProjAux& x, int64_t row, int col,
+                                                    int nv, int N) {
+    if constexpr (KIND == PJ_PLAIN) return 0;
     const int64_t at = row * N + col;
-    if (e.bias) {
+    uint32_t exp = 0;
+    if (KIND != PJ_GRAD && e.bias) {
 #pragma unroll
         for (int i = 0; i < 4; i++)
             if (8 * i < nv) {
@@ -117,48 +202,42 @@ __device__ __forceinline__ void proj_epilogue32(float* v, const ProjEpi& e, int6
                 for (int k = 0; k < 8; k++) v[8 * i + k] += b[k];
             }
     }
-    if (e.codes) {
+    if constexpr (KIND == PJ_FWD_CK) {
         uint32_t top = 0;
 #pragma unroll
         for (int i = 0; i < 32; i++) top = max(top, abs_bits(v[i]));
-        const uint32_t x = ck_exponent(top);
-        const float inv = ck_inv_scale(x);
+        exp = ck_exponent(top);
+        const float inv = ck_inv_scale(exp);
+        uint32_t w[8];
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (8 * i < nv)
-                *reinterpret_cast<uint2*>(e.codes + at + 8 * i) =
-                    make_uint2(ck_pack4(v[8 * i], v[8 * i + 1], v[8 * i + 2], v[8 * i + 3], inv),
-                               ck_pack4(v[8 * i + 4], v[8 * i + 5], v[8 * i + 6], v[8 * i + 7], inv));
-        e.exps[row * ((N + CK_GROUP - 1) / CK_GROUP) + col / CK_GROUP] = (uint8_t)x;
+        for (int i = 0; i < 8; i++) w[i] = ck_pack4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], inv);
+        const uint4 q[2] = {make_uint4(w[0], w[1], w[2], w[3]), make_uint4(w[4], w[5], w[6], w[7])};
+        proj_store_codes(e.codes + at, nv, q);
     }
-    if (e.z) {
+    if (KIND != PJ_GRAD && e.z) {
 #pragma unroll
         for (int i = 0; i < 4; i++)
             if (8 * i < nv)
                 *reinterpret_cast<uint4*>(static_cast<uint16_t*>(e.z) + at + 8 * i) = pack8_16(v + 8 * i, e.bf16);
     }
-    if (e.grad) {
-        float p[32];
-        if (e.pre_codes) {
-            const float s = ck_scale(e.pre_exps[row * ((N + CK_GROUP - 1) / CK_GROUP) + col / CK_GROUP]);
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (8 * i < nv) {
-                    const uint2 w = *reinterpret_cast<const uint2*>(e.pre_codes + at + 8 * i);
-                    ck_unpack4(w.x, s, p + 8 * i);
-                    ck_unpack4(w.y, s, p + 8 * i + 4);
-                }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (8 * i < nv) load8_16(e.pre, at + 8 * i, e.bf16, p + 8 * i);
-        }
+    if constexpr (KIND == PJ_GRAD) {
+        const float s = e.pre_codes ? ck_scale(x.exp) : 0.f;
         with_act(e.act, [&]<int ACT>() {
 #pragma unroll
-            for (int i = 0; i < 32; i++)
-                if (i < nv) v[i] *= act_grad_t<ACT, true>(p[i]);
+            for (int i = 0; i < 4; i++) {
+                float p[8];
+                if (e.pre_codes) {
+                    const uint4 c = x.pre[i / 2];
+                    ck_unpack4(i % 2 ? c.z : c.x, s, p);
+                    ck_unpack4(i % 2 ? c.w : c.y, s, p + 4);
+                } else {
+                    floats8_16(x.pre[i], e.bf16, p);
+                }
+#pragma unroll
+                for (int k = 0; k < 8; k++) v[8 * i + k] *= act_grad_t<ACT, true>(p[k]);
+            }
         });
-    } else {
+    } else if (e.act != RWKV_ACT_NONE) {
         with_act(e.act, [&]<int ACT>() {
 #pragma unroll
             for (int i = 0; i < 32; i++) v[i] = act_t<ACT, true>(v[i]);
@@ -167,31 +246,27 @@ __device__ __forceinline__ void proj_epilogue32(float* v, const ProjEpi& e, int6
     if (e.add) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            if (8 * i >= nv) break;
             float a[8];
             if (e.out_f32) {
+                if (8 * i >= nv) break;
                 const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(e.add) + at + 8 * i);
                 const float4 lo = p[0], hi = p[1];
                 a[0] = lo.x, a[1] = lo.y, a[2] = lo.z, a[3] = lo.w;
                 a[4] = hi.x, a[5] = hi.y, a[6] = hi.z, a[7] = hi.w;
             } else {
-                load8_16(e.add, at + 8 * i, e.bf16, a);
+                floats8_16(x.add[i], e.bf16, a);
             }
 #pragma unroll
             for (int k = 0; k < 8; k++) v[8 * i + k] += a[k];
         }
     }
+    return exp;
 }
 
 namespace tc {
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int c0, int c1) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(src),
                  "r"(c0), "r"(c1)
-                 : "memory");
-}
-__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2) {
-    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map),
-                 "r"(src), "r"(c0), "r"(c1), "r"(c2)
                  : "memory");
 }
 __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
@@ -207,8 +282,11 @@ struct PjCfg {
     static constexpr int A_BYTES = 128 * 128;       // 128 rows x 64 k, 16 bits
     static constexpr int B_BYTES = BN * 128;
     static constexpr int STAGE = A_BYTES + B_BYTES;
-    static constexpr int OUT_BYTES = PJ_EPI_WARPS * PJ_STAGE_OUT;
-    static constexpr int ST = 192 * 1024 / STAGE;
+    static constexpr int EW = 8;                    // epilogue warps
+    static constexpr int EC = BN / (EW / 4);        // columns of each
+    static constexpr int THREADS = 64 + 32 * EW;
+    static constexpr int OUT_BYTES = EW * PJ_STAGE_OUT;
+    static constexpr int ST = (224 * 1024 - OUT_BYTES) / STAGE;
     static constexpr int NBAR = 2 * ST + 5;
     static constexpr int O_OFF = ST * STAGE;        // output staging
     static constexpr int B_OFF = O_OFF + OUT_BYTES;
@@ -216,12 +294,13 @@ struct PjCfg {
     static constexpr int TOTAL = T_OFF + 16 + 1024;
     static constexpr int TMC = 2 * BN;
     static_assert(TOTAL <= 227 * 1024, "shared memory per CTA");
-    static_assert(BN == 64 || BN == 128 || BN == 256, "TMEM allocation is a power of two; halves in 32s");
+    static_assert(BN == 128 || BN == 256, "TMEM allocation is a power of two; shares of 32 columns");
+    static_assert(ST >= 3, "pipeline depth");
 };
 
 // AMN / BMN: the operand is MN-major.
-template <int BN, bool AMN, bool BMN>
-__global__ void __launch_bounds__(PJ_THREADS, 1) proj_kernel(const __grid_constant__ ProjArgs a) {
+template <int BN, bool AMN, bool BMN, int KIND>
+__global__ void __launch_bounds__(PjCfg<BN>::THREADS, 1) proj_kernel(const __grid_constant__ ProjArgs a) {
     using C = PjCfg<BN>;
     constexpr int ST = C::ST;
     extern __shared__ unsigned char smem_raw[];
@@ -234,8 +313,8 @@ __global__ void __launch_bounds__(PJ_THREADS, 1) proj_kernel(const __grid_consta
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::T_OFF);
     int* skip_slot = reinterpret_cast<int*>(smem + C::T_OFF + 8);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int ntiles = a.mt * a.nt * a.S;
-    const int my_tiles = (int)blockIdx.x < ntiles ? (ntiles - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
+    const int units = a.full + (a.mt * a.nt - a.full) * a.S;
+    const int my_tiles = (int)blockIdx.x < units ? (units - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
     int* err = a.err;
 
     if (tid == 0) {
@@ -245,7 +324,7 @@ __global__ void __launch_bounds__(PJ_THREADS, 1) proj_kernel(const __grid_consta
         }
         for (int b = 0; b < 2; b++) {
             tc::mbar_init(accf + b, 1);
-            tc::mbar_init(acce + b, PJ_EPI_WARPS);
+            tc::mbar_init(acce + b, C::EW);
         }
         tc::mbar_init(done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -260,26 +339,35 @@ __global__ void __launch_bounds__(PJ_THREADS, 1) proj_kernel(const __grid_consta
     tc::tc_before();
     __syncthreads();
     tc::tc_after();
+    pdl_wait();  // everything before read only this kernel's arguments and the flag
     const uint32_t tmem = *tmem_slot;
     const bool skip = *skip_slot != 0;
     bool ok = !skip;
     const int tiles = skip ? 0 : my_tiles;
 
-    // tile i of this CTA: first row and column, split, stages [k0, k1)
+    // unit i of this CTA: first row and column, stages [k0, k1), and for a split
+    // the row of its tile in the workspace (-1: a whole tile)
     struct Tile {
-        int m0, n0, z, k0, k1;
+        int m0, n0, k0, k1, part;
     };
     auto tile_at = [&](int i) {
-        int t = (int)blockIdx.x + i * (int)gridDim.x;
+        const int u = (int)blockIdx.x + i * (int)gridDim.x;
         Tile r;
-        r.z = t % a.S;
-        t /= a.S;
+        int t = u;
+        r.k0 = 0;
+        r.k1 = a.nk;
+        r.part = -1;
+        if (u >= a.full && a.S > 1) {
+            const int j = (u - a.full) / a.S, z = u - a.full - j * a.S;
+            t = a.full + j;
+            r.k0 = (int)((int64_t)a.nk * z / a.S);
+            r.k1 = (int)((int64_t)a.nk * (z + 1) / a.S);
+            r.part = (u - a.full) * 128;
+        }
         const int per = PJ_GROUP_M * a.nt, g = t / per, rem = t - g * per;
         const int gm = min(PJ_GROUP_M, a.mt - g * PJ_GROUP_M);
         r.m0 = (g * PJ_GROUP_M + rem % gm) * 128;
         r.n0 = rem / gm * BN;
-        r.k0 = (int)((int64_t)a.nk * r.z / a.S);
-        r.k1 = (int)((int64_t)a.nk * (r.z + 1) / a.S);
         return r;
     };
 
@@ -352,30 +440,38 @@ __global__ void __launch_bounds__(PJ_THREADS, 1) proj_kernel(const __grid_consta
         }
     } else {
         // ---- epilogue
-        const int q = warp & 3, half = (warp - 2) >> 2;
+        const int q = warp & 3, c0 = (warp - 2) / 4 * C::EC;
         const uint32_t lane_base = (uint32_t)(32 * q) << 16;
         const uint32_t stage = tc::saddr(smem + C::O_OFF + (warp - 2) * PJ_STAGE_OUT);
-        const bool wide = a.S > 1 || a.e.out_f32;  // 4-byte results
-        int nst = 0;                                // stores issued by this warp
+        int nst = 0;  // stores issued by this warp
         for (int i = 0; i < tiles; i++) {
             const Tile t = tile_at(i);
-            const int b = i & 1;
+            const int b = i & 1, row = t.m0 + 32 * q + lane;
+            const bool part = t.part >= 0, wide = part || a.e.out_f32;  // 4-byte results
+            const bool live = !part && row < a.M;
+            // this warp's columns c0 .. c1 of the tile that exist, in whole steps of 32
+            const int c1 = t.m0 + 32 * q >= a.M ? c0 : min(c0 + C::EC, a.N - t.n0);
+            ProjAux aux;
+            if (live && c0 < c1) proj_load_aux<KIND>(a.e, row, t.n0 + c0, min(32, a.N - t.n0 - c0), a.N, aux);
             if (!tc::mbar_wait(accf + b, (i >> 1) & 1, err)) {
                 ok = false;
                 break;
             }
             tc::tc_after();
-            const int row = t.m0 + 32 * q + lane;
-            for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 32) {
+            uint32_t exps = 0;
+            for (int c = c0; c < c1; c += 32) {
                 const int col = t.n0 + c;
-                if (col >= a.N || t.m0 + 32 * q >= a.M) break;  // whole warps
                 uint32_t r[32];
                 tc::tmem_ld32_async(tmem + lane_base + b * BN + c, r);
                 tc::tmem_ld_wait();
                 float v[32];
 #pragma unroll
                 for (int k = 0; k < 32; k++) v[k] = __uint_as_float(r[k]);
-                if (a.S == 1 && row < a.M) proj_epilogue32(v, a.e, row, col, min(32, a.N - col), a.N);
+                if (live) {
+                    const ProjAux now = aux;
+                    if (c + 32 < c1) proj_load_aux<KIND>(a.e, row, col + 32, min(32, a.N - col - 32), a.N, aux);
+                    exps |= proj_epilogue32<KIND>(v, a.e, now, row, col, min(32, a.N - col), a.N) << ((c - c0) / 4);
+                }
                 // the staging tile is free once the store that read it last is done
                 if (lane == 0) {
                     if (wide) tc::bulk_wait_read<0>();
@@ -400,7 +496,7 @@ __global__ void __launch_bounds__(PJ_THREADS, 1) proj_kernel(const __grid_consta
                 tc::fence_async_smem();
                 __syncwarp();
                 if (lane == 0) {
-                    if (a.S > 1) tc::tma_store_3d(&a.dmap, base, col, t.m0 + 32 * q, t.z);
+                    if (part) tc::tma_store_2d(&a.pmap, base, c, t.part + 32 * q);
                     else tc::tma_store_2d(&a.dmap, base, col, t.m0 + 32 * q);
                     tc::bulk_commit();
                 }
@@ -409,6 +505,16 @@ __global__ void __launch_bounds__(PJ_THREADS, 1) proj_kernel(const __grid_consta
             tc::tc_before();
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(acce + b);
+            if (KIND == PJ_FWD_CK && live && c0 < c1) {
+                // the exponents of this warp's groups, together where they are a word
+                uint8_t* p = a.e.exps + proj_group(row, t.n0 + c0, a.N);
+                const int n = (c1 - c0 + 31) / 32;
+                if (n == 4 && ((uintptr_t)p & 3) == 0) {
+                    *reinterpret_cast<uint32_t*>(p) = exps;
+                } else {
+                    for (int k = 0; k < n; k++) p[k] = (uint8_t)(exps >> (8 * k));
+                }
+            }
         }
         if (lane == 0) tc::bulk_wait<0>();
     }
@@ -424,60 +530,110 @@ __global__ void __launch_bounds__(PJ_THREADS, 1) proj_kernel(const __grid_consta
     }
 }
 
-// Joins split-K partials: part [S][M][N] fp32.  A thread takes 32 columns of a row.
-static __global__ void __launch_bounds__(128) proj_join_kernel(const float* __restrict__ part, const ProjEpi e, void* d, int M,
-                                                        int N, int S) {
-    const int per = (N + 31) / 32;
-    const int64_t i = blockIdx.x * (int64_t)128 + threadIdx.x;
-    if (i >= (int64_t)M * per) return;
-    const int64_t row = i / per;
-    const int col = (int)(i - row * per) * 32, nv = min(32, N - col);
-    const int64_t at = row * N + col;
+struct ProjJoin {
+    const float* part;  // [(tile - full) S + split][128][BN]
+    ProjEpi e;
+    void* d;
+    int M, N, mt, nt, full, S, BN;
+};
+// Joins the splits of the tiles full ..: thread i takes 32 columns of a row of a tile.
+template <int KIND>
+__device__ __forceinline__ void proj_join(const ProjJoin& a, int64_t i) {
+    const int per = a.BN / 32;
+    const int chunk = (int)(i % per), r = (int)(i / per % 128);
+    const int64_t j = i / per / 128;
+    int t = a.full + (int)j;
+    if (t >= a.mt * a.nt) return;
+    const int pg = PJ_GROUP_M * a.nt, g = t / pg, rem = t - g * pg;
+    const int gm = min(PJ_GROUP_M, a.mt - g * PJ_GROUP_M);
+    const int64_t row = (g * PJ_GROUP_M + rem % gm) * 128 + r;
+    const int col = rem / gm * a.BN + 32 * chunk;
+    if (row >= a.M || col >= a.N) return;
+    const int nv = min(32, a.N - col);
+    ProjAux x;
+    proj_load_aux<KIND>(a.e, row, col, nv, a.N, x);
     float v[32];
 #pragma unroll
     for (int k = 0; k < 32; k++) v[k] = 0.f;
-    for (int z = 0; z < S; z++) {
-        const float4* p = reinterpret_cast<const float4*>(part + (int64_t)z * M * N + at);
+    const float* p = a.part + (j * a.S * 128 + r) * a.BN + 32 * chunk;
+    for (int z = 0; z < a.S; z++, p += 128 * a.BN) {
 #pragma unroll
-        for (int k = 0; k < 8; k++)
-            if (4 * k < nv) {
-                const float4 f = p[k];
-                v[4 * k] += f.x, v[4 * k + 1] += f.y, v[4 * k + 2] += f.z, v[4 * k + 3] += f.w;
-            }
+        for (int k = 0; k < 8; k++) {
+            const float4 f = reinterpret_cast<const float4*>(p)[k];
+            v[4 * k] += f.x, v[4 * k + 1] += f.y, v[4 * k + 2] += f.z, v[4 * k + 3] += f.w;
+        }
     }
-    proj_epilogue32(v, e, row, col, nv, N);
+    const uint32_t exp = proj_epilogue32<KIND>(v, a.e, x, row, col, nv, a.N);
+    if (KIND == PJ_FWD_CK) a.e.exps[proj_group(row, col, a.N)] = (uint8_t)exp;
+    const int64_t at = row * a.N + col;
 #pragma unroll
     for (int k = 0; k < 4; k++)
         if (8 * k < nv) {
-            if (e.out_f32) {
-                float4* o = reinterpret_cast<float4*>(static_cast<float*>(d) + at + 8 * k);
+            if (a.e.out_f32) {
+                float4* o = reinterpret_cast<float4*>(static_cast<float*>(a.d) + at + 8 * k);
                 o[0] = make_float4(v[8 * k], v[8 * k + 1], v[8 * k + 2], v[8 * k + 3]);
                 o[1] = make_float4(v[8 * k + 4], v[8 * k + 5], v[8 * k + 6], v[8 * k + 7]);
             } else {
-                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(d) + at + 8 * k) = pack8_16(v + 8 * k, e.bf16);
+                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.d) + at + 8 * k) = pack8_16(v + 8 * k, a.e.bf16);
             }
         }
+}
+// Column sums of dY, joined beside the tiles (rwkv_projection_dw's db): blocks from
+// `first` on take 128 columns each and add the slices in order.
+struct ColJoin {
+    const float* part;  // [slices][N]
+    float* out;
+    int N, slices;
+};
+constexpr int PJ_JOIN_T = 128;
+template <int KIND>
+__global__ void __launch_bounds__(PJ_JOIN_T) proj_join_kernel(const ProjJoin a, const ColJoin c, int first) {
+    pdl_wait();
+    if ((int)blockIdx.x < first) {
+        proj_join<KIND>(a, blockIdx.x * (int64_t)PJ_JOIN_T + threadIdx.x);
+        return;
+    }
+    const int col = ((int)blockIdx.x - first) * PJ_JOIN_T + threadIdx.x;
+    if (col >= c.N) return;
+    float s = 0.f;
+#pragma unroll 8
+    for (int k = 0; k < c.slices; k++) s += c.part[(int64_t)k * c.N + col];
+    c.out[col] = s;
 }
 
 // ------------------------------------------------------------------ host side
 
-// Tile width and splits for an M x N product over nk stages, from the sizes
-// alone (the workspace query has to agree with the call).
+// Tile width, whole tiles and splits of the others for an M x N product, from the
+// sizes alone (the workspace query has to agree with the call).
+//  - Tiles of 256 columns where they fill the SMs; of 128 for products too short
+//    to hide a wide tile's epilogue (K <= 512: 4093 x 2048 over 96 with a sigmoid
+//    takes __ us in 128s, 27.5 in 256s) and where they give more SMs work.
+//  - The tiles past the last whole wave are split the way that the estimate below
+//    finds shortest: a stage of 64 takes 0.35 us on a 256-wide tile; joining takes
+//    3 us and writes and reads each split's tile once (4 TB/s).
 struct ProjPlan {
-    int BN, mt, nt, S;
-    int64_t ws_bytes;  // split-K partials
+    int BN, mt, nt, full, S;
+    int64_t ws_bytes;  // the splits' tiles
 };
 inline ProjPlan proj_plan(int64_t M, int64_t N, int64_t K) {
     ProjPlan p{};
     const int nk = (int)((K + PJ_BK - 1) / PJ_BK);
     p.mt = (int)((M + 127) / 128);
-    p.BN = 256;
-    while (p.BN > 64 && (int64_t)p.mt * ((N + p.BN - 1) / p.BN) < 148) p.BN /= 2;
+    p.BN = K > 512 && (int64_t)p.mt * ((N + 255) / 256) >= PJ_SMS ? 256 : 128;
     p.nt = (int)((N + p.BN - 1) / p.BN);
-    const int64_t tiles = (int64_t)p.mt * p.nt;
-    // split K until every SM has a tile, with at least 4 stages per split
-    p.S = (int)std::max<int64_t>(1, std::min<int64_t>(148 / std::max<int64_t>(1, tiles), nk / 4));
-    p.ws_bytes = p.S > 1 ? (int64_t)p.S * M * N * 4 : 0;
+    const int tiles = p.mt * p.nt, rem = tiles % PJ_SMS;
+    p.full = tiles - rem;
+    p.S = 1;
+    if (rem == 0) return p;
+    double best = 0.0;
+    for (int S = 1; S <= 16 && (S == 1 || nk / S >= 2); S++) {
+        const double stage = 0.35 * p.BN / 256, bytes = 2.0 * rem * S * 128 * p.BN * 4;
+        const double us = (double)((rem * S + PJ_SMS - 1) / PJ_SMS) * ((nk + S - 1) / S) * stage +
+                          (S > 1 ? 3.0 + bytes / 4e6 : 0.0);
+        if (S == 1 || us < best) best = us, p.S = S;
+    }
+    if (p.S == 1) p.full = tiles;
+    else p.ws_bytes = (int64_t)rem * p.S * 128 * p.BN * 4;
     return p;
 }
 
@@ -493,21 +649,27 @@ inline bool proj_map_2d(CUtensorMap* m, CUtensorMapDataType type, int esize, con
                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int BN, bool AMN, bool BMN>
-inline cudaError_t proj_launch_t(const ProjArgs& a, int sm_count, cudaStream_t st) {
+template <int BN, bool AMN, bool BMN, int KIND>
+inline cudaError_t proj_launch_t(const ProjArgs& a, int sm_count, bool after_own, cudaStream_t st) {
     using C = PjCfg<BN>;
-    auto kern = proj_kernel<BN, AMN, BMN>;
+    auto kern = proj_kernel<BN, AMN, BMN, KIND>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::TOTAL);
     if (e != cudaSuccess) return e;
-    const int64_t tiles = (int64_t)a.mt * a.nt * a.S;
-    kern<<<(int)std::min<int64_t>(tiles, sm_count), PJ_THREADS, C::TOTAL, st>>>(a);
+    const int units = a.full + (a.mt * a.nt - a.full) * a.S;
+    const dim3 grid(std::min(units, sm_count)), block(C::THREADS);
+    if (after_own) return launch_pdl(kern, grid, block, C::TOTAL, st, a);
+    kern<<<grid, block, C::TOTAL, st>>>(a);
     return cudaGetLastError();
 }
 
-// D [M, N] = epilogue(A B^T), A [M, K] (AMN: stored [K, M]), B [N, K] (BMN: stored [K, N]).
-template <bool AMN, bool BMN>
+// D [M, N] = epilogue(A B^T), A [M, K] (AMN: stored [K, M]), B [N, K] (BMN: stored
+// [K, N]); with `cols` the column sums beside it.  after_own: the launch before
+// this one on the stream is this call's own, of a kernel without TMEM, so that this
+// one may start its set-up beside it.
+template <bool AMN, bool BMN, int KIND>
 inline cudaError_t proj_gemm(const void* A, const void* B, void* D, int64_t M, int64_t N, int64_t K, const ProjEpi& e,
-                             float* ws, int* err, int* err_host, int sm_count, cudaStream_t st) {
+                             float* ws, int* err, int* err_host, int sm_count, cudaStream_t st, bool after_own = false,
+                             const ColJoin* cols = nullptr) {
     const ProjPlan p = proj_plan(M, N, K);
     ProjArgs a{};
     a.e = e;
@@ -516,37 +678,31 @@ inline cudaError_t proj_gemm(const void* A, const void* B, void* D, int64_t M, i
     a.nk = (int)((K + PJ_BK - 1) / PJ_BK);
     a.mt = p.mt;
     a.nt = p.nt;
+    a.full = p.full;
     a.S = p.S;
     a.idesc = tc::idesc_f16(128, p.BN, e.bf16 != 0) | (AMN ? 1u << 15 : 0u) | (BMN ? 1u << 16 : 0u);
     a.err = err;
     a.err_host = err_host;
+    const int rem = p.mt * p.nt - p.full;
     const CUtensorMapDataType t16 = e.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     const auto sw128 = CU_TENSOR_MAP_SWIZZLE_128B;
     bool ok = AMN ? proj_map_2d(&a.amap, t16, 2, A, M, K, 64, PJ_BK, sw128)
                   : proj_map_2d(&a.amap, t16, 2, A, K, M, PJ_BK, 128, sw128);
     ok = ok && (BMN ? proj_map_2d(&a.bmap, t16, 2, B, N, K, 64, PJ_BK, sw128)
                     : proj_map_2d(&a.bmap, t16, 2, B, K, N, PJ_BK, p.BN, sw128));
-    if (p.S > 1) {
-        auto enc = tensor_map_encoder();
-        cuuint32_t es[3] = {1, 1, 1}, box[3] = {32, 32, 1};
-        cuuint64_t dims[3] = {(cuuint64_t)N, (cuuint64_t)M, (cuuint64_t)p.S};
-        cuuint64_t strides[2] = {(cuuint64_t)N * 4, (cuuint64_t)(M * N) * 4};
-        ok = ok && enc(&a.dmap, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, ws, dims, strides, box, es,
-                       CU_TENSOR_MAP_INTERLEAVE_NONE, sw128, CU_TENSOR_MAP_L2_PROMOTION_NONE,
-                       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-    } else if (e.out_f32) {
-        ok = ok && proj_map_2d(&a.dmap, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, D, N, M, 32, 32, sw128);
-    } else {
-        ok = ok && proj_map_2d(&a.dmap, t16, 2, D, N, M, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
-    }
+    ok = ok && (e.out_f32 ? proj_map_2d(&a.dmap, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, D, N, M, 32, 32, sw128)
+                          : proj_map_2d(&a.dmap, t16, 2, D, N, M, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B));
+    if (p.S > 1)
+        ok = ok && proj_map_2d(&a.pmap, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, ws, p.BN, (int64_t)rem * p.S * 128, 32, 32,
+                               sw128);
     if (!ok) return cudaErrorInvalidValue;
-    cudaError_t rc = p.BN == 64    ? proj_launch_t<64, AMN, BMN>(a, sm_count, st)
-                     : p.BN == 128 ? proj_launch_t<128, AMN, BMN>(a, sm_count, st)
-                                   : proj_launch_t<256, AMN, BMN>(a, sm_count, st);
-    if (rc != cudaSuccess || p.S == 1) return rc;
-    const int64_t threads = M * ((N + 31) / 32);
-    proj_join_kernel<<<ceil_div(threads, 128), 128, 0, st>>>(ws, e, D, (int)M, (int)N, p.S);
-    return cudaGetLastError();
+    const cudaError_t rc = p.BN == 128 ? proj_launch_t<128, AMN, BMN, KIND>(a, sm_count, after_own, st)
+                                       : proj_launch_t<256, AMN, BMN, KIND>(a, sm_count, after_own, st);
+    if (rc != cudaSuccess || (p.S == 1 && !cols)) return rc;
+    const ProjJoin j{ws, e, D, (int)M, (int)N, p.mt, p.nt, p.full, p.S, p.BN};
+    const int first = p.S > 1 ? ceil_div((int64_t)rem * 128 * (p.BN / 32), PJ_JOIN_T) : 0;
+    const ColJoin c = cols ? *cols : ColJoin{};
+    return launch_pdl(proj_join_kernel<KIND>, dim3(first + ceil_div(c.N, PJ_JOIN_T)), dim3(PJ_JOIN_T), 0, st, j, c, first);
 }
 
 }  // namespace rwkv

@@ -5,51 +5,116 @@
 
 namespace rwkv {
 
-// qaffine.cu, ckpt8.cu
+// qaffine.cu
 int gemm_wait_record(cudaStream_t st, const char* fn, int** err, int** err_host, int* sm_count);
-int launch_ckpt8_values(const int8_t* codes, const uint8_t* exps, int act, int odtype, void* out, int rows, int D,
-                        cudaStream_t st);
-int launch_act(int dtype, const void* z, int act, void* out, int rows, int D, cudaStream_t st);
 
 namespace {
 
-// Column sums of dY [rows, OUT] (16 bits): a thread takes 8 columns of every
-// 8th row of its block's slice; the 8 row lanes meet in shared memory.
-constexpr int CS_COLS = 256;
-__global__ void __launch_bounds__(256) col_sum_kernel(const void* __restrict__ dy, float* __restrict__ part, int rows,
-                                                      int OUT, int bf16) {
-    __shared__ float red[8][CS_COLS];
-    const int cv = threadIdx.x & 31, rl = threadIdx.x >> 5;
-    const int col = blockIdx.x * CS_COLS + cv * 8;
-    float s[8] = {};
-    if (col < OUT)
-        for (int64_t r = (int64_t)blockIdx.y * 8 + rl; r < rows; r += 8 * (int64_t)gridDim.y) {
+// What dW needs before its product, in one launch: blocks below `first` write act(X)
+// in the operands' type (from the dense pre-activation or its checkpoint), the
+// others sum slices of dY's columns.
+//
+// Restoring the operand in a pass of its own reads and writes it once (8192 x 8192:
+// 32 us of 320); decoding inside the product would repeat the work for every 128
+// outputs of dW, 64 times here.
+struct DwPrep {
+    const void* x;         // dense, or
+    const int8_t* codes;   // its checkpoint
+    const uint8_t* exps;
+    void* operand;         // [rows, IN] or NULL
+    int act, IN;
+    int64_t units;         // of 8 channels
+    const void* dy;        // [rows, OUT]
+    float* part;           // [slices][OUT] or NULL
+    int rows, OUT, slices, bf16;
+    int first;
+};
+constexpr int PREP_T = 256, PREP_U = 4, CS_COLS = 256;
+
+__device__ __forceinline__ void restore_operand(const DwPrep& a) {
+    const int64_t i0 = blockIdx.x * (int64_t)(PREP_T * PREP_U) + threadIdx.x;
+    const int G = (a.IN + CK_GROUP - 1) / CK_GROUP, per = a.IN / 8;
+    uint4 raw[PREP_U];
+    uint32_t e[PREP_U];
+#pragma unroll
+    for (int j = 0; j < PREP_U; j++) {
+        const int64_t i = i0 + j * PREP_T;
+        if (i >= a.units) continue;
+        if (a.codes) {
+            const uint2 w = __ldcs(reinterpret_cast<const uint2*>(a.codes + 8 * i));
+            raw[j] = make_uint4(w.x, w.y, 0, 0);
+            int64_t group = i >> 2;
+            if (a.IN % CK_GROUP) {
+                const int64_t row = a.units < (1ll << 32) ? (uint32_t)i / (uint32_t)per : i / per;
+                group = row * G + ((int)(i - row * per) >> 2);
+            }
+            e[j] = a.exps[group];
+        } else {
+            raw[j] = __ldcs(static_cast<const uint4*>(a.x) + i);
+        }
+    }
+    with_act(a.act, [&]<int ACT>() {
+#pragma unroll
+        for (int j = 0; j < PREP_U; j++) {
+            const int64_t i = i0 + j * PREP_T;
+            if (i >= a.units) continue;
             float v[8];
-            load8_16(dy, r * OUT + col, bf16, v);
+            if (a.codes) {
+                const float s = ck_scale(e[j]);
+                ck_unpack4(raw[j].x, s, v);
+                ck_unpack4(raw[j].y, s, v + 4);
+            } else {
+                floats8_16(raw[j], a.bf16, v);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] = act_t<ACT, true>(v[k]);
+            static_cast<uint4*>(a.operand)[i] = pack8_16(v, a.bf16);
+        }
+    });
+}
+
+// A block sums 256 columns of every (8 slices)th group of 8 rows: a thread takes 8
+// columns of one row of each group, the 8 row lanes meet in shared memory.
+__device__ __forceinline__ void sum_columns(const DwPrep& a, int block) {
+    __shared__ float red[8][CS_COLS];
+    const int cv = threadIdx.x & 31, rl = threadIdx.x >> 5, cblocks = (a.OUT + CS_COLS - 1) / CS_COLS;
+    const int slice = block / cblocks, c0 = (block - slice * cblocks) * CS_COLS, col = c0 + cv * 8;
+    float s[8] = {};
+    if (col < a.OUT)
+#pragma unroll 4
+        for (int64_t r = (int64_t)slice * 8 + rl; r < a.rows; r += 8 * (int64_t)a.slices) {
+            float v[8];
+            load8_16(a.dy, r * a.OUT + col, a.bf16, v);
 #pragma unroll
             for (int k = 0; k < 8; k++) s[k] += v[k];
         }
 #pragma unroll
     for (int k = 0; k < 8; k++) red[rl][cv * 8 + k] = s[k];
     __syncthreads();
-    const int c = blockIdx.x * CS_COLS + threadIdx.x;
-    if (c < OUT) {
+    const int c = c0 + threadIdx.x;
+    if (c < a.OUT) {
         float t = 0.f;
 #pragma unroll
         for (int k = 0; k < 8; k++) t += red[k][threadIdx.x];
-        part[(int64_t)blockIdx.y * OUT + c] = t;
+        a.part[(int64_t)slice * a.OUT + c] = t;
     }
 }
-__global__ void __launch_bounds__(256) col_join_kernel(const float* __restrict__ part, float* __restrict__ db, int OUT,
-                                                       int slices) {
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= OUT) return;
-    float s = 0.f;
-    for (int k = 0; k < slices; k++) s += part[(int64_t)k * OUT + c];
-    db[c] = s;
+__global__ void __launch_bounds__(PREP_T, 1) dw_prep_kernel(const DwPrep a) {
+    if ((int)blockIdx.x < a.first) restore_operand(a);
+    else sum_columns(a, (int)blockIdx.x - a.first);
 }
 int col_slices(int rows, int OUT) {
     return std::max(1, std::min(ceil_div(rows, 64), 148 * 4 / ceil_div(OUT, CS_COLS)));
+}
+
+template <typename F>
+cudaError_t by_kind(const ProjEpi& e, F&& f) {
+    switch (e.kind()) {
+        case PJ_GRAD: return f.template operator()<PJ_GRAD>();
+        case PJ_FWD_CK: return f.template operator()<PJ_FWD_CK>();
+        case PJ_FWD: return f.template operator()<PJ_FWD>();
+        default: return f.template operator()<PJ_PLAIN>();
+    }
 }
 
 int64_t al256(int64_t n) { return (n + 255) / 256 * 256; }
@@ -118,8 +183,10 @@ extern "C" int rwkv_projection_forward(int dtype, const void* x, const void* w, 
     e.z = z;
     const cudaError_t rc =
         few ? launch_gemv_proj(GemvProjArgs{x, w, y, e, rows, OUT, IN}, sms, (cudaStream_t)stream)
-            : proj_gemm<false, false>(x, w, y, rows, OUT, IN, e, static_cast<float*>(workspace), err, err_host, sms,
-                                      (cudaStream_t)stream);
+            : by_kind(e, [&]<int KIND>() {
+                  return proj_gemm<false, false, KIND>(x, w, y, rows, OUT, IN, e, static_cast<float*>(workspace), err,
+                                                       err_host, sms, (cudaStream_t)stream);
+              });
     if (rc != cudaSuccess) return fail(RWKV_E_CUDA, "%s: %s", fn, cudaGetErrorString(rc));
     return ok();
 }
@@ -153,8 +220,10 @@ extern "C" int rwkv_projection_dx(int dtype, const void* dy, const void* w, int 
     e.pre_codes = codes;
     e.pre_exps = exps;
     e.add = addend;
-    const cudaError_t rc = proj_gemm<false, true>(dy, w, dx, rows, IN, OUT, e, static_cast<float*>(workspace), err,
-                                                  err_host, sms, (cudaStream_t)stream);
+    const cudaError_t rc = by_kind(e, [&]<int KIND>() {
+        return proj_gemm<false, true, KIND == PJ_FWD_CK ? PJ_FWD : KIND>(  // never keeps a checkpoint
+            dy, w, dx, rows, IN, OUT, e, static_cast<float*>(workspace), err, err_host, sms, (cudaStream_t)stream);
+    });
     if (rc != cudaSuccess) return fail(RWKV_E_CUDA, "%s: %s", fn, cudaGetErrorString(rc));
     return ok();
 }
@@ -197,25 +266,37 @@ extern "C" int rwkv_projection_dw(int dtype, const void* dy, int act, const void
     int *err, *err_host, sms;
     if (int rc = gemm_wait_record(st, fn, &err, &err_host, &sms)) return rc;
     char* ws = static_cast<char*>(workspace);
-    const void* operand = x;
-    if (restore) {
-        operand = ws;
-        if (int rc = codes ? launch_ckpt8_values(codes, exps, act, dtype, ws, rows, IN, st)
-                           : launch_act(dtype, x, act, ws, rows, IN, st))
-            return rc;
+    DwPrep q{};
+    q.x = x;
+    q.codes = codes;
+    q.exps = exps;
+    q.operand = ws;
+    q.act = act;
+    q.IN = IN;
+    q.units = (int64_t)rows * IN / 8;
+    q.dy = dy;
+    q.part = reinterpret_cast<float*>(ws + p.operand + p.parts);
+    q.rows = rows;
+    q.OUT = OUT;
+    q.slices = p.slices;
+    q.bf16 = dtype == RWKV_BF16;
+    q.first = restore ? ceil_div(q.units, PREP_T * PREP_U) : 0;
+    const int grid = q.first + (db ? ceil_div(OUT, CS_COLS) * p.slices : 0);
+    if (grid) {
+        dw_prep_kernel<<<grid, PREP_T, 0, st>>>(q);
+        if (int rc = check_launch("dw_prep_kernel")) return rc;
     }
-    ProjEpi e{};
-    e.bf16 = dtype == RWKV_BF16;
-    e.out_f32 = dwdtype == RWKV_F32;
+    const ColJoin cols{q.part, db, OUT, p.slices};
+    cudaError_t rc;
     if (dw) {
-        const cudaError_t rc = proj_gemm<true, true>(dy, operand, dw, OUT, IN, rows, e,
-                                                     reinterpret_cast<float*>(ws + p.operand), err, err_host, sms, st);
-        if (rc != cudaSuccess) return fail(RWKV_E_CUDA, "%s: %s", fn, cudaGetErrorString(rc));
+        ProjEpi e{};
+        e.bf16 = q.bf16;
+        e.out_f32 = dwdtype == RWKV_F32;
+        rc = proj_gemm<true, true, PJ_PLAIN>(dy, restore ? ws : x, dw, OUT, IN, rows, e, reinterpret_cast<float*>(ws + p.operand),
+                                   err, err_host, sms, st, grid != 0, db ? &cols : nullptr);
+    } else {
+        rc = launch_pdl(proj_join_kernel<PJ_PLAIN>, dim3(ceil_div(OUT, PJ_JOIN_T)), dim3(PJ_JOIN_T), 0, st, ProjJoin{}, cols, 0);
     }
-    if (!db) return ok();
-    float* part = reinterpret_cast<float*>(ws + p.operand + p.parts);
-    col_sum_kernel<<<dim3(ceil_div(OUT, CS_COLS), p.slices), 256, 0, st>>>(dy, part, rows, OUT, e.bf16);
-    if (int r = check_launch("col_sum_kernel")) return r;
-    col_join_kernel<<<ceil_div(OUT, 256), 256, 0, st>>>(part, db, OUT, p.slices);
-    return check_launch("col_join_kernel");
+    if (rc != cudaSuccess) return fail(RWKV_E_CUDA, "%s: %s", fn, cudaGetErrorString(rc));
+    return ok();
 }
