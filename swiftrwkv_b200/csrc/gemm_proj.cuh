@@ -85,11 +85,13 @@ struct ProjEpi {
 struct ProjArgs {
     CUtensorMap amap, bmap;
     CUtensorMap dmap;   // D, box {32, 32}
+    CUtensorMap cmap;   // checkpoint codes, box {32, 32} (N % 16 == 0)
     CUtensorMap pmap;   // the splits' tiles {BN, 128 units} fp32, box {32, 32}
     ProjEpi e;
     int M, N, nk;       // D's size, K stages
     int mt, nt;         // tiles along M and N
     int full, S;        // tiles that run whole; splits of each of the others
+    int ctma;           // codes leave by TMA
     uint32_t idesc;
     int* err;           // device flag: a wait gave up
     int* err_host;      // mapped host record
@@ -120,12 +122,6 @@ __device__ __forceinline__ uint4 pack8_16(const float* v, int bf16) {
                       pack2(v[6], v[7], bf16));
 }
 
-// The other inputs of 32 columns of one row, as read.
-struct ProjAux {
-    uint4 add[4];  // residual / addend in 16 bits (an fp32 one is read where it is added)
-    uint4 pre[4];  // pre-activation, or its 32 codes in the first two
-    uint32_t exp;  // and their exponent
-};
 __device__ __forceinline__ int64_t proj_group(int64_t row, int col, int N) {
     return row * ((N + CK_GROUP - 1) / CK_GROUP) + col / CK_GROUP;
 }
@@ -143,21 +139,24 @@ __device__ __forceinline__ void proj_load_codes(const int8_t* p, int nv, uint4* 
     }
 }
 __device__ __forceinline__ void proj_store_codes(int8_t* p, int nv, const uint4* w) {
-    if (nv == 32 && ((uintptr_t)p & 15) == 0) {
-        reinterpret_cast<uint4*>(p)[0] = w[0];
-        reinterpret_cast<uint4*>(p)[1] = w[1];
-    } else {
-        uint2* q = reinterpret_cast<uint2*>(p);
-        if (nv > 0) q[0] = make_uint2(w[0].x, w[0].y);
-        if (nv > 8) q[1] = make_uint2(w[0].z, w[0].w);
-        if (nv > 16) q[2] = make_uint2(w[1].x, w[1].y);
-        if (nv > 24) q[3] = make_uint2(w[1].z, w[1].w);
-    }
+    uint2* q = reinterpret_cast<uint2*>(p);
+    if (nv > 0) q[0] = make_uint2(w[0].x, w[0].y);
+    if (nv > 8) q[1] = make_uint2(w[0].z, w[0].w);
+    if (nv > 16) q[2] = make_uint2(w[1].x, w[1].y);
+    if (nv > 24) q[3] = make_uint2(w[1].z, w[1].w);
 }
+
+// The other inputs of 32 columns of one row, as read.
+struct ProjAux {
+    uint4 add[4];  // residual / addend, 16 bits
+    uint4 pre[4];  // pre-activation, or its 32 codes in the first two
+    uint32_t exp;  // and their exponent
+    float bias;    // of column (lane)
+};
 template <int KIND>
-__device__ __forceinline__ void proj_load_aux(const ProjEpi& e, int64_t row, int col, int nv, int N, ProjAux& x) {
-    const int64_t at = row * N + col;
+__device__ __forceinline__ void proj_load_pre(const ProjEpi& e, int64_t row, int col, int nv, int N, ProjAux& x) {
     if constexpr (KIND == PJ_GRAD) {
+        const int64_t at = row * N + col;
         if (e.pre_codes) {
             proj_load_codes(e.pre_codes + at, nv, x.pre);
             x.exp = e.pre_exps[proj_group(row, col, N)];
@@ -167,10 +166,28 @@ __device__ __forceinline__ void proj_load_aux(const ProjEpi& e, int64_t row, int
             for (int i = 0; i < 4; i++) x.pre[i] = 8 * i < nv ? p[i] : make_uint4(0, 0, 0, 0);
         }
     }
-    if (KIND != PJ_PLAIN && e.add && !e.out_f32) {
-        const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(e.add) + at);
+}
+__device__ __forceinline__ const uint4* proj_add16(const ProjEpi& e, int64_t row, int col, int N) {
+    return reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(e.add) + row * N + col);
+}
+// A warp's inputs of the 32 rows row0 .. by 32 columns col ..: the pre-activation
+// and its exponent by row (lane); the bias by column (lane), broadcast from there
+// when it is added; and the residual as the rows (lane / 4) + 8 i, piece lane % 4 of
+// 16 bytes, so that an instruction covers 8 rows' 64 bytes (a row per lane takes
+// 4 times as many wavefronts from the port that also feeds the tensor core: 16384 x
+// 8192 over 2048 with a residual 493 us, without 391).
+template <int KIND>
+__device__ __forceinline__ void proj_load_aux(const ProjEpi& e, int row0, int col, int nv, int M, int N, int lane,
+                                              ProjAux& x) {
+    if constexpr (KIND == PJ_PLAIN) return;
+    if (row0 + lane < M) proj_load_pre<KIND>(e, row0 + lane, col, nv, N, x);
+    if (KIND != PJ_GRAD && e.bias) x.bias = lane < nv ? load_param(e.bias, e.bias_dtype, col + lane) : 0.f;
+    if (e.add && !e.out_f32) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) x.add[i] = 8 * i < nv ? p[i] : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < 4; i++) {
+            const int r = row0 + lane / 4 + 8 * i;
+            x.add[i] = r < M && 8 * (lane % 4) < nv ? __ldcs(proj_add16(e, r, col, N) + lane % 4) : make_uint4(0, 0, 0, 0);
+        }
     }
 }
 __device__ __forceinline__ void floats8_16(const uint4& r, int bf16, float* v) {
@@ -183,42 +200,32 @@ __device__ __forceinline__ void floats8_16(const uint4& r, int bf16, float* v) {
     }
 }
 
-// The epilogue of columns col .. col + 31 of one row, of which the first nv (a
-// multiple of 8) exist; v holds the sums, 0 in columns that do not exist.
-// Returns the exponent byte of the checkpoint group, which the caller stores.
+// The epilogue of columns col .. col + 31 of one row up to the residual; the first
+// nv (a multiple of 8) columns exist; v holds the sums, 0 in columns that do not
+// exist, with the bias added.  PJ_FWD_CK: the codes go to w and the exponent byte
+// is returned, for the caller to store.
 template <int KIND>
 __device__ __forceinline__ uint32_t proj_epilogue32(float* v, const ProjEpi& e, const ProjAux& x, int64_t row, int col,
-                                                    int nv, int N) {
-    if constexpr (KIND == PJ_PLAIN) return 0;
-    const int64_t at = row * N + col;
+                                                    int nv, int N, uint4* w) {
     uint32_t exp = 0;
-    if (KIND != PJ_GRAD && e.bias) {
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (8 * i < nv) {
-                float b[8];
-                load_params<8>(e.bias, e.bias_dtype, col + 8 * i, b);
-#pragma unroll
-                for (int k = 0; k < 8; k++) v[8 * i + k] += b[k];
-            }
-    }
     if constexpr (KIND == PJ_FWD_CK) {
         uint32_t top = 0;
 #pragma unroll
         for (int i = 0; i < 32; i++) top = max(top, abs_bits(v[i]));
         exp = ck_exponent(top);
         const float inv = ck_inv_scale(exp);
-        uint32_t w[8];
+        uint32_t c[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) w[i] = ck_pack4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], inv);
-        const uint4 q[2] = {make_uint4(w[0], w[1], w[2], w[3]), make_uint4(w[4], w[5], w[6], w[7])};
-        proj_store_codes(e.codes + at, nv, q);
+        for (int i = 0; i < 8; i++) c[i] = ck_pack4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], inv);
+        w[0] = make_uint4(c[0], c[1], c[2], c[3]);
+        w[1] = make_uint4(c[4], c[5], c[6], c[7]);
     }
-    if (KIND != PJ_GRAD && e.z) {
+    if ((KIND == PJ_FWD || KIND == PJ_FWD_CK) && e.z) {
 #pragma unroll
         for (int i = 0; i < 4; i++)
             if (8 * i < nv)
-                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(e.z) + at + 8 * i) = pack8_16(v + 8 * i, e.bf16);
+                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(e.z) + row * N + col + 8 * i) =
+                    pack8_16(v + 8 * i, e.bf16);
     }
     if constexpr (KIND == PJ_GRAD) {
         const float s = e.pre_codes ? ck_scale(x.exp) : 0.f;
@@ -237,30 +244,24 @@ __device__ __forceinline__ uint32_t proj_epilogue32(float* v, const ProjEpi& e, 
                 for (int k = 0; k < 8; k++) v[8 * i + k] *= act_grad_t<ACT, true>(p[k]);
             }
         });
-    } else if (e.act != RWKV_ACT_NONE) {
-        with_act(e.act, [&]<int ACT>() {
+    } else if constexpr (KIND != PJ_PLAIN) {
+        if (e.act != RWKV_ACT_NONE)
+            with_act(e.act, [&]<int ACT>() {
 #pragma unroll
-            for (int i = 0; i < 32; i++) v[i] = act_t<ACT, true>(v[i]);
-        });
-    }
-    if (e.add) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            float a[8];
-            if (e.out_f32) {
-                if (8 * i >= nv) break;
-                const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(e.add) + at + 8 * i);
-                const float4 lo = p[0], hi = p[1];
-                a[0] = lo.x, a[1] = lo.y, a[2] = lo.z, a[3] = lo.w;
-                a[4] = hi.x, a[5] = hi.y, a[6] = hi.z, a[7] = hi.w;
-            } else {
-                floats8_16(x.add[i], e.bf16, a);
-            }
-#pragma unroll
-            for (int k = 0; k < 8; k++) v[8 * i + k] += a[k];
-        }
+                for (int i = 0; i < 32; i++) v[i] = act_t<ACT, true>(v[i]);
+            });
     }
     return exp;
+}
+// fp32 residual, read where it is added (a residual stream kept in fp32)
+__device__ __forceinline__ void proj_add_f32(float* v, const ProjEpi& e, int64_t at, int nv) {
+    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(e.add) + at);
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        if (4 * i < nv) {
+            const float4 f = p[i];
+            v[4 * i] += f.x, v[4 * i + 1] += f.y, v[4 * i + 2] += f.z, v[4 * i + 3] += f.w;
+        }
 }
 
 namespace tc {
@@ -269,6 +270,12 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t sr
                  "r"(c0), "r"(c1)
                  : "memory");
 }
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
+    uint4 r;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(addr));
+    return r;
+}
+__device__ __forceinline__ void st_shared_u4(uint32_t addr, const uint4& v) { st_shared_v4(addr, v.x, v.y, v.z, v.w); }
 __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 // at most N of this thread's bulk stores still read their shared memory
 template <int N>
@@ -446,13 +453,13 @@ __global__ void __launch_bounds__(PjCfg<BN>::THREADS, 1) proj_kernel(const __gri
         int nst = 0;  // stores issued by this warp
         for (int i = 0; i < tiles; i++) {
             const Tile t = tile_at(i);
-            const int b = i & 1, row = t.m0 + 32 * q + lane;
+            const int b = i & 1, row0 = t.m0 + 32 * q, row = row0 + lane;
             const bool part = t.part >= 0, wide = part || a.e.out_f32;  // 4-byte results
-            const bool live = !part && row < a.M;
+            const bool epi = KIND != PJ_PLAIN && !part, add16 = epi && a.e.add && !a.e.out_f32;
             // this warp's columns c0 .. c1 of the tile that exist, in whole steps of 32
-            const int c1 = t.m0 + 32 * q >= a.M ? c0 : min(c0 + C::EC, a.N - t.n0);
+            const int c1 = row0 >= a.M ? c0 : min(c0 + C::EC, a.N - t.n0);
             ProjAux aux;
-            if (live && c0 < c1) proj_load_aux<KIND>(a.e, row, t.n0 + c0, min(32, a.N - t.n0 - c0), a.N, aux);
+            if (epi && c0 < c1) proj_load_aux<KIND>(a.e, row0, t.n0 + c0, min(32, a.N - t.n0 - c0), a.M, a.N, lane, aux);
             if (!tc::mbar_wait(accf + b, (i >> 1) & 1, err)) {
                 ok = false;
                 break;
@@ -460,44 +467,78 @@ __global__ void __launch_bounds__(PjCfg<BN>::THREADS, 1) proj_kernel(const __gri
             tc::tc_after();
             uint32_t exps = 0;
             for (int c = c0; c < c1; c += 32) {
-                const int col = t.n0 + c;
+                const int col = t.n0 + c, nv = min(32, a.N - col);
                 uint32_t r[32];
                 tc::tmem_ld32_async(tmem + lane_base + b * BN + c, r);
-                tc::tmem_ld_wait();
-                float v[32];
-#pragma unroll
-                for (int k = 0; k < 32; k++) v[k] = __uint_as_float(r[k]);
-                if (live) {
-                    const ProjAux now = aux;
-                    if (c + 32 < c1) proj_load_aux<KIND>(a.e, row, col + 32, min(32, a.N - col - 32), a.N, aux);
-                    exps |= proj_epilogue32<KIND>(v, a.e, now, row, col, min(32, a.N - col), a.N) << ((c - c0) / 4);
+                ProjAux now;
+                if (epi) {
+                    now = aux;
+                    if (c + 32 < c1)
+                        proj_load_aux<KIND>(a.e, row0, col + 32, min(32, a.N - col - 32), a.M, a.N, lane, aux);
                 }
                 // the staging tile is free once the store that read it last is done
                 if (lane == 0) {
-                    if (wide) tc::bulk_wait_read<0>();
+                    if (wide || KIND == PJ_FWD_CK) tc::bulk_wait_read<0>();
                     else tc::bulk_wait_read<1>();
                 }
                 __syncwarp();
                 uint32_t base = stage;
+                if (!wide && KIND != PJ_FWD_CK) base += (nst & 1) * 2048;
+                // 16 bits: 64-byte rows, chunks swizzled by row / 2 (mod 4)
+                auto slot = [&](int rr, int k) { return base + rr * 64 + ((k ^ ((rr >> 1) & 3)) << 4); };
+                if (add16) {
+#pragma unroll
+                    for (int k = 0; k < 4; k++) tc::st_shared_u4(slot(lane / 4 + 8 * k, lane % 4), now.add[k]);
+                    __syncwarp();
+                }
+                tc::tmem_ld_wait();
+                float v[32];
+#pragma unroll
+                for (int k = 0; k < 32; k++) v[k] = __uint_as_float(r[k]);
+                uint4 codes[2];
+                if (epi) {
+                    if (KIND != PJ_GRAD && a.e.bias) {
+#pragma unroll
+                        for (int k = 0; k < 32; k++) v[k] += __shfl_sync(0xffffffffu, now.bias, k);
+                    }
+                    if (row < a.M) {
+                        exps |= proj_epilogue32<KIND>(v, a.e, now, row, col, nv, a.N, codes) << ((c - c0) / 4);
+                        if (a.e.add && a.e.out_f32) proj_add_f32(v, a.e, (int64_t)row * a.N + col, nv);
+                    }
+                }
                 if (wide) {  // 128-byte rows, 16-byte chunks swizzled by the row (mod 8)
 #pragma unroll
                     for (int k = 0; k < 8; k++)
                         tc::st_shared_v4(base + lane * 128 + ((k ^ (lane & 7)) << 4), __float_as_uint(v[4 * k]),
                                          __float_as_uint(v[4 * k + 1]), __float_as_uint(v[4 * k + 2]),
                                          __float_as_uint(v[4 * k + 3]));
-                } else {     // 64-byte rows, chunks swizzled by row / 2 (mod 4)
-                    base += (nst & 1) * 2048;
+                } else {
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
-                        const uint4 p = pack8_16(v + 8 * k, a.e.bf16);
-                        tc::st_shared_v4(base + lane * 64 + ((k ^ ((lane >> 1) & 3)) << 4), p.x, p.y, p.z, p.w);
+                        if (add16) {
+                            float f[8];
+                            floats8_16(tc::ld_shared_v4(slot(lane, k)), a.e.bf16, f);
+#pragma unroll
+                            for (int j = 0; j < 8; j++) v[8 * k + j] += f[j];
+                        }
+                        tc::st_shared_u4(slot(lane, k), pack8_16(v + 8 * k, a.e.bf16));
+                    }
+                }
+                if constexpr (KIND == PJ_FWD_CK) {
+                    // codes: 32-byte rows behind a 16-bit tile, or straight to memory
+                    if (epi && a.ctma && !wide) {
+                        tc::st_shared_u4(base + 2048 + lane * 32, codes[0]);
+                        tc::st_shared_u4(base + 2048 + lane * 32 + 16, codes[1]);
+                    } else if (epi && row < a.M) {
+                        proj_store_codes(a.e.codes + (int64_t)row * a.N + col, nv, codes);
                     }
                 }
                 tc::fence_async_smem();
                 __syncwarp();
                 if (lane == 0) {
                     if (part) tc::tma_store_2d(&a.pmap, base, c, t.part + 32 * q);
-                    else tc::tma_store_2d(&a.dmap, base, col, t.m0 + 32 * q);
+                    else tc::tma_store_2d(&a.dmap, base, col, row0);
+                    if (KIND == PJ_FWD_CK && epi && a.ctma && !wide) tc::tma_store_2d(&a.cmap, base + 2048, col, row0);
                     tc::bulk_commit();
                 }
                 nst++;
@@ -505,7 +546,7 @@ __global__ void __launch_bounds__(PjCfg<BN>::THREADS, 1) proj_kernel(const __gri
             tc::tc_before();
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(acce + b);
-            if (KIND == PJ_FWD_CK && live && c0 < c1) {
+            if (KIND == PJ_FWD_CK && epi && row < a.M && c0 < c1) {
                 // the exponents of this warp's groups, together where they are a word
                 uint8_t* p = a.e.exps + proj_group(row, t.n0 + c0, a.N);
                 const int n = (c1 - c0 + 31) / 32;
@@ -551,7 +592,7 @@ __device__ __forceinline__ void proj_join(const ProjJoin& a, int64_t i) {
     if (row >= a.M || col >= a.N) return;
     const int nv = min(32, a.N - col);
     ProjAux x;
-    proj_load_aux<KIND>(a.e, row, col, nv, a.N, x);
+    proj_load_pre<KIND>(a.e, row, col, nv, a.N, x);
     float v[32];
 #pragma unroll
     for (int k = 0; k < 32; k++) v[k] = 0.f;
@@ -563,9 +604,37 @@ __device__ __forceinline__ void proj_join(const ProjJoin& a, int64_t i) {
             v[4 * k] += f.x, v[4 * k + 1] += f.y, v[4 * k + 2] += f.z, v[4 * k + 3] += f.w;
         }
     }
-    const uint32_t exp = proj_epilogue32<KIND>(v, a.e, x, row, col, nv, a.N);
-    if (KIND == PJ_FWD_CK) a.e.exps[proj_group(row, col, a.N)] = (uint8_t)exp;
     const int64_t at = row * a.N + col;
+    if ((KIND == PJ_FWD || KIND == PJ_FWD_CK) && a.e.bias) {
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (8 * k < nv) {
+                float b[8];
+                load_params<8>(a.e.bias, a.e.bias_dtype, col + 8 * k, b);
+#pragma unroll
+                for (int m = 0; m < 8; m++) v[8 * k + m] += b[m];
+            }
+    }
+    uint4 codes[2];
+    const uint32_t exp = proj_epilogue32<KIND>(v, a.e, x, row, col, nv, a.N, codes);
+    if constexpr (KIND == PJ_FWD_CK) {
+        proj_store_codes(a.e.codes + at, nv, codes);
+        a.e.exps[proj_group(row, col, a.N)] = (uint8_t)exp;
+    }
+    if (KIND != PJ_PLAIN && a.e.add) {
+        if (a.e.out_f32) {
+            proj_add_f32(v, a.e, at, nv);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (8 * k < nv) {
+                    float f[8];
+                    floats8_16(proj_add16(a.e, row, col, a.N)[k], a.e.bf16, f);
+#pragma unroll
+                    for (int m = 0; m < 8; m++) v[8 * k + m] += f[m];
+                }
+        }
+    }
 #pragma unroll
     for (int k = 0; k < 4; k++)
         if (8 * k < nv) {
@@ -692,6 +761,9 @@ inline cudaError_t proj_gemm(const void* A, const void* B, void* D, int64_t M, i
                     : proj_map_2d(&a.bmap, t16, 2, B, K, N, PJ_BK, p.BN, sw128));
     ok = ok && (e.out_f32 ? proj_map_2d(&a.dmap, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, D, N, M, 32, 32, sw128)
                           : proj_map_2d(&a.dmap, t16, 2, D, N, M, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B));
+    a.ctma = KIND == PJ_FWD_CK && N % 16 == 0;
+    if (a.ctma)
+        ok = ok && proj_map_2d(&a.cmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, e.codes, N, M, 32, 32, CU_TENSOR_MAP_SWIZZLE_NONE);
     if (p.S > 1)
         ok = ok && proj_map_2d(&a.pmap, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, ws, p.BN, (int64_t)rem * p.S * 128, 32, 32,
                                sw128);
