@@ -25,7 +25,6 @@ backward calls.
 """
 from __future__ import annotations
 
-import math
 from dataclasses import dataclass
 
 import torch
@@ -61,6 +60,10 @@ class Checkpoint8:
 
 
 # ---------------------------------------------------------------- plumbing
+#
+# A small call costs about as much on the host as on the device, so the functions
+# below test what a correct call satisfies in one expression (_fits) and leave the
+# finding of what is wrong, or the copying of what is strided, to _tensor.
 
 # what torch.cuda.current_device() and current_stream(...).cuda_stream return,
 # without building a Stream object (2 us of a small call's 10)
@@ -81,6 +84,13 @@ def _call(dev, name, *args):
         raise _lib.RWKVError(name, st, L.rwkv_last_error().decode())
 
 
+def _fits(t, dev, dtype, shape):
+    return (type(t) in _TENSORS and t.dtype is dtype and t.shape == shape and t.device == dev and t.is_contiguous())
+
+
+_TENSORS = (torch.Tensor, torch.nn.Parameter)
+
+
 def _p(t):
     return None if t is None else t.data_ptr()
 
@@ -98,7 +108,9 @@ def _tensor(name, t, dev=None, dtypes=None, shape=None):
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _some(name, t):
+def _some(name, t, dtypes=None):
+    """A call's first tensor [..., D], D >= 1, after its checks."""
+    t = _tensor(name, t, None, dtypes)
     if t.dim() < 1 or t.shape[-1] < 1:
         raise ValueError(f"{name} {tuple(t.shape)} must be [..., D] with D >= 1")
     return t
@@ -109,10 +121,6 @@ def _aligned(t):
     return t if t is None or t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
-def _rows(shape):
-    return math.prod(shape[:-1])
-
-
 def _act(act):
     if act not in ACTS:
         raise ValueError(f"activation {act!r}: one of {sorted(ACTS)}")
@@ -121,11 +129,17 @@ def _act(act):
 
 def _activation(name, x, dev, dtype, shape):
     """An activation given as a tensor or as its checkpoint: (x, codes, exps)."""
-    if isinstance(x, Checkpoint8):
+    if type(x) is Checkpoint8 or isinstance(x, Checkpoint8):
         groups = shape[:-1] + (-(-shape[-1] // CKPT_GROUP),)
-        return (None, _tensor(f"{name}.codes", x.codes, dev, (torch.int8,), shape),
-                _tensor(f"{name}.exps", x.exps, dev, (torch.uint8,), torch.Size(groups)))
-    return _tensor(name, x, dev, (dtype,), shape), None, None
+        codes, exps = x.codes, x.exps
+        if not _fits(codes, dev, torch.int8, shape):
+            codes = _tensor(f"{name}.codes", codes, dev, (torch.int8,), shape)
+        if not _fits(exps, dev, torch.uint8, groups):
+            exps = _tensor(f"{name}.exps", exps, dev, (torch.uint8,), groups)
+        return None, codes, exps
+    if not _fits(x, dev, dtype, shape):
+        x = _tensor(name, x, dev, (dtype,), shape)
+    return x, None, None
 
 
 def _new_checkpoint(shape, like):
@@ -141,12 +155,11 @@ def _workspace(nbytes, like):
 
 def checkpoint8(x) -> Checkpoint8:
     """The 8-bit checkpoint of x [..., D]."""
-    x = _some("x", _tensor("x", x))
+    x = _some("x", x)
     ck = _new_checkpoint(x.shape, x)
-    rows = _rows(x.shape)
-    if rows:
-        _call(x.device, "rwkv_ckpt8_pack", _DT[x.dtype], x.data_ptr(), ck.codes.data_ptr(), ck.exps.data_ptr(), rows,
-              x.shape[-1])
+    n, D = x.numel(), x.shape[-1]
+    if n:
+        _call(x.device, "rwkv_ckpt8_pack", _DT[x.dtype], x.data_ptr(), ck.codes.data_ptr(), ck.exps.data_ptr(), n // D, D)
     return ck
 
 
@@ -156,25 +169,27 @@ def checkpoint8Values(ck: Checkpoint8, act: str = "none", dtype=None):
     a, dtype = _act(act), dtype or ck.dtype
     if dtype not in _DT:
         raise ValueError(f"checkpoint8Values: dtype {dtype} not taken")
-    _, codes, exps = _activation("ck", ck, ck.codes.device, None, ck.codes.shape)
-    out = codes.new_empty(codes.shape, dtype=dtype)
-    rows = _rows(codes.shape)
-    if rows:
-        _call(codes.device, "rwkv_ckpt8_values", codes.data_ptr(), exps.data_ptr(), a, _DT[dtype], out.data_ptr(), rows,
-              codes.shape[-1])
+    codes = ck.codes
+    dev, shape = codes.device, codes.shape
+    _, codes, exps = _activation("ck", ck, dev, None, shape)
+    out = torch.empty_like(codes, dtype=dtype)
+    n, D = codes.numel(), shape[-1]
+    if n:
+        _call(dev, "rwkv_ckpt8_values", codes.data_ptr(), exps.data_ptr(), a, _DT[dtype], out.data_ptr(), n // D, D)
     return out
 
 
 def activationBackward(dy, pre, act: str):
     """dy * act'(pre) in dy's dtype; `pre` is a tensor or a Checkpoint8."""
     a = _act(act)
-    dy = _some("dy", _tensor("dy", dy))
-    z, codes, exps = _activation("pre", pre, dy.device, dy.dtype, dy.shape)
+    dy = _some("dy", dy)
+    dev, shape = dy.device, dy.shape
+    z, codes, exps = _activation("pre", pre, dev, dy.dtype, shape)
     dz = torch.empty_like(dy)
-    rows = _rows(dy.shape)
-    if rows:
-        _call(dy.device, "rwkv_act_backward", _DT[dy.dtype], dy.data_ptr(), _p(z), _p(codes), _p(exps), a, dz.data_ptr(),
-              rows, dy.shape[-1])
+    n, D = dy.numel(), shape[-1]
+    if n:
+        _call(dev, "rwkv_act_backward", _DT[dy.dtype], dy.data_ptr(), _p(z), _p(codes), _p(exps), a, dz.data_ptr(),
+              n // D, D)
     return dz
 
 
@@ -184,19 +199,24 @@ def layerNormForward(x, weight, bias, eps: float = 1e-5, checkpoint: bool = Fals
     """Layer norm over the last dimension: (y, mean, rstd, ck).  mean / rstd
     [...] fp32 are what the backward pass needs; ck is the 8-bit checkpoint of x
     (None without `checkpoint`)."""
-    x = _some("x", _tensor("x", x))
-    dev, D = x.device, x.shape[-1]
-    weight = _tensor("weight", weight, dev, None, (D,))
-    bias = _tensor("bias", bias, dev, (weight.dtype,), (D,))
+    x = _some("x", x)
+    dev, shape = x.device, x.shape
+    D = shape[-1]
+    if not _fits(weight, dev, torch.float32, (D,)):
+        weight = _tensor("weight", weight, dev, None, (D,))
+    if not _fits(bias, dev, weight.dtype, (D,)):
+        bias = _tensor("bias", bias, dev, (weight.dtype,), (D,))
     y = torch.empty_like(x)
-    mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    mean = x.new_empty(shape[:-1], dtype=torch.float32)
     rstd = torch.empty_like(mean)
-    ck = _new_checkpoint(x.shape, x) if checkpoint else None
-    rows = x.numel() // D
-    if rows:
+    codes = exps = ck = None
+    if checkpoint:
+        ck = _new_checkpoint(shape, x)
+        codes, exps = ck.codes.data_ptr(), ck.exps.data_ptr()
+    n = x.numel()
+    if n:
         _call(dev, "rwkv_layer_norm_forward", _DT[x.dtype], x.data_ptr(), _DT[weight.dtype], weight.data_ptr(),
-              bias.data_ptr(), eps, y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), ck and ck.codes.data_ptr(),
-              ck and ck.exps.data_ptr(), rows, D)
+              bias.data_ptr(), eps, y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), codes, exps, n // D, D)
     return y, mean, rstd, ck
 
 
@@ -205,23 +225,28 @@ def layerNormBackward(dy, x, weight, mean, rstd, dres=None, params: bool = True)
     checkpoint of it; mean, rstd: its statistics; dres: the gradient that
     reaches x past the norm, added to dx.  Without `params` dweight and dbias
     are None."""
-    dy = _some("dy", _tensor("dy", dy))
-    dev, D = dy.device, dy.shape[-1]
-    xt, codes, exps = _activation("x", x, dev, dy.dtype, dy.shape)
-    weight = _tensor("weight", weight, dev, None, (D,))
-    mean = _tensor("mean", mean, dev, (torch.float32,), dy.shape[:-1])
-    rstd = _tensor("rstd", rstd, dev, (torch.float32,), dy.shape[:-1])
-    if dres is not None:
-        dres = _tensor("dres", dres, dev, (dy.dtype,), dy.shape)
+    dy = _some("dy", dy)
+    dev, dt, shape = dy.device, dy.dtype, dy.shape
+    D = shape[-1]
+    xt, codes, exps = _activation("x", x, dev, dt, shape)
+    if not _fits(weight, dev, torch.float32, (D,)):
+        weight = _tensor("weight", weight, dev, None, (D,))
+    lead = shape[:-1]
+    if not _fits(mean, dev, torch.float32, lead):
+        mean = _tensor("mean", mean, dev, (torch.float32,), lead)
+    if not _fits(rstd, dev, torch.float32, lead):
+        rstd = _tensor("rstd", rstd, dev, (torch.float32,), lead)
+    if dres is not None and not _fits(dres, dev, dt, shape):
+        dres = _tensor("dres", dres, dev, (dt,), shape)
     dx = torch.empty_like(dy)
-    rows = _rows(dy.shape)
+    rows = dy.numel() // D
     dw = torch.empty_like(weight) if params else None
     db = torch.empty_like(weight) if params else None
     if not rows:
         return dx, dw.zero_() if params else None, db.zero_() if params else None
     n = _lib.lib().rwkv_layer_norm_backward_workspace_size(rows, D) if params else 0
     ws = _workspace(n, dy)
-    _call(dev, "rwkv_layer_norm_backward", _DT[dy.dtype], dy.data_ptr(), _p(xt), _p(codes), _p(exps), _DT[weight.dtype],
+    _call(dev, "rwkv_layer_norm_backward", _DT[dt], dy.data_ptr(), _p(xt), _p(codes), _p(exps), _DT[weight.dtype],
           weight.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _p(dres), dx.data_ptr(), _p(dw), _p(db), rows, D, _p(ws),
           n)
     return dx, dw, db
@@ -229,13 +254,21 @@ def layerNormBackward(dy, x, weight, mean, rstd, dres=None, params: bool = True)
 
 # -------------------------------------------------------------- projections
 
-def _weight(w, dev=None, dtype=None):
-    w = _tensor("w", w, dev, _HALF if dtype is None else (dtype,))
+def _weight(w, dev, dtype):
+    w = _tensor("w", w, dev, (dtype,))
     if w.dim() != 2:
         raise ValueError(f"w {tuple(w.shape)} must be [OUT, IN]")
     if w.shape[0] % 8 or w.shape[1] % 8 or not w.numel():
         raise ValueError(f"w {tuple(w.shape)}: OUT and IN must be multiples of 8")
     return _aligned(w)
+
+
+def _result_dtype(fn, dtype, own):
+    if dtype is None or dtype is own:
+        return own
+    if dtype is not torch.float32:
+        raise ValueError(f"{fn}: out_dtype {dtype} ({own} or fp32)")
+    return dtype
 
 
 def projectionForward(x, w, bias=None, act: str = "none", residual=None, checkpoint: bool = False,
@@ -245,33 +278,39 @@ def projectionForward(x, w, bias=None, act: str = "none", residual=None, checkpo
     kept is the 8-bit checkpoint of z = x w^T + bias with `checkpoint`, z itself
     with `preactivation`, else None."""
     a = _act(act)
-    x = _aligned(_tensor("x", x, None, _HALF))
-    dev = x.device
-    w = _weight(w, dev, x.dtype)
+    x = _aligned(_some("x", x, _HALF))
+    dev, dt = x.device, x.dtype
+    w = _weight(w, dev, dt)
     OUT, IN = w.shape
-    if x.dim() < 1 or x.shape[-1] != IN:
+    if x.shape[-1] != IN:
         raise ValueError(f"x {tuple(x.shape)} must be [..., {IN}]")
     if checkpoint and preactivation:
         raise ValueError("projectionForward: keep either the checkpoint or the pre-activation")
-    ydt = out_dtype or x.dtype
-    if ydt != x.dtype and ydt != torch.float32:
-        raise ValueError(f"projectionForward: out_dtype {ydt} (x's own type or fp32)")
+    ydt = _result_dtype("projectionForward", out_dtype, dt)
     shape = x.shape[:-1] + (OUT,)
+    bdt = F32
     if bias is not None:
         bias = _aligned(_tensor("bias", bias, dev, None, (OUT,)))
+        bdt = _DT[bias.dtype]
     if residual is not None:
-        residual = _aligned(_tensor("residual", residual, dev, (ydt,), shape))
+        if not _fits(residual, dev, ydt, shape):
+            residual = _tensor("residual", residual, dev, (ydt,), shape)
+        residual = _aligned(residual)
     y = x.new_empty(shape, dtype=ydt)
-    ck = _new_checkpoint(shape, x) if checkpoint else None
-    z = x.new_empty(shape) if preactivation else None
-    rows = _rows(shape)
+    codes = exps = kept = z = None
+    if checkpoint:
+        kept = _new_checkpoint(shape, x)
+        codes, exps = kept.codes.data_ptr(), kept.exps.data_ptr()
+    elif preactivation:
+        kept = x.new_empty(shape)
+        z = kept.data_ptr()
+    rows = x.numel() // IN
     if rows:
         n = _lib.lib().rwkv_projection_forward_workspace_size(rows, OUT, IN)
         ws = _workspace(n, x)
-        _call(dev, "rwkv_projection_forward", _DT[x.dtype], x.data_ptr(), w.data_ptr(),
-              F32 if bias is None else _DT[bias.dtype], _p(bias), a, _DT[ydt], _p(residual), y.data_ptr(), _p(z),
-              ck and ck.codes.data_ptr(), ck and ck.exps.data_ptr(), rows, OUT, IN, _p(ws), n)
-    return y, ck if checkpoint else z
+        _call(dev, "rwkv_projection_forward", _DT[dt], x.data_ptr(), w.data_ptr(), bdt, _p(bias), a, _DT[ydt],
+              _p(residual), y.data_ptr(), z, codes, exps, rows, OUT, IN, _p(ws), n)
+    return y, kept
 
 
 def projectionBackwardInput(dy, w, pre=None, act: str = "none", addend=None, out_dtype=None):
@@ -279,31 +318,31 @@ def projectionBackwardInput(dy, w, pre=None, act: str = "none", addend=None, out
     pre [..., IN]: the pre-activation of the layer below, a tensor or a
     Checkpoint8 (None: the plain product); addend in dx's type."""
     a = _act(act)
-    dy = _aligned(_tensor("dy", dy, None, _HALF))
-    dev = dy.device
-    w = _weight(w, dev, dy.dtype)
+    dy = _aligned(_some("dy", dy, _HALF))
+    dev, dt = dy.device, dy.dtype
+    w = _weight(w, dev, dt)
     OUT, IN = w.shape
-    if dy.dim() < 1 or dy.shape[-1] != OUT:
+    if dy.shape[-1] != OUT:
         raise ValueError(f"dy {tuple(dy.shape)} must be [..., {OUT}]")
-    xdt = out_dtype or dy.dtype
-    if xdt != dy.dtype and xdt != torch.float32:
-        raise ValueError(f"projectionBackwardInput: out_dtype {xdt} (dy's own type or fp32)")
-    shape = torch.Size(dy.shape[:-1] + (IN,))
+    xdt = _result_dtype("projectionBackwardInput", out_dtype, dt)
+    shape = dy.shape[:-1] + (IN,)
     z = codes = exps = None
     if pre is not None:
-        z, codes, exps = _activation("pre", pre, dev, dy.dtype, shape)
+        z, codes, exps = _activation("pre", pre, dev, dt, shape)
         z, codes = _aligned(z), _aligned(codes)
-    elif act != "none":
+    elif a:
         raise ValueError(f"projectionBackwardInput: act {act!r} needs pre")
     if addend is not None:
-        addend = _aligned(_tensor("addend", addend, dev, (xdt,), shape))
+        if not _fits(addend, dev, xdt, shape):
+            addend = _tensor("addend", addend, dev, (xdt,), shape)
+        addend = _aligned(addend)
     dx = dy.new_empty(shape, dtype=xdt)
-    rows = _rows(shape)
+    rows = dy.numel() // OUT
     if rows:
         n = _lib.lib().rwkv_projection_dx_workspace_size(rows, OUT, IN)
         ws = _workspace(n, dy)
-        _call(dev, "rwkv_projection_dx", _DT[dy.dtype], dy.data_ptr(), w.data_ptr(), a, _p(z), _p(codes), _p(exps),
-              _DT[xdt], _p(addend), dx.data_ptr(), rows, OUT, IN, _p(ws), n)
+        _call(dev, "rwkv_projection_dx", _DT[dt], dy.data_ptr(), w.data_ptr(), a, _p(z), _p(codes), _p(exps), _DT[xdt],
+              _p(addend), dx.data_ptr(), rows, OUT, IN, _p(ws), n)
     return dx
 
 
@@ -314,8 +353,8 @@ def projectionBackwardWeight(dy, x, act: str = "none", bias: bool = False, out_d
     pre-activation behind it; a tensor or a Checkpoint8; None: only db (dw is
     None)."""
     a = _act(act)
-    dy = _aligned(_some("dy", _tensor("dy", dy, None, _HALF)))
-    dev = dy.device
+    dy = _aligned(_some("dy", dy, _HALF))
+    dev, dt = dy.device, dy.dtype
     if x is None:
         if not bias or a:
             raise ValueError("projectionBackwardWeight: without x only db can be asked for")
@@ -324,22 +363,20 @@ def projectionBackwardWeight(dy, x, act: str = "none", bias: bool = False, out_d
     OUT, IN = dy.shape[-1], 8 if x is None else x.shape[-1]
     if OUT % 8 or IN % 8 or not IN:
         raise ValueError(f"projectionBackwardWeight: OUT={OUT} and IN={IN} must be multiples of 8")
-    wdt = out_dtype or dy.dtype
-    if wdt != dy.dtype and wdt != torch.float32:
-        raise ValueError(f"projectionBackwardWeight: out_dtype {wdt} (dy's own type or fp32)")
+    wdt = _result_dtype("projectionBackwardWeight", out_dtype, dt)
     xt = codes = exps = dw = None
     if x is not None:
-        xt, codes, exps = _activation("x", x, dev, dy.dtype, torch.Size(dy.shape[:-1] + (IN,)))
+        xt, codes, exps = _activation("x", x, dev, dt, dy.shape[:-1] + (IN,))
         xt, codes = _aligned(xt), _aligned(codes)
         dw = dy.new_empty((OUT, IN), dtype=wdt)
-    db = dy.new_empty(OUT, dtype=torch.float32) if bias else None
-    rows = _rows(dy.shape)
+    db = dy.new_empty((OUT,), dtype=torch.float32) if bias else None
+    rows = dy.numel() // OUT
     if not rows:
         return dw if dw is None else dw.zero_(), db.zero_() if bias else None
     n = _lib.lib().rwkv_projection_dw_workspace_size(rows, OUT, IN, int(codes is not None or a != 0))
     ws = _workspace(n, dy)
-    _call(dev, "rwkv_projection_dw", _DT[dy.dtype], dy.data_ptr(), a, _p(xt), _p(codes), _p(exps), _DT[wdt],
-          _p(dw), _p(db), rows, OUT, IN, _p(ws), n)
+    _call(dev, "rwkv_projection_dw", _DT[dt], dy.data_ptr(), a, _p(xt), _p(codes), _p(exps), _DT[wdt], _p(dw), _p(db),
+          rows, OUT, IN, _p(ws), n)
     return dw, db
 
 
