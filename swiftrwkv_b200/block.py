@@ -130,7 +130,7 @@ def _act(act):
 def _activation(name, x, dev, dtype, shape):
     """An activation given as a tensor or as its checkpoint: (x, codes, exps)."""
     if type(x) is Checkpoint8 or isinstance(x, Checkpoint8):
-        groups = shape[:-1] + (-(-shape[-1] // CKPT_GROUP),)
+        groups = (*shape[:-1], -(-shape[-1] // CKPT_GROUP))
         codes, exps = x.codes, x.exps
         if not _fits(codes, dev, torch.int8, shape):
             codes = _tensor(f"{name}.codes", codes, dev, (torch.int8,), shape)
@@ -142,9 +142,11 @@ def _activation(name, x, dev, dtype, shape):
     return x, None, None
 
 
-def _new_checkpoint(shape, like):
-    return Checkpoint8(like.new_empty(shape, dtype=torch.int8),
-                       like.new_empty(shape[:-1] + (-(-shape[-1] // CKPT_GROUP),), dtype=torch.uint8), like.dtype)
+def _new_checkpoint(y, dtype):
+    """An empty checkpoint of a tensor like y."""
+    *lead, D = y.shape
+    return Checkpoint8(torch.empty_like(y, dtype=torch.int8),
+                       y.new_empty((*lead, -(-D // CKPT_GROUP)), dtype=torch.uint8), dtype)
 
 
 def _workspace(nbytes, like):
@@ -156,7 +158,7 @@ def _workspace(nbytes, like):
 def checkpoint8(x) -> Checkpoint8:
     """The 8-bit checkpoint of x [..., D]."""
     x = _some("x", x)
-    ck = _new_checkpoint(x.shape, x)
+    ck = _new_checkpoint(x, x.dtype)
     n, D = x.numel(), x.shape[-1]
     if n:
         _call(x.device, "rwkv_ckpt8_pack", _DT[x.dtype], x.data_ptr(), ck.codes.data_ptr(), ck.exps.data_ptr(), n // D, D)
@@ -207,11 +209,11 @@ def layerNormForward(x, weight, bias, eps: float = 1e-5, checkpoint: bool = Fals
     if not _fits(bias, dev, weight.dtype, (D,)):
         bias = _tensor("bias", bias, dev, (weight.dtype,), (D,))
     y = torch.empty_like(x)
-    mean = x.new_empty(shape[:-1], dtype=torch.float32)
+    mean = x.new_empty((*shape[:-1],), dtype=torch.float32)
     rstd = torch.empty_like(mean)
     codes = exps = ck = None
     if checkpoint:
-        ck = _new_checkpoint(shape, x)
+        ck = _new_checkpoint(x, x.dtype)
         codes, exps = ck.codes.data_ptr(), ck.exps.data_ptr()
     n = x.numel()
     if n:
@@ -287,7 +289,7 @@ def projectionForward(x, w, bias=None, act: str = "none", residual=None, checkpo
     if checkpoint and preactivation:
         raise ValueError("projectionForward: keep either the checkpoint or the pre-activation")
     ydt = _result_dtype("projectionForward", out_dtype, dt)
-    shape = x.shape[:-1] + (OUT,)
+    shape = (*x.shape[:-1], OUT)
     bdt = F32
     if bias is not None:
         bias = _aligned(_tensor("bias", bias, dev, None, (OUT,)))
@@ -299,7 +301,7 @@ def projectionForward(x, w, bias=None, act: str = "none", residual=None, checkpo
     y = x.new_empty(shape, dtype=ydt)
     codes = exps = kept = z = None
     if checkpoint:
-        kept = _new_checkpoint(shape, x)
+        kept = _new_checkpoint(y, dt)
         codes, exps = kept.codes.data_ptr(), kept.exps.data_ptr()
     elif preactivation:
         kept = x.new_empty(shape)
@@ -325,7 +327,7 @@ def projectionBackwardInput(dy, w, pre=None, act: str = "none", addend=None, out
     if dy.shape[-1] != OUT:
         raise ValueError(f"dy {tuple(dy.shape)} must be [..., {OUT}]")
     xdt = _result_dtype("projectionBackwardInput", out_dtype, dt)
-    shape = dy.shape[:-1] + (IN,)
+    shape = (*dy.shape[:-1], IN)
     z = codes = exps = None
     if pre is not None:
         z, codes, exps = _activation("pre", pre, dev, dt, shape)
@@ -366,7 +368,7 @@ def projectionBackwardWeight(dy, x, act: str = "none", bias: bool = False, out_d
     wdt = _result_dtype("projectionBackwardWeight", out_dtype, dt)
     xt = codes = exps = dw = None
     if x is not None:
-        xt, codes, exps = _activation("x", x, dev, dt, dy.shape[:-1] + (IN,))
+        xt, codes, exps = _activation("x", x, dev, dt, (*dy.shape[:-1], IN))
         xt, codes = _aligned(xt), _aligned(codes)
         dw = dy.new_empty((OUT, IN), dtype=wdt)
     db = dy.new_empty((OUT,), dtype=torch.float32) if bias else None
