@@ -20,13 +20,13 @@
 //   warp 0      TMA producer, ST stages
 //   warp 1      TMEM owner; one thread issues 4 tcgen05.mma (M=128, N=BN, K=16)
 //               per stage and commits the stage / the tile
-//   warps 2-9   epilogue: TMEM lane quadrant (warp & 3) = 32 rows of D, half of the
-//               columns per 4 warps, 32 columns at a time, the other inputs
-//               (residual, pre-activation) one step ahead.  A thread holds 32 consecutive
-//               columns of one row, exactly a checkpoint group, so a group's largest
-//               |z| needs no exchange.  Results go through a swizzled 32 x 32 tile in
-//               shared memory and leave by TMA store (full 64-byte row pieces, clipped
-//               at the tensor's end).
+//   warps 2 ..  epilogue, 16 warps (a sigmoid over 4093 x 2048 sums of 96 takes 21 us
+//               with 8): TMEM lane quadrant (warp & 3) = 32 rows of D, an equal share
+//               of the columns per 4 warps, 32 columns at a time in two halves.
+//               With a checkpoint 8 warps, a thread holding the 32 columns of a
+//               group, so that its largest |z| needs no exchange.  Results go
+//               through a swizzled 32 x 32 tile in shared memory and leave by TMA
+//               store (full 64-byte row pieces, clipped at the tensor's end).
 // Tiles are walked in groups of 8 row blocks, so that the CTAs at work at one
 // time share a few row blocks of A and a few of B in L2.
 //
@@ -49,7 +49,7 @@ namespace rwkv {
 constexpr int PJ_BK = 64;
 constexpr int PJ_GROUP_M = 8;      // row blocks walked together
 constexpr int PJ_SMS = 148;
-constexpr int PJ_STAGE_OUT = 4096;  // staging bytes per epilogue warp: 32 x 32 fp32, or two 32 x 32 of 16 bits
+constexpr int PJ_OUT_BYTES = 32 * 1024;  // output staging, shared by the epilogue warps
 
 // Which epilogue a kernel has, at compile time: one that can do everything keeps
 // the registers of everything alive (16384 x 8192 over 96 takes 270 us with a
@@ -84,9 +84,9 @@ struct ProjEpi {
 
 struct ProjArgs {
     CUtensorMap amap, bmap;
-    CUtensorMap dmap;   // D, box {32, 32}
+    CUtensorMap dmap;   // D, box {32, 32}, or {16, 32} in fp32
     CUtensorMap cmap;   // checkpoint codes, box {32, 32} (N % 16 == 0)
-    CUtensorMap pmap;   // the splits' tiles {BN, 128 units} fp32, box {32, 32}
+    CUtensorMap pmap;   // the splits' tiles {BN, 128 units} fp32, box {16, 32}
     ProjEpi e;
     int M, N, nk;       // D's size, K stages
     int mt, nt;         // tiles along M and N
@@ -138,49 +138,47 @@ __device__ __forceinline__ void proj_load_codes(const int8_t* p, int nv, uint4* 
         w[1] = make_uint4(c.x, c.y, d.x, d.y);
     }
 }
-__device__ __forceinline__ void proj_store_codes(int8_t* p, int nv, const uint4* w) {
+__device__ __forceinline__ void proj_store_codes(int8_t* p, int nv, const uint32_t* w) {
     uint2* q = reinterpret_cast<uint2*>(p);
-    if (nv > 0) q[0] = make_uint2(w[0].x, w[0].y);
-    if (nv > 8) q[1] = make_uint2(w[0].z, w[0].w);
-    if (nv > 16) q[2] = make_uint2(w[1].x, w[1].y);
-    if (nv > 24) q[3] = make_uint2(w[1].z, w[1].w);
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (8 * i < nv) q[i] = make_uint2(w[2 * i], w[2 * i + 1]);
 }
 
-// The other inputs of 32 columns of one row, as read.
+// A warp's other inputs of 32 rows by 32 columns, as read.
 struct ProjAux {
     uint4 add[4];  // residual / addend, 16 bits
-    uint4 pre[4];  // pre-activation, or its 32 codes in the first two
+    uint4 pre[4];  // pre-activation of row (lane), or its 32 codes in the first two
     uint32_t exp;  // and their exponent
     float bias;    // of column (lane)
 };
-template <int KIND>
-__device__ __forceinline__ void proj_load_pre(const ProjEpi& e, int64_t row, int col, int nv, int N, ProjAux& x) {
-    if constexpr (KIND == PJ_GRAD) {
-        const int64_t at = row * N + col;
-        if (e.pre_codes) {
-            proj_load_codes(e.pre_codes + at, nv, x.pre);
-            x.exp = e.pre_exps[proj_group(row, col, N)];
-        } else {
-            const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(e.pre) + at);
-#pragma unroll
-            for (int i = 0; i < 4; i++) x.pre[i] = 8 * i < nv ? p[i] : make_uint4(0, 0, 0, 0);
-        }
-    }
-}
 __device__ __forceinline__ const uint4* proj_add16(const ProjEpi& e, int64_t row, int col, int N) {
     return reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(e.add) + row * N + col);
 }
-// A warp's inputs of the 32 rows row0 .. by 32 columns col ..: the pre-activation
-// and its exponent by row (lane); the bias by column (lane), broadcast from there
-// when it is added; and the residual as the rows (lane / 4) + 8 i, piece lane % 4 of
-// 16 bytes, so that an instruction covers 8 rows' 64 bytes (a row per lane takes
-// 4 times as many wavefronts from the port that also feeds the tensor core: 16384 x
-// 8192 over 2048 with a residual 493 us, without 391).
+__device__ __forceinline__ const uint4* proj_pre16(const ProjEpi& e, int64_t row, int col, int N) {
+    return reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(e.pre) + row * N + col);
+}
+// The rows row0 .. by the columns col ..: the pre-activation and its exponent by
+// row; the bias by column, broadcast from there when it is added; and the residual
+// as the rows (lane / 4) + 8 i, piece lane % 4 of 16 bytes, so that an instruction
+// covers 8 rows' 64 bytes (a row per lane takes 4 times as many wavefronts from the
+// port that also feeds the tensor core: 16384 x 8192 over 2048 with a residual 493
+// us, this way 451, without 391).
 template <int KIND>
 __device__ __forceinline__ void proj_load_aux(const ProjEpi& e, int row0, int col, int nv, int M, int N, int lane,
                                               ProjAux& x) {
     if constexpr (KIND == PJ_PLAIN) return;
-    if (row0 + lane < M) proj_load_pre<KIND>(e, row0 + lane, col, nv, N, x);
+    const int64_t row = row0 + lane;
+    if (KIND == PJ_GRAD && row < M) {
+        if (e.pre_codes) {
+            proj_load_codes(e.pre_codes + row * N + col, nv, x.pre);
+            x.exp = e.pre_exps[proj_group(row, col, N)];
+        } else {
+            const uint4* p = proj_pre16(e, row, col, N);
+#pragma unroll
+            for (int i = 0; i < 4; i++) x.pre[i] = 8 * i < nv ? p[i] : make_uint4(0, 0, 0, 0);
+        }
+    }
     if (KIND != PJ_GRAD && e.bias) x.bias = lane < nv ? load_param(e.bias, e.bias_dtype, col + lane) : 0.f;
     if (e.add && !e.out_f32) {
 #pragma unroll
@@ -200,45 +198,48 @@ __device__ __forceinline__ void floats8_16(const uint4& r, int bf16, float* v) {
     }
 }
 
-// The epilogue of columns col .. col + 31 of one row up to the residual; the first
-// nv (a multiple of 8) columns exist; v holds the sums, 0 in columns that do not
-// exist, with the bias added.  PJ_FWD_CK: the codes go to w and the exponent byte
-// is returned, for the caller to store.
-template <int KIND>
-__device__ __forceinline__ uint32_t proj_epilogue32(float* v, const ProjEpi& e, const ProjAux& x, int64_t row, int col,
-                                                    int nv, int N, uint4* w) {
+// The epilogue of W columns col .. of one row up to the residual; the first nv (a
+// multiple of 8) columns exist; v holds the sums, 0 in columns that do not exist,
+// with the bias added; pre / exp as in ProjAux.  PJ_FWD_CK: the codes go to w and the
+// exponent byte is returned, for the caller to store; the group is the thread's own
+// 32 columns, or (W = 8) those of four neighbouring lanes.
+template <int KIND, int W>
+__device__ __forceinline__ uint32_t proj_epilogue(float* v, const ProjEpi& e, const uint4* pre, uint32_t pexp,
+                                                  int64_t row, int col, int nv, int N, uint32_t* w) {
     uint32_t exp = 0;
     if constexpr (KIND == PJ_FWD_CK) {
+        static_assert(W == 32 || W == 8, "whole groups");
         uint32_t top = 0;
 #pragma unroll
-        for (int i = 0; i < 32; i++) top = max(top, abs_bits(v[i]));
+        for (int i = 0; i < W; i++) top = max(top, abs_bits(v[i]));
+        if constexpr (W == 8) {
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        }
         exp = ck_exponent(top);
         const float inv = ck_inv_scale(exp);
-        uint32_t c[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) c[i] = ck_pack4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], inv);
-        w[0] = make_uint4(c[0], c[1], c[2], c[3]);
-        w[1] = make_uint4(c[4], c[5], c[6], c[7]);
+        for (int i = 0; i < W / 4; i++) w[i] = ck_pack4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3], inv);
     }
     if ((KIND == PJ_FWD || KIND == PJ_FWD_CK) && e.z) {
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int i = 0; i < W / 8; i++)
             if (8 * i < nv)
                 *reinterpret_cast<uint4*>(static_cast<uint16_t*>(e.z) + row * N + col + 8 * i) =
                     pack8_16(v + 8 * i, e.bf16);
     }
     if constexpr (KIND == PJ_GRAD) {
-        const float s = e.pre_codes ? ck_scale(x.exp) : 0.f;
+        const float s = e.pre_codes ? ck_scale(pexp) : 0.f;
         with_act(e.act, [&]<int ACT>() {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
+            for (int i = 0; i < W / 8; i++) {
                 float p[8];
                 if (e.pre_codes) {
-                    const uint4 c = x.pre[i / 2];
+                    const uint4 c = pre[i / 2];
                     ck_unpack4(i % 2 ? c.z : c.x, s, p);
                     ck_unpack4(i % 2 ? c.w : c.y, s, p + 4);
                 } else {
-                    floats8_16(x.pre[i], e.bf16, p);
+                    floats8_16(pre[i], e.bf16, p);
                 }
 #pragma unroll
                 for (int k = 0; k < 8; k++) v[8 * i + k] *= act_grad_t<ACT, true>(p[k]);
@@ -248,16 +249,17 @@ __device__ __forceinline__ uint32_t proj_epilogue32(float* v, const ProjEpi& e, 
         if (e.act != RWKV_ACT_NONE)
             with_act(e.act, [&]<int ACT>() {
 #pragma unroll
-                for (int i = 0; i < 32; i++) v[i] = act_t<ACT, true>(v[i]);
+                for (int i = 0; i < W; i++) v[i] = act_t<ACT, true>(v[i]);
             });
     }
     return exp;
 }
 // fp32 residual, read where it is added (a residual stream kept in fp32)
+template <int W>
 __device__ __forceinline__ void proj_add_f32(float* v, const ProjEpi& e, int64_t at, int nv) {
     const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(e.add) + at);
 #pragma unroll
-    for (int i = 0; i < 8; i++)
+    for (int i = 0; i < W / 4; i++)
         if (4 * i < nv) {
             const float4 f = p[i];
             v[4 * i] += f.x, v[4 * i + 1] += f.y, v[4 * i + 2] += f.z, v[4 * i + 3] += f.w;
@@ -265,6 +267,17 @@ __device__ __forceinline__ void proj_add_f32(float* v, const ProjEpi& e, int64_t
 }
 
 namespace tc {
+template <int W>
+__device__ __forceinline__ void tmem_ld_async(uint32_t taddr, uint32_t* r) {
+    if constexpr (W == 32)
+        tmem_ld32_async(taddr, r);
+    else
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+              "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+            : "r"(taddr));
+}
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int c0, int c1) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(src),
                  "r"(c0), "r"(c1)
@@ -284,19 +297,20 @@ template <int N>
 __device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_group %0;" ::"n"(N) : "memory"); }
 }  // namespace tc
 
-template <int BN>
+template <int BN, int KIND>
 struct PjCfg {
     static constexpr int A_BYTES = 128 * 128;       // 128 rows x 64 k, 16 bits
     static constexpr int B_BYTES = BN * 128;
     static constexpr int STAGE = A_BYTES + B_BYTES;
-    static constexpr int EW = 8;                    // epilogue warps
-    static constexpr int EC = BN / (EW / 4);        // columns of each
+    static constexpr int EW = KIND == PJ_FWD_CK ? 8 : 16;  // epilogue warps
+    static constexpr int W = KIND == PJ_FWD_CK ? 32 : 16;  // columns a thread holds
+    static constexpr int EC = BN / (EW / 4);               // columns of each warp
     static constexpr int THREADS = 64 + 32 * EW;
-    static constexpr int OUT_BYTES = EW * PJ_STAGE_OUT;
-    static constexpr int ST = (224 * 1024 - OUT_BYTES) / STAGE;
+    static constexpr int SLOT = PJ_OUT_BYTES / EW;         // staging bytes per warp
+    static constexpr int ST = 192 * 1024 / STAGE;
     static constexpr int NBAR = 2 * ST + 5;
     static constexpr int O_OFF = ST * STAGE;        // output staging
-    static constexpr int B_OFF = O_OFF + OUT_BYTES;
+    static constexpr int B_OFF = O_OFF + PJ_OUT_BYTES;
     static constexpr int T_OFF = B_OFF + NBAR * 8;
     static constexpr int TOTAL = T_OFF + 16 + 1024;
     static constexpr int TMC = 2 * BN;
@@ -307,8 +321,8 @@ struct PjCfg {
 
 // AMN / BMN: the operand is MN-major.
 template <int BN, bool AMN, bool BMN, int KIND>
-__global__ void __launch_bounds__(PjCfg<BN>::THREADS, 1) proj_kernel(const __grid_constant__ ProjArgs a) {
-    using C = PjCfg<BN>;
+__global__ void __launch_bounds__(PjCfg<BN, KIND>::THREADS, 1) proj_kernel(const __grid_constant__ ProjArgs a) {
+    using C = PjCfg<BN, KIND>;
     constexpr int ST = C::ST;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -449,8 +463,10 @@ __global__ void __launch_bounds__(PjCfg<BN>::THREADS, 1) proj_kernel(const __gri
         // ---- epilogue
         const int q = warp & 3, c0 = (warp - 2) / 4 * C::EC;
         const uint32_t lane_base = (uint32_t)(32 * q) << 16;
-        const uint32_t stage = tc::saddr(smem + C::O_OFF + (warp - 2) * PJ_STAGE_OUT);
-        int nst = 0;  // stores issued by this warp
+        const uint32_t base = tc::saddr(smem + C::O_OFF + (warp - 2) * C::SLOT);
+        constexpr int W = C::W;
+        // 64-byte rows (32 values of 16 bits, or 16 fp32), 16-byte chunks swizzled by row / 2
+        auto slot = [&](int r, int k) { return base + r * 64 + ((k ^ ((r >> 1) & 3)) << 4); };
         for (int i = 0; i < tiles; i++) {
             const Tile t = tile_at(i);
             const int b = i & 1, row0 = t.m0 + 32 * q, row = row0 + lane;
@@ -468,80 +484,89 @@ __global__ void __launch_bounds__(PjCfg<BN>::THREADS, 1) proj_kernel(const __gri
             uint32_t exps = 0;
             for (int c = c0; c < c1; c += 32) {
                 const int col = t.n0 + c, nv = min(32, a.N - col);
-                uint32_t r[32];
-                tc::tmem_ld32_async(tmem + lane_base + b * BN + c, r);
-                ProjAux now;
-                if (epi) {
-                    now = aux;
-                    if (c + 32 < c1)
-                        proj_load_aux<KIND>(a.e, row0, col + 32, min(32, a.N - col - 32), a.M, a.N, lane, aux);
-                }
-                // the staging tile is free once the store that read it last is done
-                if (lane == 0) {
-                    if (wide || KIND == PJ_FWD_CK) tc::bulk_wait_read<0>();
-                    else tc::bulk_wait_read<1>();
-                }
-                __syncwarp();
-                uint32_t base = stage;
-                if (!wide && KIND != PJ_FWD_CK) base += (nst & 1) * 2048;
-                // 16 bits: 64-byte rows, chunks swizzled by row / 2 (mod 4)
-                auto slot = [&](int rr, int k) { return base + rr * 64 + ((k ^ ((rr >> 1) & 3)) << 4); };
-                if (add16) {
+                if (epi && c > c0) proj_load_aux<KIND>(a.e, row0, col, nv, a.M, a.N, lane, aux);
+                uint32_t codes[8];
 #pragma unroll
-                    for (int k = 0; k < 4; k++) tc::st_shared_u4(slot(lane / 4 + 8 * k, lane % 4), now.add[k]);
-                    __syncwarp();
-                }
-                tc::tmem_ld_wait();
-                float v[32];
-#pragma unroll
-                for (int k = 0; k < 32; k++) v[k] = __uint_as_float(r[k]);
-                uint4 codes[2];
-                if (epi) {
-                    if (KIND != PJ_GRAD && a.e.bias) {
-#pragma unroll
-                        for (int k = 0; k < 32; k++) v[k] += __shfl_sync(0xffffffffu, now.bias, k);
+                for (int h = 0; h < 32 / W; h++) {
+                    uint32_t r[W];
+                    tc::tmem_ld_async<W>(tmem + lane_base + b * BN + c + h * W, r);
+                    if (h == 0 || wide) {
+                        // the staging tile is free once the store that read it last is done
+                        if (lane == 0) tc::bulk_wait_read<0>();
+                        __syncwarp();
                     }
-                    if (row < a.M) {
-                        exps |= proj_epilogue32<KIND>(v, a.e, now, row, col, nv, a.N, codes) << ((c - c0) / 4);
-                        if (a.e.add && a.e.out_f32) proj_add_f32(v, a.e, (int64_t)row * a.N + col, nv);
+                    if (h == 0 && add16) {
+#pragma unroll
+                        for (int k = 0; k < 4; k++) tc::st_shared_u4(slot(lane / 4 + 8 * k, lane % 4), aux.add[k]);
+                        __syncwarp();
                     }
-                }
-                if (wide) {  // 128-byte rows, 16-byte chunks swizzled by the row (mod 8)
+                    tc::tmem_ld_wait();
+                    float v[W];
 #pragma unroll
-                    for (int k = 0; k < 8; k++)
-                        tc::st_shared_v4(base + lane * 128 + ((k ^ (lane & 7)) << 4), __float_as_uint(v[4 * k]),
-                                         __float_as_uint(v[4 * k + 1]), __float_as_uint(v[4 * k + 2]),
-                                         __float_as_uint(v[4 * k + 3]));
-                } else {
+                    for (int k = 0; k < W; k++) v[k] = __uint_as_float(r[k]);
+                    if (epi) {
+                        if (KIND != PJ_GRAD && a.e.bias) {
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        if (add16) {
-                            float f[8];
-                            floats8_16(tc::ld_shared_v4(slot(lane, k)), a.e.bf16, f);
-#pragma unroll
-                            for (int j = 0; j < 8; j++) v[8 * k + j] += f[j];
+                            for (int k = 0; k < W; k++) v[k] += __shfl_sync(0xffffffffu, aux.bias, h * W + k);
                         }
-                        tc::st_shared_u4(slot(lane, k), pack8_16(v + 8 * k, a.e.bf16));
+                        if (row < a.M) {
+                            // W / 8 vectors of a dense pre-activation, half as many of codes
+                            const uint4 p[2] = {a.e.pre_codes ? aux.pre[h * W / 16] : aux.pre[h * W / 8],
+                                                aux.pre[(h * W / 8 + 1) % 4]};
+                            exps |= proj_epilogue<KIND, W>(v, a.e, p, aux.exp, row, col + h * W, nv - h * W, a.N, codes)
+                                    << ((c - c0) / 4);
+                            if (a.e.add && a.e.out_f32)
+                                proj_add_f32<W>(v, a.e, (int64_t)row * a.N + col + h * W, nv - h * W);
+                        }
+                    }
+                    if (wide) {  // 16 columns to a box
+#pragma unroll
+                        for (int k = 0; k < W / 4; k++)
+                            tc::st_shared_v4(slot(lane, k % 4) + k / 4 * 2048, __float_as_uint(v[4 * k]),
+                                             __float_as_uint(v[4 * k + 1]), __float_as_uint(v[4 * k + 2]),
+                                             __float_as_uint(v[4 * k + 3]));
+                        tc::fence_async_smem();
+                        __syncwarp();
+                        if (lane == 0) {
+#pragma unroll
+                            for (int k = 0; k < W / 16; k++) {
+                                if (part) tc::tma_store_2d(&a.pmap, base + k * 2048, c + h * W + 16 * k, t.part + 32 * q);
+                                else if (h * W + 16 * k < nv) tc::tma_store_2d(&a.dmap, base + k * 2048, col + h * W + 16 * k, row0);
+                            }
+                            tc::bulk_commit();
+                        }
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < W / 8; k++) {
+                            const uint32_t at = slot(lane, h * W / 8 + k);
+                            if (add16) {
+                                float f[8];
+                                floats8_16(tc::ld_shared_v4(at), a.e.bf16, f);
+#pragma unroll
+                                for (int j = 0; j < 8; j++) v[8 * k + j] += f[j];
+                            }
+                            tc::st_shared_u4(at, pack8_16(v + 8 * k, a.e.bf16));
+                        }
                     }
                 }
                 if constexpr (KIND == PJ_FWD_CK) {
                     // codes: 32-byte rows behind a 16-bit tile, or straight to memory
                     if (epi && a.ctma && !wide) {
-                        tc::st_shared_u4(base + 2048 + lane * 32, codes[0]);
-                        tc::st_shared_u4(base + 2048 + lane * 32 + 16, codes[1]);
+                        tc::st_shared_v4(base + 2048 + lane * 32, codes[0], codes[1], codes[2], codes[3]);
+                        tc::st_shared_v4(base + 2048 + lane * 32 + 16, codes[4], codes[5], codes[6], codes[7]);
                     } else if (epi && row < a.M) {
                         proj_store_codes(a.e.codes + (int64_t)row * a.N + col, nv, codes);
                     }
                 }
-                tc::fence_async_smem();
-                __syncwarp();
-                if (lane == 0) {
-                    if (part) tc::tma_store_2d(&a.pmap, base, c, t.part + 32 * q);
-                    else tc::tma_store_2d(&a.dmap, base, col, row0);
-                    if (KIND == PJ_FWD_CK && epi && a.ctma && !wide) tc::tma_store_2d(&a.cmap, base + 2048, col, row0);
-                    tc::bulk_commit();
+                if (!wide) {
+                    tc::fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        tc::tma_store_2d(&a.dmap, base, col, row0);
+                        if (KIND == PJ_FWD_CK && a.ctma) tc::tma_store_2d(&a.cmap, base + 2048, col, row0);
+                        tc::bulk_commit();
+                    }
                 }
-                nst++;
             }
             tc::tc_before();
             __syncwarp();
@@ -577,75 +602,74 @@ struct ProjJoin {
     void* d;
     int M, N, mt, nt, full, S, BN;
 };
-// Joins the splits of the tiles full ..: thread i takes 32 columns of a row of a tile.
+// Joins the splits of the tiles full ..: thread i takes 8 columns of a row of a
+// tile (four neighbouring lanes hold a checkpoint group), the splits' loads all in
+// flight, 16 at most.
 template <int KIND>
 __device__ __forceinline__ void proj_join(const ProjJoin& a, int64_t i) {
-    const int per = a.BN / 32;
-    const int chunk = (int)(i % per), r = (int)(i / per % 128);
+    const int per = a.BN / 8;
+    const int piece = (int)(i % per), r = (int)(i / per % 128);
     const int64_t j = i / per / 128;
-    int t = a.full + (int)j;
-    if (t >= a.mt * a.nt) return;
+    const int t = a.full + (int)j;  // the grid covers whole tiles
     const int pg = PJ_GROUP_M * a.nt, g = t / pg, rem = t - g * pg;
     const int gm = min(PJ_GROUP_M, a.mt - g * PJ_GROUP_M);
     const int64_t row = (g * PJ_GROUP_M + rem % gm) * 128 + r;
-    const int col = rem / gm * a.BN + 32 * chunk;
-    if (row >= a.M || col >= a.N) return;
-    const int nv = min(32, a.N - col);
-    ProjAux x;
-    proj_load_pre<KIND>(a.e, row, col, nv, a.N, x);
-    float v[32];
-#pragma unroll
-    for (int k = 0; k < 32; k++) v[k] = 0.f;
-    const float* p = a.part + (j * a.S * 128 + r) * a.BN + 32 * chunk;
-    for (int z = 0; z < a.S; z++, p += 128 * a.BN) {
-#pragma unroll
-        for (int k = 0; k < 8; k++) {
-            const float4 f = reinterpret_cast<const float4*>(p)[k];
-            v[4 * k] += f.x, v[4 * k + 1] += f.y, v[4 * k + 2] += f.z, v[4 * k + 3] += f.w;
+    const int col = rem / gm * a.BN + 8 * piece;
+    const bool in = row < a.M && col < a.N;
+    if (__all_sync(0xffffffffu, !in)) return;
+    const int64_t at = row * a.N + col;
+    float v[8] = {};
+    const float* p = a.part + (j * a.S * 128 + r) * a.BN + 8 * piece;
+    if (in) {
+#pragma unroll 8
+        for (int z = 0; z < a.S; z++) {
+            const float4* q = reinterpret_cast<const float4*>(p + (int64_t)z * 128 * a.BN);
+            const float4 x = q[0], y = q[1];
+            v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
+            v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
         }
     }
-    const int64_t at = row * a.N + col;
-    if ((KIND == PJ_FWD || KIND == PJ_FWD_CK) && a.e.bias) {
+    if ((KIND == PJ_FWD || KIND == PJ_FWD_CK) && a.e.bias && in) {
+        float b[8];
+        load_params<8>(a.e.bias, a.e.bias_dtype, col, b);
 #pragma unroll
-        for (int k = 0; k < 4; k++)
-            if (8 * k < nv) {
-                float b[8];
-                load_params<8>(a.e.bias, a.e.bias_dtype, col + 8 * k, b);
-#pragma unroll
-                for (int m = 0; m < 8; m++) v[8 * k + m] += b[m];
-            }
+        for (int m = 0; m < 8; m++) v[m] += b[m];
     }
-    uint4 codes[2];
-    const uint32_t exp = proj_epilogue32<KIND>(v, a.e, x, row, col, nv, a.N, codes);
+    uint4 pre[1] = {};
+    uint32_t pexp = 0, codes[2];
+    if (KIND == PJ_GRAD && in) {
+        if (a.e.pre_codes) {
+            const uint2 w = *reinterpret_cast<const uint2*>(a.e.pre_codes + at);
+            pre[0] = make_uint4(w.x, w.y, 0, 0);
+            pexp = a.e.pre_exps[proj_group(row, col, a.N)];
+        } else {
+            pre[0] = *proj_pre16(a.e, row, col, a.N);
+        }
+    }
+    if (KIND != PJ_FWD_CK && !in) return;
+    const uint32_t exp = proj_epilogue<KIND, 8>(v, a.e, pre, pexp, row, col, in ? 8 : 0, a.N, codes);
+    if (!in) return;
     if constexpr (KIND == PJ_FWD_CK) {
-        proj_store_codes(a.e.codes + at, nv, codes);
-        a.e.exps[proj_group(row, col, a.N)] = (uint8_t)exp;
+        *reinterpret_cast<uint2*>(a.e.codes + at) = make_uint2(codes[0], codes[1]);
+        if (piece % 4 == 0) a.e.exps[proj_group(row, col, a.N)] = (uint8_t)exp;
     }
     if (KIND != PJ_PLAIN && a.e.add) {
         if (a.e.out_f32) {
-            proj_add_f32(v, a.e, at, nv);
+            proj_add_f32<8>(v, a.e, at, 8);
         } else {
+            float f[8];
+            floats8_16(*proj_add16(a.e, row, col, a.N), a.e.bf16, f);
 #pragma unroll
-            for (int k = 0; k < 4; k++)
-                if (8 * k < nv) {
-                    float f[8];
-                    floats8_16(proj_add16(a.e, row, col, a.N)[k], a.e.bf16, f);
-#pragma unroll
-                    for (int m = 0; m < 8; m++) v[8 * k + m] += f[m];
-                }
+            for (int m = 0; m < 8; m++) v[m] += f[m];
         }
     }
-#pragma unroll
-    for (int k = 0; k < 4; k++)
-        if (8 * k < nv) {
-            if (a.e.out_f32) {
-                float4* o = reinterpret_cast<float4*>(static_cast<float*>(a.d) + at + 8 * k);
-                o[0] = make_float4(v[8 * k], v[8 * k + 1], v[8 * k + 2], v[8 * k + 3]);
-                o[1] = make_float4(v[8 * k + 4], v[8 * k + 5], v[8 * k + 6], v[8 * k + 7]);
-            } else {
-                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.d) + at + 8 * k) = pack8_16(v + 8 * k, a.e.bf16);
-            }
-        }
+    if (a.e.out_f32) {
+        float4* o = reinterpret_cast<float4*>(static_cast<float*>(a.d) + at);
+        o[0] = make_float4(v[0], v[1], v[2], v[3]);
+        o[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.d) + at) = pack8_16(v, a.e.bf16);
+    }
 }
 // Column sums of dY, joined beside the tiles (rwkv_projection_dw's db): blocks from
 // `first` on take 128 columns each and add the slices in order.
@@ -720,7 +744,7 @@ inline bool proj_map_2d(CUtensorMap* m, CUtensorMapDataType type, int esize, con
 
 template <int BN, bool AMN, bool BMN, int KIND>
 inline cudaError_t proj_launch_t(const ProjArgs& a, int sm_count, bool after_own, cudaStream_t st) {
-    using C = PjCfg<BN>;
+    using C = PjCfg<BN, KIND>;
     auto kern = proj_kernel<BN, AMN, BMN, KIND>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::TOTAL);
     if (e != cudaSuccess) return e;
@@ -759,20 +783,20 @@ inline cudaError_t proj_gemm(const void* A, const void* B, void* D, int64_t M, i
                   : proj_map_2d(&a.amap, t16, 2, A, K, M, PJ_BK, 128, sw128);
     ok = ok && (BMN ? proj_map_2d(&a.bmap, t16, 2, B, N, K, 64, PJ_BK, sw128)
                     : proj_map_2d(&a.bmap, t16, 2, B, K, N, PJ_BK, p.BN, sw128));
-    ok = ok && (e.out_f32 ? proj_map_2d(&a.dmap, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, D, N, M, 32, 32, sw128)
+    ok = ok && (e.out_f32 ? proj_map_2d(&a.dmap, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, D, N, M, 16, 32, CU_TENSOR_MAP_SWIZZLE_64B)
                           : proj_map_2d(&a.dmap, t16, 2, D, N, M, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B));
     a.ctma = KIND == PJ_FWD_CK && N % 16 == 0;
     if (a.ctma)
         ok = ok && proj_map_2d(&a.cmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, e.codes, N, M, 32, 32, CU_TENSOR_MAP_SWIZZLE_NONE);
     if (p.S > 1)
-        ok = ok && proj_map_2d(&a.pmap, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, ws, p.BN, (int64_t)rem * p.S * 128, 32, 32,
-                               sw128);
+        ok = ok && proj_map_2d(&a.pmap, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, ws, p.BN, (int64_t)rem * p.S * 128, 16, 32,
+                               CU_TENSOR_MAP_SWIZZLE_64B);
     if (!ok) return cudaErrorInvalidValue;
     const cudaError_t rc = p.BN == 128 ? proj_launch_t<128, AMN, BMN, KIND>(a, sm_count, after_own, st)
                                        : proj_launch_t<256, AMN, BMN, KIND>(a, sm_count, after_own, st);
     if (rc != cudaSuccess || (p.S == 1 && !cols)) return rc;
     const ProjJoin j{ws, e, D, (int)M, (int)N, p.mt, p.nt, p.full, p.S, p.BN};
-    const int first = p.S > 1 ? ceil_div((int64_t)rem * 128 * (p.BN / 32), PJ_JOIN_T) : 0;
+    const int first = p.S > 1 ? ceil_div((int64_t)rem * 128 * (p.BN / 8), PJ_JOIN_T) : 0;
     const ColJoin c = cols ? *cols : ColJoin{};
     return launch_pdl(proj_join_kernel<KIND>, dim3(first + ceil_div(c.N, PJ_JOIN_T)), dim3(PJ_JOIN_T), 0, st, j, c, first);
 }

@@ -10,9 +10,9 @@ int gemm_wait_record(cudaStream_t st, const char* fn, int** err, int** err_host,
 
 namespace {
 
-// What dW needs before its product, in one launch: blocks below `first` write act(X)
-// in the operands' type (from the dense pre-activation or its checkpoint), the
-// others sum slices of dY's columns.
+// What dW needs before its product, in one launch: blocks below `first` sum slices of
+// dY's columns (few and long, so they start first), the others write act(X) in the
+// operands' type (from the dense pre-activation or its checkpoint).
 //
 // Restoring the operand in a pass of its own reads and writes it once (8192 x 8192:
 // 32 us of 320); decoding inside the product would repeat the work for every 128
@@ -32,7 +32,7 @@ struct DwPrep {
 constexpr int PREP_T = 256, PREP_U = 4, CS_COLS = 256;
 
 __device__ __forceinline__ void restore_operand(const DwPrep& a) {
-    const int64_t i0 = blockIdx.x * (int64_t)(PREP_T * PREP_U) + threadIdx.x;
+    const int64_t i0 = ((int)blockIdx.x - a.first) * (int64_t)(PREP_T * PREP_U) + threadIdx.x;
     const int G = (a.IN + CK_GROUP - 1) / CK_GROUP, per = a.IN / 8;
     uint4 raw[PREP_U];
     uint32_t e[PREP_U];
@@ -100,8 +100,8 @@ __device__ __forceinline__ void sum_columns(const DwPrep& a, int block) {
     }
 }
 __global__ void __launch_bounds__(PREP_T, 1) dw_prep_kernel(const DwPrep a) {
-    if ((int)blockIdx.x < a.first) restore_operand(a);
-    else sum_columns(a, (int)blockIdx.x - a.first);
+    if ((int)blockIdx.x < a.first) sum_columns(a, (int)blockIdx.x);
+    else restore_operand(a);
 }
 int col_slices(int rows, int OUT) {
     return std::max(1, std::min(ceil_div(rows, 64), 148 * 4 / ceil_div(OUT, CS_COLS)));
@@ -280,8 +280,8 @@ extern "C" int rwkv_projection_dw(int dtype, const void* dy, int act, const void
     q.OUT = OUT;
     q.slices = p.slices;
     q.bf16 = dtype == RWKV_BF16;
-    q.first = restore ? ceil_div(q.units, PREP_T * PREP_U) : 0;
-    const int grid = q.first + (db ? ceil_div(OUT, CS_COLS) * p.slices : 0);
+    q.first = db ? ceil_div(OUT, CS_COLS) * p.slices : 0;
+    const int grid = q.first + (restore ? ceil_div(q.units, PREP_T * PREP_U) : 0);
     if (grid) {
         dw_prep_kernel<<<grid, PREP_T, 0, st>>>(q);
         if (int rc = check_launch("dw_prep_kernel")) return rc;
