@@ -293,8 +293,9 @@ __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.comm
 // at most N of this thread's bulk stores still read their shared memory
 template <int N>
 __device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
-template <int N>
-__device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* m) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
+}
 }  // namespace tc
 
 template <int BN, int KIND>
@@ -338,6 +339,11 @@ __global__ void __launch_bounds__(PjCfg<BN, KIND>::THREADS, 1) proj_kernel(const
     const int my_tiles = (int)blockIdx.x < units ? (units - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
     int* err = a.err;
 
+    if (tid == 64) {
+        tc::prefetch_map(&a.amap);
+        tc::prefetch_map(&a.bmap);
+        tc::prefetch_map(&a.dmap);
+    }
     if (tid == 0) {
         for (int s = 0; s < ST; s++) {
             tc::mbar_init(full + s, 1);
@@ -582,7 +588,7 @@ __global__ void __launch_bounds__(PjCfg<BN, KIND>::THREADS, 1) proj_kernel(const
                 }
             }
         }
-        if (lane == 0) tc::bulk_wait<0>();
+        if (lane == 0) tc::bulk_wait_read<0>();  // the staging tiles may go; the stores end with the grid
     }
     tc::tc_before();
     const int bad = __syncthreads_or(!ok && (warp >= 2 || lane == 0));
@@ -672,7 +678,7 @@ __device__ __forceinline__ void proj_join(const ProjJoin& a, int64_t i) {
     }
 }
 // Column sums of dY, joined beside the tiles (rwkv_projection_dw's db): blocks from
-// `first` on take 128 columns each and add the slices in order.
+// `first` on take 32 columns each, warp w the slices w, w + 4, ...; fixed order.
 struct ColJoin {
     const float* part;  // [slices][N]
     float* out;
@@ -686,12 +692,16 @@ __global__ void __launch_bounds__(PJ_JOIN_T) proj_join_kernel(const ProjJoin a, 
         proj_join<KIND>(a, blockIdx.x * (int64_t)PJ_JOIN_T + threadIdx.x);
         return;
     }
-    const int col = ((int)blockIdx.x - first) * PJ_JOIN_T + threadIdx.x;
-    if (col >= c.N) return;
+    __shared__ float red[PJ_JOIN_T / 32][32];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, col = ((int)blockIdx.x - first) * 32 + lane;
     float s = 0.f;
+    if (col < c.N) {
 #pragma unroll 8
-    for (int k = 0; k < c.slices; k++) s += c.part[(int64_t)k * c.N + col];
-    c.out[col] = s;
+        for (int k = w; k < c.slices; k += PJ_JOIN_T / 32) s += c.part[(int64_t)k * c.N + col];
+    }
+    red[w][lane] = s;
+    __syncthreads();
+    if (w == 0 && col < c.N) c.out[col] = red[0][lane] + red[1][lane] + red[2][lane] + red[3][lane];
 }
 
 // ------------------------------------------------------------------ host side
@@ -702,8 +712,9 @@ __global__ void __launch_bounds__(PJ_JOIN_T) proj_join_kernel(const ProjJoin a, 
 //    to hide a wide tile's epilogue (K <= 512: 4093 x 2048 over 96 with a sigmoid
 //    takes __ us in 128s, 27.5 in 256s) and where they give more SMs work.
 //  - The tiles past the last whole wave are split the way that the estimate below
-//    finds shortest: a stage of 64 takes 0.35 us on a 256-wide tile; joining takes
-//    3 us and writes and reads each split's tile once (4 TB/s).
+//    finds shortest: a stage of 64 takes 0.4 us on a 256-wide tile and 0.27 on a
+//    128-wide one (an SM's share of L2 bandwidth); joining takes 3.5 us and writes
+//    and reads each split's tile once in L2 (8 TB/s).
 struct ProjPlan {
     int BN, mt, nt, full, S;
     int64_t ws_bytes;  // the splits' tiles
@@ -720,9 +731,9 @@ inline ProjPlan proj_plan(int64_t M, int64_t N, int64_t K) {
     if (rem == 0) return p;
     double best = 0.0;
     for (int S = 1; S <= 16 && (S == 1 || nk / S >= 2); S++) {
-        const double stage = 0.35 * p.BN / 256, bytes = 2.0 * rem * S * 128 * p.BN * 4;
+        const double stage = p.BN == 256 ? 0.4 : 0.27, bytes = 2.0 * rem * S * 128 * p.BN * 4;
         const double us = (double)((rem * S + PJ_SMS - 1) / PJ_SMS) * ((nk + S - 1) / S) * stage +
-                          (S > 1 ? 3.0 + bytes / 4e6 : 0.0);
+                          (S > 1 ? 3.5 + bytes / 8e6 : 0.0);
         if (S == 1 || us < best) best = us, p.S = S;
     }
     if (p.S == 1) p.full = tiles;
@@ -798,7 +809,7 @@ inline cudaError_t proj_gemm(const void* A, const void* B, void* D, int64_t M, i
     const ProjJoin j{ws, e, D, (int)M, (int)N, p.mt, p.nt, p.full, p.S, p.BN};
     const int first = p.S > 1 ? ceil_div((int64_t)rem * 128 * (p.BN / 8), PJ_JOIN_T) : 0;
     const ColJoin c = cols ? *cols : ColJoin{};
-    return launch_pdl(proj_join_kernel<KIND>, dim3(first + ceil_div(c.N, PJ_JOIN_T)), dim3(PJ_JOIN_T), 0, st, j, c, first);
+    return launch_pdl(proj_join_kernel<KIND>, dim3(first + ceil_div(c.N, 32)), dim3(PJ_JOIN_T), 0, st, j, c, first);
 }
 
 }  // namespace rwkv

@@ -361,31 +361,41 @@ __global__ void __launch_bounds__(512, 1) ln_bwd_kernel(const LnBwdArgs a) {
     const int nvec = a.D / VE;
     const float inv_d = 1.f / (float)a.D;
     float w[NV][VE], sw[NV][VE], sb[NV][VE];
+    bool has[NV];
 #pragma unroll
     for (int j = 0; j < NV; j++) {
         const int v = t + j * nt;
+        has[j] = v < nvec;
 #pragma unroll
         for (int k = 0; k < VE; k++) w[j][k] = sw[j][k] = sb[j][k] = 0.f;
-        if (v < nvec) load_params<VE>(a.w, a.wdtype, (int64_t)v * VE, w[j]);
+        if (has[j]) load_params<VE>(a.w, a.wdtype, (int64_t)v * VE, w[j]);
     }
-    const int64_t step = (int64_t)gridDim.x * R;
-    auto slot = [&](int stage, int r, int part, int j) {
-        return ring + t + (uint32_t)nt * (uint32_t)(((stage * R + r) * 3 + part) * NV + j);
-    };
-    auto fetch = [&](int64_t r0, int stage) {
+    const int step = (int)gridDim.x * R;
+    const int64_t vstep = (int64_t)step * nvec;  // in vectors
+    const uint4* const dy = static_cast<const uint4*>(a.dy) + t;
+    const uint4* const xs = static_cast<const uint4*>(a.x) + t;
+    const uint4* const dres = static_cast<const uint4*>(a.dres) + t;
+    using Codes = std::conditional_t<VE == 8, uint2, uint32_t>;  // of one vector
+    const Codes* const cs = reinterpret_cast<const Codes*>(a.codes) + t;
+    // one row at a time always exists inside the loop
+    auto exists = [&](int64_t r0, int r) { return R == 1 || r0 + r < a.rows; };
+    // ring slot of (row, part, vector) in the stage that starts at `base`
+    auto slot = [&](int base, int r, int part, int j) { return ring + base + ((r * 3 + part) * NV + j) * nt; };
+    const int stage_n = R * 3 * NV * nt;
+    auto fetch = [&](int64_t r0, int64_t at, int base) {
+        if (r0 < a.rows) {
 #pragma unroll
-        for (int r = 0; r < R; r++)
+            for (int r = 0; r < R; r++)
 #pragma unroll
-            for (int j = 0; j < NV; j++) {
-                const int v = t + j * nt;
-                if (r0 + r < a.rows && v < nvec) {
-                    const int64_t at = (r0 + r) * a.D + (int64_t)v * VE;
-                    copy_async<16>(slot(stage, r, 0, j), static_cast<const T*>(a.dy) + at);
-                    if constexpr (CK) copy_async<VE>(slot(stage, r, 1, j), a.codes + at);
-                    else copy_async<16>(slot(stage, r, 1, j), static_cast<const T*>(a.x) + at);
-                    if (a.dres) copy_async<16>(slot(stage, r, 2, j), static_cast<const T*>(a.dres) + at);
-                }
-            }
+                for (int j = 0; j < NV; j++)
+                    if (exists(r0, r) && has[j]) {
+                        const int64_t o = at + r * nvec + j * nt;
+                        copy_async<16>(slot(base, r, 0, j), dy + o);
+                        if constexpr (CK) copy_async<VE>(slot(base, r, 1, j), cs + o);
+                        else copy_async<16>(slot(base, r, 1, j), xs + o);
+                        if (a.dres) copy_async<16>(slot(base, r, 2, j), dres + o);
+                    }
+        }
         copy_commit();
     };
     // the rows' statistics and exponents, one step ahead in registers
@@ -394,25 +404,24 @@ __global__ void __launch_bounds__(512, 1) ln_bwd_kernel(const LnBwdArgs a) {
     auto fetch_small = [&](int64_t r0) {
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            const bool ok = r0 + r < a.rows;
-            nmean[r] = ok ? a.mean[r0 + r] : 0.f;
-            nrstd[r] = ok ? a.rstd[r0 + r] : 0.f;
+            const int64_t row = min(r0 + r, (int64_t)a.rows - 1);  // of no use past the end
+            nmean[r] = a.mean[row];
+            nrstd[r] = a.rstd[row];
             if constexpr (CK) {
 #pragma unroll
-                for (int j = 0; j < NV; j++) {
-                    const int v = t + j * nt;
-                    nex[r][j] = ok && v < nvec ? a.exps[(r0 + r) * a.G + v / (CK_GROUP / VE)] : 0u;
-                }
+                for (int j = 0; j < NV; j++)
+                    nex[r][j] = has[j] ? a.exps[row * a.G + (t + j * nt) / (CK_GROUP / VE)] : 0u;
             }
         }
     };
     const int64_t first = (int64_t)blockIdx.x * R;
+    int64_t at = first * nvec, fat = at;
 #pragma unroll
-    for (int i = 0; i < LN_STAGES - 1; i++) fetch(first + i * step, i);
+    for (int i = 0; i < LN_STAGES - 1; i++, fat += vstep) fetch(first + (int64_t)i * step, fat, t + i * stage_n);
     fetch_small(first);
-    int stage = 0, buf = 0;
-    for (int64_t r0 = first; r0 < a.rows; r0 += step, buf ^= 1) {
-        fetch(r0 + (LN_STAGES - 1) * step, stage == 0 ? LN_STAGES - 1 : stage - 1);
+    int cur = t, put = t + (LN_STAGES - 1) * stage_n, buf = 0;
+    for (int64_t r0 = first; r0 < a.rows; r0 += step, at += vstep, fat += vstep, buf ^= 1) {
+        fetch(r0 + (int64_t)(LN_STAGES - 1) * step, fat, put);
         copy_wait<LN_STAGES - 1>();
 #pragma unroll
         for (int r = 0; r < R; r++) {
@@ -430,18 +439,18 @@ __global__ void __launch_bounds__(512, 1) ln_bwd_kernel(const LnBwdArgs a) {
             rs[2 * r] = rs[2 * r + 1] = 0.f;
 #pragma unroll
             for (int j = 0; j < NV; j++) {
-                if (r0 + r >= a.rows || t + j * nt >= nvec) continue;
+                if (!exists(r0, r) || !has[j]) continue;
                 float dy[VE];
-                Vec16<T>::unpack(*slot(stage, r, 0, j), dy);
+                Vec16<T>::unpack(*slot(cur, r, 0, j), dy);
                 const float shift = -mean[r] * rstd[r];
                 float scale = rstd[r];
                 if constexpr (CK) {
-                    const uint32_t* c = reinterpret_cast<const uint32_t*>(slot(stage, r, 1, j));
+                    const uint32_t* c = reinterpret_cast<const uint32_t*>(slot(cur, r, 1, j));
                     ck_codes4(c[0], h[r][j]);
                     if constexpr (VE == 8) ck_codes4(c[1], h[r][j] + 4);
                     scale *= ck_scale(ex[r][j]);
                 } else {
-                    Vec16<T>::unpack(*slot(stage, r, 1, j), h[r][j]);
+                    Vec16<T>::unpack(*slot(cur, r, 1, j), h[r][j]);
                 }
 #pragma unroll
                 for (int k = 0; k < VE; k++) {
@@ -473,15 +482,13 @@ __global__ void __launch_bounds__(512, 1) ln_bwd_kernel(const LnBwdArgs a) {
         for (int r = 0; r < R; r++) {
             const float c0 = -rstd[r] * __shfl_sync(0xffffffffu, tot, 2 * r * L);
             const float c1 = -rstd[r] * __shfl_sync(0xffffffffu, tot, (2 * r + 1) * L);
-            const int64_t row = r0 + r;
 #pragma unroll
             for (int j = 0; j < NV; j++) {
-                const int v = t + j * nt;
-                if (row >= a.rows || v >= nvec) continue;
+                if (!exists(r0, r) || !has[j]) continue;
                 float dy[VE], o[VE];
-                Vec16<T>::unpack(*slot(stage, r, 0, j), dy);
+                Vec16<T>::unpack(*slot(cur, r, 0, j), dy);
                 if (a.dres) {
-                    Vec16<T>::unpack(*slot(stage, r, 2, j), o);
+                    Vec16<T>::unpack(*slot(cur, r, 2, j), o);
 #pragma unroll
                     for (int k = 0; k < VE; k++) o[k] += c0;
                 } else {
@@ -490,10 +497,11 @@ __global__ void __launch_bounds__(512, 1) ln_bwd_kernel(const LnBwdArgs a) {
                 }
 #pragma unroll
                 for (int k = 0; k < VE; k++) o[k] = fmaf(dy[k] * w[j][k], rstd[r], fmaf(h[r][j][k], c1, o[k]));
-                __stcs(reinterpret_cast<uint4*>(static_cast<T*>(a.dx) + row * a.D + (int64_t)v * VE), Vec16<T>::pack(o));
+                __stcs(static_cast<uint4*>(a.dx) + t + at + r * nvec + j * nt, Vec16<T>::pack(o));
             }
         }
-        stage = stage == LN_STAGES - 1 ? 0 : stage + 1;
+        put = cur;
+        cur = cur == t + (LN_STAGES - 1) * stage_n ? t : cur + stage_n;
     }
     copy_wait<0>();
     if (!a.part) return;

@@ -31,6 +31,8 @@ struct DwPrep {
 };
 constexpr int PREP_T = 256, PREP_U = 4, CS_COLS = 256;
 
+// FLAT: whole groups per row (IN % 32 == 0, or a dense x), nothing is divided.
+template <bool CK, bool FLAT>
 __device__ __forceinline__ void restore_operand(const DwPrep& a) {
     const int64_t i0 = ((int)blockIdx.x - a.first) * (int64_t)(PREP_T * PREP_U) + threadIdx.x;
     const int G = (a.IN + CK_GROUP - 1) / CK_GROUP, per = a.IN / 8;
@@ -38,13 +40,12 @@ __device__ __forceinline__ void restore_operand(const DwPrep& a) {
     uint32_t e[PREP_U];
 #pragma unroll
     for (int j = 0; j < PREP_U; j++) {
-        const int64_t i = i0 + j * PREP_T;
-        if (i >= a.units) continue;
-        if (a.codes) {
+        const int64_t i = min(i0 + j * PREP_T, a.units - 1);
+        if constexpr (CK) {
             const uint2 w = __ldcs(reinterpret_cast<const uint2*>(a.codes + 8 * i));
             raw[j] = make_uint4(w.x, w.y, 0, 0);
             int64_t group = i >> 2;
-            if (a.IN % CK_GROUP) {
+            if constexpr (!FLAT) {
                 const int64_t row = a.units < (1ll << 32) ? (uint32_t)i / (uint32_t)per : i / per;
                 group = row * G + ((int)(i - row * per) >> 2);
             }
@@ -56,10 +57,8 @@ __device__ __forceinline__ void restore_operand(const DwPrep& a) {
     with_act(a.act, [&]<int ACT>() {
 #pragma unroll
         for (int j = 0; j < PREP_U; j++) {
-            const int64_t i = i0 + j * PREP_T;
-            if (i >= a.units) continue;
             float v[8];
-            if (a.codes) {
+            if constexpr (CK) {
                 const float s = ck_scale(e[j]);
                 ck_unpack4(raw[j].x, s, v);
                 ck_unpack4(raw[j].y, s, v + 4);
@@ -68,7 +67,7 @@ __device__ __forceinline__ void restore_operand(const DwPrep& a) {
             }
 #pragma unroll
             for (int k = 0; k < 8; k++) v[k] = act_t<ACT, true>(v[k]);
-            static_cast<uint4*>(a.operand)[i] = pack8_16(v, a.bf16);
+            if (i0 + j * PREP_T < a.units) static_cast<uint4*>(a.operand)[i0 + j * PREP_T] = pack8_16(v, a.bf16);
         }
     });
 }
@@ -101,7 +100,9 @@ __device__ __forceinline__ void sum_columns(const DwPrep& a, int block) {
 }
 __global__ void __launch_bounds__(PREP_T, 1) dw_prep_kernel(const DwPrep a) {
     if ((int)blockIdx.x < a.first) sum_columns(a, (int)blockIdx.x);
-    else restore_operand(a);
+    else if (!a.codes) restore_operand<false, true>(a);
+    else if (a.IN % CK_GROUP == 0) restore_operand<true, true>(a);
+    else restore_operand<true, false>(a);
 }
 int col_slices(int rows, int OUT) {
     return std::max(1, std::min(ceil_div(rows, 64), 148 * 4 / ceil_div(OUT, CS_COLS)));
@@ -295,7 +296,7 @@ extern "C" int rwkv_projection_dw(int dtype, const void* dy, int act, const void
         rc = proj_gemm<true, true, PJ_PLAIN>(dy, restore ? ws : x, dw, OUT, IN, rows, e, reinterpret_cast<float*>(ws + p.operand),
                                    err, err_host, sms, st, grid != 0, db ? &cols : nullptr);
     } else {
-        rc = launch_pdl(proj_join_kernel<PJ_PLAIN>, dim3(ceil_div(OUT, PJ_JOIN_T)), dim3(PJ_JOIN_T), 0, st, ProjJoin{}, cols, 0);
+        rc = launch_pdl(proj_join_kernel<PJ_PLAIN>, dim3(ceil_div(OUT, 32)), dim3(PJ_JOIN_T), 0, st, ProjJoin{}, cols, 0);
     }
     if (rc != cudaSuccess) return fail(RWKV_E_CUDA, "%s: %s", fn, cudaGetErrorString(rc));
     return ok();
