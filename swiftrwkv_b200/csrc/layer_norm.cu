@@ -12,6 +12,7 @@
 // vectors are kept (half the registers of fp32 for 16-bit types) and unpacked
 // in each pass.
 #include <algorithm>
+#include <atomic>
 
 #include "ckpt8.cuh"
 
@@ -352,8 +353,8 @@ constexpr int LN_STAGES = 3;
 // (cp.async) and reads only its own vectors, so the ring needs no barrier, and
 // HBM stays busy while the block computes and waits at its barrier: one per R
 // rows, for the two row sums (buffers alternating).
-template <typename T, bool CK, int NV, int R>
-__global__ void __launch_bounds__(512, 1) ln_bwd_kernel(const LnBwdArgs a) {
+template <typename T, bool CK, int NV, int R, int MAXT, int MINB>
+__global__ void __launch_bounds__(MAXT, MINB) ln_bwd_kernel(const LnBwdArgs a) {
     constexpr int VE = Vec16<T>::N;
     extern __shared__ uint4 ring[];  // [stage][row][dy | x | dres][NV][thread]
     __shared__ float red[2][16][2 * R];
@@ -665,15 +666,22 @@ __global__ void __launch_bounds__(1024) ln_bwd_params_kernel(const float* __rest
 
 constexpr int LN_BWD_BLOCKS = 148 * 4;  // at most: four resident blocks per SM
 
-template <typename T, bool CK, int NV, int R>
+template <typename T, bool CK, int NV, int R, int MAXT = 512, int MINB = 1>
 cudaError_t launch_ln_bwd_t(const LnBwdArgs& a, int* blocks, cudaStream_t st) {
-    auto kern = ln_bwd_kernel<T, CK, NV, R>;
+    auto kern = ln_bwd_kernel<T, CK, NV, R, MAXT, MINB>;
     const int nt = ceil_div(ceil_div(a.D / Vec16<T>::N, NV), 32) * 32;
     const int smem = LN_STAGES * R * 3 * NV * nt * 16;
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
-    // as many blocks as are resident by shared memory and threads
-    const int per_sm = std::max(1, std::min({4, 220 * 1024 / (smem + 2048), 1280 / nt}));
+    // as many blocks as are resident, so that they all run in one wave
+    static std::atomic<int> resident[17];  // by warps
+    int per_sm = resident[nt / 32].load(std::memory_order_relaxed);
+    if (per_sm == 0) {
+        const cudaError_t q = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, nt, smem);
+        if (q != cudaSuccess) return q;
+        per_sm = std::max(1, per_sm);
+        resident[nt / 32].store(per_sm, std::memory_order_relaxed);
+    }
     *blocks = std::min({ceil_div(a.rows, R), 148 * per_sm, LN_BWD_BLOCKS});
     kern<<<*blocks, nt, smem, st>>>(a);
     return cudaGetLastError();
@@ -685,10 +693,13 @@ int launch_ln_bwd(LnBwdArgs a, bool vec, void* dw, void* db, cudaStream_t st) {
     int blocks;
     if (vec && nvec <= 512 * 3) {
         // vectors per thread: the fewest with at most 512 threads.  Two rows
-        // at a time from a dense x (16384 x 2048 bf16: 51 us, one row 65 us), one
-        // from a checkpoint, whose decoding takes more registers (65 against 68 us)
+        // at a time from a dense x (16384 x 2048 bf16: 50 us, one row 65 us), one
+        // from a checkpoint, whose decoding takes more registers; there up to 320
+        // threads with registers for two blocks per SM (54 us, unbounded 60 us; the
+        // dense kernel 62 us with that bound)
         const cudaError_t e = nvec > 1024  ? launch_ln_bwd_t<T, CK, 3, 1>(a, &blocks, st)
                               : nvec > 512 ? launch_ln_bwd_t<T, CK, 2, 1>(a, &blocks, st)
+                              : CK && nvec <= 320 ? launch_ln_bwd_t<T, CK, 1, 1, 320, 2>(a, &blocks, st)
                                            : launch_ln_bwd_t<T, CK, 1, CK ? 1 : 2>(a, &blocks, st);
         if (e != cudaSuccess) return fail(RWKV_E_CUDA, "ln_bwd_kernel: %s", cudaGetErrorString(e));
     } else if (a.D <= 512 * 20) {
