@@ -556,7 +556,7 @@ int rwkv_act_backward(int dtype, const void* dy, const void* z, const int8_t* co
  * gradients; x, w and dY in `dtype`, BF16 or F16 (both operands of a
  * tensor-core product in one type); accumulation in fp32, one rounding at the
  * store.  IN % 8 == 0 and OUT % 8 == 0, tensors 16-byte aligned (exps and db to
- * their element); any rows >= 1.  tcgen05 tensor cores; these calls
+ * their element); rows in 1..2^24, IN and OUT up to 2^20.  tcgen05 tensor cores; these calls
  * share rwkv_q_gemm's wait-error record (rwkv_q_gemm_status), and a stream may
  * be captured once one call has run on its device.  `workspace`: device memory of
  * the matching _workspace_size bytes, 16-byte aligned (NULL when that is 0);

@@ -14,12 +14,15 @@
 // a multiple of a tile; row pitches must be multiples of 16 bytes (IN and OUT
 // multiples of 8).
 //
-// Tile = 128 rows of D (TMEM lanes) x BN columns, K in stages of 64.  A persistent
-// CTA walks its tiles; the accumulator of tile t lives in TMEM half (t & 1), so
-// the epilogue of one tile runs beside the MMAs of the next.
-//   warp 0      TMA producer, ST stages
-//   warp 1      TMEM owner; one thread issues 4 tcgen05.mma (M=128, N=BN, K=16)
-//               per stage and commits the stage / the tile
+// Tile = 128 rows of D (TMEM lanes) x 128 columns on one CTA, or 256 x 256 on a pair
+// of CTAs (cta_group::2: each holds 128 rows of A and of B and its 128 rows of D; the
+// first issues the MMAs for both), K in stages of 64.  A persistent CTA or pair
+// walks its tiles; the accumulator of tile t lives in TMEM half (t & 1), so the
+// epilogue of one tile runs beside the MMAs of the next.
+//   warp 0      TMA producer, ST stages; a pair's loads count on the first CTA's
+//               barriers
+//   warp 1      TMEM owner; one thread issues 4 tcgen05.mma (K=16) per stage and
+//               commits the stage / the tile (to both CTAs)
 //   warps 2 ..  epilogue, 16 warps (a sigmoid over 4093 x 2048 sums of 96 takes 21 us
 //               with 8): TMEM lane quadrant (warp & 3) = 32 rows of D, an equal share
 //               of the columns per 4 warps, 32 columns at a time in two halves.
@@ -53,7 +56,7 @@ constexpr int PJ_OUT_BYTES = 32 * 1024;  // output staging, shared by the epilog
 
 // Which epilogue a kernel has, at compile time: one that can do everything keeps
 // the registers of everything alive (16384 x 8192 over 96 takes 270 us with a
-// plain result in it, __ us in its own kernel).
+// plain result in it, 72 us in its own kernel).
 enum : int {
     PJ_PLAIN = 0,  // the sums
     PJ_FWD = 1,    // bias, z, activation, residual
@@ -293,15 +296,44 @@ __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.comm
 // at most N of this thread's bulk stores still read their shared memory
 template <int N>
 __device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
+// Two SMs on one tile (cta_group::2).  The loads are plain ones into this CTA's own
+// shared memory; their bytes are counted on the barrier at `bar` (a shared::cluster
+// address), the first CTA's.
+__device__ __forceinline__ void tma_2d_pair(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+        ::"r"(saddr(dst)), "l"(map), "r"(bar), "r"(c0), "r"(c1)
+        : "memory");
+}
+__device__ __forceinline__ void umma_ss_pair(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc,
+                                             uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+// arrives at the same barrier of both CTAs once the MMAs issued so far are done
+__device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            saddr(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* m) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
 }
 }  // namespace tc
 
-template <int BN, int KIND>
+// CG: CTAs on a tile of 128 CG rows; each holds 128 rows of A and BN / CG of B.
+template <int BN, int CG, int KIND>
 struct PjCfg {
     static constexpr int A_BYTES = 128 * 128;       // 128 rows x 64 k, 16 bits
-    static constexpr int B_BYTES = BN * 128;
+    static constexpr int B_BYTES = BN / CG * 128;
     static constexpr int STAGE = A_BYTES + B_BYTES;
     static constexpr int EW = KIND == PJ_FWD_CK ? 8 : 16;  // epilogue warps
     static constexpr int W = KIND == PJ_FWD_CK ? 32 : 16;  // columns a thread holds
@@ -318,12 +350,13 @@ struct PjCfg {
     static_assert(TOTAL <= 227 * 1024, "shared memory per CTA");
     static_assert(BN == 128 || BN == 256, "TMEM allocation is a power of two; shares of 32 columns");
     static_assert(ST >= 3, "pipeline depth");
+    static_assert(CG == 1 || BN == 256, "a pair of CTAs takes 256 x 256");
 };
 
 // AMN / BMN: the operand is MN-major.
-template <int BN, bool AMN, bool BMN, int KIND>
-__global__ void __launch_bounds__(PjCfg<BN, KIND>::THREADS, 1) proj_kernel(const __grid_constant__ ProjArgs a) {
-    using C = PjCfg<BN, KIND>;
+template <int BN, int CG, bool AMN, bool BMN, int KIND>
+__global__ void __launch_bounds__(PjCfg<BN, CG, KIND>::THREADS, 1) proj_kernel(const __grid_constant__ ProjArgs a) {
+    using C = PjCfg<BN, CG, KIND>;
     constexpr int ST = C::ST;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -335,9 +368,13 @@ __global__ void __launch_bounds__(PjCfg<BN, KIND>::THREADS, 1) proj_kernel(const
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::T_OFF);
     int* skip_slot = reinterpret_cast<int*>(smem + C::T_OFF + 8);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rank = CG == 2 ? (int)blockIdx.x & 1 : 0;  // within the pair; rank 0 issues the MMAs
+    const int first = (int)blockIdx.x / CG, stride = (int)gridDim.x / CG;
     const int units = a.full + (a.mt * a.nt - a.full) * a.S;
-    const int my_tiles = (int)blockIdx.x < units ? (units - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
+    const int my_tiles = first < units ? (units - 1 - first) / stride + 1 : 0;
     int* err = a.err;
+    // rank 0's barriers, as both CTAs address them
+    auto lead = [&](uint64_t* bar) { return CG == 2 ? tc::map_rank(tc::saddr(bar), 0) : tc::saddr(bar); };
 
     if (tid == 64) {
         tc::prefetch_map(&a.amap);
@@ -351,7 +388,7 @@ __global__ void __launch_bounds__(PjCfg<BN, KIND>::THREADS, 1) proj_kernel(const
         }
         for (int b = 0; b < 2; b++) {
             tc::mbar_init(accf + b, 1);
-            tc::mbar_init(acce + b, C::EW);
+            tc::mbar_init(acce + b, CG * C::EW);
         }
         tc::mbar_init(done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -359,12 +396,19 @@ __global__ void __launch_bounds__(PjCfg<BN, KIND>::THREADS, 1) proj_kernel(const
         *skip_slot = *(volatile int*)err;
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-                     ::"r"(tc::saddr(tmem_slot)), "r"(C::TMC));
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        if constexpr (CG == 2) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
+                         ::"r"(tc::saddr(tmem_slot)), "r"(C::TMC));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                         ::"r"(tc::saddr(tmem_slot)), "r"(C::TMC));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        }
     }
     tc::tc_before();
     __syncthreads();
+    if constexpr (CG == 2) tc::cluster_sync();  // both CTAs' barriers exist
     tc::tc_after();
     pdl_wait();  // everything before read only this kernel's arguments and the flag
     const uint32_t tmem = *tmem_slot;
@@ -378,7 +422,7 @@ __global__ void __launch_bounds__(PjCfg<BN, KIND>::THREADS, 1) proj_kernel(const
         int m0, n0, k0, k1, part;
     };
     auto tile_at = [&](int i) {
-        const int u = (int)blockIdx.x + i * (int)gridDim.x;
+        const int u = first + i * stride;
         Tile r;
         int t = u;
         r.k0 = 0;
@@ -389,11 +433,11 @@ __global__ void __launch_bounds__(PjCfg<BN, KIND>::THREADS, 1) proj_kernel(const
             t = a.full + j;
             r.k0 = (int)((int64_t)a.nk * z / a.S);
             r.k1 = (int)((int64_t)a.nk * (z + 1) / a.S);
-            r.part = (u - a.full) * 128;
+            r.part = ((u - a.full) * CG + rank) * 128;
         }
         const int per = PJ_GROUP_M * a.nt, g = t / per, rem = t - g * per;
         const int gm = min(PJ_GROUP_M, a.mt - g * PJ_GROUP_M);
-        r.m0 = (g * PJ_GROUP_M + rem % gm) * 128;
+        r.m0 = ((g * PJ_GROUP_M + rem % gm) * CG + rank) * 128;
         r.n0 = rem / gm * BN;
         return r;
     };
@@ -411,30 +455,45 @@ __global__ void __launch_bounds__(PjCfg<BN, KIND>::THREADS, 1) proj_kernel(const
                     }
                     unsigned char* sa = smem + s * C::STAGE;
                     unsigned char* sb = sa + C::A_BYTES;
-                    tc::mbar_expect_tx(full + s, C::STAGE);
+                    const uint32_t bar = lead(full + s);
+                    if (rank == 0) tc::mbar_expect_tx(full + s, CG * C::STAGE);
+                    auto load = [&](void* dst, const CUtensorMap* map, int x, int y) {
+                        if constexpr (CG == 2) tc::tma_2d_pair(dst, map, bar, x, y);
+                        else tc::tma_2d(dst, map, full + s, x, y);
+                    };
+                    const int nb = t.n0 + rank * (BN / CG);
                     if constexpr (AMN) {
-                        tc::tma_2d(sa, &a.amap, full + s, t.m0, ks * PJ_BK);
-                        tc::tma_2d(sa + 8192, &a.amap, full + s, t.m0 + 64, ks * PJ_BK);
+                        load(sa, &a.amap, t.m0, ks * PJ_BK);
+                        load(sa + 8192, &a.amap, t.m0 + 64, ks * PJ_BK);
                     } else {
-                        tc::tma_2d(sa, &a.amap, full + s, ks * PJ_BK, t.m0);
+                        load(sa, &a.amap, ks * PJ_BK, t.m0);
                     }
                     if constexpr (BMN) {
 #pragma unroll
-                        for (int c = 0; c < BN / 64; c++)
-                            tc::tma_2d(sb + c * 8192, &a.bmap, full + s, t.n0 + 64 * c, ks * PJ_BK);
+                        for (int c = 0; c < BN / CG / 64; c++) load(sb + c * 8192, &a.bmap, nb + 64 * c, ks * PJ_BK);
                     } else {
-                        tc::tma_2d(sb, &a.bmap, full + s, ks * PJ_BK, t.n0);
+                        load(sb, &a.bmap, ks * PJ_BK, nb);
                     }
                 }
             }
-            // the copies issued here land before the CTA may exit
-            for (int j = max(0, g - ST); j < g; j++)
-                if (!tc::mbar_wait_own(full + (j % ST), (j / ST) & 1, err)) ok = false;
+            // the copies issued here land before the CTA may exit (a pair's second CTA
+            // counts them on the first's barriers: its own are done when every MMA is,
+            // and after a wait that gave up it allows them 2 ms)
+            if (rank == 0) {
+                for (int j = max(0, g - ST); j < g; j++)
+                    if (!tc::mbar_wait_own(full + (j % ST), (j / ST) & 1, err)) ok = false;
+            } else if (!ok) {
+                for (const uint64_t t0 = tc::gtime(); tc::gtime() - t0 < 2000000;) __nanosleep(1000);
+            }
         }
     } else if (warp == 1) {
-        if (lane == 0) {  // ---- MMA issuer
+        if (lane == 0) {  // ---- MMA issuer (of a pair, the first CTA's)
+            auto commit = [&](uint64_t* bar) {
+                if constexpr (CG == 2) tc::umma_commit_pair(bar);
+                else tc::umma_commit(bar);
+            };
             int g = 0;
-            for (int i = 0; i < tiles && ok; i++) {
+            for (int i = 0; i < tiles && ok && rank == 0; i++) {
                 const Tile t = tile_at(i);
                 const int b = i & 1;
                 if (i >= 2 && !tc::mbar_wait(acce + b, ((i >> 1) - 1) & 1, err)) {
@@ -455,15 +514,18 @@ __global__ void __launch_bounds__(PjCfg<BN, KIND>::THREADS, 1) proj_kernel(const
                     for (int kk = 0; kk < 4; kk++) {
                         const uint64_t ad = AMN ? tc::mn_sw128_desc(sa + kk * 2048, 8192) : tc::sw128_desc(sa) + 2 * kk;
                         const uint64_t bd = BMN ? tc::mn_sw128_desc(sb + kk * 2048, 8192) : tc::sw128_desc(sb) + 2 * kk;
-                        tc::umma_ss(d, ad, bd, a.idesc, (ks > t.k0 || kk) ? 1u : 0u);
+                        if constexpr (CG == 2) tc::umma_ss_pair(d, ad, bd, a.idesc, (ks > t.k0 || kk) ? 1u : 0u);
+                        else tc::umma_ss(d, ad, bd, a.idesc, (ks > t.k0 || kk) ? 1u : 0u);
                     }
-                    tc::umma_commit(empty + s);
+                    commit(empty + s);
                 }
                 if (!ok) break;
-                tc::umma_commit(accf + b);
+                commit(accf + b);
             }
-            tc::umma_commit(done);  // also after an early exit: TMEM is freed after the MMAs
-            if (!tc::mbar_wait_own(done, 0, err)) ok = false;
+            if (rank == 0) {
+                commit(done);  // also after an early exit: TMEM is freed after the MMAs
+                if (!tc::mbar_wait_own(done, 0, err)) ok = false;
+            }
         }
     } else {
         // ---- epilogue
@@ -576,7 +638,10 @@ __global__ void __launch_bounds__(PjCfg<BN, KIND>::THREADS, 1) proj_kernel(const
             }
             tc::tc_before();
             __syncwarp();
-            if (lane == 0) tc::mbar_arrive(acce + b);
+            if (lane == 0) {
+                if constexpr (CG == 2) tc::mbar_arrive_cluster(lead(acce + b));
+                else tc::mbar_arrive(acce + b);
+            }
             if (KIND == PJ_FWD_CK && epi && row < a.M && c0 < c1) {
                 // the exponents of this warp's groups, together where they are a word
                 uint8_t* p = a.e.exps + proj_group(row, t.n0 + c0, a.N);
@@ -592,9 +657,18 @@ __global__ void __launch_bounds__(PjCfg<BN, KIND>::THREADS, 1) proj_kernel(const
     }
     tc::tc_before();
     const int bad = __syncthreads_or(!ok && (warp >= 2 || lane == 0));
+    if constexpr (CG == 2) {
+        // the second CTA's epilogue has seen its last tile: the MMAs are as good as done
+        if (rank == 1 && warp == 1 && lane == 0) tc::mbar_wait_own(done, 0, err);
+        __syncwarp();
+        tc::cluster_sync();  // neither CTA's memory is in use by the other
+    }
     if (warp == 1) {
         tc::tc_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMC));
+        if constexpr (CG == 2)
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMC));
+        else
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMC));
     }
     if (tid == 0 && bad) {
         *(volatile int*)a.err_host = 1;
@@ -603,10 +677,10 @@ __global__ void __launch_bounds__(PjCfg<BN, KIND>::THREADS, 1) proj_kernel(const
 }
 
 struct ProjJoin {
-    const float* part;  // [(tile - full) S + split][128][BN]
+    const float* part;  // [(tile - full) S + split][BM][BN]
     ProjEpi e;
     void* d;
-    int M, N, mt, nt, full, S, BN;
+    int M, N, mt, nt, full, S, BM, BN;
 };
 // Joins the splits of the tiles full ..: thread i takes 8 columns of a row of a
 // tile (four neighbouring lanes hold a checkpoint group), the splits' loads all in
@@ -614,22 +688,22 @@ struct ProjJoin {
 template <int KIND>
 __device__ __forceinline__ void proj_join(const ProjJoin& a, int64_t i) {
     const int per = a.BN / 8;
-    const int piece = (int)(i % per), r = (int)(i / per % 128);
-    const int64_t j = i / per / 128;
+    const int piece = (int)(i % per), r = (int)(i / per % a.BM);
+    const int64_t j = i / per / a.BM;
     const int t = a.full + (int)j;  // the grid covers whole tiles
     const int pg = PJ_GROUP_M * a.nt, g = t / pg, rem = t - g * pg;
     const int gm = min(PJ_GROUP_M, a.mt - g * PJ_GROUP_M);
-    const int64_t row = (g * PJ_GROUP_M + rem % gm) * 128 + r;
+    const int64_t row = (int64_t)(g * PJ_GROUP_M + rem % gm) * a.BM + r;
     const int col = rem / gm * a.BN + 8 * piece;
     const bool in = row < a.M && col < a.N;
     if (__all_sync(0xffffffffu, !in)) return;
     const int64_t at = row * a.N + col;
     float v[8] = {};
-    const float* p = a.part + (j * a.S * 128 + r) * a.BN + 8 * piece;
+    const float* p = a.part + (j * a.S * a.BM + r) * a.BN + 8 * piece;
     if (in) {
 #pragma unroll 8
         for (int z = 0; z < a.S; z++) {
-            const float4* q = reinterpret_cast<const float4*>(p + (int64_t)z * 128 * a.BN);
+            const float4* q = reinterpret_cast<const float4*>(p + (int64_t)z * a.BM * a.BN);
             const float4 x = q[0], y = q[1];
             v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
             v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
@@ -706,38 +780,43 @@ __global__ void __launch_bounds__(PJ_JOIN_T) proj_join_kernel(const ProjJoin a, 
 
 // ------------------------------------------------------------------ host side
 
-// Tile width, whole tiles and splits of the others for an M x N product, from the
-// sizes alone (the workspace query has to agree with the call).
-//  - Tiles of 256 columns where they fill the SMs; of 128 for products too short
-//    to hide a wide tile's epilogue (K <= 512: 4093 x 2048 over 96 with a sigmoid
-//    takes __ us in 128s, 27.5 in 256s) and where they give more SMs work.
+// Tile, whole tiles and splits of the others for an M x N product, from the sizes
+// alone (the workspace query has to agree with the call).
+//  - 256 x 256 on a pair of CTAs where such tiles fill the pairs: half the shared
+//    memory traffic per product of 128 x 256 on one CTA (dX 8192 x 8192 over 2048
+//    186 us against 204, dW 2048 x 8192 over 8192 165 against 190).
+//  - 128 x 128 otherwise, and for products too short to hide a wide tile's epilogue
+//    (K <= 512).
 //  - The tiles past the last whole wave are split the way that the estimate below
-//    finds shortest: a stage of 64 takes 0.4 us on a 256-wide tile and 0.27 on a
-//    128-wide one (an SM's share of L2 bandwidth); joining takes 3.5 us and writes
-//    and reads each split's tile once in L2 (8 TB/s).
+//    finds shortest: a stage of 64 takes 0.45 us on a pair and 0.27 us on a CTA (an SM's
+//    share of L2 bandwidth); joining takes 3.5 us and writes and reads each split's
+//    tile once in L2 (8 TB/s).
 struct ProjPlan {
-    int BN, mt, nt, full, S;
+    int CG, BN, mt, nt, full, S;
     int64_t ws_bytes;  // the splits' tiles
+    int BM() const { return 128 * CG; }
 };
 inline ProjPlan proj_plan(int64_t M, int64_t N, int64_t K) {
     ProjPlan p{};
     const int nk = (int)((K + PJ_BK - 1) / PJ_BK);
-    p.mt = (int)((M + 127) / 128);
-    p.BN = K > 512 && (int64_t)p.mt * ((N + 255) / 256) >= PJ_SMS ? 256 : 128;
+    const bool pair = K > 512 && (M + 255) / 256 * ((N + 255) / 256) >= PJ_SMS / 2;
+    p.CG = pair ? 2 : 1;
+    p.BN = pair ? 256 : 128;
+    p.mt = (int)((M + p.BM() - 1) / p.BM());
     p.nt = (int)((N + p.BN - 1) / p.BN);
-    const int tiles = p.mt * p.nt, rem = tiles % PJ_SMS;
+    const int wave = PJ_SMS / p.CG, tiles = p.mt * p.nt, rem = tiles % wave;
     p.full = tiles - rem;
     p.S = 1;
     if (rem == 0) return p;
     double best = 0.0;
     for (int S = 1; S <= 16 && (S == 1 || nk / S >= 2); S++) {
-        const double stage = p.BN == 256 ? 0.4 : 0.27, bytes = 2.0 * rem * S * 128 * p.BN * 4;
-        const double us = (double)((rem * S + PJ_SMS - 1) / PJ_SMS) * ((nk + S - 1) / S) * stage +
+        const double stage = pair ? 0.45 : 0.27, bytes = 2.0 * rem * S * p.BM() * p.BN * 4;
+        const double us = (double)((rem * S + wave - 1) / wave) * ((nk + S - 1) / S) * stage +
                           (S > 1 ? 3.5 + bytes / 8e6 : 0.0);
         if (S == 1 || us < best) best = us, p.S = S;
     }
     if (p.S == 1) p.full = tiles;
-    else p.ws_bytes = (int64_t)rem * p.S * 128 * p.BN * 4;
+    else p.ws_bytes = (int64_t)rem * p.S * p.BM() * p.BN * 4;
     return p;
 }
 
@@ -753,17 +832,31 @@ inline bool proj_map_2d(CUtensorMap* m, CUtensorMapDataType type, int esize, con
                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int BN, bool AMN, bool BMN, int KIND>
+template <int BN, int CG, bool AMN, bool BMN, int KIND>
 inline cudaError_t proj_launch_t(const ProjArgs& a, int sm_count, bool after_own, cudaStream_t st) {
-    using C = PjCfg<BN, KIND>;
-    auto kern = proj_kernel<BN, AMN, BMN, KIND>;
+    using C = PjCfg<BN, CG, KIND>;
+    auto kern = proj_kernel<BN, CG, AMN, BMN, KIND>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::TOTAL);
     if (e != cudaSuccess) return e;
     const int units = a.full + (a.mt * a.nt - a.full) * a.S;
-    const dim3 grid(std::min(units, sm_count)), block(C::THREADS);
-    if (after_own) return launch_pdl(kern, grid, block, C::TOTAL, st, a);
-    kern<<<grid, block, C::TOTAL, st>>>(a);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(std::min(units, sm_count / CG) * CG);
+    cfg.blockDim = dim3(C::THREADS);
+    cfg.dynamicSmemBytes = C::TOTAL;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    cfg.attrs = at;
+    if (CG == 2) {
+        at[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        at[cfg.numAttrs].val.clusterDim.x = 2;
+        at[cfg.numAttrs].val.clusterDim.y = 1;
+        at[cfg.numAttrs++].val.clusterDim.z = 1;
+    }
+    if (after_own) {
+        at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    return cudaLaunchKernelEx(&cfg, kern, a);
 }
 
 // D [M, N] = epilogue(A B^T), A [M, K] (AMN: stored [K, M]), B [N, K] (BMN: stored
@@ -784,7 +877,7 @@ inline cudaError_t proj_gemm(const void* A, const void* B, void* D, int64_t M, i
     a.nt = p.nt;
     a.full = p.full;
     a.S = p.S;
-    a.idesc = tc::idesc_f16(128, p.BN, e.bf16 != 0) | (AMN ? 1u << 15 : 0u) | (BMN ? 1u << 16 : 0u);
+    a.idesc = tc::idesc_f16(p.BM(), p.BN, e.bf16 != 0) | (AMN ? 1u << 15 : 0u) | (BMN ? 1u << 16 : 0u);
     a.err = err;
     a.err_host = err_host;
     const int rem = p.mt * p.nt - p.full;
@@ -793,21 +886,21 @@ inline cudaError_t proj_gemm(const void* A, const void* B, void* D, int64_t M, i
     bool ok = AMN ? proj_map_2d(&a.amap, t16, 2, A, M, K, 64, PJ_BK, sw128)
                   : proj_map_2d(&a.amap, t16, 2, A, K, M, PJ_BK, 128, sw128);
     ok = ok && (BMN ? proj_map_2d(&a.bmap, t16, 2, B, N, K, 64, PJ_BK, sw128)
-                    : proj_map_2d(&a.bmap, t16, 2, B, K, N, PJ_BK, p.BN, sw128));
+                    : proj_map_2d(&a.bmap, t16, 2, B, K, N, PJ_BK, 128, sw128));
     ok = ok && (e.out_f32 ? proj_map_2d(&a.dmap, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, D, N, M, 16, 32, CU_TENSOR_MAP_SWIZZLE_64B)
                           : proj_map_2d(&a.dmap, t16, 2, D, N, M, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B));
     a.ctma = KIND == PJ_FWD_CK && N % 16 == 0;
     if (a.ctma)
         ok = ok && proj_map_2d(&a.cmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, e.codes, N, M, 32, 32, CU_TENSOR_MAP_SWIZZLE_NONE);
     if (p.S > 1)
-        ok = ok && proj_map_2d(&a.pmap, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, ws, p.BN, (int64_t)rem * p.S * 128, 16, 32,
+        ok = ok && proj_map_2d(&a.pmap, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, ws, p.BN, (int64_t)rem * p.S * p.BM(), 16, 32,
                                CU_TENSOR_MAP_SWIZZLE_64B);
     if (!ok) return cudaErrorInvalidValue;
-    const cudaError_t rc = p.BN == 128 ? proj_launch_t<128, AMN, BMN, KIND>(a, sm_count, after_own, st)
-                                       : proj_launch_t<256, AMN, BMN, KIND>(a, sm_count, after_own, st);
+    const cudaError_t rc = p.CG == 2 ? proj_launch_t<256, 2, AMN, BMN, KIND>(a, sm_count, after_own, st)
+                                     : proj_launch_t<128, 1, AMN, BMN, KIND>(a, sm_count, after_own, st);
     if (rc != cudaSuccess || (p.S == 1 && !cols)) return rc;
-    const ProjJoin j{ws, e, D, (int)M, (int)N, p.mt, p.nt, p.full, p.S, p.BN};
-    const int first = p.S > 1 ? ceil_div((int64_t)rem * 128 * (p.BN / 8), PJ_JOIN_T) : 0;
+    const ProjJoin j{ws, e, D, (int)M, (int)N, p.mt, p.nt, p.full, p.S, p.BM(), p.BN};
+    const int first = p.S > 1 ? ceil_div((int64_t)rem * p.BM() * (p.BN / 8), PJ_JOIN_T) : 0;
     const ColJoin c = cols ? *cols : ColJoin{};
     return launch_pdl(proj_join_kernel<KIND>, dim3(first + ceil_div(c.N, 32)), dim3(PJ_JOIN_T), 0, st, j, c, first);
 }

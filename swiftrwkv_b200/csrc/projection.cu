@@ -127,7 +127,8 @@ int check_common(int dtype, int rows, int OUT, int IN, const char* fn) {
                  IN);
     RWKV_REQUIRE(IN % 8 == 0 && OUT % 8 == 0, RWKV_E_UNSUPPORTED, "%s: IN=%d and OUT=%d must be multiples of 8", fn,
                  IN, OUT);
-    RWKV_REQUIRE(rows <= 1 << 26 && OUT <= 1 << 20 && IN <= 1 << 20 &&
+    // (a tile's sums take one bounded wait: 2^24 terms are 0.1 s)
+    RWKV_REQUIRE(rows <= 1 << 24 && OUT <= 1 << 20 && IN <= 1 << 20 &&
                      (int64_t)ceil_div(rows, 128) * ceil_div(std::max(OUT, IN), 64) < 1 << 30,
                  RWKV_E_SHAPE, "%s: rows=%d OUT=%d IN=%d too large", fn, rows, OUT, IN);
     return RWKV_OK;

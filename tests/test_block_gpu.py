@@ -718,3 +718,38 @@ def test_wait_errors_are_reported_by_the_projections(cuda):
     B.projectionBackwardInput(x, w)                       # skips its work: the device flag is set
     assert _lib.status("rwkv_q_gemm_status", torch.cuda.current_stream().cuda_stream) == _lib.E_TIMEOUT
     assert torch.equal(B.projectionForward(x, w)[0], want)
+
+
+@pytest.mark.parametrize("rows,OUT,IN", [(2304, 2304, 576), (2049, 2312, 1032), (4608, 1288, 520), (2500, 2048, 2048)])
+def test_products_large_enough_for_pairs_of_sms(cuda, rows, OUT, IN):
+    """Products that run on pairs of SMs (256 x 256 tiles, more than 512 terms),
+    whole and ragged, with every epilogue; dW sums over the rows."""
+    from swiftrwkv_b200 import block as B
+    t = torch.bfloat16
+    x, w, dy = rnd((rows, IN), 120, t), rnd((OUT, IN), 121, t, IN ** -0.5), rnd((rows, OUT), 122, t)
+    bias, res = rnd((OUT,), 123), rnd((rows, OUT), 124, t)
+    z0, s0 = proj_sums(x, w)
+    y, _ = B.projectionForward(x, w)
+    check(y, z0, TC * s0 + u(t) * (z0.abs() + TC * s0), "plain")
+    z, dz = z0 + bias.double(), TC * (s0 + bias.double().abs())
+    y, ck = B.projectionForward(x, w, bias, "relu2", res, checkpoint=True)
+    want = act64(z, "relu2") + res.double()
+    tol = slope(z, "relu2", dz) + 32 * U32 * (act64(z, "relu2").abs() + want.abs())
+    check(y, want, tol + u(t) * (want.abs() + tol), "relu2")
+    v = B.checkpoint8Values(ck, dtype=torch.float32)
+    check(v, z, (top_of_group(z) + top_of_group(dz)) / 127.5 + top_of_group(dz), "checkpoint")
+    f, _ = B.projectionForward(x, w, residual=res.float(), out_dtype=torch.float32)
+    check(f, z0 + res.double(), TC * s0 + 4 * U32 * (z0.abs() + res.double().abs()), "fp32 out")
+    ckx = B.checkpoint8(x)
+    g, s = proj_sums(dy, w.t())
+    d = grad64(values64(x), "relu2")
+    got = B.projectionBackwardInput(dy, w, pre=ckx, act="relu2", addend=x)
+    want = g * d + x.double()
+    tol = TC * s * d.abs() + 64 * U32 * ((g * d).abs() + want.abs())
+    check(got, want, tol + u(t) * (want.abs() + tol), "dx")
+    want, s = proj_sums(dy.t(), values64(x).t())
+    f, db = B.projectionBackwardWeight(dy, ckx, bias=True, out_dtype=torch.float32)
+    check(f, want, TC * s + U32 * want.abs(), "dw")
+    check(db, dy.double().sum(0), (rows + 16) * U32 * dy.double().abs().sum(0) + 1e-38, "db")
+    again, _ = B.projectionBackwardWeight(dy, ckx, out_dtype=torch.float32)
+    assert torch.equal(again, f)
