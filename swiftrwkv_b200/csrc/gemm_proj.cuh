@@ -751,12 +751,14 @@ __device__ __forceinline__ void proj_join(const ProjJoin& a, int64_t i) {
         *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.d) + at) = pack8_16(v, a.e.bf16);
     }
 }
-// Column sums of dY, joined beside the tiles (rwkv_projection_dw's db): blocks from
-// `first` on take 32 columns each, warp w the slices w, w + 4, ...; fixed order.
+// Column sums of dY beside the joined tiles (rwkv_projection_dw's db): blocks from
+// `first` on take 32 columns each, warp w the slices (or, of a short dY, its rows) w, w +
+// 4, ...; fixed order.
 struct ColJoin {
-    const float* part;  // [slices][N]
+    const float* part;  // [slices][N], or NULL:
+    const void* dy;     // [slices][N] in 16 bits, the rows themselves
     float* out;
-    int N, slices;
+    int N, slices, bf16;
 };
 constexpr int PJ_JOIN_T = 128;
 template <int KIND>
@@ -770,8 +772,14 @@ __global__ void __launch_bounds__(PJ_JOIN_T) proj_join_kernel(const ProjJoin a, 
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, col = ((int)blockIdx.x - first) * 32 + lane;
     float s = 0.f;
     if (col < c.N) {
+        if (c.part) {
 #pragma unroll 8
-        for (int k = w; k < c.slices; k += PJ_JOIN_T / 32) s += c.part[(int64_t)k * c.N + col];
+            for (int k = w; k < c.slices; k += PJ_JOIN_T / 32) s += c.part[(int64_t)k * c.N + col];
+        } else {
+#pragma unroll 8
+            for (int k = w; k < c.slices; k += PJ_JOIN_T / 32)
+                s += load_param(c.dy, c.bf16 ? RWKV_BF16 : RWKV_F16, (int64_t)k * c.N + col);
+        }
     }
     red[w][lane] = s;
     __syncthreads();

@@ -30,6 +30,7 @@ struct DwPrep {
     int first;
 };
 constexpr int PREP_T = 256, PREP_U = 4, CS_COLS = 256;
+constexpr int CS_DIRECT = 128;  // rows of dY summed without slices: 32 per warp, one launch less
 
 // FLAT: whole groups per row (IN % 32 == 0, or a dense x), nothing is divided.
 template <bool CK, bool FLAT>
@@ -282,13 +283,14 @@ extern "C" int rwkv_projection_dw(int dtype, const void* dy, int act, const void
     q.OUT = OUT;
     q.slices = p.slices;
     q.bf16 = dtype == RWKV_BF16;
-    q.first = db ? ceil_div(OUT, CS_COLS) * p.slices : 0;
+    const bool direct = rows <= CS_DIRECT;  // summed beside the join, from dY itself
+    q.first = db && !direct ? ceil_div(OUT, CS_COLS) * p.slices : 0;
     const int grid = q.first + (restore ? ceil_div(q.units, PREP_T * PREP_U) : 0);
     if (grid) {
         dw_prep_kernel<<<grid, PREP_T, 0, st>>>(q);
         if (int rc = check_launch("dw_prep_kernel")) return rc;
     }
-    const ColJoin cols{q.part, db, OUT, p.slices};
+    const ColJoin cols{direct ? nullptr : q.part, dy, db, OUT, direct ? rows : p.slices, q.bf16};
     cudaError_t rc;
     if (dw) {
         ProjEpi e{};
