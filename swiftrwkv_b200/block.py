@@ -171,7 +171,9 @@ def checkpoint8Values(ck: Checkpoint8, act: str = "none", dtype=None):
     a, dtype = _act(act), dtype or ck.dtype
     if dtype not in _DT:
         raise ValueError(f"checkpoint8Values: dtype {dtype} not taken")
-    codes = ck.codes
+    if not isinstance(ck, Checkpoint8):
+        raise ValueError("checkpoint8Values: a Checkpoint8 is needed")
+    codes = _some("ck.codes", ck.codes, (torch.int8,))
     dev, shape = codes.device, codes.shape
     _, codes, exps = _activation("ck", ck, dev, None, shape)
     out = torch.empty_like(codes, dtype=dtype)

@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(TPR, 1) ln_fwd_kernel(const LnFwdArgs a) {
     }
     float x[F32 ? R : 1][F32 ? NV : 1][VE];
     auto vec = [&](int r, int j) -> float* { return x[F32 ? r : 0][F32 ? j : 0]; };
-    float mean[R], rstd[R], shift[R];
+    float mean[R], rstd[R];
 #pragma unroll
     for (int r = 0; r < R; r++) {
         mean[r] = 0.f;
@@ -145,7 +145,6 @@ __global__ void __launch_bounds__(TPR, 1) ln_fwd_kernel(const LnFwdArgs a) {
 #pragma unroll
     for (int r = 0; r < R; r++) {
         rstd[r] = 1.f / sqrtf(rstd[r] / (float)a.D + a.eps);
-        shift[r] = -mean[r] * rstd[r];
         if (t == 0 && a.mean && row0 + r < a.rows) {
             a.mean[row0 + r] = mean[r];
             a.rstd[row0 + r] = rstd[r];
@@ -165,7 +164,7 @@ __global__ void __launch_bounds__(TPR, 1) ln_fwd_kernel(const LnFwdArgs a) {
                 if constexpr (!F32) Vec16<T>::unpack(raw[r][j], f);
                 float o[VE];
 #pragma unroll
-                for (int k = 0; k < VE; k++) o[k] = fmaf(fmaf(f[k], rstd[r], shift[r]), w[k], b[k]);
+                for (int k = 0; k < VE; k++) o[k] = fmaf((f[k] - mean[r]) * rstd[r], w[k], b[k]);
                 if (row0 + r < a.rows) __stcs(yr + (int64_t)r * nvec + j * TPR, Vec16<T>::pack(o));
             }
         }
@@ -443,19 +442,22 @@ __global__ void __launch_bounds__(MAXT, MINB) ln_bwd_kernel(const LnBwdArgs a) {
                 if (!exists(r0, r) || !has[j]) continue;
                 float dy[VE];
                 Vec16<T>::unpack(*slot(cur, r, 0, j), dy);
-                const float shift = -mean[r] * rstd[r];
-                float scale = rstd[r];
+                // x - mean in one rounding: no multiple of rstd cancels where |mean| is large
                 if constexpr (CK) {
                     const uint32_t* c = reinterpret_cast<const uint32_t*>(slot(cur, r, 1, j));
                     ck_codes4(c[0], h[r][j]);
                     if constexpr (VE == 8) ck_codes4(c[1], h[r][j] + 4);
-                    scale *= ck_scale(ex[r][j]);
+                    const float s = ck_scale(ex[r][j]);
+#pragma unroll
+                    for (int k = 0; k < VE; k++) h[r][j][k] = fmaf(h[r][j][k], s, -mean[r]);
                 } else {
                     Vec16<T>::unpack(*slot(cur, r, 1, j), h[r][j]);
+#pragma unroll
+                    for (int k = 0; k < VE; k++) h[r][j][k] -= mean[r];
                 }
 #pragma unroll
                 for (int k = 0; k < VE; k++) {
-                    h[r][j][k] = fmaf(h[r][j][k], scale, shift);
+                    h[r][j][k] *= rstd[r];
                     const float g = dy[k] * w[j][k];
                     rs[2 * r] += g;
                     rs[2 * r + 1] = fmaf(g, h[r][j][k], rs[2 * r + 1]);

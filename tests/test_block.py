@@ -159,6 +159,13 @@ def test_python_refusals_come_before_any_launch():
         B.checkpoint8(x)
     with pytest.raises(ValueError, match="CUDA tensor"):
         B.projectionForward(x, torch.zeros(8, 64))
+    host = B.Checkpoint8(torch.zeros(4, 64, dtype=torch.int8), torch.ones(4, 2, dtype=torch.uint8), torch.bfloat16)
+    with pytest.raises(ValueError, match="CUDA tensor"):
+        B.checkpoint8Values(host)
+    with pytest.raises(ValueError, match="Checkpoint8"):
+        B.checkpoint8Values(x)
+    with pytest.raises(ValueError, match="CUDA tensor"):
+        B.layerNormBackward(x, host, torch.ones(64), torch.zeros(4), torch.ones(4))
     with pytest.raises(ValueError, match="activation"):
         B.activationBackward(x, x, "gelu")
     with pytest.raises(ValueError, match="activation"):

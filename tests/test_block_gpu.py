@@ -293,6 +293,28 @@ def test_layer_norm_constant_rows_and_nan(cuda):
     assert torch.isnan(dw).any()
 
 
+def test_layer_norm_far_from_zero(cuda):
+    """Rows whose mean is large against their spread: a constant row gives the
+    bias exactly, also at 1000 (its mean is exact, x - mean is 0), and its
+    gradient has no part along h; a row at 1000 with spread 1 keeps the accuracy
+    of the fp32 mean, 1000 2^-24 per rounding, 8 of them."""
+    from swiftrwkv_b200 import block as B
+    for D in (256, 2048, 2560, 100):
+        x = torch.full((4, D), 1000.0, device="cuda")
+        x[2:] += rnd((2, D), 130)
+        w, b, dy = rnd((D,), 131), rnd((D,), 132), rnd((4, D), 133)
+        y, mean, rstd, _ = B.layerNormForward(x, w, b)
+        assert torch.equal(mean[:2], x[:2, 0]) and torch.equal(y[:2], b.expand(2, D))
+        y64, m64, r64 = norm64(x, w, b, 1e-5)
+        tol = 8 * 1000 * U32 * (w.double().abs() * r64 + 1)
+        check(y[2:], y64[2:], (tol * (1 + (y64 - b.double()).abs()))[2:], "y")
+        dx, _, _ = B.layerNormBackward(dy, x, w, mean, rstd, params=False)
+        g = (dy * w).double()
+        want = rstd.double()[:2, None] * (g - g.mean(1, keepdim=True))[:2]
+        n = (D + 16) * U32
+        check(dx[:2], want, rstd.double()[:2, None] * n * (g.abs() + g.abs().mean(1, keepdim=True))[:2], "dx")
+
+
 def test_layer_norm_types_and_views(cuda):
     """Parameters in 16 bits, non-contiguous and misaligned inputs, leading
     dimensions, no rows."""
@@ -753,3 +775,79 @@ def test_products_large_enough_for_pairs_of_sms(cuda, rows, OUT, IN):
     check(db, dy.double().sum(0), (rows + 16) * U32 * dy.double().abs().sum(0) + 1e-38, "db")
     again, _ = B.projectionBackwardWeight(dy, ckx, out_dtype=torch.float32)
     assert torch.equal(again, f)
+
+
+def test_offsets_past_32_bits(cuda):
+    """Tensors of more than 2^31 elements: the last rows come out as they do
+    from a call on them alone (elementwise results and per-row statistics do not
+    depend on the other rows), and the projection's against 64 bits."""
+    from swiftrwkv_b200 import block as B
+    t, D = torch.bfloat16, 2048
+    rows = (1 << 31) // D + 1000
+    x = torch.empty(rows, D, device="cuda", dtype=t)
+    for i in range(0, rows, 1 << 18):
+        x[i:i + (1 << 18)].normal_()
+    tail = x[-300:].clone()
+    w, b = rnd((D,), 140), rnd((D,), 141)
+    y, mean, rstd, ck = B.layerNormForward(x, w, b, checkpoint=True)
+    y1, mean1, rstd1, ck1 = B.layerNormForward(tail, w, b, checkpoint=True)
+    assert torch.equal(y[-300:], y1) and torch.equal(mean[-300:], mean1) and torch.equal(rstd[-300:], rstd1)
+    assert torch.equal(ck.codes[-300:], ck1.codes) and torch.equal(ck.exps[-300:], ck1.exps)
+    v = B.checkpoint8Values(ck, "relu2")
+    assert torch.equal(v[-300:], B.checkpoint8Values(ck1, "relu2"))
+    del v
+    dz = B.activationBackward(x, ck, "tanh")
+    assert torch.equal(dz[-300:], B.activationBackward(tail, ck1, "tanh"))
+    del dz
+    dx, _, _ = B.layerNormBackward(x, ck, w, mean, rstd, dres=y)
+    assert torch.equal(dx[-300:], B.layerNormBackward(tail, ck1, w, mean1, rstd1, dres=y1)[0])
+    del dx, y
+    h, pw = rnd((rows, 64), 142, t), rnd((D, 64), 143, t, 0.125)
+    res = x
+    p, ckp = B.projectionForward(h, pw, act="relu2", residual=res, checkpoint=True)
+    z, s = proj_sums(h[-300:], pw)
+    want = act64(z, "relu2") + res[-300:].double()
+    tol = slope(z, "relu2", TC * s) + 32 * U32 * want.abs()
+    check(p[-300:], want, tol + u(t) * (want.abs() + tol), "projection")
+    last = B.Checkpoint8(ckp.codes[-300:], ckp.exps[-300:], t)
+    check(B.checkpoint8Values(last, dtype=torch.float32), z, (top_of_group(z) + top_of_group(TC * s)) / 127.5 +
+          top_of_group(TC * s), "checkpoint")
+    g = B.projectionBackwardInput(p, pw)
+    want, s = proj_sums(p[-300:], pw.t())
+    check(g[-300:], want, TC * s + u(t) * (want.abs() + TC * s), "dx")
+
+
+CAPTURE_FIRST = """
+import sys; sys.path.insert(0, {root!r})
+import torch
+from swiftrwkv_b200 import _lib, block as B
+x, w = torch.ones(32, 64, device="cuda", dtype=torch.bfloat16), torch.ones(64, 64, device="cuda", dtype=torch.bfloat16)
+g = torch.cuda.CUDAGraph()
+s = torch.cuda.Stream()
+seen = []
+with torch.cuda.stream(s):
+    g.capture_begin()
+    try:
+        B.projectionForward(x, w)
+    except _lib.RWKVError as e:
+        seen.append(str(e))
+    y = B.layerNormForward(x, w[0].float(), w[1].float())[0]   # needs nothing set up
+    g.capture_end()
+assert len(seen) == 1 and "before capturing" in seen[0], seen
+g.replay()
+torch.cuda.synchronize()
+assert bool((y == 1).all())
+assert float(B.projectionForward(x, w)[0][0, 0]) == 64.0
+print("ok")
+"""
+
+
+def test_a_first_projection_during_capture_is_refused(cuda):
+    """The wait-error record is not allocated while a stream is captured: the
+    call is refused, the capture itself goes on, and later calls work."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", CAPTURE_FIRST.format(root=root)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "ok" in r.stdout, r.stdout + r.stderr
