@@ -26,6 +26,7 @@ backward calls.
 from __future__ import annotations
 
 from dataclasses import dataclass
+from functools import lru_cache
 
 import torch
 
@@ -149,8 +150,13 @@ def _new_checkpoint(y, dtype):
                        y.new_empty((*lead, -(-D // CKPT_GROUP)), dtype=torch.uint8), dtype)
 
 
+@lru_cache(maxsize=4096)
+def _workspace_bytes(name, *sizes):
+    return int(getattr(_lib.lib(), name + "_workspace_size")(*sizes))
+
+
 def _workspace(nbytes, like):
-    return like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    return like.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
 
 
 # ------------------------------------------------------- 8-bit checkpoints
@@ -248,7 +254,7 @@ def layerNormBackward(dy, x, weight, mean, rstd, dres=None, params: bool = True)
     db = torch.empty_like(weight) if params else None
     if not rows:
         return dx, dw.zero_() if params else None, db.zero_() if params else None
-    n = _lib.lib().rwkv_layer_norm_backward_workspace_size(rows, D) if params else 0
+    n = _workspace_bytes("rwkv_layer_norm_backward", rows, D) if params else 0
     ws = _workspace(n, dy)
     _call(dev, "rwkv_layer_norm_backward", _DT[dt], dy.data_ptr(), _p(xt), _p(codes), _p(exps), _DT[weight.dtype],
           weight.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _p(dres), dx.data_ptr(), _p(dw), _p(db), rows, D, _p(ws),
@@ -310,7 +316,7 @@ def projectionForward(x, w, bias=None, act: str = "none", residual=None, checkpo
         z = kept.data_ptr()
     rows = x.numel() // IN
     if rows:
-        n = _lib.lib().rwkv_projection_forward_workspace_size(rows, OUT, IN)
+        n = _workspace_bytes("rwkv_projection_forward", rows, OUT, IN)
         ws = _workspace(n, x)
         _call(dev, "rwkv_projection_forward", _DT[dt], x.data_ptr(), w.data_ptr(), bdt, _p(bias), a, _DT[ydt],
               _p(residual), y.data_ptr(), z, codes, exps, rows, OUT, IN, _p(ws), n)
@@ -343,7 +349,7 @@ def projectionBackwardInput(dy, w, pre=None, act: str = "none", addend=None, out
     dx = dy.new_empty(shape, dtype=xdt)
     rows = dy.numel() // OUT
     if rows:
-        n = _lib.lib().rwkv_projection_dx_workspace_size(rows, OUT, IN)
+        n = _workspace_bytes("rwkv_projection_dx", rows, OUT, IN)
         ws = _workspace(n, dy)
         _call(dev, "rwkv_projection_dx", _DT[dt], dy.data_ptr(), w.data_ptr(), a, _p(z), _p(codes), _p(exps), _DT[xdt],
               _p(addend), dx.data_ptr(), rows, OUT, IN, _p(ws), n)
@@ -377,7 +383,7 @@ def projectionBackwardWeight(dy, x, act: str = "none", bias: bool = False, out_d
     rows = dy.numel() // OUT
     if not rows:
         return dw if dw is None else dw.zero_(), db.zero_() if bias else None
-    n = _lib.lib().rwkv_projection_dw_workspace_size(rows, OUT, IN, int(codes is not None or a != 0))
+    n = _workspace_bytes("rwkv_projection_dw", rows, OUT, IN, int(codes is not None or a != 0))
     ws = _workspace(n, dy)
     _call(dev, "rwkv_projection_dw", _DT[dt], dy.data_ptr(), a, _p(xt), _p(codes), _p(exps), _DT[wdt], _p(dw), _p(db),
           rows, OUT, IN, _p(ws), n)
