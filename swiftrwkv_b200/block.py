@@ -36,6 +36,8 @@ from ._lib import ACTS, BF16, F16, F32
 _DT = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
 _HALF = (torch.bfloat16, torch.float16)
 CKPT_GROUP = 32  # channels per scale of a checkpoint
+_MAX = 2**31 - 1
+_MAX_WIDTH = 1 << 20  # of a projection
 
 
 @dataclass
@@ -111,6 +113,9 @@ def _tensor(name, t, dev=None, dtypes=None, shape=None):
 
 def _some(name, t, dtypes=None):
     """A call's first tensor [..., D], D >= 1, after its checks."""
+    # the entry points take ints, to which ctypes cuts what is longer
+    if isinstance(t, torch.Tensor) and t.numel() > _MAX and t.dim() and max(t.shape[-1], t.numel() // t.shape[-1]) > _MAX:
+        raise ValueError(f"{name} {tuple(t.shape)}: more than 2^31 - 1 rows or channels")
     t = _tensor(name, t, None, dtypes)
     if t.dim() < 1 or t.shape[-1] < 1:
         raise ValueError(f"{name} {tuple(t.shape)} must be [..., D] with D >= 1")
@@ -174,11 +179,11 @@ def checkpoint8(x) -> Checkpoint8:
 def checkpoint8Values(ck: Checkpoint8, act: str = "none", dtype=None):
     """What a checkpoint stands for, or the activation behind a checkpointed
     pre-activation: act(value) in `dtype` (default: the activation's own)."""
+    if not isinstance(ck, Checkpoint8):
+        raise ValueError("checkpoint8Values: a Checkpoint8 is needed")
     a, dtype = _act(act), dtype or ck.dtype
     if dtype not in _DT:
         raise ValueError(f"checkpoint8Values: dtype {dtype} not taken")
-    if not isinstance(ck, Checkpoint8):
-        raise ValueError("checkpoint8Values: a Checkpoint8 is needed")
     codes = _some("ck.codes", ck.codes, (torch.int8,))
     dev, shape = codes.device, codes.shape
     _, codes, exps = _activation("ck", ck, dev, None, shape)
@@ -268,8 +273,8 @@ def _weight(w, dev, dtype):
     w = _tensor("w", w, dev, (dtype,))
     if w.dim() != 2:
         raise ValueError(f"w {tuple(w.shape)} must be [OUT, IN]")
-    if w.shape[0] % 8 or w.shape[1] % 8 or not w.numel():
-        raise ValueError(f"w {tuple(w.shape)}: OUT and IN must be multiples of 8")
+    if w.shape[0] % 8 or w.shape[1] % 8 or not w.numel() or max(w.shape) > _MAX_WIDTH:
+        raise ValueError(f"w {tuple(w.shape)}: OUT and IN must be multiples of 8, at most 2^20")
     return _aligned(w)
 
 
@@ -368,11 +373,11 @@ def projectionBackwardWeight(dy, x, act: str = "none", bias: bool = False, out_d
     if x is None:
         if not bias or a:
             raise ValueError("projectionBackwardWeight: without x only db can be asked for")
-    elif len(x.shape) < 1:
-        raise ValueError("projectionBackwardWeight: x must be [..., IN]")
+    elif not isinstance(x, (torch.Tensor, Checkpoint8)) or len(x.shape) < 1:
+        raise ValueError("projectionBackwardWeight: x must be a tensor [..., IN] or the Checkpoint8 of one")
     OUT, IN = dy.shape[-1], 8 if x is None else x.shape[-1]
-    if OUT % 8 or IN % 8 or not IN:
-        raise ValueError(f"projectionBackwardWeight: OUT={OUT} and IN={IN} must be multiples of 8")
+    if OUT % 8 or IN % 8 or not IN or OUT > _MAX_WIDTH or IN > _MAX_WIDTH:
+        raise ValueError(f"projectionBackwardWeight: OUT={OUT} and IN={IN} must be multiples of 8, at most 2^20")
     wdt = _result_dtype("projectionBackwardWeight", out_dtype, dt)
     xt = codes = exps = dw = None
     if x is not None:

@@ -187,3 +187,51 @@ def test_workspace_sizes_hold_whole_tiles(rows, OUT, IN):
     for n in (L.rwkv_projection_forward_workspace_size(rows, OUT, IN), L.rwkv_projection_dx_workspace_size(rows, OUT, IN)):
         assert n % (128 * 128 * 4) == 0 and n // (128 * 128 * 4) != 1
     assert rows > 16 or L.rwkv_projection_forward_workspace_size(rows, OUT, IN) == 0
+
+
+def test_sizes_past_31_bits_are_refused():
+    """The entry points' sizes are ints, to which ctypes would cut 2^31 + 5 rows
+    silently.  The tensors here are one element seen many times."""
+    one = torch.zeros(1, 1, dtype=torch.bfloat16)
+    many, wide = one.expand((1 << 32) + 5, 1), one.expand(1, (1 << 32) + 8)
+    vec = torch.ones(1)
+    for x in (many, wide, many.view(2, -1, 1) if many.is_contiguous() else many[None]):
+        with pytest.raises(ValueError, match="rows or channels"):
+            B.checkpoint8(x)
+        with pytest.raises(ValueError, match="rows or channels"):
+            B.layerNormForward(x, vec, vec)
+        with pytest.raises(ValueError, match="rows or channels"):
+            B.layerNormBackward(x, x, vec, vec, vec)
+        with pytest.raises(ValueError, match="rows or channels"):
+            B.activationBackward(x, x, "tanh")
+        with pytest.raises(ValueError, match="rows or channels"):
+            B.projectionForward(x, one)
+        with pytest.raises(ValueError, match="rows or channels"):
+            B.projectionBackwardInput(x, one)
+        with pytest.raises(ValueError, match="rows or channels"):
+            B.projectionBackwardWeight(x, x)
+    codes = torch.zeros(1, 1, dtype=torch.int8).expand((1 << 31), 1)
+    with pytest.raises(ValueError, match="rows or channels"):
+        B.checkpoint8Values(B.Checkpoint8(codes, codes, torch.bfloat16))
+
+
+def test_projection_widths_past_the_limit_are_refused(monkeypatch):
+    monkeypatch.setattr(B, "_tensor", lambda name, t, *a, **k: t)  # a CPU tensor as far as the check that raises
+    one = torch.zeros(1, 1, dtype=torch.bfloat16)
+    x = one.expand(2, 8)
+    for w in (one.expand((1 << 20) + 8, 8), one.expand(8, (1 << 32) + 8)):
+        with pytest.raises(ValueError, match="at most 2\\^20"):
+            B._weight(w, w.device, torch.bfloat16)
+    with pytest.raises(ValueError, match="at most 2\\^20"):
+        B.projectionBackwardWeight(x, one.expand(2, (1 << 20) + 8))
+
+
+def test_what_is_no_tensor_is_refused(monkeypatch):
+    with pytest.raises(ValueError, match="Checkpoint8"):
+        B.checkpoint8Values(None)
+    for x in (None, [1.0], 3.0):
+        with pytest.raises(ValueError, match="CUDA tensor"):
+            B.checkpoint8(x)
+    monkeypatch.setattr(B, "_tensor", lambda name, t, *a, **k: t)
+    with pytest.raises(ValueError, match="Checkpoint8"):
+        B.projectionBackwardWeight(torch.zeros(4, 64, dtype=torch.bfloat16), [1.0])
