@@ -556,11 +556,12 @@ int rwkv_act_backward(int dtype, const void* dy, const void* z, const int8_t* co
  * gradients; x, w and dY in `dtype`, BF16 or F16 (both operands of a
  * tensor-core product in one type); accumulation in fp32, one rounding at the
  * store.  IN % 8 == 0 and OUT % 8 == 0, tensors 16-byte aligned (exps and db to
- * their element); rows in 1..2^24, IN and OUT up to 2^20.  tcgen05 tensor cores; these calls
- * share rwkv_q_gemm's wait-error record (rwkv_q_gemm_status), and a stream may
- * be captured once one call has run on its device.  `workspace`: device memory of
- * the matching _workspace_size bytes, 16-byte aligned (NULL when that is 0);
- * calls that may overlap on the GPU need one each.
+ * their element); rows in 1..2^24, IN and OUT up to 2^20.  tcgen05 tensor
+ * cores; these calls share rwkv_q_gemm's wait-error record
+ * (rwkv_q_gemm_status), and a stream may be captured once one call has run on
+ * its device.  `workspace`: device memory of the matching _workspace_size
+ * bytes, 16-byte aligned (NULL when that is 0); calls that may overlap on the
+ * GPU need one each.
  *
  * Forward: z = x W^T + bias, y = act(z) + residual.  bias (may be NULL): [OUT]
  * in bdtype; y in ydtype (dtype or F32); residual (may be NULL): [rows, OUT] in
@@ -582,9 +583,9 @@ int rwkv_projection_dx(int dtype, const void* dy, const void* w, int act, const 
                        const uint8_t* exps, int dxdtype, const void* addend, void* dx, int rows, int OUT, int IN,
                        void* workspace, int64_t workspace_bytes, rwkv_stream_t stream);
 /* dW [OUT, IN] = dY^T act(X) in dwdtype (dtype or F32), and db [OUT] = sum over
- * rows of dY, fp32; either may be NULL (without dW, X is not read).  X [rows, IN]: dense in dtype, or
- * codes / exps its 8-bit checkpoint.  act(X) is rounded to dtype, the type the
- * tensor cores take (a checkpoint's values are exact there, so only act !=
+ * rows of dY, fp32; either may be NULL (without dW, X is not read).  X [rows,
+ * IN]: dense in dtype, or codes / exps its 8-bit checkpoint.  act(X) is rounded
+ * to dtype, the type the tensor cores take (a checkpoint's values are exact there, so only act !=
  * RWKV_ACT_NONE rounds).  `restore` of the workspace query: nonzero when act !=
  * RWKV_ACT_NONE or X comes as a checkpoint. */
 int64_t rwkv_projection_dw_workspace_size(int rows, int OUT, int IN, int restore);

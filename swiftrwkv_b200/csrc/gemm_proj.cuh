@@ -34,7 +34,7 @@
 // Tiles are walked in groups of 8 row blocks, so that the CTAs at work at one
 // time share a few row blocks of A and a few of B in L2.
 //
-// Whole waves of tiles (148 at a time) run as they are; the tiles of the last,
+// Whole waves of tiles (148 at a time, 74 on pairs) run as they are; the tiles of the last,
 // partial wave are split S ways along K, so that the SMs left over share them
 // (a product of fewer tiles than SMs is all last wave).  A split writes its fp32
 // sums as a tile into the workspace, and the join kernel adds the splits in order

@@ -8,9 +8,9 @@
 //             dw = sum_n dy h, db = sum_n dy
 //
 // Both are bound by HBM: each element is read and written once, and a row stays
-// in registers between its passes.  Rows are read in 16-byte vectors; the raw
-// vectors are kept (half the registers of fp32 for 16-bit types) and unpacked
-// in each pass.
+// in registers between its passes.  Rows are read in 16-byte vectors.  The forward
+// keeps short rows in fp32 and long ones as read (half the registers for 16-bit
+// types), unpacked in each pass.
 #include <algorithm>
 #include <atomic>
 
@@ -64,10 +64,10 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
 }
 
 // A block of TPR threads takes R rows, at most NV vectors of a row per thread:
-// vector j of thread t is t + j TPR.  The R rows share the loads of weight and bias, which in fp32 are twice a bf16 row's own
-// bytes from L1.  Rows of at most 80 elements per thread are held in fp32,
-// longer ones as read.  WF32: weight and bias in fp32 (no branch between their
-// loads); CK: write the checkpoint.
+// vector j of thread t is t + j TPR.  The R rows share the loads of weight and
+// bias, which in fp32 are four times a bf16 row's own bytes from L1.  Up to 80
+// elements per thread are held in fp32, more as read.  WF32: weight and bias in
+// fp32 (no branch between their loads); CK: write the checkpoint.
 template <typename T, int TPR, int NV, int R, bool WF32, bool CK>
 __global__ void __launch_bounds__(TPR, 1) ln_fwd_kernel(const LnFwdArgs a) {
     constexpr int VE = Vec16<T>::N;
@@ -252,43 +252,38 @@ __global__ void __launch_bounds__(256) ln_fwd_long_kernel(const LnFwdArgs a) {
     }
 }
 
-template <typename T, int TPR, int NV, int R>
+template <typename T, int TPR, int NV, int R, bool CK>
 void launch_ln_fwd_t(const LnFwdArgs& a, cudaStream_t st) {
     const int grid = ceil_div(a.rows, R);
-    if (a.wdtype == RWKV_F32) {
-        if (a.codes) ln_fwd_kernel<T, TPR, NV, R, true, true><<<grid, TPR, 0, st>>>(a);
-        else ln_fwd_kernel<T, TPR, NV, R, true, false><<<grid, TPR, 0, st>>>(a);
-    } else {
-        if (a.codes) ln_fwd_kernel<T, TPR, NV, R, false, true><<<grid, TPR, 0, st>>>(a);
-        else ln_fwd_kernel<T, TPR, NV, R, false, false><<<grid, TPR, 0, st>>>(a);
-    }
+    if (a.wdtype == RWKV_F32) ln_fwd_kernel<T, TPR, NV, R, true, CK><<<grid, TPR, 0, st>>>(a);
+    else ln_fwd_kernel<T, TPR, NV, R, false, CK><<<grid, TPR, 0, st>>>(a);
 }
 
-template <typename T>
+template <typename T, bool CK>
 int launch_ln_fwd(const LnFwdArgs& a, bool vec, cudaStream_t st) {
     const int nvec = a.D / Vec16<T>::N;
     // Threads and vectors per thread by length, two rows at a time (16384 x
     // 2560 bf16: 36 us against 40 us one by one, 16384 x 1024: 16 against 19);
-    // with a checkpoint, above 256 vectors, one row (45 against 50 us), since the
+    // with a checkpoint, above 256 vectors, one row (44 against 50 us), since the
     // packing hides the parameters' loads and two rows leave fewer threads.  A
     // row's sums run the same way with and without a checkpoint.
-    const bool one = a.codes != nullptr;
+    constexpr int R = CK ? 1 : 2;
     if (vec && nvec <= 512 * 8) {
-        if (nvec <= 64) launch_ln_fwd_t<T, 64, 1, 2>(a, st);
-        else if (nvec <= 64 * 2) launch_ln_fwd_t<T, 64, 2, 2>(a, st);
-        else if (nvec <= 64 * 3) launch_ln_fwd_t<T, 64, 3, 2>(a, st);
-        else if (nvec <= 128 * 2) launch_ln_fwd_t<T, 128, 2, 2>(a, st);
-        else if (nvec <= 64 * 5) one ? launch_ln_fwd_t<T, 64, 5, 1>(a, st) : launch_ln_fwd_t<T, 64, 5, 2>(a, st);
-        else if (nvec <= 256 * 2) one ? launch_ln_fwd_t<T, 256, 2, 1>(a, st) : launch_ln_fwd_t<T, 256, 2, 2>(a, st);
-        else if (nvec <= 256 * 5) one ? launch_ln_fwd_t<T, 256, 5, 1>(a, st) : launch_ln_fwd_t<T, 256, 5, 2>(a, st);
-        else launch_ln_fwd_t<T, 512, 8, 1>(a, st);
+        if (nvec <= 64) launch_ln_fwd_t<T, 64, 1, 2, CK>(a, st);
+        else if (nvec <= 64 * 2) launch_ln_fwd_t<T, 64, 2, 2, CK>(a, st);
+        else if (nvec <= 64 * 3) launch_ln_fwd_t<T, 64, 3, 2, CK>(a, st);
+        else if (nvec <= 128 * 2) launch_ln_fwd_t<T, 128, 2, 2, CK>(a, st);
+        else if (nvec <= 64 * 5) launch_ln_fwd_t<T, 64, 5, R, CK>(a, st);
+        else if (nvec <= 256 * 2) launch_ln_fwd_t<T, 256, 2, R, CK>(a, st);
+        else if (nvec <= 256 * 5) launch_ln_fwd_t<T, 256, 5, R, CK>(a, st);
+        else launch_ln_fwd_t<T, 512, 8, 1, CK>(a, st);
     } else if (a.D <= 32 * 8) {
         ln_fwd_any_kernel<T, 32, 8><<<ceil_div(a.rows, 4), 128, 0, st>>>(a);
     } else if (a.D <= 512 * 20) {
         if (a.D <= 128 * 4) ln_fwd_any_kernel<T, 128, 4><<<a.rows, 128, 0, st>>>(a);
         else if (a.D <= 128 * 8) ln_fwd_any_kernel<T, 128, 8><<<a.rows, 128, 0, st>>>(a);
         else if (a.D <= 256 * 8) ln_fwd_any_kernel<T, 256, 8><<<a.rows, 256, 0, st>>>(a);
-        else if (a.D <= 512 * 6) ln_fwd_any_kernel<T, 512, 6><<<a.rows, 512, 0, st>>>(a);
+        else if (a.D <= 512 * 8) ln_fwd_any_kernel<T, 512, 8><<<a.rows, 512, 0, st>>>(a);
         else if (a.D <= 512 * 12) ln_fwd_any_kernel<T, 512, 12><<<a.rows, 512, 0, st>>>(a);
         else ln_fwd_any_kernel<T, 512, 20><<<a.rows, 512, 0, st>>>(a);
     } else {
@@ -711,7 +706,6 @@ int launch_ln_bwd(LnBwdArgs a, bool vec, void* dw, void* db, cudaStream_t st) {
         else if (a.D <= 256 * 4) ln_bwd_any_kernel<T, CK, 256, 4><<<blocks, 256, 0, st>>>(a);
         else if (a.D <= 512 * 3) ln_bwd_any_kernel<T, CK, 512, 3><<<blocks, 512, 0, st>>>(a);
         else if (a.D <= 512 * 4) ln_bwd_any_kernel<T, CK, 512, 4><<<blocks, 512, 0, st>>>(a);
-        else if (a.D <= 512 * 6) ln_bwd_any_kernel<T, CK, 512, 6><<<blocks, 512, 0, st>>>(a);
         else if (a.D <= 512 * 8) ln_bwd_any_kernel<T, CK, 512, 8><<<blocks, 512, 0, st>>>(a);
         else if (a.D <= 512 * 12) ln_bwd_any_kernel<T, CK, 512, 12><<<blocks, 512, 0, st>>>(a);
         else ln_bwd_any_kernel<T, CK, 512, 20><<<blocks, 512, 0, st>>>(a);
@@ -760,7 +754,10 @@ extern "C" int rwkv_layer_norm_forward(int dtype, const void* x, int wdtype, con
                  RWKV_E_UNSUPPORTED, "%s: a tensor is not aligned to its element type", fn);
     const LnFwdArgs a{x, weight, bias, y, mean, rstd, codes, exps, wdtype, rows, D, ceil_div(D, CK_GROUP), eps};
     const bool vec = D % 8 == 0 && al(x, 16) && al(y, 16) && al(codes, 8) && al(weight, 16) && al(bias, 16);
-    return dispatch_dtype(dtype, [&]<typename T>() { return launch_ln_fwd<T>(a, vec, (cudaStream_t)stream); });
+    return dispatch_dtype(dtype, [&]<typename T>() {
+        return codes ? launch_ln_fwd<T, true>(a, vec, (cudaStream_t)stream)
+                     : launch_ln_fwd<T, false>(a, vec, (cudaStream_t)stream);
+    });
 }
 
 extern "C" int64_t rwkv_layer_norm_backward_workspace_size(int rows, int D) {

@@ -255,6 +255,49 @@ def test_layer_norm_backward(cuda, dt, kept, rows, D):
     assert torch.equal(dx3, dx) and torch.equal(dw3, dw) and torch.equal(db3, db)   # deterministic
 
 
+# on both sides of each length at which the kernels change their threads or
+# their elements per thread: whole 16-byte vectors, and odd lengths
+NORM_EDGES = [248, 256, 264, 512, 520, 768, 776, 1024, 1032, 1280, 1288, 1536, 1544, 2048, 2056, 2568, 4096, 4104, 5128,
+              8192, 10248, 12288, 12296, 16392, 32768, 32776,
+              255, 257, 511, 513, 1023, 1025, 1537, 2047, 2049, 4095, 4097, 6143, 6145, 10239, 10241]
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("D", NORM_EDGES)
+def test_layer_norm_around_the_length_classes(cuda, dt, D):
+    test_layer_norm_forward(cuda, dt, 3, D)
+    for kept in (False, True):
+        test_layer_norm_backward(cuda, dt, kept, 3, D)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("D", [96, 250, 1003, 2056, 2560, 6001, 10241, 33000])
+def test_layer_norm_may_write_over_its_inputs(cuda, dt, D):
+    """y over x; dx over dy or dres (rwkv_cuda.h); more rows than resident blocks."""
+    from swiftrwkv_b200 import _lib, block as B
+    t, rows = DTYPES[dt], 1301
+    code, st = B._DT[t], torch.cuda.current_stream().cuda_stream
+    x, dy, dres = rnd((rows, D), 51, t), rnd((rows, D), 52, t), rnd((rows, D), 53, t)
+    w, b = rnd((D,), 54) * 0.2 + 1, rnd((D,), 55)
+    y, mean, rstd, ck = B.layerNormForward(x, w, b, checkpoint=True)
+    buf, codes, exps = x.clone(), torch.empty_like(ck.codes), torch.empty_like(ck.exps)
+    _lib.call("rwkv_layer_norm_forward", code, buf.data_ptr(), _lib.F32, w.data_ptr(), b.data_ptr(), 1e-5, buf.data_ptr(),
+              None, None, codes.data_ptr(), exps.data_ptr(), rows, D, st)
+    assert torch.equal(buf, y) and torch.equal(codes, ck.codes) and torch.equal(exps, ck.exps)
+    n = _lib.lib().rwkv_layer_norm_backward_workspace_size(rows, D)
+    ws = torch.empty(n, device="cuda", dtype=torch.uint8)
+    for kept in (False, True):
+        dx, dw, db = B.layerNormBackward(dy, ck if kept else x, w, mean, rstd, dres=dres)
+        for over in ("dy", "dres"):
+            a, r = dy.clone(), dres.clone()
+            out, gw, gb = a if over == "dy" else r, torch.empty_like(w), torch.empty_like(w)
+            _lib.call("rwkv_layer_norm_backward", code, a.data_ptr(), None if kept else x.data_ptr(),
+                      ck.codes.data_ptr() if kept else None, ck.exps.data_ptr() if kept else None, _lib.F32, w.data_ptr(),
+                      mean.data_ptr(), rstd.data_ptr(), r.data_ptr(), out.data_ptr(), gw.data_ptr(), gb.data_ptr(), rows, D,
+                      ws.data_ptr(), n, st)
+            assert torch.equal(out, dx) and torch.equal(gw, dw) and torch.equal(gb, db)
+
+
 def test_layer_norm_gradient_matches_differences(cuda):
     """The gradients against central differences of the forward in fp32: 1e-2
     of the largest gradient at a step of 2^-6 (the forward's own error,
