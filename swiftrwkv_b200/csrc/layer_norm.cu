@@ -691,13 +691,15 @@ int launch_ln_bwd(LnBwdArgs a, bool vec, void* dw, void* db, cudaStream_t st) {
     if (vec && nvec <= 512 * 3) {
         // vectors per thread: the fewest with at most 512 threads.  Two rows
         // at a time from a dense x (16384 x 2048 bf16: 50 us, one row 65 us), one
-        // from a checkpoint, whose decoding takes more registers; there up to 320
-        // threads with registers for two blocks per SM (54 us, unbounded 60 us; the
-        // dense kernel 62 us with that bound)
+        // from a checkpoint, whose decoding takes more registers (2560 channels: 68
+        // us, two rows 77).  Up to 320 threads with registers for two blocks per
+        // SM (2560 channels: dense 62 us, unbounded 72; 2048 from a checkpoint 54
+        // and 60; for three: 2560 from a checkpoint 87 us)
+        constexpr int R = CK ? 1 : 2;
         const cudaError_t e = nvec > 1024  ? launch_ln_bwd_t<T, CK, 3, 1>(a, &blocks, st)
                               : nvec > 512 ? launch_ln_bwd_t<T, CK, 2, 1>(a, &blocks, st)
-                              : CK && nvec <= 320 ? launch_ln_bwd_t<T, CK, 1, 1, 320, 2>(a, &blocks, st)
-                                           : launch_ln_bwd_t<T, CK, 1, CK ? 1 : 2>(a, &blocks, st);
+                              : nvec > 320 ? launch_ln_bwd_t<T, CK, 1, R>(a, &blocks, st)
+                                           : launch_ln_bwd_t<T, CK, 1, R, 320, 2>(a, &blocks, st);
         if (e != cudaSuccess) return fail(RWKV_E_CUDA, "ln_bwd_kernel: %s", cudaGetErrorString(e));
     } else if (a.D <= 512 * 20) {
         blocks = std::min(a.rows, LN_BWD_BLOCKS);
