@@ -334,11 +334,43 @@ __device__ __forceinline__ void copy_async(void* dst, const void* src) {
     if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src) : "memory");
     else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(d), "l"(src), "n"(BYTES) : "memory");
 }
+// the first n bytes, zeros behind them
+template <int BYTES>
+__device__ __forceinline__ void copy_async_n(void* dst, const void* src, int n) {
+    const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(n) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(d), "l"(src), "n"(BYTES), "r"(n) : "memory");
+}
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 constexpr int LN_STAGES = 3;
+
+// Rows of any length in aligned vectors.  Row r starts r D mod VE elements into a
+// 16-byte vector, so rows a multiple of VE apart start at the same place: a block
+// whose rows are has its columns fixed to its threads.  A row's vectors are those
+// that it touches; of the first `head` elements and of the last those from `tail` on
+// belong to other rows.  They are read as zeros and never written (the tensor's end
+// bounds the last vector, its 16-byte aligned start the first).
+template <typename T>
+__device__ __forceinline__ void drop_head(uint4& r, int head) {
+    uint32_t w[4] = {r.x, r.y, r.z, r.w};
+    constexpr int E = sizeof(T) == 2 ? 2 : 1;  // elements per word
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if (E * i + E <= head) w[i] = 0;
+        else if (E == 2 && E * i < head) w[i] &= 0xffff0000u;
+    }
+    r = make_uint4(w[0], w[1], w[2], w[3]);
+}
+// elements lo .. hi of a vector at p
+template <typename T>
+__device__ __forceinline__ void store_part(T* p, const float* v, int lo, int hi) {
+#pragma unroll
+    for (int k = 0; k < Vec16<T>::N; k++)
+        if (k >= lo && k < hi) p[k] = from_f<T>(v[k]);
+}
 
 // A block takes R rows at a time, R (blockIdx.x + i gridDim.x); thread t owns
 // the vectors t + j blockDim.x of every row, so its sums over rows of dy h and
@@ -347,26 +379,40 @@ constexpr int LN_STAGES = 3;
 // (cp.async) and reads only its own vectors, so the ring needs no barrier, and
 // HBM stays busy while the block computes and waits at its barrier: one per R
 // rows, for the two row sums (buffers alternating).
-template <typename T, bool CK, int NV, int R, int MAXT, int MINB>
+//
+// SH: rows that need not start on a vector, one at a time, gridDim.x a multiple of VE
+// (or no block with a second row).
+template <typename T, bool CK, int NV, int R, int MAXT, int MINB, bool SH>
 __global__ void __launch_bounds__(MAXT, MINB) ln_bwd_kernel(const LnBwdArgs a) {
     constexpr int VE = Vec16<T>::N;
+    static_assert(!SH || R == 1, "neighbouring rows start at different places");
     extern __shared__ uint4 ring[];  // [stage][row][dy | x | dres][NV][thread]
     __shared__ float red[2][16][2 * R];
     const int t = threadIdx.x, nt = blockDim.x, warp = t >> 5, lane = t & 31, nw = nt >> 5;
-    const int nvec = a.D / VE;
+    const int head = SH ? (int)((int64_t)blockIdx.x * a.D % VE) : 0;
+    const int nvec = (a.D + head + VE - 1) / VE;
     const float inv_d = 1.f / (float)a.D;
     float w[NV][VE], sw[NV][VE], sb[NV][VE];
     bool has[NV];
+    int tail[NV];                                                  // of each vector, VE in the row's midst
+    auto column = [&](int j) { return (t + j * nt) * VE - head; };  // of a vector's first element
 #pragma unroll
     for (int j = 0; j < NV; j++) {
         const int v = t + j * nt;
         has[j] = v < nvec;
+        tail[j] = SH ? min(VE, a.D - column(j)) : VE;
 #pragma unroll
         for (int k = 0; k < VE; k++) w[j][k] = sw[j][k] = sb[j][k] = 0.f;
-        if (has[j]) load_params<VE>(a.w, a.wdtype, (int64_t)v * VE, w[j]);
+        if constexpr (SH) {
+#pragma unroll
+            for (int k = 0; k < VE; k++)
+                if (has[j] && column(j) + k >= 0 && k < tail[j]) w[j][k] = load_param(a.w, a.wdtype, column(j) + k);
+        } else {
+            if (has[j]) load_params<VE>(a.w, a.wdtype, (int64_t)v * VE, w[j]);
+        }
     }
     const int step = (int)gridDim.x * R;
-    const int64_t vstep = (int64_t)step * nvec;  // in vectors
+    const int64_t vstep = SH ? (int64_t)step * a.D / VE : (int64_t)step * nvec;  // in vectors
     const uint4* const dy = static_cast<const uint4*>(a.dy) + t;
     const uint4* const xs = static_cast<const uint4*>(a.x) + t;
     const uint4* const dres = static_cast<const uint4*>(a.dres) + t;
@@ -385,10 +431,18 @@ __global__ void __launch_bounds__(MAXT, MINB) ln_bwd_kernel(const LnBwdArgs a) {
                 for (int j = 0; j < NV; j++)
                     if (exists(r0, r) && has[j]) {
                         const int64_t o = at + r * nvec + j * nt;
-                        copy_async<16>(slot(base, r, 0, j), dy + o);
-                        if constexpr (CK) copy_async<VE>(slot(base, r, 1, j), cs + o);
-                        else copy_async<16>(slot(base, r, 1, j), xs + o);
-                        if (a.dres) copy_async<16>(slot(base, r, 2, j), dres + o);
+                        if constexpr (SH) {
+                            const int n = tail[j] * (int)sizeof(T);
+                            copy_async_n<16>(slot(base, r, 0, j), dy + o, n);
+                            if constexpr (CK) copy_async_n<VE>(slot(base, r, 1, j), cs + o, tail[j]);
+                            else copy_async_n<16>(slot(base, r, 1, j), xs + o, n);
+                            if (a.dres) copy_async_n<16>(slot(base, r, 2, j), dres + o, n);
+                        } else {
+                            copy_async<16>(slot(base, r, 0, j), dy + o);
+                            if constexpr (CK) copy_async<VE>(slot(base, r, 1, j), cs + o);
+                            else copy_async<16>(slot(base, r, 1, j), xs + o);
+                            if (a.dres) copy_async<16>(slot(base, r, 2, j), dres + o);
+                        }
                     }
         }
         copy_commit();
@@ -404,13 +458,20 @@ __global__ void __launch_bounds__(MAXT, MINB) ln_bwd_kernel(const LnBwdArgs a) {
             nrstd[r] = a.rstd[row];
             if constexpr (CK) {
 #pragma unroll
-                for (int j = 0; j < NV; j++)
-                    nex[r][j] = has[j] ? a.exps[row * a.G + (t + j * nt) / (CK_GROUP / VE)] : 0u;
+                for (int j = 0; j < NV; j++) {
+                    if constexpr (SH) {  // a vector may lie in two groups
+                        const uint8_t* e = a.exps + row * a.G;
+                        const int c = column(j);
+                        nex[r][j] = has[j] ? e[max(c, 0) / CK_GROUP] | (uint32_t)e[min(c + VE, a.D) - 1 >> 5] << 8 : 0u;
+                    } else {
+                        nex[r][j] = has[j] ? a.exps[row * a.G + (t + j * nt) / (CK_GROUP / VE)] : 0u;
+                    }
+                }
             }
         }
     };
     const int64_t first = (int64_t)blockIdx.x * R;
-    int64_t at = first * nvec, fat = at;
+    int64_t at = SH ? first * a.D / VE : first * nvec, fat = at;
 #pragma unroll
     for (int i = 0; i < LN_STAGES - 1; i++, fat += vstep) fetch(first + (int64_t)i * step, fat, t + i * stage_n);
     fetch_small(first);
@@ -436,15 +497,28 @@ __global__ void __launch_bounds__(MAXT, MINB) ln_bwd_kernel(const LnBwdArgs a) {
             for (int j = 0; j < NV; j++) {
                 if (!exists(r0, r) || !has[j]) continue;
                 float dy[VE];
+                if constexpr (SH) {
+                    if (j == 0 && t == 0) {
+                        drop_head<T>(*slot(cur, r, 0, j), head);
+                        if constexpr (!CK) drop_head<T>(*slot(cur, r, 1, j), head);
+                    }
+                }
                 Vec16<T>::unpack(*slot(cur, r, 0, j), dy);
                 // x - mean in one rounding: no multiple of rstd cancels where |mean| is large
                 if constexpr (CK) {
                     const uint32_t* c = reinterpret_cast<const uint32_t*>(slot(cur, r, 1, j));
                     ck_codes4(c[0], h[r][j]);
                     if constexpr (VE == 8) ck_codes4(c[1], h[r][j] + 4);
-                    const float s = ck_scale(ex[r][j]);
+                    if constexpr (SH) {
+                        const float s0 = ck_scale(ex[r][j] & 255u), s1 = ck_scale(ex[r][j] >> 8);
+                        const int other = CK_GROUP - (max(column(j), 0) & (CK_GROUP - 1)) + (column(j) < 0 ? head : 0);
 #pragma unroll
-                    for (int k = 0; k < VE; k++) h[r][j][k] = fmaf(h[r][j][k], s, -mean[r]);
+                        for (int k = 0; k < VE; k++) h[r][j][k] = fmaf(h[r][j][k], k < other ? s0 : s1, -mean[r]);
+                    } else {
+                        const float s = ck_scale(ex[r][j]);
+#pragma unroll
+                        for (int k = 0; k < VE; k++) h[r][j][k] = fmaf(h[r][j][k], s, -mean[r]);
+                    }
                 } else {
                     Vec16<T>::unpack(*slot(cur, r, 1, j), h[r][j]);
 #pragma unroll
@@ -495,7 +569,10 @@ __global__ void __launch_bounds__(MAXT, MINB) ln_bwd_kernel(const LnBwdArgs a) {
                 }
 #pragma unroll
                 for (int k = 0; k < VE; k++) o[k] = fmaf(dy[k] * w[j][k], rstd[r], fmaf(h[r][j][k], c1, o[k]));
-                __stcs(static_cast<uint4*>(a.dx) + t + at + r * nvec + j * nt, Vec16<T>::pack(o));
+                uint4* out = static_cast<uint4*>(a.dx) + t + at + r * nvec + j * nt;
+                const int lo = j == 0 && t == 0 ? head : 0;
+                if (SH && (lo > 0 || tail[j] < VE)) store_part<T>(reinterpret_cast<T*>(out), o, lo, tail[j]);
+                else __stcs(out, Vec16<T>::pack(o));
             }
         }
         put = cur;
@@ -508,6 +585,15 @@ __global__ void __launch_bounds__(MAXT, MINB) ln_bwd_kernel(const LnBwdArgs a) {
     for (int j = 0; j < NV; j++) {
         const int v = t + j * nt;
         if (v >= nvec) continue;
+        if constexpr (SH) {
+#pragma unroll
+            for (int k = 0; k < VE; k++)
+                if (column(j) + k >= 0 && k < tail[j]) {
+                    p[column(j) + k] = sw[j][k];
+                    p[a.D + column(j) + k] = sb[j][k];
+                }
+            continue;
+        }
 #pragma unroll
         for (int k = 0; k < VE; k += 4) {
             *reinterpret_cast<float4*>(p + v * VE + k) = make_float4(sw[j][k], sw[j][k + 1], sw[j][k + 2], sw[j][k + 3]);
@@ -523,8 +609,10 @@ __device__ __forceinline__ float bwd_x(const LnBwdArgs& a, int64_t row, int i) {
     else return to_f<T>(static_cast<const T*>(a.x)[row * a.D + i]);
 }
 
-// Any alignment: a block per row at a time, single elements, element t + j NT of
-// thread t, at most NE; the sums over rows stay in registers.
+// Tensors off a 16-byte boundary, and rows of more vectors than ln_bwd_kernel
+// takes: a block per row at a time, single elements, element t + j NT of thread t,
+// at most NE; the sums over rows stay in registers (10326 x 2412 fp16: 220 us, in
+// vectors 54).
 template <typename T, bool CK, int NT, int NE>
 __global__ void __launch_bounds__(NT) ln_bwd_any_kernel(const LnBwdArgs a) {
     __shared__ float2 red[2][NT / 32];
@@ -663,10 +751,17 @@ __global__ void __launch_bounds__(1024) ln_bwd_params_kernel(const float* __rest
 
 constexpr int LN_BWD_BLOCKS = 148 * 4;  // at most: four resident blocks per SM
 
-template <typename T, bool CK, int NV, int R, int MAXT = 512, int MINB = 1>
+// vectors that a row of D elements touches at most
+template <typename T>
+int most_vectors(int D) {
+    return (int)(((int64_t)D + 2 * Vec16<T>::N - 2) / Vec16<T>::N);
+}
+
+template <typename T, bool CK, int NV, int R, int MAXT, int MINB, bool SH>
 cudaError_t launch_ln_bwd_t(const LnBwdArgs& a, int* blocks, cudaStream_t st) {
-    auto kern = ln_bwd_kernel<T, CK, NV, R, MAXT, MINB>;
-    const int nt = ceil_div(ceil_div(a.D / Vec16<T>::N, NV), 32) * 32;
+    auto kern = ln_bwd_kernel<T, CK, NV, R, MAXT, MINB, SH>;
+    constexpr int VE = Vec16<T>::N;
+    const int nt = ceil_div(ceil_div(SH ? most_vectors<T>(a.D) : a.D / VE, NV), 32) * 32;
     const int smem = LN_STAGES * R * 3 * NV * nt * 16;
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
@@ -679,14 +774,16 @@ cudaError_t launch_ln_bwd_t(const LnBwdArgs& a, int* blocks, cudaStream_t st) {
         per_sm = std::max(1, per_sm);
         resident[nt / 32].store(per_sm, std::memory_order_relaxed);
     }
-    *blocks = std::min({ceil_div(a.rows, R), 148 * per_sm, LN_BWD_BLOCKS});
+    const int most = std::min(148 * per_sm, LN_BWD_BLOCKS);
+    *blocks = std::min(ceil_div(a.rows, R), SH ? most / VE * VE : most);
     kern<<<*blocks, nt, smem, st>>>(a);
     return cudaGetLastError();
 }
 
-template <typename T, bool CK>
+// SH: lengths that are not a multiple of 8
+template <typename T, bool CK, bool SH>
 int launch_ln_bwd(LnBwdArgs a, bool vec, void* dw, void* db, cudaStream_t st) {
-    const int nvec = a.D / Vec16<T>::N;
+    const int nvec = SH ? most_vectors<T>(a.D) : a.D / Vec16<T>::N;
     int blocks;
     if (vec && nvec <= 512 * 3) {
         // vectors per thread: the fewest with at most 512 threads.  Two rows
@@ -695,11 +792,11 @@ int launch_ln_bwd(LnBwdArgs a, bool vec, void* dw, void* db, cudaStream_t st) {
         // us, two rows 77).  Up to 320 threads with registers for two blocks per
         // SM (2560 channels: dense 62 us, unbounded 72; 2048 from a checkpoint 54
         // and 60; for three: 2560 from a checkpoint 87 us)
-        constexpr int R = CK ? 1 : 2;
-        const cudaError_t e = nvec > 1024  ? launch_ln_bwd_t<T, CK, 3, 1>(a, &blocks, st)
-                              : nvec > 512 ? launch_ln_bwd_t<T, CK, 2, 1>(a, &blocks, st)
-                              : nvec > 320 ? launch_ln_bwd_t<T, CK, 1, R>(a, &blocks, st)
-                                           : launch_ln_bwd_t<T, CK, 1, R, 320, 2>(a, &blocks, st);
+        constexpr int R = CK || SH ? 1 : 2;
+        const cudaError_t e = nvec > 1024  ? launch_ln_bwd_t<T, CK, 3, 1, 512, 1, SH>(a, &blocks, st)
+                              : nvec > 512 ? launch_ln_bwd_t<T, CK, 2, 1, 512, 1, SH>(a, &blocks, st)
+                              : nvec > 320 ? launch_ln_bwd_t<T, CK, 1, R, 512, 1, SH>(a, &blocks, st)
+                                           : launch_ln_bwd_t<T, CK, 1, R, 320, 2, SH>(a, &blocks, st);
         if (e != cudaSuccess) return fail(RWKV_E_CUDA, "ln_bwd_kernel: %s", cudaGetErrorString(e));
     } else if (a.D <= 512 * 20) {
         blocks = std::min(a.rows, LN_BWD_BLOCKS);
@@ -790,10 +887,14 @@ extern "C" int rwkv_layer_norm_backward(int dtype, const void* dy, const void* x
     }
     const LnBwdArgs a{dy,   x,  codes, exps, weight, mean, rstd, dres, dx, dweight ? static_cast<float*>(workspace) : nullptr,
                       wdtype, rows, D, ceil_div(D, CK_GROUP)};
-    const bool vec =
-        D % 8 == 0 && al(dy, 16) && al(x, 16) && al(codes, 8) && al(dres, 16) && al(dx, 16) && al(weight, 16);
+    const bool whole = D % 8 == 0 && al(weight, 16);
+    const bool vec = al(dy, 16) && al(x, 16) && al(codes, 8) && al(dres, 16) && al(dx, 16);
     return dispatch_dtype(dtype, [&]<typename T>() {
-        return codes ? launch_ln_bwd<T, true>(a, vec, dweight, dbias, (cudaStream_t)stream)
-                     : launch_ln_bwd<T, false>(a, vec, dweight, dbias, (cudaStream_t)stream);
+        auto st = (cudaStream_t)stream;
+        if (whole)
+            return codes ? launch_ln_bwd<T, true, false>(a, vec, dweight, dbias, st)
+                         : launch_ln_bwd<T, false, false>(a, vec, dweight, dbias, st);
+        return codes ? launch_ln_bwd<T, true, true>(a, vec, dweight, dbias, st)
+                     : launch_ln_bwd<T, false, true>(a, vec, dweight, dbias, st);
     });
 }

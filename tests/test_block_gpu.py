@@ -298,6 +298,89 @@ def test_layer_norm_may_write_over_its_inputs(cuda, dt, D):
             assert torch.equal(out, dx) and torch.equal(gw, dw) and torch.equal(gb, db)
 
 
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,D", [(1301, 1003), (1301, 250), (1300, 1002), (999, 2412), (2500, 33), (700, 3001), (640, 8003)])
+def test_layer_norm_of_odd_lengths_and_many_rows(cuda, dt, rows, D):
+    """Rows that share a 16-byte vector with their neighbours, several per block."""
+    test_layer_norm_forward(cuda, dt, rows, D)
+    for kept in (False, True):
+        test_layer_norm_backward(cuda, dt, kept, rows, D)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("D", [9, 63, 1003, 2412, 5003])
+def test_layer_norm_rows_do_not_touch_their_neighbours(cuda, dt, D):
+    """Every third row NaN or infinite: the rows between give what they give alone;
+    and what lies behind the last row stays as it was."""
+    from swiftrwkv_b200 import _lib, block as B
+    t, rows = DTYPES[dt], 700
+    code, st = B._DT[t], torch.cuda.current_stream().cuda_stream
+    x, dy, dres = rnd((rows, D), 61, t), rnd((rows, D), 62, t), rnd((rows, D), 63, t)
+    w, b = rnd((D,), 64) * 0.2 + 1, rnd((D,), 65)
+    y, mean, rstd, ck = B.layerNormForward(x, w, b, checkpoint=True)
+    good = torch.arange(rows, device="cuda") % 3 != 1
+    bad_x, bad_dy, bad_dres = x.clone(), dy.clone(), dres.clone()
+    bad_x[1::6], bad_x[4::6] = float("nan"), float("inf")
+    bad_dy[1::3], bad_dres[1::3] = float("inf"), float("nan")
+    y2, mean2, rstd2, ck2 = B.layerNormForward(bad_x, w, b, checkpoint=True)
+    assert torch.equal(y2[good], y[good]) and torch.equal(mean2[good], mean[good]) and torch.equal(rstd2[good], rstd[good])
+    assert torch.equal(ck2.codes[good], ck.codes[good]) and torch.equal(ck2.exps[good], ck.exps[good])
+    assert bool((ck2.exps[~good] == 255).all()) and bool(torch.isnan(y2[~good]).all())
+    for kept in (False, True):
+        want = B.layerNormBackward(dy, ck if kept else x, w, mean, rstd, dres=dres, params=False)[0]
+        got = B.layerNormBackward(bad_dy, ck2 if kept else bad_x, w, mean2, rstd2, dres=bad_dres, params=False)[0]
+        assert torch.equal(got[good], want[good]) and bool(torch.isnan(got[~good]).all())
+    # outputs in the middle of larger buffers
+    n, pad = rows * D, 64
+    yb, xb = torch.full((n + pad,), 7.0, device="cuda", dtype=t), torch.full((n + pad,), 7.0, device="cuda", dtype=t)
+    cb = torch.full((n + pad,), 77, device="cuda", dtype=torch.int8)
+    eb = torch.full((ck.exps.numel() + pad,), 77, device="cuda", dtype=torch.uint8)
+    _lib.call("rwkv_layer_norm_forward", code, x.data_ptr(), _lib.F32, w.data_ptr(), b.data_ptr(), 1e-5, yb.data_ptr(),
+              None, None, cb.data_ptr(), eb.data_ptr(), rows, D, st)
+    _lib.call("rwkv_layer_norm_backward", code, dy.data_ptr(), x.data_ptr(), None, None, _lib.F32, w.data_ptr(),
+              mean.data_ptr(), rstd.data_ptr(), dres.data_ptr(), xb.data_ptr(), None, None, rows, D, None, 0, st)
+    assert torch.equal(yb[:n].view(rows, D), y) and bool((yb[n:] == 7).all())
+    assert torch.equal(cb[:n].view(rows, D), ck.codes) and bool((cb[n:] == 77).all())
+    assert torch.equal(eb[:ck.exps.numel()].view_as(ck.exps), ck.exps) and bool((eb[ck.exps.numel():] == 77).all())
+    assert torch.equal(xb[:n].view(rows, D), B.layerNormBackward(dy, x, w, mean, rstd, dres=dres, params=False)[0])
+    assert bool((xb[n:] == 7).all())
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_layer_norm_of_misaligned_rows(cuda, dt):
+    """Tensors that start off a 16-byte boundary give what aligned copies give, as
+    far as the order of sums allows."""
+    from swiftrwkv_b200 import block as B
+    t = DTYPES[dt]
+    for rows, D in ((9, 64), (700, 1003), (40, 2560), (5, 5003)):
+        buf = rnd((3, rows * D + 1), 66, t)
+        x, dy, dres = (buf[i, 1:].view(rows, D) for i in range(3))
+        assert x.data_ptr() % 16
+        w, b = rnd((D,), 67) * 0.2 + 1, rnd((D,), 68)
+        y, mean, rstd, ck = B.layerNormForward(x, w, b, checkpoint=True)
+        yc, mc, rc, cc = B.layerNormForward(x.clone(), w, b, checkpoint=True)
+        # the sums' orders differ by n 2^-24 of the sum of absolute terms each, carried
+        # through as in test_layer_norm_forward; twice, and a rounding to t on both sides
+        n = (D + 16) * U32
+        m64, r64 = norm64(x, w, b, 1e-5)[1:]
+        dm = n * x.double().abs().mean(-1, keepdim=True)
+        dev = (x.double() - m64).abs()
+        drel = 0.5 * ((2 * dev * dm + dm * dm).mean(-1, keepdim=True) + n * (dev ** 2).mean(-1, keepdim=True)) * r64 ** 2 * 1.01 + 8 * U32
+        tol = w.double().abs() * r64 * (dm + dev * (drel + 4 * U32)) + 2 * U32 * (yc.double().abs() + 2 * b.double().abs())
+        check(y, yc.double(), 2 * (tol * 1.01 + u(t) * (yc.double().abs() + tol)), "y")
+        assert torch.equal(ck.codes, cc.codes) and torch.equal(ck.exps, cc.exps)
+        dx, dw, db = B.layerNormBackward(dy, x, w, mc, rc, dres=dres)
+        m, r = mc.double()[:, None], rc.double()[:, None]
+        h, g = (x.double() - m) * r, dy.double() * w.double()
+        along, mg = (g * h).mean(1, keepdim=True), g.mean(1, keepdim=True)
+        want = r * (g - mg - h * along) + dres.double()
+        hd = 3 * U32 * r * (x.double().abs() + m.abs())
+        tol = r * (g.abs() * 4 * U32 + n * g.abs().mean(1, keepdim=True) +
+                   h.abs() * (n * (g * h).abs().mean(1, keepdim=True) + (g.abs() * hd).mean(1, keepdim=True)) +
+                   hd * along.abs()) + 8 * U32 * (r * (g.abs() + mg.abs() + (h * along).abs()) + dres.double().abs())
+        check(dx, want, tol * 1.01 + u(t) * (want.abs() + tol), "dx")
+
+
 def test_layer_norm_gradient_matches_differences(cuda):
     """The gradients against central differences of the forward in fp32: 1e-2
     of the largest gradient at a step of 2^-6 (the forward's own error,
