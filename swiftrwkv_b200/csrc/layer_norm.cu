@@ -19,6 +19,69 @@
 namespace rwkv {
 namespace {
 
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* dst, const void* src) {
+    const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(d), "l"(src), "n"(BYTES) : "memory");
+}
+// the first n bytes, zeros behind them
+template <int BYTES>
+__device__ __forceinline__ void copy_async_n(void* dst, const void* src, int n) {
+    const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+    if constexpr (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(n) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(d), "l"(src), "n"(BYTES), "r"(n) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+constexpr int LN_STAGES = 3;
+
+// Rows of any length in aligned vectors.  Row r starts r D mod VE elements into a
+// 16-byte vector, so rows a multiple of VE apart start at the same place: a block
+// whose rows are has its columns fixed to its threads.  A row's vectors are those
+// that it touches; of the first `head` elements and of the last those from `tail` on
+// belong to other rows.  They are read as zeros and never written (the tensor's end
+// bounds the last vector, its 16-byte aligned start the first).
+template <typename T>
+__device__ __forceinline__ void drop_head(uint4& r, int head) {
+    uint32_t w[4] = {r.x, r.y, r.z, r.w};
+    constexpr int E = sizeof(T) == 2 ? 2 : 1;  // elements per word
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if (E * i + E <= head) w[i] = 0;
+        else if (E == 2 && E * i < head) w[i] &= 0xffff0000u;
+    }
+    r = make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <typename T>
+__device__ __forceinline__ void drop_tail(uint4& r, int tail) {
+    uint32_t w[4] = {r.x, r.y, r.z, r.w};
+    constexpr int E = sizeof(T) == 2 ? 2 : 1;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if (E * i >= tail) w[i] = 0;
+        else if (E == 2 && E * i + 1 == tail) w[i] &= 0xffffu;
+    }
+    r = make_uint4(w[0], w[1], w[2], w[3]);
+}
+// elements lo .. hi of a vector at p
+template <typename T>
+__device__ __forceinline__ void store_part(T* p, const float* v, int lo, int hi) {
+#pragma unroll
+    for (int k = 0; k < Vec16<T>::N; k++)
+        if (k >= lo && k < hi) p[k] = from_f<T>(v[k]);
+}
+
+// vectors that a row of D elements touches at most
+template <typename T>
+int most_vectors(int D) {
+    return (int)(((int64_t)D + 2 * Vec16<T>::N - 2) / Vec16<T>::N);
+}
+
 // ------------------------------------------------------------------- forward
 
 struct LnFwdArgs {
@@ -171,8 +234,160 @@ __global__ void __launch_bounds__(TPR, 1) ln_fwd_kernel(const LnFwdArgs a) {
     }
 }
 
-// Any alignment: single elements, element j of thread t is t + j TPR (a warp's
-// 32 elements are a checkpoint group), at most NE per thread, in registers.
+// Rows that need not start on a vector: a block walks rows a multiple of VE apart,
+// so that its columns, and with them weight and bias, stay in registers; x runs
+// LN_STAGES - 1 rows ahead in a ring private to each thread.  A group of a
+// checkpoint ends inside a vector, so that the groups' largest |x| meet in shared
+// memory.  16384 x 2411 bf16: 60 us (single elements 144), with checkpoint 110
+// (190); bound by the step of a row (two barriers, two sums), whatever the number
+// of resident blocks.
+template <typename T, int NV, bool CK, int MAXT, int MINB>
+__global__ void __launch_bounds__(MAXT, MINB) ln_fwd_shift_kernel(const LnFwdArgs a) {
+    constexpr int VE = Vec16<T>::N, MAXG = 512 * 3 * 8 / CK_GROUP + 8;
+    extern __shared__ uint4 ring[];  // [stage][NV][thread]
+    __shared__ float red[2][16];
+    __shared__ uint32_t tops[CK ? 2 : 1][CK ? MAXG : 1];
+    const int t = threadIdx.x, nt = blockDim.x, warp = t >> 5, lane = t & 31, nw = nt >> 5;
+    const int head = (int)((int64_t)blockIdx.x * a.D % VE), nvec = (a.D + head + VE - 1) / VE;
+    auto column = [&](int j) { return (t + j * nt) * VE - head; };  // of a vector's first element
+    float w[NV][VE], b[NV][VE];
+    bool has[NV];
+    int tail[NV], lo[NV];  // its elements lo .. tail are the row's
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+        has[j] = t + j * nt < nvec;
+        tail[j] = min(VE, a.D - column(j));
+        lo[j] = max(0, -column(j));
+#pragma unroll
+        for (int k = 0; k < VE; k++) {
+            const bool in = has[j] && k >= lo[j] && k < tail[j];
+            w[j][k] = in ? load_param(a.w, a.wdtype, column(j) + k) : 0.f;
+            b[j][k] = in ? load_param(a.b, a.wdtype, column(j) + k) : 0.f;
+        }
+    }
+    if constexpr (CK)
+        for (int g = t; g < a.G; g += nt) tops[0][g] = tops[1][g] = 0;
+    const int64_t vstep = (int64_t)gridDim.x * a.D / VE;  // in vectors
+    int64_t at = (int64_t)blockIdx.x * a.D / VE, fat = at;
+    const uint4* const x = static_cast<const uint4*>(a.x) + t;
+    const int stage_n = NV * nt;
+    auto fetch = [&](int64_t row, int base) {
+        if (row < a.rows) {
+#pragma unroll
+            for (int j = 0; j < NV; j++)
+                if (has[j]) copy_async_n<16>(ring + base + j * nt, x + fat + j * nt, tail[j] * (int)sizeof(T));
+        }
+        copy_commit();
+        fat += vstep;
+    };
+#pragma unroll
+    for (int i = 0; i < LN_STAGES - 1; i++) fetch(blockIdx.x + (int64_t)i * gridDim.x, t + i * stage_n);
+    if constexpr (CK) __syncthreads();
+    // the block's sum of v over its threads, in every thread
+    auto total = [&](float v, float* r) {
+        v = warp_sum(v);
+        if (lane == 0) r[warp] = v;
+        __syncthreads();
+        return warp_sum(lane < nw ? r[lane] : 0.f);
+    };
+    int cur = t, put = t + (LN_STAGES - 1) * stage_n, buf = 0;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, at += vstep, buf ^= 1) {
+        fetch(row + (int64_t)(LN_STAGES - 1) * gridDim.x, put);
+        copy_wait<LN_STAGES - 1>();
+        uint4 raw[NV];
+        float s = 0.f;
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            raw[j] = has[j] ? ring[cur + j * nt] : make_uint4(0, 0, 0, 0);
+            if (j == 0 && t == 0) drop_head<T>(raw[j], head);
+            float f[VE];
+            Vec16<T>::unpack(raw[j], f);
+#pragma unroll
+            for (int k = 0; k < VE; k++) s += f[k];
+            if (CK && has[j]) {
+                const int c = max(column(j), 0), g = c / CK_GROUP, other = CK_GROUP - c % CK_GROUP + lo[j];
+                uint4 first = raw[j];
+                if (other < VE) {
+                    uint4 second = raw[j];
+                    drop_head<T>(second, other);
+                    drop_tail<T>(first, other);
+                    if (g + 1 < a.G) atomicMax(&tops[buf][g + 1], top_bits<T>(second));
+                }
+                atomicMax(&tops[buf][g], top_bits<T>(first));
+            }
+        }
+        const float mean = total(s, red[0]) / (float)a.D;
+        float q = 0.f;
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            float f[VE];
+            Vec16<T>::unpack(raw[j], f);
+#pragma unroll
+            for (int k = 0; k < VE; k++) {
+                const float d = has[j] && k >= lo[j] && k < tail[j] ? f[k] - mean : 0.f;
+                q = fmaf(d, d, q);
+            }
+        }
+        if constexpr (CK) {
+            // the groups' exponents, and the codes
+            for (int g = t; g < a.G; g += nt) {
+                a.exps[row * a.G + g] = (uint8_t)ck_exponent(top_f32<T>(tops[buf][g]));
+                tops[buf ^ 1][g] = 0;  // read before this row's first barrier, added to after its second
+            }
+#pragma unroll
+            for (int j = 0; j < NV; j++) {
+                if (!has[j]) continue;
+                const int c = max(column(j), 0), g = c / CK_GROUP, other = CK_GROUP - c % CK_GROUP + lo[j];
+                const float i0 = ck_inv_scale(ck_exponent(top_f32<T>(tops[buf][g])));
+                const float i1 = ck_inv_scale(ck_exponent(top_f32<T>(tops[buf][min(g + 1, a.G - 1)])));
+                float f[VE];
+                Vec16<T>::unpack(raw[j], f);
+                uint32_t q8[VE / 4];
+#pragma unroll
+                for (int i = 0; i < VE / 4; i++) {  // codes of either group, without a branch (a branch: 5 us more)
+                    const uint32_t p0 = ck_pack4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3], i0);
+                    const uint32_t p1 = ck_pack4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3], i1);
+                    const int n = min(max(other - 4 * i, 0), 4);
+                    const uint32_t m = n == 4 ? ~0u : (1u << 8 * n) - 1;
+                    q8[i] = (p0 & m) | (p1 & ~m);
+                }
+                int8_t* out = a.codes + VE * (at + t + j * nt);
+                if (lo[j] > 0 || tail[j] < VE) {
+#pragma unroll
+                    for (int k = 0; k < VE; k++)
+                        if (k >= lo[j] && k < tail[j]) out[k] = (int8_t)(q8[k / 4] >> 8 * (k % 4));
+                } else if constexpr (VE == 8) {
+                    *reinterpret_cast<uint2*>(out) = make_uint2(q8[0], q8[VE / 4 - 1]);
+                } else {
+                    *reinterpret_cast<uint32_t*>(out) = q8[0];
+                }
+            }
+        }
+        const float rstd = 1.f / sqrtf(total(q, red[1]) / (float)a.D + a.eps);
+        if (t == 0 && a.mean) {
+            a.mean[row] = mean;
+            a.rstd[row] = rstd;
+        }
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            if (!has[j]) continue;
+            float o[VE];
+            Vec16<T>::unpack(raw[j], o);
+#pragma unroll
+            for (int k = 0; k < VE; k++) o[k] = fmaf((o[k] - mean) * rstd, w[j][k], b[j][k]);
+            uint4* out = static_cast<uint4*>(a.y) + at + t + j * nt;
+            if (lo[j] > 0 || tail[j] < VE) store_part<T>(reinterpret_cast<T*>(out), o, lo[j], tail[j]);
+            else __stcs(out, Vec16<T>::pack(o));
+        }
+        put = cur;
+        cur = cur == t + (LN_STAGES - 1) * stage_n ? t : cur + stage_n;
+    }
+    copy_wait<0>();
+}
+
+// Tensors off a 16-byte boundary, short odd rows, and rows of more vectors than the
+// kernels above take: single elements, element j of thread t is t + j TPR (a warp's 32 elements
+// are a checkpoint group), at most NE per thread, in registers.
 template <typename T, int TPR, int NE>
 __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, 1) ln_fwd_any_kernel(const LnFwdArgs a) {
     __shared__ float red[32];
@@ -259,16 +474,39 @@ void launch_ln_fwd_t(const LnFwdArgs& a, cudaStream_t st) {
     else ln_fwd_kernel<T, TPR, NV, R, false, CK><<<grid, TPR, 0, st>>>(a);
 }
 
+template <typename T, int NV, bool CK, int MAXT, int MINB>
+cudaError_t launch_ln_fwd_shift(const LnFwdArgs& a, cudaStream_t st) {
+    auto kern = ln_fwd_shift_kernel<T, NV, CK, MAXT, MINB>;
+    constexpr int VE = Vec16<T>::N;
+    const int nt = ceil_div(ceil_div(most_vectors<T>(a.D), NV), 32) * 32;
+    const int smem = LN_STAGES * NV * nt * 16;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    static std::atomic<int> resident[17];  // by warps
+    int per_sm = resident[nt / 32].load(std::memory_order_relaxed);
+    if (per_sm == 0) {
+        const cudaError_t q = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, nt, smem);
+        if (q != cudaSuccess) return q;
+        per_sm = std::max(1, per_sm);
+        resident[nt / 32].store(per_sm, std::memory_order_relaxed);
+    }
+    kern<<<std::min(a.rows, 148 * per_sm / VE * VE), nt, smem, st>>>(a);
+    return cudaGetLastError();
+}
+
+// whole: rows of whole vectors, with weight and bias on 16-byte boundaries
 template <typename T, bool CK>
-int launch_ln_fwd(const LnFwdArgs& a, bool vec, cudaStream_t st) {
-    const int nvec = a.D / Vec16<T>::N;
+int launch_ln_fwd(const LnFwdArgs& a, bool vec, bool whole, cudaStream_t st) {
+    const int nvec = a.D / Vec16<T>::N, touched = most_vectors<T>(a.D);
     // Threads and vectors per thread by length, two rows at a time (16384 x
     // 2560 bf16: 36 us against 40 us one by one, 16384 x 1024: 16 against 19);
     // with a checkpoint, above 256 vectors, one row (44 against 50 us), since the
     // packing hides the parameters' loads and two rows leave fewer threads.  A
     // row's sums run the same way with and without a checkpoint.
     constexpr int R = CK ? 1 : 2;
-    if (vec && nvec <= 512 * 8) {
+    // Lengths that are not whole vectors take vectors too, above 256 elements; below, a
+    // warp per row of single elements is faster (16384 x 250 bf16: 9.5 against 14.7 us).
+    if (vec && whole && nvec <= 512 * 8) {
         if (nvec <= 64) launch_ln_fwd_t<T, 64, 1, 2, CK>(a, st);
         else if (nvec <= 64 * 2) launch_ln_fwd_t<T, 64, 2, 2, CK>(a, st);
         else if (nvec <= 64 * 3) launch_ln_fwd_t<T, 64, 3, 2, CK>(a, st);
@@ -277,6 +515,12 @@ int launch_ln_fwd(const LnFwdArgs& a, bool vec, cudaStream_t st) {
         else if (nvec <= 256 * 2) launch_ln_fwd_t<T, 256, 2, R, CK>(a, st);
         else if (nvec <= 256 * 5) launch_ln_fwd_t<T, 256, 5, R, CK>(a, st);
         else launch_ln_fwd_t<T, 512, 8, 1, CK>(a, st);
+    } else if (vec && !whole && a.D > 32 * 8 && touched <= 512 * 3) {
+        const cudaError_t e = touched > 1024  ? launch_ln_fwd_shift<T, 3, CK, 512, 1>(a, st)
+                              : touched > 512 ? launch_ln_fwd_shift<T, 2, CK, 512, 1>(a, st)
+                              : touched > 320 ? launch_ln_fwd_shift<T, 1, CK, 512, 1>(a, st)
+                                              : launch_ln_fwd_shift<T, 1, CK, 320, 2>(a, st);
+        if (e != cudaSuccess) return fail(RWKV_E_CUDA, "ln_fwd_shift_kernel: %s", cudaGetErrorString(e));
     } else if (a.D <= 32 * 8) {
         ln_fwd_any_kernel<T, 32, 8><<<ceil_div(a.rows, 4), 128, 0, st>>>(a);
     } else if (a.D <= 512 * 20) {
@@ -326,50 +570,6 @@ __device__ __forceinline__ float lanes_sum(float* v, int lane) {
 #pragma unroll
     for (int o = 16 / N; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     return s;
-}
-
-template <int BYTES>
-__device__ __forceinline__ void copy_async(void* dst, const void* src) {
-    const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
-    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(d), "l"(src), "n"(BYTES) : "memory");
-}
-// the first n bytes, zeros behind them
-template <int BYTES>
-__device__ __forceinline__ void copy_async_n(void* dst, const void* src, int n) {
-    const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
-    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(n) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(d), "l"(src), "n"(BYTES), "r"(n) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
-constexpr int LN_STAGES = 3;
-
-// Rows of any length in aligned vectors.  Row r starts r D mod VE elements into a
-// 16-byte vector, so rows a multiple of VE apart start at the same place: a block
-// whose rows are has its columns fixed to its threads.  A row's vectors are those
-// that it touches; of the first `head` elements and of the last those from `tail` on
-// belong to other rows.  They are read as zeros and never written (the tensor's end
-// bounds the last vector, its 16-byte aligned start the first).
-template <typename T>
-__device__ __forceinline__ void drop_head(uint4& r, int head) {
-    uint32_t w[4] = {r.x, r.y, r.z, r.w};
-    constexpr int E = sizeof(T) == 2 ? 2 : 1;  // elements per word
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        if (E * i + E <= head) w[i] = 0;
-        else if (E == 2 && E * i < head) w[i] &= 0xffff0000u;
-    }
-    r = make_uint4(w[0], w[1], w[2], w[3]);
-}
-// elements lo .. hi of a vector at p
-template <typename T>
-__device__ __forceinline__ void store_part(T* p, const float* v, int lo, int hi) {
-#pragma unroll
-    for (int k = 0; k < Vec16<T>::N; k++)
-        if (k >= lo && k < hi) p[k] = from_f<T>(v[k]);
 }
 
 // A block takes R rows at a time, R (blockIdx.x + i gridDim.x); thread t owns
@@ -751,12 +951,6 @@ __global__ void __launch_bounds__(1024) ln_bwd_params_kernel(const float* __rest
 
 constexpr int LN_BWD_BLOCKS = 148 * 4;  // at most: four resident blocks per SM
 
-// vectors that a row of D elements touches at most
-template <typename T>
-int most_vectors(int D) {
-    return (int)(((int64_t)D + 2 * Vec16<T>::N - 2) / Vec16<T>::N);
-}
-
 template <typename T, bool CK, int NV, int R, int MAXT, int MINB, bool SH>
 cudaError_t launch_ln_bwd_t(const LnBwdArgs& a, int* blocks, cudaStream_t st) {
     auto kern = ln_bwd_kernel<T, CK, NV, R, MAXT, MINB, SH>;
@@ -852,10 +1046,11 @@ extern "C" int rwkv_layer_norm_forward(int dtype, const void* x, int wdtype, con
                      al(mean, 4) && al(rstd, 4),
                  RWKV_E_UNSUPPORTED, "%s: a tensor is not aligned to its element type", fn);
     const LnFwdArgs a{x, weight, bias, y, mean, rstd, codes, exps, wdtype, rows, D, ceil_div(D, CK_GROUP), eps};
-    const bool vec = D % 8 == 0 && al(x, 16) && al(y, 16) && al(codes, 8) && al(weight, 16) && al(bias, 16);
+    const bool whole = D % 8 == 0 && al(weight, 16) && al(bias, 16);
+    const bool vec = al(x, 16) && al(y, 16) && al(codes, 8);
     return dispatch_dtype(dtype, [&]<typename T>() {
-        return codes ? launch_ln_fwd<T, true>(a, vec, (cudaStream_t)stream)
-                     : launch_ln_fwd<T, false>(a, vec, (cudaStream_t)stream);
+        return codes ? launch_ln_fwd<T, true>(a, vec, whole, (cudaStream_t)stream)
+                     : launch_ln_fwd<T, false>(a, vec, whole, (cudaStream_t)stream);
     });
 }
 
