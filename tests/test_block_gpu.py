@@ -568,6 +568,28 @@ def test_projection_backward_weight(cuda, dt, rows, OUT, IN):
             check(got, want, tol + u(t) * (want.abs() + tol), act)
 
 
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("rows,OUT,IN", [(1018, 3000, 6544), (5, 24, 20000), (40, 64, 20000), (200, 20000, 136), (20000, 104, 264)])
+def test_projection_of_long_sums(cuda, dt, rows, OUT, IN):
+    """fp32 results of sums of up to 20000 terms.  The tensor core adds 16 products
+    to its fp32 accumulator at a time and cuts off what does not fit, at most 2^-23
+    of the running sum per step: K / 16 steps are off by at most (K / 16 + 1) 2^-23
+    sum|terms| (one step more where splits are joined), and the result is fp32."""
+    from swiftrwkv_b200 import block as B
+    t = DTYPES[dt]
+    x, w, dy = rnd((rows, IN), 71, t), rnd((OUT, IN), 72, t, IN ** -0.5), rnd((rows, OUT), 73, t)
+
+    def compare(got, a, b, what):
+        z, s0 = proj_sums(a, b)
+        check(got, z, (a.shape[1] / 16 + 1) * 2.0 ** -23 * s0 + U32 * z.abs(), what)
+
+    compare(B.projectionForward(x, w, out_dtype=torch.float32)[0], x, w, "y")
+    compare(B.projectionBackwardInput(dy, w, out_dtype=torch.float32), dy, w.t(), "dx")
+    dw, db = B.projectionBackwardWeight(dy, x, bias=True, out_dtype=torch.float32)
+    compare(dw, dy.t(), x.t(), "dw")
+    check(db, dy.double().sum(0), (rows + 16) * U32 * dy.double().abs().sum(0), "db")
+
+
 def test_projection_results_repeat(cuda):
     """Split products and column sums are joined in a fixed order."""
     from swiftrwkv_b200 import block as B
