@@ -474,22 +474,42 @@ void launch_ln_fwd_t(const LnFwdArgs& a, cudaStream_t st) {
     else ln_fwd_kernel<T, TPR, NV, R, false, CK><<<grid, TPR, 0, st>>>(a);
 }
 
+// Blocks of one kernel that an SM holds, by device and warps per block, asked for once.
+// The kernel may take `most` bytes of dynamic shared memory, the same whatever this
+// call needs: the attribute is the kernel's, and another host thread may be between
+// its own setting and its launch with rows of another length.
+class ResidentBlocks {
+    static constexpr int DEVICES = 64, WARPS = 16;
+    std::atomic<int> n_[DEVICES][WARPS + 1] = {};
+
+public:
+    template <typename K>
+    cudaError_t get(K kern, int threads, int smem, int most, int* per_sm) {
+        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+        if (e != cudaSuccess) return e;
+        int dev;
+        if ((e = cudaGetDevice(&dev)) != cudaSuccess) return e;
+        std::atomic<int>* kept = dev < DEVICES ? &n_[dev][threads / 32] : nullptr;
+        *per_sm = kept ? kept->load(std::memory_order_relaxed) : 0;
+        if (*per_sm > 0) return cudaSuccess;
+        e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(per_sm, kern, threads, smem);
+        if (e != cudaSuccess) return e;
+        if (*per_sm < 1) return cudaErrorInvalidConfiguration;
+        if (kept) kept->store(*per_sm, std::memory_order_relaxed);
+        return cudaSuccess;
+    }
+};
+
 template <typename T, int NV, bool CK, int MAXT, int MINB>
 cudaError_t launch_ln_fwd_shift(const LnFwdArgs& a, cudaStream_t st) {
     auto kern = ln_fwd_shift_kernel<T, NV, CK, MAXT, MINB>;
-    constexpr int VE = Vec16<T>::N;
+    constexpr int VE = Vec16<T>::N, PER_T = LN_STAGES * NV * 16;  // shared memory of a thread
     const int nt = ceil_div(ceil_div(most_vectors<T>(a.D), NV), 32) * 32;
-    const int smem = LN_STAGES * NV * nt * 16;
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    const int smem = PER_T * nt;
+    static ResidentBlocks resident;
+    int per_sm;
+    const cudaError_t e = resident.get(kern, nt, smem, PER_T * MAXT, &per_sm);
     if (e != cudaSuccess) return e;
-    static std::atomic<int> resident[17];  // by warps
-    int per_sm = resident[nt / 32].load(std::memory_order_relaxed);
-    if (per_sm == 0) {
-        const cudaError_t q = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, nt, smem);
-        if (q != cudaSuccess) return q;
-        per_sm = std::max(1, per_sm);
-        resident[nt / 32].store(per_sm, std::memory_order_relaxed);
-    }
     kern<<<std::min(a.rows, 148 * per_sm / VE * VE), nt, smem, st>>>(a);
     return cudaGetLastError();
 }
@@ -956,18 +976,13 @@ cudaError_t launch_ln_bwd_t(const LnBwdArgs& a, int* blocks, cudaStream_t st) {
     auto kern = ln_bwd_kernel<T, CK, NV, R, MAXT, MINB, SH>;
     constexpr int VE = Vec16<T>::N;
     const int nt = ceil_div(ceil_div(SH ? most_vectors<T>(a.D) : a.D / VE, NV), 32) * 32;
-    const int smem = LN_STAGES * R * 3 * NV * nt * 16;
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
+    constexpr int PER_T = LN_STAGES * R * 3 * NV * 16;  // shared memory of a thread
+    const int smem = PER_T * nt;
     // as many blocks as are resident, so that they all run in one wave
-    static std::atomic<int> resident[17];  // by warps
-    int per_sm = resident[nt / 32].load(std::memory_order_relaxed);
-    if (per_sm == 0) {
-        const cudaError_t q = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, nt, smem);
-        if (q != cudaSuccess) return q;
-        per_sm = std::max(1, per_sm);
-        resident[nt / 32].store(per_sm, std::memory_order_relaxed);
-    }
+    static ResidentBlocks resident;
+    int per_sm;
+    const cudaError_t e = resident.get(kern, nt, smem, PER_T * MAXT, &per_sm);
+    if (e != cudaSuccess) return e;
     const int most = std::min(148 * per_sm, LN_BWD_BLOCKS);
     *blocks = std::min(ceil_div(a.rows, R), SH ? most / VE * VE : most);
     kern<<<*blocks, nt, smem, st>>>(a);

@@ -11,6 +11,9 @@ u(t) |result|.
 """
 from __future__ import annotations
 
+import sys
+import threading
+
 import pytest
 import torch
 
@@ -999,3 +1002,51 @@ def test_a_first_projection_during_capture_is_refused(cuda):
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", CAPTURE_FIRST.format(root=root)], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "ok" in r.stdout, r.stdout + r.stderr
+
+
+@pytest.mark.parametrize("bwd", [False, True])
+@pytest.mark.parametrize("lengths", [(2560, 768), (8000, 4200), (2411, 259), (9001, 8301)])
+def test_layer_norms_of_two_lengths_on_two_threads(cuda, bwd, lengths):
+    """Rows of two lengths of one kernel, each in a loop on a host thread and a
+    stream of its own: no call fails, and the results are those of single calls.
+    The lengths differ in the shared memory that they need."""
+    from swiftrwkv_b200 import _lib
+    from swiftrwkv_b200 import block as B
+    L, t, rows = _lib.lib(), torch.bfloat16, 8
+
+    def job(D):
+        x, dy, w, b = rnd((rows, D), 90, t), rnd((rows, D), 91, t), rnd((D,), 92), rnd((D,), 93)
+        y, mean, rstd, _ = B.layerNormForward(x, w, b)
+        want, out = (B.layerNormBackward(dy, x, w, mean, rstd, params=False)[0] if bwd else y), torch.empty_like(x)
+        s = torch.cuda.Stream()
+        if bwd:
+            f = L.rwkv_layer_norm_backward
+            args = (_lib.BF16, dy.data_ptr(), x.data_ptr(), None, None, _lib.F32, w.data_ptr(), mean.data_ptr(),
+                    rstd.data_ptr(), None, out.data_ptr(), None, None, rows, D, None, 0, s.cuda_stream)
+        else:
+            f = L.rwkv_layer_norm_forward
+            args = (_lib.BF16, x.data_ptr(), _lib.F32, w.data_ptr(), b.data_ptr(), 1e-5, out.data_ptr(), mean.data_ptr(),
+                    rstd.data_ptr(), None, None, rows, D, s.cuda_stream)
+        return f, args, want, out, (x, dy, w, b, mean, rstd, s)
+
+    jobs, failed, go = [job(D) for D in lengths], [0, 0], threading.Barrier(2)
+    torch.cuda.synchronize()
+
+    def run(k):
+        f, args = jobs[k][:2]
+        go.wait()
+        failed[k] = sum(f(*args) != _lib.OK for _ in range(20000))
+
+    threads, interval = [threading.Thread(target=run, args=(k,)) for k in range(2)], sys.getswitchinterval()
+    sys.setswitchinterval(1e-5)
+    try:
+        for th in threads:
+            th.start()
+        for th in threads:
+            th.join()
+    finally:
+        sys.setswitchinterval(interval)
+    torch.cuda.synchronize()
+    assert failed == [0, 0]
+    for _, _, want, out, _ in jobs:
+        assert torch.equal(out, want)
