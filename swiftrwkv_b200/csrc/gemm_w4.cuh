@@ -28,6 +28,10 @@ namespace rwkv {
 
 constexpr int GW_THREADS = 128;
 constexpr int GW_BM = 64;
+// What a kernel may take of dynamic shared memory (227 KB less its static part), set
+// whatever the call needs: the limit is the kernel's, and another host thread may be
+// between setting it and launching a wider matrix.
+constexpr int GW_SMEM_MAX = 226 * 1024;
 
 struct GemmArgs {
     GemvJobs jobs;
@@ -383,7 +387,7 @@ inline cudaError_t launch_gemm_t(const GemmArgs& a, const GemmPlan& p, cudaStrea
     const size_t smem = GemmSmem<FMT, BN, STAGES, GPS>::PIPE + (FMT == 0 ? 2 * GW_BM * max_groups * 2 : 0);
     auto kern = gemm_w4_kernel<FMT, BN, MW, STAGES, GPS>;
     if (smem > 48 * 1024) {
-        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, GW_SMEM_MAX);
         if (e != cudaSuccess) return e;
     }
     dim3 grid(p.mblocks, a.njobs, p.nnb * a.S);

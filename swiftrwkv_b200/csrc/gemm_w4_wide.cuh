@@ -267,7 +267,7 @@ inline cudaError_t launch_wide_t(const GemmArgs& a, const GemmPlan& p, cudaStrea
     const size_t smem = SM::TOTAL + (FMT == 0 ? (size_t)GW_BM * max_groups * 4 : 0);
     auto kern = gemm_w4_wide_kernel<FMT, BN, STAGES>;
     if (smem > 48 * 1024) {
-        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, GW_SMEM_MAX);
         if (e != cudaSuccess) return e;
     }
     dim3 grid(p.mblocks, a.njobs, p.nnb * a.S);

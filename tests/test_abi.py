@@ -4,6 +4,8 @@ symbol include/rwkv_cuda.h declares, and rejects bad arguments on the host
 from __future__ import annotations
 
 import ctypes
+import os
+import re
 
 import pytest
 
@@ -124,3 +126,17 @@ def test_projection_backward_validates_before_any_launch():
     assert q(group=32) == _lib.E_UNSUPPORTED
     assert q(bits=8) == _lib.E_UNSUPPORTED
     assert q(sdt=BF16) == _lib.E_UNSUPPORTED
+
+
+def test_shared_memory_limits_do_not_follow_a_call():
+    """A kernel's limit of dynamic shared memory is the same in every call: set to
+    what one launch needs, it could fall between another host thread's setting and
+    that thread's wider launch."""
+    csrc = os.path.join(os.path.dirname(_lib.__file__), "csrc")
+    found = 0
+    for name in sorted(os.listdir(csrc)):
+        with open(os.path.join(csrc, name)) as f:
+            for size in re.findall(r"cudaFuncAttributeMaxDynamicSharedMemorySize,\s*([^;\n]+)", f.read()):
+                found += 1
+                assert not re.search(r"\bsmem\b", size), f"{name}: {size}"
+    assert found > 10
