@@ -19,9 +19,10 @@ MLX's autograd (Sources/RWKVGen/RWKVBlock.swift:163-307, X070Backbone.swift:
 Arrays are torch CUDA tensors of [..., D]; leading dimensions are rows, of any
 number (also none).  All arithmetic runs in librwkvcuda, on the current stream
 of the tensors' device.  Arguments that do not fit raise ValueError; a failed
-CUDA call raises RWKVError.  The differentiable forms refuse to record a graph
-while a CUDA stream is being captured: capture the explicit forward and
-backward calls.
+CUDA call raises RWKVError.  The differentiable forms are for reverse mode, once:
+they refuse inputs with a forward-mode tangent, and to record a graph while a
+CUDA stream is being captured (capture the explicit forward and backward calls).
+The explicit calls take their inputs as values: no gradient or tangent follows.
 """
 from __future__ import annotations
 
@@ -29,6 +30,7 @@ from dataclasses import dataclass
 from functools import lru_cache
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from . import _lib
 from ._lib import ACTS, BF16, F16, F32
@@ -408,9 +410,16 @@ def projectionBackwardWeight(dy, x, act: str = "none", bias: bool = False, out_d
 
 # --------------------------------------------------- the differentiable forms
 
-def _recording(*ts):
-    """Whether autograd records this call; refused while a stream is captured."""
-    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in ts):
+def _recording(**ts):
+    """Whether autograd records this call; refused while a stream is captured,
+    and for inputs that carry a forward-mode tangent, which the kernels would
+    drop (the result would read as having a derivative of zero)."""
+    for name, t in ts.items():
+        if t is not None and not isinstance(t, torch.Tensor):
+            raise ValueError(f"{name}: a CUDA tensor is needed")
+        if t is not None and unpack_dual(t).tangent is not None:
+            raise ValueError(f"{name} carries a tangent: the block operators have no forward-mode derivatives")
+    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in ts.values()):
         return False
     if torch.cuda.is_current_stream_capturing():
         raise ValueError("the differentiable block operators do not record a graph during stream capture: "
@@ -466,7 +475,7 @@ class _LayerNorm(torch.autograd.Function):
 def layerNorm(x, weight, bias, eps: float = 1e-5, checkpoint: bool = False):
     """Differentiable layer norm.  With `checkpoint` its input is kept for the
     backward pass as an 8-bit checkpoint instead of in its own type."""
-    if not _recording(x, weight, bias):
+    if not _recording(x=x, weight=weight, bias=bias):
         return layerNormForward(x, weight, bias, eps)[0]
     return _LayerNorm.apply(x, weight, bias, eps, checkpoint)
 
@@ -501,7 +510,7 @@ class _Projection(torch.autograd.Function):
 def projection(x, w, bias=None, act: str = "none", residual=None, checkpoint: bool = False):
     """Differentiable y = act(x w^T + bias) + residual.  With `checkpoint` the
     backward pass works from 8-bit checkpoints of x and of the pre-activation."""
-    if not _recording(x, w, bias, residual):
+    if not _recording(x=x, w=w, bias=bias, residual=residual):
         return projectionForward(x, w, bias, act, residual)[0]
     return _Projection.apply(x, w, bias, act, residual, checkpoint)
 
@@ -534,7 +543,7 @@ def channelMix(x, key, value, residual=None, checkpoint: bool = True):
     ReLU ends the first product and its gradient the backward's, which reads the
     pre-activation z; with `checkpoint` z and x are kept in 8 bits (1 + 1/32
     bytes per channel) and the squared ReLU itself is not kept at all."""
-    if not _recording(x, key, value, residual):
+    if not _recording(x=x, key=key, value=value, residual=residual):
         k, _ = projectionForward(x, key, act="relu2")
         return projectionForward(k, value, residual=residual)[0]
     return _ChannelMix.apply(x, key, value, residual, checkpoint)

@@ -235,3 +235,32 @@ def test_what_is_no_tensor_is_refused(monkeypatch):
     monkeypatch.setattr(B, "_tensor", lambda name, t, *a, **k: t)
     with pytest.raises(ValueError, match="Checkpoint8"):
         B.projectionBackwardWeight(torch.zeros(4, 64, dtype=torch.bfloat16), [1.0])
+
+
+def differentiable_calls():
+    """Each differentiable form on host tensors, by the name of its arguments."""
+    v, x, w, key, value = torch.ones(8), torch.ones(2, 8), torch.ones(16, 8), torch.ones(16, 8), torch.ones(8, 16)
+    return [(B.layerNorm, dict(x=x, weight=v, bias=v)),
+            (B.projection, dict(x=x, w=w, bias=torch.ones(16), residual=torch.ones(2, 16))),
+            (B.channelMix, dict(x=x, key=key, value=value, residual=x))]
+
+
+@pytest.mark.parametrize("recorded", [False, True])
+def test_tangents_are_refused(recorded):
+    """Forward mode would lose the tangent without a word: a derivative of zero."""
+    from torch.autograd import forward_ad
+    for f, args in differentiable_calls():
+        for name in args:
+            with forward_ad.dual_level():
+                dual = forward_ad.make_dual(args[name].clone().requires_grad_(recorded), torch.ones_like(args[name]))
+                with pytest.raises(ValueError, match=f"^{name} carries a tangent"):
+                    f(**{**args, name: dual})
+            with pytest.raises(ValueError, match=f"^{name} carries a tangent"):
+                torch.func.jvp(lambda t: f(**{**args, name: t}), (args[name],), (args[name],))
+
+
+def test_differentiable_forms_refuse_what_is_no_tensor():
+    for f, args in differentiable_calls():
+        for name in args:
+            with pytest.raises(ValueError, match="CUDA tensor"):
+                f(**{**args, name: [1.0]})
