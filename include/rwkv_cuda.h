@@ -555,7 +555,10 @@ int rwkv_act_backward(int dtype, const void* dy, const void* z, const int8_t* co
 /* Trainable projections.  x [rows, IN], w [OUT, IN], y [rows, OUT] and their
  * gradients; x, w and dY in `dtype`, BF16 or F16 (both operands of a
  * tensor-core product in one type); accumulation in fp32, one rounding at the
- * store.  IN % 8 == 0 and OUT % 8 == 0, tensors 16-byte aligned (exps and db to
+ * store.  The tensor cores cut off what an addition does not hold (at most 5
+ * 2^-23 of the sum per 16 terms); an accumulator takes 32768 terms at most, and
+ * longer sums are joined from several in fp32: within 2^-9.6 sum|terms| for any
+ * length and order, 2^-12 where terms of one sign and size are added.  IN % 8 == 0 and OUT % 8 == 0, tensors 16-byte aligned (exps and db to
  * their element); rows in 1..2^24, IN and OUT up to 2^20.  tcgen05 tensor
  * cores; these calls share rwkv_q_gemm's wait-error record
  * (rwkv_q_gemm_status), and a stream may be captured once one call has run on

@@ -40,6 +40,13 @@
 // sums as a tile into the workspace, and the join kernel adds the splits in order
 // (deterministic) and runs the epilogue.
 //
+// An accumulator takes 32768 terms at most; longer sums split every tile along K.  A
+// step of the tensor core cuts its 16 products and the accumulator off at 2^-25 of the
+// largest one's binade and their sum at 2^-23, toward zero (measured), so that a step
+// may lose 5 2^-23 of the sum and sums of one sign drift: 2^19 terms in [1/4, 1] come
+// out 3.0e-3 low from one accumulator, 1.6e-4 from 16.  The join's additions round to
+// nearest.
+//
 // Every mbarrier wait is bounded (tc::mbar_wait); a wait that gives up sets the
 // shared error flag, every role winds down, the producer waits (bounded) for its
 // copies in flight and TMEM is freed after the final MMA commit.
@@ -53,6 +60,7 @@ namespace rwkv {
 constexpr int PJ_BK = 64;
 constexpr int PJ_GROUP_M = 8;      // row blocks walked together
 constexpr int PJ_SMS = 148;
+constexpr int PJ_CHAIN = 32768;    // terms that one accumulator takes
 constexpr int PJ_OUT_BYTES = 32 * 1024;  // output staging, shared by the epilogue warps
 
 // Which epilogue a kernel has, at compile time: one that can do everything keeps
@@ -94,7 +102,7 @@ struct ProjArgs {
     ProjEpi e;
     int M, N, nk;       // D's size, K stages
     int mt, nt;         // tiles along M and N
-    int full, S;        // tiles that run whole; splits of each of the others
+    int full, F, S;     // tiles of whole waves, splits of each; splits of each of the others
     int ctma;           // codes leave by TMA
     uint32_t idesc;
     int* err;           // device flag: a wait gave up
@@ -371,7 +379,7 @@ __global__ void __launch_bounds__(PjCfg<BN, CG, KIND>::THREADS, 1) proj_kernel(c
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = CG == 2 ? (int)blockIdx.x & 1 : 0;  // within the pair; rank 0 issues the MMAs
     const int first = (int)blockIdx.x / CG, stride = (int)gridDim.x / CG;
-    const int units = a.full + (a.mt * a.nt - a.full) * a.S;
+    const int whole = a.full * a.F, units = whole + (a.mt * a.nt - a.full) * a.S;
     const int my_tiles = first < units ? (units - 1 - first) / stride + 1 : 0;
     int* err = a.err;
     // rank 0's barriers, as both CTAs address them
@@ -425,16 +433,28 @@ __global__ void __launch_bounds__(PjCfg<BN, CG, KIND>::THREADS, 1) proj_kernel(c
     auto tile_at = [&](int i) {
         const int u = first + i * stride;
         Tile r;
-        int t = u;
+        int t = u, z = 0, S = 1, slot = -1;
+        if (u < whole) {
+            if (a.F > 1) {  // a split of every tile, then the next: neighbours share their K
+                S = a.F;
+                z = u / a.full;
+                t = u - z * a.full;
+                slot = u;
+            }
+        } else {
+            S = a.S;
+            const int j = (u - whole) / S;
+            z = u - whole - j * S;
+            t = a.full + j;
+            slot = a.F > 1 ? u : u - whole;
+        }
         r.k0 = 0;
         r.k1 = a.nk;
         r.part = -1;
-        if (u >= a.full && a.S > 1) {
-            const int j = (u - a.full) / a.S, z = u - a.full - j * a.S;
-            t = a.full + j;
-            r.k0 = (int)((int64_t)a.nk * z / a.S);
-            r.k1 = (int)((int64_t)a.nk * (z + 1) / a.S);
-            r.part = ((u - a.full) * CG + rank) * 128;
+        if (slot >= 0) {
+            r.k0 = (int)((int64_t)a.nk * z / S);
+            r.k1 = (int)((int64_t)a.nk * (z + 1) / S);
+            r.part = (slot * CG + rank) * 128;
         }
         const int per = PJ_GROUP_M * a.nt, g = t / per, rem = t - g * per;
         const int gm = min(PJ_GROUP_M, a.mt - g * PJ_GROUP_M);
@@ -678,20 +698,23 @@ __global__ void __launch_bounds__(PjCfg<BN, CG, KIND>::THREADS, 1) proj_kernel(c
 }
 
 struct ProjJoin {
-    const float* part;  // [(tile - full) S + split][BM][BN]
+    const float* part;  // [F > 1: split full + tile, behind them][(tile - full) S + split][BM][BN]
     ProjEpi e;
     void* d;
-    int M, N, mt, nt, full, S, BM, BN;
+    int M, N, mt, nt, full, F, S, BM, BN;
 };
-// Joins the splits of the tiles full ..: thread i takes 8 columns of a row of a
+// Joins the splits of the tiles full .., with F > 1 of all: thread i takes 8 columns of a row of a
 // tile (four neighbouring lanes hold a checkpoint group), the splits' loads all in
 // flight, 16 at most.
 template <int KIND>
 __device__ __forceinline__ void proj_join(const ProjJoin& a, int64_t i) {
     const int per = a.BN / 8;
     const int piece = (int)(i % per), r = (int)(i / per % a.BM);
-    const int64_t j = i / per / a.BM;
-    const int t = a.full + (int)j;  // the grid covers whole tiles
+    // the grid covers whole tiles; t's splits are n tiles from `slot` on, `step` apart
+    const int t = (int)(i / per / a.BM) + (a.F > 1 ? 0 : a.full);
+    const bool whole = t < a.full;
+    const int n = whole ? a.F : a.S, step = whole ? a.full : 1;
+    const int64_t slot = whole ? t : (a.F > 1 ? a.full * a.F : 0) + (int64_t)(t - a.full) * a.S;
     const int pg = PJ_GROUP_M * a.nt, g = t / pg, rem = t - g * pg;
     const int gm = min(PJ_GROUP_M, a.mt - g * PJ_GROUP_M);
     const int64_t row = (int64_t)(g * PJ_GROUP_M + rem % gm) * a.BM + r;
@@ -700,11 +723,11 @@ __device__ __forceinline__ void proj_join(const ProjJoin& a, int64_t i) {
     if (__all_sync(0xffffffffu, !in)) return;
     const int64_t at = row * a.N + col;
     float v[8] = {};
-    const float* p = a.part + (j * a.S * a.BM + r) * a.BN + 8 * piece;
+    const float* p = a.part + (slot * a.BM + r) * a.BN + 8 * piece;
     if (in) {
 #pragma unroll 8
-        for (int z = 0; z < a.S; z++) {
-            const float4* q = reinterpret_cast<const float4*>(p + (int64_t)z * a.BM * a.BN);
+        for (int z = 0; z < n; z++) {
+            const float4* q = reinterpret_cast<const float4*>(p + (int64_t)z * step * a.BM * a.BN);
             const float4 x = q[0], y = q[1];
             v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
             v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
@@ -800,10 +823,16 @@ __global__ void __launch_bounds__(PJ_JOIN_T) proj_join_kernel(const ProjJoin a, 
 //    finds shortest: a stage of 64 takes 0.45 us on a pair and 0.27 us on a CTA (an SM's
 //    share of L2 bandwidth); joining takes 3.5 us and writes and reads each split's
 //    tile once in L2 (8 TB/s).
+//  - More than PJ_CHAIN terms: the tiles of whole waves are split too, into as few as
+//    that takes (2304 x 2304 over 65536: 416 us, in one drifting accumulator 408; over
+//    2^19 3340 and 3179).
 struct ProjPlan {
-    int CG, BN, mt, nt, full, S;
+    int CG, BN, mt, nt, full, F, S;
     int64_t ws_bytes;  // the splits' tiles
     int BM() const { return 128 * CG; }
+    int64_t parts() const { return (F > 1 ? (int64_t)full * F : 0) + (S > 1 ? ((int64_t)mt * nt - full) * S : 0); }
+    // the parts' rows in the workspace are counted in 31 bits
+    bool ok() const { return parts() * BM() < 1ll << 31; }
 };
 inline ProjPlan proj_plan(int64_t M, int64_t N, int64_t K) {
     ProjPlan p{};
@@ -815,17 +844,16 @@ inline ProjPlan proj_plan(int64_t M, int64_t N, int64_t K) {
     p.nt = (int)((N + p.BN - 1) / p.BN);
     const int wave = PJ_SMS / p.CG, tiles = p.mt * p.nt, rem = tiles % wave;
     p.full = tiles - rem;
-    p.S = 1;
-    if (rem == 0) return p;
+    p.F = p.S = (int)((K + PJ_CHAIN - 1) / PJ_CHAIN);
     double best = 0.0;
-    for (int S = 1; S <= 16 && (S == 1 || nk / S >= 2); S++) {
+    for (int S = p.F; rem && S <= std::max(p.F, 16) && (S == p.F || nk / S >= 2); S++) {
         const double stage = pair ? 0.45 : 0.27, bytes = 2.0 * rem * S * p.BM() * p.BN * 4;
-        const double us = (double)((rem * S + wave - 1) / wave) * ((nk + S - 1) / S) * stage +
+        const double us = (double)(((int64_t)rem * S + wave - 1) / wave) * ((nk + S - 1) / S) * stage +
                           (S > 1 ? 3.5 + bytes / 8e6 : 0.0);
-        if (S == 1 || us < best) best = us, p.S = S;
+        if (S == p.F || us < best) best = us, p.S = S;
     }
     if (p.S == 1) p.full = tiles;
-    else p.ws_bytes = (int64_t)rem * p.S * p.BM() * p.BN * 4;
+    p.ws_bytes = p.parts() * p.BM() * p.BN * 4;
     return p;
 }
 
@@ -847,7 +875,7 @@ inline cudaError_t proj_launch_t(const ProjArgs& a, int sm_count, bool after_own
     auto kern = proj_kernel<BN, CG, AMN, BMN, KIND>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::TOTAL);
     if (e != cudaSuccess) return e;
-    const int units = a.full + (a.mt * a.nt - a.full) * a.S;
+    const int units = a.full * a.F + (a.mt * a.nt - a.full) * a.S;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(std::min(units, sm_count / CG) * CG);
     cfg.blockDim = dim3(C::THREADS);
@@ -877,6 +905,7 @@ inline cudaError_t proj_gemm(const void* A, const void* B, void* D, int64_t M, i
                              float* ws, int* err, int* err_host, int sm_count, cudaStream_t st, bool after_own = false,
                              const ColJoin* cols = nullptr) {
     const ProjPlan p = proj_plan(M, N, K);
+    if (!p.ok()) return cudaErrorInvalidValue;
     ProjArgs a{};
     a.e = e;
     a.M = (int)M;
@@ -885,11 +914,11 @@ inline cudaError_t proj_gemm(const void* A, const void* B, void* D, int64_t M, i
     a.mt = p.mt;
     a.nt = p.nt;
     a.full = p.full;
+    a.F = p.F;
     a.S = p.S;
     a.idesc = tc::idesc_f16(p.BM(), p.BN, e.bf16 != 0) | (AMN ? 1u << 15 : 0u) | (BMN ? 1u << 16 : 0u);
     a.err = err;
     a.err_host = err_host;
-    const int rem = p.mt * p.nt - p.full;
     const CUtensorMapDataType t16 = e.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     const auto sw128 = CU_TENSOR_MAP_SWIZZLE_128B;
     bool ok = AMN ? proj_map_2d(&a.amap, t16, 2, A, M, K, 64, PJ_BK, sw128)
@@ -901,15 +930,16 @@ inline cudaError_t proj_gemm(const void* A, const void* B, void* D, int64_t M, i
     a.ctma = KIND == PJ_FWD_CK && N % 16 == 0;
     if (a.ctma)
         ok = ok && proj_map_2d(&a.cmap, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, e.codes, N, M, 32, 32, CU_TENSOR_MAP_SWIZZLE_NONE);
-    if (p.S > 1)
-        ok = ok && proj_map_2d(&a.pmap, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, ws, p.BN, (int64_t)rem * p.S * p.BM(), 16, 32,
+    if (p.ws_bytes)
+        ok = ok && proj_map_2d(&a.pmap, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, ws, p.BN, p.parts() * p.BM(), 16, 32,
                                CU_TENSOR_MAP_SWIZZLE_64B);
     if (!ok) return cudaErrorInvalidValue;
     const cudaError_t rc = p.CG == 2 ? proj_launch_t<256, 2, AMN, BMN, KIND>(a, sm_count, after_own, st)
                                      : proj_launch_t<128, 1, AMN, BMN, KIND>(a, sm_count, after_own, st);
-    if (rc != cudaSuccess || (p.S == 1 && !cols)) return rc;
-    const ProjJoin j{ws, e, D, (int)M, (int)N, p.mt, p.nt, p.full, p.S, p.BM(), p.BN};
-    const int first = p.S > 1 ? ceil_div((int64_t)rem * p.BM() * (p.BN / 8), PJ_JOIN_T) : 0;
+    if (rc != cudaSuccess || (!p.ws_bytes && !cols)) return rc;
+    const ProjJoin j{ws, e, D, (int)M, (int)N, p.mt, p.nt, p.full, p.F, p.S, p.BM(), p.BN};
+    const int joined = p.mt * p.nt - (p.F > 1 ? 0 : p.full);
+    const int first = ceil_div((int64_t)joined * p.BM() * (p.BN / 8), PJ_JOIN_T);
     const ColJoin c = cols ? *cols : ColJoin{};
     return launch_pdl(proj_join_kernel<KIND>, dim3(first + ceil_div(c.N, 32)), dim3(PJ_JOIN_T), 0, st, j, c, first);
 }

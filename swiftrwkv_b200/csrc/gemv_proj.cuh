@@ -22,6 +22,7 @@
 namespace rwkv {
 
 constexpr int GP_ROWS = 16;  // rows of x at most
+constexpr int GP_IN = 8 * PJ_CHAIN;  // terms at most: PJ_CHAIN for each of 8 warps
 constexpr int GP_U = 4;
 
 struct GemvProjArgs {

@@ -128,7 +128,6 @@ int check_common(int dtype, int rows, int OUT, int IN, const char* fn) {
                  IN);
     RWKV_REQUIRE(IN % 8 == 0 && OUT % 8 == 0, RWKV_E_UNSUPPORTED, "%s: IN=%d and OUT=%d must be multiples of 8", fn,
                  IN, OUT);
-    // (a tile's sums take one bounded wait: 2^24 terms are 0.1 s)
     RWKV_REQUIRE(rows <= 1 << 24 && OUT <= 1 << 20 && IN <= 1 << 20 &&
                      (int64_t)ceil_div(rows, 128) * ceil_div(std::max(OUT, IN), 64) < 1 << 30,
                  RWKV_E_SHAPE, "%s: rows=%d OUT=%d IN=%d too large", fn, rows, OUT, IN);
@@ -140,6 +139,8 @@ int check_ws(const void* ws, int64_t bytes, int64_t need, const char* fn) {
     RWKV_REQUIRE(need == 0 || al(ws, 16), RWKV_E_UNSUPPORTED, "%s: workspace not 16-byte aligned", fn);
     return RWKV_OK;
 }
+// stream the weights (gemv_proj.cuh)
+bool few_rows(int rows, int IN) { return rows <= GP_ROWS && IN <= GP_IN; }
 bool out_ok(int out, int dtype) { return out == dtype || out == RWKV_F32; }
 
 bool sizes_ok(int rows, int OUT, int IN) {
@@ -152,7 +153,7 @@ bool sizes_ok(int rows, int OUT, int IN) {
 using namespace rwkv;
 
 extern "C" int64_t rwkv_projection_forward_workspace_size(int rows, int OUT, int IN) {
-    return sizes_ok(rows, OUT, IN) && rows > GP_ROWS ? proj_plan(rows, OUT, IN).ws_bytes : 0;
+    return sizes_ok(rows, OUT, IN) && !few_rows(rows, IN) ? proj_plan(rows, OUT, IN).ws_bytes : 0;
 }
 
 extern "C" int rwkv_projection_forward(int dtype, const void* x, const void* w, int bdtype, const void* bias, int act,
@@ -169,7 +170,7 @@ extern "C" int rwkv_projection_forward(int dtype, const void* x, const void* w, 
     RWKV_REQUIRE(al(x, 16) && al(w, 16) && al(y, 16) && al(residual, 16) && al(z, 16) && al(codes, 16) &&
                      al(bias, 16),
                  RWKV_E_UNSUPPORTED, "%s: a tensor is not 16-byte aligned", fn);
-    const bool few = rows <= GP_ROWS;  // stream the weights (gemv_proj.cuh)
+    const bool few = few_rows(rows, IN);
     if (!few)
         if (int rc = check_ws(workspace, workspace_bytes, proj_plan(rows, OUT, IN).ws_bytes, fn)) return rc;
     int *err, *err_host, sms;

@@ -1050,3 +1050,36 @@ def test_layer_norms_of_two_lengths_on_two_threads(cuda, bwd, lengths):
     assert failed == [0, 0]
     for _, _, want, out, _ in jobs:
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("what,rows", [("y", 5), ("y", 2304), ("dx", 2304), ("dw", 2304)])
+def test_projection_sums_too_long_for_one_accumulator(cuda, what, rows):
+    """One product of 1 and 2^18 (in the few-row kernel 2^20) of just below 2^-25.
+    The tensor core cuts each of the 16 products of a step off at 2^-25 of the
+    largest addend's binade and the step's sum at 2^-23: less than 16 2^-25 + 2^-23 =
+    5 2^-23 of the sum is lost per step, so that an accumulator of 32768 terms is off
+    by at most 2048 steps 5 2^-23 sum|terms|; the splits' sums are joined by
+    roundings of 2^-24 each, one per split.  An accumulator of all the terms
+    loses nearly all of the small ones, 7.8e-3 (the few-row kernel's sixteen warps 1.9e-3)."""
+    from swiftrwkv_b200 import block as B
+    t, n = torch.bfloat16, 2304 if rows > 16 else 24
+    K = 1 << (18 if rows > 16 else 20)
+    small = 2.0 ** -13 * 1.984375
+
+    def operand(m, first):
+        a = torch.full((m, K) if first else (K, m), 2.0 ** -13, device="cuda", dtype=t)
+        (a if first else a.t())[:, 0] = 1.0
+        return a
+
+    if what == "y":
+        a, b = operand(rows, True), operand(n, True)
+    elif what == "dx":
+        a, b = operand(rows, True), operand(n, False)
+    else:
+        a, b = operand(rows, False), operand(n, False)
+    (a if what != "dw" else a.t())[:, 1:] = small
+    got = {"y": lambda: B.projectionForward(a, b, out_dtype=torch.float32)[0],
+           "dx": lambda: B.projectionBackwardInput(a, b, out_dtype=torch.float32),
+           "dw": lambda: B.projectionBackwardWeight(a, b, out_dtype=torch.float32)[0]}[what]()
+    want = torch.full((rows, n), 1.0 + (K - 1) * small * 2.0 ** -13, device="cuda", dtype=torch.float64)
+    check(got, want, (2048 * 5 * 2.0 ** -23 + K / 32768 * U32 + U32) * want, what)
