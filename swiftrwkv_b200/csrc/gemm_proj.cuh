@@ -710,11 +710,8 @@ template <int KIND>
 __device__ __forceinline__ void proj_join(const ProjJoin& a, int64_t i) {
     const int per = a.BN / 8;
     const int piece = (int)(i % per), r = (int)(i / per % a.BM);
-    // the grid covers whole tiles; t's splits are n tiles from `slot` on, `step` apart
-    const int t = (int)(i / per / a.BM) + (a.F > 1 ? 0 : a.full);
-    const bool whole = t < a.full;
-    const int n = whole ? a.F : a.S, step = whole ? a.full : 1;
-    const int64_t slot = whole ? t : (a.F > 1 ? a.full * a.F : 0) + (int64_t)(t - a.full) * a.S;
+    const int64_t j = i / per / a.BM;  // the grid covers whole tiles
+    const int t = (a.F > 1 ? 0 : a.full) + (int)j;
     const int pg = PJ_GROUP_M * a.nt, g = t / pg, rem = t - g * pg;
     const int gm = min(PJ_GROUP_M, a.mt - g * PJ_GROUP_M);
     const int64_t row = (int64_t)(g * PJ_GROUP_M + rem % gm) * a.BM + r;
@@ -723,15 +720,21 @@ __device__ __forceinline__ void proj_join(const ProjJoin& a, int64_t i) {
     if (__all_sync(0xffffffffu, !in)) return;
     const int64_t at = row * a.N + col;
     float v[8] = {};
-    const float* p = a.part + (slot * a.BM + r) * a.BN + 8 * piece;
     if (in) {
+        // n splits, the first in `slot`, the others `step` further each
+        auto add = [&](int64_t slot, int n, int step) {
+            const float* p = a.part + (slot * a.BM + r) * a.BN + 8 * piece;
 #pragma unroll 8
-        for (int z = 0; z < n; z++) {
-            const float4* q = reinterpret_cast<const float4*>(p + (int64_t)z * step * a.BM * a.BN);
-            const float4 x = q[0], y = q[1];
-            v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
-            v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
-        }
+            for (int z = 0; z < n; z++) {
+                const float4* q = reinterpret_cast<const float4*>(p + (int64_t)z * step * a.BM * a.BN);
+                const float4 x = q[0], y = q[1];
+                v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
+                v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
+            }
+        };
+        if (a.F == 1) add(j * a.S, a.S, 1);
+        else if (t < a.full) add(t, a.F, a.full);
+        else add((int64_t)a.full * a.F + (int64_t)(t - a.full) * a.S, a.S, 1);
     }
     if ((KIND == PJ_FWD || KIND == PJ_FWD_CK) && a.e.bias && in) {
         float b[8];
