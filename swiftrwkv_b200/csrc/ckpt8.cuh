@@ -94,11 +94,11 @@ __device__ __forceinline__ void ck_unpack4(uint32_t w, float s, float* v) {
 // which is at most 1, so that nothing overflows and no derivative cancels:
 //   tanh = (1 - e) / (1 + e) with z's sign, tanh' = 4 e / (1 + e)^2
 //   sigmoid = (1 or e) / (1 + e) by z's sign, sigmoid' = e / (1 + e)^2
-// FAST: __expf and __fdividef, relative errors of about 2^-19 over the range
-// where the result is not negligible, for results that are rounded to 16 bits
-// or come out of a tensor-core sum; below |z| = 2^-6, where 1 - e cancels,
-// tanh z = z - z^3 / 3 (next term z^5 2/15 < 2^-26 z).  Otherwise expf, tanhf
-// and IEEE division.
+// FAST: __expf (2 + |1.16 x| ulp) and __fdividef (2 ulp), for results that are rounded
+// to 16 bits: tanh within 2^-18 relative (at |z| = 2^-6, where 1 - e = 2^-5 is off by
+// 2^-23 from e), sigmoid and the derivatives within 2^-19 up to |z| = 10; below |z| =
+// 2^-6, where 1 - e cancels further, tanh z = z - z^3 / 3 (next term z^5 2/15 < 2^-26 z).
+// Otherwise expf, tanhf and IEEE division.
 template <int ACT, bool FAST>
 __device__ __forceinline__ float act_t(float z) {
     if constexpr (ACT == RWKV_ACT_RELU2) {

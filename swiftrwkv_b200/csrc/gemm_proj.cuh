@@ -72,6 +72,10 @@ enum : int {
     PJ_FWD_CK = 2, // and the checkpoint of z
     PJ_GRAD = 3,   // times act'(pre), addend
 };
+// FAST, with tanh and sigmoid: the fast functions (act_t), for results of 16 bits.  In
+// kernels of their own: both kinds of functions in one cost the 16-bit results (4093 x
+// 2048 over 96, dX with tanh: 16.2 -> 19.8 us).  The exact ones take 24.3 us there, the
+// forward's sigmoid 21.7 (fast 16.1), its tanh 17.5 (17.6).
 
 // What happens to the sums; all tensors are row-major [M, N].
 struct ProjEpi {
@@ -89,6 +93,7 @@ struct ProjEpi {
     const int8_t* pre_codes;  // its checkpoint
     const uint8_t* pre_exps;
 
+    bool fast() const { return !out_f32 || (act != RWKV_ACT_TANH && act != RWKV_ACT_SIGMOID); }
     int kind() const {
         return grad ? PJ_GRAD : codes ? PJ_FWD_CK : bias || z || add || act != RWKV_ACT_NONE ? PJ_FWD : PJ_PLAIN;
     }
@@ -215,7 +220,7 @@ __device__ __forceinline__ void floats8_16(const uint4& r, int bf16, float* v) {
 // with the bias added; pre / exp as in ProjAux.  PJ_FWD_CK: the codes go to w and the
 // exponent byte is returned, for the caller to store; the group is the thread's own
 // 32 columns, or (W = 8) those of four neighbouring lanes.
-template <int KIND, int W>
+template <int KIND, bool FAST, int W>
 __device__ __forceinline__ uint32_t proj_epilogue(float* v, const ProjEpi& e, const uint4* pre, uint32_t pexp,
                                                   int64_t row, int col, int nv, int N, uint32_t* w) {
     uint32_t exp = 0;
@@ -254,14 +259,14 @@ __device__ __forceinline__ uint32_t proj_epilogue(float* v, const ProjEpi& e, co
                     floats8_16(pre[i], e.bf16, p);
                 }
 #pragma unroll
-                for (int k = 0; k < 8; k++) v[8 * i + k] *= act_grad_t<ACT, true>(p[k]);
+                for (int k = 0; k < 8; k++) v[8 * i + k] *= act_grad_t<ACT, FAST>(p[k]);
             }
         });
     } else if constexpr (KIND != PJ_PLAIN) {
         if (e.act != RWKV_ACT_NONE)
             with_act(e.act, [&]<int ACT>() {
 #pragma unroll
-                for (int i = 0; i < W; i++) v[i] = act_t<ACT, true>(v[i]);
+                for (int i = 0; i < W; i++) v[i] = act_t<ACT, FAST>(v[i]);
             });
     }
     return exp;
@@ -363,7 +368,7 @@ struct PjCfg {
 };
 
 // AMN / BMN: the operand is MN-major.
-template <int BN, int CG, bool AMN, bool BMN, int KIND>
+template <int BN, int CG, bool AMN, bool BMN, int KIND, bool FAST>
 __global__ void __launch_bounds__(PjCfg<BN, CG, KIND>::THREADS, 1) proj_kernel(const __grid_constant__ ProjArgs a) {
     using C = PjCfg<BN, CG, KIND>;
     constexpr int ST = C::ST;
@@ -602,7 +607,7 @@ __global__ void __launch_bounds__(PjCfg<BN, CG, KIND>::THREADS, 1) proj_kernel(c
                             // W / 8 vectors of a dense pre-activation, half as many of codes
                             const uint4 p[2] = {a.e.pre_codes ? aux.pre[h * W / 16] : aux.pre[h * W / 8],
                                                 aux.pre[(h * W / 8 + 1) % 4]};
-                            exps |= proj_epilogue<KIND, W>(v, a.e, p, aux.exp, row, col + h * W, nv - h * W, a.N, codes)
+                            exps |= proj_epilogue<KIND, FAST, W>(v, a.e, p, aux.exp, row, col + h * W, nv - h * W, a.N, codes)
                                     << ((c - c0) / 4);
                             if (a.e.add && a.e.out_f32)
                                 proj_add_f32<W>(v, a.e, (int64_t)row * a.N + col + h * W, nv - h * W);
@@ -706,7 +711,7 @@ struct ProjJoin {
 // Joins the splits of the tiles full .., with F > 1 of all: thread i takes 8 columns of a row of a
 // tile (four neighbouring lanes hold a checkpoint group), the splits' loads all in
 // flight, 16 at most.
-template <int KIND>
+template <int KIND, bool FAST>
 __device__ __forceinline__ void proj_join(const ProjJoin& a, int64_t i) {
     const int per = a.BN / 8;
     const int piece = (int)(i % per), r = (int)(i / per % a.BM);
@@ -754,7 +759,7 @@ __device__ __forceinline__ void proj_join(const ProjJoin& a, int64_t i) {
         }
     }
     if (KIND != PJ_FWD_CK && !in) return;
-    const uint32_t exp = proj_epilogue<KIND, 8>(v, a.e, pre, pexp, row, col, in ? 8 : 0, a.N, codes);
+    const uint32_t exp = proj_epilogue<KIND, FAST, 8>(v, a.e, pre, pexp, row, col, in ? 8 : 0, a.N, codes);
     if (!in) return;
     if constexpr (KIND == PJ_FWD_CK) {
         *reinterpret_cast<uint2*>(a.e.codes + at) = make_uint2(codes[0], codes[1]);
@@ -788,11 +793,11 @@ struct ColJoin {
     int N, slices, bf16;
 };
 constexpr int PJ_JOIN_T = 128;
-template <int KIND>
+template <int KIND, bool FAST>
 __global__ void __launch_bounds__(PJ_JOIN_T) proj_join_kernel(const ProjJoin a, const ColJoin c, int first) {
     pdl_wait();
     if ((int)blockIdx.x < first) {
-        proj_join<KIND>(a, blockIdx.x * (int64_t)PJ_JOIN_T + threadIdx.x);
+        proj_join<KIND, FAST>(a, blockIdx.x * (int64_t)PJ_JOIN_T + threadIdx.x);
         return;
     }
     __shared__ float red[PJ_JOIN_T / 32][32];
@@ -872,10 +877,10 @@ inline bool proj_map_2d(CUtensorMap* m, CUtensorMapDataType type, int esize, con
                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int BN, int CG, bool AMN, bool BMN, int KIND>
+template <int BN, int CG, bool AMN, bool BMN, int KIND, bool FAST>
 inline cudaError_t proj_launch_t(const ProjArgs& a, int sm_count, bool after_own, cudaStream_t st) {
     using C = PjCfg<BN, CG, KIND>;
-    auto kern = proj_kernel<BN, CG, AMN, BMN, KIND>;
+    auto kern = proj_kernel<BN, CG, AMN, BMN, KIND, FAST>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::TOTAL);
     if (e != cudaSuccess) return e;
     const int units = a.full * a.F + (a.mt * a.nt - a.full) * a.S;
@@ -903,7 +908,7 @@ inline cudaError_t proj_launch_t(const ProjArgs& a, int sm_count, bool after_own
 // [K, N]); with `cols` the column sums beside it.  after_own: the launch before
 // this one on the stream is this call's own, of a kernel without TMEM, so that this
 // one may start its set-up beside it.
-template <bool AMN, bool BMN, int KIND>
+template <bool AMN, bool BMN, int KIND, bool FAST>
 inline cudaError_t proj_gemm(const void* A, const void* B, void* D, int64_t M, int64_t N, int64_t K, const ProjEpi& e,
                              float* ws, int* err, int* err_host, int sm_count, cudaStream_t st, bool after_own = false,
                              const ColJoin* cols = nullptr) {
@@ -937,14 +942,14 @@ inline cudaError_t proj_gemm(const void* A, const void* B, void* D, int64_t M, i
         ok = ok && proj_map_2d(&a.pmap, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, ws, p.BN, p.parts() * p.BM(), 16, 32,
                                CU_TENSOR_MAP_SWIZZLE_64B);
     if (!ok) return cudaErrorInvalidValue;
-    const cudaError_t rc = p.CG == 2 ? proj_launch_t<256, 2, AMN, BMN, KIND>(a, sm_count, after_own, st)
-                                     : proj_launch_t<128, 1, AMN, BMN, KIND>(a, sm_count, after_own, st);
+    const cudaError_t rc = p.CG == 2 ? proj_launch_t<256, 2, AMN, BMN, KIND, FAST>(a, sm_count, after_own, st)
+                                     : proj_launch_t<128, 1, AMN, BMN, KIND, FAST>(a, sm_count, after_own, st);
     if (rc != cudaSuccess || (!p.ws_bytes && !cols)) return rc;
     const ProjJoin j{ws, e, D, (int)M, (int)N, p.mt, p.nt, p.full, p.F, p.S, p.BM(), p.BN};
     const int joined = p.mt * p.nt - (p.F > 1 ? 0 : p.full);
     const int first = ceil_div((int64_t)joined * p.BM() * (p.BN / 8), PJ_JOIN_T);
     const ColJoin c = cols ? *cols : ColJoin{};
-    return launch_pdl(proj_join_kernel<KIND>, dim3(first + ceil_div(c.N, 32)), dim3(PJ_JOIN_T), 0, st, j, c, first);
+    return launch_pdl(proj_join_kernel<KIND, FAST>, dim3(first + ceil_div(c.N, 32)), dim3(PJ_JOIN_T), 0, st, j, c, first);
 }
 
 }  // namespace rwkv

@@ -47,7 +47,7 @@ __device__ __forceinline__ void mma_16816(float* c, uint32_t a0, uint32_t a1, ui
 }
 
 // NT: groups of 8 activation rows; NW warps; MT groups of 16 outputs.
-template <bool BF16, int NT, int NW, int MT>
+template <bool BF16, int NT, int NW, int MT, bool FAST>
 __global__ void __launch_bounds__(NW * 32, 1) gemv_proj_kernel(const GemvProjArgs a) {
     constexpr int O = 16 * MT, U = GP_U;
     __shared__ float red[NW][8 * NT][O + 1];
@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(NW * 32, 1) gemv_proj_kernel(const GemvProjArg
         };
         if (a.e.z) store(a.e.z, z);
         float y = z;
-        with_act(a.e.act, [&]<int ACT>() { y = act_t<ACT, true>(z); });
+        with_act(a.e.act, [&]<int ACT>() { y = act_t<ACT, FAST>(z); });
         if (a.e.add) y += load_param(a.e.add, a.e.out_f32 ? RWKV_F32 : BF16 ? RWKV_BF16 : RWKV_F16, at);
         if (a.e.out_f32) static_cast<float*>(a.y)[at] = y;
         else store(a.y, y);
@@ -118,20 +118,25 @@ __global__ void __launch_bounds__(NW * 32, 1) gemv_proj_kernel(const GemvProjArg
 }
 
 // 8 warps where that already gives an SM two blocks, else 16.
-template <bool BF16, int NT, int MT>
+template <bool BF16, int NT, int MT, bool FAST>
 inline void launch_gemv_proj_t(const GemvProjArgs& a, int sm_count, cudaStream_t st) {
     const int grid = ceil_div(a.OUT, 16 * MT);
-    if (ceil_div(a.OUT, 16) < 2 * sm_count) gemv_proj_kernel<BF16, NT, 16, MT><<<grid, 512, 0, st>>>(a);
-    else gemv_proj_kernel<BF16, NT, 8, MT><<<grid, 256, 0, st>>>(a);
+    if (ceil_div(a.OUT, 16) < 2 * sm_count) gemv_proj_kernel<BF16, NT, 16, MT, FAST><<<grid, 512, 0, st>>>(a);
+    else gemv_proj_kernel<BF16, NT, 8, MT, FAST><<<grid, 256, 0, st>>>(a);
+}
+template <bool BF16, bool FAST>
+inline void launch_gemv_proj_f(const GemvProjArgs& a, int sm_count, cudaStream_t st) {
+    const bool two = a.rows > 8, ck = a.e.codes != nullptr;
+    if (two && ck) launch_gemv_proj_t<BF16, 2, 2, FAST>(a, sm_count, st);
+    else if (two) launch_gemv_proj_t<BF16, 2, 1, FAST>(a, sm_count, st);
+    else if (ck) launch_gemv_proj_t<BF16, 1, 2, FAST>(a, sm_count, st);
+    else launch_gemv_proj_t<BF16, 1, 1, FAST>(a, sm_count, st);
 }
 inline cudaError_t launch_gemv_proj(const GemvProjArgs& a, int sm_count, cudaStream_t st) {
-    const bool two = a.rows > 8, ck = a.e.codes != nullptr;
-#define GP_(B) \
-    (two ? ck ? launch_gemv_proj_t<B, 2, 2>(a, sm_count, st) : launch_gemv_proj_t<B, 2, 1>(a, sm_count, st) \
-         : ck ? launch_gemv_proj_t<B, 1, 2>(a, sm_count, st) : launch_gemv_proj_t<B, 1, 1>(a, sm_count, st))
-    if (a.e.bf16) GP_(true);
-    else GP_(false);
-#undef GP_
+    if (a.e.bf16 && a.e.fast()) launch_gemv_proj_f<true, true>(a, sm_count, st);
+    else if (a.e.bf16) launch_gemv_proj_f<true, false>(a, sm_count, st);
+    else if (a.e.fast()) launch_gemv_proj_f<false, true>(a, sm_count, st);
+    else launch_gemv_proj_f<false, false>(a, sm_count, st);
     return cudaGetLastError();
 }
 

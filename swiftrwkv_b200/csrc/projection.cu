@@ -111,11 +111,12 @@ int col_slices(int rows, int OUT) {
 
 template <typename F>
 cudaError_t by_kind(const ProjEpi& e, F&& f) {
+    const bool fast = e.fast();
     switch (e.kind()) {
-        case PJ_GRAD: return f.template operator()<PJ_GRAD>();
-        case PJ_FWD_CK: return f.template operator()<PJ_FWD_CK>();
-        case PJ_FWD: return f.template operator()<PJ_FWD>();
-        default: return f.template operator()<PJ_PLAIN>();
+        case PJ_GRAD: return fast ? f.template operator()<PJ_GRAD, true>() : f.template operator()<PJ_GRAD, false>();
+        case PJ_FWD_CK: return fast ? f.template operator()<PJ_FWD_CK, true>() : f.template operator()<PJ_FWD_CK, false>();
+        case PJ_FWD: return fast ? f.template operator()<PJ_FWD, true>() : f.template operator()<PJ_FWD, false>();
+        default: return f.template operator()<PJ_PLAIN, true>();
     }
 }
 
@@ -187,9 +188,9 @@ extern "C" int rwkv_projection_forward(int dtype, const void* x, const void* w, 
     e.z = z;
     const cudaError_t rc =
         few ? launch_gemv_proj(GemvProjArgs{x, w, y, e, rows, OUT, IN}, sms, (cudaStream_t)stream)
-            : by_kind(e, [&]<int KIND>() {
-                  return proj_gemm<false, false, KIND>(x, w, y, rows, OUT, IN, e, static_cast<float*>(workspace), err,
-                                                       err_host, sms, (cudaStream_t)stream);
+            : by_kind(e, [&]<int KIND, bool FAST>() {
+                  return proj_gemm<false, false, KIND == PJ_GRAD ? PJ_PLAIN : KIND, KIND == PJ_GRAD || FAST>(  // no gradient
+                      x, w, y, rows, OUT, IN, e, static_cast<float*>(workspace), err, err_host, sms, (cudaStream_t)stream);
               });
     if (rc != cudaSuccess) return fail(RWKV_E_CUDA, "%s: %s", fn, cudaGetErrorString(rc));
     return ok();
@@ -224,8 +225,9 @@ extern "C" int rwkv_projection_dx(int dtype, const void* dy, const void* w, int 
     e.pre_codes = codes;
     e.pre_exps = exps;
     e.add = addend;
-    const cudaError_t rc = by_kind(e, [&]<int KIND>() {
-        return proj_gemm<false, true, KIND == PJ_FWD_CK ? PJ_FWD : KIND>(  // never keeps a checkpoint
+    const cudaError_t rc = by_kind(e, [&]<int KIND, bool FAST>() {
+        // (never keeps a checkpoint; an activation only as its gradient)
+        return proj_gemm<false, true, KIND == PJ_FWD_CK ? PJ_FWD : KIND, KIND != PJ_GRAD || FAST>(
             dy, w, dx, rows, IN, OUT, e, static_cast<float*>(workspace), err, err_host, sms, (cudaStream_t)stream);
     });
     if (rc != cudaSuccess) return fail(RWKV_E_CUDA, "%s: %s", fn, cudaGetErrorString(rc));
@@ -297,10 +299,10 @@ extern "C" int rwkv_projection_dw(int dtype, const void* dy, int act, const void
         ProjEpi e{};
         e.bf16 = q.bf16;
         e.out_f32 = dwdtype == RWKV_F32;
-        rc = proj_gemm<true, true, PJ_PLAIN>(dy, restore ? ws : x, dw, OUT, IN, rows, e, reinterpret_cast<float*>(ws + p.operand),
+        rc = proj_gemm<true, true, PJ_PLAIN, true>(dy, restore ? ws : x, dw, OUT, IN, rows, e, reinterpret_cast<float*>(ws + p.operand),
                                    err, err_host, sms, st, grid != 0, db ? &cols : nullptr);
     } else {
-        rc = launch_pdl(proj_join_kernel<PJ_PLAIN>, dim3(ceil_div(OUT, 32)), dim3(PJ_JOIN_T), 0, st, ProjJoin{}, cols, 0);
+        rc = launch_pdl(proj_join_kernel<PJ_PLAIN, true>, dim3(ceil_div(OUT, 32)), dim3(PJ_JOIN_T), 0, st, ProjJoin{}, cols, 0);
     }
     if (rc != cudaSuccess) return fail(RWKV_E_CUDA, "%s: %s", fn, cudaGetErrorString(rc));
     return ok();

@@ -1083,3 +1083,28 @@ def test_projection_sums_too_long_for_one_accumulator(cuda, what, rows):
            "dw": lambda: B.projectionBackwardWeight(a, b, out_dtype=torch.float32)[0]}[what]()
     want = torch.full((rows, n), 1.0 + (K - 1) * small * 2.0 ** -13, device="cuda", dtype=torch.float64)
     check(got, want, (2048 * 5 * 2.0 ** -23 + K / 32768 * U32 + U32) * want, what)
+
+
+@pytest.mark.parametrize("rows,n,K", [(5, 1024, 8), (200, 1024, 8), (40, 264, 4096), (2304, 2304, 576)])
+@pytest.mark.parametrize("act", ["tanh", "sigmoid"])
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+def test_projection_fp32_results_of_activations(cuda, dt, act, rows, n, K):
+    """Sums of one product, exact in fp32, so that what is off is the function.  CUDA
+    gives expf and tanhf to 2 ulp, 2^-22 relative.  sigmoid = 1 / (1 + e): 2^-22 from
+    e, 2^-24 for the sum and for the quotient.  The derivatives k^2 e / (1 + e)^2:
+    2^-22 from e above; below, e's share of 1 + e is half at most, twice with a
+    rounding of 2^-24 each; 2^-24 each for the square, the quotient and the product
+    with the sum: (1 + 1 + 5 / 4) 2^-22."""
+    from swiftrwkv_b200 import block as B
+    t, f32 = DTYPES[dt], torch.float32
+    x, w = torch.zeros(rows, K, device="cuda", dtype=t), torch.zeros(n, K, device="cuda", dtype=t)
+    x[:, K // 2] = torch.linspace(0.5, 1, rows, device="cuda").to(t)
+    w[:, K // 2] = torch.cat([torch.linspace(-12, 12, n // 2), torch.linspace(-0.1, 0.1, n - n // 2)]).cuda().to(t)
+    z = x.double() @ w.double().t()
+    want = act64(z, act)
+    check(B.projectionForward(x, w, act=act, out_dtype=f32)[0], want, (1.0 if act == "tanh" else 1.5) * 2.0 ** -22 * want.abs())
+    pre = z.to(t)
+    want = x.double()[:, K // 2:K // 2 + 1] * grad64(pre.double(), act)
+    ones = torch.zeros(K, n, device="cuda", dtype=t)
+    ones[K // 2] = 1
+    check(B.projectionBackwardInput(x, ones, pre=pre, act=act, out_dtype=f32), want, 3.25 * 2.0 ** -22 * want.abs())
