@@ -46,7 +46,7 @@ enum { RWKV_F32 = 0, RWKV_BF16 = 1, RWKV_F16 = 2 };
 
 /* activations of the projection epilogue: z, max(z, 0)^2, tanh z, 1 / (1 + e^-z).
  * tanh, sigmoid and their derivatives are within 2^-20 (relative) of the argument's
- * where the result is fp32, within 2^-18 before the rounding to 16 bits. */
+ * where the result is fp32, within 2^-16 before the rounding to 16 bits. */
 enum { RWKV_ACT_NONE = 0, RWKV_ACT_RELU2 = 1, RWKV_ACT_TANH = 2, RWKV_ACT_SIGMOID = 3 };
 
 #define RWKV_WKV7_HEAD_SIZE 64 /* WKV7_HEAD_SIZE, Sources/RWKVKernel/WKV7.swift:7 */

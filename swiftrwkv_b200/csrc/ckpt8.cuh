@@ -96,9 +96,9 @@ __device__ __forceinline__ void ck_unpack4(uint32_t w, float s, float* v) {
 //   sigmoid = (1 or e) / (1 + e) by z's sign, sigmoid' = e / (1 + e)^2
 // FAST: __expf (2 + |1.16 x| ulp) and __fdividef (2 ulp), for results that are rounded
 // to 16 bits: tanh within 2^-18 relative (at |z| = 2^-6, where 1 - e = 2^-5 is off by
-// 2^-23 from e), sigmoid and the derivatives within 2^-19 up to |z| = 10; below |z| =
-// 2^-6, where 1 - e cancels further, tanh z = z - z^3 / 3 (next term z^5 2/15 < 2^-26 z).
-// Otherwise expf, tanhf and IEEE division.
+// 2^-23 from e), sigmoid and the derivatives as e, 2^-18 at |z| = 10 and 2^-16 where
+// bf16 ends; below |z| = 2^-6, where 1 - e cancels further, tanh z = z - z^3 / 3 (next
+// term z^5 2/15 < 2^-26 z).  Otherwise expf, tanhf and IEEE division.
 template <int ACT, bool FAST>
 __device__ __forceinline__ float act_t(float z) {
     if constexpr (ACT == RWKV_ACT_RELU2) {
@@ -110,9 +110,8 @@ __device__ __forceinline__ float act_t(float z) {
         const float t = copysignf(__fdividef(1.f - e, 1.f + e), z);
         return fabsf(z) < 0.015625f ? fmaf(z * z * z, -1.f / 3.f, z) : t;
     } else if constexpr (ACT == RWKV_ACT_SIGMOID) {
-        if constexpr (!FAST) return 1.f / (1.f + expf(-z));
-        const float e = __expf(-fabsf(z));
-        return __fdividef(z < 0.f ? e : 1.f, 1.f + e);
+        const float e = FAST ? __expf(-fabsf(z)) : expf(-fabsf(z)), n = z < 0.f ? e : 1.f;
+        return FAST ? __fdividef(n, 1.f + e) : n / (1.f + e);
     }
     return z;
 }

@@ -1108,3 +1108,18 @@ def test_projection_fp32_results_of_activations(cuda, dt, act, rows, n, K):
     ones = torch.zeros(K, n, device="cuda", dtype=t)
     ones[K // 2] = 1
     check(B.projectionBackwardInput(x, ones, pre=pre, act=act, out_dtype=f32), want, 3.25 * 2.0 ** -22 * want.abs())
+
+
+def test_sigmoid_of_far_negative_values_in_fp32(cuda):
+    """e^z below the normal numbers is kept to half of their spacing 2^-149 and the
+    2 ulp of expf, where 1 / (1 + e^-z) would overflow to 0."""
+    from swiftrwkv_b200 import block as B
+    z = torch.linspace(-103, -60, 87, device="cuda").to(torch.bfloat16)
+    x, w = torch.ones(20, 8, device="cuda", dtype=torch.bfloat16) / 8, z[:80, None].expand(80, 8).contiguous()
+    want = act64(z.double(), "sigmoid")
+    y = B.projectionForward(x, w, act="sigmoid", out_dtype=torch.float32)[0]
+    assert bool(((y.double() - want[:80]).abs() <= 1.5 * 2.0 ** -22 * want[:80] + 2 * 2.0 ** -149).all())
+    ck = B.checkpoint8(z[:, None].contiguous())        # one channel: 7 bits hold every value
+    want = act64(B.checkpoint8Values(ck, dtype=torch.float32).double(), "sigmoid")
+    y = B.checkpoint8Values(ck, act="sigmoid", dtype=torch.float32)
+    assert bool(((y.double() - want).abs() <= 1.5 * 2.0 ** -22 * want + 2 * 2.0 ** -149).all()) and bool((y > 0).all())
