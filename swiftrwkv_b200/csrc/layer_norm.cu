@@ -970,6 +970,9 @@ __global__ void __launch_bounds__(1024) ln_bwd_params_kernel(const float* __rest
 }
 
 constexpr int LN_BWD_BLOCKS = 148 * 4;  // at most: four resident blocks per SM
+constexpr int LN_LONG_BLOCKS = 64;      // column sums of the rows that only the long kernels take
+// 512 threads with three vectors of 8 each, or 20 single elements
+constexpr int LN_BWD_VECTORS = 512 * 3, LN_BWD_ELEMENTS = 512 * 20;
 
 template <typename T, bool CK, int NV, int R, int MAXT, int MINB, bool SH>
 cudaError_t launch_ln_bwd_t(const LnBwdArgs& a, int* blocks, cudaStream_t st) {
@@ -994,7 +997,7 @@ template <typename T, bool CK, bool SH>
 int launch_ln_bwd(LnBwdArgs a, bool vec, void* dw, void* db, cudaStream_t st) {
     const int nvec = SH ? most_vectors<T>(a.D) : a.D / Vec16<T>::N;
     int blocks;
-    if (vec && nvec <= 512 * 3) {
+    if (vec && nvec <= LN_BWD_VECTORS) {
         // vectors per thread: the fewest with at most 512 threads.  Two rows
         // at a time from a dense x (16384 x 2048 bf16: 50 us, one row 65 us), one
         // from a checkpoint, whose decoding takes more registers (2560 channels: 68
@@ -1007,7 +1010,7 @@ int launch_ln_bwd(LnBwdArgs a, bool vec, void* dw, void* db, cudaStream_t st) {
                               : nvec > 320 ? launch_ln_bwd_t<T, CK, 1, R, 512, 1, SH>(a, &blocks, st)
                                            : launch_ln_bwd_t<T, CK, 1, R, 320, 2, SH>(a, &blocks, st);
         if (e != cudaSuccess) return fail(RWKV_E_CUDA, "ln_bwd_kernel: %s", cudaGetErrorString(e));
-    } else if (a.D <= 512 * 20) {
+    } else if (a.D <= LN_BWD_ELEMENTS) {
         blocks = std::min(a.rows, LN_BWD_BLOCKS);
         if (a.D <= 256) ln_bwd_any_kernel<T, CK, 256, 1><<<blocks, 256, 0, st>>>(a);
         else if (a.D <= 256 * 2) ln_bwd_any_kernel<T, CK, 256, 2><<<blocks, 256, 0, st>>>(a);
@@ -1018,7 +1021,7 @@ int launch_ln_bwd(LnBwdArgs a, bool vec, void* dw, void* db, cudaStream_t st) {
         else if (a.D <= 512 * 12) ln_bwd_any_kernel<T, CK, 512, 12><<<blocks, 512, 0, st>>>(a);
         else ln_bwd_any_kernel<T, CK, 512, 20><<<blocks, 512, 0, st>>>(a);
     } else {
-        blocks = std::min(a.rows, 64);
+        blocks = std::min(a.rows, LN_LONG_BLOCKS);
         if (a.part) {
             ln_bwd_cols_kernel<T, CK><<<dim3(ceil_div(a.D, 256), blocks), 256, 0, st>>>(a);
             if (int rc = check_launch("ln_bwd_cols_kernel")) return rc;
@@ -1071,7 +1074,9 @@ extern "C" int rwkv_layer_norm_forward(int dtype, const void* x, int wdtype, con
 
 extern "C" int64_t rwkv_layer_norm_backward_workspace_size(int rows, int D) {
     if (rows < 1 || D < 1) return 0;
-    return (int64_t)std::min(rows, LN_BWD_BLOCKS) * 2 * D * (int64_t)sizeof(float);
+    // (whatever the type and the alignment)
+    const int blocks = D > std::max(LN_BWD_VECTORS * 8, LN_BWD_ELEMENTS) ? LN_LONG_BLOCKS : LN_BWD_BLOCKS;
+    return (int64_t)std::min(rows, blocks) * 2 * D * (int64_t)sizeof(float);
 }
 
 extern "C" int rwkv_layer_norm_backward(int dtype, const void* dy, const void* x, const int8_t* codes,

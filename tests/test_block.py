@@ -264,3 +264,13 @@ def test_differentiable_forms_refuse_what_is_no_tensor():
         for name in args:
             with pytest.raises(ValueError, match="CUDA tensor"):
                 f(**{**args, name: [1.0]})
+
+
+def test_layer_norm_workspace_of_long_rows():
+    """Rows longer than the vector kernels take sum their columns in 64 blocks at
+    most, and ask for no more."""
+    size = _lib.lib().rwkv_layer_norm_backward_workspace_size
+    assert size(4096, 65536) == 64 * 2 * 65536 * 4
+    assert size(4096, 12289) == 64 * 2 * 12289 * 4
+    assert size(40, 65536) == 40 * 2 * 65536 * 4
+    assert size(4096, 12288) == 592 * 2 * 12288 * 4    # 16-bit rows of 1536 vectors

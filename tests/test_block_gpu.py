@@ -1123,3 +1123,10 @@ def test_sigmoid_of_far_negative_values_in_fp32(cuda):
     want = act64(B.checkpoint8Values(ck, dtype=torch.float32).double(), "sigmoid")
     y = B.checkpoint8Values(ck, act="sigmoid", dtype=torch.float32)
     assert bool(((y.double() - want).abs() <= 1.5 * 2.0 ** -22 * want + 2 * 2.0 ** -149).all()) and bool((y > 0).all())
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,D", [(150, 12289), (131, 16384), (65, 33000)])
+def test_layer_norm_of_long_rows_in_more_rows_than_blocks(cuda, dt, rows, D):
+    test_layer_norm_backward(cuda, dt, False, rows, D)
+    test_layer_norm_backward(cuda, dt, True, rows, D)
