@@ -72,10 +72,15 @@ class Checkpoint8:
 # come from empty_like or new_empty(*sizes): 1.3 to 1.5 us, where new_empty(tuple)
 # takes 1.8 to 2.1 and torch.empty(tuple) 2.2.
 
+def _public_raw_stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
 # what torch.cuda.current_device() and current_stream(...).cuda_stream return,
-# without building a Stream object (2 us of a small call's 10)
-_current_device = torch._C._cuda_getDevice
-_raw_stream = torch._C._cuda_getCurrentRawStream
+# without building a Stream object (2 us of a small call's 10); a torch without
+# CUDA has neither of these names
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _public_raw_stream)
 
 
 def _call(dev, name, *args):

@@ -3,6 +3,9 @@ checkpoints): every refusal happens on the host, before anything launches."""
 from __future__ import annotations
 
 import ctypes
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -274,3 +277,19 @@ def test_layer_norm_workspace_of_long_rows():
     assert size(4096, 12289) == 64 * 2 * 12289 * 4
     assert size(40, 65536) == 40 * 2 * 65536 * 4
     assert size(4096, 12288) == 592 * 2 * 12288 * 4    # 16-bit rows of 1536 vectors
+
+
+def test_a_torch_without_cuda_imports_and_refuses():
+    code = """
+import torch
+for name in ("_cuda_getDevice", "_cuda_getCurrentRawStream"):
+    delattr(torch._C, name)
+from swiftrwkv_b200 import block as B
+try:
+    B.checkpoint8(torch.zeros(4, 64))
+except ValueError as e:
+    print(e)
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(_lib.__file__)))
+    got = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert got.returncode == 0 and "a CUDA tensor is needed" in got.stdout, got.stderr

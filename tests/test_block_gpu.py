@@ -1130,3 +1130,18 @@ def test_sigmoid_of_far_negative_values_in_fp32(cuda):
 def test_layer_norm_of_long_rows_in_more_rows_than_blocks(cuda, dt, rows, D):
     test_layer_norm_backward(cuda, dt, False, rows, D)
     test_layer_norm_backward(cuda, dt, True, rows, D)
+
+
+def test_streams_by_public_names_alone(cuda, monkeypatch):
+    from swiftrwkv_b200 import block as B
+    x = rnd((5, 96), 95, torch.bfloat16)
+    want = B.checkpoint8(x).codes
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        assert B._public_raw_stream(0) == B._raw_stream(0) == s.cuda_stream
+        monkeypatch.setattr(B, "_raw_stream", B._public_raw_stream)
+        monkeypatch.setattr(B, "_current_device", torch.cuda.current_device)
+        got = B.checkpoint8(x).codes
+    s.synchronize()
+    assert torch.equal(got, want)
