@@ -115,7 +115,9 @@ inline int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 // Programmatic dependent launch.  A kernel launched with launch_pdl may start
 // while its predecessor in the stream is still running: it must call
 // pdl_wait() before it reads or writes anything the predecessor touches
-// (outside a PDL launch both are no-ops).  pdl_trigger() lets the successor
+// (outside a PDL launch both are no-ops).  Its pointers to the predecessor's results
+// are not const __restrict__: that would promise that they are only read for the
+// whole kernel, and loads of them could move above the wait.  pdl_trigger() lets the successor
 // launch once every CTA of this grid has issued it.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }

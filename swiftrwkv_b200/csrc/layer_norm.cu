@@ -947,7 +947,7 @@ __global__ void __launch_bounds__(256) ln_bwd_cols_kernel(const LnBwdArgs a) {
 // out[c] = sum over the blocks of part[block][c], c < 2D (dweight, dbias): 32
 // columns per block, 32 interleaved slices of the partials, in a fixed order.
 // Launched to start beside the row kernel's end (pdl_wait).
-__global__ void __launch_bounds__(1024) ln_bwd_params_kernel(const float* __restrict__ part, int blocks, int D,
+__global__ void __launch_bounds__(1024) ln_bwd_params_kernel(const float* part, int blocks, int D,
                                                              void* dw, void* db, int wdtype) {
     __shared__ float red[32][33];
     const int col = threadIdx.x & 31, slice = threadIdx.x >> 5;

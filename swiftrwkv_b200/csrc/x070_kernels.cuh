@@ -64,7 +64,7 @@ __device__ __forceinline__ void ln_regs(float v[GLUE_PER], int C, const float* _
 // ids -> x = ln0(emb[id]).  Embedding in the 4-bit group-64 container
 // (emb_wq != NULL) or dense bf16.
 __global__ void __launch_bounds__(GLUE_T)
-x070_embed_kernel(const int32_t* __restrict__ ids, const uint32_t* __restrict__ emb_wq,
+x070_embed_kernel(const int32_t* ids, const uint32_t* __restrict__ emb_wq,
                   const __half* __restrict__ emb_sc, const __half* __restrict__ emb_bi,
                   const __nv_bfloat16* __restrict__ emb_dense, const float* __restrict__ lnw,
                   const float* __restrict__ lnb, float* __restrict__ x, int C, int vocab) {
@@ -151,7 +151,7 @@ __device__ __forceinline__ float4 sub4(float4 a, float4 b) {
 // programmatic-launch wait; x and the shift row after it, in one round trip.
 template <typename A, int GV>
 __global__ void __launch_bounds__(GLUE_T)
-x070_tmix_in_kernel(const float* __restrict__ x, const float* __restrict__ lnw,
+x070_tmix_in_kernel(const float* x, const float* __restrict__ lnw,
                     const float* __restrict__ lnb, float* __restrict__ shift,
                     const float* __restrict__ coef, A* __restrict__ mix, int R, int C) {
     __shared__ float sh[33];
@@ -182,7 +182,7 @@ x070_tmix_in_kernel(const float* __restrict__ x, const float* __restrict__ lnw,
 // cmix input: xl = ln2(x); xx = shift - xl; shift = xl; out = xl + xx * coef.
 template <typename A, int GV>
 __global__ void __launch_bounds__(GLUE_T)
-x070_cmix_in_kernel(const float* __restrict__ x, const float* __restrict__ lnw,
+x070_cmix_in_kernel(const float* x, const float* __restrict__ lnw,
                     const float* __restrict__ lnb, float* __restrict__ shift,
                     const float* __restrict__ coef, A* __restrict__ out, int C) {
     __shared__ float sh[33];
@@ -210,7 +210,7 @@ x070_cmix_in_kernel(const float* __restrict__ x, const float* __restrict__ lnw,
 
 template <typename A, int GV>
 __global__ void __launch_bounds__(GLUE_T)
-x070_ln_out_kernel(const float* __restrict__ x, const float* __restrict__ lnw,
+x070_ln_out_kernel(const float* x, const float* __restrict__ lnw,
                    const float* __restrict__ lnb, A* __restrict__ out, int C) {
     __shared__ float sh[33];
     const int n = blockIdx.x;
@@ -241,13 +241,13 @@ x070_ln_out_kernel(const float* __restrict__ x, const float* __restrict__ lnw,
 // in the prologue, so a CTA waits on global memory about once.
 template <typename A>
 __global__ void __launch_bounds__(128)
-x070_wkv_kernel(const float* __restrict__ r, const float* __restrict__ wdec,
-                const float* __restrict__ kraw, const float* __restrict__ vraw,
-                const float* __restrict__ a, const float* __restrict__ vv,
+x070_wkv_kernel(const float* r, const float* wdec,
+                const float* kraw, const float* vraw,
+                const float* a, const float* vv,
                 float* __restrict__ vfirst, const float* __restrict__ kkw,
                 const float* __restrict__ kaw, const float* __restrict__ rkw,
                 const float* __restrict__ lnxw, const float* __restrict__ lnxb,
-                const float* __restrict__ g, float* __restrict__ state, A* __restrict__ out,
+                const float* g, float* __restrict__ state, A* __restrict__ out,
                 int H, int layer0) {
     constexpr int N = 64, RPW = 16;  // rows per warp
     __shared__ __align__(16) float r_s[N], w_s[N], kp_s[N], aw_s[N], bw_s[N], v_s[N], y_s[N];
@@ -544,7 +544,7 @@ __device__ __forceinline__ unsigned long long argmax_key(float v, int idx) {
 constexpr int ARGMAX_SLICE = 4096;
 
 __global__ void __launch_bounds__(GLUE_T)
-x070_argmax_kernel(const float* __restrict__ logits, int V, unsigned long long* __restrict__ keys) {
+x070_argmax_kernel(const float* logits, int V, unsigned long long* __restrict__ keys) {
     pdl_wait();  // launched as a programmatic dependent: predecessor outputs first
     pdl_trigger();
     __shared__ unsigned long long sk[GLUE_T / 32];
@@ -641,7 +641,7 @@ gemv_cc_kernel(const GemvJobs jobs, int R) {
 // relu(h)^2 into the activation type: the cmix key output when a LoRA
 // adapter is added before the activation (n = rows * ffn).
 template <typename A>
-__global__ void __launch_bounds__(256) x070_relu2_cast_kernel(const float* __restrict__ h, A* __restrict__ out,
+__global__ void __launch_bounds__(256) x070_relu2_cast_kernel(const float* h, A* __restrict__ out,
                                                               int n) {
     pdl_trigger();
     pdl_wait();

@@ -140,3 +140,23 @@ def test_shared_memory_limits_do_not_follow_a_call():
                 found += 1
                 assert not re.search(r"\bsmem\b", size), f"{name}: {size}"
     assert found > 10
+
+
+def test_dependent_launches_promise_nothing_about_their_predecessor():
+    """const __restrict__ says that memory is only read for a whole kernel, which lets
+    its loads move above the wait for the kernel that writes it.  Kernels launched as
+    programmatic dependents have it on weights and parameters alone."""
+    weights = {"emb_wq", "emb_sc", "emb_bi", "emb_dense", "lnw", "lnb", "coef", "kkw", "kaw", "rkw", "lnxw", "lnxb"}
+    csrc = os.path.join(os.path.dirname(_lib.__file__), "csrc")
+    text = ""
+    for name in sorted(os.listdir(csrc)):
+        with open(os.path.join(csrc, name)) as f:
+            text += f.read()
+    dependent = set(re.findall(r"launch_pdl\((\w+_kernel)\b", text))
+    assert {"ln_bwd_params_kernel", "proj_join_kernel", "x070_wkv_kernel"} <= dependent
+    for name in dependent:
+        signatures = re.findall(rf"__global__[^;{{]*?\b{name}\(([^{{;]*?)\)\s*{{", text)
+        assert signatures, name
+        for args in signatures:
+            promised = set(re.findall(r"const [\w ]+\*\s*__restrict__ (\w+)", args))
+            assert promised <= weights, f"{name}: {promised - weights}"
