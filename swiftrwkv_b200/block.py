@@ -83,6 +83,10 @@ _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _public_raw_stream)
 
 
+# what the entry points find wrong with arguments that the checks here let pass (eps, sizes)
+_BAD_ARGUMENT = (_lib.E_NULL, _lib.E_SHAPE, _lib.E_DTYPE, _lib.E_UNSUPPORTED)
+
+
 def _call(dev, name, *args):
     """An entry point on `dev` and its current stream (appended)."""
     L = _lib.lib()
@@ -92,6 +96,8 @@ def _call(dev, name, *args):
     else:
         with torch.cuda.device(dev):
             st = getattr(L, name)(*args, _raw_stream(k))
+    if st in _BAD_ARGUMENT:
+        raise ValueError(L.rwkv_last_error().decode())
     if st:
         raise _lib.RWKVError(name, st, L.rwkv_last_error().decode())
 

@@ -293,3 +293,15 @@ except ValueError as e:
     root = os.path.dirname(os.path.dirname(os.path.abspath(_lib.__file__)))
     got = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
     assert got.returncode == 0 and "a CUDA tensor is needed" in got.stdout, got.stderr
+
+
+def test_projections_of_more_than_2_24_rows_are_refused():
+    """2^24 rows are taken (here as far as the missing workspace), one more is not."""
+    L, rows = _lib.lib(), 1 << 24
+    for n, status in ((rows, _lib.E_WORKSPACE), (rows + 1, _lib.E_SHAPE)):
+        assert proj_dw(rows=n, OUT=64, IN=64, ws=None, n=0) == status
+    assert proj_fwd(rows=rows + 1, OUT=64, IN=64) == _lib.E_SHAPE
+    assert proj_dx(rows=rows + 1, OUT=64, IN=64) == _lib.E_SHAPE
+    # an accumulator takes 32768 rows: 512 splits of a 128 x 128 tile and the column sums
+    assert L.rwkv_projection_dw_workspace_size(rows, 64, 64, 0) >= 512 * 128 * 128 * 4
+    assert L.rwkv_projection_dw_workspace_size(rows + 1, 64, 64, 0) == 0

@@ -1145,3 +1145,25 @@ def test_streams_by_public_names_alone(cuda, monkeypatch):
         got = B.checkpoint8(x).codes
     s.synchronize()
     assert torch.equal(got, want)
+
+
+def test_what_the_entry_points_refuse_is_a_value_error(cuda):
+    """Arguments that only the C entry points check: eps, and sizes past the limits."""
+    from swiftrwkv_b200 import block as B
+    t = torch.bfloat16
+    x, v = rnd((4, 64), 96, t), torch.ones(64, device="cuda")
+    for eps in (-1.0, float("nan")):
+        with pytest.raises(ValueError, match="eps"):
+            B.layerNormForward(x, v, v, eps)
+    w = torch.zeros(8, 8, device="cuda", dtype=t)
+    many = torch.zeros((1 << 24) + 1, 8, device="cuda", dtype=t)
+    for f in (lambda: B.projectionForward(many, w), lambda: B.projectionBackwardInput(many, w),
+              lambda: B.projectionBackwardWeight(many, many)):
+        with pytest.raises(ValueError, match="too large"):
+            f()
+    del many
+    wide = torch.zeros((1 << 30) + 8, device="cuda", dtype=t)
+    with pytest.raises(ValueError, match="1..2\\^30"):
+        B.checkpoint8(wide)
+    with pytest.raises(ValueError, match="1..2\\^30"):
+        B.layerNormForward(wide, wide, wide)
