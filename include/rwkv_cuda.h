@@ -590,8 +590,12 @@ int rwkv_projection_dx(int dtype, const void* dy, const void* w, int act, const 
 /* dW [OUT, IN] = dY^T act(X) in dwdtype (dtype or F32), and db [OUT] = sum over
  * rows of dY, fp32; either may be NULL (without dW, X is not read).  X [rows,
  * IN]: dense in dtype, or codes / exps its 8-bit checkpoint.  act(X) is rounded
- * to dtype, the type the tensor cores take (a checkpoint's values are exact there, so only act !=
- * RWKV_ACT_NONE rounds).  `restore` of the workspace query: nonzero when act !=
+ * to dtype, the type the tensor cores take, whatever dwdtype is.  In BF16 a
+ * checkpoint's values are exact, so only act != RWKV_ACT_NONE rounds; in F16
+ * they are between 2^-14 and 65504: smaller ones round to multiples of 2^-24,
+ * larger ones (a checkpoint is taken from fp32 sums) are infinite, as RELU2 is
+ * from |z| = 256 on (its forward in F16 too), and dW then is infinite, or NaN
+ * where dY is 0.  `restore` of the workspace query: nonzero when act !=
  * RWKV_ACT_NONE or X comes as a checkpoint. */
 int64_t rwkv_projection_dw_workspace_size(int rows, int OUT, int IN, int restore);
 int rwkv_projection_dw(int dtype, const void* dy, int act, const void* x, const int8_t* codes, const uint8_t* exps,

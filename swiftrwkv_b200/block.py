@@ -389,7 +389,8 @@ def projectionBackwardWeight(dy, x, act: str = "none", bias: bool = False, out_d
     `out_dtype` fp32), db [OUT] fp32 = sum over rows of dy (None without
     `bias`).  x [..., IN]: the projection's input, or with `act` the
     pre-activation behind it; a tensor or a Checkpoint8; None: only db (dw is
-    None)."""
+    None).  act(x) is rounded to dy's dtype for the product: in fp16 it is
+    infinite past 65504 (relu2: from x = 256 on), also with fp32 results."""
     a = _act(act)
     dy = _aligned(_some("dy", dy, _HALF))
     dev, dt = dy.device, dy.dtype

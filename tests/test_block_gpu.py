@@ -1167,3 +1167,61 @@ def test_what_the_entry_points_refuse_is_a_value_error(cuda):
         B.checkpoint8(wide)
     with pytest.raises(ValueError, match="1..2\\^30"):
         B.layerNormForward(wide, wide, wide)
+
+
+@pytest.mark.parametrize("act", ["none", "relu2", "tanh"])
+@pytest.mark.parametrize("rows,OUT,IN", [(40, 24, 96), (300, 136, 40)])
+def test_weight_gradient_of_values_at_the_ends_of_fp16(cuda, act, rows, OUT, IN):
+    """The operand is act(value) in fp16: the checkpoint's values far below 2^-14 on
+    the grid of 2^-24, and infinite past 65504 (relu2: from 256 on).  Rounded fp16
+    operands from the formula, multiplied in 64 bits, give dW to the sums' bound;
+    tanh is off by 2^-18 before its rounding, which can move it to a neighbour."""
+    from swiftrwkv_b200 import block as B
+    x = rnd((rows, IN), 97)
+    x[::3] *= 2.0 ** -19          # values around 2^-20, scales below 2^-24
+    x[1, :8], x[1, 8:16] = 70000.0, 300.0
+    dy = rnd((rows, OUT), 98, torch.float16)
+    dy[1, 0] = 0
+    packed = B.checkpoint8(x)     # as a projection keeps its fp32 sums
+    ck = B.Checkpoint8(packed.codes, packed.exps, torch.float16)
+    values = B.checkpoint8Values(ck, dtype=torch.float32).double()
+    assert float(values.abs().max()) > 65504 and 0 < float(values[values != 0].abs().min()) < 2.0 ** -24
+    operand = act64(values, act).float().to(torch.float16).double()
+    want, sums = dy.double().t() @ operand, dy.double().abs().t() @ operand.abs()
+    step = dy.double().abs().t() @ (2.0 ** -10 * operand.abs() + 2.0 ** -24) if act == "tanh" else 0
+    dw, _ = B.projectionBackwardWeight(dy, ck, act=act, out_dtype=torch.float32)
+    # columns of row 1 past the end of fp16; beside 70000 the scale is 1024, and 300 is 0
+    n = 0 if act == "tanh" else 8
+    assert torch.isnan(dw[0, :n]).all() and torch.isinf(dw[1:, :n]).all() and torch.isfinite(dw[:, n:]).all()
+    check(dw[:, n:], want[:, n:], (5 * 2.0 ** -23 * (rows / 16 + 1) * sums + U32 * want.abs() + step)[:, n:])
+
+
+def test_weight_gradient_of_fp16_squares(cuda):
+    """relu2's operand in fp16: 255^2 = 65025 rounds to 65024, 256^2 is infinite."""
+    from swiftrwkv_b200 import block as B
+    z, dy = torch.zeros(4, 8, device="cuda", dtype=torch.float16), torch.ones(4, 8, device="cuda", dtype=torch.float16)
+    z[0, 0], z[0, 1], z[0, 2] = 255, 256, -300
+    for out in (torch.float32, torch.float16):
+        dw, _ = B.projectionBackwardWeight(dy, z, act="relu2", out_dtype=out)
+        assert bool((dw[:, 0] == 65024).all()) and torch.isinf(dw[:, 1]).all() and not dw[:, 2:].any()
+
+
+@pytest.mark.parametrize("act", ["none", "relu2", "tanh", "sigmoid"])
+def test_activation_gradient_matches_differences_of_the_activation(cuda, act):
+    """act' against central differences of act, both as the library computes them from
+    a checkpoint's codes q h, h = 2^-5: off by h^2 / 6 max|act'''| (tanh: 2, sigmoid:
+    1/8, the others 0 away from the corner), by act's 2^-22 |act| over h, and by the
+    gradient's own 2^-20 |act'|."""
+    from swiftrwkv_b200 import block as B
+    h, q = 2.0 ** -5, torch.arange(-112, 112, device="cuda", dtype=torch.int8)
+    def f(shift, g):
+        codes = (q + shift).view(7, 32).contiguous()
+        return g(B.Checkpoint8(codes, torch.full((7, 1), 122, dtype=torch.uint8, device="cuda"), torch.float32)).double()
+    value = lambda ck: B.checkpoint8Values(ck, act=act)
+    up, down = f(1, value), f(-1, value)
+    got = f(0, lambda ck: B.activationBackward(torch.ones(7, 32, device="cuda"), ck, act))
+    third = {"tanh": 2.0, "sigmoid": 0.125}.get(act, 0.0)
+    tol = h * h / 6 * third + 2.0 ** -22 * torch.maximum(up.abs(), down.abs()) / h + 2.0 ** -20 * got.abs()
+    if act == "relu2":
+        tol = tol + h * (q.view(7, 32) == 0)         # ((h)^2 - 0) / 2h = h / 2 beside the corner
+    assert bool((((up - down) / (2 * h) - got).abs() <= tol).all())
