@@ -511,8 +511,9 @@ int rwkv_adamw_clip_step(float* param, float* m, float* v, const float* grad, in
  * [rows, ceil(D / 32)].  A code q stands for q * 2^(e - 127).  Per group the
  * scale is the power of two with max|x| / scale in [64, 128) (e >= 1) and
  * q = round(x / scale), ties to even, clipped to [-127, 127], so that
- * |x - value| <= max|x| / 127.5; a group holding an infinity or a NaN is
- * stored as e = 255 with codes 0 and stands for NaN.
+ * |x - value| <= max|x| / 127.5 (2^-127 where max|x| < 2^-120, whose scale
+ * stays at 2^-126); a group holding an infinity or a NaN is stored as e = 255
+ * with codes 0 and stands for NaN.
  */
 
 /* Layer norm over the last dimension: y = (x - mean) * rstd * weight + bias,

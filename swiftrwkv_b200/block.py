@@ -46,7 +46,8 @@ _MAX_WIDTH = 1 << 20  # of a projection
 class Checkpoint8:
     """An activation [..., D] in 8 bits: int8 codes [..., D] and one exponent
     byte per group of 32 channels, exps [..., ceil(D / 32)]; a code q stands
-    for q * 2^(e - 127).  `dtype` is the activation's own type."""
+    for q * 2^(e - 127), within max|x| / 127.5 of the group (2^-127 where max|x| is
+    smaller than 2^-120).  `dtype` is the activation's own type."""
     codes: torch.Tensor
     exps: torch.Tensor
     dtype: torch.dtype

@@ -6,7 +6,8 @@
 // max|x| / s in [64, 128) (E >= -126), and int8 codes q = round(x / s), ties
 // to even, clipped to [-127, 127].  x / s and s q are exact in fp32 and s q is
 // exact in bf16 (7 significant bits), so decoding into a bf16 tensor-core
-// operand loses nothing; |x - s q| <= max|x| / 127.5.  (A scale max|x| / 127
+// operand loses nothing; |x - s q| <= max|x| / 127.5, or 2^-127 where max|x| < 2^-120
+// and E stays at -126.  (A scale max|x| / 127
 // would gain up to one bit where max|x| / s is near 64, and would cost an
 // inexact product in every decode and four bytes per group instead of one.)
 // A group that holds an infinity or a NaN stands for NaN: exponent byte 255

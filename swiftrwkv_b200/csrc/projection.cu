@@ -14,9 +14,9 @@ namespace {
 // dY's columns (few and long, so they start first), the others write act(X) in the
 // operands' type (from the dense pre-activation or its checkpoint).
 //
-// Restoring the operand in a pass of its own reads and writes it once (8192 x 8192:
-// 32 us of 320); decoding inside the product would repeat the work for every 128
-// outputs of dW, 64 times here.
+// Restoring the operand in a pass of its own reads and writes it once (8192 x 8192: 50
+// us, of 232 with the product for 2048 outputs); decoding inside the product would
+// repeat the work for every 256 outputs of dW, 8 times here (not measured).
 struct DwPrep {
     const void* x;         // dense, or
     const int8_t* codes;   // its checkpoint
