@@ -1225,3 +1225,41 @@ def test_activation_gradient_matches_differences_of_the_activation(cuda, act):
     if act == "relu2":
         tol = tol + h * (q.view(7, 32) == 0)         # ((h)^2 - 0) / 2h = h / 2 beside the corner
     assert bool((((up - down) / (2 * h) - got).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("rows,n,K", [(2305, 2312, 65560), (300, 200, 131080), (1, 24, 262152), (16, 2056, 262144),
+                                      (40, 136, 32776), (4100, 2048, 40000)])
+def test_projection_of_whole_numbers_over_long_sums(cuda, rows, n, K):
+    """Operands of -1, 0 and 1: every partial sum is a whole number below 2^24, exact in
+    fp32 whatever the order and the splits, and so are the epilogue's squares,
+    bias and residual: the results are equal, tile by tile, in every direction."""
+    from swiftrwkv_b200 import block as B
+    t, f32 = torch.bfloat16, torch.float32
+    g = torch.Generator(device="cuda").manual_seed(99)
+
+    def whole(*s, most=1):
+        return torch.randint(-most, most + 1, s, generator=g, device="cuda").to(t)
+
+    def product(a, b):
+        return torch.cat([a[i:i + 512].double() @ b.double().t() for i in range(0, a.shape[0], 512)])
+
+    x, w = whole(rows, K), whole(n, K)
+    z = product(x, w)
+    assert float(z.abs().max()) < 2 ** 11
+    assert torch.equal(B.projectionForward(x, w, out_dtype=f32)[0].double(), z)
+    bias, res = whole(n, most=9).float(), whole(rows, n, most=9).float()
+    y, ck = B.projectionForward(x, w, bias=bias, act="relu2", residual=res, checkpoint=True, out_dtype=f32)
+    zb = z + bias.double()
+    assert torch.equal(y.double(), act64(zb, "relu2") + res.double())
+    assert torch.equal(B.checkpoint8Values(ck, dtype=f32).double(), values64(zb))
+    del w
+    wt, pre = whole(K, n), whole(rows, n, most=9)
+    dx = B.projectionBackwardInput(x, wt, pre=B.checkpoint8(pre), act="relu2", addend=res, out_dtype=f32)
+    assert torch.equal(dx.double(), product(x, wt.t()) * grad64(pre.double(), "relu2") + res.double())
+    del wt
+    x = x[:rows // 8 * 8]
+    if rows >= 8:
+        xs = whole(K, n)
+        dw, db = B.projectionBackwardWeight(x.t().contiguous(), xs, bias=True, out_dtype=f32)
+        assert torch.equal(dw.double(), product(x, xs.t()))
+        assert torch.equal(db.double(), x.double().sum(1))
