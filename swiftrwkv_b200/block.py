@@ -423,6 +423,16 @@ def projectionBackwardWeight(dy, x, act: str = "none", bias: bool = False, out_d
 
 # --------------------------------------------------- the differentiable forms
 
+def _capturing(device):
+    """Whether the current stream of `device` is being captured."""
+    if device.type != "cuda":
+        return False
+    if device.index == _current_device():
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def _recording(**ts):
     """Whether autograd records this call; refused while a stream is captured,
     and for inputs that carry a forward-mode tangent, which the kernels would
@@ -434,7 +444,7 @@ def _recording(**ts):
             raise ValueError(f"{name} carries a tangent: the block operators have no forward-mode derivatives")
     if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in ts.values()):
         return False
-    if torch.cuda.is_current_stream_capturing():
+    if _capturing(next(t for t in ts.values() if t is not None).device):
         raise ValueError("the differentiable block operators do not record a graph during stream capture: "
                          "capture the explicit forward and backward calls")
     return True

@@ -305,3 +305,37 @@ def test_projections_of_more_than_2_24_rows_are_refused():
     # an accumulator takes 32768 rows: 512 splits of a 128 x 128 tile and the column sums
     assert L.rwkv_projection_dw_workspace_size(rows, 64, 64, 0) >= 512 * 128 * 128 * 4
     assert L.rwkv_projection_dw_workspace_size(rows + 1, 64, 64, 0) == 0
+
+
+def test_capture_is_looked_up_on_the_tensors_device(monkeypatch):
+    """A capture on another device than the tensors' is none of a call's business, one
+    on theirs is, whatever device is current."""
+    current = [0]
+
+    class Device:
+        def __init__(self, device):
+            self.index = device.index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *_):
+            current[0] = self.before
+
+    monkeypatch.setattr(B, "_current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: current[0] == 1)
+    assert not B._capturing(torch.device("cuda", 0)) and B._capturing(torch.device("cuda", 1))
+    current[0] = 1
+    assert not B._capturing(torch.device("cuda", 0)) and B._capturing(torch.device("cuda", 1))
+    assert not B._capturing(torch.device("cpu")) and current == [1]
+
+
+def test_differentiable_forms_on_the_host_are_refused():
+    """Recorded or not, and without their first argument, with a ValueError."""
+    for f, args in differentiable_calls():
+        for name, t in args.items():
+            with pytest.raises(ValueError, match="CUDA tensor"):
+                f(**{**args, name: t.clone().requires_grad_(True)})
+        with pytest.raises(ValueError, match="CUDA tensor"):
+            f(**{name: None if name == "x" else t.clone().requires_grad_(True) for name, t in args.items()})
