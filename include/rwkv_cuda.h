@@ -603,6 +603,98 @@ int rwkv_projection_dw(int dtype, const void* dy, int act, const void* x, const 
                        int dwdtype, void* dw, float* db, int rows, int OUT, int IN, void* workspace,
                        int64_t workspace_bytes, rwkv_stream_t stream);
 
+/* ------------------------------------------- between the block operators
+ * What lies between a block's projections and its WKV path, forward and
+ * backward: dropout, the residual norm, the token mix and the time mix's tail
+ * (Sources/RWKVGen/RWKVBlock.swift:163-307; the reference runs them as MLX ops under
+ * MLX's autograd and has no dropout).  Tensors in `dtype` F32, BF16 or F16, 16-byte
+ * aligned unless stated otherwise; arithmetic and sums in fp32, in a fixed order
+ * (deterministic), one rounding at each store.  Outputs overlap no input and no other
+ * output unless stated otherwise.  `workspace`: device memory of the matching
+ * _workspace_size bytes, 16-byte aligned; not needed (may be NULL) where no
+ * parameter's gradient is asked for; calls that may overlap on the GPU need one each.
+ *
+ * Dropout.  An element is dropped with probability q = t / 65536, t = round(65536 p)
+ * (ties to even), p in 0..1, and scaled by 1 / (1 - q) otherwise.  Which ones follows
+ * from seed, offset and the element's place alone, so that no mask is stored: the
+ * backward pass draws the same ones from the same numbers.  Element i (row-major) is
+ * dropped where the 16 bits in half i % 2 (low half first) of word (i % 8) / 2 of the
+ * Philox4x32-10 block with counter (i / 8, offset), 64 bits each, and key seed are
+ * below t (Salmon et al., "Parallel random numbers: as easy as 1, 2, 3", 2011).
+ * Different calls need different (seed, offset) pairs.  `state`: NULL, or device
+ * int64 [2], 8-byte aligned, read when the kernel runs: the seed, and what is added to
+ * `offset` (mod 2^64); a captured graph whose replays are to differ takes it.  What is
+ * dropped is 0, an infinity or a NaN too. */
+
+/* y = dropout(x), n elements (1..2^40); y may be x.  Its gradient is the same call on dy. */
+int rwkv_dropout(int dtype, const void* x, double p, uint64_t seed, uint64_t offset, const int64_t* state,
+                 void* y, int64_t n, rwkv_stream_t stream);
+
+/* Residual norm: sum = x + scale dropout(branch), y = (sum - mean) rstd weight +
+ * bias over each row, as rwkv_layer_norm_forward (ln1 / ln2 of the next branch
+ * after a branch's residual, RWKVBlock.swift:163-307 around X070Backbone.swift:62-65).
+ * x, branch, sum, y: [rows, D] in dtype; D % 8 == 0, D <= 12288 (6144 in F32).
+ * y, mean, rstd and the checkpoint (codes / exps, both NULL or both written; codes
+ * 8-byte aligned) are those of the sum in fp32, before it is rounded to dtype.  sum may
+ * be x or branch, y the other of them.  The dropout's element i is branch's.  scale /
+ * (1 - q) must be finite in fp32. */
+int rwkv_residual_norm_forward(int dtype, const void* x, const void* branch, double scale, double p, uint64_t seed,
+                               uint64_t offset, const int64_t* state, int wdtype, const void* weight,
+                               const void* bias, float eps, void* sum, void* y, float* mean, float* rstd,
+                               int8_t* codes, uint8_t* exps, int rows, int D, rwkv_stream_t stream);
+/* Its gradient: dx as rwkv_layer_norm_backward's of dy at sum (or its checkpoint), with
+ * dres the gradient that reaches sum past the norm; dbranch = scale dropout(dx), from
+ * dx before its rounding.  Where p = 0 and scale = 1 dbranch is dx:
+ * rwkv_layer_norm_backward.  dx may be dy or dres, dbranch the other of them. */
+int64_t rwkv_residual_norm_backward_workspace_size(int rows, int D);
+int rwkv_residual_norm_backward(int dtype, const void* dy, const void* sum, const int8_t* codes, const uint8_t* exps,
+                                int wdtype, const void* weight, const float* mean, const float* rstd,
+                                const void* dres, double scale, double p, uint64_t seed, uint64_t offset,
+                                const int64_t* state, void* dx, void* dbranch, void* dweight, void* dbias, int rows,
+                                int D, void* workspace, int64_t workspace_bytes, rwkv_stream_t stream);
+
+/* Token mix: x [B, T, D] interpolated with the token before, J ways (1..6):
+ *     y_j[b, t] = x[b, t] + (x[b, t-1] - x[b, t]) mix_j,
+ * x[b, -1] = prev[b] ([B, D] in dtype; NULL: 0).  mix: [J, D] in mdtype; y: HOST array
+ * of J device pointers to [B, T, D]; last [B, D]: each sequence's last token, what
+ * the next call takes as prev.  lengths: device int32 [B] (4-byte aligned; NULL: all T),
+ * taken as 0..T: from a sequence's length on, x is not read and y is 0, and an empty
+ * sequence's last is its prev.  D % 8 == 0, D <= 2^20.  Stands for the token shift
+ * and lerp of tmix and cmix (RWKVBlock.swift:163-307). */
+int rwkv_token_mix_forward(int dtype, const void* x, int mdtype, const void* mix, const void* prev,
+                           const int32_t* lengths, void* const* y, void* last, int B, int T, int D, int J,
+                           rwkv_stream_t stream);
+/* Its gradient.  dy: HOST array of J device pointers (NULL: zero), not read from a
+ * sequence's length on; dlast [B, D] (may be NULL: zero): last's gradient.
+ *     dx[t] = sum_j (1 - mix_j) dy_j[t] + mix_j dy_j[t+1]  (+ dlast at the last token),
+ * 0 from the length on; dmix [J, D] in mdtype (may be NULL: not written) = sum over
+ * tokens of dy_j[t] (x[t-1] - x[t]); dprev [B, D] (may be NULL) = sum_j mix_j dy_j[0],
+ * an empty sequence's is its dlast. */
+int64_t rwkv_token_mix_backward_workspace_size(int dtype, int B, int T, int D, int J);
+int rwkv_token_mix_backward(int dtype, const void* const* dy, const void* x, int mdtype, const void* mix,
+                            const void* prev, const int32_t* lengths, const void* dlast, void* dx, void* dmix,
+                            void* dprev, int B, int T, int D, int J, void* workspace, int64_t workspace_bytes,
+                            rwkv_stream_t stream);
+
+/* Tail of the time mix, per row and head of S channels (32, 64, 128 or 256):
+ *     n = (wkv - mean) rstd over the head, c = sum r k rk,
+ *     out = (n weight + bias + c v) g.
+ * wkv, r, k, v, g, out: [rows, H S] in dtype; rk, weight, bias: [H S] in wdtype.  out
+ * may be any of the inputs in dtype.  The training form of rwkv_wkv_tail
+ * (RWKVBlock.swift:280-295). */
+int rwkv_tmix_tail_forward(int dtype, const void* wkv, const void* r, const void* k, const void* v, const void* g,
+                           int wdtype, const void* rk, const void* weight, const void* bias, float eps, void* out,
+                           int rows, int H, int S, rwkv_stream_t stream);
+/* Its gradient.  The statistics are taken again from wkv.  drk, dweight, dbias: [H S]
+ * in wdtype, all NULL or all written.  Each of dwkv, dr, dk, dv, dg may be any one of the
+ * inputs in dtype (or dout) that no other output is. */
+int64_t rwkv_tmix_tail_backward_workspace_size(int rows, int H, int S);
+int rwkv_tmix_tail_backward(int dtype, const void* dout, const void* wkv, const void* r, const void* k, const void* v,
+                            const void* g, int wdtype, const void* rk, const void* weight, const void* bias,
+                            float eps, void* dwkv, void* dr, void* dk, void* dv, void* dg, void* drk, void* dweight,
+                            void* dbias, int rows, int H, int S, void* workspace, int64_t workspace_bytes,
+                            rwkv_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -32,6 +32,8 @@ P = ctypes.c_void_p
 I = ctypes.c_int
 I64 = ctypes.c_int64
 F = ctypes.c_float
+D = ctypes.c_double
+U64 = ctypes.c_uint64
 
 # name -> argtypes (restype int unless listed in _RESTYPES)
 _SIGS = {
@@ -99,6 +101,16 @@ _SIGS = {
     "rwkv_projection_dx": [I, P, P, I, P, P, P, I, P, P, I, I, I, P, I64, P],
     "rwkv_projection_dw_workspace_size": [I, I, I, I],
     "rwkv_projection_dw": [I, P, I, P, P, P, I, P, P, I, I, I, P, I64, P],
+    "rwkv_dropout": [I, P, D, U64, U64, P, P, I64, P],
+    "rwkv_residual_norm_forward": [I, P, P, D, D, U64, U64, P, I, P, P, F, P, P, P, P, P, P, I, I, P],
+    "rwkv_residual_norm_backward_workspace_size": [I, I],
+    "rwkv_residual_norm_backward": [I, P, P, P, P, I, P, P, P, P, D, D, U64, U64, P, P, P, P, P, I, I, P, I64, P],
+    "rwkv_token_mix_forward": [I, P, I, P, P, P, P, P, I, I, I, I, P],
+    "rwkv_token_mix_backward_workspace_size": [I, I, I, I, I],
+    "rwkv_token_mix_backward": [I, P, P, I, P, P, P, P, P, P, P, I, I, I, I, P, I64, P],
+    "rwkv_tmix_tail_forward": [I, P, P, P, P, P, I, P, P, P, F, P, I, I, I, P],
+    "rwkv_tmix_tail_backward_workspace_size": [I, I, I],
+    "rwkv_tmix_tail_backward": [I, P, P, P, P, P, P, I, P, P, P, F, P, P, P, P, P, P, P, P, I, I, I, P, I64, P],
 }
 _RESTYPES = {
     "rwkv_status_string": ctypes.c_char_p,
@@ -112,6 +124,9 @@ _RESTYPES = {
     "rwkv_projection_forward_workspace_size": I64,
     "rwkv_projection_dx_workspace_size": I64,
     "rwkv_projection_dw_workspace_size": I64,
+    "rwkv_residual_norm_backward_workspace_size": I64,
+    "rwkv_token_mix_backward_workspace_size": I64,
+    "rwkv_tmix_tail_backward_workspace_size": I64,
 }
 
 _lib = None

@@ -11,6 +11,14 @@
   the activation it stands for.
 * `channelMix`, the two projections of cmix around the squared ReLU,
   differentiable, with the pre-activation kept in 8 bits.
+* Between them and the WKV path (kernel.py), each with its differentiable form:
+  `tokenMixForward` / `tokenMixBackward` (`tokenMix`), the token shift and the
+  interpolations that feed the projections; `tmixTailForward` /
+  `tmixTailBackward` (`tmixTail`), the norm by head, bonus and gate that end the
+  time mix; `residualNormForward` / `residualNormBackward` (`residualNorm`), a
+  branch added to the residual stream, through dropout and scaled, and the sum
+  normed; `dropoutForward` (`dropout`), whose mask is drawn from a counter and
+  never stored.
 
 The reference runs these as MLX layerNorm / matmul / elementwise ops under
 MLX's autograd (Sources/RWKVGen/RWKVBlock.swift:163-307, X070Backbone.swift:
@@ -421,6 +429,285 @@ def projectionBackwardWeight(dy, x, act: str = "none", bias: bool = False, out_d
     return dw, db
 
 
+# ----------------------------------------------------------------- dropout
+
+_WORD = 1 << 64
+
+
+def _draw(p, seed, offset, dev):
+    """(seed, offset, the state or None) of a call with dropout, after their checks.
+    The caller holds the state, which may be a copy, until its call is made."""
+    if not isinstance(p, (int, float)) or not 0.0 <= p <= 1.0:
+        raise ValueError(f"p={p!r} must be a number in 0..1")
+    if not isinstance(offset, int) or not 0 <= offset < _WORD:
+        raise ValueError(f"offset={offset!r} must be an integer in 0..2^64 - 1")
+    if type(seed) is int or isinstance(seed, int):
+        if not 0 <= seed < _WORD:
+            raise ValueError(f"seed={seed!r} must be in 0..2^64 - 1")
+        return seed, offset, None
+    if not isinstance(seed, torch.Tensor):
+        raise ValueError(f"seed={seed!r} must be an integer or a CUDA tensor int64 [2]")
+    return 0, offset, _tensor("seed", seed, dev, (torch.int64,), (2,))
+
+
+def _number(name, v):
+    if not isinstance(v, (int, float)):
+        raise ValueError(f"{name}={v!r} must be a number")
+    return v
+
+
+def dropoutForward(x, p: float, seed, offset: int = 0):
+    """x / (1 - q) where kept and 0 where dropped, q = round(65536 p) / 65536; the
+    gradient is the same call on dy.  An element is dropped by its place in x,
+    `seed` and `offset` alone (rwkv_cuda.h has the generator), so that every call of a
+    program with masks of its own takes another (seed, offset), and the backward pass
+    the forward's.  seed: an integer, or a CUDA tensor int64 [2] that is read when the
+    kernel runs (the seed, and what is added to `offset`): a captured graph then draws
+    anew where the program changes the tensor between replays."""
+    x = _aligned(_some("x", x))
+    dev = x.device
+    seed, offset, state = _draw(p, seed, offset, dev)
+    y = torch.empty_like(x)
+    n = x.numel()
+    if n:
+        _call(dev, "rwkv_dropout", _DT[x.dtype], x.data_ptr(), p, seed, offset, _p(state), y.data_ptr(), n)
+    return y
+
+
+# ----------------------------------------------------------- residual norm
+
+def _norm_params(weight, bias, dev, D):
+    if not _fits(weight, dev, torch.float32, (D,)):
+        weight = _tensor("weight", weight, dev, None, (D,))
+    if not _fits(bias, dev, weight.dtype, (D,)):
+        bias = _tensor("bias", bias, dev, (weight.dtype,), (D,))
+    return _aligned(weight), _aligned(bias)
+
+
+def residualNormForward(x, branch, weight, bias, eps: float = 1e-5, scale: float = 1.0, p: float = 0.0, seed=0,
+                        offset: int = 0, checkpoint: bool = False):
+    """s = x + scale dropout(branch) and its layer norm y: (s, y, mean, rstd, ck).
+    x, branch [..., D] in one type, D a multiple of 8, at most 12288 (6144 in fp32).
+    y, the statistics and ck (the 8-bit checkpoint of s; None without `checkpoint`)
+    are those of the sum in fp32, before it is rounded to x's type.  p, seed,
+    offset: as in dropoutForward, by the places in branch."""
+    x = _aligned(_some("x", x))
+    dev, dt, shape = x.device, x.dtype, x.shape
+    D = shape[-1]
+    if not _fits(branch, dev, dt, shape):
+        branch = _tensor("branch", branch, dev, (dt,), shape)
+    branch = _aligned(branch)
+    weight, bias = _norm_params(weight, bias, dev, D)
+    seed, offset, state = _draw(p, seed, offset, dev)
+    s, y = torch.empty_like(x), torch.empty_like(x)
+    mean = x.new_empty(*shape[:-1], dtype=torch.float32) if len(shape) > 1 else x.new_empty((), dtype=torch.float32)
+    rstd = torch.empty_like(mean)
+    codes = exps = ck = None
+    if checkpoint:
+        ck = _new_checkpoint(x, dt)
+        codes, exps = ck.codes.data_ptr(), ck.exps.data_ptr()
+    n = x.numel()
+    if n:
+        _call(dev, "rwkv_residual_norm_forward", _DT[dt], x.data_ptr(), branch.data_ptr(), _number("scale", scale), p,
+              seed, offset, _p(state), _DT[weight.dtype], weight.data_ptr(), bias.data_ptr(), eps, s.data_ptr(),
+              y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), codes, exps, n // D, D)
+    return s, y, mean, rstd, ck
+
+
+def residualNormBackward(dy, s, weight, mean, rstd, dres=None, scale: float = 1.0, p: float = 0.0, seed=0,
+                         offset: int = 0, params: bool = True):
+    """(dx, dbranch, dweight, dbias) of residualNormForward.  s: its sum, or the
+    checkpoint of it; mean, rstd: its statistics; dres: the gradient that reaches s
+    past the norm.  Where nothing is dropped or scaled dbranch is dx itself.  Without
+    `params` dweight and dbias are None."""
+    dy = _some("dy", dy)
+    dev, dt, shape = dy.device, dy.dtype, dy.shape
+    seed, offset, state = _draw(p, seed, offset, dev)
+    if _number("scale", scale) == 1.0 and round(65536 * p) == 0:
+        dx, dw, db = layerNormBackward(dy, s, weight, mean, rstd, dres, params)
+        return dx, dx, dw, db
+    dy, D = _aligned(dy), shape[-1]
+    st, codes, exps = _activation("s", s, dev, dt, shape)
+    st, codes = _aligned(st), _aligned(codes)
+    if not _fits(weight, dev, torch.float32, (D,)):
+        weight = _tensor("weight", weight, dev, None, (D,))
+    weight = _aligned(weight)
+    lead = shape[:-1]
+    if not _fits(mean, dev, torch.float32, lead):
+        mean = _tensor("mean", mean, dev, (torch.float32,), lead)
+    if not _fits(rstd, dev, torch.float32, lead):
+        rstd = _tensor("rstd", rstd, dev, (torch.float32,), lead)
+    if dres is not None:
+        if not _fits(dres, dev, dt, shape):
+            dres = _tensor("dres", dres, dev, (dt,), shape)
+        dres = _aligned(dres)
+    dx, dbranch = torch.empty_like(dy), torch.empty_like(dy)
+    rows = dy.numel() // D
+    dw = torch.empty_like(weight) if params else None
+    db = torch.empty_like(weight) if params else None
+    if not rows:
+        return dx, dbranch, dw.zero_() if params else None, db.zero_() if params else None
+    n = _workspace_bytes("rwkv_residual_norm_backward", rows, D) if params else 0
+    ws = _workspace(n, dy)
+    _call(dev, "rwkv_residual_norm_backward", _DT[dt], dy.data_ptr(), _p(st), _p(codes), _p(exps), _DT[weight.dtype],
+          weight.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _p(dres), scale, p, seed, offset, _p(state),
+          dx.data_ptr(), dbranch.data_ptr(), _p(dw), _p(db), rows, D, _p(ws), n)
+    return dx, dbranch, dw, db
+
+
+# --------------------------------------------------------------- token mix
+
+def _mix_args(x, mix, prev, lengths):
+    """tokenMix's inputs after their checks."""
+    x = _aligned(_some("x", x))
+    if x.dim() != 3:
+        raise ValueError(f"x {tuple(x.shape)} must be [B, T, D]")
+    dev, (B, _, D) = x.device, x.shape
+    if not (type(mix) in _TENSORS and mix.dtype is torch.float32 and mix.device == dev and mix.is_contiguous()):
+        mix = _tensor("mix", mix, dev)
+    if mix.dim() != 2 or mix.shape[1] != D or not 1 <= mix.shape[0] <= 6:
+        raise ValueError(f"mix {tuple(mix.shape)} must be [J, {D}], J in 1..6")
+    if prev is not None:
+        if not _fits(prev, dev, x.dtype, (B, D)):
+            prev = _tensor("prev", prev, dev, (x.dtype,), (B, D))
+        prev = _aligned(prev)
+    if lengths is not None and not _fits(lengths, dev, torch.int32, (B,)):
+        lengths = _tensor("lengths", lengths, dev, (torch.int32,), (B,))
+    return x, _aligned(mix), prev, lengths
+
+
+def _addresses(ts):
+    """A host array of the addresses of tensors (None: NULL)."""
+    return (_lib.P * len(ts))(*[_p(t) for t in ts])
+
+
+def _token_mix(x, mix, prev, lengths, ys):
+    """tokenMixForward into the tensors or addresses ys: last."""
+    B, T, D = x.shape
+    last = x.new_empty(B, D)
+    if x.numel():
+        _call(x.device, "rwkv_token_mix_forward", _DT[x.dtype], x.data_ptr(), _DT[mix.dtype], mix.data_ptr(), _p(prev),
+              _p(lengths), ys, last.data_ptr(), B, T, D, mix.shape[0])
+    elif B:
+        last.copy_(prev) if prev is not None else last.zero_()
+    return last
+
+
+def tokenMixForward(x, mix, prev=None, lengths=None):
+    """Each token interpolated with the one before it: (y, last).  x [B, T, D], D a
+    multiple of 8; mix [J, D], J in 1..6, in fp32, bf16 or fp16; prev [B, D] in x's
+    type: the token before the first (None: zeros).
+        y[j, b, t] = x[b, t] + (x[b, t-1] - x[b, t]) mix[j]
+    lengths: int32 [B] of right-padded sequences, taken as 0..T (None: all T); from a
+    sequence's length on x is not read and y is 0.  last [B, D] is each sequence's last
+    token (prev where it is empty), the next call's prev."""
+    x, mix, prev, lengths = _mix_args(x, mix, prev, lengths)
+    J = mix.shape[0]
+    y = x.new_empty(J, *x.shape)
+    at, step = y.data_ptr(), x.numel() * x.element_size()
+    return y, _token_mix(x, mix, prev, lengths, (_lib.P * J)(*[at + j * step for j in range(J)]))
+
+
+def tokenMixBackward(dys, x, mix, prev=None, lengths=None, dlast=None, params: bool = True):
+    """(dx, dmix, dprev) of tokenMixForward.  dys: [J, B, T, D], or J tensors [B, T, D]
+    of which any may be None (zeros); dlast [B, D]: the gradient of last (None: zeros).
+    dx is 0 from a sequence's length on, where dys are not read.  dmix [J, D] in mix's
+    type, None without `params`; dprev is None without prev."""
+    x, mix, prev, lengths = _mix_args(x, mix, prev, lengths)
+    dev, dt, shape, J = x.device, x.dtype, x.shape, mix.shape[0]
+    B, T, D = shape
+    if isinstance(dys, torch.Tensor):
+        dys = _aligned(dys if _fits(dys, dev, dt, (J, *shape)) else _tensor("dys", dys, dev, (dt,), (J, *shape)))
+        at, step = dys.data_ptr(), x.numel() * x.element_size()
+        addresses = (_lib.P * J)(*[at + j * step for j in range(J)])
+    else:
+        if not isinstance(dys, (list, tuple)) or len(dys) != J:
+            raise ValueError(f"dys: a tensor [{J}, B, T, D] or {J} tensors [B, T, D] are needed")
+        dys = [t if t is None else _aligned(t if _fits(t, dev, dt, shape) else _tensor("dys", t, dev, (dt,), shape))
+               for t in dys]
+        addresses = _addresses(dys)
+    if dlast is not None:
+        dlast = _aligned(dlast if _fits(dlast, dev, dt, (B, D)) else _tensor("dlast", dlast, dev, (dt,), (B, D)))
+    dx = torch.empty_like(x)
+    dmix = torch.empty_like(mix) if params else None
+    dprev = torch.empty_like(prev) if prev is not None else None
+    if not x.numel():
+        if dprev is not None:
+            dprev.copy_(dlast) if dlast is not None else dprev.zero_()
+        return dx, dmix.zero_() if params else None, dprev
+    n = _workspace_bytes("rwkv_token_mix_backward", _DT[dt], B, T, D, J) if params else 0
+    ws = _workspace(n, x)
+    _call(dev, "rwkv_token_mix_backward", _DT[dt], addresses, x.data_ptr(), _DT[mix.dtype], mix.data_ptr(), _p(prev),
+          _p(lengths), _p(dlast), dx.data_ptr(), _p(dmix), _p(dprev), B, T, D, J, _p(ws), n)
+    return dx, dmix, dprev
+
+
+# -------------------------------------------------------- tail of the time mix
+
+def _tail_args(rk, weight, bias, tensors):
+    """(inputs, H, S) of tmixTail after their checks; tensors: name, tensor, wkv first."""
+    name, wkv = tensors[0]
+    wkv = _aligned(_some(name, wkv))
+    dev, dt, shape = wkv.device, wkv.dtype, wkv.shape
+    if not (type(rk) in _TENSORS and rk.dtype is torch.float32 and rk.device == dev and rk.is_contiguous()):
+        rk = _tensor("rk", rk, dev)
+    if rk.dim() != 2 or not rk.numel():
+        raise ValueError(f"rk {tuple(rk.shape)} must be [H, S]")
+    H, S = rk.shape
+    D = H * S
+    heads = shape[-2:] == (H, S)
+    if not heads and shape[-1] != D:
+        raise ValueError(f"{name} {tuple(shape)} must be [..., {H}, {S}] or [..., {D}]")
+    other = shape[:-2] + (D,) if heads else shape[:-1] + (H, S)
+    ins = [wkv]
+    for name, t in tensors[1:]:
+        if not _fits(t, dev, dt, other) and not _fits(t, dev, dt, shape):
+            t = _tensor(name, t, dev, (dt,))
+            if t.shape != shape and t.shape != other:
+                raise ValueError(f"{name} {tuple(t.shape)} must be {list(shape)} or {list(other)}")
+        ins.append(_aligned(t))
+    ps = [_aligned(rk)]
+    for name, t in (("weight", weight), ("bias", bias)):
+        if not _fits(t, dev, rk.dtype, (D,)):
+            t = _tensor(name, t, dev, (rk.dtype,), (D,))
+        ps.append(_aligned(t))
+    return ins, ps, H, S
+
+
+def tmixTailForward(wkv, r, k, v, g, rk, weight, bias, eps: float = 64e-5):
+    """The end of the time mix, per head of S channels (32, 64, 128 or 256):
+    ((wkv - mean) rstd weight + bias + (sum r k rk) v) g, in g's shape.  wkv, r, k, v,
+    g: [..., H, S] or [..., H S], in one type; rk [H, S], weight and bias [H S], in
+    fp32, bf16 or fp16.  The training form of kernel.wkvTail."""
+    (wkv, r, k, v, g), (rk, weight, bias), H, S = _tail_args(
+        rk, weight, bias, (("wkv", wkv), ("r", r), ("k", k), ("v", v), ("g", g)))
+    out = torch.empty_like(g)
+    n = wkv.numel()
+    if n:
+        _call(wkv.device, "rwkv_tmix_tail_forward", _DT[wkv.dtype], wkv.data_ptr(), r.data_ptr(), k.data_ptr(),
+              v.data_ptr(), g.data_ptr(), _DT[rk.dtype], rk.data_ptr(), weight.data_ptr(), bias.data_ptr(), eps,
+              out.data_ptr(), n // (H * S), H, S)
+    return out
+
+
+def tmixTailBackward(dout, wkv, r, k, v, g, rk, weight, bias, eps: float = 64e-5, params: bool = True):
+    """(dwkv, dr, dk, dv, dg, drk, dweight, dbias) of tmixTailForward, each in its
+    input's shape and type.  Without `params` the last three are None."""
+    (wkv, r, k, v, g, dout), (rk, weight, bias), H, S = _tail_args(
+        rk, weight, bias, (("wkv", wkv), ("r", r), ("k", k), ("v", v), ("g", g), ("dout", dout)))
+    grads = [torch.empty_like(t) for t in (wkv, r, k, v, g)]
+    pgrads = [torch.empty_like(t) for t in (rk, weight, bias)] if params else [None] * 3
+    rows = wkv.numel() // (H * S)
+    if not rows:
+        return (*grads, *(t if t is None else t.zero_() for t in pgrads))
+    n = _workspace_bytes("rwkv_tmix_tail_backward", rows, H, S) if params else 0
+    ws = _workspace(n, wkv)
+    _call(wkv.device, "rwkv_tmix_tail_backward", _DT[wkv.dtype], dout.data_ptr(), wkv.data_ptr(), r.data_ptr(),
+          k.data_ptr(), v.data_ptr(), g.data_ptr(), _DT[rk.dtype], rk.data_ptr(), weight.data_ptr(), bias.data_ptr(), eps,
+          *[t.data_ptr() for t in grads], *[_p(t) for t in pgrads], rows, H, S, _p(ws), n)
+    return (*grads, *pgrads)
+
+
 # --------------------------------------------------- the differentiable forms
 
 def _capturing(device):
@@ -570,3 +857,111 @@ def channelMix(x, key, value, residual=None, checkpoint: bool = True):
         k, _ = projectionForward(x, key, act="relu2")
         return projectionForward(k, value, residual=residual)[0]
     return _ChannelMix.apply(x, key, value, residual, checkpoint)
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, p, seed, offset):
+        _save(ctx, [], *([seed] if isinstance(seed, torch.Tensor) else []))
+        ctx.drawn = p, seed if isinstance(seed, int) else None, offset
+        return dropoutForward(x, p, seed, offset)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        state, _ = _saved(ctx)
+        p, seed, offset = ctx.drawn
+        return dropoutForward(dy, p, state[0] if state else seed, offset), None, None, None
+
+
+def dropout(x, p: float, seed, offset: int = 0):
+    """Differentiable dropoutForward.  A `seed` tensor keeps its values until the
+    backward pass has run (autograd refuses one that was changed in place)."""
+    if not _recording(x=x):
+        return dropoutForward(x, p, seed, offset)
+    return _Dropout.apply(x, p, seed, offset)
+
+
+class _ResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, branch, weight, bias, eps, scale, p, seed, offset, checkpoint):
+        s, y, mean, rstd, ck = residualNormForward(x, branch, weight, bias, eps, scale, p, seed, offset, checkpoint)
+        ctx.set_materialize_grads(False)
+        _save(ctx, [ck if checkpoint else s], weight, mean, rstd, *([seed] if isinstance(seed, torch.Tensor) else []))
+        ctx.drawn = scale, p, seed if isinstance(seed, int) else None, offset
+        return s, y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, ds, dy):
+        (weight, mean, rstd, *state), (s,) = _saved(ctx)
+        scale, p, seed, offset = ctx.drawn
+        need = ctx.needs_input_grad
+        if dy is None:
+            if ds is None:
+                return (None,) * 10
+            dy = torch.zeros_like(ds)
+        dx, dbranch, dw, db = residualNormBackward(dy, s, weight, mean, rstd, ds, scale, p, state[0] if state else seed,
+                                                   offset, params=need[2] or need[3])
+        return (dx, dbranch, dw, db) + (None,) * 6
+
+
+def residualNorm(x, branch, weight, bias, eps: float = 1e-5, scale: float = 1.0, p: float = 0.0, seed=0,
+                 offset: int = 0, checkpoint: bool = False):
+    """Differentiable (s, y) of residualNormForward.  With `checkpoint` the backward
+    pass works from the 8-bit checkpoint of s."""
+    if not _recording(x=x, branch=branch, weight=weight, bias=bias):
+        return residualNormForward(x, branch, weight, bias, eps, scale, p, seed, offset)[:2]
+    return _ResidualNorm.apply(x, branch, weight, bias, eps, scale, p, seed, offset, checkpoint)
+
+
+class _TokenMix(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, mix, prev, lengths):
+        x, mix, prev, lengths = _mix_args(x, mix, prev, lengths)
+        ys = [torch.empty_like(x) for _ in range(mix.shape[0])]
+        last = _token_mix(x, mix, prev, lengths, _addresses(ys))
+        ctx.set_materialize_grads(False)
+        ctx.given = prev is not None, lengths is not None
+        _save(ctx, [], x, mix, *(t for t in (prev, lengths) if t is not None))
+        return (*ys, last)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, *grads):
+        (x, mix, *rest), _ = _saved(ctx)
+        prev = rest.pop(0) if ctx.given[0] else None
+        lengths = rest.pop(0) if ctx.given[1] else None
+        *dys, dlast = grads
+        dx, dmix, dprev = tokenMixBackward(dys, x, mix, prev, lengths, dlast, params=ctx.needs_input_grad[1])
+        return dx, dmix, dprev, None
+
+
+def tokenMix(x, mix, prev=None, lengths=None):
+    """Differentiable tokenMixForward: (the J tensors y_j [B, T, D], last)."""
+    if not _recording(x=x, mix=mix, prev=prev):
+        y, last = tokenMixForward(x, mix, prev, lengths)
+        return y.unbind(0), last
+    *ys, last = _TokenMix.apply(x, mix, prev, lengths)
+    return tuple(ys), last
+
+
+class _TmixTail(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, wkv, r, k, v, g, rk, weight, bias, eps):
+        _save(ctx, [], wkv, r, k, v, g, rk, weight, bias)
+        ctx.eps = eps
+        return tmixTailForward(wkv, r, k, v, g, rk, weight, bias, eps)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        ts, _ = _saved(ctx)
+        return (*tmixTailBackward(dout, *ts, ctx.eps, params=any(ctx.needs_input_grad[5:8])), None)
+
+
+def tmixTail(wkv, r, k, v, g, rk, weight, bias, eps: float = 64e-5):
+    """Differentiable tmixTailForward."""
+    if not _recording(wkv=wkv, r=r, k=k, v=v, g=g, rk=rk, weight=weight, bias=bias):
+        return tmixTailForward(wkv, r, k, v, g, rk, weight, bias, eps)
+    return _TmixTail.apply(wkv, r, k, v, g, rk, weight, bias, eps)

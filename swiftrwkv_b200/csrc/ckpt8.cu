@@ -19,36 +19,6 @@ namespace {
 
 constexpr int CT = 256;
 
-// 8 elements of a row as read and as floats, 16-byte accesses
-template <typename T>
-struct Raw8 {
-    static constexpr int W = 8 / Vec16<T>::N;
-    uint4 r[W];
-    __device__ __forceinline__ void load(const T* p) {
-#pragma unroll
-        for (int i = 0; i < W; i++) r[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
-    }
-    __device__ __forceinline__ void zero() {
-#pragma unroll
-        for (int i = 0; i < W; i++) r[i] = make_uint4(0, 0, 0, 0);
-    }
-    __device__ __forceinline__ void floats(float* v) const {
-#pragma unroll
-        for (int i = 0; i < W; i++) Vec16<T>::unpack(r[i], v + i * Vec16<T>::N);
-    }
-    __device__ __forceinline__ uint32_t top() const {
-        uint32_t t = top_bits<T>(r[0]);
-        if constexpr (W == 2) t = max(t, top_bits<T>(r[1]));
-        return t;
-    }
-};
-template <typename T>
-__device__ __forceinline__ void store8(T* p, const float* v) {
-#pragma unroll
-    for (int i = 0; i < 8 / Vec16<T>::N; i++)
-        __stcs(reinterpret_cast<uint4*>(p) + i, Vec16<T>::pack(v + i * Vec16<T>::N));
-}
-
 constexpr int CU = 4;
 
 // FLAT: D % 32 == 0, rows run on.  Otherwise units are counted in rows padded

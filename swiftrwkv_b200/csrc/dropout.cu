@@ -1,0 +1,60 @@
+// Dropout with a mask that is never stored (philox.cuh): y = x scale where kept, 0
+// elsewhere; its gradient is the same call on dy.  One pass over memory: a thread
+// takes DU blocks of 8 elements DT apart, all loads first, and draws a block's bits
+// while they arrive.
+#include "ckpt8.cuh"
+#include "philox.cuh"
+
+namespace rwkv {
+namespace {
+
+constexpr int DT = 256, DU = 4;
+
+template <typename T>
+__global__ void __launch_bounds__(DT) dropout_kernel(const T* x, T* y, int64_t n, const Dropout d) {
+    const int64_t u0 = blockIdx.x * (int64_t)(DT * DU) + threadIdx.x, units = n / 8;
+    Raw8<T> raw[DU];
+#pragma unroll
+    for (int j = 0; j < DU; j++)
+        if (u0 + j * DT < units) raw[j].load(x + 8 * (u0 + j * DT));
+    const DropKey key = drop_key(d);
+#pragma unroll
+    for (int j = 0; j < DU; j++) {
+        const int64_t u = u0 + j * DT;
+        if (u >= units) continue;
+        float v[8];
+        raw[j].floats(v);
+        drop_at<8>(v, key, 8 * (uint64_t)u, d.threshold, d.scale);
+        store8(y + 8 * u, v);
+    }
+    // the tensor's last n % 8 elements
+    const int64_t t = 8 * units + threadIdx.x;
+    if (blockIdx.x == 0 && t < n) {
+        const uint4 r = philox(key, units);
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+        const uint32_t bits = w[threadIdx.x / 2 & 3] >> 16 * (threadIdx.x & 1) & 0xffffu;
+        y[t] = from_f<T>(bits < d.threshold ? 0.f : __fmul_rn(to_f<T>(x[t]), d.scale));
+    }
+}
+
+}  // namespace
+}  // namespace rwkv
+
+using namespace rwkv;
+
+extern "C" int rwkv_dropout(int dtype, const void* x, double p, uint64_t seed, uint64_t offset, const int64_t* state,
+                            void* y, int64_t n, rwkv_stream_t stream) {
+    const char* fn = "rwkv_dropout";
+    RWKV_REQUIRE(valid_dtype(dtype), RWKV_E_DTYPE, "%s: dtype %d", fn, dtype);
+    RWKV_REQUIRE(x && y, RWKV_E_NULL, "%s: NULL argument", fn);
+    RWKV_REQUIRE(n >= 1 && n <= 1ll << 40, RWKV_E_SHAPE, "%s: n=%lld (1..2^40)", fn, (long long)n);
+    RWKV_REQUIRE(p >= 0.0 && p <= 1.0, RWKV_E_SHAPE, "%s: p=%g must be in 0..1", fn, p);
+    RWKV_REQUIRE((((uintptr_t)x | (uintptr_t)y) & 15) == 0 && ((uintptr_t)state & 7) == 0, RWKV_E_UNSUPPORTED,
+                 "%s: x and y must be 16-byte aligned, state 8-byte", fn);
+    const Dropout d = make_dropout(p, 1.0, seed, offset, state);
+    return dispatch_dtype(dtype, [&]<typename T>() {
+        const int64_t blocks = (n / 8 + DT * DU - 1) / (DT * DU);
+        dropout_kernel<T><<<(unsigned)(blocks ? blocks : 1), DT, 0, (cudaStream_t)stream>>>((const T*)x, (T*)y, n, d);
+        return check_launch("dropout_kernel");
+    });
+}

@@ -1,0 +1,278 @@
+// The end of the time mix in training: a norm by head of the WKV output a, the
+// bonus and the gate, and their gradient.  Per row and head of S channels:
+//
+//   n = (a - mean) rstd, rstd = 1 / sqrt(var + eps);  c = sum r k rk
+//   z = n w + b + c v,  out = z g
+//   dz = dout g, dg = dout z, dv = c dz, dc = sum dz v, dr = dc k rk, dk = dc r rk
+//   e = dz w:  da = rstd (e - mean(e) - n mean(e n))
+//   dw = sum_rows dz n, db = sum_rows dz, drk = sum_rows dc r k
+//
+// Both are bound by HBM: 6 and 11 tensors.  A thread owns 8 channels, S / 8
+// neighbouring lanes a head, whose sums are shuffles between them; nothing crosses a
+// warp.  Threads are laid over [slots, D / 8] and walk over the rows of their slot,
+// so that their channels are fixed: the parameters and the sums of their gradients
+// stay in registers.  The statistics are not kept by the forward pass: the backward
+// reads a whole anyway.
+#include <algorithm>
+
+#include "ckpt8.cuh"
+#include "param_join.cuh"
+
+namespace rwkv {
+namespace {
+
+constexpr int TAIL_T = 128;
+
+struct TailArgs {
+    const void *a, *r, *k, *v, *g;  // [rows, D]
+    const void *rk, *w, *b;         // [D]
+    int wdtype, units, slots, rows;  // units: D / 8
+    float eps;
+};
+struct TailGrad {
+    const void* dout;
+    void *da, *dr, *dk, *dv, *dg;
+    float* part;  // [slots][drk, dw, db][D], or NULL
+};
+
+// L lanes a head.  All threads of a warp take the same number of steps, with or
+// without a row, for the shuffles.
+template <typename T, int L>
+__global__ void __launch_bounds__(TAIL_T) tmix_tail_kernel(const TailArgs a, T* out) {
+    const int64_t id = blockIdx.x * (int64_t)TAIL_T + threadIdx.x;
+    const int slot = (int)(id / a.units), u = (int)(id - (int64_t)slot * a.units);
+    const int64_t D = 8 * (int64_t)a.units;
+    constexpr float inv = 1.f / (8 * L);
+    float rk[8], w[8], b[8];
+    load_params<8>(a.rk, a.wdtype, 8 * u, rk);
+    load_params<8>(a.w, a.wdtype, 8 * u, w);
+    load_params<8>(a.b, a.wdtype, 8 * u, b);
+    const int steps = (a.rows + a.slots - 1) / a.slots;
+    for (int i = 0; i < steps; i++) {
+        const int64_t row = (int64_t)i * a.slots + slot, at = row * D + 8 * u;
+        const bool in = slot < a.slots && row < a.rows;
+        Raw8<T> ra, rr, rkk, rv, rg;
+        ra.zero(), rr.zero(), rkk.zero(), rv.zero(), rg.zero();
+        if (in) {
+            ra.load(static_cast<const T*>(a.a) + at);
+            rr.load(static_cast<const T*>(a.r) + at);
+            rkk.load(static_cast<const T*>(a.k) + at);
+            rv.load(static_cast<const T*>(a.v) + at);
+            rg.load(static_cast<const T*>(a.g) + at);
+        }
+        float x[8], y[8], c = 0.f, s = 0.f, q = 0.f;
+        rr.floats(x);
+        rkk.floats(y);
+#pragma unroll
+        for (int j = 0; j < 8; j++) c = fmaf(x[j] * y[j], rk[j], c);
+        ra.floats(x);
+#pragma unroll
+        for (int j = 0; j < 8; j++) s += x[j];
+        c = group_sum<L>(c);
+        const float mean = group_sum<L>(s) * inv;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            x[j] -= mean;
+            q = fmaf(x[j], x[j], q);
+        }
+        const float rstd = 1.f / sqrtf(group_sum<L>(q) * inv + a.eps);
+        float v[8], g[8];
+        rv.floats(v);
+        rg.floats(g);
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[j] = fmaf(c, v[j], fmaf(x[j] * rstd, w[j], b[j])) * g[j];
+        if (in) store8(out + at, x);
+    }
+}
+
+template <typename T, int L>
+__global__ void __launch_bounds__(TAIL_T) tmix_tail_backward_kernel(const TailArgs a, const TailGrad o) {
+    const int64_t id = blockIdx.x * (int64_t)TAIL_T + threadIdx.x;
+    const int slot = (int)(id / a.units), u = (int)(id - (int64_t)slot * a.units);
+    const int64_t D = 8 * (int64_t)a.units;
+    constexpr float inv = 1.f / (8 * L);
+    float rk[8], w[8], b[8], srk[8], sw[8], sb[8];
+    load_params<8>(a.rk, a.wdtype, 8 * u, rk);
+    load_params<8>(a.w, a.wdtype, 8 * u, w);
+    load_params<8>(a.b, a.wdtype, 8 * u, b);
+#pragma unroll
+    for (int j = 0; j < 8; j++) srk[j] = sw[j] = sb[j] = 0.f;
+    const int steps = (a.rows + a.slots - 1) / a.slots;
+    for (int i = 0; i < steps; i++) {
+        const int64_t row = (int64_t)i * a.slots + slot, at = row * D + 8 * u;
+        const bool in = slot < a.slots && row < a.rows;
+        Raw8<T> ra, rr, rkk, rv, rg, rd;
+        ra.zero(), rr.zero(), rkk.zero(), rv.zero(), rg.zero(), rd.zero();
+        if (in) {
+            ra.load(static_cast<const T*>(a.a) + at);
+            rr.load(static_cast<const T*>(a.r) + at);
+            rkk.load(static_cast<const T*>(a.k) + at);
+            rv.load(static_cast<const T*>(a.v) + at);
+            rg.load(static_cast<const T*>(a.g) + at);
+            rd.load(static_cast<const T*>(o.dout) + at);
+        }
+        float r[8], k[8], x[8], v[8], g[8], d[8], c = 0.f, s = 0.f;
+        rr.floats(r);
+        rkk.floats(k);
+        ra.floats(x);
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            c = fmaf(r[j] * k[j], rk[j], c);
+            s += x[j];
+        }
+        c = group_sum<L>(c);
+        const float mean = group_sum<L>(s) * inv;
+        rv.floats(v);
+        rg.floats(g);
+        rd.floats(d);
+        // sums over the head: (a - mean)^2, dz v, e, e (a - mean)
+        float q = 0.f, dc = 0.f, e1 = 0.f, e2 = 0.f, dz[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            x[j] -= mean;
+            dz[j] = d[j] * g[j];
+            q = fmaf(x[j], x[j], q);
+            dc = fmaf(dz[j], v[j], dc);
+            const float e = dz[j] * w[j];
+            e1 += e;
+            e2 = fmaf(e, x[j], e2);
+        }
+        q = group_sum<L>(q);
+        dc = group_sum<L>(dc);
+        const float m1 = group_sum<L>(e1) * inv;
+        const float rstd = 1.f / sqrtf(q * inv + a.eps);
+        const float m2 = group_sum<L>(e2) * inv * rstd;
+        float t[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            x[j] *= rstd;
+            t[j] = d[j] * fmaf(c, v[j], fmaf(x[j], w[j], b[j]));
+        }
+        if (in) store8(static_cast<T*>(o.dg) + at, t);
+#pragma unroll
+        for (int j = 0; j < 8; j++) t[j] = rstd * (fmaf(dz[j], w[j], -m1) - x[j] * m2);
+        if (in) store8(static_cast<T*>(o.da) + at, t);
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            sw[j] = fmaf(dz[j], x[j], sw[j]);
+            sb[j] += dz[j];
+            t[j] = c * dz[j];
+        }
+        if (in) store8(static_cast<T*>(o.dv) + at, t);
+#pragma unroll
+        for (int j = 0; j < 8; j++) t[j] = dc * rk[j] * k[j];
+        if (in) store8(static_cast<T*>(o.dr) + at, t);
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            t[j] = dc * rk[j] * r[j];
+            srk[j] = fmaf(dc * r[j], k[j], srk[j]);
+        }
+        if (in) store8(static_cast<T*>(o.dk) + at, t);
+    }
+    if (!o.part || slot >= a.slots) return;
+    float* p = o.part + (int64_t)slot * 3 * D + 8 * u;
+#pragma unroll
+    for (int j = 0; j < 8; j += 4) {
+        *reinterpret_cast<float4*>(p + j) = make_float4(srk[j], srk[j + 1], srk[j + 2], srk[j + 3]);
+        *reinterpret_cast<float4*>(p + D + j) = make_float4(sw[j], sw[j + 1], sw[j + 2], sw[j + 3]);
+        *reinterpret_cast<float4*>(p + 2 * D + j) = make_float4(sb[j], sb[j + 1], sb[j + 2], sb[j + 3]);
+    }
+}
+
+template <typename F>
+int dispatch_head(int S, F&& f) {
+    switch (S) {
+        case 32: return f.template operator()<4>();
+        case 64: return f.template operator()<8>();
+        case 128: return f.template operator()<16>();
+        default: return f.template operator()<32>();
+    }
+}
+
+constexpr int64_t FWD_THREADS = 148 * 8 * TAIL_T, BWD_THREADS = 148 * 3 * TAIL_T;
+
+// Slots of a call: enough threads for every SM, at least `least` rows each.
+int plan(int rows, int units, int64_t threads, int least) {
+    return (int)std::max<int64_t>(1, std::min<int64_t>((rows + least - 1) / least, threads / units));
+}
+constexpr int BWD_LEAST = 4;
+
+bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+int check_args(int dtype, const TailArgs& a, int rows, int H, int S, const char* fn) {
+    RWKV_REQUIRE(valid_dtype(dtype) && valid_dtype(a.wdtype), RWKV_E_DTYPE, "%s: dtypes x=%d w=%d", fn, dtype, a.wdtype);
+    RWKV_REQUIRE(a.a && a.r && a.k && a.v && a.g && a.rk && a.w && a.b, RWKV_E_NULL, "%s: NULL argument", fn);
+    RWKV_REQUIRE(rows >= 1 && H >= 1 && H <= 1 << 16, RWKV_E_SHAPE, "%s: rows=%d H=%d (rows >= 1, H in 1..2^16)", fn,
+                 rows, H);
+    RWKV_REQUIRE(S == 32 || S == 64 || S == 128 || S == 256, RWKV_E_UNSUPPORTED, "%s: S=%d (32, 64, 128 or 256)", fn, S);
+    RWKV_REQUIRE(a.eps >= 0.f, RWKV_E_SHAPE, "%s: eps=%g must be >= 0", fn, a.eps);
+    RWKV_REQUIRE(al16(a.a) && al16(a.r) && al16(a.k) && al16(a.v) && al16(a.g) && al16(a.rk) && al16(a.w) && al16(a.b),
+                 RWKV_E_UNSUPPORTED, "%s: a tensor is not 16-byte aligned", fn);
+    return RWKV_OK;
+}
+
+}  // namespace
+}  // namespace rwkv
+
+using namespace rwkv;
+
+extern "C" int rwkv_tmix_tail_forward(int dtype, const void* wkv, const void* r, const void* k, const void* v,
+                                      const void* g, int wdtype, const void* rk, const void* weight, const void* bias,
+                                      float eps, void* out, int rows, int H, int S, rwkv_stream_t stream) {
+    const char* fn = "rwkv_tmix_tail_forward";
+    TailArgs a{wkv, r, k, v, g, rk, weight, bias, wdtype, 0, 0, rows, eps};
+    RWKV_REQUIRE(out, RWKV_E_NULL, "%s: NULL argument", fn);
+    if (int rc = check_args(dtype, a, rows, H, S, fn)) return rc;
+    RWKV_REQUIRE(al16(out), RWKV_E_UNSUPPORTED, "%s: a tensor is not 16-byte aligned", fn);
+    a.units = H * (S / 8);
+    a.slots = plan(rows, a.units, FWD_THREADS, 1);
+    return dispatch_dtype(dtype, [&]<typename T>() {
+        return dispatch_head(S, [&]<int L>() {
+            const int64_t threads = (int64_t)a.slots * a.units;
+            tmix_tail_kernel<T, L>
+                <<<(unsigned)((threads + TAIL_T - 1) / TAIL_T), TAIL_T, 0, (cudaStream_t)stream>>>(a, (T*)out);
+            return check_launch("tmix_tail_kernel");
+        });
+    });
+}
+
+extern "C" int64_t rwkv_tmix_tail_backward_workspace_size(int rows, int H, int S) {
+    if (rows < 1 || H < 1 || H > 1 << 16 || (S != 32 && S != 64 && S != 128 && S != 256)) return 0;
+    return (int64_t)plan(rows, H * (S / 8), BWD_THREADS, BWD_LEAST) * 3 * H * S * (int64_t)sizeof(float);
+}
+
+extern "C" int rwkv_tmix_tail_backward(int dtype, const void* dout, const void* wkv, const void* r, const void* k,
+                                       const void* v, const void* g, int wdtype, const void* rk, const void* weight,
+                                       const void* bias, float eps, void* dwkv, void* dr, void* dk, void* dv, void* dg,
+                                       void* drk, void* dweight, void* dbias, int rows, int H, int S, void* workspace,
+                                       int64_t workspace_bytes, rwkv_stream_t stream) {
+    const char* fn = "rwkv_tmix_tail_backward";
+    TailArgs a{wkv, r, k, v, g, rk, weight, bias, wdtype, 0, 0, rows, eps};
+    TailGrad o{dout, dwkv, dr, dk, dv, dg, nullptr};
+    RWKV_REQUIRE(dout && dwkv && dr && dk && dv && dg, RWKV_E_NULL, "%s: NULL argument", fn);
+    RWKV_REQUIRE(!drk == !dweight && !drk == !dbias, RWKV_E_NULL, "%s: give drk, dweight and dbias or none of them", fn);
+    if (int rc = check_args(dtype, a, rows, H, S, fn)) return rc;
+    RWKV_REQUIRE(al16(dout) && al16(dwkv) && al16(dr) && al16(dk) && al16(dv) && al16(dg) && al16(drk) && al16(dweight) &&
+                     al16(dbias),
+                 RWKV_E_UNSUPPORTED, "%s: a tensor is not 16-byte aligned", fn);
+    if (drk) {
+        const int64_t need = rwkv_tmix_tail_backward_workspace_size(rows, H, S);
+        RWKV_REQUIRE(workspace && workspace_bytes >= need, RWKV_E_WORKSPACE, "%s: workspace of %lld bytes, need %lld",
+                     fn, (long long)workspace_bytes, (long long)need);
+        RWKV_REQUIRE(al16(workspace), RWKV_E_UNSUPPORTED, "%s: workspace not 16-byte aligned", fn);
+        o.part = static_cast<float*>(workspace);
+    }
+    a.units = H * (S / 8);
+    a.slots = plan(rows, a.units, BWD_THREADS, BWD_LEAST);
+    return dispatch_dtype(dtype, [&]<typename T>() {
+        return dispatch_head(S, [&]<int L>() {
+            const cudaStream_t st = (cudaStream_t)stream;
+            const int64_t threads = (int64_t)a.slots * a.units;
+            tmix_tail_backward_kernel<T, L><<<(unsigned)((threads + TAIL_T - 1) / TAIL_T), TAIL_T, 0, st>>>(a, o);
+            if (int rc = check_launch("tmix_tail_backward_kernel")) return rc;
+            if (!drk) return ok();
+            const int64_t D = (int64_t)H * S;
+            return launch_param_join(ParamJoin{o.part, a.slots, 3 * D, D, {drk, dweight, dbias}, wdtype}, st);
+        });
+    });
+}
