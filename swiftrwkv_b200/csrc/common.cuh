@@ -110,7 +110,7 @@ __device__ __forceinline__ float warp_max(float v) {
     return v;
 }
 
-inline int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+__host__ __device__ inline int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 // Programmatic dependent launch.  A kernel launched with launch_pdl may start
 // while its predecessor in the stream is still running: it must call

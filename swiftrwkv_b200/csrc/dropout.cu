@@ -10,30 +10,39 @@ namespace {
 
 constexpr int DT = 256, DU = 4;
 
-template <typename T>
-__global__ void __launch_bounds__(DT) dropout_kernel(const T* x, T* y, int64_t n, const Dropout d) {
-    const int64_t u0 = blockIdx.x * (int64_t)(DT * DU) + threadIdx.x, units = n / 8;
+template <typename T, int MODE>
+__global__ void __launch_bounds__(DT) dropout_kernel(const T* x, T* y, int64_t n, const __grid_constant__ Dropout d) {
+    // places within the thread block's part in 32 bits: its first unit is a multiple of
+    // DT DU, so that no carry leaves the low word of a block's number
+    const int64_t u0 = blockIdx.x * (int64_t)(DT * DU), units = n / 8;
+    const int mine = (int)min((int64_t)(DT * DU), units - u0);
+    x += 8 * u0;
+    y += 8 * u0;
     Raw8<T> raw[DU];
 #pragma unroll
-    for (int j = 0; j < DU; j++)
-        if (u0 + j * DT < units) raw[j].load(x + 8 * (u0 + j * DT));
-    const DropKey key = drop_key(d);
+    for (int j = 0; j < DU; j++) {
+        const int u = j * DT + threadIdx.x;
+        if (u < mine) raw[j].load(x + 8 * u);
+    }
+    const DropKey key = drop_key<MODE>(d);
 #pragma unroll
     for (int j = 0; j < DU; j++) {
-        const int64_t u = u0 + j * DT;
-        if (u >= units) continue;
+        const int u = j * DT + threadIdx.x;
+        if (u >= mine) continue;
         float v[8];
         raw[j].floats(v);
-        drop_at<8>(v, key, 8 * (uint64_t)u, d.threshold, d.scale);
+        if constexpr (MODE != DROP_NONE)
+            drop_block(v, philox<MODE>(d, key, (uint32_t)u0 + u, (uint32_t)(u0 >> 32)), d);
         store8(y + 8 * u, v);
     }
     // the tensor's last n % 8 elements
-    const int64_t t = 8 * units + threadIdx.x;
-    if (blockIdx.x == 0 && t < n) {
-        const uint4 r = philox(key, units);
+    const int t = threadIdx.x;
+    if (u0 + DT * DU >= units && t < (int)(n % 8)) {
+        const uint4 r = philox<MODE == DROP_STATE ? DROP_STATE : DROP_KEY>(d, key, (uint32_t)units, (uint32_t)(units >> 32));
         const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-        const uint32_t bits = w[threadIdx.x / 2 & 3] >> 16 * (threadIdx.x & 1) & 0xffffu;
-        y[t] = from_f<T>(bits < d.threshold ? 0.f : __fmul_rn(to_f<T>(x[t]), d.scale));
+        const int64_t at = 8 * (units - u0) + t;
+        const uint32_t bits = w[t / 2] >> 16 * (t & 1) & 0xffffu;
+        y[at] = from_f<T>(bits < d.threshold ? 0.f : __fmul_rn(to_f<T>(x[at]), d.scale));
     }
 }
 
@@ -54,7 +63,9 @@ extern "C" int rwkv_dropout(int dtype, const void* x, double p, uint64_t seed, u
     const Dropout d = make_dropout(p, 1.0, seed, offset, state);
     return dispatch_dtype(dtype, [&]<typename T>() {
         const int64_t blocks = (n / 8 + DT * DU - 1) / (DT * DU);
-        dropout_kernel<T><<<(unsigned)(blocks ? blocks : 1), DT, 0, (cudaStream_t)stream>>>((const T*)x, (T*)y, n, d);
-        return check_launch("dropout_kernel");
+        return dispatch_drop(d, [&]<int MODE>() {
+            dropout_kernel<T, MODE><<<(unsigned)(blocks ? blocks : 1), DT, 0, (cudaStream_t)stream>>>((const T*)x, (T*)y, n, d);
+            return check_launch("dropout_kernel");
+        });
     });
 }

@@ -2,55 +2,476 @@
 // scaled, and the sum normed for the next branch, in one pass.
 //
 //   forward   s = x + scale drop(branch), y = (s - mean) rstd w + b
-//   backward  ds as the layer norm's dx (dres: the gradient of s past the norm),
-//             dx = ds, dbranch = scale drop(ds), dw, db
+//   backward  h = (s - mean) rstd, g = dy w:
+//             dx = rstd (g - mean(g) - h mean(g h)) + dres, dbranch = scale drop(dx),
+//             dw = sum_n dy h, db = sum_n dy
 //
-// The kernels are the layer norm's (layer_norm.cuh) with the branch: 4 tensors
-// forward (x, branch, s, y) and 5 backward (dy, s, dres, dx, dbranch), or 1 + 1/32
-// bytes per element for s as a checkpoint.  s is normed and checkpointed before its
-// rounding: y is that of the sum in fp32.
-#include "layer_norm.cuh"
+// HBM's part is 4 tensors forward (x, branch, s, y) and 5 backward (dy, s, dres, dx,
+// dbranch), 1 + 1/32 bytes per element for s as a checkpoint.  s is normed and
+// checkpointed in fp32, before its rounding.  Beside that both are bound by the issue
+// of instructions: a vector of 8 elements takes 16 bytes per tensor, and 75
+// instructions for its random bits alone, so that the kernels count them: pairs of
+// fp32 in one instruction, several vectors or rows to a thread's share of a row's sums.
+#include <algorithm>
+
+#include "ckpt8.cuh"
+#include "copy_async.cuh"
+#include "f32x2.cuh"
+#include "param_join.cuh"
+#include "philox.cuh"
+#include "resident.cuh"
 
 namespace rwkv {
 namespace {
 
-template <typename T, bool CK>
-int launch_rn_fwd(const LnFwdArgs& a, cudaStream_t st) {
-    // threads, vectors per thread and rows as in the layer norm
-    constexpr int R = CK ? 1 : 2;
-    const int nvec = a.D / Vec16<T>::N;
-    if (nvec <= 64) launch_ln_fwd_t<T, 64, 1, 2, CK, true>(a, st);
-    else if (nvec <= 64 * 2) launch_ln_fwd_t<T, 64, 2, 2, CK, true>(a, st);
-    else if (nvec <= 64 * 3) launch_ln_fwd_t<T, 64, 3, 2, CK, true>(a, st);
-    else if (nvec <= 128 * 2) launch_ln_fwd_t<T, 128, 2, 2, CK, true>(a, st);
-    else if (nvec <= 64 * 5) launch_ln_fwd_t<T, 64, 5, R, CK, true>(a, st);
-    else if (nvec <= 256 * 2) launch_ln_fwd_t<T, 256, 2, R, CK, true>(a, st);
-    else if (nvec <= 256 * 5) launch_ln_fwd_t<T, 256, 5, R, CK, true>(a, st);
-    else launch_ln_fwd_t<T, 512, 3, 1, CK, true>(a, st);
-    return check_launch("ln_fwd_kernel (residual)");
+template <int MODE, typename T>
+__device__ __forceinline__ void branch_part(Pairs<T>& v, const DropKey& key, uint64_t i, const Dropout& d) {
+    if constexpr (MODE == DROP_NONE) {
+#pragma unroll
+        for (int k = 0; k < Pairs<T>::P; k++) v[k] = mul2(v[k], both(d.scale));
+    } else {
+        drop_vector<MODE, Pairs<T>::VE>(v.floats(), key, i, d);
+    }
 }
 
-template <typename T, bool CK>
-int launch_rn_bwd(const LnBwdArgs& a, void* dw, void* db, cudaStream_t st) {
-    constexpr int R = CK ? 1 : 2;
+// The sums over a warp of N values per lane (N a power of two), value i in the lanes
+// i 32 / N ..: each exchange halves the values a lane holds.
+template <int N>
+__device__ __forceinline__ float lanes_sum(float* v, int lane) {
+#pragma unroll
+    for (int n = N, o = 16; n > 1; n /= 2, o /= 2) {
+        const bool up = lane & o;
+#pragma unroll
+        for (int i = 0; i < n / 2; i++) {
+            const float keep = up ? v[i + n / 2] : v[i], send = up ? v[i] : v[i + n / 2];
+            v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+        }
+    }
+    float s = v[0];
+#pragma unroll
+    for (int o = 16 / N; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    return s;
+}
+
+// ------------------------------------------------------------------- forward
+
+struct RnFwdArgs {
+    const void *x, *branch, *w, *b;
+    void *sum, *y;
+    float *mean, *rstd;
+    int8_t* codes;
+    uint8_t* exps;
+    int wdtype, rows, D, G;
+    float eps;
+    Dropout drop;
+};
+
+// the largest magnitude of three, NaN if one is
+__device__ __forceinline__ float top3(float a, float b, float c) {
+    float d;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// four codes as ck_pack4, where none is clipped and the group holds no NaN
+__device__ __forceinline__ uint32_t pack4_within(const float2& a, const float2& b, float inv) {
+    const float2 m = both(12582912.f), p = fma2(a, both(inv), m), q = fma2(b, both(inv), m);
+    return __byte_perm(__byte_perm(__float_as_uint(p.x), __float_as_uint(p.y), 0x0040),
+                       __byte_perm(__float_as_uint(q.x), __float_as_uint(q.y), 0x0040), 0x5410);
+}
+
+// The codes of a vector, and its group's exponent byte (32 / VE neighbouring threads).
+// Clipping takes a third of the packing; only groups whose largest rounds up to 128 (or
+// that stand for NaN) need it.
+template <typename T>
+__device__ __forceinline__ void checkpoint(const Pairs<T>& s, int8_t* codes, uint8_t* exps, bool in, bool first) {
+    constexpr int VE = Pairs<T>::VE;
+    float t = top3(s[0].x, s[0].y, s[1].x);
+    if constexpr (VE == 8) t = top3(top3(t, s[1].y, s[2].x), top3(s[2].y, s[3].x, s[3].y), t);
+    else t = top3(t, s[1].y, t);
+    uint32_t top = __float_as_uint(t);
+#pragma unroll
+    for (int o = 1; o < CK_GROUP / VE; o *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const uint32_t e = ck_exponent(top);
+    const float inv = ck_inv_scale(e);
+    uint32_t c[VE / 4];
+    if (__uint_as_float(top) * inv < 127.5f) {
+#pragma unroll
+        for (int k = 0; k < VE / 4; k++) c[k] = pack4_within(s[2 * k], s[2 * k + 1], inv);
+    } else {
+#pragma unroll
+        for (int k = 0; k < VE / 4; k++) c[k] = ck_pack4(s[2 * k].x, s[2 * k].y, s[2 * k + 1].x, s[2 * k + 1].y, inv);
+    }
+    if (!in) return;
+    if constexpr (VE == 8) *reinterpret_cast<uint2*>(codes) = make_uint2(c[0], c[VE / 4 - 1]);
+    else *reinterpret_cast<uint32_t*>(codes) = c[0];
+    if (first) *exps = (uint8_t)e;
+}
+
+// A block of TPR threads takes R rows, at most NV vectors of a row per thread: vector j
+// of thread t is t + j TPR.
+//
+// Statistics of a row from one round of sums: each warp takes the mean of its first
+// lane's first vector as a pivot p and leaves p, sum(s - p) and sum (s - p)^2; around the
+// first warp's pivot these join to mean and variance.  The pivot is the mean of VE
+// elements of the row, so that (p - mean)^2 <= M / VE with M the row's centred sum of
+// squares: what cancels in a warp's share of n elements is at most n M / VE, and a fraction of M
+// for rows without outliers.  A constant row gives its value as the mean, exactly.
+template <typename T, int TPR, int NV, int R, bool CK, int MODE>
+__global__ void __launch_bounds__(TPR, 1) rn_fwd_kernel(const __grid_constant__ RnFwdArgs a) {
+    constexpr int VE = Vec16<T>::N, P = VE / 2, NW = TPR / 32;
+    __shared__ alignas(16) float red[R][NW][4];  // pivot, sum, squares of each warp
+    const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+    const int nvec = a.D / VE, row0 = blockIdx.x * R;
+    const int64_t at = (int64_t)row0 * nvec;  // in vectors
+    const uint4* const x = static_cast<const uint4*>(a.x) + at;
+    const uint4* const br = static_cast<const uint4*>(a.branch) + at;
+    Pairs<T> s[R][NV];
+    {
+        uint4 rx[R][NV], rb[R][NV];
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int j = 0; j < NV; j++) {
+                const int v = t + j * TPR;
+                const bool in = v < nvec && row0 + r < a.rows;
+                rx[r][j] = in ? __ldcs(x + r * nvec + v) : make_uint4(0, 0, 0, 0);
+                rb[r][j] = in ? __ldcs(br + r * nvec + v) : make_uint4(0, 0, 0, 0);
+            }
+        const DropKey key = drop_key<MODE>(a.drop);
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int j = 0; j < NV; j++) {
+                const int v = t + j * TPR;
+                const bool in = v < nvec && row0 + r < a.rows;
+                Pairs<T> q;
+                s[r][j].unpack(rx[r][j]);
+                q.unpack(rb[r][j]);
+                branch_part<MODE>(q, key, (uint64_t)(at + r * nvec + v), a.drop);
+#pragma unroll
+                for (int k = 0; k < P; k++) s[r][j][k] = add2(s[r][j][k], q[k]);
+                if (in) __stcs(static_cast<uint4*>(a.sum) + at + r * nvec + v, s[r][j].pack());
+                if constexpr (CK)
+                    checkpoint(s[r][j], a.codes + (at + r * nvec + v) * VE,
+                               a.exps + (int64_t)(row0 + r) * a.G + v / (CK_GROUP / VE), in, lane % (CK_GROUP / VE) == 0);
+            }
+    }
+    float sums[2 * R];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        // in halves, so that equal values add exactly
+        const Pairs<T>& f = s[r][0];
+        const float2 h = P == 4 ? add2(add2(f[0], f[1]), add2(f[2 % P], f[3 % P])) : add2(f[0], f[1]);
+        const float pivot = __shfl_sync(0xffffffffu, h.x + h.y, 0) * (1.f / VE);
+        if (lane == 0) red[r][warp][0] = pivot;
+        float2 d1 = both(0.f), d2 = both(0.f);
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            const float2 n = both(t + j * TPR < nvec ? -pivot : 0.f);  // zeros beyond the row's end
+#pragma unroll
+            for (int k = 0; k < P; k++) {
+                const float2 d = add2(s[r][j][k], n);
+                d1 = add2(d1, d);
+                d2 = fma2(d, d, d2);
+            }
+        }
+        sums[2 * r] = d1.x + d1.y;
+        sums[2 * r + 1] = d2.x + d2.y;
+    }
+    const float p = lanes_sum<2 * R>(sums, lane);
+    if (lane % (16 / R) == 0) red[lane / (32 / R)][warp][1 + lane / (16 / R) % 2] = p;
+    if constexpr (NW > 1) __syncthreads();
+    else __syncwarp();
+    float mean[R], rstd[R];
+    const float inv_d = 1.f / (float)a.D;
+    // elements of warp w's share of a row
+    auto count = [&](int w) {
+        int n = 0;
+#pragma unroll
+        for (int j = 0; j < NV; j++) n += max(0, min(32, nvec - w * 32 - j * TPR));
+        return (float)(n * VE);
+    };
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        float u = 0.f, q = 0.f;
+        const float p0 = red[r][0][0];
+        if constexpr (NW <= 4) {  // every thread joins the warps' sums
+            float e[NW], d1[NW], c[NW];
+#pragma unroll
+            for (int w = 0; w < NW; w++) {
+                const float4 f = *reinterpret_cast<const float4*>(red[r][w]);
+                e[w] = f.x - p0, d1[w] = f.y, q += f.z, c[w] = count(w);
+                u += fmaf(c[w], e[w], d1[w]);
+            }
+            u *= inv_d;
+#pragma unroll
+            for (int w = 0; w < NW; w++) {
+                const float f = e[w] - u;
+                q = fmaf(f, fmaf(c[w], f, 2.f * d1[w]), q);
+            }
+        } else {  // lane % NW has a warp's
+            const float4 f = *reinterpret_cast<const float4*>(red[r][lane % NW]);
+            const float e = f.x - p0, c = count(lane % NW);
+            u = fmaf(c, e, f.y);
+#pragma unroll
+            for (int m = NW / 2; m > 0; m >>= 1) u += __shfl_xor_sync(0xffffffffu, u, m);
+            u *= inv_d;
+            q = fmaf(e - u, fmaf(c, e - u, 2.f * f.y), f.z);
+#pragma unroll
+            for (int m = NW / 2; m > 0; m >>= 1) q += __shfl_xor_sync(0xffffffffu, q, m);
+        }
+        mean[r] = p0 + u;
+        rstd[r] = 1.f / sqrtf((q < 0.f ? 0.f : q) * inv_d + a.eps);  // (a NaN passes)
+        if (t == 0 && a.mean && row0 + r < a.rows) {
+            a.mean[row0 + r] = mean[r];
+            a.rstd[row0 + r] = rstd[r];
+        }
+    }
+    uint4* const y = static_cast<uint4*>(a.y) + at;
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+        const int v = t + j * TPR;
+        if (v >= nvec) continue;
+        Pairs<T> w, b;
+        load_params<VE>(a.w, a.wdtype, v * VE, w.floats());
+        load_params<VE>(a.b, a.wdtype, v * VE, b.floats());
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            Pairs<T> o;
+#pragma unroll
+            for (int k = 0; k < P; k++) o[k] = fma2(mul2(add2(s[r][j][k], both(-mean[r])), both(rstd[r])), w[k], b[k]);
+            if (row0 + r < a.rows) __stcs(y + r * nvec + v, o.pack());
+        }
+    }
+}
+
+// ------------------------------------------------------------------ backward
+
+struct RnBwdArgs {
+    const void *dy, *s;
+    const int8_t* codes;
+    const uint8_t* exps;
+    const void* w;
+    const float *mean, *rstd;
+    const void* dres;
+    void *dx, *dbranch;
+    float* part;  // [blocks][2][D] sums of dy h and dy over the block's rows, or NULL
+    int wdtype, rows, D, G;
+    Dropout drop;
+};
+
+constexpr int RN_STAGES = 3;
+
+// A block walks over rows; thread t owns the vectors t + j blockDim.x of every row, so
+// that the sums over rows stay in registers until the end.  dy, s (or its codes) and dres
+// run RN_STAGES - 1 rows ahead through a ring in shared memory that is private to each
+// thread (cp.async); one barrier per row, for its two sums (buffers alternating).
+//
+// 16384 x 2560 bf16: 65 us without dropout, dense or from a checkpoint (floors 64 and 58),
+// 75 and 81 with it.  Bound then by issue: 290 to 315 instructions per vector, 100 of them for the
+// random bits, at 57 % of the slots with the 13 warps per SM that the registers leave.
+template <typename T, bool CK, int MODE, int NV, int MAXT, int MINB>
+__global__ void __launch_bounds__(MAXT, MINB) rn_bwd_kernel(const __grid_constant__ RnBwdArgs a) {
+    constexpr int VE = Vec16<T>::N, P = VE / 2;
+    extern __shared__ uint4 ring[];  // [stage][dy | s | dres][NV][thread]
+    __shared__ float red[2][16][2];
+    using Codes = std::conditional_t<VE == 8, uint2, uint32_t>;  // of one vector
+    const int t = threadIdx.x, nt = blockDim.x, warp = t >> 5, lane = t & 31, nw = nt >> 5;
+    const int nvec = a.D / VE;
+    const float inv_d = 1.f / (float)a.D;
+    const DropKey key = drop_key<MODE>(a.drop);
+    Pairs<T> w[NV], sw[NV], sb[NV];
+    bool has[NV];
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+        const int v = t + j * nt;
+        has[j] = v < nvec;
+        load_params<VE>(a.w, a.wdtype, (int64_t)(has[j] ? v : 0) * VE, w[j].floats());
+#pragma unroll
+        for (int k = 0; k < P; k++) sw[j][k] = sb[j][k] = both(0.f);
+    }
+    const int stage_n = 3 * NV * nt;
+    auto slot = [&](int base, int part, int j) { return ring + base + (part * NV + j) * nt; };
+    const int64_t vstep = (int64_t)gridDim.x * nvec;  // in vectors
+    int64_t at = (int64_t)blockIdx.x * nvec + t, fat = at;
+    auto fetch = [&](int64_t row, int base) {
+        if (row < a.rows) {
+#pragma unroll
+            for (int j = 0; j < NV; j++)
+                if (has[j]) {
+                    const int64_t i = fat + j * nt;
+                    copy_async<16>(slot(base, 0, j), static_cast<const uint4*>(a.dy) + i);
+                    if constexpr (CK) copy_async<VE>(slot(base, 1, j), reinterpret_cast<const Codes*>(a.codes) + i);
+                    else copy_async<16>(slot(base, 1, j), static_cast<const uint4*>(a.s) + i);
+                    if (a.dres) copy_async<16>(slot(base, 2, j), static_cast<const uint4*>(a.dres) + i);
+                }
+        }
+        copy_commit();
+        fat += vstep;
+    };
+    // a row's statistics and exponents, one row ahead in registers (as 4-byte copies
+    // into the ring they cost 10 us of 70)
+    float nmean, nrstd;
+    uint32_t ex[NV], nex[NV];
+    auto fetch_small = [&](int64_t next) {
+        const uint32_t row = min((uint32_t)next, (uint32_t)a.rows - 1);  // of no use past the end
+        nmean = a.mean[row];
+        nrstd = a.rstd[row];
+        if constexpr (CK)
+#pragma unroll
+            for (int j = 0; j < NV; j++)
+                nex[j] = has[j] ? a.exps[(int64_t)row * a.G + (t + j * nt) / (CK_GROUP / VE)] : 0u;
+    };
+#pragma unroll
+    for (int i = 0; i < RN_STAGES - 1; i++) fetch(blockIdx.x + (int64_t)i * gridDim.x, t + i * stage_n);
+    fetch_small(blockIdx.x);
+    int cur = t, put = t + (RN_STAGES - 1) * stage_n, buf = 0;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, at += vstep, buf ^= 1) {
+        fetch(row + (int64_t)(RN_STAGES - 1) * gridDim.x, put);
+        copy_wait<RN_STAGES - 1>();
+        const float mean = nmean, rstd = nrstd;
+        if constexpr (CK)
+#pragma unroll
+            for (int j = 0; j < NV; j++) ex[j] = nex[j];
+        fetch_small(row + gridDim.x);
+        // pass 1: h, the sums over the row (g, g h) and over the rows (dy h, dy)
+        Pairs<T> h[NV];
+        float2 s1 = both(0.f), s2 = both(0.f);
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            if (!has[j]) continue;
+            Pairs<T> d;
+            d.unpack(*slot(cur, 0, j));
+            // s - mean in one rounding: no multiple of rstd cancels where |mean| is large
+            if constexpr (CK) {
+                const uint32_t* c = reinterpret_cast<const uint32_t*>(slot(cur, 1, j));
+                ck_codes4(c[0], h[j].floats());
+                if constexpr (VE == 8) ck_codes4(c[1], h[j].floats() + 4);
+                const float2 scale = both(ck_scale(ex[j]));
+#pragma unroll
+                for (int k = 0; k < P; k++) h[j][k] = fma2(h[j][k], scale, both(-mean));
+            } else {
+                h[j].unpack(*slot(cur, 1, j));
+#pragma unroll
+                for (int k = 0; k < P; k++) h[j][k] = add2(h[j][k], both(-mean));
+            }
+#pragma unroll
+            for (int k = 0; k < P; k++) {
+                h[j][k] = mul2(h[j][k], both(rstd));
+                const float2 g = mul2(d[k], w[j][k]);
+                s1 = add2(s1, g);
+                s2 = fma2(g, h[j][k], s2);
+                sw[j][k] = fma2(d[k], h[j][k], sw[j][k]);
+                sb[j][k] = add2(sb[j][k], d[k]);
+            }
+        }
+        // over the warp: the sum of g ends up in lanes 0..15, that of g h in 16..31
+        float sums[2] = {s1.x + s1.y, s2.x + s2.y};
+        const float p = lanes_sum<2>(sums, lane);
+        if ((lane & 15) == 0) red[buf][warp][lane >> 4] = p;
+        __syncthreads();
+        float tot = (lane & 15) < nw ? red[buf][lane & 15][lane >> 4] : 0.f;
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) tot += __shfl_xor_sync(0xffffffffu, tot, o);
+        tot *= inv_d * -rstd;
+        // pass 2: dx = rstd (g - m1 - h m2) + dres
+        const float2 c0 = both(__shfl_sync(0xffffffffu, tot, 0)), c1 = both(__shfl_sync(0xffffffffu, tot, 16));
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            if (!has[j]) continue;
+            Pairs<T> d, o;
+            d.unpack(*slot(cur, 0, j));
+            if (a.dres) {
+                o.unpack(*slot(cur, 2, j));
+#pragma unroll
+                for (int k = 0; k < P; k++) o[k] = add2(o[k], c0);
+            } else {
+#pragma unroll
+                for (int k = 0; k < P; k++) o[k] = c0;
+            }
+#pragma unroll
+            for (int k = 0; k < P; k++) o[k] = fma2(mul2(d[k], w[j][k]), both(rstd), fma2(h[j][k], c1, o[k]));
+            const int64_t i = at + j * nt;
+            __stcs(static_cast<uint4*>(a.dx) + i, o.pack());
+            branch_part<MODE>(o, key, (uint64_t)i, a.drop);
+            __stcs(static_cast<uint4*>(a.dbranch) + i, o.pack());
+        }
+        put = cur;
+        cur = cur == t + (RN_STAGES - 1) * stage_n ? t : cur + stage_n;
+    }
+    copy_wait<0>();
+    if (!a.part) return;
+    float* part = a.part + (int64_t)blockIdx.x * 2 * a.D;
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+        if (!has[j]) continue;
+        float* o = part + (int64_t)(t + j * nt) * VE;
+#pragma unroll
+        for (int k = 0; k < P; k += 2) {
+            *reinterpret_cast<float4*>(o + 2 * k) = make_float4(sw[j][k].x, sw[j][k].y, sw[j][k + 1].x, sw[j][k + 1].y);
+            *reinterpret_cast<float4*>(o + a.D + 2 * k) = make_float4(sb[j][k].x, sb[j][k].y, sb[j][k + 1].x, sb[j][k + 1].y);
+        }
+    }
+}
+
+// ------------------------------------------------------------------- launches
+
+constexpr int RN_VECTORS = 512 * 3;
+// Blocks of the backward at most (the partial sums of the parameters are as many rows)
+int most_blocks(int D) { return D <= 512 ? 148 * 8 : 148 * 4; }
+
+template <typename T, int TPR, int NV, int R, bool CK, int MODE>
+void launch_fwd(const RnFwdArgs& a, cudaStream_t st) {
+    rn_fwd_kernel<T, TPR, NV, R, CK, MODE><<<ceil_div(a.rows, R), TPR, 0, st>>>(a);
+}
+
+template <typename T, bool CK, int MODE>
+int forward(const RnFwdArgs& a, cudaStream_t st) {
+    const int nvec = a.D / Vec16<T>::N;
+    if (nvec <= 64) launch_fwd<T, 64, 1, 2, CK, MODE>(a, st);
+    else if (nvec <= 64 * 2) launch_fwd<T, 64, 2, 2, CK, MODE>(a, st);
+    else if (nvec <= 64 * 3) launch_fwd<T, 64, 3, 2, CK, MODE>(a, st);
+    else if (nvec <= 64 * 4) launch_fwd<T, 64, 4, 1, CK, MODE>(a, st);
+    else if (nvec <= 64 * 5) launch_fwd<T, 64, 5, 1, CK, MODE>(a, st);
+    else if (nvec <= 128 * 4) launch_fwd<T, 128, 4, 1, CK, MODE>(a, st);
+    else if (nvec <= 256 * 4) launch_fwd<T, 256, 4, 1, CK, MODE>(a, st);
+    else launch_fwd<T, 512, 3, 1, CK, MODE>(a, st);
+    return check_launch("rn_fwd_kernel");
+}
+
+template <typename T, bool CK, int MODE, int NV, int MAXT, int MINB>
+cudaError_t launch_bwd(const RnBwdArgs& a, int* blocks, cudaStream_t st) {
+    auto kern = rn_bwd_kernel<T, CK, MODE, NV, MAXT, MINB>;
+    const int nt = ceil_div(ceil_div(a.D / Vec16<T>::N, NV), 32) * 32;
+    constexpr int PER_T = RN_STAGES * 3 * NV * 16;  // shared memory of a thread
+    // as many blocks as are resident, so that they all run in one wave
+    static ResidentBlocks resident;
+    int per_sm;
+    const cudaError_t e = resident.get(kern, nt, PER_T * nt, PER_T * MAXT, &per_sm);
+    if (e != cudaSuccess) return e;
+    *blocks = std::min(a.rows, std::min(148 * per_sm, most_blocks(a.D)));
+    kern<<<*blocks, nt, PER_T * nt, st>>>(a);
+    return cudaGetLastError();
+}
+
+template <typename T, bool CK, int MODE>
+int backward(const RnBwdArgs& a, void* dw, void* db, cudaStream_t st) {
     const int nvec = a.D / Vec16<T>::N;
     int blocks;
-    cudaError_t e = nvec > 1024  ? launch_ln_bwd_t<T, CK, 3, 1, 512, 1, false, true>(a, &blocks, st)
-                    : nvec > 512 ? launch_ln_bwd_t<T, CK, 2, 1, 512, 1, false, true>(a, &blocks, st)
-                    : nvec > 320 ? launch_ln_bwd_t<T, CK, 1, R, 512, 1, false, true>(a, &blocks, st)
-                                 : launch_ln_bwd_t<T, CK, 1, R, 320, 2, false, true>(a, &blocks, st);
-    if (e != cudaSuccess) return fail(RWKV_E_CUDA, "ln_bwd_kernel (residual): %s", cudaGetErrorString(e));
-    if (int rc = check_launch("ln_bwd_kernel (residual)")) return rc;
-    if (!a.part) return ok();
-    e = launch_pdl(ln_bwd_params_kernel, dim3(ceil_div(2 * (int64_t)a.D, 32)), dim3(1024), 0, st, (const float*)a.part,
-                   blocks, a.D, dw, db, a.wdtype);
-    if (e != cudaSuccess) return fail(RWKV_E_CUDA, "ln_bwd_params_kernel: %s", cudaGetErrorString(e));
-    return ok();
+    const cudaError_t e = nvec > 1024  ? launch_bwd<T, CK, MODE, 3, 512, 1>(a, &blocks, st)
+                          : nvec > 512 ? launch_bwd<T, CK, MODE, 2, 512, 1>(a, &blocks, st)
+                          : nvec > 320 ? launch_bwd<T, CK, MODE, 2, 256, 2>(a, &blocks, st)
+                                       : launch_bwd<T, CK, MODE, 2, 160, 3>(a, &blocks, st);
+    if (e != cudaSuccess) return fail(RWKV_E_CUDA, "rn_bwd_kernel: %s", cudaGetErrorString(e));
+    return a.part ? launch_param_join(ParamJoin{a.part, blocks, 2 * (int64_t)a.D, a.D, {dw, db, nullptr}, a.wdtype}, st) : ok();
 }
+
+bool al(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+uintptr_t elem(int dtype) { return dtype == RWKV_F32 ? 4 : 2; }
 
 int check_sizes(int dtype, int wdtype, int rows, int D, double p, double scale, const char* fn) {
     RWKV_REQUIRE(valid_dtype(dtype) && valid_dtype(wdtype), RWKV_E_DTYPE, "%s: dtypes x=%d w=%d", fn, dtype, wdtype);
-    const int most = dtype == RWKV_F32 ? LN_BWD_VECTORS * 4 : LN_BWD_VECTORS * 8;
+    const int most = dtype == RWKV_F32 ? RN_VECTORS * 4 : RN_VECTORS * 8;
     RWKV_REQUIRE(rows >= 1 && D >= 1, RWKV_E_SHAPE, "%s: rows=%d D=%d", fn, rows, D);
     RWKV_REQUIRE(D % 8 == 0 && D <= most, RWKV_E_UNSUPPORTED, "%s: D=%d must be a multiple of 8, at most %d", fn, D, most);
     RWKV_REQUIRE(p >= 0.0 && p <= 1.0, RWKV_E_SHAPE, "%s: p=%g must be in 0..1", fn, p);
@@ -78,15 +499,18 @@ extern "C" int rwkv_residual_norm_forward(int dtype, const void* x, const void* 
     RWKV_REQUIRE(al(x, 16) && al(branch, 16) && al(weight, 16) && al(bias, 16) && al(sum, 16) && al(y, 16) &&
                      al(codes, 8) && al(state, 8) && al(mean, 4) && al(rstd, 4),
                  RWKV_E_UNSUPPORTED, "%s: a tensor is not 16-byte aligned (codes, state: 8; mean, rstd: 4)", fn);
-    const LnFwdArgs a{x,  weight, bias, y, mean, rstd, codes, exps, wdtype, rows, D, ceil_div(D, CK_GROUP),
-                      eps, branch, sum, make_dropout(p, scale, seed, offset, state)};
+    const RnFwdArgs a{x,    branch, weight, bias, sum, y, mean, rstd, codes, exps, wdtype, rows, D, ceil_div(D, CK_GROUP),
+                      eps, make_dropout(p, scale, seed, offset, state)};
     return dispatch_dtype(dtype, [&]<typename T>() {
-        return codes ? launch_rn_fwd<T, true>(a, (cudaStream_t)stream) : launch_rn_fwd<T, false>(a, (cudaStream_t)stream);
+        return dispatch_drop(a.drop, [&]<int MODE>() {
+            return codes ? forward<T, true, MODE>(a, (cudaStream_t)stream) : forward<T, false, MODE>(a, (cudaStream_t)stream);
+        });
     });
 }
 
 extern "C" int64_t rwkv_residual_norm_backward_workspace_size(int rows, int D) {
-    return D <= LN_BWD_VECTORS * 8 ? rwkv_layer_norm_backward_workspace_size(rows, D) : 0;
+    if (rows < 1 || D < 1 || D > RN_VECTORS * 8) return 0;
+    return (int64_t)std::min(rows, most_blocks(D)) * 2 * D * (int64_t)sizeof(float);
 }
 
 extern "C" int rwkv_residual_norm_backward(int dtype, const void* dy, const void* sum, const int8_t* codes,
@@ -110,10 +534,13 @@ extern "C" int rwkv_residual_norm_backward(int dtype, const void* dy, const void
                      fn, (long long)workspace_bytes, (long long)need);
         RWKV_REQUIRE(al(workspace, 16), RWKV_E_UNSUPPORTED, "%s: workspace not 16-byte aligned", fn);
     }
-    const LnBwdArgs a{dy,   sum,  codes, exps, weight, mean, rstd, dres, dx, dweight ? static_cast<float*>(workspace) : nullptr,
-                      wdtype, rows, D, ceil_div(D, CK_GROUP), dbranch, make_dropout(p, scale, seed, offset, state)};
+    const RnBwdArgs a{dy,   sum,  codes, exps, weight, mean, rstd, dres, dx, dbranch,
+                      dweight ? static_cast<float*>(workspace) : nullptr, wdtype, rows, D, ceil_div(D, CK_GROUP),
+                      make_dropout(p, scale, seed, offset, state)};
     return dispatch_dtype(dtype, [&]<typename T>() {
-        return codes ? launch_rn_bwd<T, true>(a, dweight, dbias, (cudaStream_t)stream)
-                     : launch_rn_bwd<T, false>(a, dweight, dbias, (cudaStream_t)stream);
+        return dispatch_drop(a.drop, [&]<int MODE>() {
+            return codes ? backward<T, true, MODE>(a, dweight, dbias, (cudaStream_t)stream)
+                         : backward<T, false, MODE>(a, dweight, dbias, (cudaStream_t)stream);
+        });
     });
 }

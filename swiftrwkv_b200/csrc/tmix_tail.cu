@@ -16,6 +16,7 @@
 #include <algorithm>
 
 #include "ckpt8.cuh"
+#include "copy_async.cuh"
 #include "param_join.cuh"
 
 namespace rwkv {
@@ -35,6 +36,30 @@ struct TailGrad {
     float* part;  // [slots][drk, dw, db][D], or NULL
 };
 
+// The vectors of a row that a thread owns run ahead of their use by a stage or two
+// through a ring in shared memory that is private to the thread (cp.async, no
+// barrier), so that HBM stays busy through a head's sums.
+template <typename T, int N>
+struct TailRing {
+    static constexpr int W = Raw8<T>::W, STAGES = sizeof(T) == 2 ? 3 : 2;
+    uint4 r[STAGES][N * W][TAIL_T];
+
+    // N tensors' 8 elements at `at`, or zeros
+    __device__ __forceinline__ void fetch(int stage, const void* const* p, int64_t at, bool in) {
+#pragma unroll
+        for (int i = 0; i < N; i++)
+#pragma unroll
+            for (int w = 0; w < W; w++)
+                copy_async_n<16>(&r[stage][i * W + w][threadIdx.x],
+                                 reinterpret_cast<const uint4*>(static_cast<const T*>(p[i]) + at) + w, in ? 16 : 0);
+        copy_commit();
+    }
+    __device__ __forceinline__ void floats(int stage, int i, float* v) const {
+#pragma unroll
+        for (int w = 0; w < W; w++) Vec16<T>::unpack(r[stage][i * W + w][threadIdx.x], v + w * Vec16<T>::N);
+    }
+};
+
 // L lanes a head.  All threads of a warp take the same number of steps, with or
 // without a row, for the shuffles.
 template <typename T, int L>
@@ -47,25 +72,33 @@ __global__ void __launch_bounds__(TAIL_T) tmix_tail_kernel(const TailArgs a, T* 
     load_params<8>(a.rk, a.wdtype, 8 * u, rk);
     load_params<8>(a.w, a.wdtype, 8 * u, w);
     load_params<8>(a.b, a.wdtype, 8 * u, b);
-    const int steps = (a.rows + a.slots - 1) / a.slots;
-    for (int i = 0; i < steps; i++) {
-        const int64_t row = (int64_t)i * a.slots + slot, at = row * D + 8 * u;
-        const bool in = slot < a.slots && row < a.rows;
-        Raw8<T> ra, rr, rkk, rv, rg;
-        ra.zero(), rr.zero(), rkk.zero(), rv.zero(), rg.zero();
-        if (in) {
-            ra.load(static_cast<const T*>(a.a) + at);
-            rr.load(static_cast<const T*>(a.r) + at);
-            rkk.load(static_cast<const T*>(a.k) + at);
-            rv.load(static_cast<const T*>(a.v) + at);
-            rg.load(static_cast<const T*>(a.g) + at);
-        }
+    using Ring = TailRing<T, 5>;
+    __shared__ Ring ring;
+    const void* const from[5] = {a.a, a.r, a.k, a.v, a.g};
+    const uint32_t rows = slot < a.slots ? a.rows : 0;  // unsigned: a step past 2^31 - 1 rows
+    const int steps = ceil_div(a.rows, a.slots);
+    const int64_t step = a.slots * D;
+    int64_t at = slot * D + 8 * u, next = at;
+    uint32_t fetched = slot;
+    auto fetch = [&](int stage) {
+        const bool in = fetched < rows;
+        ring.fetch(stage, from, in ? next : 0, in);
+        fetched += a.slots;
+        next += step;
+    };
+#pragma unroll
+    for (int i = 0; i < Ring::STAGES - 1; i++) fetch(i);
+    int stage = 0, put = Ring::STAGES - 1;
+    uint32_t row = slot;
+    for (int i = 0; i < steps; i++, row += a.slots, at += step) {
+        fetch(put);
+        copy_wait<Ring::STAGES - 1>();
         float x[8], y[8], c = 0.f, s = 0.f, q = 0.f;
-        rr.floats(x);
-        rkk.floats(y);
+        ring.floats(stage, 1, x);
+        ring.floats(stage, 2, y);
 #pragma unroll
         for (int j = 0; j < 8; j++) c = fmaf(x[j] * y[j], rk[j], c);
-        ra.floats(x);
+        ring.floats(stage, 0, x);
 #pragma unroll
         for (int j = 0; j < 8; j++) s += x[j];
         c = group_sum<L>(c);
@@ -76,13 +109,17 @@ __global__ void __launch_bounds__(TAIL_T) tmix_tail_kernel(const TailArgs a, T* 
             q = fmaf(x[j], x[j], q);
         }
         const float rstd = 1.f / sqrtf(group_sum<L>(q) * inv + a.eps);
-        float v[8], g[8];
-        rv.floats(v);
-        rg.floats(g);
+        ring.floats(stage, 3, y);
 #pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = fmaf(c, v[j], fmaf(x[j] * rstd, w[j], b[j])) * g[j];
-        if (in) store8(out + at, x);
+        for (int j = 0; j < 8; j++) x[j] = fmaf(c, y[j], fmaf(x[j] * rstd, w[j], b[j]));
+        ring.floats(stage, 4, y);
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[j] *= y[j];
+        if (row < rows) store8(out + at, x);
+        put = stage;
+        stage = stage == Ring::STAGES - 1 ? 0 : stage + 1;
     }
+    copy_wait<0>();
 }
 
 template <typename T, int L>
@@ -97,24 +134,32 @@ __global__ void __launch_bounds__(TAIL_T) tmix_tail_backward_kernel(const TailAr
     load_params<8>(a.b, a.wdtype, 8 * u, b);
 #pragma unroll
     for (int j = 0; j < 8; j++) srk[j] = sw[j] = sb[j] = 0.f;
-    const int steps = (a.rows + a.slots - 1) / a.slots;
-    for (int i = 0; i < steps; i++) {
-        const int64_t row = (int64_t)i * a.slots + slot, at = row * D + 8 * u;
-        const bool in = slot < a.slots && row < a.rows;
-        Raw8<T> ra, rr, rkk, rv, rg, rd;
-        ra.zero(), rr.zero(), rkk.zero(), rv.zero(), rg.zero(), rd.zero();
-        if (in) {
-            ra.load(static_cast<const T*>(a.a) + at);
-            rr.load(static_cast<const T*>(a.r) + at);
-            rkk.load(static_cast<const T*>(a.k) + at);
-            rv.load(static_cast<const T*>(a.v) + at);
-            rg.load(static_cast<const T*>(a.g) + at);
-            rd.load(static_cast<const T*>(o.dout) + at);
-        }
+    using Ring = TailRing<T, 6>;
+    __shared__ Ring ring;
+    const void* const from[6] = {a.a, a.r, a.k, a.v, a.g, o.dout};
+    const uint32_t rows = slot < a.slots ? a.rows : 0;  // unsigned: a step past 2^31 - 1 rows
+    const int steps = ceil_div(a.rows, a.slots);
+    const int64_t step = a.slots * D;
+    int64_t at = slot * D + 8 * u, next = at;
+    uint32_t fetched = slot;
+    auto fetch = [&](int stage) {
+        const bool in = fetched < rows;
+        ring.fetch(stage, from, in ? next : 0, in);
+        fetched += a.slots;
+        next += step;
+    };
+#pragma unroll
+    for (int i = 0; i < Ring::STAGES - 1; i++) fetch(i);
+    int stage = 0, put = Ring::STAGES - 1;
+    uint32_t row = slot;
+    for (int i = 0; i < steps; i++, row += a.slots, at += step) {
+        const bool in = row < rows;
+        fetch(put);
+        copy_wait<Ring::STAGES - 1>();
         float r[8], k[8], x[8], v[8], g[8], d[8], c = 0.f, s = 0.f;
-        rr.floats(r);
-        rkk.floats(k);
-        ra.floats(x);
+        ring.floats(stage, 1, r);
+        ring.floats(stage, 2, k);
+        ring.floats(stage, 0, x);
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             c = fmaf(r[j] * k[j], rk[j], c);
@@ -122,9 +167,9 @@ __global__ void __launch_bounds__(TAIL_T) tmix_tail_backward_kernel(const TailAr
         }
         c = group_sum<L>(c);
         const float mean = group_sum<L>(s) * inv;
-        rv.floats(v);
-        rg.floats(g);
-        rd.floats(d);
+        ring.floats(stage, 3, v);
+        ring.floats(stage, 4, g);
+        ring.floats(stage, 5, d);
         // sums over the head: (a - mean)^2, dz v, e, e (a - mean)
         float q = 0.f, dc = 0.f, e1 = 0.f, e2 = 0.f, dz[8];
 #pragma unroll
@@ -168,7 +213,10 @@ __global__ void __launch_bounds__(TAIL_T) tmix_tail_backward_kernel(const TailAr
             srk[j] = fmaf(dc * r[j], k[j], srk[j]);
         }
         if (in) store8(static_cast<T*>(o.dk) + at, t);
+        put = stage;
+        stage = stage == Ring::STAGES - 1 ? 0 : stage + 1;
     }
+    copy_wait<0>();
     if (!o.part || slot >= a.slots) return;
     float* p = o.part + (int64_t)slot * 3 * D + 8 * u;
 #pragma unroll
@@ -189,7 +237,7 @@ int dispatch_head(int S, F&& f) {
     }
 }
 
-constexpr int64_t FWD_THREADS = 148 * 8 * TAIL_T, BWD_THREADS = 148 * 3 * TAIL_T;
+constexpr int64_t FWD_THREADS = 148 * 6 * TAIL_T, BWD_THREADS = 148 * 4 * TAIL_T;
 
 // Slots of a call: enough threads for every SM, at least `least` rows each.
 int plan(int rows, int units, int64_t threads, int least) {

@@ -15,12 +15,14 @@
 #include <algorithm>
 
 #include "ckpt8.cuh"
+#include "copy_async.cuh"
+#include "f32x2.cuh"
 #include "param_join.cuh"
 
 namespace rwkv {
 namespace {
 
-constexpr int MIX_WAYS = 6, MIX_T = 128;
+constexpr int MIX_WAYS = 6, MIX_T = 128, MIX_STAGES = 3;
 
 struct MixArgs {
     const void* x;
@@ -62,143 +64,189 @@ struct Token {
     }
 };
 
-template <typename T, int J>
+// A thread takes U consecutive tokens, their loads first.
+template <typename T, int J, int U>
 __global__ void __launch_bounds__(MIX_T) token_mix_kernel(const MixArgs a, const MixOut o) {
-    constexpr int VE = Vec16<T>::N;
+    constexpr int VE = Vec16<T>::N, P = VE / 2;
     const int64_t id = blockIdx.x * (int64_t)MIX_T + threadIdx.x;
-    const int slot = (int)(id / a.nvec), v = (int)(id - (int64_t)slot * a.nvec);
-    int64_t n = slot * a.chunk;
-    const int64_t end = min(n + a.chunk, a.rows);
-    if (slot >= a.slots || n >= end) return;
-    const uint4* const x = static_cast<const uint4*>(a.x) + v;
+    const int64_t slot = id / a.nvec;
+    const int v = (int)(id - slot * a.nvec);
+    const int64_t first = slot * U;
+    if (first >= a.rows) return;
+    const uint4* const x = static_cast<const uint4*>(a.x) + first * a.nvec + v;
     const uint4* const prev = static_cast<const uint4*>(a.prev) + v;
+    uint4* const last = static_cast<uint4*>(o.last) + v;
     const uint4 zero = make_uint4(0, 0, 0, 0);
-    float m[J][VE];
+    const int n = (int)min((int64_t)U, a.rows - first);
+    Token start, k;
+    start.start(a, first);
+    k = start;
+    uint4 cur[U];  // zeros from a sequence's length on
+    uint4 before = zero;
+    if (start.t == 0) {
+        if (a.prev) before = prev[(int64_t)start.b * a.nvec];
+    } else if (start.t < start.len) {
+        before = x[-a.nvec];
+    }
 #pragma unroll
-    for (int j = 0; j < J; j++) load_params<VE>(a.mix, a.mdtype, ((int64_t)j * a.nvec + v) * VE, m[j]);
-    Token k;
-    k.start(a, n);
-    uint4 before = k.t && k.t < k.len ? x[(n - 1) * a.nvec] : zero;
-    uint4 ahead = k.t < k.len ? x[n * a.nvec] : zero;
-    while (n < end) {
-        const uint4 cur = ahead;
-        const Token here = k;
+    for (int u = 0; u < U; u++) {
+        cur[u] = u < n && k.t < k.len ? x[u * a.nvec] : zero;
         k.next(a);
-        if (n + 1 < end && k.t < k.len) ahead = x[(n + 1) * a.nvec];
-        if (here.t == 0) {
-            before = a.prev ? prev[(int64_t)here.b * a.nvec] : zero;
-            if (here.len == 0) static_cast<uint4*>(o.last)[(int64_t)here.b * a.nvec + v] = before;
-        }
-        if (here.t == here.len - 1) static_cast<uint4*>(o.last)[(int64_t)here.b * a.nvec + v] = cur;
-        float f[VE], d[VE];
-        Vec16<T>::unpack(cur, f);
-        Vec16<T>::unpack(before, d);
+    }
+    float2 m[J][P];
 #pragma unroll
-        for (int i = 0; i < VE; i++) d[i] -= f[i];
+    for (int j = 0; j < J; j++)
+        load_params<VE>(a.mix, a.mdtype, ((int64_t)j * a.nvec + v) * VE, reinterpret_cast<float*>(m[j]));
+    k = start;
+    int64_t at = first * a.nvec + v;
+    const float2 minus = both(-1.f);
+#pragma unroll
+    for (int u = 0; u < U; u++, at += a.nvec, k.next(a)) {
+        if (u >= n) break;
+        if (k.t == 0) {
+            if (u > 0) before = a.prev ? prev[(int64_t)k.b * a.nvec] : zero;
+            if (k.len == 0) last[(int64_t)k.b * a.nvec] = before;
+        }
+        if (k.t == k.len - 1) last[(int64_t)k.b * a.nvec] = cur[u];
+        if (k.t == k.len) before = zero;  // from here on both are zero, and y with them
+        Pairs<T> f, d;
+        f.unpack(cur[u]);
+        d.unpack(before);
+#pragma unroll
+        for (int i = 0; i < P; i++) d[i] = fma2(f[i], minus, d[i]);
 #pragma unroll
         for (int j = 0; j < J; j++) {
-            float y[VE];
+            Pairs<T> y;
 #pragma unroll
-            for (int i = 0; i < VE; i++) y[i] = fmaf(d[i], m[j][i], f[i]);
-            __stcs(static_cast<uint4*>(o.y[j]) + n * a.nvec + v, here.t < here.len ? Vec16<T>::pack(y) : zero);
+            for (int i = 0; i < P; i++) y[i] = fma2(d[i], m[j][i], f[i]);
+            __stcs(static_cast<uint4*>(o.y[j]) + at, y.pack());
         }
-        before = cur;
-        n++;
+        before = cur[u];
     }
 }
 
+// The gradient.  The J + 1 vectors of a token run MIX_STAGES - 1 tokens ahead through
+// a ring in shared memory that is private to the thread (cp.async, no barrier).
 template <typename T, int J>
 __global__ void __launch_bounds__(MIX_T) token_mix_backward_kernel(const MixArgs a, const MixGrad g) {
-    constexpr int VE = Vec16<T>::N;
+    constexpr int VE = Vec16<T>::N, P = VE / 2;
+    __shared__ uint4 ring[MIX_STAGES][J + 1][MIX_T];  // dy_j, x
     const int64_t id = blockIdx.x * (int64_t)MIX_T + threadIdx.x;
     const int slot = (int)(id / a.nvec), v = (int)(id - (int64_t)slot * a.nvec);
-    int64_t n = slot * a.chunk;
-    const int64_t end = min(n + a.chunk, a.rows);
     if (slot >= a.slots) return;
+    const int64_t first = slot * a.chunk, end = min(first + a.chunk, a.rows);
     const uint4* const x = static_cast<const uint4*>(a.x) + v;
     const uint4* const prev = static_cast<const uint4*>(a.prev) + v;
-    const uint4* const dlast = static_cast<const uint4*>(g.dlast) + v;
-    uint4* const dx = static_cast<uint4*>(g.dx) + v;
+    uint4* dx = static_cast<uint4*>(g.dx) + first * a.nvec + v;
     const uint4 zero = make_uint4(0, 0, 0, 0);
-    float m[J][VE], dm[J][VE];
+    float2 nm[J][P], dm[J][P];  // -m_j and dm_j, in pairs
 #pragma unroll
     for (int j = 0; j < J; j++) {
-        load_params<VE>(a.mix, a.mdtype, ((int64_t)j * a.nvec + v) * VE, m[j]);
+        float m[VE];
+        load_params<VE>(a.mix, a.mdtype, ((int64_t)j * a.nvec + v) * VE, m);
 #pragma unroll
-        for (int i = 0; i < VE; i++) dm[j][i] = 0.f;
+        for (int i = 0; i < P; i++) nm[j][i] = make_float2(-m[2 * i], -m[2 * i + 1]), dm[j][i] = make_float2(0.f, 0.f);
     }
-    auto load = [&](int64_t at, const Token& k, uint4* r) {
+    Token k, ahead;
+    k.start(a, first);
+    ahead = k;
+    // the token after the slot's last is read too, for its part in the last one's gradient
+    int64_t left = end - first + 1, at = first * a.nvec;
+    // what is not read is filled with zeros
+    auto fetch = [&](int stage) {
+        const bool real = left > 0 && ahead.t < ahead.len;
 #pragma unroll
-        for (int j = 0; j < J; j++)
-            r[j] = k.t < k.len && g.dy[j] ? __ldcs(static_cast<const uint4*>(g.dy[j]) + at * a.nvec + v) : zero;
+        for (int j = 0; j < J; j++) {
+            const bool read = real && g.dy[j];
+            const uint4* p = static_cast<const uint4*>(g.dy[j]) + v;
+            copy_async_n<16>(&ring[stage][j][threadIdx.x], read ? p + at : x, read ? 16 : 0);
+        }
+        copy_async_n<16>(&ring[stage][J][threadIdx.x], real && left > 1 ? x + at : x, real && left > 1 ? 16 : 0);
+        copy_commit();
+        at += a.nvec;
+        left--;
+        ahead.next(a);
+        if (ahead.b == a.B) left = 0;
     };
-    Token k;
-    k.start(a, n);
-    float before[VE], own[VE];  // x of the token before; the gradient so far of the token before
-    bool open = false;          // whether that is still to be stored
-    if (n < end) {
-        Vec16<T>::unpack(k.t && k.t < k.len ? x[(n - 1) * a.nvec] : zero, before);
-        for (; n < end; n++, k.next(a)) {
-            const bool real = k.t < k.len;
-            uint4 r[J];
-            load(n, k, r);
-            float f[VE], back[VE], rest[VE], d[VE];
-            Vec16<T>::unpack(real ? __ldcs(x + n * a.nvec) : zero, f);
-            if (k.t == 0) Vec16<T>::unpack(real && a.prev ? prev[(int64_t)k.b * a.nvec] : zero, before);
 #pragma unroll
-            for (int i = 0; i < VE; i++) back[i] = rest[i] = 0.f, d[i] = before[i] - f[i];
+    for (int i = 0; i < MIX_STAGES - 1; i++) fetch(i);
+    auto pairs = [](const uint4& r, float2* f) { Vec16<T>::unpack(r, reinterpret_cast<float*>(f)); };
+    auto store = [&](uint4* p, const float2* f) { __stcs(p, Vec16<T>::pack(reinterpret_cast<const float*>(f))); };
+    float2 before[P], own[P];  // x of the token before; its gradient so far
+    pairs(k.t && k.t < k.len ? x[(first - 1) * a.nvec] : zero, before);
+    int stage = 0, put = MIX_STAGES - 1;
+    const float2 minus = make_float2(-1.f, -1.f);
+    for (int64_t n = end - first, i0 = 0;; n--, i0 = 1, k.next(a)) {
+        if (n == 0 && (k.b == a.B || k.t == 0)) break;
+        fetch(put);
+        copy_wait<MIX_STAGES - 1>();
+        float2 back[P], rest[P], f[P], d[P];  // back: -sum m dy
+        if (k.t == 0) pairs(k.len > 0 && a.prev ? prev[(int64_t)k.b * a.nvec] : zero, before);
+        pairs(ring[stage][J][threadIdx.x], f);
+#pragma unroll
+        for (int i = 0; i < P; i++) {
+            back[i] = rest[i] = make_float2(0.f, 0.f);
+            d[i] = fma2(f[i], minus, before[i]);
+        }
+        if (n == 0) {  // the next slot's first token goes on with this sequence
 #pragma unroll
             for (int j = 0; j < J; j++) {
-                float dy[VE];
-                Vec16<T>::unpack(r[j], dy);
+                float2 dy[P];
+                pairs(ring[stage][j][threadIdx.x], dy);
 #pragma unroll
-                for (int i = 0; i < VE; i++) {
-                    back[i] = fmaf(m[j][i], dy[i], back[i]);
-                    rest[i] += fmaf(-m[j][i], dy[i], dy[i]);  // (1 - m) dy, rounded once
-                    dm[j][i] = fmaf(dy[i], real ? d[i] : 0.f, dm[j][i]);
-                }
+                for (int i = 0; i < P; i++) back[i] = fma2(nm[j][i], dy[i], back[i]);
             }
-            if (open) {
-                if (k.t)
 #pragma unroll
-                    for (int i = 0; i < VE; i++) own[i] += back[i];
-                __stcs(dx + (n - 1) * a.nvec, Vec16<T>::pack(own));
-            }
-            if (g.dlast && (k.t == k.len - 1 || (k.t == 0 && k.len == 0))) {
-                float l[VE];
-                Vec16<T>::unpack(dlast[(int64_t)k.b * a.nvec], l);
-#pragma unroll
-                for (int i = 0; i < VE; i++) (k.len ? rest[i] : back[i]) += l[i];
-            }
-            if (k.t == 0 && g.dprev) static_cast<uint4*>(g.dprev)[(int64_t)k.b * a.nvec + v] = Vec16<T>::pack(back);
-#pragma unroll
-            for (int i = 0; i < VE; i++) own[i] = rest[i], before[i] = f[i];
-            open = true;
+            for (int i = 0; i < P; i++) own[i] = fma2(back[i], minus, own[i]);
+            break;
         }
-        if (n < a.rows && k.t) {  // the next slot's first token goes on with this sequence
-            uint4 r[J];
-            load(n, k, r);
-            float back[VE] = {};
 #pragma unroll
-            for (int j = 0; j < J; j++) {
-                float dy[VE];
-                Vec16<T>::unpack(r[j], dy);
+        for (int j = 0; j < J; j++) {
+            float2 dy[P];
+            pairs(ring[stage][j][threadIdx.x], dy);
 #pragma unroll
-                for (int i = 0; i < VE; i++) back[i] = fmaf(m[j][i], dy[i], back[i]);
+            for (int i = 0; i < P; i++) {
+                back[i] = fma2(nm[j][i], dy[i], back[i]);
+                rest[i] = add2(rest[i], fma2(nm[j][i], dy[i], dy[i]));  // (1 - m) dy, rounded once
+                dm[j][i] = fma2(dy[i], d[i], dm[j][i]);
             }
-#pragma unroll
-            for (int i = 0; i < VE; i++) own[i] += back[i];
         }
-        __stcs(dx + (n - 1) * a.nvec, Vec16<T>::pack(own));
+        if (i0) {
+            if (k.t)
+#pragma unroll
+                for (int i = 0; i < P; i++) own[i] = fma2(back[i], minus, own[i]);
+            store(dx, own);
+            dx += a.nvec;
+        }
+        if (k.t == 0 || k.t == k.len - 1) {  // an end of its sequence
+            float2 l[P];
+            const bool last = g.dlast && (k.t == k.len - 1 || k.len == 0);
+            pairs(last ? static_cast<const uint4*>(g.dlast)[(int64_t)k.b * a.nvec + v] : zero, l);
+            if (k.len) {
+#pragma unroll
+                for (int i = 0; i < P; i++) rest[i] = add2(rest[i], l[i]);
+            }
+            if (k.t == 0 && g.dprev) {
+#pragma unroll
+                for (int i = 0; i < P; i++) back[i] = k.len ? mul2(back[i], minus) : l[i];
+                store(static_cast<uint4*>(g.dprev) + (int64_t)k.b * a.nvec + v, back);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < P; i++) own[i] = rest[i], before[i] = f[i];
+        put = stage;
+        stage = stage == MIX_STAGES - 1 ? 0 : stage + 1;
     }
+    store(dx, own);
+    copy_wait<0>();
     if (!g.part) return;
     float* p = g.part + (int64_t)slot * J * a.nvec * VE + (int64_t)v * VE;
 #pragma unroll
     for (int j = 0; j < J; j++)
 #pragma unroll
-        for (int i = 0; i < VE; i += 4)
-            *reinterpret_cast<float4*>(p + (int64_t)j * a.nvec * VE + i) =
-                make_float4(dm[j][i], dm[j][i + 1], dm[j][i + 2], dm[j][i + 3]);
+        for (int i = 0; i < P; i += 2)
+            *reinterpret_cast<float4*>(p + (int64_t)j * a.nvec * VE + 2 * i) =
+                make_float4(dm[j][i].x, dm[j][i].y, dm[j][i + 1].x, dm[j][i + 1].y);
 }
 
 template <typename F>
@@ -213,15 +261,17 @@ int dispatch_ways(int J, F&& f) {
     }
 }
 
-// Slots of a call: enough threads for every SM, at least `least` tokens each.
-void plan(MixArgs& a, int64_t threads, int least) {
+// Slots of a backward call: 256 threads per SM for six ways, more for fewer, so that as
+// many bytes are in flight (57 KB per SM; J = 1, 4096 x 2048 bf16: 16.5 us with 256
+// threads, six ways with 384: 120 us instead of 118 at 16384 x 2560), and four tokens each
+// at least.  Deterministic: by the sizes alone.
+void plan(MixArgs& a, int J) {
+    const int64_t threads = 148 * MIX_T * ((14 + (J + 1) / 2) / (J + 1));
     const int64_t most = std::max<int64_t>(1, threads / a.nvec);
-    const int64_t slots = std::max<int64_t>(1, std::min((a.rows + least - 1) / least, most));
+    const int64_t slots = std::max<int64_t>(1, std::min((a.rows + 3) / 4, most));
     a.chunk = (a.rows + slots - 1) / slots;
     a.slots = (int)((a.rows + a.chunk - 1) / a.chunk);
 }
-constexpr int64_t FWD_THREADS = 148 * 8 * 128, BWD_THREADS = 148 * 2 * 128;
-constexpr int FWD_LEAST = 1, BWD_LEAST = 4;
 
 int vectors(int dtype, int D) { return dtype == RWKV_F32 ? D / 4 : D / 8; }
 
@@ -263,12 +313,19 @@ extern "C" int rwkv_token_mix_forward(int dtype, const void* x, int mdtype, cons
     o.last = last;
     RWKV_REQUIRE(al16(x) && al16(mix) && al16(prev) && al16(last) && ((uintptr_t)lengths & 3) == 0, RWKV_E_UNSUPPORTED,
                  "%s: a tensor is not 16-byte aligned (lengths: 4)", fn);
-    MixArgs a = make_args(dtype, x, mdtype, mix, prev, lengths, B, T, D);
-    plan(a, FWD_THREADS, FWD_LEAST);
+    const MixArgs a = make_args(dtype, x, mdtype, mix, prev, lengths, B, T, D);
     return dispatch_dtype(dtype, [&]<typename T_>() {
         return dispatch_ways(J, [&]<int J_>() {
-            const int64_t threads = (int64_t)a.slots * a.nvec;
-            token_mix_kernel<T_, J_><<<(unsigned)((threads + MIX_T - 1) / MIX_T), MIX_T, 0, (cudaStream_t)stream>>>(a, o);
+            auto launch = [&]<int U>() {
+                const int64_t threads = (a.rows + U - 1) / U * a.nvec;
+                token_mix_kernel<T_, J_, U>
+                    <<<(unsigned)((threads + MIX_T - 1) / MIX_T), MIX_T, 0, (cudaStream_t)stream>>>(a, o);
+            };
+            // Few vectors are spread over threads (16384: 2.9 us, by four tokens 3.5), more
+            // share a token before and the weights (65536: 4.3 and 3.6 us; 16384 x 2560
+            // bf16, six ways: 92 us by four or eight tokens, 97 by two, floor 89).
+            if (a.rows * a.nvec > 1 << 15) launch.template operator()<4>();
+            else launch.template operator()<1>();
             return check_launch("token_mix_kernel");
         });
     });
@@ -277,7 +334,7 @@ extern "C" int rwkv_token_mix_forward(int dtype, const void* x, int mdtype, cons
 extern "C" int64_t rwkv_token_mix_backward_workspace_size(int dtype, int B, int T, int D, int J) {
     if (!valid_dtype(dtype) || B < 1 || T < 1 || D < 8 || D % 8 || D > 1 << 20 || J < 1 || J > MIX_WAYS) return 0;
     MixArgs a = make_args(dtype, nullptr, 0, nullptr, nullptr, nullptr, B, T, D);
-    plan(a, BWD_THREADS, BWD_LEAST);
+    plan(a, J);
     return (int64_t)a.slots * J * D * (int64_t)sizeof(float);
 }
 
@@ -297,7 +354,7 @@ extern "C" int rwkv_token_mix_backward(int dtype, const void* const* dy, const v
                      ((uintptr_t)lengths & 3) == 0,
                  RWKV_E_UNSUPPORTED, "%s: a tensor is not 16-byte aligned (lengths: 4)", fn);
     MixArgs a = make_args(dtype, x, mdtype, mix, prev, lengths, B, T, D);
-    plan(a, BWD_THREADS, BWD_LEAST);
+    plan(a, J);
     g.dlast = dlast;
     g.dx = dx;
     g.dprev = dprev;
