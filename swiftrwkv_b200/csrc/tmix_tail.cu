@@ -36,12 +36,38 @@ struct TailGrad {
     float* part;  // [slots][drk, dw, db][D], or NULL
 };
 
+// The 8 channels of a thread: one 16-byte vector, or of fp32 two, L vectors apart, so
+// that a head's lanes read and write whole sectors (neighbouring vectors: 109 us instead
+// of 66 at 8192 x 2048).
+template <typename T, int L>
+struct Own8 {
+    static constexpr int VE = Vec16<T>::N, W = 8 / VE, STEP = VE * L;
+    // the first one's channel, for unit u of a row
+    static __device__ __forceinline__ int channel(int u) { return u / L * (8 * L) + u % L * VE; }
+    static __device__ __forceinline__ void params(const void* p, int dtype, int c, float* v) {
+#pragma unroll
+        for (int w = 0; w < W; w++) load_params<VE>(p, dtype, c + w * STEP, v + w * VE);
+    }
+    static __device__ __forceinline__ void store(T* p, const float* v) {
+#pragma unroll
+        for (int w = 0; w < W; w++) __stcs(reinterpret_cast<uint4*>(p + w * STEP), Vec16<T>::pack(v + w * VE));
+    }
+    static __device__ __forceinline__ void sums(float* p, const float* v) {
+#pragma unroll
+        for (int w = 0; w < W; w++)
+#pragma unroll
+            for (int k = 0; k < VE; k += 4)
+                *reinterpret_cast<float4*>(p + w * STEP + k) =
+                    make_float4(v[w * VE + k], v[w * VE + k + 1], v[w * VE + k + 2], v[w * VE + k + 3]);
+    }
+};
+
 // The vectors of a row that a thread owns run ahead of their use by a stage or two
 // through a ring in shared memory that is private to the thread (cp.async, no
 // barrier), so that HBM stays busy through a head's sums.
-template <typename T, int N>
+template <typename T, int L, int N>
 struct TailRing {
-    static constexpr int W = Raw8<T>::W, STAGES = sizeof(T) == 2 ? 3 : 2;
+    static constexpr int W = Own8<T, L>::W, STAGES = sizeof(T) == 2 ? 3 : 2;
     uint4 r[STAGES][N * W][TAIL_T];
 
     // N tensors' 8 elements at `at`, or zeros
@@ -51,7 +77,7 @@ struct TailRing {
 #pragma unroll
             for (int w = 0; w < W; w++)
                 copy_async_n<16>(&r[stage][i * W + w][threadIdx.x],
-                                 reinterpret_cast<const uint4*>(static_cast<const T*>(p[i]) + at) + w, in ? 16 : 0);
+                                 static_cast<const T*>(p[i]) + at + w * Own8<T, L>::STEP, in ? 16 : 0);
         copy_commit();
     }
     __device__ __forceinline__ void floats(int stage, int i, float* v) const {
@@ -69,16 +95,18 @@ __global__ void __launch_bounds__(TAIL_T) tmix_tail_kernel(const TailArgs a, T* 
     const int64_t D = 8 * (int64_t)a.units;
     constexpr float inv = 1.f / (8 * L);
     float rk[8], w[8], b[8];
-    load_params<8>(a.rk, a.wdtype, 8 * u, rk);
-    load_params<8>(a.w, a.wdtype, 8 * u, w);
-    load_params<8>(a.b, a.wdtype, 8 * u, b);
-    using Ring = TailRing<T, 5>;
+    using Own = Own8<T, L>;
+    const int first = Own::channel(u);
+    Own::params(a.rk, a.wdtype, first, rk);
+    Own::params(a.w, a.wdtype, first, w);
+    Own::params(a.b, a.wdtype, first, b);
+    using Ring = TailRing<T, L, 5>;
     __shared__ Ring ring;
     const void* const from[5] = {a.a, a.r, a.k, a.v, a.g};
     const uint32_t rows = slot < a.slots ? a.rows : 0;  // unsigned: a step past 2^31 - 1 rows
     const int steps = ceil_div(a.rows, a.slots);
     const int64_t step = a.slots * D;
-    int64_t at = slot * D + 8 * u, next = at;
+    int64_t at = slot * D + first, next = at;
     uint32_t fetched = slot;
     auto fetch = [&](int stage) {
         const bool in = fetched < rows;
@@ -115,7 +143,7 @@ __global__ void __launch_bounds__(TAIL_T) tmix_tail_kernel(const TailArgs a, T* 
         ring.floats(stage, 4, y);
 #pragma unroll
         for (int j = 0; j < 8; j++) x[j] *= y[j];
-        if (row < rows) store8(out + at, x);
+        if (row < rows) Own::store(out + at, x);
         put = stage;
         stage = stage == Ring::STAGES - 1 ? 0 : stage + 1;
     }
@@ -129,18 +157,20 @@ __global__ void __launch_bounds__(TAIL_T) tmix_tail_backward_kernel(const TailAr
     const int64_t D = 8 * (int64_t)a.units;
     constexpr float inv = 1.f / (8 * L);
     float rk[8], w[8], b[8], srk[8], sw[8], sb[8];
-    load_params<8>(a.rk, a.wdtype, 8 * u, rk);
-    load_params<8>(a.w, a.wdtype, 8 * u, w);
-    load_params<8>(a.b, a.wdtype, 8 * u, b);
+    using Own = Own8<T, L>;
+    const int first = Own::channel(u);
+    Own::params(a.rk, a.wdtype, first, rk);
+    Own::params(a.w, a.wdtype, first, w);
+    Own::params(a.b, a.wdtype, first, b);
 #pragma unroll
     for (int j = 0; j < 8; j++) srk[j] = sw[j] = sb[j] = 0.f;
-    using Ring = TailRing<T, 6>;
+    using Ring = TailRing<T, L, 6>;
     __shared__ Ring ring;
     const void* const from[6] = {a.a, a.r, a.k, a.v, a.g, o.dout};
     const uint32_t rows = slot < a.slots ? a.rows : 0;  // unsigned: a step past 2^31 - 1 rows
     const int steps = ceil_div(a.rows, a.slots);
     const int64_t step = a.slots * D;
-    int64_t at = slot * D + 8 * u, next = at;
+    int64_t at = slot * D + first, next = at;
     uint32_t fetched = slot;
     auto fetch = [&](int stage) {
         const bool in = fetched < rows;
@@ -193,38 +223,35 @@ __global__ void __launch_bounds__(TAIL_T) tmix_tail_backward_kernel(const TailAr
             x[j] *= rstd;
             t[j] = d[j] * fmaf(c, v[j], fmaf(x[j], w[j], b[j]));
         }
-        if (in) store8(static_cast<T*>(o.dg) + at, t);
+        if (in) Own::store(static_cast<T*>(o.dg) + at, t);
 #pragma unroll
         for (int j = 0; j < 8; j++) t[j] = rstd * (fmaf(dz[j], w[j], -m1) - x[j] * m2);
-        if (in) store8(static_cast<T*>(o.da) + at, t);
+        if (in) Own::store(static_cast<T*>(o.da) + at, t);
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             sw[j] = fmaf(dz[j], x[j], sw[j]);
             sb[j] += dz[j];
             t[j] = c * dz[j];
         }
-        if (in) store8(static_cast<T*>(o.dv) + at, t);
+        if (in) Own::store(static_cast<T*>(o.dv) + at, t);
 #pragma unroll
         for (int j = 0; j < 8; j++) t[j] = dc * rk[j] * k[j];
-        if (in) store8(static_cast<T*>(o.dr) + at, t);
+        if (in) Own::store(static_cast<T*>(o.dr) + at, t);
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             t[j] = dc * rk[j] * r[j];
             srk[j] = fmaf(dc * r[j], k[j], srk[j]);
         }
-        if (in) store8(static_cast<T*>(o.dk) + at, t);
+        if (in) Own::store(static_cast<T*>(o.dk) + at, t);
         put = stage;
         stage = stage == Ring::STAGES - 1 ? 0 : stage + 1;
     }
     copy_wait<0>();
     if (!o.part || slot >= a.slots) return;
-    float* p = o.part + (int64_t)slot * 3 * D + 8 * u;
-#pragma unroll
-    for (int j = 0; j < 8; j += 4) {
-        *reinterpret_cast<float4*>(p + j) = make_float4(srk[j], srk[j + 1], srk[j + 2], srk[j + 3]);
-        *reinterpret_cast<float4*>(p + D + j) = make_float4(sw[j], sw[j + 1], sw[j + 2], sw[j + 3]);
-        *reinterpret_cast<float4*>(p + 2 * D + j) = make_float4(sb[j], sb[j + 1], sb[j + 2], sb[j + 3]);
-    }
+    float* p = o.part + (int64_t)slot * 3 * D + first;
+    Own::sums(p, srk);
+    Own::sums(p + D, sw);
+    Own::sums(p + 2 * D, sb);
 }
 
 template <typename F>
