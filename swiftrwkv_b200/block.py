@@ -560,13 +560,15 @@ def residualNormBackward(dy, s, weight, mean, rstd, dres=None, scale: float = 1.
 def _mix_args(x, mix, prev, lengths):
     """tokenMix's inputs after their checks."""
     x = _aligned(_some("x", x))
-    if x.dim() != 3:
-        raise ValueError(f"x {tuple(x.shape)} must be [B, T, D]")
-    dev, (B, _, D) = x.device, x.shape
+    shape = x.shape
+    if len(shape) != 3:
+        raise ValueError(f"x {tuple(shape)} must be [B, T, D]")
+    dev, (B, _, D) = x.device, shape
     if not (type(mix) in _TENSORS and mix.dtype is torch.float32 and mix.device == dev and mix.is_contiguous()):
         mix = _tensor("mix", mix, dev)
-    if mix.dim() != 2 or mix.shape[1] != D or not 1 <= mix.shape[0] <= 6:
-        raise ValueError(f"mix {tuple(mix.shape)} must be [J, {D}], J in 1..6")
+    ways = mix.shape
+    if len(ways) != 2 or ways[1] != D or not 1 <= ways[0] <= 6:
+        raise ValueError(f"mix {tuple(ways)} must be [J, {D}], J in 1..6")
     if prev is not None:
         if not _fits(prev, dev, x.dtype, (B, D)):
             prev = _tensor("prev", prev, dev, (x.dtype,), (B, D))
@@ -576,9 +578,18 @@ def _mix_args(x, mix, prev, lengths):
     return x, _aligned(mix), prev, lengths
 
 
+_ADDRESSES = [_lib.P * n for n in range(7)]
+
+
 def _addresses(ts):
     """A host array of the addresses of tensors (None: NULL)."""
-    return (_lib.P * len(ts))(*[_p(t) for t in ts])
+    return _ADDRESSES[len(ts)](*[_p(t) for t in ts])
+
+
+def _steps(t, n):
+    """A host array of the addresses of t[0] .. t[n - 1]."""
+    at, step = t.data_ptr(), t.stride(0) * t.element_size()
+    return _ADDRESSES[n](*range(at, at + n * step, step)) if step else _ADDRESSES[n](*[at] * n)
 
 
 def _token_mix(x, mix, prev, lengths, ys):
@@ -587,7 +598,7 @@ def _token_mix(x, mix, prev, lengths, ys):
     last = x.new_empty(B, D)
     if x.numel():
         _call(x.device, "rwkv_token_mix_forward", _DT[x.dtype], x.data_ptr(), _DT[mix.dtype], mix.data_ptr(), _p(prev),
-              _p(lengths), ys, last.data_ptr(), B, T, D, mix.shape[0])
+              _p(lengths), ys, last.data_ptr(), B, T, D, len(ys))
     elif B:
         last.copy_(prev) if prev is not None else last.zero_()
     return last
@@ -604,8 +615,7 @@ def tokenMixForward(x, mix, prev=None, lengths=None):
     x, mix, prev, lengths = _mix_args(x, mix, prev, lengths)
     J = mix.shape[0]
     y = x.new_empty(J, *x.shape)
-    at, step = y.data_ptr(), x.numel() * x.element_size()
-    return y, _token_mix(x, mix, prev, lengths, (_lib.P * J)(*[at + j * step for j in range(J)]))
+    return y, _token_mix(x, mix, prev, lengths, _steps(y, J))
 
 
 def tokenMixBackward(dys, x, mix, prev=None, lengths=None, dlast=None, params: bool = True):
@@ -618,8 +628,7 @@ def tokenMixBackward(dys, x, mix, prev=None, lengths=None, dlast=None, params: b
     B, T, D = shape
     if isinstance(dys, torch.Tensor):
         dys = _aligned(dys if _fits(dys, dev, dt, (J, *shape)) else _tensor("dys", dys, dev, (dt,), (J, *shape)))
-        at, step = dys.data_ptr(), x.numel() * x.element_size()
-        addresses = (_lib.P * J)(*[at + j * step for j in range(J)])
+        addresses = _steps(dys, J)
     else:
         if not isinstance(dys, (list, tuple)) or len(dys) != J:
             raise ValueError(f"dys: a tensor [{J}, B, T, D] or {J} tensors [B, T, D] are needed")
@@ -644,10 +653,12 @@ def tokenMixBackward(dys, x, mix, prev=None, lengths=None, dlast=None, params: b
 
 # -------------------------------------------------------- tail of the time mix
 
-def _tail_args(rk, weight, bias, tensors):
-    """(inputs, H, S) of tmixTail after their checks; tensors: name, tensor, wkv first."""
-    name, wkv = tensors[0]
-    wkv = _aligned(_some(name, wkv))
+_TAIL = ("wkv", "r", "k", "v", "g", "dout")
+
+
+def _tail_args(rk, weight, bias, *ts):
+    """(inputs, (rk, weight, bias), H, S) of tmixTail after their checks; ts as in _TAIL."""
+    wkv = _some("wkv", ts[0])
     dev, dt, shape = wkv.device, wkv.dtype, wkv.shape
     if not (type(rk) in _TENSORS and rk.dtype is torch.float32 and rk.device == dev and rk.is_contiguous()):
         rk = _tensor("rk", rk, dev)
@@ -657,21 +668,20 @@ def _tail_args(rk, weight, bias, tensors):
     D = H * S
     heads = shape[-2:] == (H, S)
     if not heads and shape[-1] != D:
-        raise ValueError(f"{name} {tuple(shape)} must be [..., {H}, {S}] or [..., {D}]")
+        raise ValueError(f"wkv {tuple(shape)} must be [..., {H}, {S}] or [..., {D}]")
     other = shape[:-2] + (D,) if heads else shape[:-1] + (H, S)
     ins = [wkv]
-    for name, t in tensors[1:]:
-        if not _fits(t, dev, dt, other) and not _fits(t, dev, dt, shape):
-            t = _tensor(name, t, dev, (dt,))
+    for i, t in enumerate(ts[1:], 1):
+        if not _fits(t, dev, dt, shape) and not _fits(t, dev, dt, other):
+            t = _tensor(_TAIL[i], t, dev, (dt,))
             if t.shape != shape and t.shape != other:
-                raise ValueError(f"{name} {tuple(t.shape)} must be {list(shape)} or {list(other)}")
-        ins.append(_aligned(t))
-    ps = [_aligned(rk)]
-    for name, t in (("weight", weight), ("bias", bias)):
-        if not _fits(t, dev, rk.dtype, (D,)):
-            t = _tensor(name, t, dev, (rk.dtype,), (D,))
-        ps.append(_aligned(t))
-    return ins, ps, H, S
+                raise ValueError(f"{_TAIL[i]} {tuple(t.shape)} must be {list(shape)} or {list(other)}")
+        ins.append(t)
+    if not _fits(weight, dev, rk.dtype, (D,)):
+        weight = _tensor("weight", weight, dev, (rk.dtype,), (D,))
+    if not _fits(bias, dev, rk.dtype, (D,)):
+        bias = _tensor("bias", bias, dev, (rk.dtype,), (D,))
+    return [_aligned(t) for t in ins], (_aligned(rk), _aligned(weight), _aligned(bias)), H, S
 
 
 def tmixTailForward(wkv, r, k, v, g, rk, weight, bias, eps: float = 64e-5):
@@ -679,8 +689,7 @@ def tmixTailForward(wkv, r, k, v, g, rk, weight, bias, eps: float = 64e-5):
     ((wkv - mean) rstd weight + bias + (sum r k rk) v) g, in g's shape.  wkv, r, k, v,
     g: [..., H, S] or [..., H S], in one type; rk [H, S], weight and bias [H S], in
     fp32, bf16 or fp16.  The training form of kernel.wkvTail."""
-    (wkv, r, k, v, g), (rk, weight, bias), H, S = _tail_args(
-        rk, weight, bias, (("wkv", wkv), ("r", r), ("k", k), ("v", v), ("g", g)))
+    (wkv, r, k, v, g), (rk, weight, bias), H, S = _tail_args(rk, weight, bias, wkv, r, k, v, g)
     out = torch.empty_like(g)
     n = wkv.numel()
     if n:
@@ -693,8 +702,7 @@ def tmixTailForward(wkv, r, k, v, g, rk, weight, bias, eps: float = 64e-5):
 def tmixTailBackward(dout, wkv, r, k, v, g, rk, weight, bias, eps: float = 64e-5, params: bool = True):
     """(dwkv, dr, dk, dv, dg, drk, dweight, dbias) of tmixTailForward, each in its
     input's shape and type.  Without `params` the last three are None."""
-    (wkv, r, k, v, g, dout), (rk, weight, bias), H, S = _tail_args(
-        rk, weight, bias, (("wkv", wkv), ("r", r), ("k", k), ("v", v), ("g", g), ("dout", dout)))
+    (wkv, r, k, v, g, dout), (rk, weight, bias), H, S = _tail_args(rk, weight, bias, wkv, r, k, v, g, dout)
     grads = [torch.empty_like(t) for t in (wkv, r, k, v, g)]
     pgrads = [torch.empty_like(t) for t in (rk, weight, bias)] if params else [None] * 3
     rows = wkv.numel() // (H * S)

@@ -107,22 +107,23 @@ __device__ __forceinline__ void checkpoint(const Pairs<T>& s, int8_t* codes, uin
     if (first) *exps = (uint8_t)e;
 }
 
-// A block of TPR threads takes R rows, at most NV vectors of a row per thread: vector j
-// of thread t is t + j TPR.
+// TPR threads take R rows, at most NV vectors of a row per thread: vector j of thread t
+// is t + j TPR.  A block is TPR threads, or 128 where a row is a warp's or a part's of one:
+// its statistics then are two sums between lanes.
 //
-// Statistics of a row from one round of sums: each warp takes the mean of its first
+// Otherwise, statistics of a row from one round of sums: each warp takes the mean of its first
 // lane's first vector as a pivot p and leaves p, sum(s - p) and sum (s - p)^2; around the
 // first warp's pivot these join to mean and variance.  The pivot is the mean of VE
 // elements of the row, so that (p - mean)^2 <= M / VE with M the row's centred sum of
 // squares: what cancels in a warp's share of n elements is at most n M / VE, and a fraction of M
 // for rows without outliers.  A constant row gives its value as the mean, exactly.
 template <typename T, int TPR, int NV, int R, bool CK, int MODE>
-__global__ void __launch_bounds__(TPR, 1) rn_fwd_kernel(const __grid_constant__ RnFwdArgs a) {
-    constexpr int VE = Vec16<T>::N, P = VE / 2, NW = TPR / 32;
-    __shared__ alignas(16) float red[R][NW][4];  // pivot, sum, squares of each warp
-    const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
-    const int nvec = a.D / VE, row0 = blockIdx.x * R;
-    const int64_t at = (int64_t)row0 * nvec;  // in vectors
+__global__ void __launch_bounds__(TPR > 32 ? TPR : 128, 1) rn_fwd_kernel(const __grid_constant__ RnFwdArgs a) {
+    constexpr int VE = Vec16<T>::N, P = VE / 2;
+    const int t = threadIdx.x % TPR, lane = threadIdx.x & 31;
+    const int nvec = a.D / VE;
+    const int64_t row0 = (TPR > 32 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * (128 / TPR) + threadIdx.x / TPR) * R;
+    const int64_t at = row0 * nvec;  // in vectors
     const uint4* const x = static_cast<const uint4*>(a.x) + at;
     const uint4* const br = static_cast<const uint4*>(a.branch) + at;
     Pairs<T> s[R][NV];
@@ -153,75 +154,103 @@ __global__ void __launch_bounds__(TPR, 1) rn_fwd_kernel(const __grid_constant__ 
                 if (in) __stcs(static_cast<uint4*>(a.sum) + at + r * nvec + v, s[r][j].pack());
                 if constexpr (CK)
                     checkpoint(s[r][j], a.codes + (at + r * nvec + v) * VE,
-                               a.exps + (int64_t)(row0 + r) * a.G + v / (CK_GROUP / VE), in, lane % (CK_GROUP / VE) == 0);
+                               a.exps + (row0 + r) * a.G + v / (CK_GROUP / VE), in, lane % (CK_GROUP / VE) == 0);
             }
     }
-    float sums[2 * R];
-#pragma unroll
-    for (int r = 0; r < R; r++) {
-        // in halves, so that equal values add exactly
-        const Pairs<T>& f = s[r][0];
-        const float2 h = P == 4 ? add2(add2(f[0], f[1]), add2(f[2 % P], f[3 % P])) : add2(f[0], f[1]);
-        const float pivot = __shfl_sync(0xffffffffu, h.x + h.y, 0) * (1.f / VE);
-        if (lane == 0) red[r][warp][0] = pivot;
-        float2 d1 = both(0.f), d2 = both(0.f);
-#pragma unroll
-        for (int j = 0; j < NV; j++) {
-            const float2 n = both(t + j * TPR < nvec ? -pivot : 0.f);  // zeros beyond the row's end
-#pragma unroll
-            for (int k = 0; k < P; k++) {
-                const float2 d = add2(s[r][j][k], n);
-                d1 = add2(d1, d);
-                d2 = fma2(d, d, d2);
-            }
-        }
-        sums[2 * r] = d1.x + d1.y;
-        sums[2 * r + 1] = d2.x + d2.y;
-    }
-    const float p = lanes_sum<2 * R>(sums, lane);
-    if (lane % (16 / R) == 0) red[lane / (32 / R)][warp][1 + lane / (16 / R) % 2] = p;
-    if constexpr (NW > 1) __syncthreads();
-    else __syncwarp();
     float mean[R], rstd[R];
     const float inv_d = 1.f / (float)a.D;
-    // elements of warp w's share of a row
-    auto count = [&](int w) {
-        int n = 0;
+    if constexpr (TPR <= 32) {
 #pragma unroll
-        for (int j = 0; j < NV; j++) n += max(0, min(32, nvec - w * 32 - j * TPR));
-        return (float)(n * VE);
-    };
+        for (int r = 0; r < R; r++) {
+            float2 sum = both(0.f), q = both(0.f);
+#pragma unroll
+            for (int j = 0; j < NV; j++)
+#pragma unroll
+                for (int k = 0; k < P; k++) sum = add2(sum, s[r][j][k]);
+            mean[r] = group_sum<TPR>(sum.x + sum.y) * inv_d;
+#pragma unroll
+            for (int j = 0; j < NV; j++) {
+                const float2 n = both(t + j * TPR < nvec ? -mean[r] : 0.f);  // zeros beyond the row's end
+#pragma unroll
+                for (int k = 0; k < P; k++) {
+                    const float2 d = add2(s[r][j][k], n);
+                    q = fma2(d, d, q);
+                }
+            }
+            rstd[r] = group_sum<TPR>(q.x + q.y);
+        }
+    } else {
+        constexpr int NW = TPR / 32;
+        __shared__ alignas(16) float red[R][NW][4];  // pivot, sum, squares of each warp
+        const int warp = t >> 5;
+        float sums[2 * R];
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            // in halves, so that equal values add exactly
+            const Pairs<T>& f = s[r][0];
+            const float2 h = P == 4 ? add2(add2(f[0], f[1]), add2(f[2 % P], f[3 % P])) : add2(f[0], f[1]);
+            const float pivot = __shfl_sync(0xffffffffu, h.x + h.y, 0) * (1.f / VE);
+            if (lane == 0) red[r][warp][0] = pivot;
+            float2 d1 = both(0.f), d2 = both(0.f);
+#pragma unroll
+            for (int j = 0; j < NV; j++) {
+                const float2 n = both(t + j * TPR < nvec ? -pivot : 0.f);  // zeros beyond the row's end
+#pragma unroll
+                for (int k = 0; k < P; k++) {
+                    const float2 d = add2(s[r][j][k], n);
+                    d1 = add2(d1, d);
+                    d2 = fma2(d, d, d2);
+                }
+            }
+            sums[2 * r] = d1.x + d1.y;
+            sums[2 * r + 1] = d2.x + d2.y;
+        }
+        const float p = lanes_sum<2 * R>(sums, lane);
+        if (lane % (16 / R) == 0) red[lane / (32 / R)][warp][1 + lane / (16 / R) % 2] = p;
+        __syncthreads();
+        // elements of warp w's share of a row
+        auto count = [&](int w) {
+            int n = 0;
+#pragma unroll
+            for (int j = 0; j < NV; j++) n += max(0, min(32, nvec - w * 32 - j * TPR));
+            return (float)(n * VE);
+        };
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            float u = 0.f, q = 0.f;
+            const float p0 = red[r][0][0];
+            if constexpr (NW <= 5) {  // every thread joins the warps' sums
+                float e[NW], d1[NW], c[NW];
+#pragma unroll
+                for (int w = 0; w < NW; w++) {
+                    const float4 f = *reinterpret_cast<const float4*>(red[r][w]);
+                    e[w] = f.x - p0, d1[w] = f.y, q += f.z, c[w] = count(w);
+                    u += fmaf(c[w], e[w], d1[w]);
+                }
+                u *= inv_d;
+#pragma unroll
+                for (int w = 0; w < NW; w++) {
+                    const float f = e[w] - u;
+                    q = fmaf(f, fmaf(c[w], f, 2.f * d1[w]), q);
+                }
+            } else {  // lane % NW has a warp's
+                const float4 f = *reinterpret_cast<const float4*>(red[r][lane % NW]);
+                const float e = f.x - p0, c = count(lane % NW);
+                u = fmaf(c, e, f.y);
+#pragma unroll
+                for (int m = NW / 2; m > 0; m >>= 1) u += __shfl_xor_sync(0xffffffffu, u, m);
+                u *= inv_d;
+                q = fmaf(e - u, fmaf(c, e - u, 2.f * f.y), f.z);
+#pragma unroll
+                for (int m = NW / 2; m > 0; m >>= 1) q += __shfl_xor_sync(0xffffffffu, q, m);
+            }
+            mean[r] = p0 + u;
+            rstd[r] = q < 0.f ? 0.f : q;  // (a NaN passes)
+        }
+    }
 #pragma unroll
     for (int r = 0; r < R; r++) {
-        float u = 0.f, q = 0.f;
-        const float p0 = red[r][0][0];
-        if constexpr (NW <= 4) {  // every thread joins the warps' sums
-            float e[NW], d1[NW], c[NW];
-#pragma unroll
-            for (int w = 0; w < NW; w++) {
-                const float4 f = *reinterpret_cast<const float4*>(red[r][w]);
-                e[w] = f.x - p0, d1[w] = f.y, q += f.z, c[w] = count(w);
-                u += fmaf(c[w], e[w], d1[w]);
-            }
-            u *= inv_d;
-#pragma unroll
-            for (int w = 0; w < NW; w++) {
-                const float f = e[w] - u;
-                q = fmaf(f, fmaf(c[w], f, 2.f * d1[w]), q);
-            }
-        } else {  // lane % NW has a warp's
-            const float4 f = *reinterpret_cast<const float4*>(red[r][lane % NW]);
-            const float e = f.x - p0, c = count(lane % NW);
-            u = fmaf(c, e, f.y);
-#pragma unroll
-            for (int m = NW / 2; m > 0; m >>= 1) u += __shfl_xor_sync(0xffffffffu, u, m);
-            u *= inv_d;
-            q = fmaf(e - u, fmaf(c, e - u, 2.f * f.y), f.z);
-#pragma unroll
-            for (int m = NW / 2; m > 0; m >>= 1) q += __shfl_xor_sync(0xffffffffu, q, m);
-        }
-        mean[r] = p0 + u;
-        rstd[r] = 1.f / sqrtf((q < 0.f ? 0.f : q) * inv_d + a.eps);  // (a NaN passes)
+        rstd[r] = 1.f / sqrtf(rstd[r] * inv_d + a.eps);
         if (t == 0 && a.mean && row0 + r < a.rows) {
             a.mean[row0 + r] = mean[r];
             a.rstd[row0 + r] = rstd[r];
@@ -414,26 +443,165 @@ __global__ void __launch_bounds__(MAXT, MINB) rn_bwd_kernel(const __grid_constan
     }
 }
 
+// Short rows (at most 32 NV vectors): TPR lanes a row, 128 / TPR rows of a block at a time,
+// the next ones read ahead into registers; no barrier until the columns' sums of a block's
+// rows meet.
+template <typename T, bool CK, int MODE, int TPR, int NV>
+__global__ void __launch_bounds__(128) rn_bwd_short_kernel(const __grid_constant__ RnBwdArgs a) {
+    constexpr int VE = Vec16<T>::N, P = VE / 2;
+    using Codes = std::conditional_t<VE == 8, uint2, uint32_t>;
+    extern __shared__ float2 sums[];  // [warp][dy h | dy][NV][P][TPR]
+    const int t = threadIdx.x % TPR, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int nvec = a.D / VE;
+    const float inv_d = 1.f / (float)a.D;
+    const DropKey key = drop_key<MODE>(a.drop);
+    Pairs<T> w[NV], sw[NV], sb[NV];
+    bool has[NV];
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+        has[j] = t + j * TPR < nvec;
+        load_params<VE>(a.w, a.wdtype, (has[j] ? t + j * TPR : 0) * VE, w[j].floats());
+#pragma unroll
+        for (int k = 0; k < P; k++) sw[j][k] = sb[j][k] = both(0.f);
+    }
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    uint4 ndy[NV], ns[NV], nres[NV];
+    float nmean = 0.f, nrstd = 0.f;
+    uint32_t nex[NV];
+    // what lies beyond a row's or the tensor's end reads as zeros
+    auto fetch = [&](int64_t row) {
+        const bool in = row < a.rows;
+        nmean = in ? a.mean[row] : 0.f;
+        nrstd = in ? a.rstd[row] : 0.f;
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            const int64_t i = row * nvec + t + j * TPR;
+            const bool h = in && has[j];
+            ndy[j] = h ? __ldcs(static_cast<const uint4*>(a.dy) + i) : zero;
+            nres[j] = h && a.dres ? __ldcs(static_cast<const uint4*>(a.dres) + i) : zero;
+            ns[j] = zero;
+            if constexpr (CK) {
+                nex[j] = h ? a.exps[row * a.G + (t + j * TPR) / (CK_GROUP / VE)] : 0u;
+                if (h) *reinterpret_cast<Codes*>(&ns[j]) = __ldcs(reinterpret_cast<const Codes*>(a.codes) + i);
+            } else {
+                if (h) ns[j] = __ldcs(static_cast<const uint4*>(a.s) + i);
+            }
+        }
+    };
+    const int64_t step = (int64_t)gridDim.x * (128 / TPR);
+    int64_t row = (int64_t)blockIdx.x * (128 / TPR) + threadIdx.x / TPR;
+    const int steps = (int)((a.rows + step - 1) / step);  // of every row's lanes alike, for the shuffles
+    fetch(row);
+    for (int n = 0; n < steps; n++, row += step) {
+        const float mean = nmean, rstd = nrstd;
+        uint4 dy[NV], res[NV];
+        Pairs<T> h[NV];
+        float2 s1 = both(0.f), s2 = both(0.f);
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            Pairs<T> d;
+            dy[j] = ndy[j], res[j] = nres[j];
+            d.unpack(dy[j]);
+            if constexpr (CK) {
+                ck_codes4(ns[j].x, h[j].floats());
+                if constexpr (VE == 8) ck_codes4(ns[j].y, h[j].floats() + 4);
+                const float2 scale = both(ck_scale(nex[j]));
+#pragma unroll
+                for (int k = 0; k < P; k++) h[j][k] = fma2(h[j][k], scale, both(-mean));
+            } else {
+                h[j].unpack(ns[j]);
+#pragma unroll
+                for (int k = 0; k < P; k++) h[j][k] = add2(h[j][k], both(-mean));
+            }
+#pragma unroll
+            for (int k = 0; k < P; k++) {  // (dy is 0 beyond the row's end, and adds nothing)
+                h[j][k] = mul2(h[j][k], both(rstd));
+                const float2 g = mul2(d[k], w[j][k]);
+                s1 = add2(s1, g);
+                s2 = fma2(g, h[j][k], s2);
+                sw[j][k] = fma2(d[k], h[j][k], sw[j][k]);
+                sb[j][k] = add2(sb[j][k], d[k]);
+            }
+        }
+        fetch(row + step);
+        const float2 c0 = both(group_sum<TPR>(s1.x + s1.y) * inv_d * -rstd);
+        const float2 c1 = both(group_sum<TPR>(s2.x + s2.y) * inv_d * -rstd);
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            if (!has[j] || row >= a.rows) continue;
+            Pairs<T> d, o;
+            d.unpack(dy[j]);
+            o.unpack(res[j]);
+#pragma unroll
+            for (int k = 0; k < P; k++)
+                o[k] = fma2(mul2(d[k], w[j][k]), both(rstd), fma2(h[j][k], c1, add2(o[k], c0)));
+            const int64_t i = row * nvec + t + j * TPR;
+            __stcs(static_cast<uint4*>(a.dx) + i, o.pack());
+            branch_part<MODE>(o, key, (uint64_t)i, a.drop);
+            __stcs(static_cast<uint4*>(a.dbranch) + i, o.pack());
+        }
+    }
+    if (!a.part) return;
+    // over the warp's rows, then the block's warps, in a fixed order
+#pragma unroll
+    for (int j = 0; j < NV; j++)
+#pragma unroll
+        for (int k = 0; k < P; k++)
+#pragma unroll
+            for (int o = TPR; o < 32; o <<= 1) {
+                const float2 f = make_float2(__shfl_xor_sync(0xffffffffu, sw[j][k].x, o), __shfl_xor_sync(0xffffffffu, sw[j][k].y, o));
+                const float2 g = make_float2(__shfl_xor_sync(0xffffffffu, sb[j][k].x, o), __shfl_xor_sync(0xffffffffu, sb[j][k].y, o));
+                sw[j][k] = add2(sw[j][k], f);
+                sb[j][k] = add2(sb[j][k], g);
+            }
+    constexpr int N = NV * P * TPR;  // pairs of one sum
+    if (lane < TPR) {
+#pragma unroll
+        for (int j = 0; j < NV; j++)
+#pragma unroll
+            for (int k = 0; k < P; k++) {
+                sums[warp * 2 * N + (j * P + k) * TPR + t] = sw[j][k];
+                sums[(warp * 2 + 1) * N + (j * P + k) * TPR + t] = sb[j][k];
+            }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * N; i += 128) {
+        float2 f = sums[i];
+#pragma unroll
+        for (int v = 1; v < 4; v++) f = add2(f, sums[v * 2 * N + i]);
+        const int which = i / N, jk = i % N / TPR, lane_of = i % TPR, v = lane_of + jk / P * TPR;
+        if (v < nvec)
+            *reinterpret_cast<float2*>(a.part + ((int64_t)blockIdx.x * 2 + which) * a.D + v * VE + jk % P * 2) = f;
+    }
+}
+
 // ------------------------------------------------------------------- launches
 
 constexpr int RN_VECTORS = 512 * 3;
-// Blocks of the backward at most (the partial sums of the parameters are as many rows)
-int most_blocks(int D) { return D <= 512 ? 148 * 8 : 148 * 4; }
+// Blocks of the backward at most (the partial sums of the parameters are as many rows):
+// four per SM, more of fewer threads.
+int most_blocks(int D) { return 148 * std::min(8, std::max(4, 8192 / D)); }
 
 template <typename T, int TPR, int NV, int R, bool CK, int MODE>
 void launch_fwd(const RnFwdArgs& a, cudaStream_t st) {
-    rn_fwd_kernel<T, TPR, NV, R, CK, MODE><<<ceil_div(a.rows, R), TPR, 0, st>>>(a);
+    constexpr int BT = TPR > 32 ? TPR : 128;
+    rn_fwd_kernel<T, TPR, NV, R, CK, MODE><<<ceil_div(a.rows, R * (BT / TPR)), BT, 0, st>>>(a);
 }
 
 template <typename T, bool CK, int MODE>
 int forward(const RnFwdArgs& a, cudaStream_t st) {
     const int nvec = a.D / Vec16<T>::N;
-    if (nvec <= 64) launch_fwd<T, 64, 1, 2, CK, MODE>(a, st);
+    if (nvec <= 8) launch_fwd<T, 8, 1, 2, CK, MODE>(a, st);
+    else if (nvec <= 16) launch_fwd<T, 16, 1, 2, CK, MODE>(a, st);
+    else if (nvec <= 32) launch_fwd<T, 32, 1, 2, CK, MODE>(a, st);
+    else if (nvec <= 32 * 2) launch_fwd<T, 32, 2, 2, CK, MODE>(a, st);
+    else if (nvec <= 32 * 3) launch_fwd<T, 32, 3, 1, CK, MODE>(a, st);
     else if (nvec <= 64 * 2) launch_fwd<T, 64, 2, 2, CK, MODE>(a, st);
     else if (nvec <= 64 * 3) launch_fwd<T, 64, 3, 2, CK, MODE>(a, st);
     else if (nvec <= 64 * 4) launch_fwd<T, 64, 4, 1, CK, MODE>(a, st);
-    else if (nvec <= 64 * 5) launch_fwd<T, 64, 5, 1, CK, MODE>(a, st);
+    else if (nvec <= 160 * 2) launch_fwd<T, 160, 2, 1, CK, MODE>(a, st);
     else if (nvec <= 128 * 4) launch_fwd<T, 128, 4, 1, CK, MODE>(a, st);
+    else if (nvec <= 256 * 3) launch_fwd<T, 256, 3, 1, CK, MODE>(a, st);
     else if (nvec <= 256 * 4) launch_fwd<T, 256, 4, 1, CK, MODE>(a, st);
     else launch_fwd<T, 512, 3, 1, CK, MODE>(a, st);
     return check_launch("rn_fwd_kernel");
@@ -454,14 +622,31 @@ cudaError_t launch_bwd(const RnBwdArgs& a, int* blocks, cudaStream_t st) {
     return cudaGetLastError();
 }
 
+template <typename T, bool CK, int MODE, int TPR, int NV>
+cudaError_t launch_short(const RnBwdArgs& a, int* blocks, cudaStream_t st) {
+    // four rows or more for each row's lanes
+    *blocks = std::min(ceil_div(a.rows, 4 * (128 / TPR)), 148 * 4);
+    rn_bwd_short_kernel<T, CK, MODE, TPR, NV>
+        <<<*blocks, 128, 4 * 2 * NV * (Vec16<T>::N / 2) * TPR * sizeof(float2), st>>>(a);
+    return cudaGetLastError();
+}
+
 template <typename T, bool CK, int MODE>
 int backward(const RnBwdArgs& a, void* dw, void* db, cudaStream_t st) {
     const int nvec = a.D / Vec16<T>::N;
+    // rows of a warp up to 96 vectors with dropout (768 channels, 42 M elements bf16: 82 us, of
+    // a block 90; 520 channels 98 and 127), up to 64 without (768: 87 and 75 us)
+    constexpr int SHORT = MODE == DROP_NONE ? 64 : 96;
     int blocks;
-    const cudaError_t e = nvec > 1024  ? launch_bwd<T, CK, MODE, 3, 512, 1>(a, &blocks, st)
-                          : nvec > 512 ? launch_bwd<T, CK, MODE, 2, 512, 1>(a, &blocks, st)
-                          : nvec > 320 ? launch_bwd<T, CK, MODE, 2, 256, 2>(a, &blocks, st)
-                                       : launch_bwd<T, CK, MODE, 2, 160, 3>(a, &blocks, st);
+    const cudaError_t e = nvec > 1024    ? launch_bwd<T, CK, MODE, 3, 512, 1>(a, &blocks, st)
+                          : nvec > 512   ? launch_bwd<T, CK, MODE, 2, 512, 1>(a, &blocks, st)
+                          : nvec > 320   ? launch_bwd<T, CK, MODE, 2, 256, 2>(a, &blocks, st)
+                          : nvec > SHORT ? launch_bwd<T, CK, MODE, 2, 160, 3>(a, &blocks, st)
+                          : nvec > 64    ? launch_short<T, CK, MODE, 32, SHORT / 32>(a, &blocks, st)
+                          : nvec > 32    ? launch_short<T, CK, MODE, 32, 2>(a, &blocks, st)
+                          : nvec > 16    ? launch_short<T, CK, MODE, 32, 1>(a, &blocks, st)
+                          : nvec > 8     ? launch_short<T, CK, MODE, 16, 1>(a, &blocks, st)
+                                         : launch_short<T, CK, MODE, 8, 1>(a, &blocks, st);
     if (e != cudaSuccess) return fail(RWKV_E_CUDA, "rn_bwd_kernel: %s", cudaGetErrorString(e));
     return a.part ? launch_param_join(ParamJoin{a.part, blocks, 2 * (int64_t)a.D, a.D, {dw, db, nullptr}, a.wdtype}, st) : ok();
 }

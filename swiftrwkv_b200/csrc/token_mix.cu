@@ -261,12 +261,11 @@ int dispatch_ways(int J, F&& f) {
     }
 }
 
-// Slots of a backward call: 256 threads per SM for six ways, more for fewer, so that as
-// many bytes are in flight (57 KB per SM; J = 1, 4096 x 2048 bf16: 16.5 us with 256
-// threads, six ways with 384: 120 us instead of 118 at 16384 x 2560), and four tokens each
-// at least.  Deterministic: by the sizes alone.
+// Slots of a backward call: 256 threads per SM for six and five ways, 384 for four, 512 for
+// fewer (more threads than these are slower: 16384 x 2560 bf16, one way, 512 45 us, 896 53; six ways,
+// 256 118 us, 384 121), four tokens each at least.  By the sizes alone: results repeat.
 void plan(MixArgs& a, int J) {
-    const int64_t threads = 148 * MIX_T * ((14 + (J + 1) / 2) / (J + 1));
+    const int64_t threads = 148 * MIX_T * std::min(4, (14 + (J + 1) / 2) / (J + 1));
     const int64_t most = std::max<int64_t>(1, threads / a.nvec);
     const int64_t slots = std::max<int64_t>(1, std::min((a.rows + 3) / 4, most));
     a.chunk = (a.rows + slots - 1) / slots;
