@@ -98,17 +98,18 @@ _BAD_ARGUMENT = (_lib.E_NULL, _lib.E_SHAPE, _lib.E_DTYPE, _lib.E_UNSUPPORTED)
 
 def _call(dev, name, *args):
     """An entry point on `dev` and its current stream (appended)."""
-    L = _lib.lib()
-    k = dev.index
+    fn, k = getattr(_lib.lib(), name), dev.index
     if k == _current_device():
-        st = getattr(L, name)(*args, _raw_stream(k))
+        st = fn(*args, _raw_stream(k))
     else:
         with torch.cuda.device(dev):
-            st = getattr(L, name)(*args, _raw_stream(k))
+            st = fn(*args, _raw_stream(k))
+    if not st:
+        return
+    why = _lib.lib().rwkv_last_error().decode()
     if st in _BAD_ARGUMENT:
-        raise ValueError(L.rwkv_last_error().decode())
-    if st:
-        raise _lib.RWKVError(name, st, L.rwkv_last_error().decode())
+        raise ValueError(why)
+    raise _lib.RWKVError(name, st, why)
 
 
 def _fits(t, dev, dtype, shape):
@@ -476,14 +477,6 @@ def dropoutForward(x, p: float, seed, offset: int = 0):
 
 # ----------------------------------------------------------- residual norm
 
-def _norm_params(weight, bias, dev, D):
-    if not _fits(weight, dev, torch.float32, (D,)):
-        weight = _tensor("weight", weight, dev, None, (D,))
-    if not _fits(bias, dev, weight.dtype, (D,)):
-        bias = _tensor("bias", bias, dev, (weight.dtype,), (D,))
-    return _aligned(weight), _aligned(bias)
-
-
 def residualNormForward(x, branch, weight, bias, eps: float = 1e-5, scale: float = 1.0, p: float = 0.0, seed=0,
                         offset: int = 0, checkpoint: bool = False):
     """s = x + scale dropout(branch) and its layer norm y: (s, y, mean, rstd, ck).
@@ -491,14 +484,20 @@ def residualNormForward(x, branch, weight, bias, eps: float = 1e-5, scale: float
     y, the statistics and ck (the 8-bit checkpoint of s; None without `checkpoint`)
     are those of the sum in fp32, before it is rounded to x's type.  p, seed,
     offset: as in dropoutForward, by the places in branch."""
-    x = _aligned(_some("x", x))
+    x = _some("x", x)
     dev, dt, shape = x.device, x.dtype, x.shape
     D = shape[-1]
     if not _fits(branch, dev, dt, shape):
         branch = _tensor("branch", branch, dev, (dt,), shape)
-    branch = _aligned(branch)
-    weight, bias = _norm_params(weight, bias, dev, D)
+    if not _fits(weight, dev, torch.float32, (D,)):
+        weight = _tensor("weight", weight, dev, None, (D,))
+    if not _fits(bias, dev, weight.dtype, (D,)):
+        bias = _tensor("bias", bias, dev, (weight.dtype,), (D,))
     seed, offset, state = _draw(p, seed, offset, dev)
+    xp, bp, wp, cp = x.data_ptr(), branch.data_ptr(), weight.data_ptr(), bias.data_ptr()
+    if (xp | bp | wp | cp) & 15:
+        x, branch, weight, bias = map(_aligned, (x, branch, weight, bias))
+        xp, bp, wp, cp = x.data_ptr(), branch.data_ptr(), weight.data_ptr(), bias.data_ptr()
     s, y = torch.empty_like(x), torch.empty_like(x)
     mean = x.new_empty(*shape[:-1], dtype=torch.float32) if len(shape) > 1 else x.new_empty((), dtype=torch.float32)
     rstd = torch.empty_like(mean)
@@ -508,9 +507,9 @@ def residualNormForward(x, branch, weight, bias, eps: float = 1e-5, scale: float
         codes, exps = ck.codes.data_ptr(), ck.exps.data_ptr()
     n = x.numel()
     if n:
-        _call(dev, "rwkv_residual_norm_forward", _DT[dt], x.data_ptr(), branch.data_ptr(), _number("scale", scale), p,
-              seed, offset, _p(state), _DT[weight.dtype], weight.data_ptr(), bias.data_ptr(), eps, s.data_ptr(),
-              y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), codes, exps, n // D, D)
+        _call(dev, "rwkv_residual_norm_forward", _DT[dt], xp, bp, _number("scale", scale), p, seed, offset, _p(state),
+              _DT[weight.dtype], wp, cp, eps, s.data_ptr(), y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), codes, exps,
+              n // D, D)
     return s, y, mean, rstd, ck
 
 
@@ -559,7 +558,7 @@ def residualNormBackward(dy, s, weight, mean, rstd, dres=None, scale: float = 1.
 
 def _mix_args(x, mix, prev, lengths):
     """tokenMix's inputs after their checks."""
-    x = _aligned(_some("x", x))
+    x = _some("x", x)
     shape = x.shape
     if len(shape) != 3:
         raise ValueError(f"x {tuple(shape)} must be [B, T, D]")
@@ -572,10 +571,11 @@ def _mix_args(x, mix, prev, lengths):
     if prev is not None:
         if not _fits(prev, dev, x.dtype, (B, D)):
             prev = _tensor("prev", prev, dev, (x.dtype,), (B, D))
-        prev = _aligned(prev)
     if lengths is not None and not _fits(lengths, dev, torch.int32, (B,)):
         lengths = _tensor("lengths", lengths, dev, (torch.int32,), (B,))
-    return x, _aligned(mix), prev, lengths
+    if (x.data_ptr() | mix.data_ptr() | (prev.data_ptr() if prev is not None else 0)) & 15:
+        x, mix, prev = map(_aligned, (x, mix, prev))
+    return x, mix, prev, lengths
 
 
 _ADDRESSES = [_lib.P * n for n in range(7)]
@@ -632,9 +632,12 @@ def tokenMixBackward(dys, x, mix, prev=None, lengths=None, dlast=None, params: b
     else:
         if not isinstance(dys, (list, tuple)) or len(dys) != J:
             raise ValueError(f"dys: a tensor [{J}, B, T, D] or {J} tensors [B, T, D] are needed")
-        dys = [t if t is None else _aligned(t if _fits(t, dev, dt, shape) else _tensor("dys", t, dev, (dt,), shape))
-               for t in dys]
-        addresses = _addresses(dys)
+        dys = [t if t is None or _fits(t, dev, dt, shape) else _tensor("dys", t, dev, (dt,), shape) for t in dys]
+        at = [0 if t is None else t.data_ptr() for t in dys]
+        if any([a & 15 for a in at]):
+            dys = [_aligned(t) for t in dys]
+            at = [0 if t is None else t.data_ptr() for t in dys]
+        addresses = _ADDRESSES[J](*at)
     if dlast is not None:
         dlast = _aligned(dlast if _fits(dlast, dev, dt, (B, D)) else _tensor("dlast", dlast, dev, (dt,), (B, D)))
     dx = torch.empty_like(x)
@@ -657,7 +660,7 @@ _TAIL = ("wkv", "r", "k", "v", "g", "dout")
 
 
 def _tail_args(rk, weight, bias, *ts):
-    """(inputs, (rk, weight, bias), H, S) of tmixTail after their checks; ts as in _TAIL."""
+    """(inputs, parameters, addresses of both, H, S) of tmixTail after their checks; ts as in _TAIL."""
     wkv = _some("wkv", ts[0])
     dev, dt, shape = wkv.device, wkv.dtype, wkv.shape
     if not (type(rk) in _TENSORS and rk.dtype is torch.float32 and rk.device == dev and rk.is_contiguous()):
@@ -681,7 +684,12 @@ def _tail_args(rk, weight, bias, *ts):
         weight = _tensor("weight", weight, dev, (rk.dtype,), (D,))
     if not _fits(bias, dev, rk.dtype, (D,)):
         bias = _tensor("bias", bias, dev, (rk.dtype,), (D,))
-    return [_aligned(t) for t in ins], (_aligned(rk), _aligned(weight), _aligned(bias)), H, S
+    ps = (rk, weight, bias)
+    at = [t.data_ptr() for t in ins], [t.data_ptr() for t in ps]
+    if any([a & 15 for a in at[0] + at[1]]):
+        ins, ps = [_aligned(t) for t in ins], [_aligned(t) for t in ps]
+        at = [t.data_ptr() for t in ins], [t.data_ptr() for t in ps]
+    return ins, ps, at, H, S
 
 
 def tmixTailForward(wkv, r, k, v, g, rk, weight, bias, eps: float = 64e-5):
@@ -689,29 +697,28 @@ def tmixTailForward(wkv, r, k, v, g, rk, weight, bias, eps: float = 64e-5):
     ((wkv - mean) rstd weight + bias + (sum r k rk) v) g, in g's shape.  wkv, r, k, v,
     g: [..., H, S] or [..., H S], in one type; rk [H, S], weight and bias [H S], in
     fp32, bf16 or fp16.  The training form of kernel.wkvTail."""
-    (wkv, r, k, v, g), (rk, weight, bias), H, S = _tail_args(rk, weight, bias, wkv, r, k, v, g)
-    out = torch.empty_like(g)
+    ins, ps, at, H, S = _tail_args(rk, weight, bias, wkv, r, k, v, g)
+    wkv, out = ins[0], torch.empty_like(ins[4])
     n = wkv.numel()
     if n:
-        _call(wkv.device, "rwkv_tmix_tail_forward", _DT[wkv.dtype], wkv.data_ptr(), r.data_ptr(), k.data_ptr(),
-              v.data_ptr(), g.data_ptr(), _DT[rk.dtype], rk.data_ptr(), weight.data_ptr(), bias.data_ptr(), eps,
-              out.data_ptr(), n // (H * S), H, S)
+        _call(wkv.device, "rwkv_tmix_tail_forward", _DT[wkv.dtype], *at[0], _DT[ps[0].dtype], *at[1], eps, out.data_ptr(),
+              n // (H * S), H, S)
     return out
 
 
 def tmixTailBackward(dout, wkv, r, k, v, g, rk, weight, bias, eps: float = 64e-5, params: bool = True):
     """(dwkv, dr, dk, dv, dg, drk, dweight, dbias) of tmixTailForward, each in its
     input's shape and type.  Without `params` the last three are None."""
-    (wkv, r, k, v, g, dout), (rk, weight, bias), H, S = _tail_args(rk, weight, bias, wkv, r, k, v, g, dout)
-    grads = [torch.empty_like(t) for t in (wkv, r, k, v, g)]
-    pgrads = [torch.empty_like(t) for t in (rk, weight, bias)] if params else [None] * 3
+    ins, ps, at, H, S = _tail_args(rk, weight, bias, wkv, r, k, v, g, dout)
+    wkv = ins[0]
+    grads = [torch.empty_like(t) for t in ins[:5]]
+    pgrads = [torch.empty_like(t) for t in ps] if params else [None] * 3
     rows = wkv.numel() // (H * S)
     if not rows:
         return (*grads, *(t if t is None else t.zero_() for t in pgrads))
     n = _workspace_bytes("rwkv_tmix_tail_backward", rows, H, S) if params else 0
     ws = _workspace(n, wkv)
-    _call(wkv.device, "rwkv_tmix_tail_backward", _DT[wkv.dtype], dout.data_ptr(), wkv.data_ptr(), r.data_ptr(),
-          k.data_ptr(), v.data_ptr(), g.data_ptr(), _DT[rk.dtype], rk.data_ptr(), weight.data_ptr(), bias.data_ptr(), eps,
+    _call(wkv.device, "rwkv_tmix_tail_backward", _DT[wkv.dtype], at[0][5], *at[0][:5], _DT[ps[0].dtype], *at[1], eps,
           *[t.data_ptr() for t in grads], *[_p(t) for t in pgrads], rows, H, S, _p(ws), n)
     return (*grads, *pgrads)
 

@@ -107,9 +107,17 @@ __device__ __forceinline__ void checkpoint(const Pairs<T>& s, int8_t* codes, uin
     if (first) *exps = (uint8_t)e;
 }
 
+// the sum of a vector, in halves, so that equal values add exactly
+template <typename T>
+__device__ __forceinline__ float vector_sum(const Pairs<T>& v) {
+    float2 h = add2(v[0], v[1]);
+    if constexpr (Pairs<T>::P == 4) h = add2(h, add2(v[2], v[3]));
+    return h.x + h.y;
+}
+
 // TPR threads take R rows, at most NV vectors of a row per thread: vector j of thread t
 // is t + j TPR.  A block is TPR threads, or 128 where a row is a warp's or a part's of one:
-// its statistics then are two sums between lanes.
+// its statistics then are two sums between lanes, around the mean of the first vector.
 //
 // Otherwise, statistics of a row from one round of sums: each warp takes the mean of its first
 // lane's first vector as a pivot p and leaves p, sum(s - p) and sum (s - p)^2; around the
@@ -162,12 +170,15 @@ __global__ void __launch_bounds__(TPR > 32 ? TPR : 128, 1) rn_fwd_kernel(const _
     if constexpr (TPR <= 32) {
 #pragma unroll
         for (int r = 0; r < R; r++) {
+            const float pivot = __shfl_sync(0xffffffffu, vector_sum(s[r][0]), 0, TPR) * (1.f / VE);
             float2 sum = both(0.f), q = both(0.f);
 #pragma unroll
-            for (int j = 0; j < NV; j++)
+            for (int j = 0; j < NV; j++) {
+                const float2 n = both(t + j * TPR < nvec ? -pivot : 0.f);
 #pragma unroll
-                for (int k = 0; k < P; k++) sum = add2(sum, s[r][j][k]);
-            mean[r] = group_sum<TPR>(sum.x + sum.y) * inv_d;
+                for (int k = 0; k < P; k++) sum = add2(sum, add2(s[r][j][k], n));
+            }
+            mean[r] = pivot + group_sum<TPR>(sum.x + sum.y) * inv_d;
 #pragma unroll
             for (int j = 0; j < NV; j++) {
                 const float2 n = both(t + j * TPR < nvec ? -mean[r] : 0.f);  // zeros beyond the row's end
@@ -186,10 +197,7 @@ __global__ void __launch_bounds__(TPR > 32 ? TPR : 128, 1) rn_fwd_kernel(const _
         float sums[2 * R];
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            // in halves, so that equal values add exactly
-            const Pairs<T>& f = s[r][0];
-            const float2 h = P == 4 ? add2(add2(f[0], f[1]), add2(f[2 % P], f[3 % P])) : add2(f[0], f[1]);
-            const float pivot = __shfl_sync(0xffffffffu, h.x + h.y, 0) * (1.f / VE);
+            const float pivot = __shfl_sync(0xffffffffu, vector_sum(s[r][0]), 0) * (1.f / VE);
             if (lane == 0) red[r][warp][0] = pivot;
             float2 d1 = both(0.f), d2 = both(0.f);
 #pragma unroll

@@ -280,8 +280,8 @@ int check_sizes(int dtype, int mdtype, int B, int T, int D, int J, const char* f
     RWKV_REQUIRE(valid_dtype(dtype) && valid_dtype(mdtype), RWKV_E_DTYPE, "%s: dtypes x=%d mix=%d", fn, dtype, mdtype);
     RWKV_REQUIRE(B >= 1 && T >= 1 && D >= 1 && D <= 1 << 20, RWKV_E_SHAPE, "%s: B=%d T=%d D=%d (B, T >= 1, D in 1..2^20)",
                  fn, B, T, D);
-    RWKV_REQUIRE((int64_t)B * T <= 1ll << 40 && (int64_t)B * T * D <= 1ll << 44, RWKV_E_SHAPE, "%s: B=%d T=%d D=%d", fn,
-                 B, T, D);
+    RWKV_REQUIRE((int64_t)B * T <= (1ll << 40) / D, RWKV_E_SHAPE, "%s: B=%d T=%d D=%d (at most 2^40 elements)",
+                 fn, B, T, D);
     RWKV_REQUIRE(J >= 1 && J <= MIX_WAYS, RWKV_E_SHAPE, "%s: J=%d (1..%d)", fn, J, MIX_WAYS);
     RWKV_REQUIRE(D % 8 == 0, RWKV_E_UNSUPPORTED, "%s: D=%d must be a multiple of 8", fn, D);
     return RWKV_OK;

@@ -126,8 +126,9 @@ def test_dropout_past_32_bits(cuda):
 # -------------------------------------------------------------- residual norm
 
 # on both sides of each length at which the kernels change their threads
-RNORM_SIZES = [(1, 8), (3, 64), (5, 520), (1, 2048), (33, 768), (2, 1032), (4, 1536), (3, 1544), (2, 2056), (7, 2560),
-               (3, 2568), (2, 4104), (5, 6144), (1003, 128)]
+RNORM_SIZES = [(1, 8), (3, 64), (9, 72), (5, 136), (6, 256), (5, 264), (5, 512), (5, 520), (1, 2048), (33, 768), (4, 776),
+               (3, 1024), (2, 1032), (4, 1536), (3, 1544), (2, 2056), (7, 2560), (3, 2568), (2, 4104), (5, 6144), (1003, 128),
+               (700, 40)]
 
 
 def rnorm64(x, branch, w, b, eps, p, seed, scale):
@@ -185,6 +186,32 @@ def test_residual_norm_of_whole_numbers(cuda, dt):
         assert torch.equal(B.checkpoint8Values(ck, dtype=torch.float32).double(), values64(want))
 
 
+@pytest.mark.parametrize("D", [8, 40, 64, 96, 128, 256, 512, 768, 776, 1024, 1536, 2048, 2560, 4096, 6144])
+def test_residual_norm_far_from_zero(cuda, D):
+    """Constant sums give the bias exactly, also at 1000.1 (their mean is exact); a row at
+    1000 with spread 1 keeps the accuracy of the fp32 mean, 1000 2^-24 per rounding, 8 of
+    them, as the layer norm's; an outlier anywhere costs at most the pivot's cancelling."""
+    from swiftrwkv_b200 import block as B
+    x = torch.full((6, D), 1000.1, device="cuda")
+    x[1] = -3.0e-5
+    x[2:4] = 1000.0 + rnd((2, D), 330)
+    x[4:] = rnd((2, D), 331)
+    x[4, 0], x[5, D - 1] = 1e4, -1e4           # an outlier in the pivot's vector, and at the end
+    zero, w, b = torch.zeros_like(x), rnd((D,), 332), rnd((D,), 333)
+    s, y, mean, rstd, _ = B.residualNormForward(x, zero, w, b)
+    assert torch.equal(s, x) and torch.equal(mean[:2], x[:2, 0]) and torch.equal(y[:2], b.expand(2, D))
+    dev = x.double() - x.double().mean(1, keepdim=True)
+    r64 = 1 / torch.sqrt((dev ** 2).mean(1, keepdim=True) + 1e-5)
+    y64 = dev * r64 * w.double() + b.double()
+    tol = 8 * 1000 * U32 * (w.double().abs() * r64 + 1) * (1 + (y64 - b.double()).abs())
+    check(y[2:4], y64[2:4], tol[2:4], "far")
+    # sums of squares that cancel 32-fold at most (7 bits of 24 with the sums' own n 2^-24)
+    n = (D + 16) * U32
+    rel = 32 * n + 8 * U32
+    tol = (w.double() * dev * r64).abs() * rel + w.double().abs() * r64 * n * x.double().abs().mean(1, keepdim=True) + 4 * U32 * (y64.abs() + b.double().abs())
+    check(y[4:], y64[4:], tol[4:], "outlier")
+
+
 @pytest.mark.parametrize("kept_", [False, True])
 @pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("rows,D", RNORM_SIZES)
@@ -229,9 +256,18 @@ def test_residual_norm_backward(cuda, dt, kept_, rows, D):
 
 
 def test_residual_norm_of_more_rows_than_blocks(cuda):
-    test_residual_norm_forward(cuda, "bf16", 3001, 776)
-    test_residual_norm_backward(cuda, "bf16", False, 3001, 776)
-    test_residual_norm_backward(cuda, "f16", True, 2999, 776)
+    for D in (40, 128, 256, 768, 776, 2560):
+        test_residual_norm_forward(cuda, "bf16", 3001, D)
+        test_residual_norm_backward(cuda, "bf16", False, 3001, D)
+        test_residual_norm_backward(cuda, "f16", True, 2999, D)
+    test_residual_norm_backward(cuda, "f32", True, 2999, 384)
+
+
+def test_residual_norm_of_16_bit_rows_past_6144(cuda):
+    for D in (6152, 8200, 12288):
+        test_residual_norm_forward(cuda, "bf16", 5, D)
+        test_residual_norm_backward(cuda, "f16", True, 5, D)
+        test_residual_norm_backward(cuda, "bf16", False, 301, D)
 
 
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
