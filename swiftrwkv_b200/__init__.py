@@ -7,7 +7,8 @@
   and the .rwkvq sb6 / sym formats (``swiftrwkv_b200.quant``).
 * The block operators around them for training and decode: layer norm,
   projections with bias, activation and residual, 8-bit activation
-  checkpoints (``swiftrwkv_b200.block``).
+  checkpoints, token mix, the time mix's tail, residual norm and dropout
+  (``swiftrwkv_b200.block``).
 
 Everything computes in ``librwkvcuda.so`` (hand-written CUDA, C ABI in
 ``include/rwkv_cuda.h``), loaded through ctypes by ``swiftrwkv_b200._lib``.

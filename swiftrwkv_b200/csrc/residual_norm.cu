@@ -115,16 +115,21 @@ __device__ __forceinline__ float vector_sum(const Pairs<T>& v) {
     return h.x + h.y;
 }
 
+// Which of two means a row takes: that of its values, whose sum rounds by the size of
+// the partial sums, or one from the values' distances to a pivot, exact for constant rows
+// and better than the other where the mean is large against the spread.
+__device__ __forceinline__ bool is_far(float mean, float variance) { return variance * 64.f < mean * mean; }
+
 // TPR threads take R rows, at most NV vectors of a row per thread: vector j of thread t
 // is t + j TPR.  A block is TPR threads, or 128 where a row is a warp's or a part's of one:
-// its statistics then are two sums between lanes, around the mean of the first vector.
+// its statistics then are sums between lanes, the pivot the values' mean.
 //
-// Otherwise, statistics of a row from one round of sums: each warp takes the mean of its first
-// lane's first vector as a pivot p and leaves p, sum(s - p) and sum (s - p)^2; around the
-// first warp's pivot these join to mean and variance.  The pivot is the mean of VE
-// elements of the row, so that (p - mean)^2 <= M / VE with M the row's centred sum of
-// squares: what cancels in a warp's share of n elements is at most n M / VE, and a fraction of M
-// for rows without outliers.  A constant row gives its value as the mean, exactly.
+// Otherwise statistics of a row come from one round of sums and one barrier: each warp
+// takes the mean of its first lane's first vector as a pivot p and leaves p, sum(s - p),
+// sum (s - p)^2 and sum(s); around the first warp's pivot these join to mean and variance.
+// A pivot is the mean of VE elements of the row, so that (p - mean)^2 <= M / VE with M the
+// row's centred sum of squares: what cancels in a warp's share of n elements is n M / VE at
+// most, a fraction of M for rows without outliers.
 template <typename T, int TPR, int NV, int R, bool CK, int MODE>
 __global__ void __launch_bounds__(TPR > 32 ? TPR : 128, 1) rn_fwd_kernel(const __grid_constant__ RnFwdArgs a) {
     constexpr int VE = Vec16<T>::N, P = VE / 2;
@@ -170,39 +175,15 @@ __global__ void __launch_bounds__(TPR > 32 ? TPR : 128, 1) rn_fwd_kernel(const _
     if constexpr (TPR <= 32) {
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            const float pivot = __shfl_sync(0xffffffffu, vector_sum(s[r][0]), 0, TPR) * (1.f / VE);
-            float2 sum = both(0.f), q = both(0.f);
+            float2 sum = both(0.f), d1 = both(0.f), d2 = both(0.f);
+#pragma unroll
+            for (int j = 0; j < NV; j++)
+#pragma unroll
+                for (int k = 0; k < P; k++) sum = add2(sum, s[r][j][k]);
+            const float m = group_sum<TPR>(sum.x + sum.y) * inv_d;
 #pragma unroll
             for (int j = 0; j < NV; j++) {
-                const float2 n = both(t + j * TPR < nvec ? -pivot : 0.f);
-#pragma unroll
-                for (int k = 0; k < P; k++) sum = add2(sum, add2(s[r][j][k], n));
-            }
-            mean[r] = pivot + group_sum<TPR>(sum.x + sum.y) * inv_d;
-#pragma unroll
-            for (int j = 0; j < NV; j++) {
-                const float2 n = both(t + j * TPR < nvec ? -mean[r] : 0.f);  // zeros beyond the row's end
-#pragma unroll
-                for (int k = 0; k < P; k++) {
-                    const float2 d = add2(s[r][j][k], n);
-                    q = fma2(d, d, q);
-                }
-            }
-            rstd[r] = group_sum<TPR>(q.x + q.y);
-        }
-    } else {
-        constexpr int NW = TPR / 32;
-        __shared__ alignas(16) float red[R][NW][4];  // pivot, sum, squares of each warp
-        const int warp = t >> 5;
-        float sums[2 * R];
-#pragma unroll
-        for (int r = 0; r < R; r++) {
-            const float pivot = __shfl_sync(0xffffffffu, vector_sum(s[r][0]), 0) * (1.f / VE);
-            if (lane == 0) red[r][warp][0] = pivot;
-            float2 d1 = both(0.f), d2 = both(0.f);
-#pragma unroll
-            for (int j = 0; j < NV; j++) {
-                const float2 n = both(t + j * TPR < nvec ? -pivot : 0.f);  // zeros beyond the row's end
+                const float2 n = both(t + j * TPR < nvec ? -m : 0.f);  // zeros beyond the row's end
 #pragma unroll
                 for (int k = 0; k < P; k++) {
                     const float2 d = add2(s[r][j][k], n);
@@ -210,11 +191,40 @@ __global__ void __launch_bounds__(TPR > 32 ? TPR : 128, 1) rn_fwd_kernel(const _
                     d2 = fma2(d, d, d2);
                 }
             }
-            sums[2 * r] = d1.x + d1.y;
-            sums[2 * r + 1] = d2.x + d2.y;
+            const float u = group_sum<TPR>(d1.x + d1.y) * inv_d, q = group_sum<TPR>(d2.x + d2.y);
+            const bool far = is_far(m, q * inv_d);
+            mean[r] = far ? m + u : m;
+            rstd[r] = far ? fmaxf(q - u * u * (float)a.D, 0.f) : q;
         }
-        const float p = lanes_sum<2 * R>(sums, lane);
-        if (lane % (16 / R) == 0) red[lane / (32 / R)][warp][1 + lane / (16 / R) % 2] = p;
+    } else {
+        constexpr int NW = TPR / 32;
+        __shared__ alignas(16) float red[R][NW][4];  // of each warp: pivot p, sums of s - p, (s - p)^2, s
+        const int warp = t >> 5;
+        float sums[4 * R];
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const float pivot = __shfl_sync(0xffffffffu, vector_sum(s[r][0]), 0) * (1.f / VE);
+            if (lane == 0) red[r][warp][0] = pivot;
+            float2 sum = both(0.f), d1 = both(0.f), d2 = both(0.f);
+#pragma unroll
+            for (int j = 0; j < NV; j++) {
+                const float2 n = both(t + j * TPR < nvec ? -pivot : 0.f);  // zeros beyond the row's end
+#pragma unroll
+                for (int k = 0; k < P; k++) {
+                    const float2 d = add2(s[r][j][k], n);
+                    sum = add2(sum, s[r][j][k]);
+                    d1 = add2(d1, d);
+                    d2 = fma2(d, d, d2);
+                }
+            }
+            sums[4 * r] = 0.f;
+            sums[4 * r + 1] = d1.x + d1.y;
+            sums[4 * r + 2] = d2.x + d2.y;
+            sums[4 * r + 3] = sum.x + sum.y;
+        }
+        const float p = lanes_sum<4 * R>(sums, lane);
+        const int which = lane / (8 / R) % 4;
+        if (lane % (8 / R) == 0 && which) red[lane / (32 / R)][warp][which] = p;
         __syncthreads();
         // elements of warp w's share of a row
         auto count = [&](int w) {
@@ -225,14 +235,14 @@ __global__ void __launch_bounds__(TPR > 32 ? TPR : 128, 1) rn_fwd_kernel(const _
         };
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            float u = 0.f, q = 0.f;
+            float u = 0.f, q = 0.f, sum = 0.f;
             const float p0 = red[r][0][0];
             if constexpr (NW <= 5) {  // every thread joins the warps' sums
                 float e[NW], d1[NW], c[NW];
 #pragma unroll
                 for (int w = 0; w < NW; w++) {
                     const float4 f = *reinterpret_cast<const float4*>(red[r][w]);
-                    e[w] = f.x - p0, d1[w] = f.y, q += f.z, c[w] = count(w);
+                    e[w] = f.x - p0, d1[w] = f.y, q += f.z, sum += f.w, c[w] = count(w);
                     u += fmaf(c[w], e[w], d1[w]);
                 }
                 u *= inv_d;
@@ -245,14 +255,18 @@ __global__ void __launch_bounds__(TPR > 32 ? TPR : 128, 1) rn_fwd_kernel(const _
                 const float4 f = *reinterpret_cast<const float4*>(red[r][lane % NW]);
                 const float e = f.x - p0, c = count(lane % NW);
                 u = fmaf(c, e, f.y);
+                sum = f.w;
 #pragma unroll
-                for (int m = NW / 2; m > 0; m >>= 1) u += __shfl_xor_sync(0xffffffffu, u, m);
+                for (int m = NW / 2; m > 0; m >>= 1) {
+                    u += __shfl_xor_sync(0xffffffffu, u, m);
+                    sum += __shfl_xor_sync(0xffffffffu, sum, m);
+                }
                 u *= inv_d;
                 q = fmaf(e - u, fmaf(c, e - u, 2.f * f.y), f.z);
 #pragma unroll
                 for (int m = NW / 2; m > 0; m >>= 1) q += __shfl_xor_sync(0xffffffffu, q, m);
             }
-            mean[r] = p0 + u;
+            mean[r] = is_far(p0 + u, q * inv_d) ? p0 + u : sum * inv_d;
             rstd[r] = q < 0.f ? 0.f : q;  // (a NaN passes)
         }
     }
@@ -305,8 +319,10 @@ constexpr int RN_STAGES = 3;
 // thread (cp.async); one barrier per row, for its two sums (buffers alternating).
 //
 // 16384 x 2560 bf16: 65 us without dropout, dense or from a checkpoint (floors 64 and 58),
-// 75 and 81 with it.  Bound then by issue: 290 to 315 instructions per vector, 100 of them for the
-// random bits, at 57 % of the slots with the 13 warps per SM that the registers leave.
+// 74 and 81 with it.  Bound then by issue: 280 to 305 instructions per vector, 90 of them for
+// the random bits, at 56 % of the slots with the 13 warps per SM that the registers leave (one
+// vector a thread, 20 warps: 83 with a checkpoint and dropout, 73 dense without; more warps of
+// fewer registers load the weights again and again: 81 to 100).
 template <typename T, bool CK, int MODE, int NV, int MAXT, int MINB>
 __global__ void __launch_bounds__(MAXT, MINB) rn_bwd_kernel(const __grid_constant__ RnBwdArgs a) {
     constexpr int VE = Vec16<T>::N, P = VE / 2;
@@ -587,7 +603,7 @@ __global__ void __launch_bounds__(128) rn_bwd_short_kernel(const __grid_constant
 
 constexpr int RN_VECTORS = 512 * 3;
 // Blocks of the backward at most (the partial sums of the parameters are as many rows):
-// four per SM, more of fewer threads.
+// four per SM, more of fewer threads (40960 x 1024 bf16 with dropout: 74 us, four per SM 89).
 int most_blocks(int D) { return 148 * std::min(8, std::max(4, 8192 / D)); }
 
 template <typename T, int TPR, int NV, int R, bool CK, int MODE>
@@ -599,6 +615,12 @@ void launch_fwd(const RnFwdArgs& a, cudaStream_t st) {
 template <typename T, bool CK, int MODE>
 int forward(const RnFwdArgs& a, cudaStream_t st) {
     const int nvec = a.D / Vec16<T>::N;
+    // As few threads as hold a row in registers: a row's sums and the weights' loads are
+    // shared by more of its vectors.  42 M elements bf16 with dropout (floor 51 us), 64 to
+    // 6144 channels: 52 to 57 us.  On the other sides of these borders: 64 channels by 64
+    // threads a row 389 us, 256 99, 768 by 64 of two vectors 62, 6144 by 256 of four 66.  2560
+    // channels by 64 threads of five and 160 of two: 62 and 60, with a checkpoint 65 and 67,
+    // without dropout 55 and 56 (by a warp of ten 57, 71 with dropout).
     if (nvec <= 8) launch_fwd<T, 8, 1, 2, CK, MODE>(a, st);
     else if (nvec <= 16) launch_fwd<T, 16, 1, 2, CK, MODE>(a, st);
     else if (nvec <= 32) launch_fwd<T, 32, 1, 2, CK, MODE>(a, st);
@@ -607,7 +629,10 @@ int forward(const RnFwdArgs& a, cudaStream_t st) {
     else if (nvec <= 64 * 2) launch_fwd<T, 64, 2, 2, CK, MODE>(a, st);
     else if (nvec <= 64 * 3) launch_fwd<T, 64, 3, 2, CK, MODE>(a, st);
     else if (nvec <= 64 * 4) launch_fwd<T, 64, 4, 1, CK, MODE>(a, st);
-    else if (nvec <= 160 * 2) launch_fwd<T, 160, 2, 1, CK, MODE>(a, st);
+    else if (nvec <= 64 * 5) {
+        if constexpr (MODE != DROP_NONE && !CK) launch_fwd<T, 160, 2, 1, CK, MODE>(a, st);
+        else launch_fwd<T, 64, 5, 1, CK, MODE>(a, st);
+    }
     else if (nvec <= 128 * 4) launch_fwd<T, 128, 4, 1, CK, MODE>(a, st);
     else if (nvec <= 256 * 3) launch_fwd<T, 256, 3, 1, CK, MODE>(a, st);
     else if (nvec <= 256 * 4) launch_fwd<T, 256, 4, 1, CK, MODE>(a, st);

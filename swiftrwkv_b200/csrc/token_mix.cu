@@ -5,13 +5,16 @@
 //   dx[t]  = sum_j (1 - m_j) dy_j[t] + sum_j m_j dy_j[t+1]  (+ dlast at the last token)
 //   dm_j   = sum over tokens of dy_j[t] (x[t-1] - x[t]),  dprev = sum_j m_j dy_j[0]
 //
-// Both are bound by HBM: 1 + J and 2 + J tensors.  A thread owns one 16-byte vector
-// of channels and walks over consecutive tokens of the flattened [B, T], so that a
-// token is read once, the interpolations' weights stay in registers and the
-// gradient of the weights is summed there.  `slots` threads share a vector's tokens;
-// each reads one token beyond its own (the one before in the forward, the one after
-// in the backward).  Tokens from a sequence's length on are not read: they give y =
-// 0 and dx = 0, whatever they and their gradients hold.
+// Both are bound by HBM: 1 + J and 2 + J tensors (16384 x 2560 bf16, six ways: 92 us
+// of a floor of 89 forward, 108 and 4 for the weights' join of 102 backward).  A thread owns
+// one 16-byte vector of channels of consecutive tokens of the flattened [B, T], so that
+// a token is read about once and the interpolations' weights stay in registers.  The
+// forward takes four tokens a thread: what is left to do are stores, and many short
+// threads keep them coming (walks over 110 tokens with x read ahead: 119 us).  The
+// backward walks over as many tokens as there are threads for, since it sums the
+// weights' gradient in registers; each thread reads one token beyond its own, for its part
+// in the last one's gradient.  Tokens from a sequence's length on are not read: they
+// give y = 0 and dx = 0, whatever they and their gradients hold.
 #include <algorithm>
 
 #include "ckpt8.cuh"
@@ -126,7 +129,9 @@ __global__ void __launch_bounds__(MIX_T) token_mix_kernel(const MixArgs a, const
 }
 
 // The gradient.  The J + 1 vectors of a token run MIX_STAGES - 1 tokens ahead through
-// a ring in shared memory that is private to the thread (cp.async, no barrier).
+// a ring in shared memory that is private to the thread (cp.async, no barrier; loads of
+// each token as it is needed: 181 us).  Products and sums in pairs of fp32.  J = 6 in 16
+// bits takes 196 registers, of them 96 for the weights and their gradient.
 template <typename T, int J>
 __global__ void __launch_bounds__(MIX_T) token_mix_backward_kernel(const MixArgs a, const MixGrad g) {
     constexpr int VE = Vec16<T>::N, P = VE / 2;

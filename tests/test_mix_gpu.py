@@ -212,6 +212,18 @@ def test_residual_norm_far_from_zero(cuda, D):
     check(y[4:], y64[4:], tol[4:], "outlier")
 
 
+@pytest.mark.parametrize("D", [64, 256, 512, 768, 1024, 1536, 2048, 2560, 4096, 6144])
+def test_residual_norm_mean_near_zero(cuda, D):
+    """Means much smaller than their rows' values: each of the D additions rounds by at most U32
+    of a partial sum, which for random signs is sqrt(D) at most: in the root mean square over rows
+    below sqrt(D) sqrt(D) U32 / D = U32."""
+    from swiftrwkv_b200 import block as B
+    x = rnd((512, D), 334)
+    _, _, mean, _, _ = B.residualNormForward(x, torch.zeros_like(x), torch.ones(D, device="cuda"), torch.zeros(D, device="cuda"))
+    off = mean.double() - x.double().mean(1)
+    assert float(off.square().mean().sqrt()) < U32
+
+
 @pytest.mark.parametrize("kept_", [False, True])
 @pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("rows,D", RNORM_SIZES)
