@@ -620,7 +620,8 @@ int forward(const RnFwdArgs& a, cudaStream_t st) {
     // 6144 channels: 52 to 57 us.  On the other sides of these borders: 64 channels by 64
     // threads a row 389 us, 256 99, 768 by 64 of two vectors 62, 6144 by 256 of four 66.  2560
     // channels by 64 threads of five and 160 of two: 62 and 60, with a checkpoint 65 and 67,
-    // without dropout 55 and 56 (by a warp of ten 57, 71 with dropout).
+    // without dropout 55 and 56 (by a warp of ten 57, 71 with dropout).  A checkpoint changes
+    // none of them: results are the same with and without.
     if (nvec <= 8) launch_fwd<T, 8, 1, 2, CK, MODE>(a, st);
     else if (nvec <= 16) launch_fwd<T, 16, 1, 2, CK, MODE>(a, st);
     else if (nvec <= 32) launch_fwd<T, 32, 1, 2, CK, MODE>(a, st);
@@ -629,10 +630,7 @@ int forward(const RnFwdArgs& a, cudaStream_t st) {
     else if (nvec <= 64 * 2) launch_fwd<T, 64, 2, 2, CK, MODE>(a, st);
     else if (nvec <= 64 * 3) launch_fwd<T, 64, 3, 2, CK, MODE>(a, st);
     else if (nvec <= 64 * 4) launch_fwd<T, 64, 4, 1, CK, MODE>(a, st);
-    else if (nvec <= 64 * 5) {
-        if constexpr (MODE != DROP_NONE && !CK) launch_fwd<T, 160, 2, 1, CK, MODE>(a, st);
-        else launch_fwd<T, 64, 5, 1, CK, MODE>(a, st);
-    }
+    else if (nvec <= 64 * 5) launch_fwd<T, 64, 5, 1, CK, MODE>(a, st);
     else if (nvec <= 128 * 4) launch_fwd<T, 128, 4, 1, CK, MODE>(a, st);
     else if (nvec <= 256 * 3) launch_fwd<T, 256, 3, 1, CK, MODE>(a, st);
     else if (nvec <= 256 * 4) launch_fwd<T, 256, 4, 1, CK, MODE>(a, st);
