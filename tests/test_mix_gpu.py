@@ -356,6 +356,59 @@ def test_residual_norm_differentiable(cuda, checkpoint):
     assert torch.equal(x1.grad, B.layerNormBackward(dy, s1, w, m1, r1)[0])
 
 
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("D", [40, 128, 256, 512, 776, 2560, 6144])
+def test_residual_norm_seeds_on_the_device(cuda, dt, D):
+    """A seed tensor draws what its values draw, in each of the kernels."""
+    from swiftrwkv_b200 import block as B
+    t = DTYPES[dt]
+    x, br, dy, dres = (rnd((37, D), 590 + i, t) for i in range(4))
+    w, b = rnd((D,), 594), rnd((D,), 595)
+    seed, state = 0xFEDCBA9876543210, torch.tensor([0xFEDCBA9876543210 - 2**64, 2**40], device="cuda")
+    for checkpoint in (False, True):
+        got = [B.residualNormForward(x, br, w, b, p=0.4, seed=s, offset=o, checkpoint=checkpoint)
+               for s, o in ((seed, 2**40 + 3), (state, 3))]
+        assert all(torch.equal(a, c) for a, c in zip(got[0][:4], got[1][:4]))
+        kept_ = got[0][4] if checkpoint else got[0][0]
+        back = [B.residualNormBackward(dy, kept_, w, *got[0][2:4], dres, 0.5, 0.4, s, o) for s, o in ((seed, 2**40 + 3), (state, 3))]
+        assert all(torch.equal(a, c) for a, c in zip(*back))
+        assert torch.equal(back[0][1] == 0, ~mask(dy.shape, 0.4, seed, 2**40 + 3))
+
+
+def test_calls_of_two_lengths_on_two_threads(cuda):
+    """A kernel's shared-memory limit does not follow the call's length."""
+    import threading
+    from swiftrwkv_b200 import block as B
+    wrong = []
+
+    def work(D, seed):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            x, dy = rnd((64, D), seed, torch.bfloat16), rnd((64, D), seed + 1, torch.bfloat16)
+            w, b = torch.ones(D, device="cuda"), torch.zeros(D, device="cuda")
+            first = None
+            for _ in range(60):
+                v, _, mean, rstd, _ = B.residualNormForward(x, dy, w, b, p=0.1, seed=seed)
+                got = B.residualNormBackward(dy, v, w, mean, rstd, p=0.1, seed=seed)
+                if first is None:
+                    first = got
+                elif not all(torch.equal(a, c) for a, c in zip(first, got)):
+                    wrong.append(D)
+        s.synchronize()
+
+    def guarded(*a):
+        try:
+            work(*a)
+        except Exception as e:  # noqa: BLE001
+            wrong.append(e)
+    threads = [threading.Thread(target=guarded, args=a) for a in ((776, 600), (2560, 602))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
 def test_residual_norm_empty_rows_views_and_types(cuda):
     from swiftrwkv_b200 import block as B
     w, b = rnd((64,), 240, torch.float16), rnd((64,), 241, torch.float16)
