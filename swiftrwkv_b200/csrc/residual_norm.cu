@@ -9,7 +9,7 @@
 // HBM's part is 4 tensors forward (x, branch, s, y) and 5 backward (dy, s, dres, dx,
 // dbranch), 1 + 1/32 bytes per element for s as a checkpoint.  s is normed and
 // checkpointed in fp32, before its rounding.  Beside that both are bound by the issue
-// of instructions: a vector of 8 elements takes 16 bytes per tensor, and 75
+// of instructions: a vector of 8 elements takes 16 bytes per tensor, and 70 to 90
 // instructions for its random bits alone, so that the kernels count them: pairs of
 // fp32 in one instruction, several vectors or rows to a thread's share of a row's sums.
 #include <algorithm>
@@ -331,6 +331,7 @@ __global__ void __launch_bounds__(MAXT, MINB) rn_bwd_kernel(const __grid_constan
     using Codes = std::conditional_t<VE == 8, uint2, uint32_t>;  // of one vector
     const int t = threadIdx.x, nt = blockDim.x, warp = t >> 5, lane = t & 31, nw = nt >> 5;
     const int nvec = a.D / VE;
+    pdl_trigger();
     const float inv_d = 1.f / (float)a.D;
     const DropKey key = drop_key<MODE>(a.drop);
     Pairs<T> w[NV], sw[NV], sb[NV];
@@ -477,6 +478,7 @@ __global__ void __launch_bounds__(128) rn_bwd_short_kernel(const __grid_constant
     extern __shared__ float2 sums[];  // [warp][dy h | dy][NV][P][TPR]
     const int t = threadIdx.x % TPR, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int nvec = a.D / VE;
+    pdl_trigger();
     const float inv_d = 1.f / (float)a.D;
     const DropKey key = drop_key<MODE>(a.drop);
     Pairs<T> w[NV], sw[NV], sb[NV];

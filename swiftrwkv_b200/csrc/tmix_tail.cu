@@ -154,6 +154,7 @@ __global__ void __launch_bounds__(TAIL_T) tmix_tail_kernel(const TailArgs a, T* 
 
 template <typename T, int L>
 __global__ void __launch_bounds__(TAIL_T) tmix_tail_backward_kernel(const TailArgs a, const TailGrad o) {
+    pdl_trigger();
     const int64_t id = blockIdx.x * (int64_t)TAIL_T + threadIdx.x;
     const int slot = (int)(id / a.units), u = (int)(id - (int64_t)slot * a.units);
     const int64_t D = 8 * (int64_t)a.units;

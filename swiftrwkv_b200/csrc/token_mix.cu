@@ -136,6 +136,7 @@ template <typename T, int J>
 __global__ void __launch_bounds__(MIX_T) token_mix_backward_kernel(const MixArgs a, const MixGrad g) {
     constexpr int VE = Vec16<T>::N, P = VE / 2;
     __shared__ uint4 ring[MIX_STAGES][J + 1][MIX_T];  // dy_j, x
+    pdl_trigger();
     const int64_t id = blockIdx.x * (int64_t)MIX_T + threadIdx.x;
     const int slot = (int)(id / a.nvec), v = (int)(id - (int64_t)slot * a.nvec);
     if (slot >= a.slots) return;
