@@ -2,8 +2,7 @@
 // elsewhere; its gradient is the same call on dy.  One pass over memory: a thread
 // takes DU blocks of 8 elements DT apart, all loads first, and draws a block's bits
 // while they arrive.  16384 x 8192 bf16: 80 us (a copy: 82), 101 instructions per block of 8
-// elements, 58 of them for its bits; one or two blocks a thread 87 and 90 us.  In long
-// runs the products draw power, and the clock falls: 90 us.
+// elements, 58 of them for its bits; one or two blocks a thread 87 and 90 us.
 #include "ckpt8.cuh"
 #include "philox.cuh"
 

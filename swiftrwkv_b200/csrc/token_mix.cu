@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(MIX_T) token_mix_kernel(const MixArgs a, const
 // The gradient.  The J + 1 vectors of a token run MIX_STAGES - 1 tokens ahead through
 // a ring in shared memory that is private to the thread (cp.async, no barrier; loads of
 // each token as it is needed: 181 us).  Products and sums in pairs of fp32.  J = 6 in 16
-// bits takes 196 registers, of them 96 for the weights and their gradient.
+// bits takes 180 registers, of them 96 for the weights and their gradient.
 template <typename T, int J>
 __global__ void __launch_bounds__(MIX_T) token_mix_backward_kernel(const MixArgs a, const MixGrad g) {
     constexpr int VE = Vec16<T>::N, P = VE / 2;
