@@ -526,6 +526,7 @@ __global__ void __launch_bounds__(128) rn_bwd_short_kernel(const __grid_constant
 #pragma unroll
         for (int j = 0; j < NV; j++) {
             Pairs<T> d;
+            const float sub = has[j] ? -mean : 0.f;  // h is 0 beyond the row's end: no -mean rstd that overflows
             dy[j] = ndy[j], res[j] = nres[j];
             d.unpack(dy[j]);
             if constexpr (CK) {
@@ -533,11 +534,11 @@ __global__ void __launch_bounds__(128) rn_bwd_short_kernel(const __grid_constant
                 if constexpr (VE == 8) ck_codes4(ns[j].y, h[j].floats() + 4);
                 const float2 scale = both(ck_scale(nex[j]));
 #pragma unroll
-                for (int k = 0; k < P; k++) h[j][k] = fma2(h[j][k], scale, both(-mean));
+                for (int k = 0; k < P; k++) h[j][k] = fma2(h[j][k], scale, both(sub));
             } else {
                 h[j].unpack(ns[j]);
 #pragma unroll
-                for (int k = 0; k < P; k++) h[j][k] = add2(h[j][k], both(-mean));
+                for (int k = 0; k < P; k++) h[j][k] = add2(h[j][k], both(sub));
             }
 #pragma unroll
             for (int k = 0; k < P; k++) {  // (dy is 0 beyond the row's end, and adds nothing)

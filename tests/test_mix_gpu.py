@@ -226,6 +226,33 @@ def test_residual_norm_mean_near_zero(cuda, D):
 
 @pytest.mark.parametrize("kept_", [False, True])
 @pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("D", [8, 40, 72, 136, 264, 520, 776, 2056])
+def test_residual_norm_backward_of_huge_constant_rows(cuda, dt, kept_, D):
+    """Rows of one value, 2^121 (2^13 in fp16), with a rstd of 2^10 (2^118): their h is 0, while
+    mean rstd, which zeros beyond a row's end would give, is beyond fp32.  g rounds
+    once, its sum D times, dx a few times more and once at the store."""
+    from swiftrwkv_b200 import block as B
+    t = DTYPES[dt]
+    top, inv, dy_unit, w_unit = (2.0**13, 2.0**118, 2.0**-14, 2.0**-104) if dt == "f16" else (2.0**121, 2.0**10, 2.0**-10, 1.0)
+    x, w, dy = torch.full((37, D), top, device="cuda", dtype=t), rnd((D,), 335, scale=w_unit), rnd((37, D), 336, t, dy_unit)
+    mean, rstd = torch.full((37,), top, device="cuda"), torch.full((37,), inv, device="cuda")
+    s = x
+    if kept_:
+        assert torch.equal(values64(x), x.double())
+        s = B.residualNormForward(x, torch.zeros_like(x), w, torch.zeros_like(w), checkpoint=True)[4]
+    for p in (0.0, 0.25):
+        dx, dbranch, dw, db = B.residualNormBackward(dy, s, w, mean, rstd, scale=0.5, p=p, seed=9)
+        g = dy.double() * w.double()
+        want = inv * (g - g.mean(1, keepdim=True))
+        tol = inv * (4 * U32 * g.abs() + (D + 16) * U32 * g.abs().mean(1, keepdim=True))
+        check(dx, want, tol + u(t) * want.abs(), p)
+        check(dbranch, drop64(want, p, 9, scale=0.5), tol + (u(t) + 3 * U32) * want.abs(), p)
+        assert not dw.any()
+        check(db, dy.double().sum(0), (37 + 16) * U32 * dy.double().abs().sum(0), p)
+
+
+@pytest.mark.parametrize("kept_", [False, True])
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("rows,D", RNORM_SIZES)
 def test_residual_norm_backward(cuda, dt, kept_, rows, D):
     from swiftrwkv_b200 import block as B
