@@ -669,15 +669,19 @@ def _tail_args(rk, weight, bias, *ts):
         raise ValueError(f"rk {tuple(rk.shape)} must be [H, S]")
     H, S = rk.shape
     D = H * S
-    heads = shape[-2:] == (H, S)
-    if not heads and shape[-1] != D:
+    if shape[-2:] == (H, S):
+        other = shape[:-2] + (D,)
+        # of one head also as [..., 1 token, D]
+        more = shape[:-1] + (H, S) if H == 1 else other
+    elif shape[-1] == D:
+        other = more = shape[:-1] + (H, S)
+    else:
         raise ValueError(f"wkv {tuple(shape)} must be [..., {H}, {S}] or [..., {D}]")
-    other = shape[:-2] + (D,) if heads else shape[:-1] + (H, S)
     ins = [wkv]
     for i, t in enumerate(ts[1:], 1):
         if not _fits(t, dev, dt, shape) and not _fits(t, dev, dt, other):
             t = _tensor(_TAIL[i], t, dev, (dt,))
-            if t.shape != shape and t.shape != other:
+            if t.shape not in (shape, other, more):
                 raise ValueError(f"{_TAIL[i]} {tuple(t.shape)} must be {list(shape)} or {list(other)}")
         ins.append(t)
     if not _fits(weight, dev, rk.dtype, (D,)):

@@ -834,6 +834,21 @@ def test_tail_forms_shapes_and_empty_batches(cuda):
         B.tmixTailForward(ins[0], ins[1], ins[2].float(), *ins[3:])
 
 
+def test_tail_of_one_head_and_one_token(cuda):
+    """[B, 1, S] is a token of [.., H S] and a head of [.., H, S]: the other form of either goes with it."""
+    from swiftrwkv_b200 import block as B
+    ins, dout = tail_inputs(3, 1, 64, torch.float32, torch.float32, 441)
+    out, grads = B.tmixTailForward(*ins), B.tmixTailBackward(dout, *ins)
+    flat, tokens, heads = [[t.view(shape) for t in ins[:5]] for shape in ((3, 64), (3, 1, 64), (3, 1, 1, 64))]
+    for first, others in ((tokens, heads), (tokens, flat), (heads, tokens)):
+        mixed = (*first[:1], *others[1:], *ins[5:])
+        assert torch.equal(B.tmixTailForward(*mixed).view(3, 64), out)
+        got = B.tmixTailBackward(dout.view(others[0].shape), *mixed)
+        assert all(a.shape == m.shape and torch.equal(a.view(c.shape), c) for a, m, c in zip(got, mixed, grads))
+    with pytest.raises(ValueError, match="r "):
+        B.tmixTailForward(flat[0], *heads[1:], *ins[5:])
+
+
 def test_tail_may_write_over_its_inputs(cuda):
     from swiftrwkv_b200 import _lib, block as B
     ins, dout = tail_inputs(1301, 4, 64, torch.bfloat16, torch.float32, 450)
