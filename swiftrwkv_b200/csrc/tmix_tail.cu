@@ -8,7 +8,7 @@
 //   dw = sum_rows dz n, db = sum_rows dz, drk = sum_rows dc r k
 //
 // Both are bound by HBM: 6 and 11 tensors (16384 x 2048 bf16 65 us of a floor of 61;
-// backward, 16384 x 2560, 157 and 5 for the parameters' join of 140).  A thread owns 8
+// backward, 16384 x 2560, 156 and 5 for the parameters' join of 140).  A thread owns 8
 // channels, S / 8 neighbouring lanes a head, whose sums are shuffles between them; nothing
 // crosses a warp.  Threads are laid over [slots, D / 8] and walk over the rows of their slot,
 // so that their channels are fixed: the parameters and the sums of their gradients
