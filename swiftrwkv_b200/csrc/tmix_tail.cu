@@ -218,7 +218,8 @@ __global__ void __launch_bounds__(TAIL_T) tmix_tail_backward_kernel(const TailAr
         q = group_sum<L>(q);
         dc = group_sum<L>(dc);
         const float m1 = group_sum<L>(e1) * inv;
-        const float rstd = 1.f / sqrtf(q * inv + a.eps);
+        // 0 without a row, whose zeros at eps = 0 would make n NaN and with it the sums over rows
+        const float rstd = in ? 1.f / sqrtf(q * inv + a.eps) : 0.f;
         const float m2 = group_sum<L>(e2) * inv * rstd;
         float t[8];
 #pragma unroll

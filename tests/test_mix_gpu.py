@@ -769,6 +769,20 @@ def test_tail(cuda, dt, rows, H, S):
         assert all(torch.equal(a, c) for a, c in zip(bare[:5], got)) and bare[5:] == (None,) * 3
 
 
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,H,S", [(5, 1, 64), (1003, 2, 32), (1003, 40, 64), (37, 3, 128), (14, 2, 256)])
+def test_tail_without_eps(cuda, dt, rows, H, S):
+    """eps = 0 over heads that vary: finite, also where a thread's last step has no row left."""
+    from swiftrwkv_b200 import block as B
+    t = DTYPES[dt]
+    ins, dout = tail_inputs(rows, H, S, t, torch.float32, 405)
+    want, tol = tail64(*ins, 0.0)
+    check(B.tmixTailForward(*ins, 0.0), want, tol + u(t) * (want.abs() + tol), "out")
+    got = B.tmixTailBackward(dout, *ins, 0.0)
+    for i, (x, (want, tol)) in enumerate(zip(got, tail64(*ins, 0.0, dout))):
+        check(x, want.view(x.shape), (tol + u(x.dtype) * (want.abs() + tol)).view(x.shape), i)
+
+
 def test_tail_agrees_with_the_decode_form(cuda):
     """kernel.wkvTail computes the same in fp32: both within the bound."""
     from swiftrwkv_b200 import block as B, kernel as K
