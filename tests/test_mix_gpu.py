@@ -212,6 +212,69 @@ def test_residual_norm_far_from_zero(cuda, D):
     check(y[4:], y64[4:], tol[4:], "outlier")
 
 
+def outlier_rows(D, VE):
+    """Rows of spread 1 with values of 1000 and 30: at the start, in the whole first vectors, in the first
+    vector of each 32 (as far as they are few), and with them at the end."""
+    x = rnd((8, D), 337)
+    heads = torch.arange(D, device="cuda") // VE % 32 == 0
+    x[0, 0] = 1000.0
+    x[1, :4] = 1000.0 + x[1, :4]
+    x[2, :8] = 1000.0 + x[2, :8]
+    x[3, :8] = -30.0
+    x[4] = torch.where(heads, 1000.0 + x[4], x[4])
+    x[5, :8] += torch.tensor([1000.0, -700.0, 300.0, 20.0, 1000.0, 5.0, 400.0, -30.0], device="cuda")
+    x[6, -8:] = 1000.0
+    x[7, 0], x[7, -1] = 1e4, -1e4
+    return x
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("D", [72, 264, 520, 776, 1032, 1280, 1536, 2056, 2560, 4096, 6144])
+def test_residual_norm_of_rows_with_outliers(cuda, dt, D):
+    """The statistics are those of a sum around the mean, wherever the row's outliers are.  A term
+    passes at most 20 additions in its thread, 1 for a pair's halves, 5 in its warp and 4 between
+    warps: a sum of squares is off by 30 U32 (each square 2 U32 by its difference), by at most
+    4 times that where it is taken from another point than the mean; rstd by half of it and 2 roundings
+    in the variance, 2 in the root and the quotient.  The mean: 32 U32 mean|s|."""
+    from swiftrwkv_b200 import block as B
+    t = DTYPES[dt]
+    x = outlier_rows(D, 4 if dt == "f32" else 8).to(t)
+    zero, w, b = torch.zeros_like(x), rnd((D,), 338), rnd((D,), 339)
+    s, y, mean, rstd, _ = B.residualNormForward(x, zero, w, b)
+    assert torch.equal(s, x)
+    s64, w64, b64 = x.double(), w.double(), b.double()
+    m64 = s64.mean(1, keepdim=True)
+    dev = s64 - m64
+    r64 = 1 / torch.sqrt((dev ** 2).mean(1, keepdim=True) + 1e-5)
+    em = 32 * U32 * s64.abs().mean(1, keepdim=True)
+    er = (4 * 32 / 2 + 4) * U32
+    check(mean, m64[:, 0], em[:, 0] + U32 * m64[:, 0].abs(), "mean")
+    check(rstd, r64[:, 0], er * r64[:, 0], "rstd")
+    # where the outliers are at the start and large: no cancelling is left
+    check(rstd[[0, 1, 2, 4]], r64[[0, 1, 2, 4], 0], (32 / 2 + 4) * U32 * r64[[0, 1, 2, 4], 0], "rstd of large outliers")
+    y64 = dev * r64 * w64 + b64
+    tol = w64.abs() * r64 * (em + U32 * dev.abs() + dev.abs() * (er + 4 * U32)) + 2 * U32 * (y64.abs() + b64.abs())
+    check(y, y64, tol + u(t) * (y64.abs() + tol), "y")
+    for i in range(8):  # a row's results are its own, whatever lies beside it
+        alone = B.residualNormForward(x[i], zero[i], w, b, checkpoint=True)
+        assert all(torch.equal(a, c[i]) for a, c in zip(alone, (s, y, mean, rstd)))
+
+
+@pytest.mark.parametrize("D", [776, 1280, 2560, 6144])
+def test_residual_norm_of_the_largest_outliers(cuda, D):
+    """One value of 2^63: its square is within fp32, the sum of the others' squared distances to
+    their vector's mean is not."""
+    from swiftrwkv_b200 import block as B
+    x = rnd((2, D), 346)
+    x[0, 0] = 2.0 ** 63
+    one, zero = torch.ones(D, device="cuda"), torch.zeros(D, device="cuda")
+    _, y, mean, rstd, _ = B.residualNormForward(x, torch.zeros_like(x), one, zero)
+    dev = x.double() - x.double().mean(1, keepdim=True)
+    r64 = 1 / torch.sqrt((dev ** 2).mean(1) + 1e-5)
+    check(rstd[0], r64[0], 20 * U32 * r64[0], "rstd")
+    check(y[0, 0], (dev[0, 0] * r64[0]), 64 * U32 * (dev[0, 0] * r64[0]).abs(), "y")
+
+
 @pytest.mark.parametrize("D", [64, 256, 512, 768, 1024, 1536, 2048, 2560, 4096, 6144])
 def test_residual_norm_mean_near_zero(cuda, D):
     """Means much smaller than their rows' values: each of the D additions rounds by at most U32
