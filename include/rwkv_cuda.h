@@ -658,8 +658,8 @@ int rwkv_residual_norm_backward(int dtype, const void* dy, const void* sum, cons
  * x[b, -1] = prev[b] ([B, D] in dtype; NULL: 0).  mix: [J, D] in mdtype; y: HOST array
  * of J device pointers to [B, T, D]; last [B, D]: each sequence's last token, what
  * the next call takes as prev.  lengths: device int32 [B] (4-byte aligned; NULL: all T),
- * taken as 0..T: from a sequence's length on, x is not read and y is 0, and an empty
- * sequence's last is its prev.  D % 8 == 0, D <= 2^20, at most 2^40 elements.  Stands for the token shift
+ * taken as 0..T: from a sequence's length on, x is not read and y is 0 (whatever mix
+ * holds), and an empty sequence's last is its prev.  D % 8 == 0, D <= 2^20, at most 2^40 elements.  Stands for the token shift
  * and lerp of tmix and cmix (RWKVBlock.swift:163-307). */
 int rwkv_token_mix_forward(int dtype, const void* x, int mdtype, const void* mix, const void* prev,
                            const int32_t* lengths, void* const* y, void* last, int B, int T, int D, int J,

@@ -111,7 +111,11 @@ __global__ void __launch_bounds__(MIX_T) token_mix_kernel(const MixArgs a, const
             if (k.len == 0) last[(int64_t)k.b * a.nvec] = before;
         }
         if (k.t == k.len - 1) last[(int64_t)k.b * a.nvec] = cur[u];
-        if (k.t == k.len) before = zero;  // from here on both are zero, and y with them
+        if (k.t >= k.len) {  // zeros whatever the weights hold
+#pragma unroll
+            for (int j = 0; j < J; j++) __stcs(static_cast<uint4*>(o.y[j]) + at, zero);
+            continue;
+        }
         Pairs<T> f, d;
         f.unpack(cur[u]);
         d.unpack(before);
@@ -194,7 +198,9 @@ __global__ void __launch_bounds__(MIX_T) token_mix_backward_kernel(const MixArgs
             back[i] = rest[i] = make_float2(0.f, 0.f);
             d[i] = fma2(f[i], minus, before[i]);
         }
+        const bool real = k.t < k.len;  // no products of what is not, which infinite weights or x would make NaN
         if (n == 0) {  // the next slot's first token goes on with this sequence
+            if (!real) break;
 #pragma unroll
             for (int j = 0; j < J; j++) {
                 float2 dy[P];
@@ -206,15 +212,17 @@ __global__ void __launch_bounds__(MIX_T) token_mix_backward_kernel(const MixArgs
             for (int i = 0; i < P; i++) own[i] = fma2(back[i], minus, own[i]);
             break;
         }
+        if (real) {
 #pragma unroll
-        for (int j = 0; j < J; j++) {
-            float2 dy[P];
-            pairs(ring[stage][j][threadIdx.x], dy);
+            for (int j = 0; j < J; j++) {
+                float2 dy[P];
+                pairs(ring[stage][j][threadIdx.x], dy);
 #pragma unroll
-            for (int i = 0; i < P; i++) {
-                back[i] = fma2(nm[j][i], dy[i], back[i]);
-                rest[i] = add2(rest[i], fma2(nm[j][i], dy[i], dy[i]));  // (1 - m) dy, rounded once
-                dm[j][i] = fma2(dy[i], d[i], dm[j][i]);
+                for (int i = 0; i < P; i++) {
+                    back[i] = fma2(nm[j][i], dy[i], back[i]);
+                    rest[i] = add2(rest[i], fma2(nm[j][i], dy[i], dy[i]));  // (1 - m) dy, rounded once
+                    dm[j][i] = fma2(dy[i], d[i], dm[j][i]);
+                }
             }
         }
         if (i0) {

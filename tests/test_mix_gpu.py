@@ -639,6 +639,39 @@ def test_token_mix(cuda, dt, J, given, ragged):
         assert all(a is c or torch.equal(a, c) for a, c in zip(B.tokenMixBackward(whole, x, mix, prev, n, dlast), again))
 
 
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("J", [1, 2, 6])
+@pytest.mark.parametrize("b,T,D", [(4, 5, 64), (5, 301, 768)])
+def test_token_mix_of_infinities_and_nan_in_padded_batches(cuda, dt, J, b, T, D):
+    """Tokens from a sequence's length on take no part: neither an infinity in its last token nor
+    weights of infinity and NaN make anything of them but zeros."""
+    from swiftrwkv_b200 import block as B
+    t = DTYPES[dt]
+    x, prev, mix = rnd((b, T, D), 353, t), rnd((b, D), 354, t), torch.rand(J, D, generator=torch.Generator(device="cuda").manual_seed(5), device="cuda")
+    n = lengths_of("ragged", b, T, 3)
+    n[3] = 3
+    dys, dlast = [rnd((b, T, D), 355 + j, t).abs() + 1 for j in range(J)], rnd((b, D), 361, t)
+    _, _, before, real = mix64(x, mix, prev, n)
+    # the last token of sequence 3 holds infinities; all weights are finite
+    x[3, 2, :8] = float("inf")
+    dx, dmix, dprev = B.tokenMixBackward(dys, x, mix, prev, n, dlast)
+    want = torch.stack([torch.where(real, dy.double() * (before - x.double()), 0.0).sum((0, 1)) for dy in dys])
+    assert torch.equal(dmix[:, :8], torch.full((J, 8), -float("inf"), device="cuda"))
+    lim = torch.stack([torch.where(real, dy.double() * (before - x.double()), 0.0).abs().sum((0, 1)) for dy in dys])
+    check(dmix[:, 8:], want[:, 8:], (b * T + 16) * U32 * lim[:, 8:], "dmix")
+    assert torch.isfinite(dx).all() and torch.isfinite(dprev).all()
+    x[3, 2, :8] = 1.0
+    mix[:, 0], mix[0, D - 1] = float("inf"), float("nan")
+    y, last = B.tokenMixForward(x, mix, prev, n)
+    assert not y[~real.expand_as(y)].any() and torch.isfinite(last).all()
+    assert torch.isnan(y[0][real[..., 0]][:, D - 1]).all() and torch.isfinite(y[..., 1:D - 1]).all()
+    dx, _, dprev = B.tokenMixBackward(dys, x, mix, prev, n, dlast)
+    assert not dx[~real.expand_as(dx)].any() and torch.isfinite(dx[..., 1:D - 1]).all()
+    assert torch.equal(dprev[0], dlast[0])                # an empty sequence's
+    # no token follows the last one: its gradient is (1 - m) dy and dlast, which the infinite weights turn to -inf
+    assert torch.equal(dx[3, 2, 0], torch.tensor(-float("inf"), device="cuda", dtype=t))
+
+
 def test_token_mix_continues_a_sequence(cuda):
     """Split anywhere, with last as the next part's prev: the whole's results; token by token too."""
     from swiftrwkv_b200 import block as B
