@@ -919,7 +919,9 @@ class _ResidualNorm(torch.autograd.Function):
         if dy is None:
             if ds is None:
                 return (None,) * 10
-            dy = torch.zeros_like(ds)
+            # ds passes as it is: zeros all round, since 0 times what a row or the weights hold may be NaN
+            dy = s = torch.zeros_like(ds, memory_format=torch.contiguous_format)
+            weight, mean, rstd = torch.zeros_like(weight), torch.zeros_like(mean), torch.zeros_like(rstd)
         dx, dbranch, dw, db = residualNormBackward(dy, s, weight, mean, rstd, ds, scale, p, state[0] if state else seed,
                                                    offset, params=need[2] or need[3])
         return (dx, dbranch, dw, db) + (None,) * 6

@@ -446,6 +446,22 @@ def test_residual_norm_differentiable(cuda, checkpoint):
     assert torch.equal(x1.grad, B.layerNormBackward(dy, s1, w, m1, r1)[0])
 
 
+@pytest.mark.parametrize("checkpoint", [False, True])
+@pytest.mark.parametrize("scale,p", [(1.0, 0.0), (0.5, 0.0), (0.5, 0.2)])
+def test_residual_norm_whose_norm_is_not_used(cuda, checkpoint, scale, p):
+    """Without a gradient of y that of s passes as it is, whatever the row and the weights hold."""
+    from swiftrwkv_b200 import block as B
+    x, br, ds = (rnd((6, 96), 348 + i) for i in range(3))
+    w, b = rnd((96,), 351), rnd((96,), 352)
+    x[1, 5], x[3, 7], w[2] = float("inf"), float("nan"), float("inf")
+    leaves = [v.clone().requires_grad_(True) for v in (x, br, w, b)]
+    B.residualNorm(*leaves, scale=scale, p=p, seed=6, checkpoint=checkpoint)[0].backward(ds)
+    want = drop64(ds, p, 6, scale=scale)
+    assert torch.equal(leaves[0].grad, ds)
+    check(leaves[1].grad, want, 4 * U32 * want.abs(), "dbranch")
+    assert not leaves[2].grad.any() and not leaves[3].grad.any()
+
+
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
 @pytest.mark.parametrize("D", [40, 128, 256, 512, 776, 2560, 6144])
 def test_residual_norm_seeds_on_the_device(cuda, dt, D):
