@@ -48,6 +48,7 @@ _HALF = (torch.bfloat16, torch.float16)
 CKPT_GROUP = 32  # channels per scale of a checkpoint
 _MAX = 2**31 - 1
 _MAX_WIDTH = 1 << 20  # of a projection
+_MAX_DROPOUT = 1 << 40  # elements
 
 
 @dataclass
@@ -462,10 +463,17 @@ def dropoutForward(x, p: float, seed, offset: int = 0):
     gradient is the same call on dy.  An element is dropped by its place in x,
     `seed` and `offset` alone (rwkv_cuda.h has the generator), so that every call of a
     program with masks of its own takes another (seed, offset), and the backward pass
-    the forward's.  seed: an integer, or a CUDA tensor int64 [2] that is read when the
-    kernel runs (the seed, and what is added to `offset`): a captured graph then draws
-    anew where the program changes the tensor between replays."""
-    x = _aligned(_some("x", x))
+    the forward's.  x [..., D]: 2^40 elements at most.  seed: an integer, or a CUDA
+    tensor int64 [2] that is read when the kernel runs (the seed, and what is added to
+    `offset`): a captured graph then draws anew where the program changes the tensor
+    between replays."""
+    if isinstance(x, torch.Tensor) and x.numel() > _MAX:  # places alone count, not rows or channels
+        if x.numel() > _MAX_DROPOUT:
+            raise ValueError(f"x {tuple(x.shape)}: more than 2^40 elements")
+        x = _tensor("x", x)
+    else:
+        x = _some("x", x)
+    x = _aligned(x)
     dev = x.device
     seed, offset, state = _draw(p, seed, offset, dev)
     y = torch.empty_like(x)

@@ -123,6 +123,18 @@ def test_dropout_past_32_bits(cuda):
         assert torch.equal(y[row] == 2, want) and torch.equal(y[row] == 0, ~want)
 
 
+def test_dropout_of_flat_tensors_past_31_bits(cuda):
+    """Dropout is by place, whatever the shape: a flat tensor of more than 2^31 - 1 elements is as
+    good as rows; more than 2^40 are refused (nothing is copied)."""
+    from swiftrwkv_b200 import block as B
+    x = torch.ones((1 << 31) + 24, device="cuda", dtype=torch.float16)
+    y = B.dropoutForward(x, 0.5, 78, 1)
+    assert torch.equal(y, B.dropoutForward(x.view(8, -1), 0.5, 78, 1).view(-1))
+    assert torch.equal(B.dropout(x[:1], 0.5, 78, 1), y[:1])
+    with pytest.raises(ValueError, match="2\\^40"):
+        B.dropoutForward(x[:1].expand((1 << 40) + 1), 0.5, 78)
+
+
 # -------------------------------------------------------------- residual norm
 
 # on both sides of each length at which the kernels change their threads
