@@ -34,6 +34,7 @@ The explicit calls take their inputs as values: no gradient or tangent follows.
 """
 from __future__ import annotations
 
+from ctypes import ArgumentError
 from dataclasses import dataclass
 from functools import lru_cache
 
@@ -100,11 +101,14 @@ _BAD_ARGUMENT = (_lib.E_NULL, _lib.E_SHAPE, _lib.E_DTYPE, _lib.E_UNSUPPORTED)
 def _call(dev, name, *args):
     """An entry point on `dev` and its current stream (appended)."""
     fn, k = getattr(_lib.lib(), name), dev.index
-    if k == _current_device():
-        st = fn(*args, _raw_stream(k))
-    else:
-        with torch.cuda.device(dev):
+    try:
+        if k == _current_device():
             st = fn(*args, _raw_stream(k))
+        else:
+            with torch.cuda.device(dev):
+                st = fn(*args, _raw_stream(k))
+    except ArgumentError as e:  # an eps or a scale that is no number or too large for one
+        raise ValueError(f"{name}: {e}") from None
     if not st:
         return
     why = _lib.lib().rwkv_last_error().decode()

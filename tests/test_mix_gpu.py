@@ -1237,6 +1237,19 @@ def test_block_run_and_its_gradients(cuda, B_, T, p):
         assert rel(a, b) < 0.08, (name, rel(a, b))
 
 
+@pytest.mark.parametrize("bad", ["1e-5", None, 10 ** 400, 1 + 0j], ids=["text", "none", "huge", "complex"])
+def test_what_is_no_number_is_refused(cuda, bad):
+    from swiftrwkv_b200 import block as B
+    x, v = rnd((2, 64), 596), torch.ones(64, device="cuda")
+    for f in (lambda: B.layerNormForward(x, v, v, bad), lambda: B.residualNormForward(x, x, v, v, bad),
+              lambda: B.residualNormForward(x, x, v, v, scale=bad), lambda: B.residualNormForward(x, x, v, v, p=bad),
+              lambda: B.residualNormBackward(x, x, v, x[:, 0], x[:, 1], scale=bad),
+              lambda: B.tmixTailForward(x, x, x, x, x, v[None], v, v, bad),
+              lambda: B.tmixTailBackward(x, x, x, x, x, x, v[None], v, v, bad), lambda: B.dropoutForward(x, bad, 1)):
+        with pytest.raises(ValueError):
+            f()
+
+
 def test_host_tensors_beside_cuda_tensors_are_refused(cuda):
     """Tensors of two devices in one call are a ValueError."""
     from swiftrwkv_b200 import block as B
