@@ -700,6 +700,17 @@ def test_token_mix_of_infinities_and_nan_in_padded_batches(cuda, dt, J, b, T, D)
     assert torch.equal(dx[3, 2, 0], torch.tensor(-float("inf"), device="cuda", dtype=t))
 
 
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("J", [1, 4, 6])
+@pytest.mark.parametrize("given", [False, True])
+@pytest.mark.parametrize("ragged", [None, "ragged"])
+def test_token_mix_of_training_batches(cuda, monkeypatch, dt, J, given, ragged):
+    """Past the size at which a thread of the forward takes four tokens, and where a thread of the
+    backward walks over many, with ends of sequences among them."""
+    monkeypatch.setitem(globals(), "MIX_SIZES", [(9, 301, 2560), (1500, 3, 2048)])
+    test_token_mix(cuda, dt, J, given, ragged)
+
+
 def test_token_mix_continues_a_sequence(cuda):
     """Split anywhere, with last as the next part's prev: the whole's results; token by token too."""
     from swiftrwkv_b200 import block as B
@@ -907,6 +918,13 @@ def test_tail_without_eps(cuda, dt, rows, H, S):
         check(x, want.view(x.shape), (tol + u(x.dtype) * (want.abs() + tol)).view(x.shape), i)
 
 
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,H,S", [(1003, 40, 64), (5003, 20, 32), (2501, 12, 128), (2999, 6, 256)])
+def test_tail_of_several_rows_a_thread(cuda, dt, rows, H, S):
+    """Past 113664 units of 8 channels, a number of rows that does not divide among the threads."""
+    test_tail(cuda, dt, rows, H, S)
+
+
 def test_tail_agrees_with_the_decode_form(cuda):
     """kernel.wkvTail computes the same in fp32: both within the bound."""
     from swiftrwkv_b200 import block as B, kernel as K
@@ -1004,6 +1022,28 @@ def test_tail_may_write_over_its_inputs(cuda):
         ps = [t.data_ptr() for t in c]
         _lib.call("rwkv_tmix_tail_backward", _lib.BF16, d.data_ptr(), *ps[:5], _lib.F32, *ps[5:], 64e-5,
                   *[t.data_ptr() for t in over[:5]], None, None, None, 1301, 4, 64, None, 0, st)
+        assert all(torch.equal(a, b) for a, b in zip(over, grads[:5]))
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_tail_may_write_over_inputs_that_are_read_ahead(cuda, dt):
+    """As above where a thread has several rows, whose later ones are on their way meanwhile."""
+    from swiftrwkv_b200 import _lib, block as B
+    rows, H, S, t = 1003, 40, 64, DTYPES[dt]
+    ins, dout = tail_inputs(rows, H, S, t, torch.float32, 451)
+    st, code = torch.cuda.current_stream().cuda_stream, B._DT[t]
+    out, grads = B.tmixTailForward(*ins), B.tmixTailBackward(dout, *ins)
+    for i in range(5):
+        c = [v.clone() for v in ins]
+        ps = [v.data_ptr() for v in c]
+        _lib.call("rwkv_tmix_tail_forward", code, *ps[:5], _lib.F32, *ps[5:], 64e-5, ps[i], rows, H, S, st)
+        assert torch.equal(c[i], out)
+    for turn in range(6):
+        c, d = [v.clone() for v in ins], dout.clone()
+        over = ([d] + c[:5])[turn:] + ([d] + c[:5])[:turn]
+        ps = [v.data_ptr() for v in c]
+        _lib.call("rwkv_tmix_tail_backward", code, d.data_ptr(), *ps[:5], _lib.F32, *ps[5:], 64e-5,
+                  *[v.data_ptr() for v in over[:5]], None, None, None, rows, H, S, None, 0, st)
         assert all(torch.equal(a, b) for a, b in zip(over, grads[:5]))
 
 
@@ -1259,3 +1299,43 @@ def test_host_tensors_beside_cuda_tensors_are_refused(cuda):
               lambda: B.tokenMixBackward([x.cpu()], x, v[None])):
         with pytest.raises(ValueError, match="CUDA tensor"):
             f()
+
+
+CAPTURE_FIRST = """
+import sys
+sys.path.insert(0, {root!r})
+import torch
+from swiftrwkv_b200 import block as B
+g = torch.Generator(device="cuda").manual_seed(1)
+def calls(dt, D):
+    rnd = lambda *s: torch.randn(s, generator=g, device="cuda").to(dt)
+    x, br, dy, prev, w = rnd(2, 37, D), rnd(2, 37, D), rnd(2, 37, D), rnd(2, D), rnd(D)
+    mix, rk, seed = rnd(6, D), rnd(D // 64, 64), torch.tensor([3, 4], device="cuda")
+    def run():
+        d = B.dropoutForward(br, 0.2, seed, 1)
+        s, y, mean, rstd, ck = B.residualNormForward(x, d, w, w, p=0.1, seed=seed, checkpoint=True)
+        m, last = B.tokenMixForward(y, mix, prev)
+        o = B.tmixTailForward(m[0], m[1], m[2], m[3], m[4], rk, w, w)
+        gs = B.tmixTailBackward(dy, m[0], m[1], m[2], m[3], m[4], rk, w, w)
+        dx, dmix, dprev = B.tokenMixBackward([*gs[:5], None], y, mix, prev, dlast=last)
+        return [d, s, y, last, o, *gs, dmix, dprev, *B.residualNormBackward(dx, ck, w, mean, rstd, dy, 0.5, 0.1, seed, 2)]
+    return run
+for f in (calls(torch.bfloat16, 256), calls(torch.float32, 2560)):
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = f()
+    graph.replay()
+    assert all(torch.equal(a, c) for a, c in zip(got, f()))
+print("ok")
+"""
+
+
+def test_first_calls_during_capture(cuda):
+    """Nothing has to run before a capture: kernels of short and of long rows."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", CAPTURE_FIRST.format(root=root)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "ok" in r.stdout, r.stderr[-2000:]
