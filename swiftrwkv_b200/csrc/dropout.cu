@@ -1,8 +1,8 @@
 // Dropout with a mask that is never stored (philox.cuh): y = x scale where kept, 0
 // elsewhere; its gradient is the same call on dy.  One pass over memory: a thread
 // takes DU blocks of 8 elements DT apart, all loads first, and draws a block's bits
-// while they arrive.  16384 x 8192 bf16: 80 us (a copy: 82), 101 instructions per block of 8
-// elements, 58 of them for its bits; one or two blocks a thread 87 and 90 us.
+// while they arrive.  16384 x 8192 bf16: 80 us (a copy: 82), 113 instructions per block of 8
+// elements (28 at p = 0), 58 of them for its bits; one or two blocks a thread 87 and 90 us.
 #include "ckpt8.cuh"
 #include "philox.cuh"
 

@@ -9,9 +9,10 @@
 // HBM's part is 4 tensors forward (x, branch, s, y) and 5 backward (dy, s, dres, dx,
 // dbranch), 1 + 1/32 bytes per element for s as a checkpoint.  s is normed and
 // checkpointed in fp32, before its rounding.  Beside that both are bound by the issue
-// of instructions: a vector of 8 elements takes 16 bytes per tensor, and 70 to 90
-// instructions for its random bits alone, so that the kernels count them: pairs of
-// fp32 in one instruction, several vectors or rows to a thread's share of a row's sums.
+// of instructions: a vector of 8 elements takes 16 bytes per tensor, and dropout 72
+// (forward) to 94 instructions (58 draw its bits, the others apply them), so that the kernels
+// count them: pairs of fp32 in one instruction, several vectors or rows to a thread's share of
+// a row's sums.
 #include <algorithm>
 
 #include "ckpt8.cuh"
@@ -366,8 +367,8 @@ constexpr int RN_STAGES = 3;
 // thread (cp.async); one barrier per row, for its two sums (buffers alternating).
 //
 // 16384 x 2560 bf16: 65 us without dropout, dense or from a checkpoint (floors 64 and 58),
-// 74 and 81 with it.  Bound then by issue: 280 to 305 instructions per vector, 90 of them for
-// the random bits, at 56 % of the slots with the 13 warps per SM that the registers leave (one
+// 74 and 81 with it.  Bound then by issue: 281 to 305 instructions per vector (187 to 217
+// without dropout), at 56 % of the slots with the 13 warps per SM that the registers leave (one
 // vector a thread, 20 warps: 83 with a checkpoint and dropout, 73 dense without; more warps of
 // fewer registers load the weights again and again: 81 to 100).
 template <typename T, bool CK, int MODE, int NV, int MAXT, int MINB>

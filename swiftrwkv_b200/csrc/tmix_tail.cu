@@ -66,7 +66,8 @@ struct Own8 {
 // The vectors of a row that a thread owns run ahead of their use by a stage or two
 // through a ring in shared memory that is private to the thread (cp.async, no
 // barrier), so that HBM stays busy through a head's sums (loads at the head of each row's
-// work: 90 us forward, 183 backward).  Two stages of fp32, which fill 48 KB.
+// work: 90 us forward, 183 backward).  Two stages of fp32, which fill 48 KB in
+// the backward (40 forward).
 template <typename T, int L, int N>
 struct TailRing {
     static constexpr int W = Own8<T, L>::W, STAGES = sizeof(T) == 2 ? 3 : 2;

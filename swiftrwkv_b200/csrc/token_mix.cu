@@ -5,8 +5,8 @@
 //   dx[t]  = sum_j (1 - m_j) dy_j[t] + sum_j m_j dy_j[t+1]  (+ dlast at the last token)
 //   dm_j   = sum over tokens of dy_j[t] (x[t-1] - x[t]),  dprev = sum_j m_j dy_j[0]
 //
-// Both are bound by HBM: 1 + J and 2 + J tensors (16384 x 2560 bf16, six ways: 92 us
-// of a floor of 89 forward, 108 and 4 for the weights' join of 102 backward).  A thread owns
+// Both are bound by HBM: 1 + J and 2 + J tensors (16384 x 2560 bf16, six ways: 91 us
+// of a floor of 89 forward, 113 with the weights' join of 102 backward, the kernels alone).  A thread owns
 // one 16-byte vector of channels of consecutive tokens of the flattened [B, T], so that
 // a token is read about once and the interpolations' weights stay in registers.  The
 // forward takes four tokens a thread: what is left to do are stores, and many short
@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(MIX_T) token_mix_kernel(const MixArgs a, const
 // The gradient.  The J + 1 vectors of a token run MIX_STAGES - 1 tokens ahead through
 // a ring in shared memory that is private to the thread (cp.async, no barrier; loads of
 // each token as it is needed: 181 us).  Products and sums in pairs of fp32.  J = 6 in 16
-// bits takes 180 registers, of them 96 for the weights and their gradient.
+// bits takes 184 registers, of them 96 for the weights and their gradient.
 template <typename T, int J>
 __global__ void __launch_bounds__(MIX_T) token_mix_backward_kernel(const MixArgs a, const MixGrad g) {
     constexpr int VE = Vec16<T>::N, P = VE / 2;
@@ -276,8 +276,8 @@ int dispatch_ways(int J, F&& f) {
 }
 
 // Slots of a backward call: 256 threads per SM for six and five ways, 384 for four, 512 for
-// fewer (more threads than these are slower: 16384 x 2560 bf16, one way, 512 45 us, 896 53; six ways,
-// 256 118 us, 384 121), four tokens each at least.  By the sizes alone: results repeat.
+// fewer (more threads than these are slower: 16384 x 2560 bf16, whole calls with the join and the host's
+// part, one way, 512 45 us, 896 53; six ways, 256 118 us, 384 121), four tokens each at least.  By the sizes alone: results repeat.
 void plan(MixArgs& a, int J) {
     const int64_t threads = 148 * MIX_T * std::min(4, (14 + (J + 1) / 2) / (J + 1));
     const int64_t most = std::max<int64_t>(1, threads / a.nvec);
