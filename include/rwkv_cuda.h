@@ -636,8 +636,8 @@ int rwkv_dropout(int dtype, const void* x, double p, uint64_t seed, uint64_t off
  * x, branch, sum, y: [rows, D] in dtype; D % 8 == 0, D <= 12288 (6144 in F32).
  * y, mean, rstd and the checkpoint (codes / exps, both NULL or both written; codes
  * 8-byte aligned) are those of the sum in fp32, before it is rounded to dtype.  sum may
- * be x or branch, y the other of them.  The dropout's element i is branch's.  scale /
- * (1 - q) must be finite in fp32. */
+ * be x or branch, y the other of them.  The dropout's element i is branch's.  scale and
+ * scale / (1 - q) must be finite in fp32 (where q = 1, scale). */
 int rwkv_residual_norm_forward(int dtype, const void* x, const void* branch, double scale, double p, uint64_t seed,
                                uint64_t offset, const int64_t* state, int wdtype, const void* weight,
                                const void* bias, float eps, void* sum, void* y, float* mean, float* rstd,

@@ -745,8 +745,9 @@ int check_sizes(int dtype, int wdtype, int rows, int D, double p, double scale, 
     RWKV_REQUIRE(rows >= 1 && D >= 1, RWKV_E_SHAPE, "%s: rows=%d D=%d", fn, rows, D);
     RWKV_REQUIRE(D % 8 == 0 && D <= most, RWKV_E_UNSUPPORTED, "%s: D=%d must be a multiple of 8, at most %d", fn, D, most);
     RWKV_REQUIRE(p >= 0.0 && p <= 1.0, RWKV_E_SHAPE, "%s: p=%g must be in 0..1", fn, p);
-    RWKV_REQUIRE(std::isfinite(make_dropout(p, scale, 0, 0, nullptr).scale), RWKV_E_SHAPE,
-                 "%s: scale=%g over 1 - p must be finite in fp32", fn, scale);
+    // (where everything is dropped the factor is 0 whatever scale is)
+    RWKV_REQUIRE(std::isfinite((float)scale) && std::isfinite(make_dropout(p, scale, 0, 0, nullptr).scale), RWKV_E_SHAPE,
+                 "%s: scale=%g and scale over 1 - p must be finite in fp32", fn, scale);
     return RWKV_OK;
 }
 

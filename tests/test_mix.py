@@ -110,6 +110,12 @@ def test_residual_norm_backward_refusals():
     assert rn_bwd(ws=HALF) == _lib.E_UNSUPPORTED
 
 
+def test_residual_norm_scale_is_finite_where_everything_is_dropped():
+    for scale in (float("inf"), float("nan"), -1e300):
+        assert rn_fwd(scale=scale, p=1.0) == _lib.E_SHAPE
+        assert rn_bwd(scale=scale, p=1.0) == _lib.E_SHAPE
+
+
 def pointers(*ps):
     return (ctypes.c_void_p * len(ps))(*[p.value if p else None for p in ps])
 
