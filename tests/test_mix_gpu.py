@@ -244,10 +244,10 @@ def outlier_rows(D, VE):
 @pytest.mark.parametrize("D", [72, 264, 520, 776, 1032, 1280, 1536, 2056, 2560, 4096, 6144])
 def test_residual_norm_of_rows_with_outliers(cuda, dt, D):
     """The statistics are those of a sum around the mean, wherever the row's outliers are.  A term
-    passes at most 20 additions in its thread, 1 for a pair's halves, 5 in its warp and 4 between
-    warps: a sum of squares is off by 30 U32 (each square 2 U32 by its difference), by at most
-    4 times that where it is taken from another point than the mean; rstd by half of it and 2 roundings
-    in the variance, 2 in the root and the quotient.  The mean: 32 U32 mean|s|."""
+    passes at most 28 additions (64 threads: 20 in its own, 1 for a pair's halves, 5 in the warp, 2
+    between warps; 512 threads: 6, 1, 5 and 16): a sum of squares is off by 30 U32 (each square 2 U32 by
+    its difference), by at most 4 times that where it is taken from another point than the mean; rstd by
+    half of it and 2 roundings in the variance, 2 in the root and the quotient.  The mean: 32 U32 mean|s|."""
     from swiftrwkv_b200 import block as B
     t = DTYPES[dt]
     x = outlier_rows(D, 4 if dt == "f32" else 8).to(t)
